@@ -292,6 +292,87 @@ int im_cuda_sdpa_f16(im_device *dev, const void *q_dev, const void *k_cache_dev,
                      int nkv, int head_dim, int max_seq, int base_pos, const int *pos_dev, int T, float scale, int num_splits,
                      void *scratch_dev, size_t scratch_bytes, void *stream);
 
+/* ------------------------------------------------------------------ KV cache in pages
+ * Keys and values of every layer in pages that sequences take as they grow, and the operators that a host runs on them between
+ * two forwards: appending with rotation, attention of new tokens (one each, a portion of a prompt, or a tree of drafted
+ * tokens), keeping the accepted path of a tree, and the reordering of a beam search.  (No counterpart in the reference, whose
+ * caches are contiguous: kv_scatter, crates/ironmill-inference/src/metal/shaders/kv/kv_scatter.metal:20-42; its speculative
+ * decoder, crates/ironmill-inference/src/speculative/, verifies trees above the engine.)
+ *
+ * Row r of sequence s lies in page page_table_dev[s * table_stride + r / page_size], slot r % page_size.  seq_len_dev[s] rows are
+ * there before a call's new tokens, whose rows follow them.  token_start_dev [num_seqs + 1], not decreasing, gives the
+ * new tokens of sequence s: rows token_start[s] .. token_start[s + 1] - 1 of the token arrays.  Token rows before the first or from
+ * the last of these on are left as they are.  What the device arrays say is checked on the device: a row past the table, a page
+ * number outside 0 .. num_pages - 1 or a negative length reads nothing (the row is not there) and writes nothing.
+ * Clear the struct before filling it. */
+typedef struct im_paged_kv {
+    void *k_dev, *v_dev;       /* layer l, page p: [num_kv_heads, page_size, head_dim] at l * layer_stride + p * page_stride; 16-byte aligned */
+    int64_t layer_stride, page_stride; /* elements, multiples of 8; 0 = packed [num_layers, num_pages, ...] */
+    int num_layers, num_pages, num_kv_heads, page_size;
+    int head_dim;              /* a multiple of 8, up to 256; paged_attention: 64, 128 or 256 */
+    int dtype;                 /* IM_DTYPE_F16 or IM_DTYPE_BF16: of the cache, queries, keys, values and outputs */
+    int num_seqs;
+    const int *page_table_dev; /* [num_seqs, table_width], rows table_stride apart (0 = table_width) */
+    int table_width;
+    int64_t table_stride;
+    const int *seq_len_dev;    /* [num_seqs] */
+} im_paged_kv;
+
+/* Keys and values of new tokens into layer `layer`, the keys and (q_dev not NULL) the queries beside them rotated on the way.
+ * k, v [num_tokens, num_kv_heads, head_dim], q, q_out [num_tokens, num_heads, head_dim], tokens *_stride elements apart (multiples of 8,
+ * 16-byte aligned: parts of one row per token do); q_out may be q.  The first rotary_dim columns are rotated by the token's angles, f32 with one
+ * rounding: columns (i, i + rotary_dim / 2), or with neighbours = 1 (2 i, 2 i + 1), by entry i of its row of cos / sin [max_pos, head_dim / 2]
+ * (table_dtype IM_DTYPE_F16, as im_cuda_rope_table writes them, or IM_DTYPE_F32); the row is the token's row in the cache, or
+ * position_dev [num_tokens] (nodes of a tree: their depth).  rotary_dim 0: nothing is rotated.  A token whose angle row is outside
+ * the table is neither written nor rotated.  No two tokens of a call may name the same cache row. */
+int im_cuda_paged_append(im_device *dev, const im_paged_kv *kv, int layer, const void *k_dev, int64_t k_stride, const void *v_dev, int64_t v_stride,
+                         const int *token_start_dev, int num_tokens, const void *q_dev, int64_t q_stride, void *q_out_dev, int64_t q_out_stride,
+                         int num_heads, const void *cos_dev, const void *sin_dev, int table_dtype, int max_pos, int rotary_dim, int neighbours,
+                         const int *position_dev, void *stream);
+
+/* out[t, h] = softmax(scale * q[t, h] . K^T) V of the new tokens, whose own rows are in the cache already.  Head h reads KV head
+ * h / (num_heads / num_kv_heads).  A token sees all seq_len rows before the new ones, and of the new rows: without a mask its own and
+ * those before it; with mask_dev [num_tokens, mask_words] the d-th where bit d % 64 of word d / 64 is set (its ancestors and itself).
+ * A row that sees nothing gets zeros; infinities and NaN in rows that a token does not see do not reach it.  f32 scores, sums
+ * and accumulation, softmax weights as a sum of two 16-bit terms, one rounding of the output.  q, out: as q in paged_append.
+ * max_new: no sequence has more new tokens (further ones are left as they are).  max_len: no sequence has more rows, the new ones
+ * included (0: the table's width); a smaller value costs time, not results.  scratch_dev: 16-byte aligned,
+ * im_cuda_paged_attention_scratch_bytes for the same kv, heads and max_new; calls whose kernels may overlap need one each. */
+size_t im_cuda_paged_attention_scratch_bytes(const im_device *dev, const im_paged_kv *kv, int num_heads, int max_new);
+int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int layer, const void *q_dev, int64_t q_stride, void *out_dev, int64_t out_stride,
+                            int num_heads, const int *token_start_dev, int num_tokens, int max_new, const uint64_t *mask_dev, int mask_words,
+                            float scale, int max_len, void *scratch_dev, size_t scratch_bytes, void *stream);
+
+/* The accepted path of a tree: in every layer row seq_len + accepted_dev[s, j] becomes row seq_len + j, j = 0 .. count_dev[s] - 1
+ * (accepted [num_seqs, max_accept], each path in order from the root: accepted[s, j] >= j; an entry below j is not moved).
+ * seq_len_out_dev [num_seqs], not over seq_len_dev: seq_len + count. */
+int im_cuda_paged_keep(im_device *dev, const im_paged_kv *kv, const int *accepted_dev, int max_accept, const int *count_dev, int *seq_len_out_dev,
+                       void *stream);
+
+/* The beams of a search after a step.  Sequences lie in groups of `group` beams (num_seqs a multiple); beam i of a group becomes
+ * a copy of beam parent_dev[i] (its number in the group; any other value: of itself).  Every sequence holds the pages of its row from index
+ * seq_len / page_size on alone (the last one and what has been set aside for it), the earlier ones may be shared.  The first child of a
+ * parent keeps its row; each further one shares the earlier pages and gets, in order, those that a beam without a child holds
+ * alone (there are as many such beams), with the rows of the parent's last page copied to the first of them, in every layer; where its row
+ * has more entries left than that beam's had, they become -1.  table_out_dev (rows table_out_stride apart, 0 = table_width) and seq_len_out_dev get the new rows and lengths; they may
+ * not lie over the old ones. */
+int im_cuda_paged_reorder(im_device *dev, const im_paged_kv *kv, const int *parent_dev, int group, int *table_out_dev, int64_t table_out_stride,
+                          int *seq_len_out_dev, void *stream);
+
+/* ------------------------------------------------------------------ beam search
+ * The `picks` best continuations of every group of beams: value[b, v] = score[b] + logit[b, v] - log(sum_v exp(logit[b, v])), compared in
+ * 64 bits, ties to the lowest b * vocab + v, best first.  logits [groups * beams, vocab] of `dtype` (IM_DTYPE_F16, F32 or BF16), rows row_stride
+ * elements apart (0 = vocab); score_dev f32 [groups * beams].  done_dev (u8 [groups * beams] or NULL): a finished beam has one continuation,
+ * end_token at its own score, and its logits are not read.  Values of -inf and NaN are not picked (nor anything of a beam whose logits
+ * hold a NaN or +inf); where fewer than `picks` are left, the rest gets score -inf, parent -1 and token -1.
+ * score_out f32, parent_out (beam in the group) and token_out i32: [groups, picks].  1 <= beams <= 64, 1 <= picks <= 64.
+ * Greedy decoding's pick (crates/ironmill-inference/src/sampling.rs:331-339) takes the last maximal index; this takes the first.
+ * scratch_dev: 16-byte aligned, calls whose kernels may overlap need one each. */
+size_t im_cuda_beam_select_scratch_bytes(const im_device *dev, int groups, int beams, int vocab, int picks);
+int im_cuda_beam_select(im_device *dev, const void *logits_dev, int dtype, int64_t row_stride, int groups, int beams, int vocab, const float *score_dev,
+                        const uint8_t *done_dev, int end_token, int picks, float *score_out_dev, int *parent_out_dev, int *token_out_dev,
+                        void *scratch_dev, size_t scratch_bytes, void *stream);
+
 /* ------------------------------------------------------------------ model-level engine
  * The CUDA counterpart of MetalInference behind the InferenceEngine trait
  * (crates/ironmill-inference/src/engine.rs:72-114; crates/ironmill-inference/src/metal/engine.rs:122-270,

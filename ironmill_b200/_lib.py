@@ -35,9 +35,22 @@ _lib = None
 _VOIDP_RESTYPE = ("im_cuda_buffer_ptr",)
 _SIZE_RESTYPE = ("im_cuda_device_allocated_bytes", "im_cuda_buffer_length", "im_cuda_affine_weight_bytes",
                  "im_cuda_model_memory_bytes", "im_cuda_model_step_bytes", "im_cuda_tq_scratch_bytes",
-                 "im_cuda_sdpa_f16_scratch_bytes", "im_cuda_tq_prefill_scratch_bytes")
+                 "im_cuda_sdpa_f16_scratch_bytes", "im_cuda_tq_prefill_scratch_bytes",
+                 "im_cuda_paged_attention_scratch_bytes", "im_cuda_beam_select_scratch_bytes")
 _VOID_RESTYPE = ("im_cuda_device_free", "im_cuda_buffer_free", "im_cuda_affine_weight_free", "im_cuda_model_free",
                  "im_cuda_tq_free", "im_cuda_tp_free")
+
+_P, _I, _L, _F, _Z = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
+# Calls between two forwards are short: with their argument types known, plain numbers and addresses are passed.
+_ARGTYPES = {
+    "im_cuda_paged_append": (_P, _P, _I, _P, _L, _P, _L, _P, _I, _P, _L, _P, _L, _I, _P, _P, _I, _I, _I, _I, _P, _P),
+    "im_cuda_paged_attention_scratch_bytes": (_P, _P, _I, _I),
+    "im_cuda_paged_attention": (_P, _P, _I, _P, _L, _P, _L, _I, _P, _I, _I, _P, _I, _F, _I, _P, _Z, _P),
+    "im_cuda_paged_keep": (_P, _P, _P, _I, _P, _P, _P),
+    "im_cuda_paged_reorder": (_P, _P, _P, _I, _P, _L, _P, _P),
+    "im_cuda_beam_select_scratch_bytes": (_P, _I, _I, _I, _I),
+    "im_cuda_beam_select": (_P, _P, _I, _L, _I, _I, _I, _P, _P, _I, _I, _P, _P, _P, _P, _Z, _P),
+}
 
 
 def use(path: str) -> None:
@@ -61,10 +74,20 @@ def lib() -> C.CDLL:
         for name in _SIZE_RESTYPE:
             if hasattr(_lib, name):
                 getattr(_lib, name).restype = C.c_size_t
+        for name, types in _ARGTYPES.items():
+            if hasattr(_lib, name):
+                getattr(_lib, name).argtypes = types
         for name in _VOID_RESTYPE:
             if hasattr(_lib, name):
                 getattr(_lib, name).restype = None
     return _lib
+
+
+class PagedKvStruct(C.Structure):
+    """im_paged_kv of include/ironmill_cuda.h."""
+    _fields_ = [("k_dev", _P), ("v_dev", _P), ("layer_stride", _L), ("page_stride", _L), ("num_layers", _I), ("num_pages", _I), ("num_kv_heads", _I),
+                ("page_size", _I), ("head_dim", _I), ("dtype", _I), ("num_seqs", _I), ("page_table_dev", _P), ("table_width", _I), ("table_stride", _L),
+                ("seq_len_dev", _P)]
 
 
 def last_error() -> str:

@@ -1,0 +1,654 @@
+// Attention of new tokens (one of each sequence, a portion of a prompt, or a tree of drafted tokens) over a paged cache.
+//
+//   out[t, h] = sum_j p_j v_j,  p = softmax over the visible rows j of scale * q[t, h] . k_j
+//
+// What bounds it is the read of K and V: every (sequence, KV head) is read once for all the rows (token, query head) that share it, up
+// to R of them in a CTA. The tiles of 64 positions of all (row tile, KV head) items form one list, cut into equal shares, one per CTA, whatever the lengths
+// are; an item that a cut divides leaves partial sums, which a second launch joins.
+//
+// In a CTA four warps take 16 positions of each tile and work on their own: each keeps a ring of K and V slices (cp.async, 16 bytes per lane, rows
+// looked up in the page table, so that any page size works and pages may end anywhere) and its own running maximum, sum and outputs of all R
+// rows; they meet only where an item ends. The ring runs ahead over the ends of items. Scores and outputs on mma.sync m16n8k16 (a
+// tile of 64 positions against 16 rows is 256 instructions for 32 KB: far from what bounds it), weights as two 16-bit terms.
+#include <limits.h>
+#include <math.h>
+
+#include <algorithm>
+
+#include "paged_attn.cuh"
+
+namespace im {
+namespace {
+
+constexpr int kPaWarps = 4, kPaThreads = kPaWarps * 32, kPaSlice = 16, kPaTile = kPaWarps * kPaSlice;
+
+template <int HD, int MT>
+struct PaShape {
+    static constexpr int kRows = 16 * MT;
+    static constexpr int kSliceBytes = kPaSlice * HD * 2;
+    static constexpr int kStages = HD == 64 ? 6 : 3;
+    static constexpr int kRing = kPaWarps * kStages * 2 * kSliceBytes;
+    static constexpr int kQ = MT > 1 ? kRows * HD * 2 : 0;        // queries in shared memory where registers do not hold them
+    static constexpr int kMergeCols = MT > 1 ? 32 : HD;           // columns that are joined at a time
+    static constexpr int kMerge = kRows * kMergeCols * 4;
+    static constexpr int kSmem = kRing + kQ + kMerge + kPaWarps * kRows * 8;
+};
+
+__device__ __forceinline__ uint32_t sm32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+template <bool BF16>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool there) {  // zeros where there is no source
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
+// Inclusive sums of v over the block's threads in sums[], the total returned.
+__device__ __forceinline__ long long block_scan(int v, long long *sums) {
+    __shared__ long long of_warp[kPaWarps];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    long long s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long t = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += t;
+    }
+    __syncthreads();
+    if (lane == 31) of_warp[w] = s;
+    __syncthreads();
+    long long before = 0, total = 0;
+#pragma unroll
+    for (int i = 0; i < kPaWarps; i++) {
+        if (i < w) before += of_warp[i];
+        total += of_warp[i];
+    }
+    sums[threadIdx.x] = s + before;
+    __syncthreads();
+    return total;
+}
+
+template <int R>
+__device__ __forceinline__ int unit_tiles(const PagedUnit &u) { return (u.end + kPaTile - 1) / kPaTile; }
+
+// Where a CTA's share starts.
+struct Share {
+    long long from, to;  // places in the list of all tiles
+    int unit, head, tile;
+};
+
+// No share is empty: CTAs without a tile of their own have none, and leave no parts.
+__device__ __forceinline__ int share_count(long long total, int ctas) { return (int)min((long long)ctas, total); }
+__device__ __forceinline__ long long share_at(long long total, int n, int c) { return c >= n ? total : total * c / n; }
+
+template <int R>
+__device__ __forceinline__ Share find_share(const PagedAttn &p, int units, long long *sums) {
+    __shared__ int found[3];
+    Share s;
+    long long total = 0;
+    for (int u0 = 0; u0 < units; u0 += kPaThreads) {
+        const int u = u0 + threadIdx.x;
+        const int n = u < units ? unit_tiles<R>(paged_unit<R>(p, u)) : 0;
+        const long long all = block_scan(n, sums);
+        if (blockIdx.x == 0 && u < units) p.first[u] = total + sums[threadIdx.x] - n;
+        total += all;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.first[units] = total;
+    total *= p.kv.nkv;
+    const int shares = share_count(total, p.ctas);
+    s.from = share_at(total, shares, blockIdx.x);
+    s.to = share_at(total, shares, blockIdx.x + 1);
+    s.unit = s.head = s.tile = 0;
+    if (s.from >= s.to) return s;
+    long long before = 0;
+    for (int u0 = 0; u0 < units; u0 += kPaThreads) {
+        const int u = u0 + threadIdx.x;
+        const int n = u < units ? unit_tiles<R>(paged_unit<R>(p, u)) : 0;
+        const long long all = block_scan(n, sums);
+        const long long a = (before + sums[threadIdx.x] - n) * p.kv.nkv;
+        if (n > 0 && s.from >= a && s.from < a + (long long)n * p.kv.nkv) {
+            const int d = (int)(s.from - a);
+            found[0] = u;
+            found[1] = d / n;
+            found[2] = d % n;
+        }
+        before += all;
+        if (before * p.kv.nkv > s.from) break;
+    }
+    __syncthreads();
+    s.unit = found[0];
+    s.head = found[1];
+    s.tile = found[2];
+    return s;
+}
+
+// A row whose sums are not finite, from the positions it sees alone: on the tensor cores a weight of zero times an infinite or missing value of a
+// position that the row does not see is a NaN. A warp per row; o: this lane's columns (lane, lane + 32, ...).
+template <bool BF16, int HD>
+__device__ __noinline__ void plain_row(const PagedAttn &p, const PagedUnit &u, int head, int r, int from, int to, float *o, float &m, float &l) {
+    const int lane = threadIdx.x & 31, t = (u.row0 + r) / p.group, h = head * p.group + (u.row0 + r) % p.group;
+    const uint16_t *q = p.q + (u.tok0 + t) * p.qs + (long long)h * HD;
+    m = -INFINITY;
+    l = 0.0f;
+    for (int i = 0; i < HD / 32; i++) o[i] = 0.0f;
+    for (int pos = from; pos < to; pos++) {
+        if (!paged_sees(p, u, t, pos)) continue;
+        long long at = p.kv.row_of(u.seq, pos);
+        if (at < 0) continue;
+        at += (long long)head * p.kv.page * HD;
+        float s = 0.0f;
+        for (int i = 0; i < HD / 32; i++) s = fmaf(one16<BF16>(q + lane + 32 * i), one16<BF16>(p.kc + at + lane + 32 * i), s);
+        s = warp_sum(s) * p.scale2;
+        if (s == -INFINITY) continue;
+        const float m_new = fmaxf(m, s), corr = ex2(m - m_new), w = ex2(s - m_new);
+        m = m_new;
+        l = l * corr + w;
+        for (int i = 0; i < HD / 32; i++) o[i] = fmaf(w, one16<BF16>(p.vc + at + lane + 32 * i), o[i] * corr);
+    }
+}
+
+template <bool BF16, int HD, int MT>
+__global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kernel(const __grid_constant__ PagedAttn p, int units) {
+    using S = PaShape<HD, MT>;
+    constexpr int R = S::kRows, KS = HD / 16, NT = HD / 8, CH = HD / 8;  // k steps, 8-column tiles, 16-byte pieces of a row
+    extern __shared__ __align__(128) unsigned char pa_smem[];
+    __shared__ long long sums[kPaThreads];
+    __shared__ unsigned rows_there[kPaWarps][8];  // of a slice in the ring: bit r where row r is in the cache
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    unsigned char *ring = pa_smem + warp * (S::kRing / kPaWarps);
+    unsigned char *qsm = pa_smem + S::kRing;
+    float *merge = reinterpret_cast<float *>(qsm + S::kQ);
+    float2 *ml = reinterpret_cast<float2 *>(reinterpret_cast<unsigned char *>(merge) + S::kMerge);  // [warps, R]
+    __shared__ unsigned bad_rows[2];  // rows of an item whose sums are not finite, every other item's
+    if (tid < 2) bad_rows[tid] = 0;
+    pdl_trigger();
+    pdl_wait();
+    const Share share = find_share<R>(p, units, sums);
+    if (share.from >= share.to) return;
+    const int count = (int)(share.to - share.from);
+
+    // ---- the copies' cursor: one slice ahead of the copies, so that a page number is there when it is needed
+    int f_unit = share.unit, f_head = share.head, f_tile = share.tile, f_left = count;
+    PagedUnit f_u = paged_unit<R>(p, f_unit);
+    int f_tiles = unit_tiles<R>(f_u);
+    int n_page = -1, n_slot = 0, n_head = 0;  // of the slice that is copied next: this lane's row (lane & 15)
+    auto fetch = [&]() {
+        n_page = -1;
+        if (f_left <= 0) return;
+        const int pos = f_tile * kPaTile + warp * kPaSlice + (lane & 15);
+        if (pos < f_u.end) {
+            const int pg = pos / p.kv.page;
+            n_slot = pos - pg * p.kv.page;
+            n_page = __ldg(p.kv.table + f_u.seq * p.kv.table_stride + pg);
+        }
+        n_head = f_head;
+        f_left--;
+        if (++f_tile == f_tiles) {
+            f_tile = 0;
+            if (++f_head == p.kv.nkv) {
+                f_head = 0;
+                while (f_left > 0 && ++f_unit < units) {
+                    f_u = paged_unit<R>(p, f_unit);
+                    f_tiles = unit_tiles<R>(f_u);
+                    if (f_tiles > 0) break;
+                }
+            }
+        }
+    };
+    auto copy = [&](int stage) {  // the slice whose rows fetch() looked up
+        const bool there = (unsigned)n_page < (unsigned)p.kv.pages;
+        const long long off = there ? n_page * p.kv.page_stride + ((long long)n_head * p.kv.page + n_slot) * HD : -1;
+        const uint32_t dst = sm32(ring) + stage * 2 * S::kSliceBytes;
+        const unsigned all = __ballot_sync(0xffffffffu, there);
+        if (lane == 0) rows_there[warp][stage] = all;
+        constexpr int RPI = 32 / CH > 0 ? 32 / CH : 1;  // rows of one request of the warp
+        constexpr int IPR = CH / 32 > 0 ? CH / 32 : 1;
+#pragma unroll
+        for (int i = 0; i < kPaSlice / RPI; i++) {
+            const int row = i * RPI + (RPI > 1 ? lane / CH : 0);
+            const long long at = __shfl_sync(0xffffffffu, off, row);
+#pragma unroll
+            for (int j = 0; j < IPR; j++) {
+                const int c = (lane & (CH < 32 ? CH - 1 : 31)) + j * 32;
+                const uint32_t d = dst + row * (HD * 2) + ((c ^ (row & 7)) << 4);
+                const long long src = at < 0 ? 0 : at + c * 8;
+                cp16(d, p.kc + src, at >= 0);
+                cp16(d + S::kSliceBytes, p.vc + src, at >= 0);
+            }
+        }
+    };
+    fetch();
+#pragma unroll
+    for (int i = 0; i < S::kStages - 1; i++) {
+        if (i < count) {
+            copy(i);
+            fetch();
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+
+    // ---- the items
+    int unit = share.unit, head = share.head, tile = share.tile, done = 0, stage = 0;
+    bool first_item = true;
+    int odd_item = 0;
+    while (done < count) {
+        PagedUnit u = paged_unit<R>(p, unit);
+        const int tiles = unit_tiles<R>(u);
+        if (tiles == 0) {
+            unit++;
+            continue;
+        }
+        const int t0 = tile, t1 = min(tiles, tile + count - done);
+        // queries: A fragments, rows lane / 4 and lane / 4 + 8 of each 16
+        uint32_t qf[MT == 1 ? KS : 1][4];
+        int tok[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int r = mt * 16 + (lane >> 2) + 8 * i;
+                tok[mt][i] = (u.row0 + min(r, u.rows - 1)) / p.group;
+            }
+        if constexpr (MT == 1) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int r = (lane >> 2) + 8 * i;
+                const uint32_t *src = reinterpret_cast<const uint32_t *>(p.q + (u.tok0 + tok[0][i]) * p.qs + (long long)(head * p.group + (u.row0 + r) % p.group) * HD);
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) qf[ks][2 * j + i] = r < u.rows ? __ldg(src + ks * 8 + j * 4 + (lane & 3)) : 0u;
+            }
+        } else {
+            __syncthreads();
+            for (int i = tid; i < R * CH; i += kPaThreads) {
+                const int r = i / CH, c = i % CH;
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (r < u.rows) {
+                    const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
+                    x = __ldg(reinterpret_cast<const uint4 *>(p.q + (u.tok0 + t) * p.qs + (long long)(head * p.group + g) * HD) + c);
+                }
+                *reinterpret_cast<uint4 *>(qsm + r * (HD * 2) + ((c ^ (r & 7)) << 4)) = x;
+            }
+            __syncthreads();
+        }
+        float m[MT][2], l[MT][2], o[MT][NT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) m[mt][i] = -INFINITY, l[mt][i] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[mt][n][j] = 0.0f;
+        }
+        for (; tile < t1; tile++, done++) {
+            // the next slice on its way, this one there
+            if (done + S::kStages - 1 < count) {
+                int to = stage + S::kStages - 1;
+                if (to >= S::kStages) to -= S::kStages;
+                copy(to);
+                fetch();
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
+            __syncwarp();
+            const uint32_t ks_at = sm32(ring) + stage * 2 * S::kSliceBytes, vs_at = ks_at + S::kSliceBytes;
+            float s[MT][2][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) s[mt][n][j] = 0.0f;
+            {
+                const int r = (lane & 7) + ((lane >> 4) << 3), hi = (lane >> 3) & 1;  // row and 16-byte half of this lane's matrix row
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    uint32_t b[4];
+                    ldsm4(b, ks_at + r * (HD * 2) + (((2 * ks + hi) ^ (r & 7)) << 4));
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        if constexpr (MT == 1) {
+                            mma16<BF16>(s[mt][0], qf[ks], b[0], b[1]);
+                            mma16<BF16>(s[mt][1], qf[ks], b[2], b[3]);
+                        } else {
+                            uint32_t a[4];
+                            const int qr = mt * 16 + (lane & 15), qc = 2 * ks + (lane >> 4);
+                            ldsm4(a, sm32(qsm) + qr * (HD * 2) + ((qc ^ (qr & 7)) << 4));
+                            mma16<BF16>(s[mt][0], a, b[0], b[1]);
+                            mma16<BF16>(s[mt][1], a, b[2], b[3]);
+                        }
+                    }
+                }
+            }
+            const int pos0 = tile * kPaTile + warp * kPaSlice;
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) s[mt][n][j] *= p.scale2;
+            const unsigned there = rows_there[warp][stage] & 0xffffu;
+            if (there != 0xffffu || pos0 + kPaSlice > u.len) {  // some row may not see some position
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int n = 0; n < 2; n++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const int at = n * 8 + (lane & 3) * 2 + (j & 1);
+                            if (!(there >> at & 1) || !paged_sees(p, u, tok[mt][j >> 1], pos0 + at)) s[mt][n][j] = -INFINITY;
+                        }
+            }
+            uint32_t w[MT][4], w2[MT][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    float top = fmaxf(fmaxf(s[mt][0][2 * i], s[mt][0][2 * i + 1]), fmaxf(s[mt][1][2 * i], s[mt][1][2 * i + 1]));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    if (__any_sync(0xffffffffu, top > m[mt][i])) {
+                        const float m_new = fmaxf(m[mt][i], top), corr = m_new == -INFINITY ? 1.0f : ex2(m[mt][i] - m_new);
+                        m[mt][i] = m_new;
+                        l[mt][i] *= corr;
+#pragma unroll
+                        for (int n = 0; n < NT; n++) o[mt][n][2 * i] *= corr, o[mt][n][2 * i + 1] *= corr;
+                    }
+                    const float base = m[mt][i] == -INFINITY ? 0.0f : m[mt][i];
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int n = 0; n < 2; n++) {
+                        const float x0 = ex2(s[mt][n][2 * i] - base), x1 = ex2(s[mt][n][2 * i + 1] - base);
+                        sum += x0 + x1;
+                        w[mt][2 * n + i] = pack16<BF16>(x0, x1);
+                        const float2 back = unpack16<BF16>(w[mt][2 * n + i]);
+                        w2[mt][2 * n + i] = pack16<BF16>(x0 - back.x, x1 - back.y);
+                    }
+                    l[mt][i] += sum;
+                }
+            {
+                const int r = (lane & 7) + (((lane >> 3) & 1) << 3), hi = lane >> 4;
+#pragma unroll
+                for (int n = 0; n < NT; n += 2) {
+                    uint32_t b[4];
+                    ldsm4t(b, vs_at + r * (HD * 2) + (((n + hi) ^ (r & 7)) << 4));
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++) {
+                        mma16<BF16>(o[mt][n], w[mt], b[0], b[1]);
+                        mma16<BF16>(o[mt][n + 1], w[mt], b[2], b[3]);
+                        mma16<BF16>(o[mt][n], w2[mt], b[0], b[1]);
+                        mma16<BF16>(o[mt][n + 1], w2[mt], b[2], b[3]);
+                    }
+                }
+            }
+            __syncwarp();  // every lane has read the slice before the copies of the one that takes its place
+            if (++stage == S::kStages) stage = 0;
+        }
+        // ---- the item's (or the share's part of it) rows: four warps' sums joined in order
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                l[mt][i] += __shfl_xor_sync(0xffffffffu, l[mt][i], 1);
+                l[mt][i] += __shfl_xor_sync(0xffffffffu, l[mt][i], 2);
+                if ((lane & 3) == 0) ml[warp * R + mt * 16 + (lane >> 2) + 8 * i] = make_float2(m[mt][i], l[mt][i]);
+            }
+        __syncthreads();
+        if (tid == 0) bad_rows[!odd_item] = 0;  // every thread has looked at the last item's
+        const bool whole = t0 == 0 && t1 == tiles;
+        const size_t part = ((size_t)blockIdx.x * 2 + (first_item ? 0 : 1)) * R;
+        float f[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int r = mt * 16 + (lane >> 2) + 8 * i;
+                float M = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kPaWarps; w++) M = fmaxf(M, ml[w * R + r].x);
+                f[mt][i] = m[mt][i] == -INFINITY && l[mt][i] == 0.0f ? 0.0f : ex2(m[mt][i] - M);
+            }
+        auto row_ml = [&](int r) {
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kPaWarps; w++) M = fmaxf(M, ml[w * R + r].x);
+#pragma unroll
+            for (int w = 0; w < kPaWarps; w++) {
+                const float2 x = ml[w * R + r];
+                L += x.x == -INFINITY && x.y == 0.0f ? 0.0f : x.y * ex2(x.x - M);
+            }
+            return make_float2(M, L);
+        };
+        constexpr int MC = S::kMergeCols;
+#pragma unroll
+        for (int c0 = 0; c0 < HD; c0 += MC) {
+#pragma unroll
+            for (int w = 0; w < kPaWarps; w++) {
+                if (warp == w) {
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                        for (int n = c0 / 8; n < (c0 + MC) / 8; n++)
+#pragma unroll
+                            for (int i = 0; i < 2; i++) {
+                                float2 *at = reinterpret_cast<float2 *>(merge + (mt * 16 + (lane >> 2) + 8 * i) * MC + ((n * 8 - c0 + (lane & 3) * 2) ^ (((lane >> 2) & 3) << 3)));
+                                float2 x = make_float2(o[mt][n][2 * i] * f[mt][i], o[mt][n][2 * i + 1] * f[mt][i]);
+                                if (f[mt][i] == 0.0f) x = make_float2(0.0f, 0.0f);
+                                if (w > 0) {
+                                    const float2 y = *at;
+                                    x.x += y.x;
+                                    x.y += y.y;
+                                }
+                                *at = x;
+                            }
+                }
+                __syncthreads();
+            }
+            for (int i = tid; i < u.rows * (MC / 8); i += kPaThreads) {
+                const int r = i / (MC / 8), c = i % (MC / 8) * 8;
+                const float *src = merge + r * MC + (c ^ ((r & 3) << 3));
+                float v[8], worst = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; j += 4) *reinterpret_cast<float4 *>(v + j) = *reinterpret_cast<const float4 *>(src + j);
+#pragma unroll
+                for (int j = 0; j < 8; j++) worst += v[j] * 0.0f;  // zero unless a value is not finite
+                if (worst != 0.0f) atomicOr(&bad_rows[odd_item], 1u << r);
+                if (whole) {
+                    const float2 x = row_ml(r);
+                    const float inv = x.y > 0.0f ? 1.0f / x.y : x.y == 0.0f ? 0.0f : x.y;
+                    const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
+                    *reinterpret_cast<uint4 *>(p.out + (u.tok0 + t) * p.os + (long long)(head * p.group + g) * HD + c0 + c) =
+                        make_uint4(pack16<BF16>(v[0] * inv, v[1] * inv), pack16<BF16>(v[2] * inv, v[3] * inv), pack16<BF16>(v[4] * inv, v[5] * inv),
+                                   pack16<BF16>(v[6] * inv, v[7] * inv));
+                } else {
+                    float4 *dst = reinterpret_cast<float4 *>(p.part_o + (part + r) * HD + c0 + c);
+                    dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+                    dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+                }
+            }
+            if (!whole && c0 == 0)
+                for (int r = tid; r < u.rows; r += kPaThreads) p.part_ml[part + r] = row_ml(r);
+            __syncthreads();
+        }
+        if (const unsigned bad = bad_rows[odd_item]) {
+            for (int r = warp; r < u.rows; r += kPaWarps) {
+                if (!(bad >> r & 1)) continue;
+                float x[HD / 32], M, L;
+                plain_row<BF16, HD>(p, u, head, r, t0 * kPaTile, min(t1 * kPaTile, u.end), x, M, L);
+                const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
+                const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
+                for (int i = 0; i < HD / 32; i++) {
+                    if (whole) p.out[(u.tok0 + t) * p.os + (long long)(head * p.group + g) * HD + lane + 32 * i] = (uint16_t)pack16<BF16>(x[i] * inv, 0.0f);
+                    else p.part_o[(part + r) * HD + lane + 32 * i] = x[i];
+                }
+                if (!whole && lane == 0) p.part_ml[part + r] = make_float2(M, L);
+            }
+            __syncthreads();
+        }
+        first_item = false;
+        odd_item ^= 1;
+        if (t1 == tiles) {
+            tile = 0;
+            if (++head == p.kv.nkv) {
+                head = 0;
+                unit++;
+            }
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// Items that a cut divides: a block per (item, row), a thread per column. The parts of an item lie with the CTAs that its tiles fall to.
+template <bool BF16, int R>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttn p, int units) {
+    pdl_trigger();
+    pdl_wait();
+    const int item = blockIdx.x, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, r = blockIdx.y, hd = p.kv.hd, d = threadIdx.x;
+    const long long before = p.first[unit];
+    const int tiles = (int)(p.first[unit + 1] - before);
+    if (tiles == 0) return;
+    const long long total = p.first[units] * p.kv.nkv, a = before * p.kv.nkv + (long long)head * tiles, b = a + tiles;
+    const int n = share_count(total, p.ctas);
+    int c = (int)(a * n / total);
+    while (share_at(total, n, c + 1) <= a) c++;
+    while (share_at(total, n, c) > a) c--;
+    if (share_at(total, n, c + 1) >= b) return;  // one CTA had all of it
+    const PagedUnit u = paged_unit<R>(p, unit);
+    if (r >= u.rows) return;
+    const int slot0 = share_at(total, n, c) == a ? 0 : 1;
+    int c1 = c;
+    while (share_at(total, n, c1 + 1) < b) c1++;
+    float M = -INFINITY, L = 0.0f, o = 0.0f;
+    auto at = [&](int i) { return ((size_t)i * 2 + (i == c ? slot0 : 0)) * R + r; };
+    for (int i = c; i <= c1; i++) M = fmaxf(M, p.part_ml[at(i)].x);
+    for (int i = c; i <= c1; i++) {
+        const size_t w = at(i);
+        const float2 x = p.part_ml[w];
+        if (x.x == -INFINITY && x.y == 0.0f) continue;  // sees nothing of this part
+        const float f = ex2(x.x - M);
+        L += x.y * f;
+        o += p.part_o[w * hd + d] * f;
+    }
+    const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
+    const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
+    p.out[(u.tok0 + t) * p.os + (long long)(head * p.group + g) * hd + d] = (uint16_t)pack16<BF16>(o * inv, 0.0f);
+}
+
+struct AttnPlan {
+    int rows, row_tiles, units, ctas;
+    size_t bytes;
+};
+AttnPlan attn_plan(const Device *dev, int nseq, int nkv, int hd, int group, int max_new) {
+    AttnPlan a;
+    // up to 16 rows of a KV head: one m16 tile; more: two, so that half the row tiles read the cache again (heads of 256: one, registers)
+    a.rows = hd == 256 || (long long)group * max_new <= 16 ? 16 : 32;
+    a.row_tiles = (int)(((long long)group * max_new + a.rows - 1) / a.rows);
+    a.units = nseq * a.row_tiles;
+    a.ctas = dev->sm_count * (hd == 256 ? 1 : 2);
+    const size_t slots = (size_t)a.ctas * 2 * a.rows;
+    a.bytes = slots * hd * 4 + slots * 8 + ((size_t)a.units + 1) * 8;
+    return a;
+}
+
+template <bool BF16, int HD, int MT>
+int attn_launch(const Device *dev, const PagedAttn &p, int units, cudaStream_t st) {
+    using S = PaShape<HD, MT>;
+    static DeviceOnce once;
+    if (once.first(dev->ordinal)) IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, MT>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+    IM_CUDA_CHECK(launch_k(paged_attn_kernel<BF16, HD, MT>, dim3(p.ctas), dim3(kPaThreads), (size_t)S::kSmem, st, p, units));
+    IM_CUDA_CHECK(launch_k(paged_join_kernel<BF16, S::kRows>, dim3((unsigned)(units * p.kv.nkv), (unsigned)std::min<long long>(S::kRows, (long long)p.max_new * p.group)), dim3(HD),
+                           0, st, p, units));
+    return IM_OK;
+}
+
+int attn_check(const im_paged_kv *kv, int num_heads, int max_new) {
+    IM_REQUIRE(kv->head_dim == 64 || kv->head_dim == 128 || kv->head_dim == 256, "paged attention is built for heads of 64, 128 and 256 (got %d)", kv->head_dim);
+    IM_REQUIRE(num_heads > 0 && num_heads % kv->num_kv_heads == 0, "num_heads has to be a multiple of num_kv_heads (got %d and %d)", num_heads, kv->num_kv_heads);
+    IM_REQUIRE(max_new >= 1, "max_new has to be at least 1 (got %d)", max_new);
+    const long long tiles = ((long long)(num_heads / kv->num_kv_heads) * max_new + 15) / 16;
+    IM_REQUIRE(tiles * std::max(kv->num_seqs, 1) * kv->num_kv_heads <= 1 << 24, "%d sequences of %d new tokens are too many for one call", kv->num_seqs, max_new);
+    return IM_OK;
+}
+
+}  // namespace
+}  // namespace im
+
+IM_EXPORT size_t im_cuda_paged_attention_scratch_bytes(const im_device *dev, const im_paged_kv *kv, int num_heads, int max_new) {
+    im::PagedView v;
+    if (!dev || im::paged_view(kv, 0, &v) != IM_OK || im::attn_check(kv, num_heads, max_new) != IM_OK) return 0;
+    return im::attn_plan(dev, v.nseq, v.nkv, v.hd, num_heads / v.nkv, max_new).bytes;
+}
+
+IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int layer, const void *q_dev, int64_t q_stride, void *out_dev, int64_t out_stride,
+                                      int num_heads, const int *token_start_dev, int num_tokens, int max_new, const uint64_t *mask_dev, int mask_words,
+                                      float scale, int max_len, void *scratch_dev, size_t scratch_bytes, void *stream) {
+    IM_GUARD_BEGIN
+    using namespace im;
+    PagedAttn p;
+    IM_REQUIRE(layer >= 0, "layer %d", layer);
+    int rc = paged_view(kv, layer, &p.kv);
+    if (rc == IM_OK) rc = attn_check(kv, num_heads, max_new);
+    if (rc != IM_OK) return rc;
+    IM_REQUIRE(num_tokens >= 0 && max_len >= 0, "bad argument");
+    if (num_tokens == 0 || kv->num_seqs == 0) return paged_device(dev);
+    IM_REQUIRE(q_dev && out_dev && token_start_dev, "bad argument");
+    const int64_t row = (int64_t)num_heads * kv->head_dim, most = (int64_t)1 << 40;
+    IM_REQUIRE(q_stride >= row && out_stride >= row && q_stride <= most && out_stride <= most && q_stride % 8 == 0 && out_stride % 8 == 0 && aligned16(q_dev) && aligned16(out_dev),
+               "rows of queries and outputs have to be 16-byte aligned and apart");
+    IM_REQUIRE(!mask_dev || (mask_words >= 1 && mask_words <= 1 << 20), "a mask of %d words a token", mask_words);
+    IM_REQUIRE(scale == scale && scale - scale == 0.0f, "scale is not finite");
+    rc = paged_device(dev);
+    if (rc != IM_OK) return rc;
+    const AttnPlan plan = attn_plan(dev, p.kv.nseq, p.kv.nkv, p.kv.hd, num_heads / kv->num_kv_heads, max_new);
+    IM_REQUIRE(scratch_dev && aligned16(scratch_dev) && scratch_bytes >= plan.bytes, "paged attention needs %zu bytes of 16-byte aligned scratch (got %zu)", plan.bytes,
+               scratch_dev ? scratch_bytes : (size_t)0);
+    const int64_t at = layer * (int64_t)p.kv.layer_stride;
+    p.kc = static_cast<const uint16_t *>(kv->k_dev) + at;
+    p.vc = static_cast<const uint16_t *>(kv->v_dev) + at;
+    p.q = static_cast<const uint16_t *>(q_dev);
+    p.out = static_cast<uint16_t *>(out_dev);
+    p.qs = q_stride; p.os = out_stride;
+    p.start = token_start_dev;
+    p.mask = mask_dev; p.mask_words = mask_words;
+    p.nh = num_heads; p.group = num_heads / kv->num_kv_heads; p.tokens = num_tokens; p.max_new = max_new;
+    p.scale2 = scale * 1.4426950408889634f;
+    p.row_tiles = plan.row_tiles;
+    p.ctas = plan.ctas;
+    if (max_len > 0) {  // no more CTAs than tiles
+        const long long tiles = (long long)plan.units * p.kv.nkv * ((max_len + kPaTile - 1) / kPaTile);
+        p.ctas = (int)std::max(1ll, std::min<long long>(p.ctas, tiles));
+    }
+    const size_t slots = (size_t)plan.ctas * 2 * plan.rows;
+    p.part_o = static_cast<float *>(scratch_dev);
+    p.part_ml = reinterpret_cast<float2 *>(p.part_o + slots * p.kv.hd);
+    p.first = reinterpret_cast<long long *>(p.part_ml + slots);
+    const cudaStream_t st = as_stream(stream);
+    const bool bf16 = kv->dtype == IM_DTYPE_BF16;
+#define IM_RUN(HD, MT) (bf16 ? attn_launch<true, HD, MT>(dev, p, plan.units, st) : attn_launch<false, HD, MT>(dev, p, plan.units, st))
+    switch (kv->head_dim) {
+    case 64: return plan.rows == 16 ? IM_RUN(64, 1) : IM_RUN(64, 2);
+    case 128: return plan.rows == 16 ? IM_RUN(128, 1) : IM_RUN(128, 2);
+    default: return IM_RUN(256, 1);
+    }
+#undef IM_RUN
+    IM_GUARD_END
+}
