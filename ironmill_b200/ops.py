@@ -406,34 +406,30 @@ def sdpa_f16(dev: "Device", q, k_cache, v_cache, scale, nh, nkv, max_seq, base_p
 _DTYPES = {torch.float16: IM_DTYPE_F16, torch.float32: IM_DTYPE_F32, torch.bfloat16: IM_DTYPE_BF16}
 
 
-class _On:
-    """The device of a handle as the current one (the C ABI's rule), and its current stream."""
-
-    def __init__(self, ordinal: int):
-        self.ordinal, self.before = ordinal, None
-
-    def __enter__(self):
-        before = torch.cuda.current_device()
-        if before != self.ordinal:
-            self.before = before
-            torch.cuda.set_device(self.ordinal)
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *_):
-        if self.before is not None:
-            torch.cuda.set_device(self.before)
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream  # a call here costs a tenth of torch.cuda's
 
 
-def _rows_of(x: torch.Tensor, heads: int, dim: int, dtype, device):
-    """Elements between the tokens of x [tokens, heads, dim], whose heads lie side by side."""
-    assert x.dim() == 3 and x.shape[1] == heads and x.shape[2] == dim and x.dtype == dtype and x.device == device, (x.shape, x.dtype, x.device)
-    s = x.stride()
-    assert s[2] == 1 and (heads == 1 or s[1] == dim), s
-    return s[0] if x.shape[0] > 1 else heads * dim
+def _launch(ordinal: int, fn, *args) -> None:
+    """fn(*args, current stream) with the handle's device as the current one, as the C ABI asks for."""
+    if _current_device() != ordinal:
+        with torch.cuda.device(ordinal):
+            return _launch(ordinal, fn, *args)
+    check(fn(*args, _raw_stream(ordinal)))
 
 
-def _ints(x: torch.Tensor, device, *shape):
-    assert x.dtype == torch.int32 and x.device == device and x.is_contiguous() and x.shape == shape, (x.dtype, x.shape, x.device, shape)
+def _rows_of(x: torch.Tensor, n: int, heads: int, dim: int, dtype, ordinal: int) -> int:
+    """Elements between the tokens of x [n, heads, dim], whose heads lie side by side."""
+    tokens, h, d = x.shape
+    s, sh, sd = x.stride()
+    assert tokens == n and h == heads and d == dim and x.dtype is dtype and x.get_device() == ordinal, (x.shape, x.dtype, x.device)
+    assert sd == 1 and (sh == dim or h == 1), x.stride()
+    return s if n > 1 else heads * dim
+
+
+def _ints(x: torch.Tensor, ordinal: int, n: int, width: int = 0) -> int:
+    """Address of int32 [n] or [n, width] in one piece."""
+    assert x.dtype is torch.int32 and x.get_device() == ordinal and x.is_contiguous() and x.numel() == (n * width if width else n) and x.dim() == (2 if width else 1), \
+        (x.dtype, x.shape, x.device)
     return x.data_ptr()
 
 
@@ -448,7 +444,7 @@ class PagedKV:
         layers, pages, heads, page, dim = k_pages.shape
         s = k_pages.stride()
         assert s[4] == 1 and (page == 1 or s[3] == dim) and (heads == 1 or s[2] == page * dim), s
-        self.dev, self.k_pages, self.v_pages = dev, k_pages, v_pages
+        self.dev, self.k_pages, self.v_pages, self.ordinal = dev, k_pages, v_pages, dev.ordinal
         self.device, self.dtype, self.kv_heads, self.head_dim, self.layers = k_pages.device, k_pages.dtype, heads, dim, layers
         self.struct = PagedKvStruct(k_pages.data_ptr(), v_pages.data_ptr(), s[0] if layers > 1 else 0, s[1] if pages > 1 else 0, layers, pages, heads, page, dim,
                                     _DTYPES[k_pages.dtype])
@@ -460,10 +456,11 @@ class PagedKV:
         assert page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.device == self.device
         n, width = page_table.shape
         assert n == 0 or width == 1 or page_table.stride(1) == 1, page_table.stride()
-        self.struct.seq_len_dev = _ints(lengths, self.device, n)
+        self.struct.seq_len_dev = _ints(lengths, self.ordinal, n)
         self.struct.num_seqs, self.struct.page_table_dev, self.struct.table_width = n, page_table.data_ptr(), width
         self.struct.table_stride = page_table.stride(0) if n > 1 else 0
         self.page_table, self.lengths, self.num_seqs = page_table, lengths, n
+        self.scratch_bytes = {}  # of attention, by heads and new tokens
 
 
 def paged_append(kv: PagedKV, layer: int, k, v, token_start, q=None, cos=None, sin=None, positions=None, rotary_dim=None, neighbours=False, q_out=None):
@@ -471,74 +468,76 @@ def paged_append(kv: PagedKV, layer: int, k, v, token_start, q=None, cos=None, s
     way (returned in q_out, which may be q). token_start int32 [sequences + 1]; cos, sin [positions, head_dim / 2] fp16 or f32; positions
     int32 [tokens]: rows of the tables, where they are not the rows of the cache; neighbours: columns (2 i, 2 i + 1) belong together
     instead of the halves'. Without tables nothing is rotated."""
-    n, dim, dev = k.shape[0], kv.head_dim, kv.device
-    ks, vs = _rows_of(k, kv.kv_heads, dim, kv.dtype, dev), _rows_of(v, kv.kv_heads, dim, kv.dtype, dev)
-    assert v.shape[0] == n
-    heads = qs = qos = max_pos = 0
+    n, dim, dtype, on = k.shape[0], kv.head_dim, kv.dtype, kv.ordinal
+    ks, vs = _rows_of(k, n, kv.kv_heads, dim, dtype, on), _rows_of(v, n, kv.kv_heads, dim, dtype, on)
+    heads = qs = qos = max_pos = table = 0
+    qp = op = cp = sp = None
     if q is not None:
         heads = q.shape[1]
-        qs = _rows_of(q, heads, dim, kv.dtype, dev)
+        qs, qp = _rows_of(q, n, heads, dim, dtype, on), q.data_ptr()
         if q_out is None:
-            q_out = torch.empty((n, heads, dim), dtype=q.dtype, device=dev)
-        qos = _rows_of(q_out, heads, dim, kv.dtype, dev)
-        assert q.shape[0] == n and q_out.shape[0] == n
+            q_out = q.new_empty((n, heads, dim))
+            qos = heads * dim
+        else:
+            qos = _rows_of(q_out, n, heads, dim, dtype, on)
+        op = q_out.data_ptr()
     else:
         assert q_out is None
-    table = 0
     if cos is not None:
-        max_pos = cos.shape[0]
-        assert sin.shape == cos.shape and cos.shape[1] == dim // 2 and cos.dtype == sin.dtype and cos.is_contiguous() and sin.is_contiguous() and cos.device == dev == sin.device
-        table = _DTYPES[cos.dtype]
+        max_pos, half = cos.shape
+        assert sin.shape == cos.shape and half == dim // 2 and cos.dtype is sin.dtype and cos.is_contiguous() and sin.is_contiguous()
+        assert cos.get_device() == on and sin.get_device() == on
+        table, cp, sp = _DTYPES[cos.dtype], cos.data_ptr(), sin.data_ptr()
         rotary_dim = dim if rotary_dim is None else rotary_dim
     else:
         assert sin is None and not rotary_dim
         rotary_dim = 0
-    with _On(kv.dev.ordinal) as stream:
-        check(lib().im_cuda_paged_append(kv.dev.handle, kv.ref, layer, k.data_ptr(), ks, v.data_ptr(), vs, _ints(token_start, dev, kv.num_seqs + 1), n,
-                                         q.data_ptr() if heads else None, qs, q_out.data_ptr() if heads else None, qos, heads,
-                                         cos.data_ptr() if max_pos else None, sin.data_ptr() if max_pos else None, table, max_pos, rotary_dim, int(neighbours),
-                                         None if positions is None else _ints(positions, dev, n), stream))
+    _launch(on, lib().im_cuda_paged_append, kv.dev.handle, kv.ref, layer, k.data_ptr(), ks, v.data_ptr(), vs, _ints(token_start, on, kv.num_seqs + 1), n, qp, qs, op, qos,
+            heads, cp, sp, table, max_pos, rotary_dim, 1 if neighbours else 0, None if positions is None else _ints(positions, on, n))
     return q_out
 
 
 def paged_attention_scratch(kv: PagedKV, heads: int, max_new: int) -> torch.Tensor:
     """Scratch for paged_attention calls of this cache with so many heads and new tokens; calls that may overlap need one each."""
-    nbytes = int(lib().im_cuda_paged_attention_scratch_bytes(kv.dev.handle, kv.ref, heads, max_new))
-    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=kv.device)
+    nbytes = kv.scratch_bytes.get((heads, max_new))
+    if nbytes is None:
+        nbytes = kv.scratch_bytes[heads, max_new] = max(int(lib().im_cuda_paged_attention_scratch_bytes(kv.dev.handle, kv.ref, heads, max_new)), 16)
+    return torch.empty(nbytes, dtype=torch.uint8, device=kv.device)
 
 
 def paged_attention(kv: PagedKV, layer: int, q, token_start, max_new: int, scale: float, mask=None, max_len=0, out=None, scratch=None):
     """softmax(scale * q K^T) V of new tokens q [tokens, heads, head_dim] whose rows are in the pages: every token sees the `lengths` rows before
     the new ones and, without a mask, its own and the new ones before it; with mask int64 [tokens, words] the new ones whose bits
     are set (of a drafted tree: its ancestors and itself). max_new, max_len: the most new tokens and rows of a sequence."""
-    n, heads, dev = q.shape[0], q.shape[1], kv.device
-    qs = _rows_of(q, heads, kv.head_dim, kv.dtype, dev)
+    n, heads, dim = q.shape
+    on = kv.ordinal
+    qs = _rows_of(q, n, heads, kv.head_dim, kv.dtype, on)
     if out is None:
-        out = torch.empty((n, heads, kv.head_dim), dtype=q.dtype, device=dev)
-    assert out.shape[0] == n
-    os_ = _rows_of(out, heads, kv.head_dim, kv.dtype, dev)
-    words = 0
+        out = q.new_empty((n, heads, dim))
+        os_ = heads * dim
+    else:
+        os_ = _rows_of(out, n, heads, dim, kv.dtype, on)
+    words, mp = 0, None
     if mask is not None:
-        words = mask.shape[1]
-        assert mask.dtype == torch.int64 and mask.shape[0] == n and mask.is_contiguous() and mask.device == dev
+        rows, words = mask.shape
+        assert mask.dtype is torch.int64 and rows == n and mask.is_contiguous() and mask.get_device() == on
+        mp = mask.data_ptr()
     if scratch is None:
         scratch = paged_attention_scratch(kv, heads, max_new)
-    assert scratch.dtype == torch.uint8 and scratch.device == dev and scratch.is_contiguous()
-    with _On(kv.dev.ordinal) as stream:
-        check(lib().im_cuda_paged_attention(kv.dev.handle, kv.ref, layer, q.data_ptr(), qs, out.data_ptr(), os_, heads, _ints(token_start, dev, kv.num_seqs + 1), n,
-                                            max_new, mask.data_ptr() if words else None, words, scale, max_len, scratch.data_ptr(), scratch.numel(), stream))
+    else:
+        assert scratch.dtype is torch.uint8 and scratch.get_device() == on and scratch.is_contiguous()
+    _launch(on, lib().im_cuda_paged_attention, kv.dev.handle, kv.ref, layer, q.data_ptr(), qs, out.data_ptr(), os_, heads, _ints(token_start, on, kv.num_seqs + 1), n, max_new,
+            mp, words, scale, max_len, scratch.data_ptr(), scratch.numel())
     return out
 
 
 def paged_keep(kv: PagedKV, accepted, counts, lengths_out=None):
     """The accepted path of every drafted tree, accepted int32 [sequences, most] (places among the new rows, from the root on), counts int32
     [sequences], moves up behind the rows before it, in every layer. Returns the new lengths (kv.point_at)."""
-    most = accepted.shape[1]
+    most, n, on = accepted.shape[1], kv.num_seqs, kv.ordinal
     if lengths_out is None:
-        lengths_out = torch.empty(kv.num_seqs, dtype=torch.int32, device=kv.device)
-    with _On(kv.dev.ordinal) as stream:
-        check(lib().im_cuda_paged_keep(kv.dev.handle, kv.ref, _ints(accepted, kv.device, kv.num_seqs, most), most, _ints(counts, kv.device, kv.num_seqs),
-                                       _ints(lengths_out, kv.device, kv.num_seqs), stream))
+        lengths_out = torch.empty_like(kv.lengths)
+    _launch(on, lib().im_cuda_paged_keep, kv.dev.handle, kv.ref, _ints(accepted, on, n, most), most, _ints(counts, on, n), _ints(lengths_out, on, n))
     return lengths_out
 
 
@@ -546,14 +545,15 @@ def paged_reorder(kv: PagedKV, parents, group: int, table_out=None, lengths_out=
     """Beam i of every group of sequences becomes a copy of beam parents[i] (int32 [sequences]): pages are shared up to the last one, whose rows
     are copied where a parent has several children, into the pages of a beam that has none. From its last page on a row's pages are its own. Returns the new page table and lengths (kv.point_at)."""
     n, width = kv.page_table.shape
+    on = kv.ordinal
     if table_out is None:
-        table_out = torch.empty((n, width), dtype=torch.int32, device=kv.device)
+        table_out, stride = kv.page_table.new_empty((n, width)), width
+    else:
+        assert table_out.shape == (n, width) and table_out.dtype is torch.int32 and table_out.get_device() == on and (n == 0 or width == 1 or table_out.stride(1) == 1)
+        stride = table_out.stride(0) if n > 1 else 0
     if lengths_out is None:
-        lengths_out = torch.empty(n, dtype=torch.int32, device=kv.device)
-    assert table_out.shape == (n, width) and table_out.dtype == torch.int32 and table_out.device == kv.device and (n == 0 or width == 1 or table_out.stride(1) == 1)
-    with _On(kv.dev.ordinal) as stream:
-        check(lib().im_cuda_paged_reorder(kv.dev.handle, kv.ref, _ints(parents, kv.device, n), group, table_out.data_ptr(), table_out.stride(0) if n > 1 else 0,
-                                          _ints(lengths_out, kv.device, n), stream))
+        lengths_out = torch.empty_like(kv.lengths)
+    _launch(on, lib().im_cuda_paged_reorder, kv.dev.handle, kv.ref, _ints(parents, on, n), group, table_out.data_ptr(), stride, _ints(lengths_out, on, n))
     return table_out, lengths_out
 
 
@@ -569,21 +569,19 @@ def beam_select(dev: Device, logits, scores, picks: int, done=None, end_token=-1
     [groups, beams], done bool [groups, beams]. Returns scores f32, parents and tokens int32 [groups, picks], best first, ties to
     the lowest beam and token; a finished beam has one continuation, end_token at its own score."""
     groups, beams, vocab = logits.shape
-    device = logits.device
-    assert device.type == "cuda" and device.index == dev.ordinal and logits.dtype in _DTYPES
-    s = logits.stride()
-    row = s[1] if beams > 1 else s[0]
-    assert s[2] == 1 and (groups == 1 or beams == 1 or s[0] == beams * s[1]), s
-    assert scores.shape == (groups, beams) and scores.dtype == torch.float32 and scores.is_contiguous() and scores.device == device
+    on, (sg, sb, sv) = dev.ordinal, logits.stride()
+    assert logits.get_device() == on and (sv == 1 or vocab == 1) and (groups == 1 or beams == 1 or sg == beams * sb), logits.stride()
+    assert scores.shape == (groups, beams) and scores.dtype is torch.float32 and scores.is_contiguous() and scores.get_device() == on
+    dp = None
     if done is not None:
-        assert done.shape == (groups, beams) and done.dtype in (torch.bool, torch.uint8) and done.is_contiguous() and done.device == device
+        assert done.shape == (groups, beams) and done.dtype in (torch.bool, torch.uint8) and done.is_contiguous() and done.get_device() == on
+        dp = done.data_ptr()
     if scratch is None:
         scratch = beam_select_scratch(dev, groups, beams, vocab, picks)
-    assert scratch.dtype == torch.uint8 and scratch.device == device and scratch.is_contiguous()
-    score = torch.empty((groups, picks), dtype=torch.float32, device=device)
-    parent, token = torch.empty((2, groups, picks), dtype=torch.int32, device=device)
-    with _On(dev.ordinal) as stream:
-        check(lib().im_cuda_beam_select(dev.handle, logits.data_ptr(), _DTYPES[logits.dtype], row if groups * beams > 1 else 0, groups, beams, vocab, scores.data_ptr(),
-                                        None if done is None else done.data_ptr(), end_token, picks, score.data_ptr(), parent.data_ptr(), token.data_ptr(),
-                                        scratch.data_ptr(), scratch.numel(), stream))
+    else:
+        assert scratch.dtype is torch.uint8 and scratch.get_device() == on and scratch.is_contiguous()
+    score = scores.new_empty((groups, picks))
+    parent, token = score.new_empty((2, groups, picks), dtype=torch.int32).unbind(0)
+    _launch(on, lib().im_cuda_beam_select, dev.handle, logits.data_ptr(), _DTYPES[logits.dtype], (sb if beams > 1 else sg) if groups * beams > 1 else 0, groups, beams, vocab,
+            scores.data_ptr(), dp, end_token, picks, score.data_ptr(), parent.data_ptr(), token.data_ptr(), scratch.data_ptr(), scratch.numel())
     return score, parent, token
