@@ -18,14 +18,13 @@
 //
 // Bound: 2 x 128 x PN x (DK + 128 per term) products and 128 x PN exponentials (16 a clock and SM) per half and tile; both are about
 // 1000 clocks at DK = PN = 128. 2048 tokens, 16 heads: 128 columns fp16 84 us, two bf16 terms 92 us, 192/128 columns 89 us (mma.sync kernels: 221, 255, 265).
-#include <cuda_bf16.h>
 #include <math.h>
 
 #include <type_traits>
 
 #include "flash_tc.cuh"
 #include "tmap.cuh"
-#include "v2_device.cuh"
+#include "umma.cuh"
 
 namespace im {
 
@@ -54,24 +53,6 @@ struct FlashShape {
     static constexpr int kSmem = 1024 + kQ + kStages * (kK + kV + kFactors) + (4 * kStages + 7) * 8 + 16;
 };
 
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo_bytes) {
-    // shared-memory matrix descriptor, 128-byte swizzle (layout type 2), version 1; stride offset 1024 B between groups of eight
-    // rows of 128 B. The leading offset matters for MN-major operands only: bytes between 64-element column blocks.
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo_bytes >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0)
-                 : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {  // A operand in tensor memory
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0)
-                 : "memory");
-}
-__device__ __forceinline__ void commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
 __device__ __forceinline__ void tma_2d(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {  // x: a multiple of eight elements (flash_takes)
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)), "l"(map),
                  "r"(x), "r"(y), "r"(smem_u32(bar))
@@ -81,65 +62,6 @@ __device__ __forceinline__ void bulk_copy(void *dst, const void *src, uint32_t b
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
                  "r"(smem_u32(bar))
                  : "memory");
-}
-__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t *r) {  // no wait: tmem_wait_ld
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32"
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
-        " %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
-          "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
-          "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t *r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32],"
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
-        " %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};\n" ::"r"(r[0]),
-        "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
-        "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]),
-        "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// The whole warp waits; the hardware suspends a try_wait for a while, so no back-off on these short waits.
-__device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity, int *err) {
-    bool ok = mbar_try_wait(bar, parity);
-    if (!ok) {
-        const unsigned long long t0 = global_ns();
-        for (unsigned i = 1; !ok; i++) {
-            ok = mbar_try_wait(bar, parity);
-            if (!ok && (i & 255u) == 0 && global_ns() - t0 > kWaitLimitNs) {
-                atomicExch(err, 1);
-                break;
-            }
-        }
-    }
-    return __all_sync(0xffffffffu, ok);
-}
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    if (BF16) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-        return *reinterpret_cast<const uint32_t *>(&h);
-    }
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-template <bool BF16>
-__device__ __forceinline__ float2 unpack2(uint32_t u) {
-    if (BF16) return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-    return __half22float2(*reinterpret_cast<const __half2 *>(&u));
 }
 __device__ __forceinline__ int chunk_start(int chunk, int pos) { return chunk > 0 ? pos / chunk * chunk : 0; }
 

@@ -34,12 +34,6 @@ struct PaShape {
     static constexpr int kSmem = kRing + kQ + kMerge + kPaWarps * kRows * 8;
 };
 
-__device__ __forceinline__ uint32_t sm32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
@@ -61,109 +55,6 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool there) 
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 
-// Inclusive sums of v over the block's threads in sums[], the total returned.
-__device__ __forceinline__ long long block_scan(int v, long long *sums) {
-    __shared__ long long of_warp[kPaWarps];
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    long long s = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long t = __shfl_up_sync(0xffffffffu, s, o);
-        if (lane >= o) s += t;
-    }
-    __syncthreads();
-    if (lane == 31) of_warp[w] = s;
-    __syncthreads();
-    long long before = 0, total = 0;
-#pragma unroll
-    for (int i = 0; i < kPaWarps; i++) {
-        if (i < w) before += of_warp[i];
-        total += of_warp[i];
-    }
-    sums[threadIdx.x] = s + before;
-    __syncthreads();
-    return total;
-}
-
-template <int R>
-__device__ __forceinline__ int unit_tiles(const PagedUnit &u) { return (u.end + kPaTile - 1) / kPaTile; }
-
-// Where a CTA's share starts.
-struct Share {
-    long long from, to;  // places in the list of all tiles
-    int unit, head, tile;
-};
-
-// No share is empty: CTAs without a tile of their own have none, and leave no parts.
-__device__ __forceinline__ int share_count(long long total, int ctas) { return (int)min((long long)ctas, total); }
-__device__ __forceinline__ long long share_at(long long total, int n, int c) { return c >= n ? total : total * c / n; }
-
-template <int R>
-__device__ __forceinline__ Share find_share(const PagedAttn &p, int units, long long *sums) {
-    __shared__ int found[3];
-    Share s;
-    long long total = 0;
-    for (int u0 = 0; u0 < units; u0 += kPaThreads) {
-        const int u = u0 + threadIdx.x;
-        const int n = u < units ? unit_tiles<R>(paged_unit<R>(p, u)) : 0;
-        const long long all = block_scan(n, sums);
-        if (blockIdx.x == 0 && u < units) p.first[u] = total + sums[threadIdx.x] - n;
-        total += all;
-    }
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.first[units] = total;
-    total *= p.kv.nkv;
-    const int shares = share_count(total, p.ctas);
-    s.from = share_at(total, shares, blockIdx.x);
-    s.to = share_at(total, shares, blockIdx.x + 1);
-    s.unit = s.head = s.tile = 0;
-    if (s.from >= s.to) return s;
-    long long before = 0;
-    for (int u0 = 0; u0 < units; u0 += kPaThreads) {
-        const int u = u0 + threadIdx.x;
-        const int n = u < units ? unit_tiles<R>(paged_unit<R>(p, u)) : 0;
-        const long long all = block_scan(n, sums);
-        const long long a = (before + sums[threadIdx.x] - n) * p.kv.nkv;
-        if (n > 0 && s.from >= a && s.from < a + (long long)n * p.kv.nkv) {
-            const int d = (int)(s.from - a);
-            found[0] = u;
-            found[1] = d / n;
-            found[2] = d % n;
-        }
-        before += all;
-        if (before * p.kv.nkv > s.from) break;
-    }
-    __syncthreads();
-    s.unit = found[0];
-    s.head = found[1];
-    s.tile = found[2];
-    return s;
-}
-
-// A row whose sums are not finite, from the positions it sees alone: on the tensor cores a weight of zero times an infinite or missing value of a
-// position that the row does not see is a NaN. A warp per row; o: this lane's columns (lane, lane + 32, ...).
-template <bool BF16, int HD>
-__device__ __noinline__ void plain_row(const PagedAttn &p, const PagedUnit &u, int head, int r, int from, int to, float *o, float &m, float &l) {
-    const int lane = threadIdx.x & 31, t = (u.row0 + r) / p.group, h = head * p.group + (u.row0 + r) % p.group;
-    const uint16_t *q = p.q + (u.tok0 + t) * p.qs + (long long)h * HD;
-    m = -INFINITY;
-    l = 0.0f;
-    for (int i = 0; i < HD / 32; i++) o[i] = 0.0f;
-    for (int pos = from; pos < to; pos++) {
-        if (!paged_sees(p, u, t, pos)) continue;
-        long long at = p.kv.row_of(u.seq, pos);
-        if (at < 0) continue;
-        at += (long long)head * p.kv.page * HD;
-        float s = 0.0f;
-        for (int i = 0; i < HD / 32; i++) s = fmaf(one16<BF16>(q + lane + 32 * i), one16<BF16>(p.kc + at + lane + 32 * i), s);
-        s = warp_sum(s) * p.scale2;
-        if (s == -INFINITY) continue;
-        const float m_new = fmaxf(m, s), corr = ex2(m - m_new), w = ex2(s - m_new);
-        m = m_new;
-        l = l * corr + w;
-        for (int i = 0; i < HD / 32; i++) o[i] = fmaf(w, one16<BF16>(p.vc + at + lane + 32 * i), o[i] * corr);
-    }
-}
-
 template <bool BF16, int HD, int MT>
 __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kernel(const __grid_constant__ PagedAttn p, int units) {
     using S = PaShape<HD, MT>;
@@ -180,14 +71,14 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
     if (tid < 2) bad_rows[tid] = 0;
     pdl_trigger();
     pdl_wait();
-    const Share share = find_share<R>(p, units, sums);
+    const Share share = find_share<R, kPaTile, kPaThreads>(p, units, sums);
     if (share.from >= share.to) return;
     const int count = (int)(share.to - share.from);
 
     // ---- the copies' cursor: one slice ahead of the copies, so that a page number is there when it is needed
     int f_unit = share.unit, f_head = share.head, f_tile = share.tile, f_left = count;
     PagedUnit f_u = paged_unit<R>(p, f_unit);
-    int f_tiles = unit_tiles<R>(f_u);
+    int f_tiles = unit_tiles<kPaTile>(f_u);
     int n_page = -1, n_slot = 0, n_head = 0;  // of the slice that is copied next: this lane's row (lane & 15)
     auto fetch = [&]() {
         n_page = -1;
@@ -206,7 +97,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
                 f_head = 0;
                 while (f_left > 0 && ++f_unit < units) {
                     f_u = paged_unit<R>(p, f_unit);
-                    f_tiles = unit_tiles<R>(f_u);
+                    f_tiles = unit_tiles<kPaTile>(f_u);
                     if (f_tiles > 0) break;
                 }
             }
@@ -215,7 +106,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
     auto copy = [&](int stage) {  // the slice whose rows fetch() looked up
         const bool there = (unsigned)n_page < (unsigned)p.kv.pages;
         const long long off = there ? n_page * p.kv.page_stride + ((long long)n_head * p.kv.page + n_slot) * HD : -1;
-        const uint32_t dst = sm32(ring) + stage * 2 * S::kSliceBytes;
+        const uint32_t dst = smem_u32(ring) + stage * 2 * S::kSliceBytes;
         const unsigned all = __ballot_sync(0xffffffffu, there);
         if (lane == 0) rows_there[warp][stage] = all;
         constexpr int RPI = 32 / CH > 0 ? 32 / CH : 1;  // rows of one request of the warp
@@ -250,7 +141,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
     int odd_item = 0;
     while (done < count) {
         PagedUnit u = paged_unit<R>(p, unit);
-        const int tiles = unit_tiles<R>(u);
+        const int tiles = unit_tiles<kPaTile>(u);
         if (tiles == 0) {
             unit++;
             continue;
@@ -310,7 +201,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
             asm volatile("cp.async.commit_group;" ::: "memory");
             asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
             __syncwarp();
-            const uint32_t ks_at = sm32(ring) + stage * 2 * S::kSliceBytes, vs_at = ks_at + S::kSliceBytes;
+            const uint32_t ks_at = smem_u32(ring) + stage * 2 * S::kSliceBytes, vs_at = ks_at + S::kSliceBytes;
             float s[MT][2][4];
 #pragma unroll
             for (int mt = 0; mt < MT; mt++)
@@ -332,7 +223,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
                         } else {
                             uint32_t a[4];
                             const int qr = mt * 16 + (lane & 15), qc = 2 * ks + (lane >> 4);
-                            ldsm4(a, sm32(qsm) + qr * (HD * 2) + ((qc ^ (qr & 7)) << 4));
+                            ldsm4(a, smem_u32(qsm) + qr * (HD * 2) + ((qc ^ (qr & 7)) << 4));
                             mma16<BF16>(s[mt][0], a, b[0], b[1]);
                             mma16<BF16>(s[mt][1], a, b[2], b[3]);
                         }
@@ -554,19 +445,28 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttn p, int 
 }
 
 struct AttnPlan {
-    int rows, row_tiles, units, ctas;
+    int rows, tile, row_tiles, units, ctas;
     size_t bytes;
 };
 AttnPlan attn_plan(const Device *dev, int nseq, int nkv, int hd, int group, int max_new) {
     AttnPlan a;
     // up to 16 rows of a KV head: one m16 tile; more: two, so that half the row tiles read the cache again (heads of 256: one, registers)
-    a.rows = hd == 256 || (long long)group * max_new <= 16 ? 16 : 32;
+    const int tc = paged_tc_rows(hd, (long long)group * max_new);
+    a.tile = tc ? 128 : kPaTile;
+    a.rows = tc ? tc : hd == 256 || (long long)group * max_new <= 16 ? 16 : 32;
     a.row_tiles = (int)(((long long)group * max_new + a.rows - 1) / a.rows);
     a.units = nseq * a.row_tiles;
-    a.ctas = dev->sm_count * (hd == 256 ? 1 : 2);
+    a.ctas = dev->sm_count * (tc || hd == 256 ? 1 : 2);
     const size_t slots = (size_t)a.ctas * 2 * a.rows;
     a.bytes = slots * hd * 4 + slots * 8 + ((size_t)a.units + 1) * 8;
     return a;
+}
+
+template <bool BF16, int R>
+int join_launch(const PagedAttn &p, int units, cudaStream_t st) {
+    IM_CUDA_CHECK(launch_k(paged_join_kernel<BF16, R>, dim3((unsigned)(units * p.kv.nkv), (unsigned)std::min<long long>(R, (long long)p.max_new * p.group)), dim3(p.kv.hd), 0, st, p,
+                           units));
+    return IM_OK;
 }
 
 template <bool BF16, int HD, int MT>
@@ -575,9 +475,7 @@ int attn_launch(const Device *dev, const PagedAttn &p, int units, cudaStream_t s
     static DeviceOnce once;
     if (once.first(dev->ordinal)) IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, MT>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     IM_CUDA_CHECK(launch_k(paged_attn_kernel<BF16, HD, MT>, dim3(p.ctas), dim3(kPaThreads), (size_t)S::kSmem, st, p, units));
-    IM_CUDA_CHECK(launch_k(paged_join_kernel<BF16, S::kRows>, dim3((unsigned)(units * p.kv.nkv), (unsigned)std::min<long long>(S::kRows, (long long)p.max_new * p.group)), dim3(HD),
-                           0, st, p, units));
-    return IM_OK;
+    return join_launch<BF16, S::kRows>(p, units, st);
 }
 
 int attn_check(const im_paged_kv *kv, int num_heads, int max_new) {
@@ -634,7 +532,7 @@ IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int
     p.row_tiles = plan.row_tiles;
     p.ctas = plan.ctas;
     if (max_len > 0) {  // no more CTAs than tiles
-        const long long tiles = (long long)plan.units * p.kv.nkv * ((max_len + kPaTile - 1) / kPaTile);
+        const long long tiles = (long long)plan.units * p.kv.nkv * ((max_len + (long long)plan.tile - 1) / plan.tile);
         p.ctas = (int)std::max(1ll, std::min<long long>(p.ctas, tiles));
     }
     const size_t slots = (size_t)plan.ctas * 2 * plan.rows;
@@ -643,6 +541,12 @@ IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int
     p.first = reinterpret_cast<long long *>(p.part_ml + slots);
     const cudaStream_t st = as_stream(stream);
     const bool bf16 = kv->dtype == IM_DTYPE_BF16;
+    if (plan.rows >= 128) {
+        rc = paged_tc_launch(dev, p, bf16, plan.rows, plan.units, st);
+        if (rc != IM_OK) return rc;
+        if (plan.rows == 128) return bf16 ? join_launch<true, 128>(p, plan.units, st) : join_launch<false, 128>(p, plan.units, st);
+        return bf16 ? join_launch<true, 256>(p, plan.units, st) : join_launch<false, 256>(p, plan.units, st);
+    }
 #define IM_RUN(HD, MT) (bf16 ? attn_launch<true, HD, MT>(dev, p, plan.units, st) : attn_launch<false, HD, MT>(dev, p, plan.units, st))
     switch (kv->head_dim) {
     case 64: return plan.rows == 16 ? IM_RUN(64, 1) : IM_RUN(64, 2);

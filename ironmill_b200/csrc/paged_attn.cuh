@@ -1,6 +1,7 @@
 // Attention over a paged cache: what its kernels share (paged_attn.cu).
 #pragma once
 #include "paged.cuh"
+#include "umma.cuh"
 
 namespace im {
 
@@ -53,5 +54,114 @@ __device__ __forceinline__ bool paged_sees(const PagedAttn &p, const PagedUnit &
     if (!p.mask) return d <= t;
     return d < 64 * p.mask_words && ((__ldg(p.mask + (long long)(u.tok0 + t) * p.mask_words + (d >> 6)) >> (d & 63)) & 1);
 }
+
+// Inclusive sums of v over the block's threads in sums[], the total returned.
+template <int THREADS>
+__device__ __forceinline__ long long block_scan(int v, long long *sums) {
+    __shared__ long long of_warp[THREADS / 32];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    long long s = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long t = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += t;
+    }
+    __syncthreads();
+    if (lane == 31) of_warp[w] = s;
+    __syncthreads();
+    long long before = 0, total = 0;
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; i++) {
+        if (i < w) before += of_warp[i];
+        total += of_warp[i];
+    }
+    sums[threadIdx.x] = s + before;
+    __syncthreads();
+    return total;
+}
+
+template <int TILE>
+__device__ __forceinline__ int unit_tiles(const PagedUnit &u) { return (u.end + TILE - 1) / TILE; }
+
+// Where a CTA's share starts.
+struct Share {
+    long long from, to;  // places in the list of all tiles
+    int unit, head, tile;
+};
+
+// No share is empty: CTAs without a tile of their own have none, and leave no parts.
+__device__ __forceinline__ int share_count(long long total, int ctas) { return (int)min((long long)ctas, total); }
+__device__ __forceinline__ long long share_at(long long total, int n, int c) { return c >= n ? total : total * c / n; }
+
+template <int R, int TILE, int THREADS>
+__device__ __forceinline__ Share find_share(const PagedAttn &p, int units, long long *sums) {
+    __shared__ int found[3];
+    Share s;
+    long long total = 0;
+    for (int u0 = 0; u0 < units; u0 += THREADS) {
+        const int u = u0 + threadIdx.x;
+        const int n = u < units ? unit_tiles<TILE>(paged_unit<R>(p, u)) : 0;
+        const long long all = block_scan<THREADS>(n, sums);
+        if (blockIdx.x == 0 && u < units) p.first[u] = total + sums[threadIdx.x] - n;
+        total += all;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.first[units] = total;
+    total *= p.kv.nkv;
+    const int shares = share_count(total, p.ctas);
+    s.from = share_at(total, shares, blockIdx.x);
+    s.to = share_at(total, shares, blockIdx.x + 1);
+    s.unit = s.head = s.tile = 0;
+    if (s.from >= s.to) return s;
+    long long before = 0;
+    for (int u0 = 0; u0 < units; u0 += THREADS) {
+        const int u = u0 + threadIdx.x;
+        const int n = u < units ? unit_tiles<TILE>(paged_unit<R>(p, u)) : 0;
+        const long long all = block_scan<THREADS>(n, sums);
+        const long long a = (before + sums[threadIdx.x] - n) * p.kv.nkv;
+        if (n > 0 && s.from >= a && s.from < a + (long long)n * p.kv.nkv) {
+            const int d = (int)(s.from - a);
+            found[0] = u;
+            found[1] = d / n;
+            found[2] = d % n;
+        }
+        before += all;
+        if (before * p.kv.nkv > s.from) break;
+    }
+    __syncthreads();
+    s.unit = found[0];
+    s.head = found[1];
+    s.tile = found[2];
+    return s;
+}
+
+// A row whose sums are not finite, from the positions it sees alone: on the tensor cores a weight of zero times an infinite or missing value of a
+// position that the row does not see is a NaN. A warp per row; o: this lane's columns (lane, lane + 32, ...).
+template <bool BF16, int HD>
+__device__ __noinline__ void plain_row(const PagedAttn &p, const PagedUnit &u, int head, int r, int from, int to, float *o, float &m, float &l) {
+    const int lane = threadIdx.x & 31, t = (u.row0 + r) / p.group, h = head * p.group + (u.row0 + r) % p.group;
+    const uint16_t *q = p.q + (u.tok0 + t) * p.qs + (long long)h * HD;
+    m = -INFINITY;
+    l = 0.0f;
+    for (int i = 0; i < HD / 32; i++) o[i] = 0.0f;
+    for (int pos = from; pos < to; pos++) {
+        if (!paged_sees(p, u, t, pos)) continue;
+        long long at = p.kv.row_of(u.seq, pos);
+        if (at < 0) continue;
+        at += (long long)head * p.kv.page * HD;
+        float s = 0.0f;
+        for (int i = 0; i < HD / 32; i++) s = fmaf(one16<BF16>(q + lane + 32 * i), one16<BF16>(p.kc + at + lane + 32 * i), s);
+        s = warp_sum(s) * p.scale2;
+        if (s == -INFINITY) continue;
+        const float m_new = fmaxf(m, s), corr = ex2(m - m_new), w = ex2(s - m_new);
+        m = m_new;
+        l = l * corr + w;
+        for (int i = 0; i < HD / 32; i++) o[i] = fmaf(w, one16<BF16>(p.vc + at + lane + 32 * i), o[i] * corr);
+    }
+}
+
+// Many rows of a KV head on the tcgen05 tensor cores (paged_attn_tc.cu): rows of a tile for so many rows of a sequence, 0 where the
+// kernel of paged_attn.cu is the one to use; CTAs = SMs.
+int paged_tc_rows(int hd, long long rows);
+int paged_tc_launch(const Device *dev, const PagedAttn &p, bool bf16, int rows, int units, cudaStream_t st);
 
 }  // namespace im

@@ -1,0 +1,517 @@
+// Attention over a paged cache on the 5th-generation tensor cores, for many rows (token, query head) of a KV head: trees and portions of prompts.
+//
+// One CTA per SM walks an equal share of the list of all (row tile, KV head) items' tiles of 128 positions (paged_attn.cu has the scheme and joins
+// what the cuts divide). Two sets of four warps ("halves") turn scores into weights, a row per thread; while one of them works, the other's products run:
+//     S = Q K^T    both operands in shared memory, accumulator in tensor memory (f32)
+//     P = exp2(S)  to registers, running maximum and sum in f32, weights back over the scores as two 16-bit terms (weight, and what its rounding left)
+//     O += P V     P from tensor memory, V with the head dimension contiguous
+// A tile of up to 256 rows (WIDE): the halves own 128 rows each and every tile of K and V serves both. Up to 128 rows: the halves own the even
+// and the odd tiles of the share, with accumulators of their own that are joined where the item ends.
+// A row's accumulator is rescaled only when its maximum has grown by more than 2^8 (as in flash_tc.cu).
+//
+// K, V and queries come by 16-byte cp.async of two warps, rows looked up in the page table: any page size, rows that are not there are zeros and
+// known to be none (a bit per row). The copies run ahead over the ends of items; each is announced when it has landed and been made
+// visible to the tensor cores, the announcement lagging kLag copies behind the requests, or at once where the ring is full.
+//
+// All waits are bounded: one that runs out sets the device error word, every warp then runs to its end.
+#include <limits.h>
+#include <math.h>
+
+#include <algorithm>
+
+#include "paged_attn.cuh"
+
+namespace im {
+namespace {
+
+constexpr int kTcTile = 128, kTcThreads = 11 * 32, kTcMma = 8, kTcCopy = 9, kTcCopyWarps = 2;
+constexpr int kLag = 2;          // copies in flight behind the one that is requested
+constexpr float kTcLazy = 8.0f;  // growth of a row's maximum (in powers of two) that is left in the weights
+
+template <int KB, bool WIDE>
+struct TcShape {
+    static constexpr int kRows = WIDE ? 256 : 128;
+    static constexpr int kBlock = 128 * 128;  // bytes of 128 rows of 64 columns
+    static constexpr int kQ = (WIDE ? 2 : 1) * KB * kBlock, kSlot = KB * kBlock;
+    static constexpr int kK = 3, kV = WIDE ? 2 : 3;  // slots
+    static constexpr int kBars = 2 * kK + 2 * kV + 2 + 8 + 1;
+    static constexpr int kSmem = 1024 + kQ + (kK + kV) * kSlot + kBars * 8 + 8 * 16 + 128 * 8 + 16;
+};
+
+// The items of a CTA's share, one after the other; every warp walks them for itself.
+template <int R>
+struct Items {
+    const PagedAttn &p;
+    const int units;
+    int unit, head, tile;
+    long long left;
+    PagedUnit u;
+    int tiles, t0, t1, index;
+    __device__ __forceinline__ Items(const PagedAttn &p, int units, const Share &s)
+        : p(p), units(units), unit(s.unit - 1), head(p.kv.nkv - 1), tile(0), left(s.to - s.from), tiles(0), t0(0), t1(0), index(-1) {
+        if (left > 0) {
+            unit = s.unit;
+            head = s.head - 1;
+            u = paged_unit<R>(p, unit);
+            tiles = unit_tiles<kTcTile>(u);
+            tile = s.tile;
+        }
+    }
+    __device__ __forceinline__ bool next() {
+        if (left <= 0) return false;
+        if (++head == p.kv.nkv) {
+            head = 0;
+            do {
+                if (++unit >= units) return false;
+                u = paged_unit<R>(p, unit);
+                tiles = unit_tiles<kTcTile>(u);
+            } while (tiles == 0);
+        }
+        t0 = tile;
+        t1 = (int)min((long long)tiles, t0 + left);
+        left -= t1 - t0;
+        tile = 0;
+        index++;
+        return true;
+    }
+};
+
+// Bit j: the t-th new token sees position pos + j (32 of them); the rows' being there is another matter.
+__device__ __forceinline__ uint32_t sees32(const PagedAttn &p, const PagedUnit &u, int t, int pos) {
+    const int d = pos - u.len;
+    if (d + 32 <= 0) return 0xffffffffu;
+    if (d >= u.fresh) return 0u;
+    const int from = max(d, 0), shift = from - d;  // bits below `shift` are rows before the new ones
+    uint32_t bits;
+    if (!p.mask) {
+        const int n = t + 1 - from;
+        bits = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
+    } else {
+        const uint64_t *m = p.mask + (long long)(u.tok0 + t) * p.mask_words;
+        const int w = from >> 6, s = from & 63;
+        uint64_t x = w < p.mask_words ? __ldg(m + w) >> s : 0;
+        if (s > 32 && w + 1 < p.mask_words) x |= __ldg(m + w + 1) << (64 - s);
+        bits = (uint32_t)x;
+    }
+    const int n = u.fresh - from;
+    if (n < 32) bits &= (1u << n) - 1;
+    return shift == 0 ? bits : bits << shift | ((1u << shift) - 1);
+}
+
+__device__ __forceinline__ void zcopy(uint32_t dst, const void *src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
+template <bool BF16, int KB, bool WIDE>
+__global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_constant__ PagedAttn p, int units, int *err) {
+    using Shape = TcShape<KB, WIDE>;
+    constexpr int R = Shape::kRows, HD = 64 * KB, SK = Shape::kK, SV = Shape::kV, BLK = Shape::kBlock;
+    extern __shared__ __align__(16) unsigned char tc_smem[];
+    unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(tc_smem) + 1023) & ~(uintptr_t)1023);
+    unsigned char *Qs = smem, *Ks = Qs + Shape::kQ, *Vs = Ks + SK * Shape::kSlot;
+    uint32_t *there = reinterpret_cast<uint32_t *>(Vs + SV * Shape::kSlot);    // [8 tiles][4]: bit j of word w: row 32 w + j of the tile is in the cache
+    float2 *ml = reinterpret_cast<float2 *>(there + 32);                       // [128]: the second half's maximum and sum (not WIDE)
+    uint64_t *kfull = reinterpret_cast<uint64_t *>(ml + 128), *kempty = kfull + SK, *vfull = kempty + SK, *vempty = vfull + SV, *qfull = vempty + SV,
+             *qempty = qfull + 1, *sfull = qempty + 1, *pfull = sfull + 2, *ofull = pfull + 2, *oempty = ofull + 2, *mlfull = oempty + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mlfull + 1);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) {
+        for (int i = 0; i < SK; i++) {
+            mbar_init(&kfull[i], kTcCopyWarps);
+            mbar_init(&kempty[i], 1);
+        }
+        for (int i = 0; i < SV; i++) {
+            mbar_init(&vfull[i], kTcCopyWarps);
+            mbar_init(&vempty[i], 1);
+        }
+        mbar_init(qfull, kTcCopyWarps);
+        mbar_init(qempty, 1);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&sfull[i], 1);
+            mbar_init(&pfull[i], 4);
+            mbar_init(&ofull[i], 1);
+            mbar_init(&oempty[i], 4);
+        }
+        mbar_init(mlfull, 4);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kTcMma) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_trigger();  // after the allocation: a successor on this SM cannot take the columns first
+    pdl_wait();
+    const Share share = find_share<R, kTcTile, kTcThreads>(p, units, reinterpret_cast<long long *>(Qs));  // (no copy is under way yet)
+    Items<R> it(p, units, share);
+    bool ok = true;
+
+    if (warp >= kTcCopy) {
+        // ---- copies: this warp's 64 rows of every 128
+        const int w0 = (warp - kTcCopy) * 64;
+        uint64_t *pending[kLag];  // announcements that are due, oldest first
+        int due = 0;
+        auto announce = [&](uint64_t *bar) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        auto flush = [&]() {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            for (int i = 0; i < kLag; i++)
+                if (i < due) announce(pending[i]);
+            due = 0;
+        };
+        auto room = [&](uint64_t *bar, uint32_t parity) {  // nothing that others wait for is held back while this warp waits
+            if (!ok || __all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return;
+            flush();
+            if (!wait_for(bar, parity, err)) ok = false;
+        };
+        auto requested = [&](uint64_t *bar) {
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (due == kLag) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
+                announce(pending[0]);
+#pragma unroll
+                for (int i = 0; i + 1 < kLag; i++) pending[i] = pending[i + 1];
+                pending[kLag - 1] = bar;
+            } else {
+#pragma unroll
+                for (int i = 0; i < kLag; i++)
+                    if (i == due) pending[i] = bar;
+                due++;
+            }
+        };
+        // 64 rows whose offsets (elements from base; -1: none) the lanes hold two each, row 2 * lane + i in off[i]
+        auto rows64 = [&](unsigned char *dst, const uint16_t *base, long long off0, long long off1) {
+            constexpr int CH = 8 * KB, RPI = 32 / CH;
+            const int c = lane % CH;
+            const uint32_t at = smem_u32(dst) + (c >> 3) * BLK;
+#pragma unroll 8
+            for (int i = 0; i < 64 / RPI; i++) {
+                const int r = i * RPI + lane / CH;
+                const long long a = __shfl_sync(0xffffffffu, off0, r >> 1), b = __shfl_sync(0xffffffffu, off1, r >> 1);
+                const long long o = r & 1 ? b : a;
+                zcopy(at + (w0 + r) * 128 + (((c & 7) ^ (r & 7)) << 4), base + (o < 0 ? 0 : o + c * 8), o >= 0);
+            }
+        };
+        int kc = 0, vc = 0;
+        auto lookup = [&](const PagedUnit &u, int head, int pos) -> long long {
+            if (pos >= u.end) return -1;
+            const long long o = p.kv.row_of(u.seq, pos);
+            return o < 0 ? -1 : o + (long long)head * p.kv.page * HD;
+        };
+        while (it.next()) {
+            const PagedUnit &u = it.u;
+            long long o0 = lookup(u, it.head, it.t0 * kTcTile + w0 + 2 * lane), o1 = lookup(u, it.head, it.t0 * kTcTile + w0 + 2 * lane + 1);
+            if (it.index > 0) room(qempty, (it.index - 1) & 1);
+            for (int h = 0; h < (WIDE && u.rows > 128 ? 2 : 1); h++) {
+                long long off[2];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int r = h * 128 + w0 + 2 * lane + i;
+                    off[i] = -1;
+                    if (r < u.rows) off[i] = (u.tok0 + (u.row0 + r) / p.group) * p.qs + (long long)(it.head * p.group + (u.row0 + r) % p.group) * HD;
+                }
+                rows64(Qs + h * KB * BLK, p.q, off[0], off[1]);
+            }
+            requested(qfull);
+            for (int t = it.t0; t < it.t1; t++) {
+                const int ks = kc % SK, vs = vc % SV;
+                // the places of the next tile's rows are looked up while this one is requested
+                const long long n0 = t + 1 < it.t1 ? lookup(u, it.head, (t + 1) * kTcTile + w0 + 2 * lane) : -1;
+                const long long n1 = t + 1 < it.t1 ? lookup(u, it.head, (t + 1) * kTcTile + w0 + 2 * lane + 1) : -1;
+                if (kc >= SK) room(&kempty[ks], (kc / SK - 1) & 1);
+                const unsigned b0 = __ballot_sync(0xffffffffu, o0 >= 0), b1 = __ballot_sync(0xffffffffu, o1 >= 0);
+                if (lane < 2) {  // even rows' bits and odd rows' bits, interleaved: word `lane` has rows 32 lane .. of this warp's 64
+                    uint32_t word = 0;
+                    for (int j = 0; j < 16; j++) word |= (b0 >> (16 * lane + j) & 1u) << (2 * j) | (b1 >> (16 * lane + j) & 1u) << (2 * j + 1);
+                    there[(kc & 7) * 4 + w0 / 32 + lane] = word;
+                }
+                rows64(Ks + ks * Shape::kSlot, p.kc, o0, o1);
+                requested(&kfull[ks]);
+                kc++;
+                if (vc >= SV) room(&vempty[vs], (vc / SV - 1) & 1);
+                rows64(Vs + vs * Shape::kSlot, p.vc, o0, o1);
+                requested(&vfull[vs]);
+                vc++;
+                o0 = n0;
+                o1 = n1;
+            }
+        }
+        flush();
+    } else if (warp == kTcMma) {
+        // ---- products, one thread issues them all. Instruction descriptors as in flash_tc.cu: f32 accumulator, fp16 (0) or bf16 (1) operands in bits
+        // 7-9 and 10-12, B MN-major in bit 16, N >> 3 in bits 17-22, M >> 4 in bits 24-28
+        constexpr uint32_t kType = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(128 >> 4) << 24);
+        constexpr uint32_t kS = kType | ((uint32_t)(kTcTile >> 3) << 17), kPV = kType | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
+        int kc = 0, vc = 0, turn[2] = {0, 0};
+        auto scores = [&](int h) {
+            const int s = kc % SK;
+            if (ok && !wait_for(&kfull[s], (kc / SK) & 1, err)) ok = false;
+            fence_after();
+            if (lane == 0 && ok) {
+                const uint32_t q0 = smem_u32(Qs) + (WIDE ? h * KB * BLK : 0), k0 = smem_u32(Ks) + s * Shape::kSlot;
+#pragma unroll
+                for (int j = 0; j < KB * 4; j++)
+                    mma_ss(tmem + (uint32_t)(h * kTcTile), desc_sw128(q0 + (j >> 2) * BLK + (j & 3) * 32, 16), desc_sw128(k0 + (j >> 2) * BLK + (j & 3) * 32, 16), kS, j > 0 ? 1u : 0u);
+                commit(&sfull[h]);
+            }
+            __syncwarp();
+        };
+        auto values = [&](int h, bool first, bool last) {
+            const int s = vc % SV;
+            if (ok && !wait_for(&pfull[h], turn[h] & 1, err)) ok = false;
+            turn[h]++;
+            if (ok && !wait_for(&vfull[s], (vc / SV) & 1, err)) ok = false;
+            fence_after();
+            if (lane == 0 && ok) {
+                const uint32_t v0 = smem_u32(Vs) + s * Shape::kSlot, w = tmem + (uint32_t)(h * kTcTile), o = tmem + 256u + (uint32_t)(h * 128);
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int j = 0; j < kTcTile / 16; j++)
+                        mma_ts(o, w + (uint32_t)(t * kTcTile / 2 + j * 8), desc_sw128(v0 + j * 2048, BLK), kPV, (!first || t > 0 || j > 0) ? 1u : 0u);
+                if (last) commit(&ofull[h]);
+            }
+            __syncwarp();
+        };
+        auto release = [&](uint64_t *bar) {  // once the products issued so far are done
+            if (lane == 0 && ok) commit(bar);
+            __syncwarp();
+        };
+        while (it.next()) {
+            const int T = it.t1 - it.t0;
+            if (ok && !wait_for(qfull, it.index & 1, err)) ok = false;
+            auto drained = [&]() {  // the outputs of the item before have been read
+                if (it.index > 0)
+                    for (int h = 0; h < 2; h++)
+                        if (ok && !wait_for(&oempty[h], (it.index - 1) & 1, err)) ok = false;
+            };
+            if constexpr (WIDE) {
+                const int halves = it.u.rows > 128 ? 2 : 1;
+                for (int t = 0; t <= T; t++) {
+                    if (t == 1) drained();
+                    for (int h = 0; h < halves; h++) {
+                        if (t > 0) values(h, t == 1, t == T);
+                        if (t < T) scores(h);
+                    }
+                    if (t > 0) release(&vempty[vc++ % SV]);
+                    if (t < T) release(&kempty[kc++ % SK]);
+                    if (t == T - 1) release(qempty);
+                }
+            } else {
+                for (int t = 0; t < T + 2; t++) {
+                    if (t == 2) drained();
+                    if (t >= 2) {
+                        values(t & 1, t < 4, t >= T);
+                        release(&vempty[vc++ % SV]);
+                    }
+                    if (t < T) {
+                        scores(t & 1);
+                        release(&kempty[kc++ % SK]);
+                    }
+                    if (t == T - 1) release(qempty);
+                }
+            }
+        }
+    } else {
+        // ---- weights: a row per thread
+        const int h = warp >> 2, r = (warp & 3) * 32 + lane, R_ = WIDE ? h * 128 + r : r;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + lanes + (uint32_t)(h * kTcTile), to = tmem + lanes + 256u + (uint32_t)(h * 128);
+        const float scale = fabsf(p.scale2);
+        int seen = 0, tiles_before = 0, finished = 0, others = 0;  // scores of this half; tiles and items with tiles of the half (others: of the other one) so far
+        while (it.next()) {
+            const PagedUnit &u = it.u;
+            const int T = it.t1 - it.t0, jobs = WIDE ? (u.rows > h * 128 ? T : 0) : (T - h + 1) / 2;
+            const int token = (u.row0 + min(R_, u.rows - 1)) / p.group;
+            float m = -INFINITY, l = 0.0f;
+            for (int job = 0; job < jobs; job++) {
+                const int t = WIDE ? job : 2 * job + h;
+                if (ok && !wait_for(&sfull[h], seen & 1, err)) ok = false;
+                seen++;
+                fence_after();
+                const int p0 = (it.t0 + t) * kTcTile;
+                float s[kTcTile];
+#pragma unroll
+                for (int c = 0; c < kTcTile; c += 32) ld32(ts + (uint32_t)c, reinterpret_cast<uint32_t *>(s) + c);
+                const uint4 rows = *reinterpret_cast<const uint4 *>(there + ((tiles_before + t) & 7) * 4);
+                tmem_wait_ld();
+                if (p.scale2 < 0.0f) {
+#pragma unroll
+                    for (int c = 0; c < kTcTile; c++) s[c] = -s[c];
+                }
+                if ((rows.x & rows.y & rows.z & rows.w) != 0xffffffffu || p0 + kTcTile > u.len) {  // some row does not see all of the tile
+                    const uint32_t w[4] = {rows.x & sees32(p, u, token, p0), rows.y & sees32(p, u, token, p0 + 32), rows.z & sees32(p, u, token, p0 + 64),
+                                           rows.w & sees32(p, u, token, p0 + 96)};
+#pragma unroll
+                    for (int c = 0; c < kTcTile; c++) s[c] = w[c >> 5] >> (c & 31) & 1u ? s[c] : -INFINITY;
+                }
+                float mx[4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) mx[c] = s[c];
+#pragma unroll
+                for (int c = 4; c < kTcTile; c++) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+                if (__any_sync(0xffffffffu, top > m + kTcLazy)) {  // (-inf + anything is -inf: a row's first visible position is one)
+                    const float m_new = fmaxf(m, top), corr = m_new == -INFINITY ? 1.0f : ex2(m - m_new);
+                    m = m_new;
+                    l *= corr;
+                    if (job > 0) {
+#pragma unroll 1
+                        for (int c = 0; c < HD; c += 32) {
+                            uint32_t o[32];
+                            ld32(to + (uint32_t)c, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 32; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+                            st32(to + (uint32_t)c, o);
+                        }
+                    }
+                }
+                const float base = m == -INFINITY ? 0.0f : m;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < kTcTile; c += 32) {  // (weights of columns that have been read: the scores are in registers)
+                    uint32_t w[16], w2[16];
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        const float x0 = ex2(fmaf(s[c + 2 * j], scale, -base)), x1 = ex2(fmaf(s[c + 2 * j + 1], scale, -base));
+                        sum[(2 * j) & 3] += x0;
+                        sum[(2 * j + 1) & 3] += x1;
+                        w[j] = pack2<BF16>(x0, x1);
+                        const float2 back = unpack2<BF16>(w[j]);
+                        w2[j] = pack2<BF16>(x0 - back.x, x1 - back.y);
+                    }
+                    st16(ts + (uint32_t)(c / 2), w);
+                    st16(ts + (uint32_t)(kTcTile / 2 + c / 2), w2);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_wait_st();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&pfull[h]);
+            }
+            tiles_before += T;
+            // ---- the item's (or the share's part of it) rows
+            if (jobs > 0 && ok && !wait_for(&ofull[h], finished & 1, err)) ok = false;
+            finished += jobs > 0;
+            float f0 = 1.0f, f1 = 0.0f;
+            if constexpr (!WIDE) {
+                if (h == 1) {
+                    // the first half has read what this one left for the item before
+                    if (it.index > 0 && ok && !wait_for(&oempty[1], (it.index - 1) & 1, err)) ok = false;
+                    ml[r] = make_float2(m, l);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(mlfull);
+                    continue;
+                }
+                if (ok && !wait_for(mlfull, it.index & 1, err)) ok = false;
+                if (T > 1) {
+                    if (ok && !wait_for(&ofull[1], others & 1, err)) ok = false;
+                    others++;
+                }
+                const float2 o = ml[r];
+                const float M = fmaxf(m, o.x);
+                f0 = m == -INFINITY && l == 0.0f ? 0.0f : ex2(m - M);
+                f1 = o.x == -INFINITY && o.y == 0.0f ? 0.0f : ex2(o.x - M);
+                l = (f0 == 0.0f ? 0.0f : l * f0) + (f1 == 0.0f ? 0.0f : o.y * f1);
+                m = M;
+            }
+            fence_after();
+            const bool live = R_ < u.rows && ok;
+            const bool whole = it.t0 == 0 && it.t1 == it.tiles;
+            const size_t part = ((size_t)blockIdx.x * 2 + (it.index == 0 ? 0 : 1)) * R + R_;
+            const float inv = whole ? (l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l) : 1.0f;
+            uint16_t *out = p.out + (u.tok0 + token) * p.os + (long long)(it.head * p.group + (u.row0 + min(R_, u.rows - 1)) % p.group) * HD;
+            float worst = 0.0f;
+            if (WIDE ? jobs > 0 : true) {
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t a[32];
+                    float v[32];
+                    ld32(to + (uint32_t)c, a);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 32; j++) v[j] = f0 == 0.0f ? 0.0f : __uint_as_float(a[j]) * f0;
+                    if (!WIDE && T > 1) {
+                        ld32(to + 128u + (uint32_t)c, a);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; j++) v[j] += f1 == 0.0f ? 0.0f : __uint_as_float(a[j]) * f1;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; j++) worst += v[j] * 0.0f;  // zero unless a value is not finite
+                    if (!live) continue;
+                    if (whole) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 8)
+                            *reinterpret_cast<uint4 *>(out + c + j) = make_uint4(pack2<BF16>(v[j] * inv, v[j + 1] * inv), pack2<BF16>(v[j + 2] * inv, v[j + 3] * inv),
+                                                                                 pack2<BF16>(v[j + 4] * inv, v[j + 5] * inv), pack2<BF16>(v[j + 6] * inv, v[j + 7] * inv));
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(p.part_o + part * HD + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                    }
+                }
+                if (live && !whole) p.part_ml[part] = make_float2(m, l);
+            }
+            fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&oempty[h]);
+                if (!WIDE) mbar_arrive(&oempty[1]);
+            }
+            unsigned bad = __ballot_sync(0xffffffffu, live && !(worst == 0.0f));
+            while (bad) {
+                const int b = __ffs(bad) - 1, row = WIDE ? h * 128 + (warp & 3) * 32 + b : (warp & 3) * 32 + b;
+                bad &= bad - 1;
+                float x[HD / 32], M, L;
+                plain_row<BF16, HD>(p, u, it.head, row, it.t0 * kTcTile, min(it.t1 * kTcTile, u.end), x, M, L);
+                const float n = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
+                const size_t at = ((size_t)blockIdx.x * 2 + (it.index == 0 ? 0 : 1)) * R + row;
+                uint16_t *to_row = p.out + (u.tok0 + (u.row0 + row) / p.group) * p.os + (long long)(it.head * p.group + (u.row0 + row) % p.group) * HD;
+                for (int i = 0; i < HD / 32; i++) {
+                    if (whole) to_row[lane + 32 * i] = (uint16_t)pack2<BF16>(x[i] * n, 0.0f);
+                    else p.part_o[at * HD + lane + 32 * i] = x[i];
+                }
+                if (!whole && lane == 0) p.part_ml[at] = make_float2(M, L);
+            }
+        }
+    }
+    fence_before();
+    sync_and_settle(ok);
+    if (warp == kTcMma) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+template <bool BF16, int KB, bool WIDE>
+int tc_launch(const Device *dev, const PagedAttn &p, int units, cudaStream_t st) {
+    using S = TcShape<KB, WIDE>;
+    static DeviceOnce once;
+    if (once.first(dev->ordinal)) IM_CUDA_CHECK(cudaFuncSetAttribute((paged_tc_kernel<BF16, KB, WIDE>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+    IM_CUDA_CHECK(launch_k(paged_tc_kernel<BF16, KB, WIDE>, dim3(p.ctas), dim3(kTcThreads), (size_t)S::kSmem, st, p, units, dev->err_flag));
+    return IM_OK;
+}
+
+}  // namespace
+
+int paged_tc_rows(int hd, long long rows) {
+    if (hd != 64 && hd != 128) return 0;
+    return rows <= 32 ? 0 : rows <= 128 ? 128 : 256;
+}
+
+int paged_tc_launch(const Device *dev, const PagedAttn &p, bool bf16, int rows, int units, cudaStream_t st) {
+    const bool wide = rows == 256;
+#define IM_RUN(B, KB) (wide ? tc_launch<B, KB, true>(dev, p, units, st) : tc_launch<B, KB, false>(dev, p, units, st))
+    if (p.kv.hd == 64) return bf16 ? IM_RUN(true, 1) : IM_RUN(false, 1);
+    return bf16 ? IM_RUN(true, 2) : IM_RUN(false, 2);
+#undef IM_RUN
+}
+
+}  // namespace im
