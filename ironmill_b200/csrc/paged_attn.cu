@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
     using S = PaShape<HD, MT>;
     constexpr int R = S::kRows, KS = HD / 16, NT = HD / 8, CH = HD / 8;  // k steps, 8-column tiles, 16-byte pieces of a row
     extern __shared__ __align__(128) unsigned char pa_smem[];
-    __shared__ long long sums[kPaThreads];
+    __shared__ long long sums[kPaThreads + kShareMore];
     __shared__ unsigned rows_there[kPaWarps][8];  // of a slice in the ring: bit r where row r is in the cache
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     unsigned char *ring = pa_smem + warp * (S::kRing / kPaWarps);

@@ -55,10 +55,11 @@ __device__ __forceinline__ bool paged_sees(const PagedAttn &p, const PagedUnit &
     return d < 64 * p.mask_words && ((__ldg(p.mask + (long long)(u.tok0 + t) * p.mask_words + (d >> 6)) >> (d & 63)) & 1);
 }
 
-// Inclusive sums of v over the block's threads in sums[], the total returned.
+// Inclusive sums of v over the block's threads in sums[], the total returned. sums: room for the threads and kShareMore more.
+constexpr int kShareMore = 34;  // one per warp, and what find_share() found
 template <int THREADS>
 __device__ __forceinline__ long long block_scan(int v, long long *sums) {
-    __shared__ long long of_warp[THREADS / 32];
+    long long *of_warp = sums + THREADS;
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     long long s = v;
 #pragma unroll
@@ -95,37 +96,46 @@ __device__ __forceinline__ long long share_at(long long total, int n, int c) { r
 
 template <int R, int TILE, int THREADS>
 __device__ __forceinline__ Share find_share(const PagedAttn &p, int units, long long *sums) {
-    __shared__ int found[3];
+    int *found = reinterpret_cast<int *>(sums + THREADS + 32);  // unit, head, tile
     Share s;
-    long long total = 0;
-    for (int u0 = 0; u0 < units; u0 += THREADS) {
-        const int u = u0 + threadIdx.x;
-        const int n = u < units ? unit_tiles<TILE>(paged_unit<R>(p, u)) : 0;
-        const long long all = block_scan<THREADS>(n, sums);
-        if (blockIdx.x == 0 && u < units) p.first[u] = total + sums[threadIdx.x] - n;
-        total += all;
-    }
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.first[units] = total;
-    total *= p.kv.nkv;
-    const int shares = share_count(total, p.ctas);
-    s.from = share_at(total, shares, blockIdx.x);
-    s.to = share_at(total, shares, blockIdx.x + 1);
+    long long total = 0, before = 0;
+    s.from = s.to = 0;
     s.unit = s.head = s.tile = 0;
-    if (s.from >= s.to) return s;
-    long long before = 0;
-    for (int u0 = 0; u0 < units; u0 += THREADS) {
-        const int u = u0 + threadIdx.x;
-        const int n = u < units ? unit_tiles<TILE>(paged_unit<R>(p, u)) : 0;
-        const long long all = block_scan<THREADS>(n, sums);
-        const long long a = (before + sums[threadIdx.x] - n) * p.kv.nkv;
-        if (n > 0 && s.from >= a && s.from < a + (long long)n * p.kv.nkv) {
-            const int d = (int)(s.from - a);
-            found[0] = u;
-            found[1] = d / n;
-            found[2] = d % n;
+    const bool once = units <= THREADS;  // the first pass over the units has all that the second one needs
+    int n = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; pass++) {
+#pragma unroll 1
+        for (int u0 = 0; u0 < units; u0 += THREADS) {
+            const int u = u0 + threadIdx.x;
+            long long all = total;
+            if (pass == 0 || !once) {
+                n = u < units ? unit_tiles<TILE>(paged_unit<R>(p, u)) : 0;
+                all = block_scan<THREADS>(n, sums);
+            }
+            if (pass == 0) {
+                if (blockIdx.x == 0 && u < units) p.first[u] = total + sums[threadIdx.x] - n;
+                total += all;
+                continue;
+            }
+            const long long a = (before + sums[threadIdx.x] - n) * p.kv.nkv;
+            if (n > 0 && s.from >= a && s.from < a + (long long)n * p.kv.nkv) {
+                const int d = (int)(s.from - a);
+                found[0] = u;
+                found[1] = d / n;
+                found[2] = d % n;
+            }
+            before += all;
+            if (before * p.kv.nkv > s.from) break;
         }
-        before += all;
-        if (before * p.kv.nkv > s.from) break;
+        if (pass == 0) {
+            if (blockIdx.x == 0 && threadIdx.x == 0) p.first[units] = total;
+            const long long tiles = total * p.kv.nkv;
+            const int shares = share_count(tiles, p.ctas);
+            s.from = share_at(tiles, shares, blockIdx.x);
+            s.to = share_at(tiles, shares, blockIdx.x + 1);
+            if (s.from >= s.to) return s;
+        }
     }
     __syncthreads();
     s.unit = found[0];

@@ -9,7 +9,7 @@
 // and the odd tiles of the share, with accumulators of their own that are joined where the item ends.
 // A row's accumulator is rescaled only when its maximum has grown by more than 2^8 (as in flash_tc.cu).
 //
-// K, V and queries come by 16-byte cp.async of two warps, rows looked up in the page table: any page size, rows that are not there are zeros and
+// K, V and queries come by 16-byte cp.async of four warps, rows looked up in the page table: any page size, rows that are not there are zeros and
 // known to be none (a bit per row). The copies run ahead over the ends of items; each is announced when it has landed and been made
 // visible to the tensor cores, the announcement lagging kLag copies behind the requests, or at once where the ring is full.
 //
@@ -24,7 +24,8 @@
 namespace im {
 namespace {
 
-constexpr int kTcTile = 128, kTcThreads = 11 * 32, kTcMma = 8, kTcCopy = 9, kTcCopyWarps = 2;
+// warps 0-7: weights; 8: products; 9-12: copies
+constexpr int kTcTile = 128, kTcThreads = 13 * 32, kTcMma = 8, kTcCopy = 9, kTcCopyWarps = 4;
 constexpr int kLag = 2;          // copies in flight behind the one that is requested
 constexpr float kTcLazy = 8.0f;  // growth of a row's maximum (in powers of two) that is left in the weights
 
@@ -35,7 +36,10 @@ struct TcShape {
     static constexpr int kQ = (WIDE ? 2 : 1) * KB * kBlock, kSlot = KB * kBlock;
     static constexpr int kK = 3, kV = WIDE ? 2 : 3;  // slots
     static constexpr int kBars = 2 * kK + 2 * kV + 2 + 8 + 1;
-    static constexpr int kSmem = 1024 + kQ + (kK + kV) * kSlot + kBars * 8 + 8 * 16 + 128 * 8 + 16;
+    static constexpr int kSmall = 8 * 16 + 128 * 8 + kTcCopyWarps * 32 * 8 + kBars * 8 + 8;  // presence bits, maxima and sums, offsets, barriers, address
+    static constexpr int kTiles = kQ + (kK + kV) * kSlot;
+    static constexpr int kSmem = (kSmall + 1023) / 1024 * 1024 + kTiles;
+    static_assert(kSmem <= 232448, "shared memory of an SM");
 };
 
 // The items of a CTA's share, one after the other; every warp walks them for itself.
@@ -98,6 +102,30 @@ __device__ __forceinline__ uint32_t sees32(const PagedAttn &p, const PagedUnit &
     return shift == 0 ? bits : bits << shift | ((1u << shift) - 1);
 }
 
+// Products issued by one elected lane of a converged warp. Everything they name is the same in all lanes (uniform() says so to the compiler): operands
+// that it had to move to uniform registers one by one cost more than the product.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile("{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+                 : "memory");
+}
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {  // A operand in tensor memory
+    asm volatile("{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+                 : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint32_t bar) {
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(bar)
+                 : "memory");
+}
+// Looks without waiting: try_wait may suspend the warp for a while.
+__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ void zcopy(uint32_t dst, const void *src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
@@ -107,13 +135,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     using Shape = TcShape<KB, WIDE>;
     constexpr int R = Shape::kRows, HD = 64 * KB, SK = Shape::kK, SV = Shape::kV, BLK = Shape::kBlock;
     extern __shared__ __align__(16) unsigned char tc_smem[];
-    unsigned char *smem = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(tc_smem) + 1023) & ~(uintptr_t)1023);
-    unsigned char *Qs = smem, *Ks = Qs + Shape::kQ, *Vs = Ks + SK * Shape::kSlot;
-    uint32_t *there = reinterpret_cast<uint32_t *>(Vs + SV * Shape::kSlot);    // [8 tiles][4]: bit j of word w: row 32 w + j of the tile is in the cache
+    uint32_t *there = reinterpret_cast<uint32_t *>(tc_smem);                   // [8 tiles][4]: bit j of word w: row 32 w + j of the tile is in the cache
     float2 *ml = reinterpret_cast<float2 *>(there + 32);                       // [128]: the second half's maximum and sum (not WIDE)
-    uint64_t *kfull = reinterpret_cast<uint64_t *>(ml + 128), *kempty = kfull + SK, *vfull = kempty + SK, *vempty = vfull + SV, *qfull = vempty + SV,
+    long long *offs = reinterpret_cast<long long *>(ml + 128);                 // [copying warps][32]: where the rows that a warp copies lie
+    uint64_t *kfull = reinterpret_cast<uint64_t *>(offs + kTcCopyWarps * 32), *kempty = kfull + SK, *vfull = kempty + SK, *vempty = vfull + SV, *qfull = vempty + SV,
              *qempty = qfull + 1, *sfull = qempty + 1, *pfull = sfull + 2, *ofull = pfull + 2, *oempty = ofull + 2, *mlfull = oempty + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mlfull + 1);
+    // (shared memory starts at a multiple of 1024: checked, the tiles would not fit otherwise)
+    unsigned char *Qs = tc_smem + (Shape::kSmem - Shape::kTiles), *Ks = Qs + Shape::kQ, *Vs = Ks + SK * Shape::kSlot;
+    if (smem_u32(Qs) % 1024 != 0) {
+        if (threadIdx.x == 0) atomicExch(err, 1);
+        return;
+    }
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         for (int i = 0; i < SK; i++) {
@@ -148,10 +181,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     const Share share = find_share<R, kTcTile, kTcThreads>(p, units, reinterpret_cast<long long *>(Qs));  // (no copy is under way yet)
     Items<R> it(p, units, share);
     bool ok = true;
-
     if (warp >= kTcCopy) {
-        // ---- copies: this warp's 64 rows of every 128
-        const int w0 = (warp - kTcCopy) * 64;
+        // ---- copies: this warp's 32 rows of every 128
+        const int w0 = (warp - kTcCopy) * 32;
+        long long *mine = offs + w0;
         uint64_t *pending[kLag];  // announcements that are due, oldest first
         int due = 0;
         auto announce = [&](uint64_t *bar) {
@@ -166,7 +199,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             due = 0;
         };
         auto room = [&](uint64_t *bar, uint32_t parity) {  // nothing that others wait for is held back while this warp waits
-            if (!ok || __all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return;
+            if (!ok || __all_sync(0xffffffffu, mbar_test(bar, parity))) return;
             flush();
             if (!wait_for(bar, parity, err)) ok = false;
         };
@@ -185,18 +218,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 due++;
             }
         };
-        // 64 rows whose offsets (elements from base; -1: none) the lanes hold two each, row 2 * lane + i in off[i]
-        auto rows64 = [&](unsigned char *dst, const uint16_t *base, long long off0, long long off1) {
+        // 32 rows whose offsets (elements from base; -1: none) are in mine[]
+        auto rows32 = [&](unsigned char *dst, const uint16_t *base) {
             constexpr int CH = 8 * KB, RPI = 32 / CH;
-            const int c = lane % CH;
-            const uint32_t at = smem_u32(dst) + (c >> 3) * BLK;
-#pragma unroll 8
-            for (int i = 0; i < 64 / RPI; i++) {
-                const int r = i * RPI + lane / CH;
-                const long long a = __shfl_sync(0xffffffffu, off0, r >> 1), b = __shfl_sync(0xffffffffu, off1, r >> 1);
-                const long long o = r & 1 ? b : a;
-                zcopy(at + (w0 + r) * 128 + (((c & 7) ^ (r & 7)) << 4), base + (o < 0 ? 0 : o + c * 8), o >= 0);
+            const int c = lane % CH, r0 = lane / CH;
+            const uint32_t at = smem_u32(dst) + (c >> 3) * BLK + (w0 + r0) * 128;
+#pragma unroll 1
+            for (int i0 = 0; i0 < 32 / RPI; i0 += 8) {
+                long long o[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) o[i] = mine[(i0 + i) * RPI + r0];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int r = (i0 + i) * RPI;
+                    zcopy(at + r * 128 + (((c & 7) ^ ((r + r0) & 7)) << 4), base + (o[i] < 0 ? 0 : o[i] + c * 8), o[i] >= 0);
+                }
             }
+        };
+        auto place = [&](long long o) {
+            __syncwarp();
+            mine[lane] = o;
+            __syncwarp();
         };
         int kc = 0, vc = 0;
         auto lookup = [&](const PagedUnit &u, int head, int pos) -> long long {
@@ -206,40 +248,30 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
         };
         while (it.next()) {
             const PagedUnit &u = it.u;
-            long long o0 = lookup(u, it.head, it.t0 * kTcTile + w0 + 2 * lane), o1 = lookup(u, it.head, it.t0 * kTcTile + w0 + 2 * lane + 1);
+            long long o = lookup(u, it.head, it.t0 * kTcTile + w0 + lane);
             if (it.index > 0) room(qempty, (it.index - 1) & 1);
             for (int h = 0; h < (WIDE && u.rows > 128 ? 2 : 1); h++) {
-                long long off[2];
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const int r = h * 128 + w0 + 2 * lane + i;
-                    off[i] = -1;
-                    if (r < u.rows) off[i] = (u.tok0 + (u.row0 + r) / p.group) * p.qs + (long long)(it.head * p.group + (u.row0 + r) % p.group) * HD;
-                }
-                rows64(Qs + h * KB * BLK, p.q, off[0], off[1]);
+                const int r = h * 128 + w0 + lane;
+                place(r < u.rows ? (u.tok0 + (u.row0 + r) / p.group) * p.qs + (long long)(it.head * p.group + (u.row0 + r) % p.group) * HD : -1);
+                rows32(Qs + h * KB * BLK, p.q);
             }
             requested(qfull);
             for (int t = it.t0; t < it.t1; t++) {
                 const int ks = kc % SK, vs = vc % SV;
                 // the places of the next tile's rows are looked up while this one is requested
-                const long long n0 = t + 1 < it.t1 ? lookup(u, it.head, (t + 1) * kTcTile + w0 + 2 * lane) : -1;
-                const long long n1 = t + 1 < it.t1 ? lookup(u, it.head, (t + 1) * kTcTile + w0 + 2 * lane + 1) : -1;
+                const long long next = t + 1 < it.t1 ? lookup(u, it.head, (t + 1) * kTcTile + w0 + lane) : -1;
                 if (kc >= SK) room(&kempty[ks], (kc / SK - 1) & 1);
-                const unsigned b0 = __ballot_sync(0xffffffffu, o0 >= 0), b1 = __ballot_sync(0xffffffffu, o1 >= 0);
-                if (lane < 2) {  // even rows' bits and odd rows' bits, interleaved: word `lane` has rows 32 lane .. of this warp's 64
-                    uint32_t word = 0;
-                    for (int j = 0; j < 16; j++) word |= (b0 >> (16 * lane + j) & 1u) << (2 * j) | (b1 >> (16 * lane + j) & 1u) << (2 * j + 1);
-                    there[(kc & 7) * 4 + w0 / 32 + lane] = word;
-                }
-                rows64(Ks + ks * Shape::kSlot, p.kc, o0, o1);
+                const unsigned word = __ballot_sync(0xffffffffu, o >= 0);
+                if (lane == 0) there[(kc & 7) * 4 + w0 / 32] = word;
+                place(o);
+                rows32(Ks + ks * Shape::kSlot, p.kc);
                 requested(&kfull[ks]);
                 kc++;
                 if (vc >= SV) room(&vempty[vs], (vc / SV - 1) & 1);
-                rows64(Vs + vs * Shape::kSlot, p.vc, o0, o1);
+                rows32(Vs + vs * Shape::kSlot, p.vc);
                 requested(&vfull[vs]);
                 vc++;
-                o0 = n0;
-                o1 = n1;
+                o = next;
             }
         }
         flush();
@@ -253,12 +285,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             const int s = kc % SK;
             if (ok && !wait_for(&kfull[s], (kc / SK) & 1, err)) ok = false;
             fence_after();
-            if (lane == 0 && ok) {
-                const uint32_t q0 = smem_u32(Qs) + (WIDE ? h * KB * BLK : 0), k0 = smem_u32(Ks) + s * Shape::kSlot;
+            if (ok) {
+                const uint32_t k0 = uniform(smem_u32(Ks) + s * Shape::kSlot), q0 = uniform(smem_u32(Qs) + (WIDE ? h * KB * BLK : 0)), d = uniform(tmem + (uint32_t)(h * kTcTile));
+                const uint64_t qd = desc_sw128(q0, 16), kd = desc_sw128(k0, 16);
+#pragma unroll 1
+                for (int j = 0; j < KB * 4; j += 4)
 #pragma unroll
-                for (int j = 0; j < KB * 4; j++)
-                    mma_ss(tmem + (uint32_t)(h * kTcTile), desc_sw128(q0 + (j >> 2) * BLK + (j & 3) * 32, 16), desc_sw128(k0 + (j >> 2) * BLK + (j & 3) * 32, 16), kS, j > 0 ? 1u : 0u);
-                commit(&sfull[h]);
+                    for (int i = 0; i < 4; i++) umma_ss(d, qd + (j / 4 * BLK + i * 32) / 16, kd + (j / 4 * BLK + i * 32) / 16, kS, i > 0 || j > 0);
+                umma_commit(uniform(smem_u32(&sfull[h])));
             }
             __syncwarp();
         };
@@ -268,19 +302,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             turn[h]++;
             if (ok && !wait_for(&vfull[s], (vc / SV) & 1, err)) ok = false;
             fence_after();
-            if (lane == 0 && ok) {
-                const uint32_t v0 = smem_u32(Vs) + s * Shape::kSlot, w = tmem + (uint32_t)(h * kTcTile), o = tmem + 256u + (uint32_t)(h * 128);
+            if (ok) {
+                const uint32_t v0 = uniform(smem_u32(Vs) + s * Shape::kSlot), w = uniform(tmem + (uint32_t)(h * kTcTile)), o = uniform(tmem + 256u + (uint32_t)(h * 128));
+                const uint64_t vd = desc_sw128(v0, BLK);
+                uint32_t more = uniform(first ? 0 : 1);
+                // (64 positions' weights: 32 columns of the first terms, 32 of the second)
+#pragma unroll 1
+                for (int j = 0; j < kTcTile / 16; j += 4) {
 #pragma unroll
-                for (int t = 0; t < 2; t++)
-#pragma unroll
-                    for (int j = 0; j < kTcTile / 16; j++)
-                        mma_ts(o, w + (uint32_t)(t * kTcTile / 2 + j * 8), desc_sw128(v0 + j * 2048, BLK), kPV, (!first || t > 0 || j > 0) ? 1u : 0u);
-                if (last) commit(&ofull[h]);
+                    for (int i = 0; i < 8; i++) umma_ts(o, w + (uint32_t)(j * 16 + (i & 1) * 32 + (i >> 1) * 8), vd + (j + (i >> 1)) * 2048 / 16, kPV, i > 0 || more);
+                    more = 1;
+                }
+                if (last) umma_commit(uniform(smem_u32(&ofull[h])));
             }
             __syncwarp();
         };
         auto release = [&](uint64_t *bar) {  // once the products issued so far are done
-            if (lane == 0 && ok) commit(bar);
+            if (ok) umma_commit(uniform(smem_u32(bar)));
             __syncwarp();
         };
         while (it.next()) {
@@ -336,27 +374,31 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 seen++;
                 fence_after();
                 const int p0 = (it.t0 + t) * kTcTile;
-                float s[kTcTile];
+                const uint32_t *rows = there + ((tiles_before + t) & 7) * 4;
+                const bool part = (rows[0] & rows[1] & rows[2] & rows[3]) != 0xffffffffu || p0 + kTcTile > u.len;  // some row does not see all of the tile
+                float top = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < kTcTile; c += 64) {
+                    float s[64];
+                    ld32(ts + (uint32_t)c, reinterpret_cast<uint32_t *>(s));
+                    ld32(ts + (uint32_t)c + 32u, reinterpret_cast<uint32_t *>(s) + 32);
+                    tmem_wait_ld();
+                    if (part || p.scale2 < 0.0f) {
+                        const float sign = p.scale2 < 0.0f ? -1.0f : 1.0f;
+                        const uint32_t w0 = rows[c / 32] & sees32(p, u, token, p0 + c), w1 = rows[c / 32 + 1] & sees32(p, u, token, p0 + c + 32);
 #pragma unroll
-                for (int c = 0; c < kTcTile; c += 32) ld32(ts + (uint32_t)c, reinterpret_cast<uint32_t *>(s) + c);
-                const uint4 rows = *reinterpret_cast<const uint4 *>(there + ((tiles_before + t) & 7) * 4);
-                tmem_wait_ld();
-                if (p.scale2 < 0.0f) {
+                        for (int j = 0; j < 64; j++) s[j] = (j < 32 ? w0 : w1) >> (j & 31) & 1u ? s[j] * sign : -INFINITY;
+                        st32(ts + (uint32_t)c, reinterpret_cast<uint32_t *>(s));
+                        st32(ts + (uint32_t)c + 32u, reinterpret_cast<uint32_t *>(s) + 32);
+                    }
+                    float mx[4];
 #pragma unroll
-                    for (int c = 0; c < kTcTile; c++) s[c] = -s[c];
+                    for (int j = 0; j < 4; j++) mx[j] = s[j];
+#pragma unroll
+                    for (int j = 4; j < 64; j++) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
+                    top = fmaxf(fmaxf(top, fmaxf(mx[0], mx[1])), fmaxf(mx[2], mx[3]));
                 }
-                if ((rows.x & rows.y & rows.z & rows.w) != 0xffffffffu || p0 + kTcTile > u.len) {  // some row does not see all of the tile
-                    const uint32_t w[4] = {rows.x & sees32(p, u, token, p0), rows.y & sees32(p, u, token, p0 + 32), rows.z & sees32(p, u, token, p0 + 64),
-                                           rows.w & sees32(p, u, token, p0 + 96)};
-#pragma unroll
-                    for (int c = 0; c < kTcTile; c++) s[c] = w[c >> 5] >> (c & 31) & 1u ? s[c] : -INFINITY;
-                }
-                float mx[4];
-#pragma unroll
-                for (int c = 0; c < 4; c++) mx[c] = s[c];
-#pragma unroll
-                for (int c = 4; c < kTcTile; c++) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+                top *= scale;
                 if (__any_sync(0xffffffffu, top > m + kTcLazy)) {  // (-inf + anything is -inf: a row's first visible position is one)
                     const float m_new = fmaxf(m, top), corr = m_new == -INFINITY ? 1.0f : ex2(m - m_new);
                     m = m_new;
@@ -374,21 +416,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                     }
                 }
                 const float base = m == -INFINITY ? 0.0f : m;
+                tmem_wait_st();
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+                for (int c = 0; c < kTcTile; c += 64) {  // weights of 64 positions over their scores: first terms, second terms
+                    uint32_t s[64];
+                    ld32(ts + (uint32_t)c, s);
+                    ld32(ts + (uint32_t)c + 32u, s + 32);
+                    tmem_wait_ld();
 #pragma unroll
-                for (int c = 0; c < kTcTile; c += 32) {  // (weights of columns that have been read: the scores are in registers)
-                    uint32_t w[16], w2[16];
+                    for (int h2 = 0; h2 < 2; h2++) {
+                        uint32_t w[16], w2[16];
 #pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        const float x0 = ex2(fmaf(s[c + 2 * j], scale, -base)), x1 = ex2(fmaf(s[c + 2 * j + 1], scale, -base));
-                        sum[(2 * j) & 3] += x0;
-                        sum[(2 * j + 1) & 3] += x1;
-                        w[j] = pack2<BF16>(x0, x1);
-                        const float2 back = unpack2<BF16>(w[j]);
-                        w2[j] = pack2<BF16>(x0 - back.x, x1 - back.y);
+                        for (int j = 0; j < 16; j++) {
+                            const float x0 = ex2(fmaf(__uint_as_float(s[32 * h2 + 2 * j]), scale, -base)), x1 = ex2(fmaf(__uint_as_float(s[32 * h2 + 2 * j + 1]), scale, -base));
+                            sum[(2 * j) & 3] += x0;
+                            sum[(2 * j + 1) & 3] += x1;
+                            w[j] = pack2<BF16>(x0, x1);
+                            const float2 back = unpack2<BF16>(w[j]);
+                            w2[j] = pack2<BF16>(x0 - back.x, x1 - back.y);
+                        }
+                        st16(ts + (uint32_t)(c + 16 * h2), w);
+                        st16(ts + (uint32_t)(c + 32 + 16 * h2), w2);
                     }
-                    st16(ts + (uint32_t)(c / 2), w);
-                    st16(ts + (uint32_t)(kTcTile / 2 + c / 2), w2);
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 tmem_wait_st();
