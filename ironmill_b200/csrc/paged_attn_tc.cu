@@ -35,7 +35,7 @@ struct TcShape {
     static constexpr int kBlock = 128 * 128;  // bytes of 128 rows of 64 columns
     static constexpr int kQ = (WIDE ? 2 : 1) * KB * kBlock, kSlot = KB * kBlock;
     static constexpr int kK = 3, kV = WIDE ? 2 : 3;  // slots
-    static constexpr int kBars = 2 * kK + 2 * kV + 2 + 8 + 1;
+    static constexpr int kBars = 2 * kK + 2 * kV + 2 + 2 + 4 + 2 + 2 + 1;
     static constexpr int kSmall = 8 * 16 + 128 * 8 + kTcCopyWarps * 32 * 8 + kBars * 8 + 8;  // presence bits, maxima and sums, offsets, barriers, address
     static constexpr int kTiles = kQ + (kK + kV) * kSlot;
     static constexpr int kSmem = (kSmall + 1023) / 1024 * 1024 + kTiles;
@@ -102,22 +102,27 @@ __device__ __forceinline__ uint32_t sees32(const PagedAttn &p, const PagedUnit &
     return shift == 0 ? bits : bits << shift | ((1u << shift) - 1);
 }
 
-// Products issued by one elected lane of a converged warp. Everything they name is the same in all lanes (uniform() says so to the compiler): operands
-// that it had to move to uniform registers one by one cost more than the product.
+// Products and commits of one lane (`one`) of a converged warp: what they name is the same in all lanes, and uniform() says so where the compiler
+// cannot see it; from registers of a single lane it would move every operand of every product to a uniform register first.
 __device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
-    asm volatile("{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+__device__ __forceinline__ uint32_t elected() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}\n" : "=r"(one));
+    return one;
+}
+__device__ __forceinline__ void umma_ss(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %5, 0;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(one)
                  : "memory");
 }
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {  // A operand in tensor memory
-    asm volatile("{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+__device__ __forceinline__ void umma_ts(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {  // A operand in tensor memory
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %5, 0;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(one)
                  : "memory");
 }
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
-                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(bar)
+__device__ __forceinline__ void umma_commit(uint32_t one, uint64_t *bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)), "r"(one)
                  : "memory");
 }
 // Looks without waiting: try_wait may suspend the warp for a while.
@@ -139,7 +144,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     float2 *ml = reinterpret_cast<float2 *>(there + 32);                       // [128]: the second half's maximum and sum (not WIDE)
     long long *offs = reinterpret_cast<long long *>(ml + 128);                 // [copying warps][32]: where the rows that a warp copies lie
     uint64_t *kfull = reinterpret_cast<uint64_t *>(offs + kTcCopyWarps * 32), *kempty = kfull + SK, *vfull = kempty + SK, *vempty = vfull + SV, *qfull = vempty + SV,
-             *qempty = qfull + 1, *sfull = qempty + 1, *pfull = sfull + 2, *ofull = pfull + 2, *oempty = ofull + 2, *mlfull = oempty + 2;
+             *qempty = qfull + 1, *sfull = qempty + 1, *pfull = sfull + 2, *ofull = pfull + 4, *oempty = ofull + 2, *mlfull = oempty + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mlfull + 1);
     // (shared memory starts at a multiple of 1024: checked, the tiles would not fit otherwise)
     unsigned char *Qs = tc_smem + (Shape::kSmem - Shape::kTiles), *Ks = Qs + Shape::kQ, *Vs = Ks + SK * Shape::kSlot;
@@ -161,7 +166,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
         mbar_init(qempty, 1);
         for (int i = 0; i < 2; i++) {
             mbar_init(&sfull[i], 1);
-            mbar_init(&pfull[i], 4);
+            mbar_init(&pfull[2 * i], 4);
+            mbar_init(&pfull[2 * i + 1], 4);
             mbar_init(&ofull[i], 1);
             mbar_init(&oempty[i], 4);
         }
@@ -175,7 +181,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = uniform(*tmem_slot);
     pdl_trigger();  // after the allocation: a successor on this SM cannot take the columns first
     pdl_wait();
     const Share share = find_share<R, kTcTile, kTcThreads>(p, units, reinterpret_cast<long long *>(Qs));  // (no copy is under way yet)
@@ -276,86 +282,104 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
         }
         flush();
     } else if (warp == kTcMma) {
-        // ---- products, one thread issues them all. Instruction descriptors as in flash_tc.cu: f32 accumulator, fp16 (0) or bf16 (1) operands in bits
-        // 7-9 and 10-12, B MN-major in bit 16, N >> 3 in bits 17-22, M >> 4 in bits 24-28
+        // ---- products: one thread waits and issues them all; what it does between them is kept short, the tensor cores' queue holds only a few.
+        // Instruction descriptors as in flash_tc.cu: f32 accumulator, fp16 (0) or bf16 (1) operands in bits 7-9 and 10-12, B MN-major in bit 16, N >> 3 in
+        // bits 17-22, M >> 4 in bits 24-28
         constexpr uint32_t kType = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(128 >> 4) << 24);
         constexpr uint32_t kS = kType | ((uint32_t)(kTcTile >> 3) << 17), kPV = kType | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
-        int kc = 0, vc = 0, turn[2] = {0, 0};
-        auto scores = [&](int h) {
-            const int s = kc % SK;
-            if (ok && !wait_for(&kfull[s], (kc / SK) & 1, err)) ok = false;
-            fence_after();
-            if (ok) {
-                const uint32_t k0 = uniform(smem_u32(Ks) + s * Shape::kSlot), q0 = uniform(smem_u32(Qs) + (WIDE ? h * KB * BLK : 0)), d = uniform(tmem + (uint32_t)(h * kTcTile));
-                const uint64_t qd = desc_sw128(q0, 16), kd = desc_sw128(k0, 16);
-#pragma unroll 1
-                for (int j = 0; j < KB * 4; j += 4)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) umma_ss(d, qd + (j / 4 * BLK + i * 32) / 16, kd + (j / 4 * BLK + i * 32) / 16, kS, i > 0 || j > 0);
-                umma_commit(uniform(smem_u32(&sfull[h])));
-            }
-            __syncwarp();
-        };
-        auto values = [&](int h, bool first, bool last) {
-            const int s = vc % SV;
-            if (ok && !wait_for(&pfull[h], turn[h] & 1, err)) ok = false;
-            turn[h]++;
-            if (ok && !wait_for(&vfull[s], (vc / SV) & 1, err)) ok = false;
-            fence_after();
-            if (ok) {
-                const uint32_t v0 = uniform(smem_u32(Vs) + s * Shape::kSlot), w = uniform(tmem + (uint32_t)(h * kTcTile)), o = uniform(tmem + 256u + (uint32_t)(h * 128));
-                const uint64_t vd = desc_sw128(v0, BLK);
-                uint32_t more = uniform(first ? 0 : 1);
-                // (64 positions' weights: 32 columns of the first terms, 32 of the second)
-#pragma unroll 1
-                for (int j = 0; j < kTcTile / 16; j += 4) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) umma_ts(o, w + (uint32_t)(j * 16 + (i & 1) * 32 + (i >> 1) * 8), vd + (j + (i >> 1)) * 2048 / 16, kPV, i > 0 || more);
-                    more = 1;
-                }
-                if (last) umma_commit(uniform(smem_u32(&ofull[h])));
-            }
-            __syncwarp();
-        };
-        auto release = [&](uint64_t *bar) {  // once the products issued so far are done
-            if (ok) umma_commit(uniform(smem_u32(bar)));
-            __syncwarp();
-        };
-        while (it.next()) {
-            const int T = it.t1 - it.t0;
-            if (ok && !wait_for(qfull, it.index & 1, err)) ok = false;
-            auto drained = [&]() {  // the outputs of the item before have been read
-                if (it.index > 0)
-                    for (int h = 0; h < 2; h++)
-                        if (ok && !wait_for(&oempty[h], (it.index - 1) & 1, err)) ok = false;
+        {
+            const uint32_t one = elected();
+            const uint64_t qd = desc_sw128(smem_u32(Qs), 16), kd = desc_sw128(smem_u32(Ks), 16), vd = desc_sw128(smem_u32(Vs), BLK);
+            int ks = 0, vs = 0, turn0 = 0, turn1 = 0;     // slots; weights of the halves that were waited for
+            uint32_t kturn = 0, vturn = 0;                // parities of the slots' turns
+            auto wait = [&](uint64_t *bar, uint32_t parity) {
+                if (ok && !mbar_try_wait(bar, parity)) ok = wait_for(bar, parity, err);
+                __syncwarp();
             };
-            if constexpr (WIDE) {
-                const int halves = it.u.rows > 128 ? 2 : 1;
-                for (int t = 0; t <= T; t++) {
-                    if (t == 1) drained();
-                    for (int h = 0; h < halves; h++) {
-                        if (t > 0) values(h, t == 1, t == T);
-                        if (t < T) scores(h);
-                    }
-                    if (t > 0) release(&vempty[vc++ % SV]);
-                    if (t < T) release(&kempty[kc++ % SK]);
-                    if (t == T - 1) release(qempty);
+            auto scores = [&](int h) {
+                fence_after();
+                if (!ok) return;
+                const uint64_t a = qd + (WIDE && h ? KB * BLK / 16 : 0), b = kd + ks * (Shape::kSlot / 16);
+#pragma unroll
+                for (int j = 0; j < KB * 4; j++) umma_ss(one, tmem + (uint32_t)(h * kTcTile), a + (j / 4 * BLK + (j & 3) * 32) / 16, b + (j / 4 * BLK + (j & 3) * 32) / 16, kS, j > 0);
+                umma_commit(one, &sfull[h]);
+            };
+            auto values = [&](int h, bool first, bool last) {
+                const uint32_t w = tmem + (uint32_t)(h * kTcTile), o = tmem + 256u + (uint32_t)(h * 128), turn = (h ? turn1 : turn0) & 1;
+                const uint64_t b = vd + vs * (Shape::kSlot / 16);
+#pragma unroll 1
+                for (int c = 0; c < 2; c++) {  // 64 positions: 32 columns of the weights' first terms, 32 of the second
+                    wait(&pfull[2 * h + c], turn);
+                    fence_after();
+                    if (!ok) return;
+#pragma unroll
+                    for (int i = 0; i < 8; i++)
+                        umma_ts(one, o, w + (uint32_t)(c * 64 + (i & 1) * 32 + (i >> 1) * 8), b + (c * 4 + (i >> 1)) * (2048 / 16), kPV, i > 0 || c > 0 || !first);
                 }
-            } else {
-                for (int t = 0; t < T + 2; t++) {
-                    if (t == 2) drained();
-                    if (t >= 2) {
-                        values(t & 1, t < 4, t >= T);
-                        release(&vempty[vc++ % SV]);
+                turn0 += !h;
+                turn1 += h;
+                if (last) umma_commit(one, &ofull[h]);
+            };
+            auto release = [&](uint64_t *bar) {  // once the products issued so far are done
+                if (ok) umma_commit(one, bar);
+            };
+            auto k_done = [&]() {
+                release(&kempty[ks]);
+                if (++ks == SK) ks = 0, kturn ^= 1;
+            };
+            auto v_done = [&]() {
+                release(&vempty[vs]);
+                if (++vs == SV) vs = 0, vturn ^= 1;
+            };
+            while (it.next()) {
+                const int T = (int)uniform(it.t1 - it.t0);
+                wait(qfull, it.index & 1);
+                auto drained = [&]() {  // the outputs of the item before have been read
+                    if (it.index > 0) {
+                        wait(&oempty[0], (it.index - 1) & 1);
+                        wait(&oempty[1], (it.index - 1) & 1);
                     }
-                    if (t < T) {
-                        scores(t & 1);
-                        release(&kempty[kc++ % SK]);
+                };
+                if constexpr (WIDE) {
+                    const int halves = (int)uniform(it.u.rows > 128 ? 2 : 1);
+#pragma unroll 1
+                    for (int t = 0; t <= T; t++) {
+                        if (t == 1) drained();
+#pragma unroll 1
+                        for (int h = 0; h < halves; h++) {
+                            if (t > 0) {
+                                if (h == 0) wait(&vfull[vs], vturn);
+                                values(h, t == 1, t == T);
+                            }
+                            if (t < T) {
+                                if (h == 0) wait(&kfull[ks], kturn);
+                                scores(h);
+                            }
+                        }
+                        if (t > 0) v_done();
+                        if (t < T) k_done();
+                        if (t == T - 1) release(qempty);
                     }
-                    if (t == T - 1) release(qempty);
+                } else {
+#pragma unroll 1
+                    for (int t = 0; t < T + 2; t++) {
+                        if (t == 2) drained();
+                        if (t >= 2) {
+                            wait(&vfull[vs], vturn);
+                            values(t & 1, t < 4, t >= T);
+                            v_done();
+                        }
+                        if (t < T) {
+                            wait(&kfull[ks], kturn);
+                            scores(t & 1);
+                            k_done();
+                        }
+                        if (t == T - 1) release(qempty);
+                    }
                 }
             }
         }
+        __syncwarp();
     } else {
         // ---- weights: a row per thread
         const int h = warp >> 2, r = (warp & 3) * 32 + lane, R_ = WIDE ? h * 128 + r : r;
@@ -439,12 +463,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                         st16(ts + (uint32_t)(c + 16 * h2), w);
                         st16(ts + (uint32_t)(c + 32 + 16 * h2), w2);
                     }
+                    tmem_wait_st();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&pfull[2 * h + c / 64]);
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tmem_wait_st();
-                fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&pfull[h]);
             }
             tiles_before += T;
             // ---- the item's (or the share's part of it) rows
