@@ -408,40 +408,56 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
-// Items that a cut divides: a block per (item, row), a thread per column. The parts of an item lie with the CTAs that its tiles fall to.
-template <bool BF16, int R>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttn p, int units) {
+// Items that a cut divides: a warp per row, HD / 32 columns a lane. The parts of an item lie with the CTAs that its tiles fall to; a lane per part
+// brings maxima and sums. (A block per row with the shares' divisions in loops took 25 us for 64 items of 104 rows.)
+constexpr int kJoinWarps = 8;
+template <bool BF16, int R, int HD>
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __grid_constant__ PagedAttn p, int units) {
+    constexpr int V = HD / 32;
     pdl_trigger();
     pdl_wait();
-    const int item = blockIdx.x, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, r = blockIdx.y, hd = p.kv.hd, d = threadIdx.x;
-    const long long before = p.first[unit];
+    const int item = blockIdx.x, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, lane = threadIdx.x & 31, r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5);
+    const long long before = p.first[unit], all = p.first[units];
     const int tiles = (int)(p.first[unit + 1] - before);
     if (tiles == 0) return;
-    const long long total = p.first[units] * p.kv.nkv, a = before * p.kv.nkv + (long long)head * tiles, b = a + tiles;
+    const long long total = all * p.kv.nkv, a = before * p.kv.nkv + (long long)head * tiles;
     const int n = share_count(total, p.ctas);
-    int c = (int)(a * n / total);
-    while (share_at(total, n, c + 1) <= a) c++;
-    while (share_at(total, n, c) > a) c--;
-    if (share_at(total, n, c + 1) >= b) return;  // one CTA had all of it
+    const int c = share_of(total, n, a), parts = share_of(total, n, a + tiles - 1) - c + 1;
+    if (parts == 1) return;  // one CTA had all of it
     const PagedUnit u = paged_unit<R>(p, unit);
     if (r >= u.rows) return;
-    const int slot0 = share_at(total, n, c) == a ? 0 : 1;
-    int c1 = c;
-    while (share_at(total, n, c1 + 1) < b) c1++;
-    float M = -INFINITY, L = 0.0f, o = 0.0f;
-    auto at = [&](int i) { return ((size_t)i * 2 + (i == c ? slot0 : 0)) * R + r; };
-    for (int i = c; i <= c1; i++) M = fmaxf(M, p.part_ml[at(i)].x);
-    for (int i = c; i <= c1; i++) {
-        const size_t w = at(i);
-        const float2 x = p.part_ml[w];
-        if (x.x == -INFINITY && x.y == 0.0f) continue;  // sees nothing of this part
-        const float f = ex2(x.x - M);
-        L += x.y * f;
-        o += p.part_o[w * hd + d] * f;
+    const size_t slot0 = (size_t)c * 2 + (share_at(total, n, c) == a ? 0 : 1);
+    auto at = [&](int i) { return (i == 0 ? slot0 : (size_t)(c + i) * 2) * R + r; };
+    float M = -INFINITY, L = 0.0f, o[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) o[j] = 0.0f;
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+        const float2 x = i0 + lane < parts ? p.part_ml[at(i0 + lane)] : make_float2(-INFINITY, 0.0f);
+        const float top = fmaxf(M, warp_max(x.x)), corr = M == top ? 1.0f : ex2(M - top);
+        const float f = x.x == -INFINITY && x.y == 0.0f ? 0.0f : ex2(x.x - top);  // (nothing seen in this part)
+        M = top;
+        L = L * corr + warp_sum(x.y * f);
+#pragma unroll
+        for (int j = 0; j < V; j++) o[j] *= corr;
+        const int m = min(32, parts - i0);
+#pragma unroll 4
+        for (int i = 0; i < m; i++) {
+            const float *src = p.part_o + at(i0 + i) * HD + lane * V;
+            const float g = __shfl_sync(0xffffffffu, f, i);
+            float v[V];
+            if constexpr (V == 2) *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(src);
+            else
+#pragma unroll
+                for (int j = 0; j < V; j += 4) *reinterpret_cast<float4 *>(v + j) = *reinterpret_cast<const float4 *>(src + j);
+#pragma unroll
+            for (int j = 0; j < V; j++) o[j] += g == 0.0f ? 0.0f : v[j] * g;
+        }
     }
     const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
     const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
-    p.out[(u.tok0 + t) * p.os + (long long)(head * p.group + g) * hd + d] = (uint16_t)pack16<BF16>(o * inv, 0.0f);
+    uint32_t *dst = reinterpret_cast<uint32_t *>(p.out + (u.tok0 + t) * p.os + (long long)(head * p.group + g) * HD + lane * V);
+#pragma unroll
+    for (int j = 0; j < V; j += 2) dst[j / 2] = pack16<BF16>(o[j] * inv, o[j + 1] * inv);
 }
 
 struct AttnPlan {
@@ -462,9 +478,10 @@ AttnPlan attn_plan(const Device *dev, int nseq, int nkv, int hd, int group, int 
     return a;
 }
 
-template <bool BF16, int R>
+template <bool BF16, int R, int HD>
 int join_launch(const PagedAttn &p, int units, cudaStream_t st) {
-    IM_CUDA_CHECK(launch_k(paged_join_kernel<BF16, R>, dim3((unsigned)(units * p.kv.nkv), (unsigned)std::min<long long>(R, (long long)p.max_new * p.group)), dim3(p.kv.hd), 0, st, p,
+    const long long rows = std::min<long long>(R, (long long)p.max_new * p.group);
+    IM_CUDA_CHECK(launch_k(paged_join_kernel<BF16, R, HD>, dim3((unsigned)(units * p.kv.nkv), (unsigned)((rows + kJoinWarps - 1) / kJoinWarps)), dim3(kJoinWarps * 32), 0, st, p,
                            units));
     return IM_OK;
 }
@@ -475,7 +492,7 @@ int attn_launch(const Device *dev, const PagedAttn &p, int units, cudaStream_t s
     static DeviceOnce once;
     if (once.first(dev->ordinal)) IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, MT>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     IM_CUDA_CHECK(launch_k(paged_attn_kernel<BF16, HD, MT>, dim3(p.ctas), dim3(kPaThreads), (size_t)S::kSmem, st, p, units));
-    return join_launch<BF16, S::kRows>(p, units, st);
+    return join_launch<BF16, S::kRows, HD>(p, units, st);
 }
 
 int attn_check(const im_paged_kv *kv, int num_heads, int max_new) {
@@ -544,8 +561,10 @@ IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int
     if (plan.rows >= 128) {
         rc = paged_tc_launch(dev, p, bf16, plan.rows, plan.units, st);
         if (rc != IM_OK) return rc;
-        if (plan.rows == 128) return bf16 ? join_launch<true, 128>(p, plan.units, st) : join_launch<false, 128>(p, plan.units, st);
-        return bf16 ? join_launch<true, 256>(p, plan.units, st) : join_launch<false, 256>(p, plan.units, st);
+#define IM_JOIN(R, HD) (bf16 ? join_launch<true, R, HD>(p, plan.units, st) : join_launch<false, R, HD>(p, plan.units, st))
+        if (kv->head_dim == 64) return plan.rows == 128 ? IM_JOIN(128, 64) : IM_JOIN(256, 64);
+        return plan.rows == 128 ? IM_JOIN(128, 128) : IM_JOIN(256, 128);
+#undef IM_JOIN
     }
 #define IM_RUN(HD, MT) (bf16 ? attn_launch<true, HD, MT>(dev, p, plan.units, st) : attn_launch<false, HD, MT>(dev, p, plan.units, st))
     switch (kv->head_dim) {

@@ -94,6 +94,9 @@ struct Share {
 __device__ __forceinline__ int share_count(long long total, int ctas) { return (int)min((long long)ctas, total); }
 __device__ __forceinline__ long long share_at(long long total, int n, int c) { return c >= n ? total : total * c / n; }
 
+// The share that place a falls to: the last c with total * c / n <= a.
+__device__ __forceinline__ int share_of(long long total, int n, long long a) { return (int)(((a + 1) * n - 1) / total); }
+
 template <int R, int TILE, int THREADS>
 __device__ __forceinline__ Share find_share(const PagedAttn &p, int units, long long *sums) {
     int *found = reinterpret_cast<int *>(sums + THREADS + 32);  // unit, head, tile
