@@ -558,14 +558,7 @@ IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int
     p.first = reinterpret_cast<long long *>(p.part_ml + slots);
     const cudaStream_t st = as_stream(stream);
     const bool bf16 = kv->dtype == IM_DTYPE_BF16;
-    if (plan.rows >= 128) {
-        rc = paged_tc_launch(dev, p, bf16, plan.rows, plan.units, st);
-        if (rc != IM_OK) return rc;
-#define IM_JOIN(R, HD) (bf16 ? join_launch<true, R, HD>(p, plan.units, st) : join_launch<false, R, HD>(p, plan.units, st))
-        if (kv->head_dim == 64) return plan.rows == 128 ? IM_JOIN(128, 64) : IM_JOIN(256, 64);
-        return plan.rows == 128 ? IM_JOIN(128, 128) : IM_JOIN(256, 128);
-#undef IM_JOIN
-    }
+    if (plan.rows >= 128) return paged_tc_launch(dev, p, bf16, plan.rows, plan.units, st);
 #define IM_RUN(HD, MT) (bf16 ? attn_launch<true, HD, MT>(dev, p, plan.units, st) : attn_launch<false, HD, MT>(dev, p, plan.units, st))
     switch (kv->head_dim) {
     case 64: return plan.rows == 16 ? IM_RUN(64, 1) : IM_RUN(64, 2);

@@ -131,6 +131,10 @@ __device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
     asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
     return ok != 0;
 }
+// Sums of weighted values that a share leaves: four columns of all rows after another, since a warp that writes (and one that joins) has a row per lane.
+template <int R>
+__device__ __forceinline__ float *tc_part(float *part_o, size_t slot, int hd, int row, int col) { return part_o + (slot * (hd / 4) + col / 4) * (R * 4) + row * 4 + col % 4; }
+
 __device__ __forceinline__ void zcopy(uint32_t dst, const void *src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
@@ -499,7 +503,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             fence_after();
             const bool live = R_ < u.rows && ok;
             const bool whole = it.t0 == 0 && it.t1 == it.tiles;
-            const size_t part = ((size_t)blockIdx.x * 2 + (it.index == 0 ? 0 : 1)) * R + R_;
+            const size_t slot = (size_t)blockIdx.x * 2 + (it.index == 0 ? 0 : 1);
             const float inv = whole ? (l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l) : 1.0f;
             uint16_t *out = p.out + (u.tok0 + token) * p.os + (long long)(it.head * p.group + (u.row0 + min(R_, u.rows - 1)) % p.group) * HD;
             float worst = 0.0f;
@@ -528,10 +532,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                                                                                  pack2<BF16>(v[j + 4] * inv, v[j + 5] * inv), pack2<BF16>(v[j + 6] * inv, v[j + 7] * inv));
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(p.part_o + part * HD + c + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                        for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(tc_part<R>(p.part_o, slot, HD, R_, c + j)) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
                     }
                 }
-                if (live && !whole) p.part_ml[part] = make_float2(m, l);
+                if (live && !whole) p.part_ml[slot * R + R_] = make_float2(m, l);
             }
             fence_before();
             __syncwarp();
@@ -546,13 +550,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 float x[HD / 32], M, L;
                 plain_row<BF16, HD>(p, u, it.head, row, it.t0 * kTcTile, min(it.t1 * kTcTile, u.end), x, M, L);
                 const float n = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
-                const size_t at = ((size_t)blockIdx.x * 2 + (it.index == 0 ? 0 : 1)) * R + row;
                 uint16_t *to_row = p.out + (u.tok0 + (u.row0 + row) / p.group) * p.os + (long long)(it.head * p.group + (u.row0 + row) % p.group) * HD;
                 for (int i = 0; i < HD / 32; i++) {
                     if (whole) to_row[lane + 32 * i] = (uint16_t)pack2<BF16>(x[i] * n, 0.0f);
-                    else p.part_o[at * HD + lane + 32 * i] = x[i];
+                    else *tc_part<R>(p.part_o, slot, HD, row, lane + 32 * i) = x[i];
                 }
-                if (!whole && lane == 0) p.part_ml[at] = make_float2(M, L);
+                if (!whole && lane == 0) p.part_ml[slot * R + row] = make_float2(M, L);
             }
         }
     }
@@ -564,12 +567,54 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     }
 }
 
+// Items that a cut divides: a warp per 32 rows and eight columns, a row per lane.
+template <bool BF16, int KB, bool WIDE>
+__global__ void __launch_bounds__(256) paged_tc_join_kernel(const __grid_constant__ PagedAttn p, int units) {
+    constexpr int R = TcShape<KB, WIDE>::kRows, HD = 64 * KB;
+    pdl_trigger();
+    pdl_wait();
+    const int item = blockIdx.x, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, lane = threadIdx.x & 31;
+    const int w = blockIdx.y * 8 + (threadIdx.x >> 5), r = w / (HD / 8) * 32 + lane, c = w % (HD / 8) * 8;
+    const long long before = p.first[unit], all = p.first[units];
+    const int tiles = (int)(p.first[unit + 1] - before);
+    if (tiles == 0) return;
+    const long long total = all * p.kv.nkv, a = before * p.kv.nkv + (long long)head * tiles;
+    const int n = share_count(total, p.ctas);
+    const int first = share_of(total, n, a), parts = share_of(total, n, a + tiles - 1) - first + 1;
+    if (parts == 1) return;  // one CTA had all of it
+    const PagedUnit u = paged_unit<R>(p, unit);
+    if (r >= u.rows) return;
+    const size_t slot0 = (size_t)first * 2 + (share_at(total, n, first) == a ? 0 : 1);
+    float M = -INFINITY, L = 0.0f, o[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) o[j] = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < parts; i++) M = fmaxf(M, p.part_ml[(i == 0 ? slot0 : (size_t)(first + i) * 2) * R + r].x);
+#pragma unroll 4
+    for (int i = 0; i < parts; i++) {
+        const size_t slot = i == 0 ? slot0 : (size_t)(first + i) * 2;
+        const float2 x = p.part_ml[slot * R + r];
+        const float4 v = *reinterpret_cast<const float4 *>(tc_part<R>(p.part_o, slot, HD, r, c)), y = *reinterpret_cast<const float4 *>(tc_part<R>(p.part_o, slot, HD, r, c + 4));
+        if (x.x == -INFINITY && x.y == 0.0f) continue;  // nothing seen in this part
+        const float f = ex2(x.x - M);
+        L += x.y * f;
+        o[0] += v.x * f; o[1] += v.y * f; o[2] += v.z * f; o[3] += v.w * f;
+        o[4] += y.x * f; o[5] += y.y * f; o[6] += y.z * f; o[7] += y.w * f;
+    }
+    const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
+    const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
+    *reinterpret_cast<uint4 *>(p.out + (u.tok0 + t) * p.os + (long long)(head * p.group + g) * HD + c) =
+        make_uint4(pack2<BF16>(o[0] * inv, o[1] * inv), pack2<BF16>(o[2] * inv, o[3] * inv), pack2<BF16>(o[4] * inv, o[5] * inv), pack2<BF16>(o[6] * inv, o[7] * inv));
+}
+
 template <bool BF16, int KB, bool WIDE>
 int tc_launch(const Device *dev, const PagedAttn &p, int units, cudaStream_t st) {
     using S = TcShape<KB, WIDE>;
     static DeviceOnce once;
     if (once.first(dev->ordinal)) IM_CUDA_CHECK(cudaFuncSetAttribute((paged_tc_kernel<BF16, KB, WIDE>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     IM_CUDA_CHECK(launch_k(paged_tc_kernel<BF16, KB, WIDE>, dim3(p.ctas), dim3(kTcThreads), (size_t)S::kSmem, st, p, units, dev->err_flag));
+    const long long rows = std::min<long long>(S::kRows, (long long)p.max_new * p.group);
+    IM_CUDA_CHECK(launch_k(paged_tc_join_kernel<BF16, KB, WIDE>, dim3((unsigned)(units * p.kv.nkv), (unsigned)((rows + 31) / 32 * KB)), dim3(256), 0, st, p, units));
     return IM_OK;
 }
 
