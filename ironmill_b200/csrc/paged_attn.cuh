@@ -92,7 +92,12 @@ struct Share {
 
 // No share is empty: CTAs without a tile of their own have none, and leave no parts.
 __device__ __forceinline__ int share_count(long long total, int ctas) { return (int)min((long long)ctas, total); }
-__device__ __forceinline__ long long share_at(long long total, int n, int c) { return c >= n ? total : total * c / n; }
+// floor(total * c / n); n at most 2^15
+__device__ __forceinline__ long long share_at(long long total, int n, int c) {
+    if (c >= n) return total;
+    const long long q = total >> 32 ? total / n : (long long)((uint32_t)total / (uint32_t)n);
+    return q * c + (uint32_t)((int)(total - q * n) * c) / (uint32_t)n;
+}
 
 // The share that place a falls to: the last c with total * c / n <= a.
 __device__ __forceinline__ int share_of(long long total, int n, long long a) { return (int)(((a + 1) * n - 1) / total); }

@@ -10,8 +10,7 @@
 // A row's accumulator is rescaled only when its maximum has grown by more than 2^8 (as in flash_tc.cu).
 //
 // K, V and queries come by 16-byte cp.async of four warps, rows looked up in the page table: any page size, rows that are not there are zeros and
-// known to be none (a bit per row). The copies run ahead over the ends of items; each is announced when it has landed and been made
-// visible to the tensor cores, the announcement lagging kLag copies behind the requests, or at once where the ring is full.
+// known to be none (a bit per row). The copies run ahead over the ends of items as far as the slots allow.
 //
 // All waits are bounded: one that runs out sets the device error word, every warp then runs to its end.
 #include <limits.h>
@@ -26,7 +25,6 @@ namespace {
 
 // warps 0-7: weights; 8: products; 9-12: copies
 constexpr int kTcTile = 128, kTcThreads = 13 * 32, kTcMma = 8, kTcCopy = 9, kTcCopyWarps = 4;
-constexpr int kLag = 2;          // copies in flight behind the one that is requested
 constexpr float kTcLazy = 8.0f;  // growth of a row's maximum (in powers of two) that is left in the weights
 
 template <int KB, bool WIDE>
@@ -125,12 +123,29 @@ __device__ __forceinline__ void umma_commit(uint32_t one, uint64_t *bar) {
                  "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)), "r"(one)
                  : "memory");
 }
-// Looks without waiting: try_wait may suspend the warp for a while.
-__device__ __forceinline__ bool mbar_test(uint64_t *bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-    return ok != 0;
+// Two f32 side by side.
+__device__ __forceinline__ uint64_t two(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
 }
+__device__ __forceinline__ float2 of_two(uint64_t x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// What copies of other threads have written, once their barrier says so, before the tensor cores read it.
+__device__ __forceinline__ void copies_landed() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // Sums of weighted values that a share leaves: four columns of all rows after another, since a warp that writes (and one that joins) has a row per lane.
 template <int R>
 __device__ __forceinline__ float *tc_part(float *part_o, size_t slot, int hd, int row, int col) { return part_o + (slot * (hd / 4) + col / 4) * (R * 4) + row * 4 + col % 4; }
@@ -159,14 +174,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         for (int i = 0; i < SK; i++) {
-            mbar_init(&kfull[i], kTcCopyWarps);
+            mbar_init(&kfull[i], kTcCopyWarps * 33);  // threads whose copies are there; warps that have said which rows are
             mbar_init(&kempty[i], 1);
         }
         for (int i = 0; i < SV; i++) {
-            mbar_init(&vfull[i], kTcCopyWarps);
+            mbar_init(&vfull[i], kTcCopyWarps * 32);
             mbar_init(&vempty[i], 1);
         }
-        mbar_init(qfull, kTcCopyWarps);
+        mbar_init(qfull, kTcCopyWarps * 32);
         mbar_init(qempty, 1);
         for (int i = 0; i < 2; i++) {
             mbar_init(&sfull[i], 1);
@@ -195,38 +210,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
         // ---- copies: this warp's 32 rows of every 128
         const int w0 = (warp - kTcCopy) * 32;
         long long *mine = offs + w0;
-        uint64_t *pending[kLag];  // announcements that are due, oldest first
-        int due = 0;
-        auto announce = [&](uint64_t *bar) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        auto room = [&](uint64_t *bar, uint32_t parity) {
+            if (ok && !mbar_try_wait(bar, parity)) ok = wait_for(bar, parity, err);
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar);
         };
-        auto flush = [&]() {
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            for (int i = 0; i < kLag; i++)
-                if (i < due) announce(pending[i]);
-            due = 0;
-        };
-        auto room = [&](uint64_t *bar, uint32_t parity) {  // nothing that others wait for is held back while this warp waits
-            if (!ok || __all_sync(0xffffffffu, mbar_test(bar, parity))) return;
-            flush();
-            if (!wait_for(bar, parity, err)) ok = false;
-        };
-        auto requested = [&](uint64_t *bar) {
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            if (due == kLag) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
-                announce(pending[0]);
-#pragma unroll
-                for (int i = 0; i + 1 < kLag; i++) pending[i] = pending[i + 1];
-                pending[kLag - 1] = bar;
-            } else {
-#pragma unroll
-                for (int i = 0; i < kLag; i++)
-                    if (i == due) pending[i] = bar;
-                due++;
-            }
+        auto requested = [&](uint64_t *bar) {  // each thread arrives when what it has requested is there
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
         };
         // 32 rows whose offsets (elements from base; -1: none) are in mine[]
         auto rows32 = [&](unsigned char *dst, const uint16_t *base) {
@@ -272,7 +261,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 const long long next = t + 1 < it.t1 ? lookup(u, it.head, (t + 1) * kTcTile + w0 + lane) : -1;
                 if (kc >= SK) room(&kempty[ks], (kc / SK - 1) & 1);
                 const unsigned word = __ballot_sync(0xffffffffu, o >= 0);
-                if (lane == 0) there[(kc & 7) * 4 + w0 / 32] = word;
+                if (lane == 0) {
+                    there[(kc & 7) * 4 + w0 / 32] = word;
+                    mbar_arrive(&kfull[ks]);
+                }
                 place(o);
                 rows32(Ks + ks * Shape::kSlot, p.kc);
                 requested(&kfull[ks]);
@@ -284,7 +276,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 o = next;
             }
         }
-        flush();
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == kTcMma) {
         // ---- products: one thread waits and issues them all; what it does between them is kept short, the tensor cores' queue holds only a few.
         // Instruction descriptors as in flash_tc.cu: f32 accumulator, fp16 (0) or bf16 (1) operands in bits 7-9 and 10-12, B MN-major in bit 16, N >> 3 in
@@ -301,6 +293,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 __syncwarp();
             };
             auto scores = [&](int h) {
+                copies_landed();
                 fence_after();
                 if (!ok) return;
                 const uint64_t a = qd + (WIDE && h ? KB * BLK / 16 : 0), b = kd + ks * (Shape::kSlot / 16);
@@ -314,6 +307,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
 #pragma unroll 1
                 for (int c = 0; c < 2; c++) {  // 64 positions: 32 columns of the weights' first terms, 32 of the second
                     wait(&pfull[2 * h + c], turn);
+                    copies_landed();
                     fence_after();
                     if (!ok) return;
 #pragma unroll
@@ -445,7 +439,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 }
                 const float base = m == -INFINITY ? 0.0f : m;
                 tmem_wait_st();
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const uint64_t scale_two = two(scale, scale), base_two = two(-base, -base), minus_one = two(-1.0f, -1.0f);
+                uint64_t sum[2] = {0, 0};
 #pragma unroll 1
                 for (int c = 0; c < kTcTile; c += 64) {  // weights of 64 positions over their scores: first terms, second terms
                     uint32_t s[64];
@@ -457,12 +452,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                         uint32_t w[16], w2[16];
 #pragma unroll
                         for (int j = 0; j < 16; j++) {
-                            const float x0 = ex2(fmaf(__uint_as_float(s[32 * h2 + 2 * j]), scale, -base)), x1 = ex2(fmaf(__uint_as_float(s[32 * h2 + 2 * j + 1]), scale, -base));
-                            sum[(2 * j) & 3] += x0;
-                            sum[(2 * j + 1) & 3] += x1;
+                            const float2 e = of_two(fma_two(two(__uint_as_float(s[32 * h2 + 2 * j]), __uint_as_float(s[32 * h2 + 2 * j + 1])), scale_two, base_two));
+                            const float x0 = ex2(e.x), x1 = ex2(e.y);
+                            const uint64_t x = two(x0, x1);
+                            sum[j & 1] = add_two(sum[j & 1], x);
                             w[j] = pack2<BF16>(x0, x1);
                             const float2 back = unpack2<BF16>(w[j]);
-                            w2[j] = pack2<BF16>(x0 - back.x, x1 - back.y);
+                            const float2 left = of_two(fma_two(two(back.x, back.y), minus_one, x));
+                            w2[j] = pack2<BF16>(left.x, left.y);
                         }
                         st16(ts + (uint32_t)(c + 16 * h2), w);
                         st16(ts + (uint32_t)(c + 32 + 16 * h2), w2);
@@ -472,7 +469,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&pfull[2 * h + c / 64]);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                const float2 sums = of_two(add_two(sum[0], sum[1]));
+                l += sums.x + sums.y;
             }
             tiles_before += T;
             // ---- the item's (or the share's part of it) rows
