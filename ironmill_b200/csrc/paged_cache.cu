@@ -69,34 +69,37 @@ struct Append {
     int nh, tokens, max_pos, rot;
 };
 
-// One row of 8 angles' cosines or sines (entries at .. at + 7 of a row; entries from `most` on are not read)
+// Four entries of a table at a multiple of four: rows have head_dim / 2 of them, a multiple of four.
 template <bool F32>
-__device__ __forceinline__ void angles8(const void *table, long long at, int n, float *out) {
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        out[i] = 0.0f;
-        if (i < n) out[i] = F32 ? __ldg(static_cast<const float *>(table) + at + i) : __half2float(__ldg(static_cast<const __half *>(table) + at + i));
+__device__ __forceinline__ void angles4(const void *table, long long at, float *out) {
+    if (F32) {
+        *reinterpret_cast<float4 *>(out) = __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(table) + at));
+    } else {
+        const uint2 u = __ldg(reinterpret_cast<const uint2 *>(static_cast<const __half *>(table) + at));
+        const float2 lo = unpack16<false>(u.x), hi = unpack16<false>(u.y);
+        out[0] = lo.x; out[1] = lo.y; out[2] = hi.x; out[3] = hi.y;
     }
 }
 
-// A block per token; LANES lanes (the power of two from head_dim / 8 up) hold a head, eight columns each, and walk the heads with the same
-// cosines and sines. All heads of a thread are requested before the lookups of the token's place: one latency for the loads, one
-// chain for the place.
+// A block per token; `lanes` lanes (the power of two from head_dim / 8 up) hold a head, eight columns each, and walk the heads with the same
+// cosines and sines. The first heads of a thread are requested before the lookups of the token's place (its sequence, the sequence's length,
+// its page): one latency for the loads, one chain for the place, hidden by the other blocks of the SM.
+// FORM: 0 nothing is rotated; 1 halves, a column's partner a whole number of lanes away; 2 neighbours; 3 halves, partners anywhere.
 constexpr int kAppendThreads = 256;
 constexpr int kAppendHeads = 4;  // heads that a thread holds at a time
 
-template <bool BF16, bool NEIGH, bool F32>
-__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Append a, int lanes) {
+template <bool BF16, int FORM, bool F32>
+__global__ void __launch_bounds__(kAppendThreads, FORM == 3 ? 2 : 4) paged_append_kernel(const __grid_constant__ Append a, int lanes) {
     pdl_trigger();
     pdl_wait();
     const int token = blockIdx.x, tid = threadIdx.x;
     const int c = tid & (lanes - 1), first = tid / lanes, per = kAppendThreads / lanes;
-    const int hd = a.kv.hd, heads = a.nh + 2 * a.kv.nkv, d0 = 8 * c;
+    const int hd = a.kv.hd, heads = a.nh + 2 * a.kv.nkv, d0 = 8 * c, half = a.rot / 2;
     const bool mine = d0 < hd;
-    int row = 0, seq = 0;
     bool placed = false;
     long long at = -1;
     float cs[8], sn[8];
+#pragma unroll 1
     for (int h0 = first; h0 - first < heads; h0 += per * kAppendHeads) {  // the same count for every lane of a warp
         uint4 x[kAppendHeads];
 #pragma unroll
@@ -113,83 +116,77 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
             placed = true;
             const int lo = __ldg(a.start), hi = __ldg(a.start + a.kv.nseq);
             if (token < lo || token >= hi) return;
-            seq = paged_seq_of(a.start, a.kv.nseq, token);
-            const int place = token - __ldg(a.start + seq);
+            const int seq = paged_seq_of(a.start, a.kv.nseq, token), place = token - __ldg(a.start + seq);
             const long long r = (long long)a.kv.length(seq) + place;
             if (place < 0 || r > INT_MAX) return;
-            row = (int)r;
-            const int p = a.pos ? __ldg(a.pos + token) : row;
-            if (a.rot > 0) {
+            const int p = a.pos ? __ldg(a.pos + token) : (int)r;
+            if (FORM > 0) {
                 if ((unsigned)p >= (unsigned)a.max_pos) return;
-                const int half = a.rot / 2, e0 = NEIGH ? d0 / 2 : d0 < half ? d0 : d0 - half;
-                if (NEIGH || half % 8 == 0) {
-                    const int n = d0 < a.rot ? (NEIGH ? min(4, half - e0) : 8) : 0;
-                    angles8<F32>(a.cosc, (long long)p * (hd / 2) + e0, n, cs);
-                    angles8<F32>(a.sinc, (long long)p * (hd / 2) + e0, n, sn);
-                } else {  // a chunk may hold the end of one half and the start of the other
+                const long long row = (long long)p * (hd / 2);
+                if (FORM == 1 && d0 < a.rot) {
+                    const int e0 = d0 < half ? d0 : d0 - half;
+                    angles4<F32>(a.cosc, row + e0, cs);
+                    angles4<F32>(a.cosc, row + e0 + 4, cs + 4);
+                    angles4<F32>(a.sinc, row + e0, sn);
+                    angles4<F32>(a.sinc, row + e0 + 4, sn + 4);
+                }
+                if (FORM == 2 && mine) {
+                    angles4<F32>(a.cosc, row + d0 / 2, cs);
+                    angles4<F32>(a.sinc, row + d0 / 2, sn);
+                }
+                if (FORM == 3) {  // a chunk may hold the end of one half and the start of the other
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         const int d = d0 + i, e = d < half ? d : d - half;
                         cs[i] = sn[i] = 0.0f;
                         if (d < a.rot) {
-                            const long long w = (long long)p * (hd / 2) + e;
-                            cs[i] = F32 ? __ldg(static_cast<const float *>(a.cosc) + w) : __half2float(__ldg(static_cast<const __half *>(a.cosc) + w));
-                            sn[i] = F32 ? __ldg(static_cast<const float *>(a.sinc) + w) : __half2float(__ldg(static_cast<const __half *>(a.sinc) + w));
+                            cs[i] = F32 ? __ldg(static_cast<const float *>(a.cosc) + row + e) : __half2float(__ldg(static_cast<const __half *>(a.cosc) + row + e));
+                            sn[i] = F32 ? __ldg(static_cast<const float *>(a.sinc) + row + e) : __half2float(__ldg(static_cast<const __half *>(a.sinc) + row + e));
                         }
                     }
                 }
             }
-            at = a.kv.row_of(seq, row);
+            at = a.kv.row_of(seq, (int)r);
         }
 #pragma unroll
         for (int i = 0; i < kAppendHeads; i++) {
             const int h = h0 + i * per;
             const bool is_v = h >= a.nh + a.kv.nkv;
-            if (a.rot > 0) {
+            if (FORM > 0) {
                 uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-                float f[8], o[8];
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float2 t = unpack16<BF16>(w[j]);
-                    f[2 * j] = t.x;
-                    f[2 * j + 1] = t.y;
-                }
-                const int half = a.rot / 2;
-                if (NEIGH) {
+                float g[8];  // partners, where they are not in the same word
+                if (FORM == 1) {
+                    const int from = (threadIdx.x & 31 & ~(lanes - 1)) + ((c + (d0 < half ? half / 8 : lanes - half / 8)) & (lanes - 1));
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        o[2 * j] = f[2 * j] * cs[j] - f[2 * j + 1] * sn[j];
-                        o[2 * j + 1] = f[2 * j + 1] * cs[j] + f[2 * j] * sn[j];
+                        const float2 t = unpack16<BF16>(__shfl_sync(0xffffffffu, w[j], from));
+                        g[2 * j] = t.x;
+                        g[2 * j + 1] = t.y;
                     }
-                } else {
-                    float g[8];
-                    if (half % 8 == 0) {  // the partners are a lane's eight columns
-                        const int from = (threadIdx.x & 31 & ~(lanes - 1)) + ((c + (d0 < half ? half / 8 : lanes - half / 8)) & (lanes - 1));
+                }
+                if (FORM == 3) {
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const float2 t = unpack16<BF16>(__shfl_sync(0xffffffffu, w[j], from));
-                            g[2 * j] = t.x;
-                            g[2 * j + 1] = t.y;
+                    for (int j = 0; j < 8; j++) {
+                        const int d = d0 + j, partner = d < half ? d + half : d - half;
+                        g[j] = 0.0f;
+                        if (mine && h < heads && !is_v && d < a.rot) {
+                            const uint16_t *src = h < a.nh ? a.q + token * a.qs + (long long)h * hd : a.k + token * a.ks + (long long)(h - a.nh) * hd;
+                            g[j] = one16<BF16>(src + partner);
                         }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            const int d = d0 + j, partner = d < half ? d + half : d - half;
-                            g[j] = 0.0f;
-                            if (mine && h < heads && !is_v && d < a.rot) {
-                                const uint16_t *src = h < a.nh ? a.q + token * a.qs + (long long)h * hd : a.k + token * a.ks + (long long)(h - a.nh) * hd;
-                                g[j] = one16<BF16>(src + partner);
-                            }
-                        }
-                        __syncwarp();  // queries may be written over what was read
                     }
-#pragma unroll
-                    for (int j = 0; j < 8; j++) o[j] = d0 + j < half ? f[j] * cs[j] - g[j] * sn[j] : f[j] * cs[j] + g[j] * sn[j];
+                    __syncwarp();  // queries may be written over what was read
                 }
                 if (!is_v) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {  // rot is even: both columns of a word are rotated or neither is
-                        if (d0 + 2 * j < a.rot) w[j] = pack16<BF16>(o[2 * j], o[2 * j + 1]);
+                    for (int j = 0; j < 4; j++) {
+                        if (d0 + 2 * j >= a.rot) continue;  // (rot is even: both columns of a word are rotated or neither is)
+                        const float2 f = unpack16<BF16>(w[j]);
+                        if (FORM == 2) {
+                            w[j] = pack16<BF16>(f.x * cs[j] - f.y * sn[j], f.y * cs[j] + f.x * sn[j]);
+                        } else {
+                            const float y0 = d0 + 2 * j < half ? -g[2 * j] : g[2 * j], y1 = d0 + 2 * j + 1 < half ? -g[2 * j + 1] : g[2 * j + 1];
+                            w[j] = pack16<BF16>(f.x * cs[2 * j] + y0 * sn[2 * j], f.y * cs[2 * j + 1] + y1 * sn[2 * j + 1]);
+                        }
                     }
                 }
                 x[i] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -350,6 +347,7 @@ IM_EXPORT int im_cuda_paged_append(im_device *dev, const im_paged_kv *kv, int la
     IM_REQUIRE(rotary_dim >= 0 && rotary_dim <= kv->head_dim && rotary_dim % 2 == 0, "rotary_dim %d of %d", rotary_dim, kv->head_dim);
     IM_REQUIRE(rotary_dim == 0 || (cos_dev && sin_dev && max_pos > 0 && (table_dtype == IM_DTYPE_F16 || table_dtype == IM_DTYPE_F32)),
                "rotation needs tables of cosines and sines in fp16 or f32");
+    IM_REQUIRE(rotary_dim == 0 || (aligned16(cos_dev) && aligned16(sin_dev)), "tables of cosines and sines have to be 16-byte aligned");
     IM_REQUIRE(neighbours == 0 || neighbours == 1, "neighbours is 0 or 1");
     rc = paged_device(dev);
     if (rc != IM_OK) return rc;
@@ -366,14 +364,17 @@ IM_EXPORT int im_cuda_paged_append(im_device *dev, const im_paged_kv *kv, int la
     a.nh = num_heads; a.tokens = num_tokens; a.max_pos = max_pos; a.rot = rotary_dim;
     int lanes = 1;
     while (lanes * 8 < kv->head_dim) lanes *= 2;
-    const bool bf16 = kv->dtype == IM_DTYPE_BF16, f32 = rotary_dim > 0 && table_dtype == IM_DTYPE_F32;
+    const bool bf16 = kv->dtype == IM_DTYPE_BF16, f32 = table_dtype == IM_DTYPE_F32;
+    const int form = rotary_dim == 0 ? 0 : neighbours ? 2 : rotary_dim % 16 == 0 ? 1 : 3;
     void (*kern)(Append, int) = nullptr;
-    if (bf16)
-        kern = neighbours ? (f32 ? paged_append_kernel<true, true, true> : paged_append_kernel<true, true, false>)
-                          : (f32 ? paged_append_kernel<true, false, true> : paged_append_kernel<true, false, false>);
-    else
-        kern = neighbours ? (f32 ? paged_append_kernel<false, true, true> : paged_append_kernel<false, true, false>)
-                          : (f32 ? paged_append_kernel<false, false, true> : paged_append_kernel<false, false, false>);
+#define IM_FORM(F) (bf16 ? (f32 ? paged_append_kernel<true, F, true> : paged_append_kernel<true, F, false>) : (f32 ? paged_append_kernel<false, F, true> : paged_append_kernel<false, F, false>))
+    switch (form) {
+    case 0: kern = bf16 ? paged_append_kernel<true, 0, false> : paged_append_kernel<false, 0, false>; break;
+    case 1: kern = IM_FORM(1); break;
+    case 2: kern = IM_FORM(2); break;
+    default: kern = IM_FORM(3); break;
+    }
+#undef IM_FORM
     IM_CUDA_CHECK(launch_k(kern, dim3((unsigned)num_tokens), dim3(kAppendThreads), 0, as_stream(stream), a, lanes));
     return IM_OK;
     IM_GUARD_END

@@ -79,7 +79,7 @@ def test_layers_inside_pages_are_taken(lib):
 @pytest.mark.parametrize("change, word", [
     (dict(layer=2), "layer"), (dict(layer=-1), "layer"), (dict(k=None), "bad argument"), (dict(n=-1), "bad argument"), (dict(qo=None), "queries"), (dict(heads=0), "queries"),
     (dict(ks=248), "keys"), (dict(vs=260), "keys"), (dict(k=PTR + 2), "keys"), (dict(qs=8), "queries"), (dict(q=PTR + 4), "queries"), (dict(rot=130), "rotary"), (dict(rot=3), "rotary"),
-    (dict(cos=None), "tables"), (dict(table=2), "tables"), (dict(max_pos=0), "tables"), (dict(nb=2), "neighbours")])
+    (dict(cos=None), "tables"), (dict(table=2), "tables"), (dict(max_pos=0), "tables"), (dict(cos=PTR + 8), "aligned"), (dict(nb=2), "neighbours")])
 def test_appends_that_are_refused(lib, change, word):
     assert word in _message(lib, _append(lib, _kv(), **change))
 
