@@ -4,10 +4,11 @@
 // The logits are read once, from HBM; what bounds the pass is that read. Within a beam the order of the values is the order of its
 // logits, so nothing needs lse before the end: a block walks a slice of a row once for both the running maximum and sum of
 // exponentials and the slice's best `picks` logits, and a block per group joins the slices.
-//   best of a slice   a thread keeps only the maximum of the elements it meets. The picks-th largest of the threads' maxima, T, is a bound: at
-//                     least `picks` elements are >= T. Threads whose maximum reaches T look at their elements again (a few threads, from L2) and
-//                     collect those >= T; the rank of each collected element is the number of those before it. Where ties make the collection overflow
-//                     the elements are picked one after the other instead.
+//   best of a slice   the threads form at least `picks` sets; each thread knows the maximum of what it has met, and the lowest of the sets' maxima
+//                     is a bound that at least `picks` elements reach. What reaches it is collected as it comes; the bound is taken after the
+//                     first, second, fourth, eighth ... piece of the slice, so that few elements that do not belong to the best are collected (about
+//                     picks * ln(picks) for each doubling). A collected element's rank is the number of better ones. Where the collection overflows (ties,
+//                     rising rows) the elements are picked one after the other from memory instead.
 //   joining           the same with the slices' picks as elements and 64-bit values.
 // Sums are f32 per thread over its elements with one running maximum, joined in a fixed order: a run repeats bit by bit, and equal rows
 // get equal sums.
@@ -23,6 +24,7 @@ namespace im {
 namespace {
 
 constexpr int kSelThreads = 256, kSelMost = 64, kSelBuf = 1024;
+constexpr int kSelResident = 6;  // blocks of an SM
 constexpr int kSelLeast = 2048;  // elements of a slice: one request of 16-bit logits for every thread
 
 struct Select {
@@ -70,88 +72,103 @@ struct Logit<IM_DTYPE_F16> : Logit16<false> {};
 template <>
 struct Logit<IM_DTYPE_BF16> : Logit16<true> {};
 
-// Rank of a key among n keys in shared memory, larger first; keys differ.
+// Larger values first, then lower indexes.
 __device__ __forceinline__ bool before(double a, long long ia, double b, long long ib) { return a > b || (a == b && ia < ib); }
+__device__ __forceinline__ bool before(float a, int ia, float b, int ib) { return a > b || (a == b && ia < ib); }
 
-// The best of the block: value and index by all threads. `red` holds a value and an index per warp.
-__device__ __forceinline__ void block_best(double &v, long long &i, double *red_v, long long *red_i) {
+// What reaches the bound, and the best of it.
+template <typename V, typename I>
+struct Best {
+    V buf_v[kSelBuf];
+    I buf_i[kSelBuf];
+    V out_v[kSelMost];
+    I out_i[kSelMost];
+    V tops[kSelThreads];
+    int count;
+
+    __device__ __forceinline__ void clear(int picks) {  // no synchronisation: the first bound() has one
+        if (threadIdx.x == 0) count = 0;
+        for (int i = threadIdx.x; i < picks; i += kSelThreads) out_v[i] = -INFINITY, out_i[i] = -1;
+    }
+    // The lowest of the maxima of 8, 16, 32 or 64 >= picks sets of threads; top: this thread's maximum so far. A set has every so-many-th thread, so that
+    // none is without elements where the first threads have some.
+    __device__ __forceinline__ V bound(V top, int picks) {
+        __syncthreads();
+        tops[threadIdx.x] = top;
+        __syncthreads();
+        const int lane = threadIdx.x & 31;
+        V a = tops[lane], b = tops[32 + lane];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const double v2 = __shfl_xor_sync(0xffffffffu, v, o);
-        const long long i2 = __shfl_xor_sync(0xffffffffu, i, o);
-        if (before(v2, i2, v, i)) v = v2, i = i2;
+        for (int w = 2; w < kSelThreads / 32; w += 2) {
+            const V x = tops[32 * w + lane], y = tops[32 * w + 32 + lane];
+            a = a > x ? a : x;
+            b = b > y ? b : y;
+        }
+        V v = picks > 32 ? (a < b ? a : b) : a > b ? a : b;
+        const int sets = picks <= 8 ? 8 : picks <= 16 ? 16 : 32;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const V x = __shfl_xor_sync(0xffffffffu, v, o);
+            v = o >= sets ? (v > x ? v : x) : v < x ? v : x;
+        }
+        return v;
     }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) red_v[threadIdx.x >> 5] = v, red_i[threadIdx.x >> 5] = i;
-    __syncthreads();
-    v = red_v[0], i = red_i[0];
-    for (int w = 1; w < kSelThreads / 32; w++)
-        if (before(red_v[w], red_i[w], v, i)) v = red_v[w], i = red_i[w];
-}
-
-// The `picks` best of the elements that visit(f) hands to f(value, index) thread by thread, the same ones at every call, into out_v / out_i in order
-// (the rest -inf, -1). top: the largest value this thread hands out. Elements of -inf (and NaN) are none.
-template <typename Visit>
-__device__ __forceinline__ void pick_best(Visit visit, double top, int picks, double *out_v, long long *out_i) {
-    __shared__ double tops[kSelThreads], buf_v[kSelBuf];
-    __shared__ long long buf_i[kSelBuf];
-    __shared__ double bound;
-    __shared__ int count;
-    const int t = threadIdx.x;
-    tops[t] = top;
-    if (t == 0) count = 0, bound = -INFINITY;
-    for (int i = t; i < picks; i += kSelThreads) out_v[i] = -INFINITY, out_i[i] = -1;
-    __syncthreads();
-    int rank = 0;
-    for (int j = 0; j < kSelThreads; j++) rank += before(tops[j], j, top, t);
-    if (rank == picks - 1) bound = top;
-    __syncthreads();
-    if (top >= bound && top > -INFINITY)
-        visit([&](float v, double value, long long index) {
-            if (value >= bound && value > -INFINITY) {
-                const int at = atomicAdd(&count, 1);
-                if (at < kSelBuf) buf_v[at] = value, buf_i[at] = index;
+    __device__ __forceinline__ void collect(V v, I i) {
+        const int at = atomicAdd(&count, 1);
+        if (at < kSelBuf) buf_v[at] = v, buf_i[at] = i;
+    }
+    // The best into out_v, out_i, in order. visit(f) hands all elements of this thread to f(value, index).
+    template <typename Visit>
+    __device__ __forceinline__ void rank(int picks, Visit visit) {
+        __syncthreads();
+        const int t = threadIdx.x, n = count;
+        if (n <= kSelBuf) {
+            for (int i = t; i < n; i += kSelThreads) {
+                const V v = buf_v[i];
+                const I x = buf_i[i];
+                int r = 0;
+                for (int j = 0; j < n; j++) r += before(buf_v[j], buf_i[j], v, x);
+                if (r < picks) out_v[r] = v, out_i[r] = x;
             }
-            (void)v;
-        });
-    __syncthreads();
-    const int n = count;
-    if (n <= kSelBuf) {
-        for (int i = t; i < n; i += kSelThreads) {
-            const double v = buf_v[i];
-            const long long x = buf_i[i];
-            int r = 0;
-            for (int j = 0; j < n && r < picks; j++) r += before(buf_v[j], buf_i[j], v, x);
-            if (r < picks) out_v[r] = v, out_i[r] = x;
+        } else {
+            V last_v = INFINITY;
+            I last_i = -1;
+            for (int k = 0; k < picks; k++) {
+                V v = -INFINITY;
+                I x = 0x7fffffff;
+                visit([&](V value, I index) {
+                    if (value > -INFINITY && before(last_v, last_i, value, index) && (before(value, index, v, x) || !(v > -INFINITY))) v = value, x = index;
+                });
+#pragma unroll 1
+                for (int o = 16; o > 0; o >>= 1) {
+                    const V v2 = __shfl_xor_sync(0xffffffffu, v, o);
+                    const I x2 = __shfl_xor_sync(0xffffffffu, x, o);
+                    if (before(v2, x2, v, x)) v = v2, x = x2;
+                }
+                __syncthreads();
+                if ((t & 31) == 0) buf_v[t >> 5] = v, buf_i[t >> 5] = x;
+                __syncthreads();
+                v = buf_v[0], x = buf_i[0];
+                for (int w = 1; w < kSelThreads / 32; w++)
+                    if (before(buf_v[w], buf_i[w], v, x)) v = buf_v[w], x = buf_i[w];
+                if (!(v > -INFINITY)) break;
+                if (t == 0) out_v[k] = v, out_i[k] = x;
+                last_v = v;
+                last_i = x;
+            }
         }
-    } else {
-        double last_v = INFINITY;
-        long long last_i = -1;
-        for (int k = 0; k < picks; k++) {
-            double v = -INFINITY;
-            long long x = LLONG_MAX;
-            visit([&](float, double value, long long index) {
-                if (value > -INFINITY && before(last_v, last_i, value, index) && before(value, index, v, x)) v = value, x = index;
-            });
-            block_best(v, x, buf_v, buf_i);
-            if (!(v > -INFINITY)) break;
-            if (t == 0) out_v[k] = v, out_i[k] = x;
-            last_v = v;
-            last_i = x;
-        }
+        __syncthreads();
     }
-    __syncthreads();
-}
+};
 
 // grid (slices, rows)
 template <int DT>
-__global__ void __launch_bounds__(kSelThreads) beam_slice_kernel(const Select p) {
+__global__ void __launch_bounds__(kSelThreads, kSelResident) beam_slice_kernel(const __grid_constant__ Select p) {
     using L = Logit<DT>;
     using T = typename L::T;
-    constexpr int V = L::kVec;
+    constexpr int V = L::kVec, Q = 16 / V;  // requests of a piece: 16 elements of each thread
+    __shared__ Best<float, int> best;
     __shared__ float red_m[kSelThreads / 32], red_s[kSelThreads / 32];
-    __shared__ double out_v[kSelMost];
-    __shared__ long long out_i[kSelMost];
     pdl_trigger();
     pdl_wait();
     const int slice = blockIdx.x, t = threadIdx.x;
@@ -160,64 +177,79 @@ __global__ void __launch_bounds__(kSelThreads) beam_slice_kernel(const Select p)
     const T *x = static_cast<const T *>(p.x) + row * p.stride;
     const int a = slice * p.slice, b = min(a + p.slice, p.vocab);
     // 16-byte requests from the first aligned element on; what is before and behind them is read one by one
-    const int head = min(b - a, (int)((16 - (reinterpret_cast<uintptr_t>(x + a) & 15)) % 16 / sizeof(T)));
-    const int vecs = (b - a - head) / V, tail = a + head + vecs * V;
+    const int head = max(min(b - a, (int)((16 - (reinterpret_cast<uintptr_t>(x + a) & 15)) % 16 / sizeof(T))), 0);
+    const int vecs = max(b - a - head, 0) / V, tail = a + head + vecs * V;
     const uint4 *xv = reinterpret_cast<const uint4 *>(x + a + head);
+    best.clear(p.picks);
     float m = -INFINITY, s = 0.0f;
-    auto take = [&](const float *f, int n) {
+    auto take = [&](const float *f, int n) {  // running maximum and sum
         float top = m;
+#pragma unroll
         for (int j = 0; j < n; j++) top = fmaxf(top, f[j]);
         if (top > m) {
             s *= __expf(m - top);
             m = top;
         }
         const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
         for (int j = 0; j < n; j++) s += __expf(f[j] - base);
     };
-    int i = t;
-    for (; i + 3 * kSelThreads < vecs; i += 4 * kSelThreads) {
-        uint4 u[4];
+    // the odd ends: up to 7 elements each, the first threads' (with no bound yet: collected where they reach the first one)
+    const int ends = head + max(b - tail, 0);
+    const int end_at = t < head ? a + t : tail + t - head;
+    float end = -INFINITY;
+    if (t < ends) {
+        end = L::get(x[end_at]);
+        take(&end, 1);
+    }
+    const int pieces = (vecs + Q * kSelThreads - 1) / (Q * kSelThreads);
+    float bound = -INFINITY;
+#pragma unroll 1
+    for (int k = 0; k < max(pieces, 1); k++) {
+        const int i0 = k * Q * kSelThreads + t;
+        float f[16];
+        if (i0 + (Q - 1) * kSelThreads < vecs) {
+            uint4 u[Q];
 #pragma unroll
-        for (int k = 0; k < 4; k++) u[k] = ldg_stream_v4(xv + i + k * kSelThreads);
-        float f[4 * V];
+            for (int q = 0; q < Q; q++) u[q] = ldg_stream_v4(xv + i0 + q * kSelThreads);
 #pragma unroll
-        for (int k = 0; k < 4; k++) L::split(u[k], f + k * V);
-        take(f, 4 * V);
-    }
-    for (; i < vecs; i += kSelThreads) {
-        float f[V];
-        L::split(ldg_stream_v4(xv + i), f);
-        take(f, V);
-    }
-    for (int e = a + t; e < a + head; e += kSelThreads) {
-        const float f = L::get(x[e]);
-        take(&f, 1);
-    }
-    for (int e = tail + t; e < b; e += kSelThreads) {
-        const float f = L::get(x[e]);
-        take(&f, 1);
-    }
-    auto visit = [&](auto f) {
-        for (int i = t; i < vecs; i += kSelThreads) {
-            float g[V];
-            L::split(__ldg(xv + i), g);
+            for (int q = 0; q < Q; q++) L::split(u[q], f + q * V);
+        } else {
 #pragma unroll
-            for (int j = 0; j < V; j++) f(g[j], (double)g[j], (long long)(a + head + i * V + j));
+            for (int q = 0; q < Q; q++) {
+                const bool in = i0 + q * kSelThreads < vecs;
+                uint4 u = make_uint4(0, 0, 0, 0);
+                if (in) u = ldg_stream_v4(xv + i0 + q * kSelThreads);
+                L::split(u, f + q * V);
+                if (!in)
+#pragma unroll
+                    for (int j = 0; j < V; j++) f[q * V + j] = -INFINITY;
+            }
         }
-        for (int e = a + t; e < a + head; e += kSelThreads) {
-            const float g = L::get(x[e]);
-            f(g, (double)g, (long long)e);
+        take(f, 16);
+        if ((k & (k - 1)) == 0) bound = best.bound(m, p.picks);
+        if (k == 0 && end >= bound && end > -INFINITY) best.collect(end, end_at);
+        float top = f[0];
+#pragma unroll
+        for (int j = 1; j < 16; j++) top = fmaxf(top, f[j]);
+        if (top >= bound && top > -INFINITY) {
+#pragma unroll
+            for (int j = 0; j < 16; j++)
+                if (f[j] >= bound && f[j] > -INFINITY) best.collect(f[j], a + head + (i0 + j / V * kSelThreads) * V + j % V);
         }
-        for (int e = tail + t; e < b; e += kSelThreads) {
-            const float g = L::get(x[e]);
-            f(g, (double)g, (long long)e);
-        }
-    };
+    }
     // joined over lanes, then warps, in a fixed order
     float M = warp_max(m);
     float S = warp_sum(m == -INFINITY && s == 0.0f ? 0.0f : s * __expf(m - M));
     if ((t & 31) == 0) red_m[t >> 5] = M, red_s[t >> 5] = S;
-    pick_best(visit, (double)m, p.picks, out_v, out_i);
+    best.rank(p.picks, [&](auto f) {
+        if (t < ends) f(end, end_at);
+        for (int i = t; i < vecs; i += kSelThreads) {
+            float g[V];
+            L::split(__ldg(xv + i), g);
+            for (int j = 0; j < V; j++) f(g[j], a + head + i * V + j);
+        }
+    });
     if (t == 0) {
         M = -INFINITY;
         for (int w = 0; w < kSelThreads / 32; w++) M = fmaxf(M, red_m[w]);
@@ -227,67 +259,96 @@ __global__ void __launch_bounds__(kSelThreads) beam_slice_kernel(const Select p)
     }
     const long long at = (row * p.slices + slice) * p.picks;
     for (int k = t; k < p.picks; k += kSelThreads) {
-        p.part_v[at + k] = (float)out_v[k];
-        p.part_i[at + k] = (int)out_i[k];
+        p.part_v[at + k] = best.out_v[k];
+        p.part_i[at + k] = best.out_i[k];
     }
 }
 
 // grid (groups)
-__global__ void __launch_bounds__(kSelThreads) beam_join_kernel(const Select p) {
+__global__ void __launch_bounds__(kSelThreads) beam_join_kernel(const __grid_constant__ Select p) {
+    __shared__ Best<double, long long> best;
     __shared__ double offset[kSelMost];  // score - lse of each beam; NaN: nothing of it is picked
-    __shared__ double out_v[kSelMost];
-    __shared__ long long out_i[kSelMost];
     pdl_trigger();
     pdl_wait();
     const int group = blockIdx.x, t = threadIdx.x, lane = t & 31;
     const long long row0 = (long long)group * p.beams;
+    const int per = p.slices * p.picks, n = p.beams * per;
+    // what the slices found is on its way while lse is computed
+    constexpr int kHeld = 4;
+    __shared__ float held_v[kHeld * kSelThreads];
+    __shared__ int held_i[kHeld * kSelThreads];
+    const bool held = n <= kHeld * kSelThreads;
+    if (held) {
+        for (int i = t; i < n; i += kSelThreads) {
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(held_v + i)), "l"(p.part_v + row0 * per + i) : "memory");
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(held_i + i)), "l"(p.part_i + row0 * per + i) : "memory");
+        }
+    }
+    best.clear(p.picks);
     for (int b = t >> 5; b < p.beams; b += kSelThreads / 32) {
         const bool done = p.done && p.done[row0 + b];
-        float m = -INFINITY;
-        double s = 0.0;
+        float m = -INFINITY, s = 0.0f;
         if (!done) {
             const float2 *ms = p.part_ms + (row0 + b) * p.slices;
-            for (int i = lane; i < p.slices; i += 32) m = fmaxf(m, ms[i].x);
-            m = warp_max(m);
-            for (int i = lane; i < p.slices; i += 32)
-                if (!(ms[i].x == -INFINITY && ms[i].y == 0.0f)) s += (double)ms[i].y * exp((double)ms[i].x - (double)m);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            const float2 x = lane < p.slices ? ms[lane] : make_float2(-INFINITY, 0.0f), y = lane + 32 < p.slices ? ms[lane + 32] : make_float2(-INFINITY, 0.0f);
+            m = warp_max(fmaxf(x.x, y.x));
+            if (!(x.x == -INFINITY && x.y == 0.0f)) s += x.y * expf(x.x - m);
+            if (!(y.x == -INFINITY && y.y == 0.0f)) s += y.y * expf(y.x - m);
+            s = warp_sum(s);
         }
         if (lane == 0) {
-            const double lse = (double)m + log(s);
+            const double lse = (double)m + log((double)s);
             offset[b] = done ? (double)p.score[row0 + b] : lse > -INFINITY && lse < INFINITY ? (double)p.score[row0 + b] - lse : NAN;
         }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
-    const int per = p.slices * p.picks, n = p.beams * per;
-    auto visit = [&](auto f) {
-        for (int i = t; i < n; i += kSelThreads) {
-            const int b = i / per, k = i - b * per;
-            if (p.done && p.done[row0 + b]) {
-                if (k == 0) f(0.0f, offset[b], (long long)b * p.vocab + p.end_token);
-                continue;
-            }
-            const float v = p.part_v[row0 * per + i];
-            const int token = p.part_i[row0 * per + i];
-            if (token >= 0) f(v, offset[b] + (double)v, (long long)b * p.vocab + token);
+    auto value_of = [&](int i, float v, int token, auto f) {  // an index is (beam, token)
+        const int b = i / per, k = i - b * per;
+        if (p.done && p.done[row0 + b]) {
+            if (k == 0) f(offset[b], (long long)b << 32 | p.end_token);
+        } else if (token >= 0) {
+            f(offset[b] + (double)v, (long long)b << 32 | token);
         }
     };
+    auto visit = [&](auto f) {
+#pragma unroll 1
+        for (int i = t; i < n; i += kSelThreads) value_of(i, p.part_v[row0 * per + i], p.part_i[row0 * per + i], f);
+    };
     double top = -INFINITY;
-    visit([&](float, double value, long long) { if (value > top) top = value; });
-    pick_best(visit, top, p.picks, out_v, out_i);
+    auto higher = [&](double value, long long) { if (value > top) top = value; };
+    if (held) {
+#pragma unroll 1
+        for (int k = 0; k < kHeld; k++)
+            if (t + k * kSelThreads < n) value_of(t + k * kSelThreads, held_v[k * kSelThreads + t], held_i[k * kSelThreads + t], higher);
+    } else {
+        visit(higher);
+    }
+    const double bound = best.bound(top, p.picks);
+    if (top >= bound && top > -INFINITY) {
+        auto collect = [&](double value, long long index) { if (value >= bound && value > -INFINITY) best.collect(value, index); };
+        if (held) {
+#pragma unroll 1
+            for (int k = 0; k < kHeld; k++)
+                if (t + k * kSelThreads < n) value_of(t + k * kSelThreads, held_v[k * kSelThreads + t], held_i[k * kSelThreads + t], collect);
+        } else {
+            visit(collect);
+        }
+    }
+    best.rank(p.picks, visit);
     for (int k = t; k < p.picks; k += kSelThreads) {
-        const long long i = out_i[k], at = (long long)group * p.picks + k;
-        p.score_out[at] = (float)out_v[k];
-        p.parent_out[at] = i < 0 ? -1 : (int)(i / p.vocab);
-        p.token_out[at] = i < 0 ? -1 : (int)(i % p.vocab);
+        const long long i = best.out_i[k], at = (long long)group * p.picks + k;
+        p.score_out[at] = (float)best.out_v[k];
+        p.parent_out[at] = i < 0 ? -1 : (int)(i >> 32);
+        p.token_out[at] = i < 0 ? -1 : (int)i;
     }
 }
 
-// Slices of a row: about eight blocks of all rows for every SM, none below kSelLeast elements.
+// Slices of a row: as many as the GPU holds blocks of all rows at a time (a second wave of a few would cost as much as a full one), none below kSelLeast
+// elements.
 int select_slices(const Device *dev, int groups, int beams, int vocab) {
     const long long rows = (long long)groups * beams;
-    const long long want = (8ll * dev->sm_count + rows - 1) / rows, most = (vocab + kSelLeast - 1) / kSelLeast;
+    const long long want = (long long)kSelResident * dev->sm_count / rows, most = (vocab + kSelLeast - 1) / kSelLeast;
     return (int)std::max(1ll, std::min(std::min(want, most), 64ll));
 }
 size_t select_bytes(long long rows, int slices, int picks) { return (size_t)rows * slices * (8 + 8 * (size_t)picks) + 16; }

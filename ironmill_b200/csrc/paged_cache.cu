@@ -85,15 +85,17 @@ __device__ __forceinline__ void angles4(const void *table, long long at, float *
 // cosines and sines. The first heads of a thread are requested before the lookups of the token's place (its sequence, the sequence's length,
 // its page): one latency for the loads, one chain for the place, hidden by the other blocks of the SM.
 // FORM: 0 nothing is rotated; 1 halves, a column's partner a whole number of lanes away; 2 neighbours; 3 halves, partners anywhere.
-constexpr int kAppendThreads = 256;
-constexpr int kAppendHeads = 4;  // heads that a thread holds at a time
+// Blocks of 64 threads where there are many (8 x 1900 tokens of 48 heads: 59 us in blocks of 256, 51 of 128, 49 of 64), of 256 where a block more or less
+// costs nothing (32 tokens: 3.3 us, 6.4 in blocks of 64).
+constexpr int kAppendThreads = 256, kAppendSmall = 64;
+constexpr int kAppendHeads = 3;  // heads that a thread holds at a time
 
 template <bool BF16, int FORM, bool F32>
-__global__ void __launch_bounds__(kAppendThreads, FORM == 3 ? 2 : 4) paged_append_kernel(const __grid_constant__ Append a, int lanes) {
+__global__ void __launch_bounds__(kAppendThreads, FORM == 3 ? 2 : 5) paged_append_kernel(const __grid_constant__ Append a, int lanes) {
     pdl_trigger();
     pdl_wait();
     const int token = blockIdx.x, tid = threadIdx.x;
-    const int c = tid & (lanes - 1), first = tid / lanes, per = kAppendThreads / lanes;
+    const int c = tid & (lanes - 1), first = tid / lanes, per = blockDim.x / lanes;
     const int hd = a.kv.hd, heads = a.nh + 2 * a.kv.nkv, d0 = 8 * c, half = a.rot / 2;
     const bool mine = d0 < hd;
     bool placed = false;
@@ -375,7 +377,7 @@ IM_EXPORT int im_cuda_paged_append(im_device *dev, const im_paged_kv *kv, int la
     default: kern = IM_FORM(3); break;
     }
 #undef IM_FORM
-    IM_CUDA_CHECK(launch_k(kern, dim3((unsigned)num_tokens), dim3(kAppendThreads), 0, as_stream(stream), a, lanes));
+    IM_CUDA_CHECK(launch_k(kern, dim3((unsigned)num_tokens), dim3(num_tokens > 4 * dev->sm_count ? kAppendSmall : kAppendThreads), 0, as_stream(stream), a, lanes));
     return IM_OK;
     IM_GUARD_END
 }

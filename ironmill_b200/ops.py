@@ -26,6 +26,8 @@ class Device:
         self.handle = C.c_void_p()
         check(lib().im_cuda_device_open(C.c_int(ordinal), C.byref(self.handle)))
         self.ordinal = ordinal
+        self.torch_device = torch.device("cuda", ordinal)
+        self.select_bytes = {}  # scratch of beam_select, by sizes
 
     @property
     def name(self) -> str:
@@ -560,8 +562,11 @@ def paged_reorder(kv: PagedKV, parents, group: int, table_out=None, lengths_out=
 # ---------------------------------------------------------------- beam search
 def beam_select_scratch(dev: Device, groups: int, beams: int, vocab: int, picks: int) -> torch.Tensor:
     """Scratch for beam_select calls of these sizes; calls that may overlap need one each."""
-    nbytes = int(lib().im_cuda_beam_select_scratch_bytes(dev.handle, groups, beams, vocab, picks))
-    return torch.empty(max(nbytes, 16), dtype=torch.uint8, device=f"cuda:{dev.ordinal}")
+    key = (groups, beams, vocab, picks)
+    nbytes = dev.select_bytes.get(key)
+    if nbytes is None:
+        nbytes = dev.select_bytes[key] = max(int(lib().im_cuda_beam_select_scratch_bytes(dev.handle, *key)), 16)
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev.torch_device)
 
 
 def beam_select(dev: Device, logits, scores, picks: int, done=None, end_token=-1, scratch=None):
@@ -581,7 +586,8 @@ def beam_select(dev: Device, logits, scores, picks: int, done=None, end_token=-1
     else:
         assert scratch.dtype is torch.uint8 and scratch.get_device() == on and scratch.is_contiguous()
     score = scores.new_empty((groups, picks))
-    parent, token = score.new_empty((2, groups, picks), dtype=torch.int32).unbind(0)
+    parent = torch.empty_like(score, dtype=torch.int32)
+    token = torch.empty_like(parent)
     _launch(on, lib().im_cuda_beam_select, dev.handle, logits.data_ptr(), _DTYPES[logits.dtype], (sb if beams > 1 else sg) if groups * beams > 1 else 0, groups, beams, vocab,
             scores.data_ptr(), dp, end_token, picks, score.data_ptr(), parent.data_ptr(), token.data_ptr(), scratch.data_ptr(), scratch.numel())
     return score, parent, token
