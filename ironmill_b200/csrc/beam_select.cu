@@ -4,11 +4,12 @@
 // The logits are read once, from HBM; what bounds the pass is that read. Within a beam the order of the values is the order of its
 // logits, so nothing needs lse before the end: a block walks a slice of a row once for both the running maximum and sum of
 // exponentials and the slice's best `picks` logits, and a block per group joins the slices.
-//   best of a slice   the threads form at least `picks` sets; each thread knows the maximum of what it has met, and the lowest of the sets' maxima
-//                     is a bound that at least `picks` elements reach. What reaches it is collected as it comes; the bound is taken after the
-//                     first, second, fourth, eighth ... piece of the slice, so that few elements that do not belong to the best are collected (about
-//                     picks * ln(picks) for each doubling). A collected element's rank is the number of better ones. Where the collection overflows (ties,
-//                     rising rows) the elements are picked one after the other from memory instead.
+//   best of a slice   each thread knows the maximum of what it has met; the picks-th largest of the maxima of 64 sets of threads is a bound that at
+//                     least `picks` elements reach. It is taken after the
+//                     first, second, fourth, eighth ... piece of the slice and after the last; few elements that do not belong to the best reach it. A
+//                     thread only notes which sixteen elements of a piece reach the bound; those that reach the last one are read again and collected.
+//                     A collected element's rank is the number of better ones. Where a list overflows (ties, rising rows) the elements are picked one
+//                     after the other from memory instead.
 //   joining           the same with the slices' picks as elements and 64-bit values.
 // Sums are f32 per thread over its elements with one running maximum, joined in a fixed order: a run repeats bit by bit, and equal rows
 // get equal sums.
@@ -76,6 +77,13 @@ struct Logit<IM_DTYPE_BF16> : Logit16<true> {};
 __device__ __forceinline__ bool before(double a, long long ia, double b, long long ib) { return a > b || (a == b && ia < ib); }
 __device__ __forceinline__ bool before(float a, int ia, float b, int ib) { return a > b || (a == b && ia < ib); }
 
+// exp(x), zero where it would be denormal
+__device__ __forceinline__ float exp_of(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+    return y;
+}
+
 // What reaches the bound, and the best of it.
 template <typename V, typename I>
 struct Best {
@@ -83,35 +91,46 @@ struct Best {
     I buf_i[kSelBuf];
     V out_v[kSelMost];
     I out_i[kSelMost];
-    V tops[kSelThreads];
+    V tops[kSelThreads], low;
     int count;
 
     __device__ __forceinline__ void clear(int picks) {  // no synchronisation: the first bound() has one
         if (threadIdx.x == 0) count = 0;
         for (int i = threadIdx.x; i < picks; i += kSelThreads) out_v[i] = -INFINITY, out_i[i] = -1;
     }
-    // The lowest of the maxima of 8, 16, 32 or 64 >= picks sets of threads; top: this thread's maximum so far. A set has every so-many-th thread, so that
-    // none is without elements where the first threads have some.
+    // The picks-th largest of the maxima of 64 sets of threads; top: this thread's maximum so far. A set has every 64th thread, so that none is without
+    // elements where the first threads have some. (Of random elements ln 2 a set reach the bound for 32 picks, 1 / 4 for 16.)
     __device__ __forceinline__ V bound(V top, int picks) {
         __syncthreads();
         tops[threadIdx.x] = top;
         __syncthreads();
-        const int lane = threadIdx.x & 31;
-        V a = tops[lane], b = tops[32 + lane];
+        if (threadIdx.x < 32) {
+            V a = tops[threadIdx.x], b = tops[32 + threadIdx.x];
 #pragma unroll
-        for (int w = 2; w < kSelThreads / 32; w += 2) {
-            const V x = tops[32 * w + lane], y = tops[32 * w + 32 + lane];
-            a = a > x ? a : x;
-            b = b > y ? b : y;
-        }
-        V v = picks > 32 ? (a < b ? a : b) : a > b ? a : b;
-        const int sets = picks <= 8 ? 8 : picks <= 16 ? 16 : 32;
+            for (int w = 2; w < kSelThreads / 32; w += 2) {
+                const V x = tops[32 * w + threadIdx.x], y = tops[32 * w + 32 + threadIdx.x];
+                a = a > x ? a : x;
+                b = b > y ? b : y;
+            }
+            int above_a = 0, above_b = 0;
+#pragma unroll 8
+            for (int j = 0; j < 32; j++) {
+                const V x = __shfl_sync(0xffffffffu, a, j), y = __shfl_sync(0xffffffffu, b, j);
+                above_a += (x > a) + (y > a);
+                above_b += (x > b) + (y > b);
+            }
+            V v = INFINITY;  // the lowest of those with fewer than `picks` above
+            if (above_a < picks) v = a;
+            if (above_b < picks) v = v < b ? v : b;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const V x = __shfl_xor_sync(0xffffffffu, v, o);
-            v = o >= sets ? (v > x ? v : x) : v < x ? v : x;
+            for (int o = 16; o > 0; o >>= 1) {
+                const V x = __shfl_xor_sync(0xffffffffu, v, o);
+                v = v < x ? v : x;
+            }
+            if (threadIdx.x == 0) low = v;
         }
-        return v;
+        __syncthreads();
+        return low;
     }
     __device__ __forceinline__ void collect(V v, I i) {
         const int at = atomicAdd(&count, 1);
@@ -169,6 +188,8 @@ __global__ void __launch_bounds__(kSelThreads, kSelResident) beam_slice_kernel(c
     constexpr int V = L::kVec, Q = 16 / V;  // requests of a piece: 16 elements of each thread
     __shared__ Best<float, int> best;
     __shared__ float red_m[kSelThreads / 32], red_s[kSelThreads / 32];
+    __shared__ float met_v[kSelBuf];  // sixteen elements of a thread that reach the bound: their maximum, and which
+    __shared__ int met_i[kSelBuf], kept[kSelBuf], met, keep;
     pdl_trigger();
     pdl_wait();
     const int slice = blockIdx.x, t = threadIdx.x;
@@ -181,18 +202,22 @@ __global__ void __launch_bounds__(kSelThreads, kSelResident) beam_slice_kernel(c
     const int vecs = max(b - a - head, 0) / V, tail = a + head + vecs * V;
     const uint4 *xv = reinterpret_cast<const uint4 *>(x + a + head);
     best.clear(p.picks);
+    if (t == 0) met = keep = 0;
     float m = -INFINITY, s = 0.0f;
-    auto take = [&](const float *f, int n) {  // running maximum and sum
-        float top = m;
-#pragma unroll
-        for (int j = 0; j < n; j++) top = fmaxf(top, f[j]);
+    // running maximum and sum; (x - m) first: it is exact where it matters, a product with log2(e) is not
+    auto take = [&](const float *f, int n, float top) {
         if (top > m) {
-            s *= __expf(m - top);
+            s *= exp_of(m - top);
             m = top;
         }
         const float base = m == -INFINITY ? 0.0f : m;
+        float a = 0.0f, b = 0.0f;
 #pragma unroll
-        for (int j = 0; j < n; j++) s += __expf(f[j] - base);
+        for (int j = 0; j < n; j += 2) {
+            a += exp_of(f[j] - base);
+            if (j + 1 < n) b += exp_of(f[j + 1] - base);
+        }
+        s += a + b;
     };
     // the odd ends: up to 7 elements each, the first threads' (with no bound yet: collected where they reach the first one)
     const int ends = head + max(b - tail, 0);
@@ -200,7 +225,7 @@ __global__ void __launch_bounds__(kSelThreads, kSelResident) beam_slice_kernel(c
     float end = -INFINITY;
     if (t < ends) {
         end = L::get(x[end_at]);
-        take(&end, 1);
+        take(&end, 1, end);
     }
     const int pieces = (vecs + Q * kSelThreads - 1) / (Q * kSelThreads);
     float bound = -INFINITY;
@@ -226,21 +251,37 @@ __global__ void __launch_bounds__(kSelThreads, kSelResident) beam_slice_kernel(c
                     for (int j = 0; j < V; j++) f[q * V + j] = -INFINITY;
             }
         }
-        take(f, 16);
+        float top4[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) top4[j] = fmaxf(fmaxf(f[4 * j], f[4 * j + 1]), fmaxf(f[4 * j + 2], f[4 * j + 3]));
+        const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+        take(f, 16, top);
         if ((k & (k - 1)) == 0) bound = best.bound(m, p.picks);
-        if (k == 0 && end >= bound && end > -INFINITY) best.collect(end, end_at);
-        float top = f[0];
-#pragma unroll
-        for (int j = 1; j < 16; j++) top = fmaxf(top, f[j]);
         if (top >= bound && top > -INFINITY) {
-#pragma unroll
-            for (int j = 0; j < 16; j++)
-                if (f[j] >= bound && f[j] > -INFINITY) best.collect(f[j], a + head + (i0 + j / V * kSelThreads) * V + j % V);
+            const int at = atomicAdd(&met, 1);
+            if (at < kSelBuf) met_v[at] = top, met_i[at] = i0;
         }
+    }
+    if (pieces > 1) bound = best.bound(m, p.picks);
+    else __syncthreads();
+    const int n = met;
+    if (n <= kSelBuf) {
+        for (int i = t; i < n; i += kSelThreads)
+            if (met_v[i] >= bound) kept[atomicAdd(&keep, 1)] = met_i[i];
+        __syncthreads();
+        for (int i = t; i < keep * 16; i += kSelThreads) {
+            const int v = kept[i >> 4] + (i & 15) / V * kSelThreads, e = a + head + v * V + (i & 15) % V;
+            if (v >= vecs) continue;
+            const float f = L::get(x[e]);
+            if (f >= bound && f > -INFINITY) best.collect(f, e);
+        }
+        if (end >= bound && end > -INFINITY) best.collect(end, end_at);
+    } else if (t == 0) {
+        best.count = INT_MAX;  // too many: one after the other
     }
     // joined over lanes, then warps, in a fixed order
     float M = warp_max(m);
-    float S = warp_sum(m == -INFINITY && s == 0.0f ? 0.0f : s * __expf(m - M));
+    float S = warp_sum(m == -INFINITY && s == 0.0f ? 0.0f : s * exp_of(m - M));
     if ((t & 31) == 0) red_m[t >> 5] = M, red_s[t >> 5] = S;
     best.rank(p.picks, [&](auto f) {
         if (t < ends) f(end, end_at);
@@ -254,7 +295,7 @@ __global__ void __launch_bounds__(kSelThreads, kSelResident) beam_slice_kernel(c
         M = -INFINITY;
         for (int w = 0; w < kSelThreads / 32; w++) M = fmaxf(M, red_m[w]);
         S = 0.0f;
-        for (int w = 0; w < kSelThreads / 32; w++) S += red_m[w] == -INFINITY && red_s[w] == 0.0f ? 0.0f : red_s[w] * __expf(red_m[w] - M);
+        for (int w = 0; w < kSelThreads / 32; w++) S += red_m[w] == -INFINITY && red_s[w] == 0.0f ? 0.0f : red_s[w] * exp_of(red_m[w] - M);
         p.part_ms[row * p.slices + slice] = make_float2(M, S);
     }
     const long long at = (row * p.slices + slice) * p.picks;
