@@ -6,7 +6,7 @@
 // exponentials and the slice's best `picks` logits, and a block per group joins the slices.
 //   best of a slice   each thread knows the maximum of what it has met; the picks-th largest of the maxima of 64 sets of threads is a bound that at
 //                     least `picks` elements reach. It is taken after the
-//                     first, second, fourth, eighth ... piece of the slice and after the last; few elements that do not belong to the best reach it. A
+//                     first, third, ninth and every 32nd piece of the slice and after the last; few elements that do not belong to the best reach it. A
 //                     thread only notes which sixteen elements of a piece reach the bound; those that reach the last one are read again and collected.
 //                     A collected element's rank is the number of better ones. Where a list overflows (ties, rising rows) the elements are picked one
 //                     after the other from memory instead.
@@ -25,7 +25,7 @@ namespace im {
 namespace {
 
 constexpr int kSelThreads = 256, kSelMost = 64, kSelBuf = 1024;
-constexpr int kSelResident = 6;  // blocks of an SM
+constexpr int kSelResident = 7;  // blocks of an SM
 constexpr int kSelLeast = 2048;  // elements of a slice: one request of 16-bit logits for every thread
 
 struct Select {
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kSelThreads, kSelResident) beam_slice_kernel(c
         for (int j = 0; j < 4; j++) top4[j] = fmaxf(fmaxf(f[4 * j], f[4 * j + 1]), fmaxf(f[4 * j + 2], f[4 * j + 3]));
         const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
         take(f, 16, top);
-        if ((k & (k - 1)) == 0) bound = best.bound(m, p.picks);
+        if (k == 0 || k == 2 || k == 8 || (k & 31) == 31) bound = best.bound(m, p.picks);
         if (top >= bound && top > -INFINITY) {
             const int at = atomicAdd(&met, 1);
             if (at < kSelBuf) met_v[at] = top, met_i[at] = i0;
