@@ -337,8 +337,9 @@ int im_cuda_paged_append(im_device *dev, const im_paged_kv *kv, int layer, const
  * and accumulation, softmax weights as a sum of two 16-bit terms, one rounding of the output.  q, out: as q in paged_append.
  * max_new: no sequence has more new tokens (further ones are left as they are).  max_len: no sequence has more rows, the new ones
  * included (0: the table's width); a smaller value costs time, not results.  scratch_dev: 16-byte aligned,
- * im_cuda_paged_attention_scratch_bytes for the same kv, heads and max_new; calls whose kernels may overlap need one each. */
-size_t im_cuda_paged_attention_scratch_bytes(const im_device *dev, const im_paged_kv *kv, int num_heads, int max_new);
+ * im_cuda_paged_attention_scratch_bytes for the same kv, heads, max_new and max_len (short contexts need none; those of a larger
+ * max_len are enough for a smaller one); calls whose kernels may overlap need one each. */
+size_t im_cuda_paged_attention_scratch_bytes(const im_device *dev, const im_paged_kv *kv, int num_heads, int max_new, int max_len);
 int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int layer, const void *q_dev, int64_t q_stride, void *out_dev, int64_t out_stride,
                             int num_heads, const int *token_start_dev, int num_tokens, int max_new, const uint64_t *mask_dev, int mask_words,
                             float scale, int max_len, void *scratch_dev, size_t scratch_bytes, void *stream);

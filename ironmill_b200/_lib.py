@@ -44,7 +44,7 @@ _P, _I, _L, _F, _Z = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
 # Calls between two forwards are short: with their argument types known, plain numbers and addresses are passed.
 _ARGTYPES = {
     "im_cuda_paged_append": (_P, _P, _I, _P, _L, _P, _L, _P, _I, _P, _L, _P, _L, _I, _P, _P, _I, _I, _I, _I, _P, _P),
-    "im_cuda_paged_attention_scratch_bytes": (_P, _P, _I, _I),
+    "im_cuda_paged_attention_scratch_bytes": (_P, _P, _I, _I, _I),
     "im_cuda_paged_attention": (_P, _P, _I, _P, _L, _P, _L, _I, _P, _I, _I, _P, _I, _F, _I, _P, _Z, _P),
     "im_cuda_paged_keep": (_P, _P, _P, _I, _P, _P, _P),
     "im_cuda_paged_reorder": (_P, _P, _P, _I, _P, _L, _P, _P),

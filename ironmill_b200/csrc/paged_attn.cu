@@ -55,7 +55,38 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool there) 
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 
-template <bool BF16, int HD, int MT>
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t of_rank(const void *mine, uint32_t rank) {  // the same place in another CTA of the cluster
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(mine)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float4 remote4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 remote2(uint32_t at) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+    return v;
+}
+
+// CL: instead of shares of the list of all tiles, a cluster of CTAs per item, each with an equal run of its tiles; they join what they have
+// through each other's shared memory, in the same launch and without scratch.
+template <bool BF16, int HD, int MT, bool CL>
 __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kernel(const __grid_constant__ PagedAttn p, int units) {
     using S = PaShape<HD, MT>;
     constexpr int R = S::kRows, KS = HD / 16, NT = HD / 8, CH = HD / 8;  // k steps, 8-column tiles, 16-byte pieces of a row
@@ -68,11 +99,24 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
     float *merge = reinterpret_cast<float *>(qsm + S::kQ);
     float2 *ml = reinterpret_cast<float2 *>(reinterpret_cast<unsigned char *>(merge) + S::kMerge);  // [warps, R]
     __shared__ unsigned bad_rows[2];  // rows of an item whose sums are not finite, every other item's
+    __shared__ float2 joint[CL ? R : 1];  // maximum and sum of this CTA's part of each row
     if (tid < 2) bad_rows[tid] = 0;
     pdl_trigger();
     pdl_wait();
-    const Share share = find_share<R, kPaTile, kPaThreads>(p, units, sums);
-    if (share.from >= share.to) return;
+    static_assert(!CL || MT == 1, "the join reads all columns of a row");
+    Share share;
+    if constexpr (CL) {
+        const int C = (int)cluster_size(), item = blockIdx.x / C, rank = (int)cluster_rank();
+        share.unit = item / p.kv.nkv;
+        share.head = item - share.unit * p.kv.nkv;
+        const int n = unit_tiles<kPaTile>(paged_unit<R>(p, share.unit));
+        if (n == 0) return;  // all of the cluster
+        share.from = share.tile = (int)((long long)n * rank / C);
+        share.to = (long long)n * (rank + 1) / C;
+    } else {
+        share = find_share<R, kPaTile, kPaThreads>(p, units, sums);
+        if (share.from >= share.to) return;
+    }
     const int count = (int)(share.to - share.from);
 
     // ---- the copies' cursor: one slice ahead of the copies, so that a page number is there when it is needed
@@ -305,7 +349,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
             }
         __syncthreads();
         if (tid == 0) bad_rows[!odd_item] = 0;  // every thread has looked at the last item's
-        const bool whole = t0 == 0 && t1 == tiles;
+        const bool whole = !CL && t0 == 0 && t1 == tiles;
         const size_t part = ((size_t)blockIdx.x * 2 + (first_item ? 0 : 1)) * R;
         float f[MT][2];
 #pragma unroll
@@ -332,7 +376,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
         constexpr int MC = S::kMergeCols;
 #pragma unroll
         for (int c0 = 0; c0 < HD; c0 += MC) {
-#pragma unroll
+#pragma unroll 1
             for (int w = 0; w < kPaWarps; w++) {
                 if (warp == w) {
 #pragma unroll
@@ -370,14 +414,17 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
                     *reinterpret_cast<uint4 *>(p.out + (u.tok0 + t) * p.os + (long long)(head * p.group + g) * HD + c0 + c) =
                         make_uint4(pack16<BF16>(v[0] * inv, v[1] * inv), pack16<BF16>(v[2] * inv, v[3] * inv), pack16<BF16>(v[4] * inv, v[5] * inv),
                                    pack16<BF16>(v[6] * inv, v[7] * inv));
-                } else {
+                } else if (!CL) {
                     float4 *dst = reinterpret_cast<float4 *>(p.part_o + (part + r) * HD + c0 + c);
                     dst[0] = make_float4(v[0], v[1], v[2], v[3]);
                     dst[1] = make_float4(v[4], v[5], v[6], v[7]);
                 }
             }
             if (!whole && c0 == 0)
-                for (int r = tid; r < u.rows; r += kPaThreads) p.part_ml[part + r] = row_ml(r);
+                for (int r = tid; r < u.rows; r += kPaThreads) {
+                    if (CL) joint[r] = row_ml(r);
+                    else p.part_ml[part + r] = row_ml(r);
+                }
             __syncthreads();
         }
         if (const unsigned bad = bad_rows[odd_item]) {
@@ -389,9 +436,10 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
                 const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
                 for (int i = 0; i < HD / 32; i++) {
                     if (whole) p.out[(u.tok0 + t) * p.os + (long long)(head * p.group + g) * HD + lane + 32 * i] = (uint16_t)pack16<BF16>(x[i] * inv, 0.0f);
+                    else if (CL) merge[r * MC + ((lane + 32 * i) ^ ((r & 3) << 3))] = x[i];
                     else p.part_o[(part + r) * HD + lane + 32 * i] = x[i];
                 }
-                if (!whole && lane == 0) p.part_ml[part + r] = make_float2(M, L);
+                if (!whole && lane == 0) (CL ? joint[r] : p.part_ml[part + r]) = make_float2(M, L);
             }
             __syncthreads();
         }
@@ -406,6 +454,35 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
         }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if constexpr (CL) {
+        const int C = (int)cluster_size(), rank = (int)cluster_rank();
+        if (count == 0 && tid < R) joint[tid] = make_float2(-INFINITY, 0.0f);
+        cluster_sync();
+        const PagedUnit u = paged_unit<R>(p, share.unit);
+        for (int i = rank * kPaThreads + tid; i < u.rows * CH; i += C * kPaThreads) {
+            const int r = i / CH, c = i % CH * 8;
+            float M = -INFINITY, L = 0.0f, o[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) o[j] = 0.0f;
+            for (int k = 0; k < C; k++) M = fmaxf(M, remote2(of_rank(joint + r, k)).x);
+#pragma unroll 1
+            for (int k = 0; k < C; k++) {
+                const float2 x = remote2(of_rank(joint + r, k));
+                if (x.x == -INFINITY && x.y == 0.0f) continue;  // nothing seen in this part
+                const uint32_t at = of_rank(merge + r * HD + (c ^ ((r & 3) << 3)), k);
+                const float4 a = remote4(at), b = remote4(at + 16);
+                const float f = ex2(x.x - M);
+                L += x.y * f;
+                o[0] += a.x * f; o[1] += a.y * f; o[2] += a.z * f; o[3] += a.w * f;
+                o[4] += b.x * f; o[5] += b.y * f; o[6] += b.z * f; o[7] += b.w * f;
+            }
+            const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
+            const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
+            *reinterpret_cast<uint4 *>(p.out + (u.tok0 + t) * p.os + (long long)(share.head * p.group + g) * HD + c) =
+                make_uint4(pack16<BF16>(o[0] * inv, o[1] * inv), pack16<BF16>(o[2] * inv, o[3] * inv), pack16<BF16>(o[4] * inv, o[5] * inv), pack16<BF16>(o[6] * inv, o[7] * inv));
+        }
+        cluster_sync();  // nobody leaves while another reads what it has
+    }
 }
 
 // Items that a cut divides: a warp per row, HD / 32 columns a lane. The parts of an item lie with the CTAs that its tiles fall to; a lane per part
@@ -462,9 +539,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __gri
 
 struct AttnPlan {
     int rows, tile, row_tiles, units, ctas;
+    int cluster;  // CTAs per item that join in the launch; 0: shares
     size_t bytes;
 };
-AttnPlan attn_plan(const Device *dev, int nseq, int nkv, int hd, int group, int max_new) {
+constexpr int kClusterMost = 8, kClusterTiles = 8;
+AttnPlan attn_plan(const Device *dev, int nseq, int nkv, int hd, int group, int max_new, int max_len) {
     AttnPlan a;
     // up to 16 rows of a KV head: one m16 tile; more: two, so that half the row tiles read the cache again (heads of 256: one, registers)
     const int tc = paged_tc_rows(hd, (long long)group * max_new);
@@ -473,6 +552,14 @@ AttnPlan attn_plan(const Device *dev, int nseq, int nkv, int hd, int group, int 
     a.row_tiles = (int)(((long long)group * max_new + a.rows - 1) / a.rows);
     a.units = nseq * a.row_tiles;
     a.ctas = dev->sm_count * (tc || hd == 256 ? 1 : 2);
+    // Contexts that a few CTAs per item read in a few tiles each: a cluster per item, one launch
+    const long long items = (long long)a.units * nkv, tiles = (max_len + (long long)kPaTile - 1) / kPaTile;
+    a.cluster = (int)std::max(1ll, std::min({(long long)a.ctas / std::max(items, 1ll), tiles, (long long)kClusterMost}));
+    if (a.rows != 16 || tiles > (long long)kClusterTiles * a.cluster) a.cluster = 0;
+    if (a.cluster) {
+        a.bytes = 0;
+        return a;
+    }
     const size_t slots = (size_t)a.ctas * 2 * a.rows;
     a.bytes = slots * hd * 4 + slots * 8 + ((size_t)a.units + 1) * 8;
     return a;
@@ -487,13 +574,36 @@ int join_launch(const PagedAttn &p, int units, cudaStream_t st) {
 }
 
 template <bool BF16, int HD, int MT>
-int attn_launch(const Device *dev, const PagedAttn &p, int units, cudaStream_t st) {
+int attn_launch(const Device *dev, const PagedAttn &p, int units, int cluster, cudaStream_t st) {
     using S = PaShape<HD, MT>;
     static DeviceOnce once;
-    if (once.first(dev->ordinal)) IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, MT>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
-    IM_CUDA_CHECK(launch_k(paged_attn_kernel<BF16, HD, MT>, dim3(p.ctas), dim3(kPaThreads), (size_t)S::kSmem, st, p, units));
+    if (once.first(dev->ordinal)) {
+        IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, MT, false>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+        if (MT == 1) IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, 1, true>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+    }
+    if (MT == 1 && cluster) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)(units * p.kv.nkv * cluster));
+        cfg.blockDim = dim3(kPaThreads);
+        cfg.dynamicSmemBytes = S::kSmem;
+        cfg.stream = st;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = cluster;
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 2;
+        IM_CUDA_CHECK(cudaLaunchKernelEx(&cfg, paged_attn_kernel<BF16, HD, 1, true>, p, units));
+        return IM_OK;
+    }
+    IM_CUDA_CHECK(launch_k(paged_attn_kernel<BF16, HD, MT, false>, dim3(p.ctas), dim3(kPaThreads), (size_t)S::kSmem, st, p, units));
     return join_launch<BF16, S::kRows, HD>(p, units, st);
 }
+
+// Rows that no sequence passes.
+int attn_length(const PagedView &v, int max_len) { return max_len > 0 && max_len < v.rows ? max_len : v.rows; }
 
 int attn_check(const im_paged_kv *kv, int num_heads, int max_new) {
     IM_REQUIRE(kv->head_dim == 64 || kv->head_dim == 128 || kv->head_dim == 256, "paged attention is built for heads of 64, 128 and 256 (got %d)", kv->head_dim);
@@ -507,10 +617,11 @@ int attn_check(const im_paged_kv *kv, int num_heads, int max_new) {
 }  // namespace
 }  // namespace im
 
-IM_EXPORT size_t im_cuda_paged_attention_scratch_bytes(const im_device *dev, const im_paged_kv *kv, int num_heads, int max_new) {
+IM_EXPORT size_t im_cuda_paged_attention_scratch_bytes(const im_device *dev, const im_paged_kv *kv, int num_heads, int max_new, int max_len) {
     im::PagedView v;
     if (!dev || im::paged_view(kv, 0, &v) != IM_OK || im::attn_check(kv, num_heads, max_new) != IM_OK) return 0;
-    return im::attn_plan(dev, v.nseq, v.nkv, v.hd, num_heads / v.nkv, max_new).bytes;
+    if (max_len < 0) return 0;
+    return im::attn_plan(dev, v.nseq, v.nkv, v.hd, num_heads / v.nkv, max_new, im::attn_length(v, max_len)).bytes;
 }
 
 IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int layer, const void *q_dev, int64_t q_stride, void *out_dev, int64_t out_stride,
@@ -533,8 +644,9 @@ IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int
     IM_REQUIRE(scale == scale && scale - scale == 0.0f, "scale is not finite");
     rc = paged_device(dev);
     if (rc != IM_OK) return rc;
-    const AttnPlan plan = attn_plan(dev, p.kv.nseq, p.kv.nkv, p.kv.hd, num_heads / kv->num_kv_heads, max_new);
-    IM_REQUIRE(scratch_dev && aligned16(scratch_dev) && scratch_bytes >= plan.bytes, "paged attention needs %zu bytes of 16-byte aligned scratch (got %zu)", plan.bytes,
+    max_len = attn_length(p.kv, max_len);
+    const AttnPlan plan = attn_plan(dev, p.kv.nseq, p.kv.nkv, p.kv.hd, num_heads / kv->num_kv_heads, max_new, max_len);
+    IM_REQUIRE(plan.bytes == 0 || (scratch_dev && aligned16(scratch_dev) && scratch_bytes >= plan.bytes), "paged attention needs %zu bytes of 16-byte aligned scratch (got %zu)", plan.bytes,
                scratch_dev ? scratch_bytes : (size_t)0);
     const int64_t at = layer * (int64_t)p.kv.layer_stride;
     p.kc = static_cast<const uint16_t *>(kv->k_dev) + at;
@@ -548,10 +660,9 @@ IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int
     p.scale2 = scale * 1.4426950408889634f;
     p.row_tiles = plan.row_tiles;
     p.ctas = plan.ctas;
-    if (max_len > 0) {  // no more CTAs than tiles
-        const long long tiles = (long long)plan.units * p.kv.nkv * ((max_len + (long long)plan.tile - 1) / plan.tile);
-        p.ctas = (int)std::max(1ll, std::min<long long>(p.ctas, tiles));
-    }
+    // no more CTAs than tiles
+    const long long tiles = (long long)plan.units * p.kv.nkv * ((max_len + (long long)plan.tile - 1) / plan.tile);
+    p.ctas = (int)std::max(1ll, std::min<long long>(p.ctas, tiles));
     const size_t slots = (size_t)plan.ctas * 2 * plan.rows;
     p.part_o = static_cast<float *>(scratch_dev);
     p.part_ml = reinterpret_cast<float2 *>(p.part_o + slots * p.kv.hd);
@@ -559,7 +670,7 @@ IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int
     const cudaStream_t st = as_stream(stream);
     const bool bf16 = kv->dtype == IM_DTYPE_BF16;
     if (plan.rows >= 128) return paged_tc_launch(dev, p, bf16, plan.rows, plan.units, st);
-#define IM_RUN(HD, MT) (bf16 ? attn_launch<true, HD, MT>(dev, p, plan.units, st) : attn_launch<false, HD, MT>(dev, p, plan.units, st))
+#define IM_RUN(HD, MT) (bf16 ? attn_launch<true, HD, MT>(dev, p, plan.units, plan.cluster, st) : attn_launch<false, HD, MT>(dev, p, plan.units, plan.cluster, st))
     switch (kv->head_dim) {
     case 64: return plan.rows == 16 ? IM_RUN(64, 1) : IM_RUN(64, 2);
     case 128: return plan.rows == 16 ? IM_RUN(128, 1) : IM_RUN(128, 2);

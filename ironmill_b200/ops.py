@@ -499,12 +499,19 @@ def paged_append(kv: PagedKV, layer: int, k, v, token_start, q=None, cos=None, s
     return q_out
 
 
-def paged_attention_scratch(kv: PagedKV, heads: int, max_new: int) -> torch.Tensor:
-    """Scratch for paged_attention calls of this cache with so many heads and new tokens; calls that may overlap need one each."""
-    nbytes = kv.scratch_bytes.get((heads, max_new))
+def _attention_bytes(kv: PagedKV, heads: int, max_new: int, max_len: int) -> int:
+    key = (heads, max_new, max_len.bit_length())  # what is enough for the next power of two
+    nbytes = kv.scratch_bytes.get(key)
     if nbytes is None:
-        nbytes = kv.scratch_bytes[heads, max_new] = max(int(lib().im_cuda_paged_attention_scratch_bytes(kv.dev.handle, kv.ref, heads, max_new)), 16)
-    return torch.empty(nbytes, dtype=torch.uint8, device=kv.device)
+        most = min(1 << max_len.bit_length(), 2 ** 31 - 1) if max_len else 0
+        nbytes = kv.scratch_bytes[key] = int(lib().im_cuda_paged_attention_scratch_bytes(kv.dev.handle, kv.ref, heads, max_new, most))
+    return nbytes
+
+
+def paged_attention_scratch(kv: PagedKV, heads: int, max_new: int, max_len: int = 0) -> torch.Tensor:
+    """Scratch for paged_attention calls of this cache with so many heads, new tokens and rows (or fewer rows); calls that may overlap need
+    one each."""
+    return torch.empty(max(_attention_bytes(kv, heads, max_new, max_len), 16), dtype=torch.uint8, device=kv.device)
 
 
 def paged_attention(kv: PagedKV, layer: int, q, token_start, max_new: int, scale: float, mask=None, max_len=0, out=None, scratch=None):
@@ -524,12 +531,17 @@ def paged_attention(kv: PagedKV, layer: int, q, token_start, max_new: int, scale
         rows, words = mask.shape
         assert mask.dtype is torch.int64 and rows == n and mask.is_contiguous() and mask.get_device() == on
         mp = mask.data_ptr()
+    nbytes, at = 0, None
     if scratch is None:
-        scratch = paged_attention_scratch(kv, heads, max_new)
+        nbytes = _attention_bytes(kv, heads, max_new, max_len)
+        if nbytes:
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=kv.device)
+            at = scratch.data_ptr()
     else:
         assert scratch.dtype is torch.uint8 and scratch.get_device() == on and scratch.is_contiguous()
+        nbytes, at = scratch.numel(), scratch.data_ptr()
     _launch(on, lib().im_cuda_paged_attention, kv.dev.handle, kv.ref, layer, q.data_ptr(), qs, out.data_ptr(), os_, heads, _ints(token_start, on, kv.num_seqs + 1), n, max_new,
-            mp, words, scale, max_len, scratch.data_ptr(), scratch.numel())
+            mp, words, scale, max_len, at, nbytes)
     return out
 
 

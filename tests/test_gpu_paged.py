@@ -203,6 +203,25 @@ def test_one_token_of_sequences_of_all_lengths(dev, dtype, dim, heads, kv_heads)
     _check_attention(dev, c, rng, [1] * len(lengths), heads, dtype)
 
 
+@pytest.mark.parametrize("dtype, dim, heads, kv_heads", [("f16", 128, 8, 2), ("bf16", 64, 5, 1), ("f16", 256, 6, 3), ("bf16", 128, 16, 1)])
+def test_short_contexts_where_long_ones_are_announced(dev, dtype, dim, heads, kv_heads):
+    """Nothing says that the contexts are short: they go by shares of all tiles instead of a cluster per item; NaN and missing pages too."""
+    rng = H.rng_for("announced-long", dim + heads)
+    lengths = [0, 1, 15, 16, 63, 64, 65, 200, 130]
+    c = Cache(dev, rng, [6000] + [n + 2 for n in lengths[1:]], lengths, kv_heads=kv_heads, dim=dim, page=16, dtype=dtype)
+    c.table[7, 3] = 1 << 20
+    c.kv.point_at(_ints(c.table), _ints(lengths))
+    _check_attention(dev, c, rng, [1] * len(lengths), heads, dtype, max_len=0)
+    mask = np.array([[1], [2]] * len(lengths), dtype=np.uint64)      # no node sees the other one
+    for i, n in enumerate(lengths):
+        for x in (c.k, c.v):
+            x[0, c.table[i, n // 16], :, n % 16] = 1.0 if i % 2 else -1.0
+            x[0, c.table[i, (n + 1) // 16], :, (n + 1) % 16] = np.nan if i % 3 == 0 else 2.0
+    mask[1::2] = 1
+    _check_attention(dev, c, rng, [2] * len(lengths), heads, dtype, mask=mask, max_len=0)
+    _check_attention(dev, c, rng, [2] * len(lengths), heads, dtype, mask=mask)
+
+
 @pytest.mark.parametrize("page", [1, 5, 8, 24, 64, 100, 256])
 def test_pages_of_any_size_end_inside_a_tile(dev, page):
     rng = H.rng_for("pages", page)
@@ -689,7 +708,7 @@ def test_two_streams_with_scratch_of_their_own(dev):
 def test_refusals_on_a_device(dev):
     from ironmill_b200 import CudaSysError, ops
     rng = H.rng_for("refusals")
-    c = Cache(dev, rng, [64], [40])
+    c = Cache(dev, rng, [9000], [40], page=64)
     q = _randn(rng, (1, 4, 128), "f16")
     with pytest.raises(CudaSysError, match="scratch"):
         ops.paged_attention(c.kv, 0, q, _ints([0, 1]), 1, 0.1, scratch=torch.empty(64, dtype=torch.uint8, device="cuda"))

@@ -94,7 +94,7 @@ def test_attention_that_is_refused(lib, change, word):
 
 def test_heads_that_attention_is_not_built_for(lib):
     assert "64, 128 and 256" in _message(lib, _attend(lib, _kv(head_dim=96)))
-    assert lib.im_cuda_paged_attention_scratch_bytes(None, C.addressof(_kv()), 4, 1) == 0
+    assert lib.im_cuda_paged_attention_scratch_bytes(None, C.addressof(_kv()), 4, 1, 0) == 0
 
 
 @pytest.mark.parametrize("change, word", [
