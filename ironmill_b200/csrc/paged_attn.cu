@@ -105,23 +105,24 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
     pdl_wait();
     static_assert(!CL || MT == 1, "the join reads all columns of a row");
     Share share;
+    PagedUnit f_u;  // the unit that the copies are at
     if constexpr (CL) {
         const int C = (int)cluster_size(), item = blockIdx.x / C, rank = (int)cluster_rank();
         share.unit = item / p.kv.nkv;
         share.head = item - share.unit * p.kv.nkv;
-        const int n = unit_tiles<kPaTile>(paged_unit<R>(p, share.unit));
+        f_u = paged_unit<R>(p, share.unit);
+        const int n = unit_tiles<kPaTile>(f_u);
         if (n == 0) return;  // all of the cluster
         share.from = share.tile = (int)((long long)n * rank / C);
         share.to = (long long)n * (rank + 1) / C;
     } else {
-        share = find_share<R, kPaTile, kPaThreads>(p, units, sums);
+        share = units <= 32 ? warp_share<R, kPaTile>(p, units, f_u) : find_share<R, kPaTile, kPaThreads>(p, units, sums, f_u);
         if (share.from >= share.to) return;
     }
     const int count = (int)(share.to - share.from);
 
     // ---- the copies' cursor: one slice ahead of the copies, so that a page number is there when it is needed
     int f_unit = share.unit, f_head = share.head, f_tile = share.tile, f_left = count;
-    PagedUnit f_u = paged_unit<R>(p, f_unit);
     int f_tiles = unit_tiles<kPaTile>(f_u);
     int n_page = -1, n_slot = 0, n_head = 0;  // of the slice that is copied next: this lane's row (lane & 15)
     auto fetch = [&]() {

@@ -103,7 +103,7 @@ __device__ __forceinline__ long long share_at(long long total, int n, int c) {
 __device__ __forceinline__ int share_of(long long total, int n, long long a) { return (int)(((a + 1) * n - 1) / total); }
 
 template <int R, int TILE, int THREADS>
-__device__ __forceinline__ Share find_share(const PagedAttn &p, int units, long long *sums) {
+__device__ __forceinline__ Share find_share(const PagedAttn &p, int units, long long *sums, PagedUnit &at) {
     int *found = reinterpret_cast<int *>(sums + THREADS + 32);  // unit, head, tile
     Share s;
     long long total = 0, before = 0;
@@ -149,6 +149,48 @@ __device__ __forceinline__ Share find_share(const PagedAttn &p, int units, long 
     s.unit = found[0];
     s.head = found[1];
     s.tile = found[2];
+    at = paged_unit<R>(p, s.unit);
+    return s;
+}
+
+// The same by every warp for itself, for up to 32 units: a lane per unit, no synchronisation of the block.
+template <int R, int TILE>
+__device__ __forceinline__ Share warp_share(const PagedAttn &p, int units, PagedUnit &at) {
+    const int lane = threadIdx.x & 31;
+    PagedUnit u = paged_unit<R>(p, min(lane, units - 1));
+    const int n = lane < units ? unit_tiles<TILE>(u) : 0;  // (32 sequences of 2^31 rows in tiles of 64: 2^30)
+    int sum = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += t;
+    }
+    const int all = __shfl_sync(0xffffffffu, sum, 31);
+    if (blockIdx.x == 0 && threadIdx.x < 32) {
+        if (lane < units) p.first[lane] = sum - n;
+        if (lane == 0) p.first[units] = all;
+    }
+    Share s;
+    const long long total = (long long)all * p.kv.nkv;
+    const int shares = share_count(total, p.ctas);
+    s.from = share_at(total, shares, blockIdx.x);
+    s.to = share_at(total, shares, blockIdx.x + 1);
+    s.unit = s.head = s.tile = 0;
+    const long long a = (long long)(sum - n) * p.kv.nkv;
+    const unsigned mine = __ballot_sync(0xffffffffu, n > 0 && s.from >= a && s.from < a + (long long)n * p.kv.nkv);
+    if (s.from < s.to) {
+        s.unit = __ffs(mine) - 1;
+        const int d = (int)(s.from - a);
+        s.head = __shfl_sync(0xffffffffu, n > 0 ? d / n : 0, s.unit);
+        s.tile = __shfl_sync(0xffffffffu, n > 0 ? d % n : 0, s.unit);
+    }
+    at.seq = __shfl_sync(0xffffffffu, u.seq, s.unit);
+    at.row0 = __shfl_sync(0xffffffffu, u.row0, s.unit);
+    at.rows = __shfl_sync(0xffffffffu, u.rows, s.unit);
+    at.tok0 = __shfl_sync(0xffffffffu, u.tok0, s.unit);
+    at.len = __shfl_sync(0xffffffffu, u.len, s.unit);
+    at.fresh = __shfl_sync(0xffffffffu, u.fresh, s.unit);
+    at.end = __shfl_sync(0xffffffffu, u.end, s.unit);
     return s;
 }
 

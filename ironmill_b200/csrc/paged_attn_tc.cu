@@ -3,10 +3,13 @@
 // One CTA per SM walks an equal share of the list of all (row tile, KV head) items' tiles of 128 positions (paged_attn.cu has the scheme and joins
 // what the cuts divide). Two sets of four warps ("halves") turn scores into weights, a row per thread; while one of them works, the other's products run:
 //     S = Q K^T    both operands in shared memory, accumulator in tensor memory (f32)
-//     P = exp2(S)  to registers, running maximum and sum in f32, weights back over the scores as two 16-bit terms (weight, and what its rounding left)
+//     P = exp2(S)  to registers, running maximum and sum in f32, weights back over the scores in 16 bits (up to 128 rows: as two terms, the weight and what
+//                  its rounding left)
 //     O += P V     P from tensor memory, V with the head dimension contiguous
 // A tile of up to 256 rows (WIDE): the halves own 128 rows each and every tile of K and V serves both. Up to 128 rows: the halves own the even
-// and the odd tiles of the share, with accumulators of their own that are joined where the item ends.
+// and the odd tiles of the share, with accumulators of their own that are joined where the item ends. There the copies set the pace and the second
+// term of the weights is free; in a wide tile the chain of scores, weights and products does, and one term is what it takes: rounding a weight by half a
+// step (2^-9 bf16, 2^-12 fp16, relative) moves an output by what rounding the output itself does.
 // A row's accumulator is rescaled only when its maximum has grown by more than 2^8 (as in flash_tc.cu).
 //
 // K, V and queries come by 16-byte cp.async of four warps, rows looked up in the page table: any page size, rows that are not there are zeros and
@@ -33,8 +36,8 @@ struct TcShape {
     static constexpr int kBlock = 128 * 128;  // bytes of 128 rows of 64 columns
     static constexpr int kQ = (WIDE ? 2 : 1) * KB * kBlock, kSlot = KB * kBlock;
     static constexpr int kK = 3, kV = WIDE ? 2 : 3;  // slots
-    static constexpr int kBars = 2 * kK + 2 * kV + 2 + 2 + 4 + 2 + 2 + 1;
-    static constexpr int kSmall = 8 * 16 + 128 * 8 + kTcCopyWarps * 32 * 8 + kBars * 8 + 8;  // presence bits, maxima and sums, offsets, barriers, address
+    static constexpr int kBars = 2 * kK + 2 * kV + 2 + 2 + 4 + 2 + 2;
+    static constexpr int kSmall = 8 * 16 + 128 * 8 + kTcCopyWarps * 32 * 8 + kBars * 8 + 48;  // presence bits, maxima and sums, offsets, barriers, address
     static constexpr int kTiles = kQ + (kK + kV) * kSlot;
     static constexpr int kSmem = (kSmall + 1023) / 1024 * 1024 + kTiles;
     static_assert(kSmem <= 232448, "shared memory of an SM");
@@ -49,12 +52,12 @@ struct Items {
     long long left;
     PagedUnit u;
     int tiles, t0, t1, index;
-    __device__ __forceinline__ Items(const PagedAttn &p, int units, const Share &s)
+    __device__ __forceinline__ Items(const PagedAttn &p, int units, const Share &s, const PagedUnit &first)
         : p(p), units(units), unit(s.unit - 1), head(p.kv.nkv - 1), tile(0), left(s.to - s.from), tiles(0), t0(0), t1(0), index(-1) {
         if (left > 0) {
             unit = s.unit;
             head = s.head - 1;
-            u = paged_unit<R>(p, unit);
+            u = first;
             tiles = unit_tiles<kTcTile>(u);
             tile = s.tile;
         }
@@ -144,6 +147,8 @@ __device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+// The 256 threads of both halves.
+__device__ __forceinline__ void both_halves() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 // What copies of other threads have written, once their barrier says so, before the tensor cores read it.
 __device__ __forceinline__ void copies_landed() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // Sums of weighted values that a share leaves: four columns of all rows after another, since a warp that writes (and one that joins) has a row per lane.
@@ -157,14 +162,16 @@ __device__ __forceinline__ void zcopy(uint32_t dst, const void *src, bool there)
 template <bool BF16, int KB, bool WIDE>
 __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_constant__ PagedAttn p, int units, int *err) {
     using Shape = TcShape<KB, WIDE>;
+    constexpr int kTerms = WIDE ? 1 : 2;  // 16-bit terms of a weight
     constexpr int R = Shape::kRows, HD = 64 * KB, SK = Shape::kK, SV = Shape::kV, BLK = Shape::kBlock;
     extern __shared__ __align__(16) unsigned char tc_smem[];
     uint32_t *there = reinterpret_cast<uint32_t *>(tc_smem);                   // [8 tiles][4]: bit j of word w: row 32 w + j of the tile is in the cache
-    float2 *ml = reinterpret_cast<float2 *>(there + 32);                       // [128]: the second half's maximum and sum (not WIDE)
+    float2 *ml = reinterpret_cast<float2 *>(there + 32);                       // [128]: maxima and sums, from half to half (not WIDE)
     long long *offs = reinterpret_cast<long long *>(ml + 128);                 // [copying warps][32]: where the rows that a warp copies lie
     uint64_t *kfull = reinterpret_cast<uint64_t *>(offs + kTcCopyWarps * 32), *kempty = kfull + SK, *vfull = kempty + SK, *vempty = vfull + SV, *qfull = vempty + SV,
-             *qempty = qfull + 1, *sfull = qempty + 1, *pfull = sfull + 2, *ofull = pfull + 4, *oempty = ofull + 2, *mlfull = oempty + 2;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mlfull + 1);
+             *qempty = qfull + 1, *sfull = qempty + 1, *pfull = sfull + 2, *ofull = pfull + 4, *oempty = ofull + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(oempty + 2);
+    uint32_t *odd_rows = tmem_slot + 1;  // [8 warps]
     // (shared memory starts at a multiple of 1024: checked, the tiles would not fit otherwise)
     unsigned char *Qs = tc_smem + (Shape::kSmem - Shape::kTiles), *Ks = Qs + Shape::kQ, *Vs = Ks + SK * Shape::kSlot;
     if (smem_u32(Qs) % 1024 != 0) {
@@ -190,8 +197,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             mbar_init(&ofull[i], 1);
             mbar_init(&oempty[i], 4);
         }
-        mbar_init(mlfull, 4);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+                asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kTcMma) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
@@ -203,8 +209,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     const uint32_t tmem = uniform(*tmem_slot);
     pdl_trigger();  // after the allocation: a successor on this SM cannot take the columns first
     pdl_wait();
-    const Share share = find_share<R, kTcTile, kTcThreads>(p, units, reinterpret_cast<long long *>(Qs));  // (no copy is under way yet)
-    Items<R> it(p, units, share);
+    PagedUnit at;
+    const Share share = units <= 32 ? warp_share<R, kTcTile>(p, units, at) : find_share<R, kTcTile, kTcThreads>(p, units, reinterpret_cast<long long *>(Qs), at);  // (no copy is under way yet)
+    Items<R> it(p, units, share, at);
     bool ok = true;
     if (warp >= kTcCopy) {
         // ---- copies: this warp's 32 rows of every 128
@@ -311,8 +318,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                     fence_after();
                     if (!ok) return;
 #pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        umma_ts(one, o, w + (uint32_t)(c * 64 + (i & 1) * 32 + (i >> 1) * 8), b + (c * 4 + (i >> 1)) * (2048 / 16), kPV, i > 0 || c > 0 || !first);
+                    for (int i = 0; i < 4 * kTerms; i++)
+                        umma_ts(one, o, w + (uint32_t)(c * 64 + i % kTerms * 32 + i / kTerms * 8), b + (c * 4 + i / kTerms) * (2048 / 16), kPV, i > 0 || c > 0 || !first);
                 }
                 turn0 += !h;
                 turn1 += h;
@@ -384,7 +391,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + (uint32_t)(h * kTcTile), to = tmem + lanes + 256u + (uint32_t)(h * 128);
         const float scale = fabsf(p.scale2);
-        int seen = 0, tiles_before = 0, finished = 0, others = 0;  // scores of this half; tiles and items with tiles of the half (others: of the other one) so far
+        int seen = 0, tiles_before = 0, finished = 0;  // scores of this half; tiles and items with tiles of the half so far
         while (it.next()) {
             const PagedUnit &u = it.u;
             const int T = it.t1 - it.t0, jobs = WIDE ? (u.rows > h * 128 ? T : 0) : (T - h + 1) / 2;
@@ -457,12 +464,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                             const uint64_t x = two(x0, x1);
                             sum[j & 1] = add_two(sum[j & 1], x);
                             w[j] = pack2<BF16>(x0, x1);
+                            if (kTerms == 1) continue;
                             const float2 back = unpack2<BF16>(w[j]);
                             const float2 left = of_two(fma_two(two(back.x, back.y), minus_one, x));
                             w2[j] = pack2<BF16>(left.x, left.y);
                         }
                         st16(ts + (uint32_t)(c + 16 * h2), w);
-                        st16(ts + (uint32_t)(c + 32 + 16 * h2), w2);
+                        if (kTerms > 1) st16(ts + (uint32_t)(c + 32 + 16 * h2), w2);
                     }
                     tmem_wait_st();
                     fence_before();
@@ -477,25 +485,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             if (jobs > 0 && ok && !wait_for(&ofull[h], finished & 1, err)) ok = false;
             finished += jobs > 0;
             float f0 = 1.0f, f1 = 0.0f;
-            if constexpr (!WIDE) {
-                if (h == 1) {
-                    // the first half has read what this one left for the item before
-                    if (it.index > 0 && ok && !wait_for(&oempty[1], (it.index - 1) & 1, err)) ok = false;
-                    ml[r] = make_float2(m, l);
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(mlfull);
-                    continue;
+            if constexpr (!WIDE) {  // each half takes half of the columns, of both accumulators
+                const float2 mine = make_float2(m, l);
+                float2 o;
+                fence_before();
+                if (h) {  // (one place for a row, where each half finds what the other one has)
+                    ml[r] = mine;
+                    both_halves();
+                    both_halves();
+                    o = ml[r];
+                } else {
+                    both_halves();
+                    o = ml[r];
+                    ml[r] = mine;
+                    both_halves();
                 }
-                if (ok && !wait_for(mlfull, it.index & 1, err)) ok = false;
-                if (T > 1) {
-                    if (ok && !wait_for(&ofull[1], others & 1, err)) ok = false;
-                    others++;
-                }
-                const float2 o = ml[r];
                 const float M = fmaxf(m, o.x);
                 f0 = m == -INFINITY && l == 0.0f ? 0.0f : ex2(m - M);
                 f1 = o.x == -INFINITY && o.y == 0.0f ? 0.0f : ex2(o.x - M);
-                l = (f0 == 0.0f ? 0.0f : l * f0) + (f1 == 0.0f ? 0.0f : o.y * f1);
+                // (added in the order of the halves, by both of them)
+                const float own = f0 == 0.0f ? 0.0f : l * f0, other = f1 == 0.0f ? 0.0f : o.y * f1;
+                l = h ? other + own : own + other;
                 m = M;
             }
             fence_after();
@@ -505,17 +515,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             const float inv = whole ? (l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l) : 1.0f;
             uint16_t *out = p.out + (u.tok0 + token) * p.os + (long long)(it.head * p.group + (u.row0 + min(R_, u.rows - 1)) % p.group) * HD;
             float worst = 0.0f;
+            bool any_other = false;  // (a half without tiles has left nothing)
+            const uint32_t other_half = tmem + lanes + 256u + (uint32_t)((1 - h) * 128);
             if (WIDE ? jobs > 0 : true) {
 #pragma unroll 1
-                for (int c = 0; c < HD; c += 32) {
+                for (int c = WIDE ? 0 : h * (HD / 2); c < (WIDE ? HD : (h + 1) * (HD / 2)); c += 32) {
                     uint32_t a[32];
                     float v[32];
                     ld32(to + (uint32_t)c, a);
                     tmem_wait_ld();
 #pragma unroll
                     for (int j = 0; j < 32; j++) v[j] = f0 == 0.0f ? 0.0f : __uint_as_float(a[j]) * f0;
-                    if (!WIDE && T > 1) {
-                        ld32(to + 128u + (uint32_t)c, a);
+                    if (!WIDE && f1 != 0.0f) any_other = true;
+                    if (!WIDE && __any_sync(0xffffffffu, any_other)) {
+                        ld32(other_half + (uint32_t)c, a);
                         tmem_wait_ld();
 #pragma unroll
                         for (int j = 0; j < 32; j++) v[j] += f1 == 0.0f ? 0.0f : __uint_as_float(a[j]) * f1;
@@ -533,15 +546,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                         for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(tc_part<R>(p.part_o, slot, HD, R_, c + j)) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
                     }
                 }
-                if (live && !whole) p.part_ml[slot * R + R_] = make_float2(m, l);
+                if (live && !whole && (WIDE || h == 0)) p.part_ml[slot * R + R_] = make_float2(m, l);
             }
             fence_before();
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&oempty[h]);
-                if (!WIDE) mbar_arrive(&oempty[1]);
-            }
+            if (lane == 0) mbar_arrive(&oempty[h]);
             unsigned bad = __ballot_sync(0xffffffffu, live && !(worst == 0.0f));
+            if constexpr (!WIDE) {  // the first half's warps see to the rows that either found
+                if (lane == 0) odd_rows[warp] = bad;
+                both_halves();
+                bad = h ? 0u : bad | odd_rows[warp + 4];
+            }
             while (bad) {
                 const int b = __ffs(bad) - 1, row = WIDE ? h * 128 + (warp & 3) * 32 + b : (warp & 3) * 32 + b;
                 bad &= bad - 1;
@@ -587,17 +602,17 @@ __global__ void __launch_bounds__(256) paged_tc_join_kernel(const __grid_constan
 #pragma unroll
     for (int j = 0; j < 8; j++) o[j] = 0.0f;
 #pragma unroll 4
-    for (int i = 0; i < parts; i++) M = fmaxf(M, p.part_ml[(i == 0 ? slot0 : (size_t)(first + i) * 2) * R + r].x);
-#pragma unroll 4
     for (int i = 0; i < parts; i++) {
         const size_t slot = i == 0 ? slot0 : (size_t)(first + i) * 2;
         const float2 x = p.part_ml[slot * R + r];
         const float4 v = *reinterpret_cast<const float4 *>(tc_part<R>(p.part_o, slot, HD, r, c)), y = *reinterpret_cast<const float4 *>(tc_part<R>(p.part_o, slot, HD, r, c + 4));
         if (x.x == -INFINITY && x.y == 0.0f) continue;  // nothing seen in this part
-        const float f = ex2(x.x - M);
-        L += x.y * f;
-        o[0] += v.x * f; o[1] += v.y * f; o[2] += v.z * f; o[3] += v.w * f;
-        o[4] += y.x * f; o[5] += y.y * f; o[6] += y.z * f; o[7] += y.w * f;
+        const float top = fmaxf(M, x.x), g = M == top ? 1.0f : ex2(M - top), f = ex2(x.x - top);
+        M = top;
+        L = L * g + x.y * f;
+        const float w[8] = {v.x, v.y, v.z, v.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int j = 0; j < 8; j++) o[j] = o[j] * g + w[j] * f;
     }
     const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
     const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
