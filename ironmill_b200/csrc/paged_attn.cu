@@ -352,6 +352,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
         if (tid == 0) bad_rows[!odd_item] = 0;  // every thread has looked at the last item's
         const bool whole = !CL && t0 == 0 && t1 == tiles;
         const size_t part = ((size_t)blockIdx.x * 2 + (first_item ? 0 : 1)) * R;
+        if (!CL && tid == 0) note_span(p, unit, head, t0, t1, tiles, blockIdx.x, first_item ? 0 : 1);
         float f[MT][2];
 #pragma unroll
         for (int mt = 0; mt < MT; mt++)
@@ -495,16 +496,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __gri
     pdl_trigger();
     pdl_wait();
     const int item = blockIdx.x, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, lane = threadIdx.x & 31, r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5);
-    const long long before = p.first[unit], all = p.first[units];
-    const int tiles = (int)(p.first[unit + 1] - before);
-    if (tiles == 0) return;
-    const long long total = all * p.kv.nkv, a = before * p.kv.nkv + (long long)head * tiles;
-    const int n = share_count(total, p.ctas);
-    const int c = share_of(total, n, a), parts = share_of(total, n, a + tiles - 1) - c + 1;
-    if (parts == 1) return;  // one CTA had all of it
+    const int2 span = *reinterpret_cast<const int2 *>(p.spans + 2 * (long long)item);
     const PagedUnit u = paged_unit<R>(p, unit);
-    if (r >= u.rows) return;
-    const size_t slot0 = (size_t)c * 2 + (share_at(total, n, c) == a ? 0 : 1);
+    if (r >= u.rows || span.x < 0) return;  // (a unit without tiles has no rows)
+    const size_t slot0 = span.x;
+    const int c = span.x >> 1, parts = span.y - c + 1;
     auto at = [&](int i) { return (i == 0 ? slot0 : (size_t)(c + i) * 2) * R + r; };
     float M = -INFINITY, L = 0.0f, o[V];
 #pragma unroll
@@ -562,7 +558,7 @@ AttnPlan attn_plan(const Device *dev, int nseq, int nkv, int hd, int group, int 
         return a;
     }
     const size_t slots = (size_t)a.ctas * 2 * a.rows;
-    a.bytes = slots * hd * 4 + slots * 8 + ((size_t)a.units + 1) * 8;
+    a.bytes = slots * hd * 4 + slots * 8 + (size_t)items * 8;
     return a;
 }
 
@@ -667,7 +663,7 @@ IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int
     const size_t slots = (size_t)plan.ctas * 2 * plan.rows;
     p.part_o = static_cast<float *>(scratch_dev);
     p.part_ml = reinterpret_cast<float2 *>(p.part_o + slots * p.kv.hd);
-    p.first = reinterpret_cast<long long *>(p.part_ml + slots);
+    p.spans = reinterpret_cast<int *>(p.part_ml + slots);
     const cudaStream_t st = as_stream(stream);
     const bool bf16 = kv->dtype == IM_DTYPE_BF16;
     if (plan.rows >= 128) return paged_tc_launch(dev, p, bf16, plan.rows, plan.units, st);

@@ -19,7 +19,7 @@ struct PagedAttn {
     int ctas;                 // CTAs of the attention kernel
     float *part_o;            // [ctas, 2, rows of a tile, head_dim]: sums of weighted values
     float2 *part_ml;          // [ctas, 2, rows of a tile]: maximum, sum of weights
-    long long *first;         // [units + 1]: tiles of one KV head before a unit
+    int *spans;               // [units, KV heads, 2]: the slot of an item's first part (-1: one CTA had all of it), the CTA of its last one
 };
 
 // A unit: a tile of rows (token, query head of the KV head) of one sequence, rows token-major.
@@ -84,6 +84,13 @@ __device__ __forceinline__ long long block_scan(int v, long long *sums) {
 template <int TILE>
 __device__ __forceinline__ int unit_tiles(const PagedUnit &u) { return (u.end + TILE - 1) / TILE; }
 
+// Says where the parts of an item lie that CTA `cta` has tiles t0 .. t1 - 1 of, its `slot`-th (0, 1) part if it does not have all of them.
+__device__ __forceinline__ void note_span(const PagedAttn &p, int unit, int head, int t0, int t1, int tiles, int cta, int slot) {
+    int *span = p.spans + 2 * ((long long)unit * p.kv.nkv + head);
+    if (t0 == 0) span[0] = t1 == tiles ? -1 : 2 * cta + slot;
+    if (t1 == tiles) span[1] = cta;
+}
+
 // Where a CTA's share starts.
 struct Share {
     long long from, to;  // places in the list of all tiles
@@ -98,9 +105,6 @@ __device__ __forceinline__ long long share_at(long long total, int n, int c) {
     const long long q = total >> 32 ? total / n : (long long)((uint32_t)total / (uint32_t)n);
     return q * c + (uint32_t)((int)(total - q * n) * c) / (uint32_t)n;
 }
-
-// The share that place a falls to: the last c with total * c / n <= a.
-__device__ __forceinline__ int share_of(long long total, int n, long long a) { return (int)(((a + 1) * n - 1) / total); }
 
 template <int R, int TILE, int THREADS>
 __device__ __forceinline__ Share find_share(const PagedAttn &p, int units, long long *sums, PagedUnit &at) {
@@ -122,7 +126,6 @@ __device__ __forceinline__ Share find_share(const PagedAttn &p, int units, long 
                 all = block_scan<THREADS>(n, sums);
             }
             if (pass == 0) {
-                if (blockIdx.x == 0 && u < units) p.first[u] = total + sums[threadIdx.x] - n;
                 total += all;
                 continue;
             }
@@ -137,7 +140,6 @@ __device__ __forceinline__ Share find_share(const PagedAttn &p, int units, long 
             if (before * p.kv.nkv > s.from) break;
         }
         if (pass == 0) {
-            if (blockIdx.x == 0 && threadIdx.x == 0) p.first[units] = total;
             const long long tiles = total * p.kv.nkv;
             const int shares = share_count(tiles, p.ctas);
             s.from = share_at(tiles, shares, blockIdx.x);
@@ -166,10 +168,6 @@ __device__ __forceinline__ Share warp_share(const PagedAttn &p, int units, Paged
         if (lane >= o) sum += t;
     }
     const int all = __shfl_sync(0xffffffffu, sum, 31);
-    if (blockIdx.x == 0 && threadIdx.x < 32) {
-        if (lane < units) p.first[lane] = sum - n;
-        if (lane == 0) p.first[units] = all;
-    }
     Share s;
     const long long total = (long long)all * p.kv.nkv;
     const int shares = share_count(total, p.ctas);

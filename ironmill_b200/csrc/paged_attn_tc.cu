@@ -512,6 +512,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             const bool live = R_ < u.rows && ok;
             const bool whole = it.t0 == 0 && it.t1 == it.tiles;
             const size_t slot = (size_t)blockIdx.x * 2 + (it.index == 0 ? 0 : 1);
+            if (tid == 0) note_span(p, it.unit, it.head, it.t0, it.t1, it.tiles, blockIdx.x, it.index == 0 ? 0 : 1);
             const float inv = whole ? (l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l) : 1.0f;
             uint16_t *out = p.out + (u.tok0 + token) * p.os + (long long)(it.head * p.group + (u.row0 + min(R_, u.rows - 1)) % p.group) * HD;
             float worst = 0.0f;
@@ -588,31 +589,45 @@ __global__ void __launch_bounds__(256) paged_tc_join_kernel(const __grid_constan
     pdl_wait();
     const int item = blockIdx.x, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, lane = threadIdx.x & 31;
     const int w = blockIdx.y * 8 + (threadIdx.x >> 5), r = w / (HD / 8) * 32 + lane, c = w % (HD / 8) * 8;
-    const long long before = p.first[unit], all = p.first[units];
-    const int tiles = (int)(p.first[unit + 1] - before);
-    if (tiles == 0) return;
-    const long long total = all * p.kv.nkv, a = before * p.kv.nkv + (long long)head * tiles;
-    const int n = share_count(total, p.ctas);
-    const int first = share_of(total, n, a), parts = share_of(total, n, a + tiles - 1) - first + 1;
-    if (parts == 1) return;  // one CTA had all of it
+    const int2 span = *reinterpret_cast<const int2 *>(p.spans + 2 * (long long)item);
     const PagedUnit u = paged_unit<R>(p, unit);
-    if (r >= u.rows) return;
-    const size_t slot0 = (size_t)first * 2 + (share_at(total, n, first) == a ? 0 : 1);
+    if (r >= u.rows || span.x < 0) return;  // (a unit without tiles has no rows)
+    const size_t slot0 = span.x;
+    const int first = span.x >> 1, parts = span.y - first + 1;
     float M = -INFINITY, L = 0.0f, o[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) o[j] = 0.0f;
-#pragma unroll 4
-    for (int i = 0; i < parts; i++) {
-        const size_t slot = i == 0 ? slot0 : (size_t)(first + i) * 2;
-        const float2 x = p.part_ml[slot * R + r];
-        const float4 v = *reinterpret_cast<const float4 *>(tc_part<R>(p.part_o, slot, HD, r, c)), y = *reinterpret_cast<const float4 *>(tc_part<R>(p.part_o, slot, HD, r, c + 4));
-        if (x.x == -INFINITY && x.y == 0.0f) continue;  // nothing seen in this part
-        const float top = fmaxf(M, x.x), g = M == top ? 1.0f : ex2(M - top), f = ex2(x.x - top);
-        M = top;
-        L = L * g + x.y * f;
-        const float w[8] = {v.x, v.y, v.z, v.w, y.x, y.y, y.z, y.w};
+    constexpr int kAtOnce = 4;  // parts that are requested together
+#pragma unroll 1
+    for (int i0 = 0; i0 < parts; i0 += kAtOnce) {
+        float2 x[kAtOnce];
+        float4 v[kAtOnce], y[kAtOnce];
 #pragma unroll
-        for (int j = 0; j < 8; j++) o[j] = o[j] * g + w[j] * f;
+        for (int i = 0; i < kAtOnce; i++) {
+            const int k = min(i0 + i, parts - 1);
+            const size_t slot = k == 0 ? slot0 : (size_t)(first + k) * 2;
+            x[i] = p.part_ml[slot * R + r];
+            v[i] = *reinterpret_cast<const float4 *>(tc_part<R>(p.part_o, slot, HD, r, c));
+            y[i] = *reinterpret_cast<const float4 *>(tc_part<R>(p.part_o, slot, HD, r, c + 4));
+            if (i0 + i >= parts) x[i] = make_float2(-INFINITY, 0.0f);
+        }
+        float top = M;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; i++) top = fmaxf(top, x[i].x);
+        const float corr = M == top ? 1.0f : ex2(M - top);
+        M = top;
+        L *= corr;
+#pragma unroll
+        for (int j = 0; j < 8; j++) o[j] *= corr;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; i++) {
+            const bool none = x[i].x == -INFINITY && x[i].y == 0.0f;  // nothing seen in this part
+            const float f = none ? 0.0f : ex2(x[i].x - top);
+            L += x[i].y * f;
+            const float w[8] = {v[i].x, v[i].y, v[i].z, v[i].w, y[i].x, y[i].y, y[i].z, y[i].w};
+#pragma unroll
+            for (int j = 0; j < 8; j++) o[j] += none ? 0.0f : w[j] * f;
+        }
     }
     const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
     const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
