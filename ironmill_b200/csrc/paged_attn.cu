@@ -22,16 +22,14 @@ namespace {
 
 constexpr int kPaWarps = 4, kPaThreads = kPaWarps * 32, kPaSlice = 16, kPaTile = kPaWarps * kPaSlice;
 
-template <int HD, int MT>
+template <int HD>
 struct PaShape {
-    static constexpr int kRows = 16 * MT;
+    static constexpr int kRows = 16;
     static constexpr int kSliceBytes = kPaSlice * HD * 2;
     static constexpr int kStages = HD == 64 ? 6 : 3;
     static constexpr int kRing = kPaWarps * kStages * 2 * kSliceBytes;
-    static constexpr int kQ = MT > 1 ? kRows * HD * 2 : 0;        // queries in shared memory where registers do not hold them
-    static constexpr int kMergeCols = MT > 1 ? 32 : HD;           // columns that are joined at a time
-    static constexpr int kMerge = kRows * kMergeCols * 4;
-    static constexpr int kSmem = kRing + kQ + kMerge + kPaWarps * kRows * 8;
+    static constexpr int kMerge = kRows * HD * 4;
+    static constexpr int kSmem = kRing + kMerge + kPaWarps * kRows * 8;
 };
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
@@ -86,24 +84,22 @@ __device__ __forceinline__ float2 remote2(uint32_t at) {
 
 // CL: instead of shares of the list of all tiles, a cluster of CTAs per item, each with an equal run of its tiles; they join what they have
 // through each other's shared memory, in the same launch and without scratch.
-template <bool BF16, int HD, int MT, bool CL>
+template <bool BF16, int HD, bool CL>
 __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kernel(const __grid_constant__ PagedAttn p, int units) {
-    using S = PaShape<HD, MT>;
+    using S = PaShape<HD>;
     constexpr int R = S::kRows, KS = HD / 16, NT = HD / 8, CH = HD / 8;  // k steps, 8-column tiles, 16-byte pieces of a row
     extern __shared__ __align__(128) unsigned char pa_smem[];
     __shared__ long long sums[kPaThreads + kShareMore];
     __shared__ unsigned rows_there[kPaWarps][8];  // of a slice in the ring: bit r where row r is in the cache
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     unsigned char *ring = pa_smem + warp * (S::kRing / kPaWarps);
-    unsigned char *qsm = pa_smem + S::kRing;
-    float *merge = reinterpret_cast<float *>(qsm + S::kQ);
+    float *merge = reinterpret_cast<float *>(pa_smem + S::kRing);
     float2 *ml = reinterpret_cast<float2 *>(reinterpret_cast<unsigned char *>(merge) + S::kMerge);  // [warps, R]
     __shared__ unsigned bad_rows[2];  // rows of an item whose sums are not finite, every other item's
     __shared__ float2 joint[CL ? R : 1];  // maximum and sum of this CTA's part of each row
     if (tid < 2) bad_rows[tid] = 0;
     pdl_trigger();
     pdl_wait();
-    static_assert(!CL || MT == 1, "the join reads all columns of a row");
     Share share;
     PagedUnit f_u;  // the unit that the copies are at
     if constexpr (CL) {
@@ -193,48 +189,29 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
         }
         const int t0 = tile, t1 = min(tiles, tile + count - done);
         // queries: A fragments, rows lane / 4 and lane / 4 + 8 of each 16
-        uint32_t qf[MT == 1 ? KS : 1][4];
-        int tok[MT][2];
+        uint32_t qf[KS][4];
+        int tok[2];
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int r = mt * 16 + (lane >> 2) + 8 * i;
-                tok[mt][i] = (u.row0 + min(r, u.rows - 1)) / p.group;
-            }
-        if constexpr (MT == 1) {
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int r = (lane >> 2) + 8 * i;
-                const uint32_t *src = reinterpret_cast<const uint32_t *>(p.q + (u.tok0 + tok[0][i]) * p.qs + (long long)(head * p.group + (u.row0 + r) % p.group) * HD);
-#pragma unroll
-                for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++) qf[ks][2 * j + i] = r < u.rows ? __ldg(src + ks * 8 + j * 4 + (lane & 3)) : 0u;
-            }
-        } else {
-            __syncthreads();
-            for (int i = tid; i < R * CH; i += kPaThreads) {
-                const int r = i / CH, c = i % CH;
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (r < u.rows) {
-                    const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
-                    x = __ldg(reinterpret_cast<const uint4 *>(p.q + (u.tok0 + t) * p.qs + (long long)(head * p.group + g) * HD) + c);
-                }
-                *reinterpret_cast<uint4 *>(qsm + r * (HD * 2) + ((c ^ (r & 7)) << 4)) = x;
-            }
-            __syncthreads();
+        for (int i = 0; i < 2; i++) {
+            const int r = (lane >> 2) + 8 * i;
+            tok[i] = (u.row0 + min(r, u.rows - 1)) / p.group;
         }
-        float m[MT][2], l[MT][2], o[MT][NT][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
+        for (int i = 0; i < 2; i++) {
+            const int r = (lane >> 2) + 8 * i;
+            const uint32_t *src = reinterpret_cast<const uint32_t *>(p.q + (u.tok0 + tok[i]) * p.qs + (long long)(head * p.group + (u.row0 + r) % p.group) * HD);
 #pragma unroll
-            for (int i = 0; i < 2; i++) m[mt][i] = -INFINITY, l[mt][i] = 0.0f;
+            for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) o[mt][n][j] = 0.0f;
+                for (int j = 0; j < 2; j++) qf[ks][2 * j + i] = r < u.rows ? __ldg(src + ks * 8 + j * 4 + (lane & 3)) : 0u;
         }
+        float m[2], l[2], o[NT][4];
+#pragma unroll
+        for (int i = 0; i < 2; i++) m[i] = -INFINITY, l[i] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[n][j] = 0.0f;
         for (; tile < t1; tile++, done++) {
             // the next slice on its way, this one there
             if (done + S::kStages - 1 < count) {
@@ -247,93 +224,71 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
             asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
             __syncwarp();
             const uint32_t ks_at = smem_u32(ring) + stage * 2 * S::kSliceBytes, vs_at = ks_at + S::kSliceBytes;
-            float s[MT][2][4];
+            float s[2][4];
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+            for (int n = 0; n < 2; n++)
 #pragma unroll
-                for (int n = 0; n < 2; n++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) s[mt][n][j] = 0.0f;
+                for (int j = 0; j < 4; j++) s[n][j] = 0.0f;
             {
                 const int r = (lane & 7) + ((lane >> 4) << 3), hi = (lane >> 3) & 1;  // row and 16-byte half of this lane's matrix row
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
                     uint32_t b[4];
                     ldsm4(b, ks_at + r * (HD * 2) + (((2 * ks + hi) ^ (r & 7)) << 4));
-#pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-                        if constexpr (MT == 1) {
-                            mma16<BF16>(s[mt][0], qf[ks], b[0], b[1]);
-                            mma16<BF16>(s[mt][1], qf[ks], b[2], b[3]);
-                        } else {
-                            uint32_t a[4];
-                            const int qr = mt * 16 + (lane & 15), qc = 2 * ks + (lane >> 4);
-                            ldsm4(a, smem_u32(qsm) + qr * (HD * 2) + ((qc ^ (qr & 7)) << 4));
-                            mma16<BF16>(s[mt][0], a, b[0], b[1]);
-                            mma16<BF16>(s[mt][1], a, b[2], b[3]);
-                        }
-                    }
+                    mma16<BF16>(s[0], qf[ks], b[0], b[1]);
+                    mma16<BF16>(s[1], qf[ks], b[2], b[3]);
                 }
             }
             const int pos0 = tile * kPaTile + warp * kPaSlice;
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+            for (int n = 0; n < 2; n++)
 #pragma unroll
-                for (int n = 0; n < 2; n++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) s[mt][n][j] *= p.scale2;
+                for (int j = 0; j < 4; j++) s[n][j] *= p.scale2;
             const unsigned there = rows_there[warp][stage] & 0xffffu;
             if (there != 0xffffu || pos0 + kPaSlice > u.len) {  // some row may not see some position
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++)
+                for (int n = 0; n < 2; n++)
 #pragma unroll
-                    for (int n = 0; n < 2; n++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const int at = n * 8 + (lane & 3) * 2 + (j & 1);
-                            if (!(there >> at & 1) || !paged_sees(p, u, tok[mt][j >> 1], pos0 + at)) s[mt][n][j] = -INFINITY;
-                        }
+                    for (int j = 0; j < 4; j++) {
+                        const int at = n * 8 + (lane & 3) * 2 + (j & 1);
+                        if (!(there >> at & 1) || !paged_sees(p, u, tok[j >> 1], pos0 + at)) s[n][j] = -INFINITY;
+                    }
             }
-            uint32_t w[MT][4], w2[MT][4];
+            uint32_t w[4], w2[4];
 #pragma unroll
-            for (int mt = 0; mt < MT; mt++)
+            for (int i = 0; i < 2; i++) {
+                float top = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                if (__any_sync(0xffffffffu, top > m[i])) {
+                    const float m_new = fmaxf(m[i], top), corr = m_new == -INFINITY ? 1.0f : ex2(m[i] - m_new);
+                    m[i] = m_new;
+                    l[i] *= corr;
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    float top = fmaxf(fmaxf(s[mt][0][2 * i], s[mt][0][2 * i + 1]), fmaxf(s[mt][1][2 * i], s[mt][1][2 * i + 1]));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    if (__any_sync(0xffffffffu, top > m[mt][i])) {
-                        const float m_new = fmaxf(m[mt][i], top), corr = m_new == -INFINITY ? 1.0f : ex2(m[mt][i] - m_new);
-                        m[mt][i] = m_new;
-                        l[mt][i] *= corr;
-#pragma unroll
-                        for (int n = 0; n < NT; n++) o[mt][n][2 * i] *= corr, o[mt][n][2 * i + 1] *= corr;
-                    }
-                    const float base = m[mt][i] == -INFINITY ? 0.0f : m[mt][i];
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int n = 0; n < 2; n++) {
-                        const float x0 = ex2(s[mt][n][2 * i] - base), x1 = ex2(s[mt][n][2 * i + 1] - base);
-                        sum += x0 + x1;
-                        w[mt][2 * n + i] = pack16<BF16>(x0, x1);
-                        const float2 back = unpack16<BF16>(w[mt][2 * n + i]);
-                        w2[mt][2 * n + i] = pack16<BF16>(x0 - back.x, x1 - back.y);
-                    }
-                    l[mt][i] += sum;
+                    for (int n = 0; n < NT; n++) o[n][2 * i] *= corr, o[n][2 * i + 1] *= corr;
                 }
+                const float base = m[i] == -INFINITY ? 0.0f : m[i];
+                float sum = 0.0f;
+#pragma unroll
+                for (int n = 0; n < 2; n++) {
+                    const float x0 = ex2(s[n][2 * i] - base), x1 = ex2(s[n][2 * i + 1] - base);
+                    sum += x0 + x1;
+                    w[2 * n + i] = pack16<BF16>(x0, x1);
+                    const float2 back = unpack16<BF16>(w[2 * n + i]);
+                    w2[2 * n + i] = pack16<BF16>(x0 - back.x, x1 - back.y);
+                }
+                l[i] += sum;
+            }
             {
                 const int r = (lane & 7) + (((lane >> 3) & 1) << 3), hi = lane >> 4;
 #pragma unroll
                 for (int n = 0; n < NT; n += 2) {
                     uint32_t b[4];
                     ldsm4t(b, vs_at + r * (HD * 2) + (((n + hi) ^ (r & 7)) << 4));
-#pragma unroll
-                    for (int mt = 0; mt < MT; mt++) {
-                        mma16<BF16>(o[mt][n], w[mt], b[0], b[1]);
-                        mma16<BF16>(o[mt][n + 1], w[mt], b[2], b[3]);
-                        mma16<BF16>(o[mt][n], w2[mt], b[0], b[1]);
-                        mma16<BF16>(o[mt][n + 1], w2[mt], b[2], b[3]);
-                    }
+                    mma16<BF16>(o[n], w, b[0], b[1]);
+                    mma16<BF16>(o[n + 1], w, b[2], b[3]);
+                    mma16<BF16>(o[n], w2, b[0], b[1]);
+                    mma16<BF16>(o[n + 1], w2, b[2], b[3]);
                 }
             }
             __syncwarp();  // every lane has read the slice before the copies of the one that takes its place
@@ -341,29 +296,25 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
         }
         // ---- the item's (or the share's part of it) rows: four warps' sums joined in order
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                l[mt][i] += __shfl_xor_sync(0xffffffffu, l[mt][i], 1);
-                l[mt][i] += __shfl_xor_sync(0xffffffffu, l[mt][i], 2);
-                if ((lane & 3) == 0) ml[warp * R + mt * 16 + (lane >> 2) + 8 * i] = make_float2(m[mt][i], l[mt][i]);
-            }
+        for (int i = 0; i < 2; i++) {
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+            if ((lane & 3) == 0) ml[warp * R + (lane >> 2) + 8 * i] = make_float2(m[i], l[i]);
+        }
         __syncthreads();
         if (tid == 0) bad_rows[!odd_item] = 0;  // every thread has looked at the last item's
         const bool whole = !CL && t0 == 0 && t1 == tiles;
         const size_t part = ((size_t)blockIdx.x * 2 + (first_item ? 0 : 1)) * R;
         if (!CL && tid == 0) note_span(p, unit, head, t0, t1, tiles, blockIdx.x, first_item ? 0 : 1);
-        float f[MT][2];
+        float f[2];
 #pragma unroll
-        for (int mt = 0; mt < MT; mt++)
+        for (int i = 0; i < 2; i++) {
+            const int r = (lane >> 2) + 8 * i;
+            float M = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int r = mt * 16 + (lane >> 2) + 8 * i;
-                float M = -INFINITY;
-#pragma unroll
-                for (int w = 0; w < kPaWarps; w++) M = fmaxf(M, ml[w * R + r].x);
-                f[mt][i] = m[mt][i] == -INFINITY && l[mt][i] == 0.0f ? 0.0f : ex2(m[mt][i] - M);
-            }
+            for (int w = 0; w < kPaWarps; w++) M = fmaxf(M, ml[w * R + r].x);
+            f[i] = m[i] == -INFINITY && l[i] == 0.0f ? 0.0f : ex2(m[i] - M);
+        }
         auto row_ml = [&](int r) {
             float M = -INFINITY, L = 0.0f;
 #pragma unroll
@@ -375,60 +326,54 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
             }
             return make_float2(M, L);
         };
-        constexpr int MC = S::kMergeCols;
-#pragma unroll
-        for (int c0 = 0; c0 < HD; c0 += MC) {
 #pragma unroll 1
-            for (int w = 0; w < kPaWarps; w++) {
-                if (warp == w) {
+        for (int w = 0; w < kPaWarps; w++) {
+            if (warp == w) {
 #pragma unroll
-                    for (int mt = 0; mt < MT; mt++)
+                for (int n = 0; n < NT; n++)
 #pragma unroll
-                        for (int n = c0 / 8; n < (c0 + MC) / 8; n++)
-#pragma unroll
-                            for (int i = 0; i < 2; i++) {
-                                float2 *at = reinterpret_cast<float2 *>(merge + (mt * 16 + (lane >> 2) + 8 * i) * MC + ((n * 8 - c0 + (lane & 3) * 2) ^ (((lane >> 2) & 3) << 3)));
-                                float2 x = make_float2(o[mt][n][2 * i] * f[mt][i], o[mt][n][2 * i + 1] * f[mt][i]);
-                                if (f[mt][i] == 0.0f) x = make_float2(0.0f, 0.0f);
-                                if (w > 0) {
-                                    const float2 y = *at;
-                                    x.x += y.x;
-                                    x.y += y.y;
-                                }
-                                *at = x;
-                            }
-                }
-                __syncthreads();
+                    for (int i = 0; i < 2; i++) {
+                        float2 *at = reinterpret_cast<float2 *>(merge + ((lane >> 2) + 8 * i) * HD + ((n * 8 + (lane & 3) * 2) ^ (((lane >> 2) & 3) << 3)));
+                        float2 x = make_float2(o[n][2 * i] * f[i], o[n][2 * i + 1] * f[i]);
+                        if (f[i] == 0.0f) x = make_float2(0.0f, 0.0f);
+                        if (w > 0) {
+                            const float2 y = *at;
+                            x.x += y.x;
+                            x.y += y.y;
+                        }
+                        *at = x;
+                    }
             }
-            for (int i = tid; i < u.rows * (MC / 8); i += kPaThreads) {
-                const int r = i / (MC / 8), c = i % (MC / 8) * 8;
-                const float *src = merge + r * MC + (c ^ ((r & 3) << 3));
-                float v[8], worst = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; j += 4) *reinterpret_cast<float4 *>(v + j) = *reinterpret_cast<const float4 *>(src + j);
-#pragma unroll
-                for (int j = 0; j < 8; j++) worst += v[j] * 0.0f;  // zero unless a value is not finite
-                if (worst != 0.0f) atomicOr(&bad_rows[odd_item], 1u << r);
-                if (whole) {
-                    const float2 x = row_ml(r);
-                    const float inv = x.y > 0.0f ? 1.0f / x.y : x.y == 0.0f ? 0.0f : x.y;
-                    const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
-                    *reinterpret_cast<uint4 *>(p.out + (u.tok0 + t) * p.os + (long long)(head * p.group + g) * HD + c0 + c) =
-                        make_uint4(pack16<BF16>(v[0] * inv, v[1] * inv), pack16<BF16>(v[2] * inv, v[3] * inv), pack16<BF16>(v[4] * inv, v[5] * inv),
-                                   pack16<BF16>(v[6] * inv, v[7] * inv));
-                } else if (!CL) {
-                    float4 *dst = reinterpret_cast<float4 *>(p.part_o + (part + r) * HD + c0 + c);
-                    dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-                    dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-                }
-            }
-            if (!whole && c0 == 0)
-                for (int r = tid; r < u.rows; r += kPaThreads) {
-                    if (CL) joint[r] = row_ml(r);
-                    else p.part_ml[part + r] = row_ml(r);
-                }
             __syncthreads();
         }
+        for (int i = tid; i < u.rows * CH; i += kPaThreads) {
+            const int r = i / CH, c = i % CH * 8;
+            const float *src = merge + r * HD + (c ^ ((r & 3) << 3));
+            float v[8], worst = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) *reinterpret_cast<float4 *>(v + j) = *reinterpret_cast<const float4 *>(src + j);
+#pragma unroll
+            for (int j = 0; j < 8; j++) worst += v[j] * 0.0f;  // zero unless a value is not finite
+            if (worst != 0.0f) atomicOr(&bad_rows[odd_item], 1u << r);
+            if (whole) {
+                const float2 x = row_ml(r);
+                const float inv = x.y > 0.0f ? 1.0f / x.y : x.y == 0.0f ? 0.0f : x.y;
+                const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
+                *reinterpret_cast<uint4 *>(p.out + (u.tok0 + t) * p.os + (long long)(head * p.group + g) * HD + c) =
+                    make_uint4(pack16<BF16>(v[0] * inv, v[1] * inv), pack16<BF16>(v[2] * inv, v[3] * inv), pack16<BF16>(v[4] * inv, v[5] * inv),
+                               pack16<BF16>(v[6] * inv, v[7] * inv));
+            } else if (!CL) {
+                float4 *dst = reinterpret_cast<float4 *>(p.part_o + (part + r) * HD + c);
+                dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+                dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+            }
+        }
+        if (!whole)
+            for (int r = tid; r < u.rows; r += kPaThreads) {
+                if (CL) joint[r] = row_ml(r);
+                else p.part_ml[part + r] = row_ml(r);
+            }
+        __syncthreads();
         if (const unsigned bad = bad_rows[odd_item]) {
             for (int r = warp; r < u.rows; r += kPaWarps) {
                 if (!(bad >> r & 1)) continue;
@@ -438,7 +383,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
                 const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
                 for (int i = 0; i < HD / 32; i++) {
                     if (whole) p.out[(u.tok0 + t) * p.os + (long long)(head * p.group + g) * HD + lane + 32 * i] = (uint16_t)pack16<BF16>(x[i] * inv, 0.0f);
-                    else if (CL) merge[r * MC + ((lane + 32 * i) ^ ((r & 3) << 3))] = x[i];
+                    else if (CL) merge[r * HD + ((lane + 32 * i) ^ ((r & 3) << 3))] = x[i];
                     else p.part_o[(part + r) * HD + lane + 32 * i] = x[i];
                 }
                 if (!whole && lane == 0) (CL ? joint[r] : p.part_ml[part + r]) = make_float2(M, L);
@@ -542,10 +487,12 @@ struct AttnPlan {
 constexpr int kClusterMost = 8, kClusterTiles = 8;
 AttnPlan attn_plan(const Device *dev, int nseq, int nkv, int hd, int group, int max_new, int max_len) {
     AttnPlan a;
-    // up to 16 rows of a KV head: one m16 tile; more: two, so that half the row tiles read the cache again (heads of 256: one, registers)
+    // Up to 16 rows of a KV head (and heads of 256, whose scores and outputs tensor memory does not hold twice) on mma.sync, more on tcgen05. Eight sequences of
+    // up to 4001 rows: 16 rows 29.7 us here, 28.6 there; 8 rows 27.6 and 28.5; 20 rows as two tiles of 16: 40 and 29. 32 sequences of up to 8192, one token
+    // each (4 rows): 103 and 122.
     const int tc = paged_tc_rows(hd, (long long)group * max_new);
     a.tile = tc ? 128 : kPaTile;
-    a.rows = tc ? tc : hd == 256 || (long long)group * max_new <= 16 ? 16 : 32;
+    a.rows = tc ? tc : 16;
     a.row_tiles = (int)(((long long)group * max_new + a.rows - 1) / a.rows);
     a.units = nseq * a.row_tiles;
     a.ctas = dev->sm_count * (tc || hd == 256 ? 1 : 2);
@@ -570,15 +517,15 @@ int join_launch(const PagedAttn &p, int units, cudaStream_t st) {
     return IM_OK;
 }
 
-template <bool BF16, int HD, int MT>
+template <bool BF16, int HD>
 int attn_launch(const Device *dev, const PagedAttn &p, int units, int cluster, cudaStream_t st) {
-    using S = PaShape<HD, MT>;
+    using S = PaShape<HD>;
     static DeviceOnce once;
     if (once.first(dev->ordinal)) {
-        IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, MT, false>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
-        if (MT == 1) IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, 1, true>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+        IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, false>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+        IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, true>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     }
-    if (MT == 1 && cluster) {
+    if (cluster) {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)(units * p.kv.nkv * cluster));
         cfg.blockDim = dim3(kPaThreads);
@@ -592,10 +539,10 @@ int attn_launch(const Device *dev, const PagedAttn &p, int units, int cluster, c
         attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 2;
-        IM_CUDA_CHECK(cudaLaunchKernelEx(&cfg, paged_attn_kernel<BF16, HD, 1, true>, p, units));
+        IM_CUDA_CHECK(cudaLaunchKernelEx(&cfg, paged_attn_kernel<BF16, HD, true>, p, units));
         return IM_OK;
     }
-    IM_CUDA_CHECK(launch_k(paged_attn_kernel<BF16, HD, MT, false>, dim3(p.ctas), dim3(kPaThreads), (size_t)S::kSmem, st, p, units));
+    IM_CUDA_CHECK(launch_k(paged_attn_kernel<BF16, HD, false>, dim3(p.ctas), dim3(kPaThreads), (size_t)S::kSmem, st, p, units));
     return join_launch<BF16, S::kRows, HD>(p, units, st);
 }
 
@@ -667,11 +614,11 @@ IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int
     const cudaStream_t st = as_stream(stream);
     const bool bf16 = kv->dtype == IM_DTYPE_BF16;
     if (plan.rows >= 128) return paged_tc_launch(dev, p, bf16, plan.rows, plan.units, st);
-#define IM_RUN(HD, MT) (bf16 ? attn_launch<true, HD, MT>(dev, p, plan.units, plan.cluster, st) : attn_launch<false, HD, MT>(dev, p, plan.units, plan.cluster, st))
+#define IM_RUN(HD) (bf16 ? attn_launch<true, HD>(dev, p, plan.units, plan.cluster, st) : attn_launch<false, HD>(dev, p, plan.units, plan.cluster, st))
     switch (kv->head_dim) {
-    case 64: return plan.rows == 16 ? IM_RUN(64, 1) : IM_RUN(64, 2);
-    case 128: return plan.rows == 16 ? IM_RUN(128, 1) : IM_RUN(128, 2);
-    default: return IM_RUN(256, 1);
+    case 64: return IM_RUN(64);
+    case 128: return IM_RUN(128);
+    default: return IM_RUN(256);
     }
 #undef IM_RUN
     IM_GUARD_END

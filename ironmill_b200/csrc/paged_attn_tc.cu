@@ -650,7 +650,7 @@ int tc_launch(const Device *dev, const PagedAttn &p, int units, cudaStream_t st)
 
 int paged_tc_rows(int hd, long long rows) {
     if (hd != 64 && hd != 128) return 0;
-    return rows <= 32 ? 0 : rows <= 128 ? 128 : 256;
+    return rows <= 16 ? 0 : rows <= 128 ? 128 : 256;
 }
 
 int paged_tc_launch(const Device *dev, const PagedAttn &p, bool bf16, int rows, int units, cudaStream_t st) {
