@@ -369,7 +369,7 @@ int im_cuda_paged_reorder(im_device *dev, const im_paged_kv *kv, const int *pare
  * hold a NaN or +inf); where fewer than `picks` are left, the rest gets score -inf, parent -1 and token -1.
  * score_out f32, parent_out (beam in the group) and token_out i32: [groups, picks].  1 <= beams <= 64, 1 <= picks <= 64.
  * Greedy decoding's pick (crates/ironmill-inference/src/sampling.rs:331-339) takes the last maximal index; this takes the first.
- * scratch_dev: 16-byte aligned, calls whose kernels may overlap need one each. */
+ * scratch_dev: 16-byte aligned, calls whose kernels may overlap need one each; few beams over few logits need none. */
 size_t im_cuda_beam_select_scratch_bytes(const im_device *dev, int groups, int beams, int vocab, int picks);
 int im_cuda_beam_select(im_device *dev, const void *logits_dev, int dtype, int64_t row_stride, int groups, int beams, int vocab, const float *score_dev,
                         const uint8_t *done_dev, int end_token, int picks, float *score_out_dev, int *parent_out_dev, int *token_out_dev,

@@ -19,6 +19,7 @@
 
 #include <algorithm>
 
+#include "cluster.cuh"
 #include "paged.cuh"
 
 namespace im {
@@ -85,10 +86,10 @@ __device__ __forceinline__ float exp_of(float x) {
 }
 
 // What reaches the bound, and the best of it.
-template <typename V, typename I>
+template <typename V, typename I, int BUF>
 struct Best {
-    V buf_v[kSelBuf];
-    I buf_i[kSelBuf];
+    V buf_v[BUF];
+    I buf_i[BUF];
     V out_v[kSelMost];
     I out_i[kSelMost];
     V tops[kSelThreads], low;
@@ -134,14 +135,14 @@ struct Best {
     }
     __device__ __forceinline__ void collect(V v, I i) {
         const int at = atomicAdd(&count, 1);
-        if (at < kSelBuf) buf_v[at] = v, buf_i[at] = i;
+        if (at < BUF) buf_v[at] = v, buf_i[at] = i;
     }
     // The best into out_v, out_i, in order. visit(f) hands all elements of this thread to f(value, index).
     template <typename Visit>
     __device__ __forceinline__ void rank(int picks, Visit visit) {
         __syncthreads();
         const int t = threadIdx.x, n = count;
-        if (n <= kSelBuf) {
+        if (n <= BUF) {
             for (int i = t; i < n; i += kSelThreads) {
                 const V v = buf_v[i];
                 const I x = buf_i[i];
@@ -180,21 +181,26 @@ struct Best {
     }
 };
 
-// grid (slices, rows)
+// A slice of a row: its best logits in order in best.out_v / out_i, its maximum and sum of exponentials.
+struct SliceSpace {
+    Best<float, int, kSelBuf> best;
+    float red_m[kSelThreads / 32], red_s[kSelThreads / 32];
+    float met_v[kSelBuf];  // sixteen elements of a thread that reach the bound: their maximum, and which
+    int met_i[kSelBuf], kept[kSelBuf], met, keep;
+    float2 ms;
+};
+
 template <int DT>
-__global__ void __launch_bounds__(kSelThreads, kSelResident) beam_slice_kernel(const __grid_constant__ Select p) {
+__device__ __forceinline__ void slice_best(const Select &p, long long row, int slice, SliceSpace &sp) {
     using L = Logit<DT>;
     using T = typename L::T;
     constexpr int V = L::kVec, Q = 16 / V;  // requests of a piece: 16 elements of each thread
-    __shared__ Best<float, int> best;
-    __shared__ float red_m[kSelThreads / 32], red_s[kSelThreads / 32];
-    __shared__ float met_v[kSelBuf];  // sixteen elements of a thread that reach the bound: their maximum, and which
-    __shared__ int met_i[kSelBuf], kept[kSelBuf], met, keep;
-    pdl_trigger();
-    pdl_wait();
-    const int slice = blockIdx.x, t = threadIdx.x;
-    const long long row = blockIdx.y;
-    if (p.done && p.done[row]) return;
+    auto &best = sp.best;
+    auto &met = sp.met;
+    auto &keep = sp.keep;
+    float *red_m = sp.red_m, *red_s = sp.red_s, *met_v = sp.met_v;
+    int *met_i = sp.met_i, *kept = sp.kept;
+    const int t = threadIdx.x;
     const T *x = static_cast<const T *>(p.x) + row * p.stride;
     const int a = slice * p.slice, b = min(a + p.slice, p.vocab);
     // 16-byte requests from the first aligned element on; what is before and behind them is read one by one
@@ -296,42 +302,51 @@ __global__ void __launch_bounds__(kSelThreads, kSelResident) beam_slice_kernel(c
         for (int w = 0; w < kSelThreads / 32; w++) M = fmaxf(M, red_m[w]);
         S = 0.0f;
         for (int w = 0; w < kSelThreads / 32; w++) S += red_m[w] == -INFINITY && red_s[w] == 0.0f ? 0.0f : red_s[w] * exp_of(red_m[w] - M);
-        p.part_ms[row * p.slices + slice] = make_float2(M, S);
+        sp.ms = make_float2(M, S);
     }
+    __syncthreads();
+}
+
+// grid (slices, rows)
+template <int DT>
+__global__ void __launch_bounds__(kSelThreads, kSelResident) beam_slice_kernel(const __grid_constant__ Select p) {
+    __shared__ SliceSpace sp;
+    pdl_trigger();
+    pdl_wait();
+    const int slice = blockIdx.x, t = threadIdx.x;
+    const long long row = blockIdx.y;
+    if (p.done && p.done[row]) return;
+    slice_best<DT>(p, row, slice, sp);
+    if (t == 0) p.part_ms[row * p.slices + slice] = sp.ms;
     const long long at = (row * p.slices + slice) * p.picks;
     for (int k = t; k < p.picks; k += kSelThreads) {
-        p.part_v[at + k] = best.out_v[k];
-        p.part_i[at + k] = best.out_i[k];
+        p.part_v[at + k] = sp.best.out_v[k];
+        p.part_i[at + k] = sp.best.out_i[k];
     }
 }
 
-// grid (groups)
-__global__ void __launch_bounds__(kSelThreads) beam_join_kernel(const __grid_constant__ Select p) {
-    __shared__ Best<double, long long> best;
-    __shared__ double offset[kSelMost];  // score - lse of each beam; NaN: nothing of it is picked
-    pdl_trigger();
-    pdl_wait();
-    const int group = blockIdx.x, t = threadIdx.x, lane = t & 31;
+// What the slices of a group's beams found, joined.
+constexpr int kHeld = 4 * kSelThreads;  // candidates that fit shared memory
+struct JoinSpace {
+    Best<double, long long, kSelBuf / 2> best;
+    double offset[kSelMost];  // score - lse of each beam; NaN: nothing of it is picked
+    float held_v[kHeld];
+    int held_i[kHeld];
+};
+
+// ms: maxima and sums of the beams' slices; held: all candidates (on their way, where they come from memory) are in held_v, held_i
+__device__ __forceinline__ void join_group(const Select &p, int group, const float2 *ms, bool held, JoinSpace &sp) {
+    auto &best = sp.best;
+    double *offset = sp.offset;
+    const int t = threadIdx.x, lane = t & 31;
     const long long row0 = (long long)group * p.beams;
     const int per = p.slices * p.picks, n = p.beams * per;
-    // what the slices found is on its way while lse is computed
-    constexpr int kHeld = 4;
-    __shared__ float held_v[kHeld * kSelThreads];
-    __shared__ int held_i[kHeld * kSelThreads];
-    const bool held = n <= kHeld * kSelThreads;
-    if (held) {
-        for (int i = t; i < n; i += kSelThreads) {
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(held_v + i)), "l"(p.part_v + row0 * per + i) : "memory");
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(held_i + i)), "l"(p.part_i + row0 * per + i) : "memory");
-        }
-    }
     best.clear(p.picks);
     for (int b = t >> 5; b < p.beams; b += kSelThreads / 32) {
         const bool done = p.done && p.done[row0 + b];
         float m = -INFINITY, s = 0.0f;
         if (!done) {
-            const float2 *ms = p.part_ms + (row0 + b) * p.slices;
-            const float2 x = lane < p.slices ? ms[lane] : make_float2(-INFINITY, 0.0f), y = lane + 32 < p.slices ? ms[lane + 32] : make_float2(-INFINITY, 0.0f);
+            const float2 none = make_float2(-INFINITY, 0.0f), x = lane < p.slices ? ms[b * p.slices + lane] : none, y = lane + 32 < p.slices ? ms[b * p.slices + lane + 32] : none;
             m = warp_max(fmaxf(x.x, y.x));
             if (!(x.x == -INFINITY && x.y == 0.0f)) s += x.y * expf(x.x - m);
             if (!(y.x == -INFINITY && y.y == 0.0f)) s += y.y * expf(y.x - m);
@@ -344,38 +359,23 @@ __global__ void __launch_bounds__(kSelThreads) beam_join_kernel(const __grid_con
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
-    auto value_of = [&](int i, float v, int token, auto f) {  // an index is (beam, token)
-        const int b = i / per, k = i - b * per;
-        if (p.done && p.done[row0 + b]) {
-            if (k == 0) f(offset[b], (long long)b << 32 | p.end_token);
-        } else if (token >= 0) {
-            f(offset[b] + (double)v, (long long)b << 32 | token);
-        }
-    };
-    auto visit = [&](auto f) {
+    auto visit = [&](auto f) {  // an index is (beam, token)
 #pragma unroll 1
-        for (int i = t; i < n; i += kSelThreads) value_of(i, p.part_v[row0 * per + i], p.part_i[row0 * per + i], f);
+        for (int i = t; i < n; i += kSelThreads) {
+            const float v = held ? sp.held_v[i] : p.part_v[row0 * per + i];
+            const int token = held ? sp.held_i[i] : p.part_i[row0 * per + i], b = i / per, k = i - b * per;
+            if (p.done && p.done[row0 + b]) {
+                if (k == 0) f(offset[b], (long long)b << 32 | p.end_token);
+            } else if (token >= 0) {
+                f(offset[b] + (double)v, (long long)b << 32 | token);
+            }
+        }
     };
     double top = -INFINITY;
-    auto higher = [&](double value, long long) { if (value > top) top = value; };
-    if (held) {
-#pragma unroll 1
-        for (int k = 0; k < kHeld; k++)
-            if (t + k * kSelThreads < n) value_of(t + k * kSelThreads, held_v[k * kSelThreads + t], held_i[k * kSelThreads + t], higher);
-    } else {
-        visit(higher);
-    }
+    visit([&](double value, long long) { if (value > top) top = value; });
     const double bound = best.bound(top, p.picks);
-    if (top >= bound && top > -INFINITY) {
-        auto collect = [&](double value, long long index) { if (value >= bound && value > -INFINITY) best.collect(value, index); };
-        if (held) {
-#pragma unroll 1
-            for (int k = 0; k < kHeld; k++)
-                if (t + k * kSelThreads < n) value_of(t + k * kSelThreads, held_v[k * kSelThreads + t], held_i[k * kSelThreads + t], collect);
-        } else {
-            visit(collect);
-        }
-    }
+    if (top >= bound && top > -INFINITY)
+        visit([&](double value, long long index) { if (value >= bound && value > -INFINITY) best.collect(value, index); });
     best.rank(p.picks, visit);
     for (int k = t; k < p.picks; k += kSelThreads) {
         const long long i = best.out_i[k], at = (long long)group * p.picks + k;
@@ -385,8 +385,57 @@ __global__ void __launch_bounds__(kSelThreads) beam_join_kernel(const __grid_con
     }
 }
 
+// grid (groups)
+__global__ void __launch_bounds__(kSelThreads) beam_join_kernel(const __grid_constant__ Select p) {
+    __shared__ JoinSpace sp;
+    pdl_trigger();
+    pdl_wait();
+    const int per = p.slices * p.picks, n = p.beams * per;
+    const long long row0 = (long long)blockIdx.x * p.beams;
+    if (n <= kHeld) {  // on its way while lse is computed
+        for (int i = threadIdx.x; i < n; i += kSelThreads) {
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(sp.held_v + i)), "l"(p.part_v + row0 * per + i) : "memory");
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(sp.held_i + i)), "l"(p.part_i + row0 * per + i) : "memory");
+        }
+    }
+    join_group(p, blockIdx.x, p.part_ms + row0 * p.slices, n <= kHeld, sp);
+}
+
+// Few beams over few elements: a cluster per group, a CTA per slice of a beam; the first one joins what it finds in the others' shared memory. One
+// launch, no scratch.
+constexpr int kSelCluster = 8, kSelClusterSlice = 32768;
+template <int DT>
+__global__ void __launch_bounds__(kSelThreads) beam_cluster_kernel(const __grid_constant__ Select p) {
+    __shared__ SliceSpace sp;
+    __shared__ JoinSpace js;
+    __shared__ float2 ms[kSelCluster];
+    pdl_trigger();
+    pdl_wait();
+    const int C = p.beams * p.slices, group = blockIdx.x / C, rank = blockIdx.x - group * C, beam = rank / p.slices;
+    const long long row = (long long)group * p.beams + beam;
+    if (!(p.done && p.done[row])) slice_best<DT>(p, row, rank - beam * p.slices, sp);
+    cluster_sync();
+    if (rank == 0) {
+        for (int i = threadIdx.x; i < C * p.picks; i += kSelThreads) {  // (what a finished beam's CTA holds is not looked at)
+            const int from = i / p.picks, k = i - from * p.picks;
+            js.held_v[i] = __uint_as_float(remote1(of_rank(sp.best.out_v + k, from)));
+            js.held_i[i] = (int)remote1(of_rank(sp.best.out_i + k, from));
+        }
+        if (threadIdx.x < C) ms[threadIdx.x] = remote2(of_rank(&sp.ms, threadIdx.x));
+        __syncthreads();
+    }
+    cluster_sync();  // nobody leaves while another reads what it has
+    if (rank == 0) join_group(p, group, ms, true, js);
+}
+
 // Slices of a row: as many as the GPU holds blocks of all rows at a time (a second wave of a few would cost as much as a full one), none below kSelLeast
 // elements.
+// Slices of a beam where a cluster takes a group, 0 where it does not.
+int cluster_slices(const Device *dev, int groups, int beams, int vocab) {
+    if (beams > kSelCluster) return 0;
+    const int n = std::max(1, std::min(kSelCluster / beams, (vocab + kSelLeast - 1) / kSelLeast));
+    return (vocab + n - 1) / n <= kSelClusterSlice && (long long)groups * beams * n <= 2ll * dev->sm_count ? n : 0;
+}
 int select_slices(const Device *dev, int groups, int beams, int vocab) {
     const long long rows = (long long)groups * beams;
     const long long want = (long long)kSelResident * dev->sm_count / rows, most = (vocab + kSelLeast - 1) / kSelLeast;
@@ -398,6 +447,7 @@ size_t select_bytes(long long rows, int slices, int picks) { return (size_t)rows
 }  // namespace im
 
 IM_EXPORT size_t im_cuda_beam_select_scratch_bytes(const im_device *dev, int groups, int beams, int vocab, int picks) {
+    if (dev && groups >= 1 && beams >= 1 && vocab >= 1 && im::cluster_slices(dev, groups, beams, vocab)) return 0;
     if (!dev || groups < 1 || beams < 1 || beams > im::kSelMost || vocab < 1 || picks < 1 || picks > im::kSelMost || (long long)groups * beams > 65535) return 0;
     return im::select_bytes((long long)groups * beams, im::select_slices(dev, groups, beams, vocab), picks);
 }
@@ -419,11 +469,13 @@ IM_EXPORT int im_cuda_beam_select(im_device *dev, const void *logits_dev, int dt
     if (rc != IM_OK) return rc;
     if (groups == 0) return IM_OK;
     Select p;
-    p.slices = select_slices(dev, groups, beams, vocab);
+    const int clustered = cluster_slices(dev, groups, beams, vocab);
+    p.slices = clustered ? clustered : select_slices(dev, groups, beams, vocab);
     p.slice = ((vocab + p.slices - 1) / p.slices + 7) / 8 * 8;
     const long long rows = (long long)groups * beams;
-    IM_REQUIRE(scratch_dev && aligned16(scratch_dev) && scratch_bytes >= select_bytes(rows, p.slices, picks), "beam selection needs %zu bytes of 16-byte aligned scratch (got %zu)",
-               select_bytes(rows, p.slices, picks), scratch_dev ? scratch_bytes : (size_t)0);
+    const size_t need = clustered ? 0 : select_bytes(rows, p.slices, picks);
+    IM_REQUIRE(need == 0 || (scratch_dev && aligned16(scratch_dev) && scratch_bytes >= need), "beam selection needs %zu bytes of 16-byte aligned scratch (got %zu)", need,
+               scratch_dev ? scratch_bytes : (size_t)0);
     p.x = logits_dev; p.stride = row_stride ? row_stride : vocab;
     p.groups = groups; p.beams = beams; p.vocab = vocab; p.picks = picks;
     p.score = score_dev; p.done = done_dev; p.end_token = end_token;
@@ -431,6 +483,11 @@ IM_EXPORT int im_cuda_beam_select(im_device *dev, const void *logits_dev, int dt
     p.part_ms = static_cast<float2 *>(scratch_dev);
     p.part_v = reinterpret_cast<float *>(p.part_ms + rows * p.slices);
     p.part_i = reinterpret_cast<int *>(p.part_v + rows * p.slices * picks);
+    if (clustered) {
+        void (*one)(Select) = dtype == IM_DTYPE_F32 ? beam_cluster_kernel<IM_DTYPE_F32> : dtype == IM_DTYPE_F16 ? beam_cluster_kernel<IM_DTYPE_F16> : beam_cluster_kernel<IM_DTYPE_BF16>;
+        IM_CUDA_CHECK(launch_cluster(one, dim3((unsigned)(rows * p.slices)), dim3(kSelThreads), beams * p.slices, 0, as_stream(stream), p));
+        return IM_OK;
+    }
     void (*kern)(Select) = dtype == IM_DTYPE_F32 ? beam_slice_kernel<IM_DTYPE_F32> : dtype == IM_DTYPE_F16 ? beam_slice_kernel<IM_DTYPE_F16> : beam_slice_kernel<IM_DTYPE_BF16>;
     IM_CUDA_CHECK(launch_k(kern, dim3(p.slices, (unsigned)rows), dim3(kSelThreads), 0, as_stream(stream), p));
     IM_CUDA_CHECK(launch_k(beam_join_kernel, dim3(groups), dim3(kSelThreads), 0, as_stream(stream), p));

@@ -15,6 +15,7 @@
 
 #include <algorithm>
 
+#include "cluster.cuh"
 #include "paged_attn.cuh"
 
 namespace im {
@@ -51,35 +52,6 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uin
 }
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool there) {  // zeros where there is no source
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t of_rank(const void *mine, uint32_t rank) {  // the same place in another CTA of the cluster
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(mine)), "r"(rank));
-    return a;
-}
-__device__ __forceinline__ float4 remote4(uint32_t at) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
-    return v;
-}
-__device__ __forceinline__ float2 remote2(uint32_t at) {
-    float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
-    return v;
 }
 
 // CL: instead of shares of the list of all tiles, a cluster of CTAs per item, each with an equal run of its tiles; they join what they have
@@ -526,20 +498,7 @@ int attn_launch(const Device *dev, const PagedAttn &p, int units, int cluster, c
         IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, true>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     }
     if (cluster) {
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3((unsigned)(units * p.kv.nkv * cluster));
-        cfg.blockDim = dim3(kPaThreads);
-        cfg.dynamicSmemBytes = S::kSmem;
-        cfg.stream = st;
-        cudaLaunchAttribute attr[2];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        attr[1].id = cudaLaunchAttributeClusterDimension;
-        attr[1].val.clusterDim.x = cluster;
-        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 2;
-        IM_CUDA_CHECK(cudaLaunchKernelEx(&cfg, paged_attn_kernel<BF16, HD, true>, p, units));
+        IM_CUDA_CHECK(launch_cluster(paged_attn_kernel<BF16, HD, true>, dim3((unsigned)(units * p.kv.nkv * cluster)), dim3(kPaThreads), cluster, (size_t)S::kSmem, st, p, units));
         return IM_OK;
     }
     IM_CUDA_CHECK(launch_k(paged_attn_kernel<BF16, HD, false>, dim3(p.ctas), dim3(kPaThreads), (size_t)S::kSmem, st, p, units));

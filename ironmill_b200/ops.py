@@ -574,11 +574,14 @@ def paged_reorder(kv: PagedKV, parents, group: int, table_out=None, lengths_out=
 # ---------------------------------------------------------------- beam search
 def beam_select_scratch(dev: Device, groups: int, beams: int, vocab: int, picks: int) -> torch.Tensor:
     """Scratch for beam_select calls of these sizes; calls that may overlap need one each."""
-    key = (groups, beams, vocab, picks)
+    return torch.empty(max(_select_bytes(dev, (groups, beams, vocab, picks)), 16), dtype=torch.uint8, device=dev.torch_device)
+
+
+def _select_bytes(dev: Device, key) -> int:
     nbytes = dev.select_bytes.get(key)
     if nbytes is None:
-        nbytes = dev.select_bytes[key] = max(int(lib().im_cuda_beam_select_scratch_bytes(dev.handle, *key)), 16)
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev.torch_device)
+        nbytes = dev.select_bytes[key] = int(lib().im_cuda_beam_select_scratch_bytes(dev.handle, *key))
+    return nbytes
 
 
 def beam_select(dev: Device, logits, scores, picks: int, done=None, end_token=-1, scratch=None):
@@ -593,13 +596,18 @@ def beam_select(dev: Device, logits, scores, picks: int, done=None, end_token=-1
     if done is not None:
         assert done.shape == (groups, beams) and done.dtype in (torch.bool, torch.uint8) and done.is_contiguous() and done.get_device() == on
         dp = done.data_ptr()
+    nbytes, at = 0, None
     if scratch is None:
-        scratch = beam_select_scratch(dev, groups, beams, vocab, picks)
+        nbytes = _select_bytes(dev, (groups, beams, vocab, picks))
+        if nbytes:
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev.torch_device)
+            at = scratch.data_ptr()
     else:
         assert scratch.dtype is torch.uint8 and scratch.get_device() == on and scratch.is_contiguous()
+        nbytes, at = scratch.numel(), scratch.data_ptr()
     score = scores.new_empty((groups, picks))
     parent = torch.empty_like(score, dtype=torch.int32)
     token = torch.empty_like(parent)
     _launch(on, lib().im_cuda_beam_select, dev.handle, logits.data_ptr(), _DTYPES[logits.dtype], (sb if beams > 1 else sg) if groups * beams > 1 else 0, groups, beams, vocab,
-            scores.data_ptr(), dp, end_token, picks, score.data_ptr(), parent.data_ptr(), token.data_ptr(), scratch.data_ptr(), scratch.numel())
+            scores.data_ptr(), dp, end_token, picks, score.data_ptr(), parent.data_ptr(), token.data_ptr(), at, nbytes)
     return score, parent, token

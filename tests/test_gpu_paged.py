@@ -486,7 +486,7 @@ def _check_select(dev, logits, scores, picks, done=None, end_token=-1):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
-@pytest.mark.parametrize("groups, beams, vocab, picks", [(1, 1, 1, 1), (1, 4, 7, 64), (3, 2, 500, 4), (2, 5, 2049, 10), (1, 8, 32768, 16), (40, 3, 1001, 3), (1, 64, 4096, 64), (2, 4, 151936, 8)])
+@pytest.mark.parametrize("groups, beams, vocab, picks", [(1, 1, 1, 1), (1, 4, 7, 64), (3, 2, 500, 4), (2, 5, 2049, 10), (1, 8, 32768, 16), (40, 3, 1001, 3), (60, 8, 700, 5), (1, 3, 90000, 6), (1, 7, 20011, 64), (5, 2, 65536, 2), (1, 64, 4096, 64), (2, 4, 151936, 8)])
 def test_selection(dev, dtype, groups, beams, vocab, picks):
     rng = H.rng_for("select", vocab + beams)
     _check_select(dev, _randn(rng, (groups, beams, vocab), dtype, 3.0), _randn(rng, (groups, beams), "f32", 2.0), picks)
@@ -714,7 +714,7 @@ def test_refusals_on_a_device(dev):
     with pytest.raises(CudaSysError, match="scratch"):
         ops.paged_attention(c.kv, 0, q, _ints([0, 1]), 1, 0.1, scratch=torch.empty(64, dtype=torch.uint8, device="cuda"))
     with pytest.raises(CudaSysError, match="scratch"):
-        ops.beam_select(dev, torch.zeros((1, 1, 10), device="cuda"), torch.zeros((1, 1), device="cuda"), 1, scratch=torch.empty(8, dtype=torch.uint8, device="cuda"))
+        ops.beam_select(dev, torch.zeros((1, 9, 10), device="cuda"), torch.zeros((1, 9), device="cuda"), 1, scratch=torch.empty(8, dtype=torch.uint8, device="cuda"))
     with pytest.raises(CudaSysError, match="layer"):
         ops.paged_append(c.kv, 1, q[:, :2].contiguous(), q[:, 2:].contiguous(), _ints([0, 1]))
     for call in (lambda: ops.paged_attention(c.kv, 0, q.bfloat16(), _ints([0, 1]), 1, 0.1), lambda: ops.paged_attention(c.kv, 0, q, _ints([0, 1, 2]), 1, 0.1),
