@@ -463,6 +463,7 @@ IM_EXPORT int im_cuda_beam_select(im_device *dev, const void *logits_dev, int dt
     IM_REQUIRE((long long)groups * beams <= 65535, "at most 65535 beams in all (got %lld)", (long long)groups * beams);
     IM_REQUIRE(row_stride == 0 || (row_stride >= vocab && row_stride <= (int64_t)1 << 40), "rows of logits overlap");
     IM_REQUIRE(groups == 0 || (logits_dev && score_dev && score_out_dev && parent_out_dev && token_out_dev), "a pointer is NULL");
+    IM_REQUIRE(!share_memory(score_out_dev, 4ll * groups * picks, score_dev, 4ll * groups * beams), "the new scores lie over the old ones");
     IM_REQUIRE(reinterpret_cast<uintptr_t>(logits_dev) % (dtype == IM_DTYPE_F32 ? 4 : 2) == 0, "logits are not aligned to their type");
     IM_REQUIRE(!done_dev || (end_token >= 0 && end_token < vocab), "end_token %d of %d", end_token, vocab);
     int rc = paged_device(dev);

@@ -27,6 +27,11 @@ struct PagedView {
     }
 };
 
+// Whether two arrays share memory; sizes in bytes.
+inline bool share_memory(const void *a, long long na, const void *b, long long nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
+}
 inline bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // Checks what the host can see of a cache and fills the kernels' view; layer < 0: all of them.

@@ -521,10 +521,14 @@ int attn_check(const im_paged_kv *kv, int num_heads, int max_new) {
 }  // namespace im
 
 IM_EXPORT size_t im_cuda_paged_attention_scratch_bytes(const im_device *dev, const im_paged_kv *kv, int num_heads, int max_new, int max_len) {
-    im::PagedView v;
-    if (!dev || im::paged_view(kv, 0, &v) != IM_OK || im::attn_check(kv, num_heads, max_new) != IM_OK) return 0;
-    if (max_len < 0) return 0;
-    return im::attn_plan(dev, v.nseq, v.nkv, v.hd, num_heads / v.nkv, max_new, im::attn_length(v, max_len)).bytes;
+    try {
+        im::PagedView v;
+        if (!dev || im::paged_view(kv, 0, &v) != IM_OK || im::attn_check(kv, num_heads, max_new) != IM_OK) return 0;
+        if (max_len < 0) return 0;
+        return im::attn_plan(dev, v.nseq, v.nkv, v.hd, num_heads / v.nkv, max_new, im::attn_length(v, max_len)).bytes;
+    } catch (...) {
+        return 0;
+    }
 }
 
 IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int layer, const void *q_dev, int64_t q_stride, void *out_dev, int64_t out_stride,
@@ -543,6 +547,7 @@ IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int
     const int64_t row = (int64_t)num_heads * kv->head_dim, most = (int64_t)1 << 40;
     IM_REQUIRE(q_stride >= row && out_stride >= row && q_stride <= most && out_stride <= most && q_stride % 8 == 0 && out_stride % 8 == 0 && aligned16(q_dev) && aligned16(out_dev),
                "rows of queries and outputs have to be 16-byte aligned and apart");
+    IM_REQUIRE(q_dev != out_dev, "the outputs lie over the queries");
     IM_REQUIRE(!mask_dev || (mask_words >= 1 && mask_words <= 1 << 20), "a mask of %d words a token", mask_words);
     IM_REQUIRE(scale == scale && scale - scale == 0.0f, "scale is not finite");
     rc = paged_device(dev);
@@ -561,6 +566,7 @@ IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int
     p.mask = mask_dev; p.mask_words = mask_words;
     p.nh = num_heads; p.group = num_heads / kv->num_kv_heads; p.tokens = num_tokens; p.max_new = max_new;
     p.scale2 = scale * 1.4426950408889634f;
+    if (p.scale2 == 0.0f) p.scale2 = 1e-30f;  // every position alike, without 0 * inf at the hidden ones
     p.row_tiles = plan.row_tiles;
     p.ctas = plan.ctas;
     // no more CTAs than tiles

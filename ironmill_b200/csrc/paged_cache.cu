@@ -317,11 +317,6 @@ __global__ void __launch_bounds__(kReorderThreads)
     }
 }
 
-bool overlap(const void *a, long long na, const void *b, long long nb) {  // ints
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return x < y + (uintptr_t)nb * 4 && y < x + (uintptr_t)na * 4;
-}
-
 }  // namespace
 }  // namespace im
 
@@ -391,7 +386,9 @@ IM_EXPORT int im_cuda_paged_keep(im_device *dev, const im_paged_kv *kv, const in
     if (rc != IM_OK) return rc;
     IM_REQUIRE(max_accept >= 1 && (v.nseq == 0 || (accepted_dev && count_dev && seq_len_out_dev)), "bad argument");
     IM_REQUIRE(kv->num_seqs <= 65535, "at most 65535 sequences (got %d)", kv->num_seqs);
-    IM_REQUIRE(!overlap(seq_len_out_dev, v.nseq, v.len, v.nseq), "the new lengths lie over the old ones");
+    IM_REQUIRE(!share_memory(seq_len_out_dev, 4ll * v.nseq, v.len, 4ll * v.nseq), "the new lengths lie over the old ones");
+    IM_REQUIRE(!share_memory(seq_len_out_dev, 4ll * v.nseq, count_dev, 4ll * v.nseq) && !share_memory(seq_len_out_dev, 4ll * v.nseq, accepted_dev, 4ll * v.nseq * max_accept),
+               "the new lengths lie over the accepted places");
     const long long cols = (long long)v.layers * 2 * v.nkv * (v.hd / 8);
     IM_REQUIRE(cols <= INT_MAX - kKeepThreads, "too many layers and heads");
     rc = paged_device(dev);
@@ -416,9 +413,13 @@ IM_EXPORT int im_cuda_paged_reorder(im_device *dev, const im_paged_kv *kv, const
     const int64_t stride = table_out_stride ? table_out_stride : v.width;
     IM_REQUIRE(stride >= v.width, "rows of the new page table overlap");
     if (v.nseq > 0) {
-        const long long old_n = (v.nseq - 1) * v.table_stride + v.width, new_n = (v.nseq - 1) * stride + v.width;
-        IM_REQUIRE(!overlap(table_out_dev, new_n, v.table, old_n) && !overlap(table_out_dev, new_n, v.len, v.nseq), "the new page table lies over the old one or the lengths");
-        IM_REQUIRE(!overlap(seq_len_out_dev, v.nseq, v.len, v.nseq) && !overlap(seq_len_out_dev, v.nseq, v.table, old_n), "the new lengths lie over the old ones or the page table");
+        const long long lens = 4ll * v.nseq, old_n = 4 * ((v.nseq - 1) * v.table_stride + v.width), new_n = 4 * ((v.nseq - 1) * stride + v.width);
+        IM_REQUIRE(!share_memory(table_out_dev, new_n, v.table, old_n) && !share_memory(table_out_dev, new_n, v.len, lens), "the new page table lies over the old one or the lengths");
+        IM_REQUIRE(!share_memory(seq_len_out_dev, lens, v.len, lens) && !share_memory(seq_len_out_dev, lens, v.table, old_n),
+                   "the new lengths lie over the old ones or the page table");
+        IM_REQUIRE(!share_memory(table_out_dev, new_n, parent_dev, lens) && !share_memory(seq_len_out_dev, lens, parent_dev, lens) &&
+                       !share_memory(table_out_dev, new_n, seq_len_out_dev, lens),
+                   "the new page table and lengths lie over the parents or each other");
     }
     rc = paged_device(dev);
     if (rc != IM_OK) return rc;

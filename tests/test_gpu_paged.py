@@ -323,7 +323,49 @@ def test_largest_values_and_scores_far_apart(dev):
     c.k *= 8
     _check_attention(dev, c, rng, [4], 8, "f16", scale=4.0)
     _check_attention(dev, c, rng, [4], 8, "f16", scale=-0.5)
-    got, _ = _check_attention(dev, c, rng, [4], 8, "f16", scale=0.0)
+    _check_attention(dev, c, rng, [4], 8, "f16", scale=0.0)
+    for nodes in (9, 40):           # the tensor cores' tiles, narrow and wide
+        c = Cache(dev, rng, [330], [290])
+        c.k *= 8
+        mask = _tree(rng, nodes)
+        for scale in (4.0, -0.5, 0.0):
+            _check_attention(dev, c, rng, [nodes], 8, "f16", scale=scale, mask=mask)
+            _check_attention(dev, c, rng, [nodes], 8, "f16", scale=scale)
+        c.v.copy_(torch.where(c.v > 0, 65504.0, -65504.0))
+        _check_attention(dev, c, rng, [nodes], 8, "f16", scale=4.0)
+
+
+@pytest.mark.parametrize("heads, new", [(2, 1), (2, 11), (40, 1)])
+@pytest.mark.parametrize("dim", [64, 256])
+def test_more_sequences_than_threads(dev, heads, new, dim):
+    """Shares of 700 sequences: places found in several rounds; nothing says that the contexts are short."""
+    rng = H.rng_for("many", heads + new)
+    n = 700
+    lengths = rng.integers(0, 150, n).tolist()
+    counts = [int(x) for x in rng.integers(0, new + 1, n)]
+    c = Cache(dev, rng, [a + b for a, b in zip(lengths, counts)] + [], lengths, kv_heads=1, dim=dim, page=32)
+    wide = np.concatenate([c.table, np.full((n, 60), -1)], 1)
+    c.kv.point_at(_ints(wide), _ints(lengths))
+    c.table = wide
+    _check_attention(dev, c, rng, counts, heads, "f16", max_len=0, max_new=new)
+
+
+@pytest.mark.parametrize("heads, nodes", [(8, 10), (16, 40)])
+def test_tensor_core_tiles_with_missing_pages_and_empty_rows(dev, heads, nodes):
+    rng = H.rng_for("tc-bad", nodes)
+    lengths = [200, 40, 0, 64]
+    c = Cache(dev, rng, [n + nodes for n in lengths], lengths, page=16)
+    c.table[0, 1], c.table[0, 12], c.table[1, 0], c.table[2, :] = 1 << 30, -7, 99999, -1
+    c.kv.point_at(_ints(c.table), _ints(lengths))
+    mask = np.concatenate([_tree(rng, nodes) for _ in lengths])
+    mask[3 * nodes + 2] = 0
+    got, _ = _check_attention(dev, c, rng, [nodes] * 4, heads, "f16", mask=mask)
+    assert (got[2 * nodes:3 * nodes] == 0).all()            # a sequence without any page
+    mask = np.zeros((nodes, 1), dtype=np.uint64)            # an empty cache, and nodes that see nothing but for one
+    mask[5] = 33
+    c = Cache(dev, rng, [nodes], [0])
+    got, _ = _check_attention(dev, c, rng, [nodes], heads, "f16", mask=mask)
+    assert (np.delete(got, 5, 0) == 0).all() and (got[5] != 0).all()
 
 
 @pytest.mark.parametrize("dtype, nodes", [("f16", 1), ("bf16", 26), ("bf16", 64)])

@@ -38,12 +38,12 @@ def _append(lib, kv, **more):
 
 
 def _attend(lib, kv, **more):
-    a = dict(dict(layer=0, q=PTR, qs=512, out=PTR, os=512, heads=4, start=PTR, n=3, max_new=1, mask=None, words=0, scale=0.1, max_len=0, scratch=PTR, size=1 << 30), **more)
+    a = dict(dict(layer=0, q=PTR, qs=512, out=5 * PTR, os=512, heads=4, start=PTR, n=3, max_new=1, mask=None, words=0, scale=0.1, max_len=0, scratch=PTR, size=1 << 30), **more)
     return lib.im_cuda_paged_attention(None, C.addressof(kv) if kv is not None else None, *a.values(), None)
 
 
 def _select(lib, **more):
-    a = dict(dict(x=PTR, dtype=1, stride=0, groups=2, beams=4, vocab=100, score=PTR, done=None, end=-1, picks=4, so=PTR, po=PTR, to=PTR, scratch=PTR, size=1 << 30), **more)
+    a = dict(dict(x=PTR, dtype=1, stride=0, groups=2, beams=4, vocab=100, score=PTR, done=None, end=-1, picks=4, so=5 * PTR, po=PTR, to=PTR, scratch=PTR, size=1 << 30), **more)
     return lib.im_cuda_beam_select(None, *a.values(), None)
 
 
@@ -56,8 +56,8 @@ def test_right_arguments_are_only_short_of_a_device(lib):
     assert _message(lib, _attend(lib, _kv())) == GOOD
     assert _message(lib, _select(lib)) == GOOD
     kv = _kv()
-    assert _message(lib, lib.im_cuda_paged_keep(None, C.addressof(kv), PTR, 4, PTR, PTR, None)) == GOOD
-    assert _message(lib, lib.im_cuda_paged_reorder(None, C.addressof(kv), PTR, 3, PTR, 0, PTR, None)) == GOOD
+    assert _message(lib, lib.im_cuda_paged_keep(None, C.addressof(kv), PTR, 4, PTR, 5 * PTR, None)) == GOOD
+    assert _message(lib, lib.im_cuda_paged_reorder(None, C.addressof(kv), PTR, 3, 5 * PTR, 0, 6 * PTR, None)) == GOOD
 
 
 @pytest.mark.parametrize("change, word", [
@@ -67,8 +67,8 @@ def test_right_arguments_are_only_short_of_a_device(lib):
     (dict(page_stride=4097), "strides"), (dict(layer_stride=4096), "overlap"), (dict(table_stride=3), "overlap"), (dict(num_pages=1 << 30, page_size=1 << 20, table_width=1), "shape")])
 def test_caches_that_are_refused(lib, change, word):
     kv = _kv(**change)
-    for call in (lambda: _append(lib, kv), lambda: _attend(lib, kv), lambda: lib.im_cuda_paged_keep(None, C.addressof(kv), PTR, 4, PTR, PTR, None),
-                 lambda: lib.im_cuda_paged_reorder(None, C.addressof(kv), PTR, 3, PTR, 0, PTR, None)):
+    for call in (lambda: _append(lib, kv), lambda: _attend(lib, kv), lambda: lib.im_cuda_paged_keep(None, C.addressof(kv), PTR, 4, PTR, 5 * PTR, None),
+                 lambda: lib.im_cuda_paged_reorder(None, C.addressof(kv), PTR, 3, 5 * PTR, 0, 6 * PTR, None)):
         assert word in _message(lib, call())
 
 
@@ -87,7 +87,7 @@ def test_appends_that_are_refused(lib, change, word):
 @pytest.mark.parametrize("change, word", [
     (dict(layer=2), "layer"), (dict(q=None), "bad argument"), (dict(max_len=-1), "bad argument"), (dict(heads=3), "multiple"), (dict(heads=0), "multiple"), (dict(max_new=0), "max_new"),
     (dict(qs=500), "queries"), (dict(os=8), "queries"), (dict(out=PTR + 8), "queries"), (dict(mask=PTR, words=0), "mask"), (dict(scale=float("nan")), "scale"),
-    (dict(scale=float("inf")), "scale"), (dict(max_new=1 << 30), "too many")])
+    (dict(scale=float("inf")), "scale"), (dict(out=PTR), "over the queries"), (dict(max_new=1 << 30), "too many")])
 def test_attention_that_is_refused(lib, change, word):
     assert word in _message(lib, _attend(lib, _kv(), **change))
 
@@ -100,7 +100,7 @@ def test_heads_that_attention_is_not_built_for(lib):
 @pytest.mark.parametrize("change, word", [
     (dict(dtype=3), "dtype"), (dict(beams=0), "beams"), (dict(beams=65), "beams"), (dict(vocab=0), "tokens"), (dict(groups=-1), "groups"), (dict(picks=0), "picks"), (dict(picks=65), "picks"),
     (dict(groups=40000), "65535"), (dict(stride=99), "overlap"), (dict(x=None), "NULL"), (dict(x=PTR + 2), "aligned"), (dict(done=PTR, end=100), "end_token"),
-    (dict(done=PTR, end=-1), "end_token"), (dict(so=None), "NULL")])
+    (dict(done=PTR, end=-1), "end_token"), (dict(so=None), "NULL"), (dict(so=PTR + 28), "old ones")])
 def test_selections_that_are_refused(lib, change, word):
     assert word in _message(lib, _select(lib, **change))
 
@@ -109,6 +109,10 @@ def test_results_may_not_lie_over_what_is_read(lib):
     kv = _kv()
     at = C.addressof(kv)
     assert "old ones" in _message(lib, lib.im_cuda_paged_keep(None, at, PTR, 4, PTR, 4 * PTR + 8, None))
+    assert "accepted" in _message(lib, lib.im_cuda_paged_keep(None, at, PTR, 4, 5 * PTR, PTR + 47, None))
+    assert "accepted" in _message(lib, lib.im_cuda_paged_keep(None, at, PTR, 4, 5 * PTR, 5 * PTR - 11, None))
+    assert "parents" in _message(lib, lib.im_cuda_paged_reorder(None, at, PTR, 3, 5 * PTR, 0, PTR + 8, None))
+    assert "each other" in _message(lib, lib.im_cuda_paged_reorder(None, at, PTR, 3, 5 * PTR, 0, 5 * PTR + 44, None))
     assert "old one" in _message(lib, lib.im_cuda_paged_reorder(None, at, PTR, 3, 3 * PTR + 16, 0, PTR, None))
     assert "old ones" in _message(lib, lib.im_cuda_paged_reorder(None, at, PTR, 3, PTR, 0, 4 * PTR, None))
     assert "groups of 2" in _message(lib, lib.im_cuda_paged_reorder(None, at, PTR, 2, PTR, 0, PTR, None))
