@@ -456,7 +456,7 @@ struct AttnPlan {
     int cluster;  // CTAs per item that join in the launch; 0: shares
     size_t bytes;
 };
-constexpr int kClusterMost = 8, kClusterTiles = 8;
+constexpr int kClusterMost = 8;
 AttnPlan attn_plan(const Device *dev, int nseq, int nkv, int hd, int group, int max_new, int max_len) {
     AttnPlan a;
     // Up to 16 rows of a KV head (and heads of 256, whose scores and outputs tensor memory does not hold twice) on mma.sync, more on tcgen05. Eight sequences of
@@ -468,10 +468,12 @@ AttnPlan attn_plan(const Device *dev, int nseq, int nkv, int hd, int group, int 
     a.row_tiles = (int)(((long long)group * max_new + a.rows - 1) / a.rows);
     a.units = nseq * a.row_tiles;
     a.ctas = dev->sm_count * (tc || hd == 256 ? 1 : 2);
-    // Contexts that a few CTAs per item read in a few tiles each: a cluster per item, one launch
+    // Contexts that the GPU's CTAs, as many for every item, read in up to 16 tiles each (8 where an item has eight CTAs and not all of the GPU's are used): a cluster
+    // per item, one launch. 32 sequences of up to 1000 rows 25 us, 33 in shares; of 2000 (32 tiles) 42 and 43, of 8192 140 and 102; one of 4000 (8 tiles for
+    // each of eight CTAs) 16.8 and 17.2, of 8000 24 and 20.
     const long long items = (long long)a.units * nkv, tiles = (max_len + (long long)kPaTile - 1) / kPaTile;
     a.cluster = (int)std::max(1ll, std::min({(long long)a.ctas / std::max(items, 1ll), tiles, (long long)kClusterMost}));
-    if (a.rows != 16 || tiles > (long long)kClusterTiles * a.cluster) a.cluster = 0;
+    if (a.rows != 16 || tiles > (a.cluster < kClusterMost ? 16ll : 8ll) * a.cluster) a.cluster = 0;
     if (a.cluster) {
         a.bytes = 0;
         return a;

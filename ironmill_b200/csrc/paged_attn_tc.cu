@@ -1,6 +1,6 @@
 // Attention over a paged cache on the 5th-generation tensor cores, for many rows (token, query head) of a KV head: trees and portions of prompts.
 //
-// One CTA per SM walks an equal share of the list of all (row tile, KV head) items' tiles of 128 positions (paged_attn.cu has the scheme and joins
+// One CTA per SM walks an equal share of the list of all (row tile, KV head) items' tiles of 128 positions (paged_attn.cu has the scheme; a second launch joins
 // what the cuts divide). Two sets of four warps ("halves") turn scores into weights, a row per thread; while one of them works, the other's products run:
 //     S = Q K^T    both operands in shared memory, accumulator in tensor memory (f32)
 //     P = exp2(S)  to registers, running maximum and sum in f32, weights back over the scores in 16 bits (up to 128 rows: as two terms, the weight and what
@@ -9,7 +9,7 @@
 // A tile of up to 256 rows (WIDE): the halves own 128 rows each and every tile of K and V serves both. Up to 128 rows: the halves own the even
 // and the odd tiles of the share, with accumulators of their own that are joined where the item ends. There the copies set the pace and the second
 // term of the weights is free; in a wide tile the chain of scores, weights and products does, and one term is what it takes: rounding a weight by half a
-// step (2^-9 bf16, 2^-12 fp16, relative) moves an output by what rounding the output itself does.
+// step (2^-8 bf16, 2^-11 fp16, relative) at most moves an output by what rounding the output itself does.
 // A row's accumulator is rescaled only when its maximum has grown by more than 2^8 (as in flash_tc.cu).
 //
 // K, V and queries come by 16-byte cp.async of four warps, rows looked up in the page table: any page size, rows that are not there are zeros and
