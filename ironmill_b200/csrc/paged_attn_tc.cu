@@ -586,58 +586,53 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     }
 }
 
-// Items that a cut divides: a warp per 32 rows and eight columns, a row per lane.
+// Items that a cut divides: a warp per 32 rows and four columns, a row per lane. Blocks are small enough to wait beside a CTA of the kernel above.
+constexpr int kTcJoinThreads = 128;
 template <bool BF16, int KB, bool WIDE>
-__global__ void __launch_bounds__(256) paged_tc_join_kernel(const __grid_constant__ PagedAttn p, int units) {
-    constexpr int R = TcShape<KB, WIDE>::kRows, HD = 64 * KB;
+__global__ void __launch_bounds__(kTcJoinThreads) paged_tc_join_kernel(const __grid_constant__ PagedAttn p, int units) {
+    constexpr int R = TcShape<KB, WIDE>::kRows, HD = 64 * KB, N = WIDE ? 8 : 4;  // N: parts that are requested together
     pdl_trigger();
     pdl_wait();
     const int item = blockIdx.x, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, lane = threadIdx.x & 31;
-    const int w = blockIdx.y * 8 + (threadIdx.x >> 5), r = w / (HD / 8) * 32 + lane, c = w % (HD / 8) * 8;
+    const int w = blockIdx.y * (kTcJoinThreads / 32) + (threadIdx.x >> 5), r = w / (HD / 4) * 32 + lane, c = w % (HD / 4) * 4;
     const int2 span = *reinterpret_cast<const int2 *>(p.spans + 2 * (long long)item);
     const PagedUnit u = paged_unit<R>(p, unit);
     if (r >= u.rows || span.x < 0) return;  // (a unit without tiles has no rows)
-    const size_t slot0 = span.x;
     const int first = span.x >> 1, parts = span.y - first + 1;
-    float M = -INFINITY, L = 0.0f, o[8];
-#pragma unroll
-    for (int j = 0; j < 8; j++) o[j] = 0.0f;
-    constexpr int kAtOnce = 4;  // parts that are requested together
+    float M = -INFINITY, L = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 1
-    for (int i0 = 0; i0 < parts; i0 += kAtOnce) {
-        float2 x[kAtOnce];
-        float4 v[kAtOnce], y[kAtOnce];
+    for (int i0 = 0; i0 < parts; i0 += N) {
+        float2 x[N];
+        float4 v[N];
 #pragma unroll
-        for (int i = 0; i < kAtOnce; i++) {
+        for (int i = 0; i < N; i++) {
             const int k = min(i0 + i, parts - 1);
-            const size_t slot = k == 0 ? slot0 : (size_t)(first + k) * 2;
+            const size_t slot = k == 0 ? (size_t)span.x : (size_t)(first + k) * 2;
             x[i] = p.part_ml[slot * R + r];
             v[i] = *reinterpret_cast<const float4 *>(tc_part<R>(p.part_o, slot, HD, r, c));
-            y[i] = *reinterpret_cast<const float4 *>(tc_part<R>(p.part_o, slot, HD, r, c + 4));
-            if (i0 + i >= parts) x[i] = make_float2(-INFINITY, 0.0f);
         }
         float top = M;
 #pragma unroll
-        for (int i = 0; i < kAtOnce; i++) top = fmaxf(top, x[i].x);
+        for (int i = 0; i < N; i++) {
+            if (i0 + i >= parts) x[i] = make_float2(-INFINITY, 0.0f);
+            top = fmaxf(top, x[i].x);
+        }
         const float corr = M == top ? 1.0f : ex2(M - top);
         M = top;
         L *= corr;
+        o = make_float4(o.x * corr, o.y * corr, o.z * corr, o.w * corr);
 #pragma unroll
-        for (int j = 0; j < 8; j++) o[j] *= corr;
-#pragma unroll
-        for (int i = 0; i < kAtOnce; i++) {
-            const bool none = x[i].x == -INFINITY && x[i].y == 0.0f;  // nothing seen in this part
-            const float f = none ? 0.0f : ex2(x[i].x - top);
+        for (int i = 0; i < N; i++) {
+            if (x[i].x == -INFINITY && x[i].y == 0.0f) continue;  // nothing seen in this part
+            const float f = ex2(x[i].x - top);
             L += x[i].y * f;
-            const float w[8] = {v[i].x, v[i].y, v[i].z, v[i].w, y[i].x, y[i].y, y[i].z, y[i].w};
-#pragma unroll
-            for (int j = 0; j < 8; j++) o[j] += none ? 0.0f : w[j] * f;
+            o.x += v[i].x * f; o.y += v[i].y * f; o.z += v[i].z * f; o.w += v[i].w * f;
         }
     }
     const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
     const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
-    *reinterpret_cast<uint4 *>(p.out + (u.tok0 + t) * p.os + (long long)(head * p.group + g) * HD + c) =
-        make_uint4(pack2<BF16>(o[0] * inv, o[1] * inv), pack2<BF16>(o[2] * inv, o[3] * inv), pack2<BF16>(o[4] * inv, o[5] * inv), pack2<BF16>(o[6] * inv, o[7] * inv));
+    *reinterpret_cast<uint2 *>(p.out + (u.tok0 + t) * p.os + (long long)(head * p.group + g) * HD + c) = make_uint2(pack2<BF16>(o.x * inv, o.y * inv), pack2<BF16>(o.z * inv, o.w * inv));
 }
 
 template <bool BF16, int KB, bool WIDE>
@@ -647,7 +642,8 @@ int tc_launch(const Device *dev, const PagedAttn &p, int units, cudaStream_t st)
     if (once.first(dev->ordinal)) IM_CUDA_CHECK(cudaFuncSetAttribute((paged_tc_kernel<BF16, KB, WIDE>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     IM_CUDA_CHECK(launch_k(paged_tc_kernel<BF16, KB, WIDE>, dim3(p.ctas), dim3(kTcThreads), (size_t)S::kSmem, st, p, units, dev->err_flag));
     const long long rows = std::min<long long>(S::kRows, (long long)p.max_new * p.group);
-    IM_CUDA_CHECK(launch_k(paged_tc_join_kernel<BF16, KB, WIDE>, dim3((unsigned)(units * p.kv.nkv), (unsigned)((rows + 31) / 32 * KB)), dim3(256), 0, st, p, units));
+    IM_CUDA_CHECK(launch_k(paged_tc_join_kernel<BF16, KB, WIDE>, dim3((unsigned)(units * p.kv.nkv), (unsigned)((rows + 31) / 32 * (16 * KB) / (kTcJoinThreads / 32))),
+                           dim3(kTcJoinThreads), 0, st, p, units));
     return IM_OK;
 }
 

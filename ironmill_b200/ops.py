@@ -478,7 +478,7 @@ def paged_append(kv: PagedKV, layer: int, k, v, token_start, q=None, cos=None, s
         heads = q.shape[1]
         qs, qp = _rows_of(q, n, heads, dim, dtype, on), q.data_ptr()
         if q_out is None:
-            q_out = q.new_empty((n, heads, dim))
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
             qos = heads * dim
         else:
             qos = _rows_of(q_out, n, heads, dim, dtype, on)
@@ -522,7 +522,7 @@ def paged_attention(kv: PagedKV, layer: int, q, token_start, max_new: int, scale
     on = kv.ordinal
     qs = _rows_of(q, n, heads, kv.head_dim, kv.dtype, on)
     if out is None:
-        out = q.new_empty((n, heads, dim))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         os_ = heads * dim
     else:
         os_ = _rows_of(out, n, heads, dim, kv.dtype, on)
