@@ -320,7 +320,7 @@ typedef struct im_paged_kv {
 
 /* Keys and values of new tokens into layer `layer`, the keys and (q_dev not NULL) the queries beside them rotated on the way.
  * k, v [num_tokens, num_kv_heads, head_dim], q, q_out [num_tokens, num_heads, head_dim], tokens *_stride elements apart (multiples of 8,
- * 16-byte aligned: parts of one row per token do); q_out may be q.  The first rotary_dim columns are rotated by the token's angles, f32 with one
+ * 16-byte aligned: parts of one row per token do); q_out may be q at the same stride and lies over nothing else that is read.  The first rotary_dim columns are rotated by the token's angles, f32 with one
  * rounding: columns (i, i + rotary_dim / 2), or with neighbours = 1 (2 i, 2 i + 1), by entry i of its row of cos / sin [max_pos, head_dim / 2]
  * (16-byte aligned; table_dtype IM_DTYPE_F16, as im_cuda_rope_table writes them, or IM_DTYPE_F32); the row is the token's row in the cache, or
  * position_dev [num_tokens] (nodes of a tree: their depth).  rotary_dim 0: nothing is rotated.  A token whose angle row is outside

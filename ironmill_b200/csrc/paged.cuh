@@ -32,6 +32,15 @@ inline bool share_memory(const void *a, long long na, const void *b, long long n
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
     return x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
 }
+// Whether n rows of `row` bytes, sa bytes apart from a on, share memory with such rows sb apart from b on. Rows of the same stride may lie between one
+// another; of others it is their whole span that counts.
+inline bool share_rows(const void *a, long long sa, const void *b, long long sb, long long row, long long n) {
+    const auto span = [&](long long stride) { return (n - 1 > (1ll << 60) / stride ? 1ll << 60 : (n - 1) * stride) + row; };
+    if (n < 1 || !share_memory(a, span(sa), b, span(sb))) return false;
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    const long long d = (long long)((x < y ? y - x : x - y) % (uintptr_t)sa);
+    return sa != sb || d < row || sa - d < row;
+}
 inline bool aligned16(const void *p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // Checks what the host can see of a cache and fills the kernels' view; layer < 0: all of them.

@@ -549,7 +549,7 @@ IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int
     const int64_t row = (int64_t)num_heads * kv->head_dim, most = (int64_t)1 << 40;
     IM_REQUIRE(q_stride >= row && out_stride >= row && q_stride <= most && out_stride <= most && q_stride % 8 == 0 && out_stride % 8 == 0 && aligned16(q_dev) && aligned16(out_dev),
                "rows of queries and outputs have to be 16-byte aligned and apart");
-    IM_REQUIRE(q_dev != out_dev, "the outputs lie over the queries");
+    IM_REQUIRE(!share_rows(q_dev, 2 * q_stride, out_dev, 2 * out_stride, 2 * row, num_tokens), "the outputs lie over the queries");
     IM_REQUIRE(!mask_dev || (mask_words >= 1 && mask_words <= 1 << 20), "a mask of %d words a token", mask_words);
     IM_REQUIRE(scale == scale && scale - scale == 0.0f, "scale is not finite");
     rc = paged_device(dev);

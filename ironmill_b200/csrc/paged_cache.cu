@@ -88,6 +88,7 @@ __device__ __forceinline__ void angles4(const void *table, long long at, float *
 // Blocks of 64 threads where there are many (8 x 1900 tokens of 48 heads: 59 us in blocks of 256, 51 of 128, 49 of 64), of 256 where a block more or less
 // costs nothing (32 tokens: 3.3 us, 6.4 in blocks of 64).
 constexpr int kAppendThreads = 256, kAppendSmall = 64;
+constexpr int kAppendMost = 1 << 20;  // heads of a call
 constexpr int kAppendHeads = 3;  // heads that a thread holds at a time
 
 template <bool BF16, int FORM, bool F32>
@@ -342,6 +343,9 @@ IM_EXPORT int im_cuda_paged_append(im_device *dev, const im_paged_kv *kv, int la
     IM_REQUIRE(!q_dev || (q_stride >= q_row && q_out_stride >= q_row && q_stride <= most && q_out_stride <= most && q_stride % 8 == 0 && q_out_stride % 8 == 0 &&
                           aligned16(q_dev) && aligned16(q_out_dev)),
                "rows of queries have to be 16-byte aligned and apart");
+    IM_REQUIRE(num_heads <= kAppendMost && kv->num_kv_heads <= kAppendMost, "%d and %d heads (at most %d)", num_heads, kv->num_kv_heads, kAppendMost);
+    IM_REQUIRE(!q_dev || (q_out_dev == q_dev && (q_out_stride == q_stride || num_tokens == 1)) || !share_rows(q_dev, 2 * q_stride, q_out_dev, 2 * q_out_stride, 2 * q_row, num_tokens),
+               "the rotated queries lie over other tokens' queries");
     IM_REQUIRE(rotary_dim >= 0 && rotary_dim <= kv->head_dim && rotary_dim % 2 == 0, "rotary_dim %d of %d", rotary_dim, kv->head_dim);
     IM_REQUIRE(rotary_dim == 0 || (cos_dev && sin_dev && max_pos > 0 && (table_dtype == IM_DTYPE_F16 || table_dtype == IM_DTYPE_F32)),
                "rotation needs tables of cosines and sines in fp16 or f32");

@@ -120,6 +120,22 @@ def test_results_may_not_lie_over_what_is_read(lib):
     assert "bad argument" in _message(lib, lib.im_cuda_paged_keep(None, at, PTR, 0, PTR, PTR, None))
 
 
+@pytest.mark.parametrize("change, word", [
+    (dict(qos=520), "other tokens"), (dict(qo=PTR + 1024), "other tokens"), (dict(q=PTR + 1024), "other tokens"), (dict(qs=1024, qos=1024, qo=PTR + 1008), "other tokens"),
+    (dict(qs=1024, qos=1024, qo=PTR + 2048 - 16), "other tokens"), (dict(qs=1024, qos=1024, qo=PTR + 1024), GOOD), (dict(qos=520, n=1), GOOD), (dict(qo=PTR + 3 * 1024 - 16), "other tokens"),
+    (dict(qo=PTR + 3 * 1024), GOOD), (dict(n=(1 << 31) - 1, qs=1 << 40, qos=1 << 40), GOOD), (dict(n=(1 << 31) - 1, qs=1 << 40, qos=(1 << 40) - 8), "other tokens"),
+    (dict(heads=1 << 21, qs=1 << 40, qos=1 << 40), "heads")])
+def test_rotated_queries_over_other_tokens_queries(lib, change, word):
+    assert word in _message(lib, _append(lib, _kv(), **change))
+
+
+@pytest.mark.parametrize("change, word", [
+    (dict(out=PTR + 1024), "over the queries"), (dict(q=PTR + 1024, out=PTR), "over the queries"), (dict(os=520, out=PTR + 16), "over the queries"),
+    (dict(qs=1024, os=1024, out=PTR + 1024), GOOD), (dict(qs=1024, os=1024, out=PTR + 1040), "over the queries"), (dict(qs=1024, os=1024, out=PTR + 1008), "over the queries")])
+def test_outputs_over_the_queries(lib, change, word):
+    assert word in _message(lib, _attend(lib, _kv(), **change))
+
+
 # ------------------------------------------------------------------------------------------------ the restatement itself
 def test_plain_reorder_by_hand():
     # beams with rows [0 0 | 0 .], pages of two: page 9 shared, last pages 0..2; children of beams 1, 1, 2: beam 0 is childless
