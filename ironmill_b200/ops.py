@@ -446,6 +446,7 @@ class PagedKV:
         layers, pages, heads, page, dim = k_pages.shape
         s = k_pages.stride()
         assert s[4] == 1 and (page == 1 or s[3] == dim) and (heads == 1 or s[2] == page * dim), s
+        assert (layers == 1 or s[0] > 0) and (pages == 1 or s[1] > 0), s  # an expanded axis would be taken for a packed one
         self.dev, self.k_pages, self.v_pages, self.ordinal = dev, k_pages, v_pages, dev.ordinal
         self.device, self.dtype, self.kv_heads, self.head_dim, self.layers = k_pages.device, k_pages.dtype, heads, dim, layers
         self.struct = PagedKvStruct(k_pages.data_ptr(), v_pages.data_ptr(), s[0] if layers > 1 else 0, s[1] if pages > 1 else 0, layers, pages, heads, page, dim,
@@ -457,7 +458,7 @@ class PagedKV:
         """Another page table and other lengths, as paged_keep and paged_reorder return them."""
         assert page_table.dim() == 2 and page_table.dtype == torch.int32 and page_table.device == self.device
         n, width = page_table.shape
-        assert n == 0 or width == 1 or page_table.stride(1) == 1, page_table.stride()
+        assert (n == 0 or width == 1 or page_table.stride(1) == 1) and (n <= 1 or page_table.stride(0) >= width), page_table.stride()
         self.struct.seq_len_dev = _ints(lengths, self.ordinal, n)
         self.struct.num_seqs, self.struct.page_table_dev, self.struct.table_width = n, page_table.data_ptr(), width
         self.struct.table_stride = page_table.stride(0) if n > 1 else 0
@@ -564,6 +565,7 @@ def paged_reorder(kv: PagedKV, parents, group: int, table_out=None, lengths_out=
         table_out, stride = kv.page_table.new_empty((n, width)), width
     else:
         assert table_out.shape == (n, width) and table_out.dtype is torch.int32 and table_out.get_device() == on and (n == 0 or width == 1 or table_out.stride(1) == 1)
+        assert n <= 1 or table_out.stride(0) >= width, table_out.stride()
         stride = table_out.stride(0) if n > 1 else 0
     if lengths_out is None:
         lengths_out = torch.empty_like(kv.lengths)
@@ -591,6 +593,8 @@ def beam_select(dev: Device, logits, scores, picks: int, done=None, end_token=-1
     groups, beams, vocab = logits.shape
     on, (sg, sb, sv) = dev.ordinal, logits.stride()
     assert logits.get_device() == on and (sv == 1 or vocab == 1) and (groups == 1 or beams == 1 or sg == beams * sb), logits.stride()
+    stride = (sb if beams > 1 else sg) if groups * beams > 1 else 0
+    assert groups * beams <= 1 or stride >= vocab, logits.stride()  # rows in common would be taken for packed ones
     assert scores.shape == (groups, beams) and scores.dtype is torch.float32 and scores.is_contiguous() and scores.get_device() == on
     dp = None
     if done is not None:
@@ -608,6 +612,6 @@ def beam_select(dev: Device, logits, scores, picks: int, done=None, end_token=-1
     score = scores.new_empty((groups, picks))
     parent = torch.empty_like(score, dtype=torch.int32)
     token = torch.empty_like(parent)
-    _launch(on, lib().im_cuda_beam_select, dev.handle, logits.data_ptr(), _DTYPES[logits.dtype], (sb if beams > 1 else sg) if groups * beams > 1 else 0, groups, beams, vocab,
+    _launch(on, lib().im_cuda_beam_select, dev.handle, logits.data_ptr(), _DTYPES[logits.dtype], stride, groups, beams, vocab,
             scores.data_ptr(), dp, end_token, picks, score.data_ptr(), parent.data_ptr(), token.data_ptr(), at, nbytes)
     return score, parent, token

@@ -764,3 +764,23 @@ def test_refusals_on_a_device(dev):
                  lambda: ops.paged_keep(c.kv, _ints([[0]]), _ints([0, 0])), lambda: c.kv.point_at(c.kv.page_table, _ints([1, 2]))):
         with pytest.raises(AssertionError):
             call()
+
+
+def test_expanded_tensors_are_refused(dev):
+    """A stride of zero means packed to the kernels: an axis that a caller has expanded must not reach them."""
+    from ironmill_b200 import ops
+    rng = H.rng_for("expanded")
+    c = Cache(dev, rng, [40, 40, 40, 40], [20, 20, 20, 20], layers=2)
+    row, scores = torch.zeros((1, 1, 100), device="cuda"), torch.zeros((2, 4), device="cuda")
+    parents = _ints([0, 0, 0, 0])
+    shared = c.kv.page_table[:1].expand(4, -1)
+    for call in (lambda: ops.beam_select(dev, row.expand(2, 4, 100), scores, 4), lambda: ops.beam_select(dev, row.expand(1, 4, 100), scores[:1], 4),
+                 lambda: ops.beam_select(dev, row.expand(2, 1, 100), scores[:, :1].contiguous(), 4), lambda: c.kv.point_at(shared, c.kv.lengths),
+                 lambda: ops.PagedKV(dev, c.k[:1].expand(2, -1, -1, -1, -1), c.v[:1].expand(2, -1, -1, -1, -1), c.kv.page_table, c.kv.lengths),
+                 lambda: ops.PagedKV(dev, c.k[:, :1].expand(-1, 9, -1, -1, -1), c.v[:, :1].expand(-1, 9, -1, -1, -1), c.kv.page_table, c.kv.lengths),
+                 lambda: ops.paged_reorder(c.kv, parents, 4, table_out=_ints([[0] * shared.shape[1]]).expand(4, -1))):
+        with pytest.raises(AssertionError):
+            call()
+    assert c.kv.num_seqs == 4 and c.kv.struct.table_width == shared.shape[1]
+    want = ops.beam_select(dev, row.expand(2, 4, 100).contiguous(), scores, 4)  # what the caller writes instead
+    assert want[1].tolist() == [[0, 0, 0, 0]] * 2 and want[2].tolist() == [[0, 1, 2, 3]] * 2
