@@ -152,6 +152,7 @@ __device__ __forceinline__ Share find_share(const PagedAttn &p, int units, long 
     s.head = found[1];
     s.tile = found[2];
     at = paged_unit<R>(p, s.unit);
+    __syncthreads();  // everyone has read found[]: `sums` may lie where the caller's warps, not all at a time, write next
     return s;
 }
 

@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     pdl_trigger();  // after the allocation: a successor on this SM cannot take the columns first
     pdl_wait();
     PagedUnit at;
-    const Share share = units <= 32 ? warp_share<R, kTcTile>(p, units, at) : find_share<R, kTcTile, kTcThreads>(p, units, reinterpret_cast<long long *>(Qs), at);  // (no copy is under way yet)
+    const Share share = units <= 32 ? warp_share<R, kTcTile>(p, units, at) : find_share<R, kTcTile, kTcThreads>(p, units, reinterpret_cast<long long *>(Qs), at);  // (the copies start behind its last barrier)
     Items<R> it(p, units, share, at);
     bool ok = true;
     if (warp >= kTcCopy) {

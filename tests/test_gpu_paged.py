@@ -784,3 +784,17 @@ def test_expanded_tensors_are_refused(dev):
     assert c.kv.num_seqs == 4 and c.kv.struct.table_width == shared.shape[1]
     want = ops.beam_select(dev, row.expand(2, 4, 100).contiguous(), scores, 4)  # what the caller writes instead
     assert want[1].tolist() == [[0, 0, 0, 0]] * 2 and want[2].tolist() == [[0, 1, 2, 3]] * 2
+
+
+# ------------------------------------------------------------------------------------------------ many units on the tensor cores
+@pytest.mark.parametrize("seqs, heads, kv_heads, dim, dtype, most", [
+    (40, 8, 2, 128, "f16", 10), (40, 12, 1, 128, "bf16", 40), (45, 16, 2, 64, "f16", 33), (37, 24, 1, 64, "bf16", 5), (450, 20, 1, 128, "f16", 2), (430, 132, 1, 64, "bf16", 2)])
+def test_tensor_core_tiles_of_more_units_than_a_warp_has_lanes(dev, seqs, heads, kv_heads, dim, dtype, most):
+    """Narrow and wide tiles of more units than a warp has lanes, and than a block has threads; some sequences have no new token."""
+    rng = H.rng_for("units", seqs + heads)
+    lengths = rng.integers(0, 300, seqs).tolist()
+    new = [most, *(int(x) for x in rng.integers(0, most + 1, seqs - 1))]
+    c = Cache(dev, rng, [a + b for a, b in zip(lengths, new)], lengths, kv_heads=kv_heads, dim=dim, page=24, dtype=dtype)
+    first = _check_attention(dev, c, H.rng_for("units-q"), new, heads, dtype)[0]
+    for _ in range(3):
+        assert (_check_attention(dev, c, H.rng_for("units-q"), new, heads, dtype)[0] == first).all()
