@@ -479,7 +479,7 @@ AttnPlan attn_plan(const Device *dev, int nseq, int nkv, int hd, int group, int 
         return a;
     }
     const size_t slots = (size_t)a.ctas * 2 * a.rows;
-    a.bytes = slots * hd * 4 + slots * 8 + (size_t)items * 8;
+    a.bytes = slots * hd * 4 + slots * 8 + (size_t)items * (tc ? 40 : 8);
     return a;
 }
 
@@ -578,6 +578,7 @@ IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int
     p.part_o = static_cast<float *>(scratch_dev);
     p.part_ml = reinterpret_cast<float2 *>(p.part_o + slots * p.kv.hd);
     p.spans = reinterpret_cast<int *>(p.part_ml + slots);
+    p.odd = reinterpret_cast<unsigned *>(p.spans + 2ll * plan.units * p.kv.nkv);
     const cudaStream_t st = as_stream(stream);
     const bool bf16 = kv->dtype == IM_DTYPE_BF16;
     if (plan.rows >= 128) return paged_tc_launch(dev, p, bf16, plan.rows, plan.units, st);

@@ -20,6 +20,7 @@ struct PagedAttn {
     float *part_o;            // [ctas, 2, rows of a tile, head_dim]: sums of weighted values
     float2 *part_ml;          // [ctas, 2, rows of a tile]: maximum, sum of weights
     int *spans;               // [units, KV heads, 2]: the slot of an item's first part (-1: one CTA had all of it), the CTA of its last one
+    unsigned *odd;            // tcgen05: [units, KV heads, 8]: rows of an item that one CTA had whose sums are not finite (rows of parts: a NaN in part_ml)
 };
 
 // A unit: a tile of rows (token, query head of the KV head) of one sequence, rows token-major.
@@ -194,27 +195,60 @@ __device__ __forceinline__ Share warp_share(const PagedAttn &p, int units, Paged
 }
 
 // A row whose sums are not finite, from the positions it sees alone: on the tensor cores a weight of zero times an infinite or missing value of a
-// position that the row does not see is a NaN. A warp per row; o: this lane's columns (lane, lane + 32, ...).
+// position that the row does not see is a NaN. A warp, 32 positions at a time, one a lane for the scores; o: this lane's columns (lane, lane + 32, ...).
 template <bool BF16, int HD>
 __device__ __noinline__ void plain_row(const PagedAttn &p, const PagedUnit &u, int head, int r, int from, int to, float *o, float &m, float &l) {
     const int lane = threadIdx.x & 31, t = (u.row0 + r) / p.group, h = head * p.group + (u.row0 + r) % p.group;
     const uint16_t *q = p.q + (u.tok0 + t) * p.qs + (long long)h * HD;
+    const uint16_t *kc = p.kc + (long long)head * p.kv.page * HD, *vc = p.vc + (long long)head * p.kv.page * HD + lane;
     m = -INFINITY;
     l = 0.0f;
+#pragma unroll
     for (int i = 0; i < HD / 32; i++) o[i] = 0.0f;
-    for (int pos = from; pos < to; pos++) {
-        if (!paged_sees(p, u, t, pos)) continue;
-        long long at = p.kv.row_of(u.seq, pos);
-        if (at < 0) continue;
-        at += (long long)head * p.kv.page * HD;
-        float s = 0.0f;
-        for (int i = 0; i < HD / 32; i++) s = fmaf(one16<BF16>(q + lane + 32 * i), one16<BF16>(p.kc + at + lane + 32 * i), s);
-        s = warp_sum(s) * p.scale2;
-        if (s == -INFINITY) continue;
-        const float m_new = fmaxf(m, s), corr = ex2(m - m_new), w = ex2(s - m_new);
+#pragma unroll 1
+    for (int left = to - from; left > 0; left -= 32) {
+        const int pos = to - left + lane;
+        const long long at = lane < left && paged_sees(p, u, t, pos) ? p.kv.row_of(u.seq, pos) : -1;
+        float s = -INFINITY;
+        if (at >= 0) {
+            float d = 0.0f;
+#pragma unroll 4
+            for (int c = 0; c < HD; c += 8) {
+                const uint4 a = *reinterpret_cast<const uint4 *>(q + c), b = *reinterpret_cast<const uint4 *>(kc + at + c);
+                const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float2 f = unpack16<BF16>(x[j]), g = unpack16<BF16>(y[j]);
+                    d = fmaf(f.x, g.x, d);
+                    d = fmaf(f.y, g.y, d);
+                }
+            }
+            s = d * p.scale2;
+        }
+        const unsigned seen = __ballot_sync(0xffffffffu, !(s == -INFINITY));
+        if (seen == 0) continue;
+        const float m_new = fmaxf(m, warp_max(s)), corr = m == m_new ? 1.0f : ex2(m - m_new), w = s == -INFINITY ? 0.0f : ex2(s - m_new);
         m = m_new;
-        l = l * corr + w;
-        for (int i = 0; i < HD / 32; i++) o[i] = fmaf(w, one16<BF16>(p.vc + at + lane + 32 * i), o[i] * corr);
+        l = l * corr + warp_sum(w);
+#pragma unroll
+        for (int i = 0; i < HD / 32; i++) o[i] *= corr;
+#pragma unroll 1
+        for (int j0 = 0; j0 < 32; j0 += 4) {
+            if (!(seen >> j0 & 15u)) continue;
+            float x[4][HD / 32];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const long long from_row = __shfl_sync(0xffffffffu, at, j0 + j);
+#pragma unroll
+                for (int i = 0; i < HD / 32; i++) x[j][i] = seen >> (j0 + j) & 1u ? one16<BF16>(vc + from_row + 32 * i) : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float f = __shfl_sync(0xffffffffu, w, j0 + j);
+#pragma unroll
+                for (int i = 0; i < HD / 32; i++) o[i] = fmaf(f, x[j][i], o[i]);
+            }
+        }
     }
 }
 

@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     uint64_t *kfull = reinterpret_cast<uint64_t *>(offs + kTcCopyWarps * 32), *kempty = kfull + SK, *vfull = kempty + SK, *vempty = vfull + SV, *qfull = vempty + SV,
              *qempty = qfull + 1, *sfull = qempty + 1, *pfull = sfull + 2, *ofull = pfull + 4, *oempty = ofull + 2;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(oempty + 2);
-    uint32_t *odd_rows = tmem_slot + 1;  // [8 warps]
+    uint32_t *odd_rows = tmem_slot + 1;  // [4 warps]
     // (shared memory starts at a multiple of 1024: checked, the tiles would not fit otherwise)
     unsigned char *Qs = tc_smem + (Shape::kSmem - Shape::kTiles), *Ks = Qs + Shape::kQ, *Vs = Ks + SK * Shape::kSlot;
     if (smem_u32(Qs) % 1024 != 0) {
@@ -552,29 +552,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                         for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(tc_part<R>(p.part_o, slot, HD, R_, c + j)) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
                     }
                 }
-                if (live && !whole && (WIDE || h == 0)) p.part_ml[slot * R + R_] = make_float2(m, l);
             }
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&oempty[h]);
+            // Rows whose sums are not finite are noted and left to the joining launch: nothing here waits for them
             unsigned bad = __ballot_sync(0xffffffffu, live && !(worst == 0.0f));
-            if constexpr (!WIDE) {  // the first half's warps see to the rows that either found
-                if (lane == 0) odd_rows[warp] = bad;
+            if constexpr (!WIDE) {  // the first half's warps note what either found
+                if (h && lane == 0) odd_rows[warp & 3] = bad;
                 both_halves();
-                bad = h ? 0u : bad | odd_rows[warp + 4];
+                if (!h) bad |= odd_rows[warp];
             }
-            while (bad) {
-                const int b = __ffs(bad) - 1, row = WIDE ? h * 128 + (warp & 3) * 32 + b : (warp & 3) * 32 + b;
-                bad &= bad - 1;
-                float x[HD / 32], M, L;
-                plain_row<BF16, HD>(p, u, it.head, row, it.t0 * kTcTile, min(it.t1 * kTcTile, u.end), x, M, L);
-                const float n = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
-                uint16_t *to_row = p.out + (u.tok0 + (u.row0 + row) / p.group) * p.os + (long long)(it.head * p.group + (u.row0 + row) % p.group) * HD;
-                for (int i = 0; i < HD / 32; i++) {
-                    if (whole) to_row[lane + 32 * i] = (uint16_t)pack2<BF16>(x[i] * n, 0.0f);
-                    else *tc_part<R>(p.part_o, slot, HD, row, lane + 32 * i) = x[i];
-                }
-                if (!whole && lane == 0) p.part_ml[slot * R + row] = make_float2(M, L);
+            if (WIDE || h == 0) {
+                if (whole && lane == 0) p.odd[((long long)it.unit * p.kv.nkv + it.head) * 8 + warp] = bad;
+                if (live && !whole) p.part_ml[slot * R + R_] = make_float2(m, bad >> lane & 1u ? NAN : l);
             }
         }
     }
@@ -586,19 +577,38 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     }
 }
 
-// Items that a cut divides: a warp per 32 rows and four columns, a row per lane. Blocks are small enough to wait beside a CTA of the kernel above.
-constexpr int kTcJoinThreads = 128;
-template <bool BF16, int KB, bool WIDE>
-__global__ void __launch_bounds__(kTcJoinThreads) paged_tc_join_kernel(const __grid_constant__ PagedAttn p, int units) {
-    constexpr int R = TcShape<KB, WIDE>::kRows, HD = 64 * KB, N = WIDE ? 8 : 4;  // N: parts that are requested together
-    pdl_trigger();
-    pdl_wait();
-    const int item = blockIdx.x, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, lane = threadIdx.x & 31;
-    const int w = blockIdx.y * (kTcJoinThreads / 32) + (threadIdx.x >> 5), r = w / (HD / 4) * 32 + lane, c = w % (HD / 4) * 4;
-    const int2 span = *reinterpret_cast<const int2 *>(p.spans + 2 * (long long)item);
-    const PagedUnit u = paged_unit<R>(p, unit);
-    if (r >= u.rows || span.x < 0) return;  // (a unit without tiles has no rows)
-    const int first = span.x >> 1, parts = span.y - first + 1;
+// A row of an item from the positions it sees alone, by a block: a warp per quarter of them.
+constexpr int kTcJoinThreads = 128, kTcJoinWarps = kTcJoinThreads / 32;
+template <bool BF16, int HD>
+__device__ __noinline__ void repair_row(const PagedAttn &p, const PagedUnit &u, int head, int r, float (*sums)[HD], float2 *ml) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long per = ((long long)u.end + 32 * kTcJoinWarps - 1) / (32 * kTcJoinWarps) * 32;
+    float o[HD / 32], m, l;
+    plain_row<BF16, HD>(p, u, head, r, (int)min((long long)u.end, warp * per), (int)min((long long)u.end, (warp + 1) * per), o, m, l);
+#pragma unroll
+    for (int i = 0; i < HD / 32; i++) sums[warp][lane + 32 * i] = o[i];
+    if (lane == 0) ml[warp] = make_float2(m, l);
+    __syncthreads();
+    float M = -INFINITY, L = 0.0f, x = 0.0f;
+    for (int w = 0; w < kTcJoinWarps; w++) M = fmaxf(M, ml[w].x);
+    const int c = threadIdx.x % HD;
+    for (int w = 0; w < kTcJoinWarps; w++) {
+        if (ml[w].x == -INFINITY && ml[w].y == 0.0f) continue;  // nothing seen there
+        const float f = ex2(ml[w].x - M);
+        L += ml[w].y * f;
+        x += sums[w][c] * f;
+    }
+    const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
+    const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
+    if (threadIdx.x < HD) p.out[(u.tok0 + t) * p.os + (long long)(head * p.group + g) * HD + c] = (uint16_t)pack2<BF16>(x * inv, 0.0f);
+    __syncthreads();
+}
+
+// Four columns of row r of an item that a cut divides. Returns the lanes whose rows are not finite: those are not written.
+template <bool BF16, int HD, int R, int N>
+__device__ __forceinline__ unsigned join_parts(const PagedAttn &p, const PagedUnit &u, int2 span, int head, int r, int c) {
+    const bool live = r < u.rows;
+    const int first = span.x >> 1, parts = span.y - first + 1, at = min(r, u.rows - 1);
     float M = -INFINITY, L = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 1
@@ -609,8 +619,8 @@ __global__ void __launch_bounds__(kTcJoinThreads) paged_tc_join_kernel(const __g
         for (int i = 0; i < N; i++) {
             const int k = min(i0 + i, parts - 1);
             const size_t slot = k == 0 ? (size_t)span.x : (size_t)(first + k) * 2;
-            x[i] = p.part_ml[slot * R + r];
-            v[i] = *reinterpret_cast<const float4 *>(tc_part<R>(p.part_o, slot, HD, r, c));
+            x[i] = p.part_ml[slot * R + at];
+            v[i] = *reinterpret_cast<const float4 *>(tc_part<R>(p.part_o, slot, HD, at, c));
         }
         float top = M;
 #pragma unroll
@@ -630,9 +640,34 @@ __global__ void __launch_bounds__(kTcJoinThreads) paged_tc_join_kernel(const __g
             o.x += v[i].x * f; o.y += v[i].y * f; o.z += v[i].z * f; o.w += v[i].w * f;
         }
     }
-    const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
+    const unsigned bad = __ballot_sync(0xffffffffu, live && L != L);
+    if (!live || L != L) return bad;
+    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
     const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
     *reinterpret_cast<uint2 *>(p.out + (u.tok0 + t) * p.os + (long long)(head * p.group + g) * HD + c) = make_uint2(pack2<BF16>(o.x * inv, o.y * inv), pack2<BF16>(o.z * inv, o.w * inv));
+    return bad;
+}
+
+// Items that a cut divides: a warp per 32 rows and four columns, a row per lane. Blocks are small enough to wait beside a CTA of the kernel above.
+// Rows that it has noted as not finite, of any item, are done again: the blocks of 32 rows share them. (In the kernel above, where a warp had them one
+// after the other at 1.4 us a position, other warps ran out of patience. 32 rows of each of 128 items over 1000 positions: 45 ms there, 0.8 here.)
+template <bool BF16, int KB, bool WIDE>
+__global__ void __launch_bounds__(kTcJoinThreads) paged_tc_join_kernel(const __grid_constant__ PagedAttn p, int units) {
+    constexpr int R = TcShape<KB, WIDE>::kRows, HD = 64 * KB, N = WIDE ? 8 : 4;  // N: parts that are requested together
+    constexpr int kBlocks = HD / 4 / kTcJoinWarps;  // of the same 32 rows
+    __shared__ float sums[kTcJoinWarps][HD];
+    __shared__ float2 ml[kTcJoinWarps];
+    pdl_trigger();
+    pdl_wait();
+    const int item = blockIdx.x, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, lane = threadIdx.x & 31;
+    const int rows = blockIdx.y / kBlocks, r = rows * 32 + lane, c = (blockIdx.y % kBlocks * kTcJoinWarps + (threadIdx.x >> 5)) * 4;
+    const int2 span = *reinterpret_cast<const int2 *>(p.spans + 2 * (long long)item);
+    const PagedUnit u = paged_unit<R>(p, unit);
+    if (rows * 32 >= u.rows) return;  // (a unit without tiles has no rows)
+    unsigned bad = span.x < 0 ? p.odd[(long long)item * 8 + rows] : join_parts<BF16, HD, R, N>(p, u, span, head, r, c);
+#pragma unroll 1
+    for (int n = 0; bad; n++, bad &= bad - 1)
+        if (n % kBlocks == blockIdx.y % kBlocks) repair_row<BF16, HD>(p, u, head, rows * 32 + __ffs(bad) - 1, sums, ml);
 }
 
 template <bool BF16, int KB, bool WIDE>

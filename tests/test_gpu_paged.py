@@ -798,3 +798,61 @@ def test_tensor_core_tiles_of_more_units_than_a_warp_has_lanes(dev, seqs, heads,
     first = _check_attention(dev, c, H.rng_for("units-q"), new, heads, dtype)[0]
     for _ in range(3):
         assert (_check_attention(dev, c, H.rng_for("units-q"), new, heads, dtype)[0] == first).all()
+
+
+# ------------------------------------------------------------------------------------------------ rows that are not finite, beside others
+def _exact(kv, seq, q, scale, mask):
+    """Attention of a sequence's new tokens q [new, heads, dim] in 64 bits on the GPU, with the sums that bounds on rounding need: (out, mass, dot)."""
+    k, v = kv.k_pages[0], kv.v_pages[0]
+    new, heads, dim = q.shape
+    before, page, nkv = int(kv.lengths[seq]), k.shape[2], k.shape[1]
+    row = torch.arange(before + new, device="cuda")
+    at = kv.page_table[seq].long()[row // page]
+    sees = torch.ones((new, before + new), dtype=torch.bool, device="cuda")
+    sees[:, before:] = (mask[:, None, 0] >> torch.arange(new, device="cuda")) & 1 == 1
+    out, mass, dot = (torch.zeros(s, dtype=torch.float64, device="cuda") for s in (q.shape, q.shape, q.shape[:2]))
+    for h in range(heads):
+        kk, vv = (x[at, h * nkv // heads, row % page].double() for x in (k, v))
+        x = (q[:, h].double() @ torch.where(sees.any(0)[:, None], kk, 0.0).T * scale).masked_fill(~sees, -np.inf)
+        w = torch.softmax(x, 1)
+        vv = torch.where(sees.any(0)[:, None], vv, 0.0)
+        out[:, h], mass[:, h] = w @ vv, w @ vv.abs()
+        dot[:, h] = (q[:, h].double().abs() @ torch.where(sees.any(0)[:, None], kk, 0.0).abs().T).masked_fill(~sees, 0.0).amax(1) * scale
+    return [_np(x) for x in (out, mass, dot)]
+
+
+@pytest.mark.parametrize("seqs, before, heads, dtype", [(12, 24000, 8, "f16"), (12, 24000, 64, "bf16"), (3, 20000, 8, "bf16"), (60, 150, 8, "f16"), (60, 150, 64, "f16"), (1, 70000, 64, "f16")])
+def test_nodes_that_nobody_sees_may_hold_anything_in_long_batches(dev, seqs, before, heads, dtype):
+    """NaN and infinities in drafted rows of some sequences: long ones, whose repair takes its time, whole items and parts of them. Every row of every
+    sequence against 64 bits, and the sequences without them bit by bit as they are without."""
+    from ironmill_b200 import ops
+    rng = H.rng_for("odd", before + heads)
+    nodes, nkv, dim, page = 32, 8, 128, 64
+    lengths = [before - 17 * i % 40 for i in range(seqs)]
+    shared, own = 96, 2
+    table = np.array([[*rng.integers(0, shared, -(-(before + nodes) // page) + 1)] for _ in range(seqs)])
+    for i, n in enumerate(lengths):                                       # the drafted rows' pages are a sequence's own
+        table[i, n // page:n // page + own] = shared + own * i + np.arange(own)
+    torch.manual_seed(before)
+    k, v = (torch.randn((1, shared + own * seqs, nkv, page, dim), device="cuda").to(TYPES[dtype]) for _ in range(2))
+    kv = ops.PagedKV(dev, k, v, _ints(table), _ints(lengths))
+    q = torch.randn((seqs * nodes, heads, dim), device="cuda").to(TYPES[dtype])
+    starts, scale = _ints(np.arange(seqs + 1) * nodes), dim ** -0.5
+    mask = np.concatenate([_tree(rng, nodes) for _ in range(seqs)])
+    mask[:, 0] &= ~np.uint64(0b110000)                                    # nobody sees nodes 4 and 5
+    mask = torch.from_numpy(mask.view(np.int64)).cuda()
+    run = lambda: ops.paged_attention(kv, 0, q, starts, nodes, scale, mask=mask, max_len=before + nodes)  # noqa: E731
+    clean = run()
+    odd = [i for i in range(seqs) if i % 5 in (0, 3)]
+    for i in odd:
+        for node, value in ((4, np.nan), (5, np.inf)):
+            r = lengths[i] + node
+            k[0, table[i, r // page], i % nkv, r % page, 7] = value
+            v[0, table[i, r // page], :, r % page, 100] = value
+    got = run()
+    rest = torch.tensor([i not in odd for i in range(seqs)]).cuda().repeat_interleave(nodes)
+    assert torch.equal(got[rest], clean[rest])
+    for i in {*odd[:3], *range(min(seqs, 3)), seqs - 1}:
+        want, mass, dot = _exact(kv, i, q[i * nodes:i * nodes + nodes], scale, mask[i * nodes:i * nodes + nodes])
+        tol = _tolerance(want, mass, dot, dtype, dim, float(v.float().nan_to_num(0, 0, 0).abs().max()), before + nodes, nodes * heads // nkv)
+        assert (np.abs(_np(got[i * nodes:i * nodes + nodes]) - want) <= tol).all(), i
