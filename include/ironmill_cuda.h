@@ -363,7 +363,7 @@ int im_cuda_paged_reorder(im_device *dev, const im_paged_kv *kv, const int *pare
 
 /* ------------------------------------------------------------------ beam search
  * The `picks` best continuations of every group of beams: value[b, v] = score[b] + logit[b, v] - log(sum_v exp(logit[b, v])), compared in
- * 64 bits, ties to the lowest b * vocab + v, best first.  logits [groups * beams, vocab] of `dtype` (IM_DTYPE_F16, F32 or BF16), rows row_stride
+ * 64 bits, ties to the lowest b * vocab + v, best first (the sums of exponentials are f32; equal rows have equal ones).  logits [groups * beams, vocab] of `dtype` (IM_DTYPE_F16, F32 or BF16), rows row_stride
  * elements apart (0 = vocab); score_dev f32 [groups * beams].  done_dev (u8 [groups * beams] or NULL): a finished beam has one continuation,
  * end_token at its own score, and its logits are not read.  Values of -inf and NaN are not picked (nor anything of a beam whose logits
  * hold a NaN or +inf); where fewer than `picks` are left, the rest gets score -inf, parent -1 and token -1.

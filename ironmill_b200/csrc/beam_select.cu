@@ -12,8 +12,8 @@
 //                     after the other from memory instead.
 //   joining           the same with the slices' picks as elements and 64-bit values.
 // Eight beams of 32 searches over 128256 f32 logits, 16 picks (131 MB): 31 us, of them 28 for the slices (4.7 TB/s, 72 % of a copy).
-// Sums are f32 per thread over its elements with one running maximum, joined in a fixed order: a run repeats bit by bit, and equal rows
-// get equal sums.
+// Sums are f32 per thread over its elements with one running maximum, joined in a fixed order: a run repeats bit by bit. Which elements are a thread's
+// goes by their place in the row alone, wherever the row starts: equal rows get equal sums, and their candidates tie as they should.
 #include <cuda_bf16.h>
 #include <limits.h>
 #include <math.h>
@@ -191,11 +191,14 @@ struct SliceSpace {
     float2 ms;
 };
 
-template <int DT>
+// ANY: some row does not start at a multiple of 16 bytes. Elements are read one by one then, 32 of a warp side by side, from all rows (32 x 8 beams
+// over 128257 f32 logits 36 us, 128256 32; 16-bit ones 31 and 29; shifting aligned pieces into place cost more, 36 and 33).
+template <int DT, bool ANY>
 __device__ __forceinline__ void slice_best(const Select &p, long long row, int slice, SliceSpace &sp) {
     using L = Logit<DT>;
     using T = typename L::T;
     constexpr int V = L::kVec, Q = 16 / V;  // requests of a piece: 16 elements of each thread
+    constexpr int kPiece = (ANY ? 16 : Q) * kSelThreads;
     auto &best = sp.best;
     auto &met = sp.met;
     auto &keep = sp.keep;
@@ -204,10 +207,9 @@ __device__ __forceinline__ void slice_best(const Select &p, long long row, int s
     const int t = threadIdx.x;
     const T *x = static_cast<const T *>(p.x) + row * p.stride;
     const int a = slice * p.slice, b = min(a + p.slice, p.vocab);
-    // 16-byte requests from the first aligned element on; what is before and behind them is read one by one
-    const int head = max(min(b - a, (int)((16 - (reinterpret_cast<uintptr_t>(x + a) & 15)) % 16 / sizeof(T))), 0);
-    const int vecs = max(b - a - head, 0) / V, tail = a + head + vecs * V;
-    const uint4 *xv = reinterpret_cast<const uint4 *>(x + a + head);
+    // 16 bytes of elements at a time from the first one on (a is a multiple of eight elements); what is left behind them is read one by one
+    const int vecs = max(b - a, 0) / V, tail = ANY ? b : a + vecs * V;
+    const uint4 *xv = reinterpret_cast<const uint4 *>(x + a);
     best.clear(p.picks);
     if (t == 0) met = keep = 0;
     float m = -INFINITY, s = 0.0f;
@@ -226,21 +228,31 @@ __device__ __forceinline__ void slice_best(const Select &p, long long row, int s
         }
         s += a + b;
     };
-    // the odd ends: up to 7 elements each, the first threads' (with no bound yet: collected where they reach the first one)
-    const int ends = head + max(b - tail, 0);
-    const int end_at = t < head ? a + t : tail + t - head;
+    // the odd end: up to 7 elements, the first threads' (with no bound yet: collected where they reach the first one)
+    const int ends = max(b - tail, 0), end_at = tail + t;
     float end = -INFINITY;
     if (t < ends) {
         end = L::get(x[end_at]);
         take(&end, 1, end);
     }
-    const int pieces = (vecs + Q * kSelThreads - 1) / (Q * kSelThreads);
+    const int pieces = (max(b - a, 0) / (ANY ? 1 : V) + kPiece - 1) / kPiece;
     float bound = -INFINITY;
 #pragma unroll 1
     for (int k = 0; k < max(pieces, 1); k++) {
-        const int i0 = k * Q * kSelThreads + t;
+        const int i0 = ANY ? a + k * kPiece + (t & ~31) * 16 + (t & 31) : k * kPiece + t;
         float f[16];
-        if (i0 + (Q - 1) * kSelThreads < vecs) {
+        if constexpr (ANY) {
+            T e[16];
+            if (i0 + 15 * 32 < b) {
+#pragma unroll
+                for (int j = 0; j < 16; j++) e[j] = __ldg(x + i0 + j * 32);
+#pragma unroll
+                for (int j = 0; j < 16; j++) f[j] = L::get(e[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; j++) f[j] = i0 + j * 32 < b ? L::get(__ldg(x + i0 + j * 32)) : -INFINITY;
+            }
+        } else if (i0 + (Q - 1) * kSelThreads < vecs) {
             uint4 u[Q];
 #pragma unroll
             for (int q = 0; q < Q; q++) u[q] = ldg_stream_v4(xv + i0 + q * kSelThreads);
@@ -277,8 +289,8 @@ __device__ __forceinline__ void slice_best(const Select &p, long long row, int s
             if (met_v[i] >= bound) kept[atomicAdd(&keep, 1)] = met_i[i];
         __syncthreads();
         for (int i = t; i < keep * 16; i += kSelThreads) {
-            const int v = kept[i >> 4] + (i & 15) / V * kSelThreads, e = a + head + v * V + (i & 15) % V;
-            if (v >= vecs) continue;
+            const int at = kept[i >> 4], v = at + (i & 15) / V * kSelThreads, e = ANY ? at + (i & 15) * 32 : a + v * V + (i & 15) % V;
+            if (ANY ? e >= b : v >= vecs) continue;
             const float f = L::get(x[e]);
             if (f >= bound && f > -INFINITY) best.collect(f, e);
         }
@@ -292,10 +304,14 @@ __device__ __forceinline__ void slice_best(const Select &p, long long row, int s
     if ((t & 31) == 0) red_m[t >> 5] = M, red_s[t >> 5] = S;
     best.rank(p.picks, [&](auto f) {
         if (t < ends) f(end, end_at);
-        for (int i = t; i < vecs; i += kSelThreads) {
-            float g[V];
-            L::split(__ldg(xv + i), g);
-            for (int j = 0; j < V; j++) f(g[j], a + head + i * V + j);
+        if constexpr (ANY) {
+            for (int e = a + t; e < b; e += kSelThreads) f(L::get(x[e]), e);
+        } else {
+            for (int i = t; i < vecs; i += kSelThreads) {
+                float g[V];
+                L::split(__ldg(xv + i), g);
+                for (int j = 0; j < V; j++) f(g[j], a + i * V + j);
+            }
         }
     });
     if (t == 0) {
@@ -309,7 +325,7 @@ __device__ __forceinline__ void slice_best(const Select &p, long long row, int s
 }
 
 // grid (slices, rows)
-template <int DT>
+template <int DT, bool ANY>
 __global__ void __launch_bounds__(kSelThreads, kSelResident) beam_slice_kernel(const __grid_constant__ Select p) {
     __shared__ SliceSpace sp;
     pdl_trigger();
@@ -317,7 +333,7 @@ __global__ void __launch_bounds__(kSelThreads, kSelResident) beam_slice_kernel(c
     const int slice = blockIdx.x, t = threadIdx.x;
     const long long row = blockIdx.y;
     if (p.done && p.done[row]) return;
-    slice_best<DT>(p, row, slice, sp);
+    slice_best<DT, ANY>(p, row, slice, sp);
     if (t == 0) p.part_ms[row * p.slices + slice] = sp.ms;
     const long long at = (row * p.slices + slice) * p.picks;
     for (int k = t; k < p.picks; k += kSelThreads) {
@@ -405,7 +421,7 @@ __global__ void __launch_bounds__(kSelThreads) beam_join_kernel(const __grid_con
 // Few beams over few elements: a cluster per group, a CTA per slice of a beam; the first one joins what it finds in the others' shared memory. One
 // launch, no scratch.
 constexpr int kSelCluster = 8, kSelClusterSlice = 32768;
-template <int DT>
+template <int DT, bool ANY>
 __global__ void __launch_bounds__(kSelThreads) beam_cluster_kernel(const __grid_constant__ Select p) {
     __shared__ SliceSpace sp;
     __shared__ JoinSpace js;
@@ -414,7 +430,7 @@ __global__ void __launch_bounds__(kSelThreads) beam_cluster_kernel(const __grid_
     pdl_wait();
     const int C = p.beams * p.slices, group = blockIdx.x / C, rank = blockIdx.x - group * C, beam = rank / p.slices;
     const long long row = (long long)group * p.beams + beam;
-    if (!(p.done && p.done[row])) slice_best<DT>(p, row, rank - beam * p.slices, sp);
+    if (!(p.done && p.done[row])) slice_best<DT, ANY>(p, row, rank - beam * p.slices, sp);
     cluster_sync();
     if (rank == 0) {
         for (int i = threadIdx.x; i < C * p.picks; i += kSelThreads) {  // (what a finished beam's CTA holds is not looked at)
@@ -472,6 +488,7 @@ IM_EXPORT int im_cuda_beam_select(im_device *dev, const void *logits_dev, int dt
     if (groups == 0) return IM_OK;
     Select p;
     const int clustered = cluster_slices(dev, groups, beams, vocab);
+    const bool any = !aligned16(logits_dev) || ((long long)groups * beams > 1 && (row_stride ? row_stride : vocab) * (dtype == IM_DTYPE_F32 ? 4 : 2) % 16 != 0);
     p.slices = clustered ? clustered : select_slices(dev, groups, beams, vocab);
     p.slice = ((vocab + p.slices - 1) / p.slices + 7) / 8 * 8;
     const long long rows = (long long)groups * beams;
@@ -485,12 +502,17 @@ IM_EXPORT int im_cuda_beam_select(im_device *dev, const void *logits_dev, int dt
     p.part_ms = static_cast<float2 *>(scratch_dev);
     p.part_v = reinterpret_cast<float *>(p.part_ms + rows * p.slices);
     p.part_i = reinterpret_cast<int *>(p.part_v + rows * p.slices * picks);
+#define IM_KERNEL(K) \
+    (dtype == IM_DTYPE_F32   ? (any ? K<IM_DTYPE_F32, true> : K<IM_DTYPE_F32, false>) \
+     : dtype == IM_DTYPE_F16 ? (any ? K<IM_DTYPE_F16, true> : K<IM_DTYPE_F16, false>) \
+                             : (any ? K<IM_DTYPE_BF16, true> : K<IM_DTYPE_BF16, false>))
     if (clustered) {
-        void (*one)(Select) = dtype == IM_DTYPE_F32 ? beam_cluster_kernel<IM_DTYPE_F32> : dtype == IM_DTYPE_F16 ? beam_cluster_kernel<IM_DTYPE_F16> : beam_cluster_kernel<IM_DTYPE_BF16>;
+        void (*one)(Select) = IM_KERNEL(beam_cluster_kernel);
         IM_CUDA_CHECK(launch_cluster(one, dim3((unsigned)(rows * p.slices)), dim3(kSelThreads), beams * p.slices, 0, as_stream(stream), p));
         return IM_OK;
     }
-    void (*kern)(Select) = dtype == IM_DTYPE_F32 ? beam_slice_kernel<IM_DTYPE_F32> : dtype == IM_DTYPE_F16 ? beam_slice_kernel<IM_DTYPE_F16> : beam_slice_kernel<IM_DTYPE_BF16>;
+    void (*kern)(Select) = IM_KERNEL(beam_slice_kernel);
+#undef IM_KERNEL
     IM_CUDA_CHECK(launch_k(kern, dim3(p.slices, (unsigned)rows), dim3(kSelThreads), 0, as_stream(stream), p));
     IM_CUDA_CHECK(launch_k(beam_join_kernel, dim3(groups), dim3(kSelThreads), 0, as_stream(stream), p));
     return IM_OK;

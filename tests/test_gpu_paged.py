@@ -856,3 +856,23 @@ def test_nodes_that_nobody_sees_may_hold_anything_in_long_batches(dev, seqs, bef
         want, mass, dot = _exact(kv, i, q[i * nodes:i * nodes + nodes], scale, mask[i * nodes:i * nodes + nodes])
         tol = _tolerance(want, mass, dot, dtype, dim, float(v.float().nan_to_num(0, 0, 0).abs().max()), before + nodes, nodes * heads // nkv)
         assert (np.abs(_np(got[i * nodes:i * nodes + nodes]) - want) <= tol).all(), i
+
+
+# ------------------------------------------------------------------------------------------------ equal beams
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("groups, beams, vocab", [(1, 8, 50257), (2, 3, 1001), (5, 16, 50257), (40, 5, 1003), (3, 7, 130001), (2, 2, 4099)])
+@pytest.mark.parametrize("lead", [0, 1])
+def test_equal_beams_tie_wherever_their_rows_start(dev, dtype, groups, beams, vocab, lead):
+    """Beams with the same logits and scores have the same values to the last bit: a token's beams come in order, at rows of every alignment."""
+    from ironmill_b200 import ops
+    rng = H.rng_for("equal", vocab + beams)
+    row = _randn(rng, (groups, 1, vocab), dtype)     # sums of many terms of like size, whose roundings follow their order
+    for g in range(groups):                          # the two best tokens of a group
+        row[g, 0, (17 * g + 5) % vocab], row[g, 0, vocab - 1 - g] = 6.0, 5.75
+    x = torch.empty(groups * beams * vocab + lead, dtype=TYPES[dtype], device="cuda")[lead:].view(groups, beams, vocab)
+    x.copy_(row)
+    score, parent, token = (t.cpu() for t in ops.beam_select(dev, x, torch.full((groups, beams), -1.25, device="cuda"), 2 * beams))
+    for g in range(groups):
+        assert parent[g].tolist() == [*range(beams)] * 2
+        assert token[g].tolist() == [(17 * g + 5) % vocab] * beams + [vocab - 1 - g] * beams
+        assert len(set(score[g, :beams].tolist())) == len(set(score[g, beams:].tolist())) == 1
