@@ -577,31 +577,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     }
 }
 
-// A row of an item from the positions it sees alone, by a block: a warp per quarter of them.
 constexpr int kTcJoinThreads = 128, kTcJoinWarps = kTcJoinThreads / 32;
-template <bool BF16, int HD>
-__device__ __noinline__ void repair_row(const PagedAttn &p, const PagedUnit &u, int head, int r, float (*sums)[HD], float2 *ml) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long per = ((long long)u.end + 32 * kTcJoinWarps - 1) / (32 * kTcJoinWarps) * 32;
-    float o[HD / 32], m, l;
-    plain_row<BF16, HD>(p, u, head, r, (int)min((long long)u.end, warp * per), (int)min((long long)u.end, (warp + 1) * per), o, m, l);
+// Rows 32 * rows + j of an item, j a bit of `bad`, from the positions they see alone: every `warps`-th of them, by a warp. (By itself and from numbers
+// alone: what it needs of registers and memory is no cost where no row is odd.)
+template <bool BF16, int R, int HD>
+__device__ __noinline__ void odd_rows_again(const PagedAttn &p, int unit, int head, int rows, unsigned bad, int warp, int warps) {
+    const int lane = threadIdx.x & 31;
+    const PagedUnit u = paged_unit<R>(p, unit);
+#pragma unroll 1
+    for (int n = 0; bad; n++, bad &= bad - 1) {
+        if (n % warps != warp) continue;
+        const int r = rows * 32 + __ffs(bad) - 1;
+        float o[HD / 32], m, l;
+        plain_row<BF16, HD>(p, u, head, r, 0, u.end, o, m, l);
+        const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
+        uint16_t *out = p.out + (u.tok0 + (u.row0 + r) / p.group) * p.os + (long long)(head * p.group + (u.row0 + r) % p.group) * HD + lane;
 #pragma unroll
-    for (int i = 0; i < HD / 32; i++) sums[warp][lane + 32 * i] = o[i];
-    if (lane == 0) ml[warp] = make_float2(m, l);
-    __syncthreads();
-    float M = -INFINITY, L = 0.0f, x = 0.0f;
-    for (int w = 0; w < kTcJoinWarps; w++) M = fmaxf(M, ml[w].x);
-    const int c = threadIdx.x % HD;
-    for (int w = 0; w < kTcJoinWarps; w++) {
-        if (ml[w].x == -INFINITY && ml[w].y == 0.0f) continue;  // nothing seen there
-        const float f = ex2(ml[w].x - M);
-        L += ml[w].y * f;
-        x += sums[w][c] * f;
+        for (int i = 0; i < HD / 32; i++) out[32 * i] = (uint16_t)pack2<BF16>(o[i] * inv, 0.0f);
     }
-    const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
-    const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
-    if (threadIdx.x < HD) p.out[(u.tok0 + t) * p.os + (long long)(head * p.group + g) * HD + c] = (uint16_t)pack2<BF16>(x * inv, 0.0f);
-    __syncthreads();
 }
 
 // Four columns of row r of an item that a cut divides. Returns the lanes whose rows are not finite: those are not written.
@@ -649,25 +642,21 @@ __device__ __forceinline__ unsigned join_parts(const PagedAttn &p, const PagedUn
 }
 
 // Items that a cut divides: a warp per 32 rows and four columns, a row per lane. Blocks are small enough to wait beside a CTA of the kernel above.
-// Rows that it has noted as not finite, of any item, are done again: the blocks of 32 rows share them. (In the kernel above, where a warp had them one
-// after the other at 1.4 us a position, other warps ran out of patience. 32 rows of each of 128 items over 1000 positions: 45 ms there, 0.8 here.)
+// Rows that it has noted as not finite, of any item, are done again: the warps of 32 rows share them. (In the kernel above, where a warp had them one
+// after the other at 1.4 us a position, other warps ran out of patience. 32 rows of each of 128 items over 1000 positions: 45 ms there, 0.9 here.)
+// No shared memory and few registers: the kernel above leaves little of them free (with 2 KB a block eight portions of 128 tokens behind 500 took 44.9 us, 43.4 so).
 template <bool BF16, int KB, bool WIDE>
-__global__ void __launch_bounds__(kTcJoinThreads) paged_tc_join_kernel(const __grid_constant__ PagedAttn p, int units) {
+__global__ void __launch_bounds__(kTcJoinThreads, WIDE ? 9 : 12) paged_tc_join_kernel(const __grid_constant__ PagedAttn p, int units) {
     constexpr int R = TcShape<KB, WIDE>::kRows, HD = 64 * KB, N = WIDE ? 8 : 4;  // N: parts that are requested together
-    constexpr int kBlocks = HD / 4 / kTcJoinWarps;  // of the same 32 rows
-    __shared__ float sums[kTcJoinWarps][HD];
-    __shared__ float2 ml[kTcJoinWarps];
     pdl_trigger();
     pdl_wait();
     const int item = blockIdx.x, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, lane = threadIdx.x & 31;
-    const int rows = blockIdx.y / kBlocks, r = rows * 32 + lane, c = (blockIdx.y % kBlocks * kTcJoinWarps + (threadIdx.x >> 5)) * 4;
+    const int w = blockIdx.y * kTcJoinWarps + (threadIdx.x >> 5), rows = w / (HD / 4), r = rows * 32 + lane, c = w % (HD / 4) * 4;
     const int2 span = *reinterpret_cast<const int2 *>(p.spans + 2 * (long long)item);
     const PagedUnit u = paged_unit<R>(p, unit);
     if (rows * 32 >= u.rows) return;  // (a unit without tiles has no rows)
-    unsigned bad = span.x < 0 ? p.odd[(long long)item * 8 + rows] : join_parts<BF16, HD, R, N>(p, u, span, head, r, c);
-#pragma unroll 1
-    for (int n = 0; bad; n++, bad &= bad - 1)
-        if (n % kBlocks == blockIdx.y % kBlocks) repair_row<BF16, HD>(p, u, head, rows * 32 + __ffs(bad) - 1, sums, ml);
+    const unsigned bad = span.x < 0 ? p.odd[(long long)item * 8 + rows] : join_parts<BF16, HD, R, N>(p, u, span, head, r, c);
+    if (bad) odd_rows_again<BF16, R, HD>(p, unit, head, rows, bad, w % (HD / 4), HD / 4);
 }
 
 template <bool BF16, int KB, bool WIDE>
