@@ -334,8 +334,9 @@ int im_cuda_paged_append(im_device *dev, const im_paged_kv *kv, int layer, const
  * h / (num_heads / num_kv_heads).  A token sees all seq_len rows before the new ones, and of the new rows: without a mask its own and
  * those before it; with mask_dev [num_tokens, mask_words] the d-th where bit d % 64 of word d / 64 is set (its ancestors and itself).
  * A row that sees nothing gets zeros; infinities and NaN in rows that a token does not see do not reach it.  f32 scores, sums
- * and accumulation, softmax weights as a sum of two 16-bit terms (of sequences with more than 128 rows (token, head) of a KV head, heads
- * of 64 and 128: one), one rounding of the output.  q, out: as q in paged_append; out does not lie over q.
+ * and accumulation, one rounding of the output.  Softmax weights enter their product as a sum of two terms of the cache's type (relative error
+ * 2^-16 in bf16, 2^-22 in fp16), or as one (2^-8, 2^-11) in every sequence of a call with max_new * num_heads / num_kv_heads > 128 and heads
+ * of 64 or 128; fp16 weights below 2^-26 of the row's largest are off by up to 2^-37 of it.  q, out: as q in paged_append; out does not lie over q.
  * max_new: no sequence has more new tokens (further ones are left as they are).  max_len: no sequence has more rows, the new ones
  * included (0: the table's width); a smaller value costs time, not results.  scratch_dev: 16-byte aligned,
  * im_cuda_paged_attention_scratch_bytes for the same kv, heads, max_new and max_len (short contexts need none; those of a larger

@@ -59,6 +59,8 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool there) 
 template <bool BF16, int HD, bool CL>
 __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kernel(const __grid_constant__ PagedAttn p, int units) {
     using S = PaShape<HD>;
+    // fp16 weights: 2^15 at the row's maximum instead of 1, so that they are normal numbers down to 2^-29 of it (exact to 2^-40 below)
+    constexpr float kLift = BF16 ? 0.0f : 15.0f;
     constexpr int R = S::kRows, KS = HD / 16, NT = HD / 8, CH = HD / 8;  // k steps, 8-column tiles, 16-byte pieces of a row
     extern __shared__ __align__(128) unsigned char pa_smem[];
     __shared__ long long sums[kPaThreads + kShareMore];
@@ -239,7 +241,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
 #pragma unroll
                     for (int n = 0; n < NT; n++) o[n][2 * i] *= corr, o[n][2 * i + 1] *= corr;
                 }
-                const float base = m[i] == -INFINITY ? 0.0f : m[i];
+                const float base = m[i] == -INFINITY ? 0.0f : m[i] - kLift;
                 float sum = 0.0f;
 #pragma unroll
                 for (int n = 0; n < 2; n++) {
@@ -296,7 +298,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
                 const float2 x = ml[w * R + r];
                 L += x.x == -INFINITY && x.y == 0.0f ? 0.0f : x.y * ex2(x.x - M);
             }
-            return make_float2(M, L);
+            return make_float2(M - kLift, L);  // (plain_row has no lift)
         };
 #pragma unroll 1
         for (int w = 0; w < kPaWarps; w++) {

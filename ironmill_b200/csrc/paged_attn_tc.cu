@@ -8,9 +8,10 @@
 //     O += P V     P from tensor memory, V with the head dimension contiguous
 // A tile of up to 256 rows (WIDE): the halves own 128 rows each and every tile of K and V serves both. Up to 128 rows: the halves own the even
 // and the odd tiles of the share, with accumulators of their own that are joined where the item ends. There the copies set the pace and the second
-// term of the weights is free; in a wide tile the chain of scores, weights and products does, and one term is what it takes: rounding a weight by half a
-// step (2^-8 bf16, 2^-11 fp16, relative) at most moves an output by what rounding the output itself does.
-// A row's accumulator is rescaled only when its maximum has grown by more than 2^8 (as in flash_tc.cu).
+// term of the weights is free; in a wide tile the chain of scores, weights and products does, and one term is what it takes: half a step of
+// a weight (2^-8 bf16, 2^-11 fp16, relative) moves an output by at most that share of the sum of its weights times |values|, as much as rounding the output
+// does where all values have one sign, more where they cancel.
+// A row's accumulator is rescaled only when its maximum has grown by more than a power of two (as in flash_tc.cu), 2^8 for bf16, 2^3 for fp16.
 //
 // K, V and queries come by 16-byte cp.async of four warps, rows looked up in the page table: any page size, rows that are not there are zeros and
 // known to be none (a bit per row). The copies run ahead over the ends of items as far as the slots allow.
@@ -33,7 +34,11 @@ namespace {
 
 // warps 0-7: weights; 8: products; 9-12: copies
 constexpr int kTcTile = 128, kTcThreads = 13 * 32, kTcMma = 8, kTcCopy = 9, kTcCopyWarps = 4;
-constexpr float kTcLazy = 8.0f;  // growth of a row's maximum (in powers of two) that is left in the weights
+// Growth of a row's maximum (in powers of two) that is left in the weights; power of two that a weight has at the maximum: fp16 weights come up to 2^15, so that
+// they are normal numbers down to 2^-26 of the maximum (exact to 2^-37 below). bf16 has the range of f32. (A growth
+// of 2^8 left in fp16 too: 120.3 us instead of 125.8 for 256 rows over 100003 positions where the scores' spread is four nats, no difference at one.)
+constexpr float tc_lazy(bool bf16) { return bf16 ? 8.0f : 3.0f; }
+constexpr float tc_lift(bool bf16) { return bf16 ? 0.0f : 12.0f; }
 
 template <int KB, bool WIDE>
 struct TcShape {
@@ -168,6 +173,7 @@ template <bool BF16, int KB, bool WIDE>
 __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_constant__ PagedAttn p, int units, int *err) {
     using Shape = TcShape<KB, WIDE>;
     constexpr int kTerms = WIDE ? 1 : 2;  // 16-bit terms of a weight
+    constexpr float kLazy = tc_lazy(BF16), kLift = tc_lift(BF16);
     constexpr int R = Shape::kRows, HD = 64 * KB, SK = Shape::kK, SV = Shape::kV, BLK = Shape::kBlock;
     extern __shared__ __align__(16) unsigned char tc_smem[];
     uint32_t *there = reinterpret_cast<uint32_t *>(tc_smem);                   // [8 tiles][4]: bit j of word w: row 32 w + j of the tile is in the cache
@@ -433,7 +439,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                     top = fmaxf(fmaxf(top, fmaxf(mx[0], mx[1])), fmaxf(mx[2], mx[3]));
                 }
                 top *= scale;
-                if (__any_sync(0xffffffffu, top > m + kTcLazy)) {  // (-inf + anything is -inf: a row's first visible position is one)
+                if (__any_sync(0xffffffffu, top > m + kLazy)) {  // (-inf + anything is -inf: a row's first visible position is one)
                     const float m_new = fmaxf(m, top), corr = m_new == -INFINITY ? 1.0f : ex2(m - m_new);
                     m = m_new;
                     l *= corr;
@@ -449,7 +455,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                         }
                     }
                 }
-                const float base = m == -INFINITY ? 0.0f : m;
+                const float base = m == -INFINITY ? 0.0f : m - kLift;
                 tmem_wait_st();
                 const uint64_t scale_two = two(scale, scale), base_two = two(-base, -base), minus_one = two(-1.0f, -1.0f);
                 uint64_t sum[2] = {0, 0};
@@ -565,7 +571,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             }
             if (WIDE || h == 0) {
                 if (whole && lane == 0) p.odd[((long long)it.unit * p.kv.nkv + it.head) * 8 + warp] = bad;
-                if (live && !whole) p.part_ml[slot * R + R_] = make_float2(m, bad >> lane & 1u ? NAN : l);
+                if (live && !whole) p.part_ml[slot * R + R_] = make_float2(m - kLift, bad >> lane & 1u ? NAN : l);
             }
         }
     }

@@ -876,3 +876,34 @@ def test_equal_beams_tie_wherever_their_rows_start(dev, dtype, groups, beams, vo
         assert parent[g].tolist() == [*range(beams)] * 2
         assert token[g].tolist() == [(17 * g + 5) % vocab] * beams + [vocab - 1 - g] * beams
         assert len(set(score[g, :beams].tolist())) == len(set(score[g, beams:].tolist())) == 1
+
+
+# ------------------------------------------------------------------------------------------------ long flat tails
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads, new, dim", [(1, 1, 128), (16, 1, 64), (4, 1, 256), (8, 4, 128), (8, 4, 64), (16, 16, 128), (16, 16, 64)])
+@pytest.mark.parametrize("low, rows", [(-17.0625, 100003), (-17.375, 100003), (-21.0, 100003), (-12.0, 900)])
+@pytest.mark.parametrize("sink_last", [False, True])
+def test_a_long_tail_of_small_weights_beside_one_large_one(dev, dtype, heads, new, dim, low, rows, sink_last):
+    """A row that takes nearly all of the weight and has a value of zero, and a tail whose weights (2^-17 to 2^-30 of it) are what the outputs come from."""
+    from ironmill_b200 import ops
+    page = 64
+    pages = -(-(rows + new) // page)
+    low = torch.tensor(low).to(TYPES[dtype]).item()
+    k, v = (torch.zeros((1, pages, 1, page, dim), dtype=TYPES[dtype], device="cuda") for _ in range(2))
+    kr, vr = k.view(-1, dim), v.view(-1, dim)              # (one KV head, pages in order)
+    kr[:rows, 0], vr[:rows] = low, 1.0
+    sink = rows - 1 if sink_last else 0
+    kr[sink, 0], vr[sink] = 0.0, 0.0
+    kr[rows:, 0] = -1000.0                                 # the new rows take nothing: 2^-1442
+    kv = ops.PagedKV(dev, k, v, _ints(np.arange(pages)[None]), _ints([rows]))
+    q = torch.zeros((new, heads, dim), dtype=TYPES[dtype], device="cuda")
+    q[:, :, 0] = 1.0
+    got = _np(ops.paged_attention(kv, 0, q, _ints([0, new]), new, 1.0, max_len=rows + new))
+    # a score is one product: off by 2^-24 of it where it is scaled to powers of two, and again where the maximum is taken off; the
+    # exponential, the sum and the join 2^-18; two 16-bit terms 2^-16 (bf16) or 2^-21, one 2^-9 or 2^-12; what of an fp16 weight is below 2^-37 of the largest; one rounding
+    tail = np.exp(float(low)) * (rows - 1)
+    want, eps = tail / (1 + tail), torch.finfo(TYPES[dtype]).eps / 2
+    weights = eps if heads * new > 128 else 2.0 ** -16 if dtype == "bf16" else 2.0 ** -21
+    tol = eps * want * (1 + 1e-3) + (weights + 2.0 ** -18 + 4 * abs(low) * 1.45 * 2.0 ** -24) * want
+    tol += rows * 2.0 ** -37 + 2.0 ** -25 if dtype == "f16" else 0.0
+    assert np.abs(got - want).max() <= tol, (got.min(), got.max(), want, tol)
