@@ -302,8 +302,9 @@ int im_cuda_sdpa_f16(im_device *dev, const void *q_dev, const void *k_cache_dev,
  * Row r of sequence s lies in page page_table_dev[s * table_stride + r / page_size], slot r % page_size.  seq_len_dev[s] rows are
  * there before a call's new tokens, whose rows follow them.  token_start_dev [num_seqs + 1], not decreasing, gives the
  * new tokens of sequence s: rows token_start[s] .. token_start[s + 1] - 1 of the token arrays.  Token rows before the first or from
- * the last of these on are left as they are.  What the device arrays say is checked on the device: a row past the table, a page
- * number outside 0 .. num_pages - 1 or a negative length reads nothing (the row is not there) and writes nothing.
+ * the last of these on are left as they are.  What the device arrays say is checked on the device: a row past the table or a page
+ * number outside 0 .. num_pages - 1 reads nothing (the row is not there) and writes nothing.  Lengths count as the nearest of 0 and
+ * the table's rows: new tokens of a sequence with a negative length are its rows 0, 1, ... (an idle sequence is one without new tokens).
  * Clear the struct before filling it. */
 typedef struct im_paged_kv {
     void *k_dev, *v_dev;       /* layer l, page p: [num_kv_heads, page_size, head_dim] at l * layer_stride + p * page_stride; 16-byte aligned */

@@ -13,7 +13,7 @@ struct PagedView {
     int rows;  // most rows of a sequence: width * page
     const int *table, *len;
 
-    // rows of a sequence before the new tokens
+    // rows of a sequence before the new tokens: a length that the table cannot hold counts as the nearest one that it can
     __device__ __forceinline__ int length(int seq) const { return min(max(__ldg(len + seq), 0), rows); }
     // element offset of slot 0 of head 0 in the page that holds row r, -1 where there is none; r in [0, rows)
     __device__ __forceinline__ long long page_of(int seq, int r) const {

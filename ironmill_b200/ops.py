@@ -437,8 +437,8 @@ def _ints(x: torch.Tensor, ordinal: int, n: int, width: int = 0) -> int:
 
 class PagedKV:
     """Keys and values of every layer in pages (im_paged_kv): k_pages, v_pages [layers, pages, kv_heads, page_size, head_dim] (fp16 or bf16; pages and
-    layers may lie apart), page_table int32 [sequences, width], lengths int32 [sequences]: rows before a call's new tokens. Holds the
-    tensors; what is written to them is what the next call sees."""
+    layers may lie apart), page_table int32 [sequences, width], lengths int32 [sequences]: rows before a call's new tokens (a negative one
+    counts as 0, one past the table as the table's rows). Holds the tensors; what is written to them is what the next call sees."""
 
     def __init__(self, dev: Device, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor):
         assert k_pages.is_cuda and k_pages.device.index == dev.ordinal and k_pages.dtype in (torch.float16, torch.bfloat16) and k_pages.dim() == 5

@@ -907,3 +907,28 @@ def test_a_long_tail_of_small_weights_beside_one_large_one(dev, dtype, heads, ne
     tol = eps * want * (1 + 1e-3) + (weights + 2.0 ** -18 + 4 * abs(low) * 1.45 * 2.0 ** -24) * want
     tol += rows * 2.0 ** -37 + 2.0 ** -25 if dtype == "f16" else 0.0
     assert np.abs(got - want).max() <= tol, (got.min(), got.max(), want, tol)
+
+
+# ------------------------------------------------------------------------------------------------ lengths that the table cannot hold
+@pytest.mark.parametrize("nodes, heads", [(1, 4), (9, 8), (40, 16)])
+def test_negative_lengths_count_as_zero_and_long_ones_as_the_table(dev, nodes, heads):
+    """On pages that are all there: every operator does what it does at the lengths that these count as."""
+    from ironmill_b200 import ops
+    runs = []
+    for lengths in ([-1, 20, -(1 << 31), 5000], [0, 20, 0, 64]):
+        rng = H.rng_for("lengths", nodes)
+        c = Cache(dev, rng, [64] * 4, [0, 20, 0, 64], page=16)
+        table = c.table[:, :4]
+        c.kv.point_at(_ints(table), _ints(lengths))
+        q, k, v = _randn(rng, (4 * nodes, heads, 128), "f16"), _randn(rng, (4 * nodes, 2, 128), "f16"), _randn(rng, (4 * nodes, 2, 128), "f16")
+        angle = np.arange(200)[:, None] * 1e4 ** (-2.0 * np.arange(64) / 128)
+        cos, sin = (torch.from_numpy(f(angle)).cuda().half() for f in (np.cos, np.sin))
+        starts = _ints(np.arange(5) * nodes)
+        got = [ops.paged_append(c.kv, 0, k, v, starts, q=q, cos=cos, sin=sin), c.k.clone(), c.v.clone()]
+        got.append(ops.paged_attention(c.kv, 0, q, starts, nodes, 0.09, max_len=0))
+        got += [ops.paged_keep(c.kv, _ints([[0, 5, 9]] * 4), _ints([3] * 4)), c.k.clone(), c.v.clone()]
+        got += [*ops.paged_reorder(c.kv, _ints([1, 1, 0, 0]), 4), c.k.clone(), c.v.clone()]
+        runs.append(got)
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+    k0 = runs[0][1]
+    assert k0[0, table[0, 0], :, 0].any() and runs[0][4].tolist() == [3, 23, 3, 67]
