@@ -394,6 +394,7 @@ IM_EXPORT int im_cuda_paged_keep(im_device *dev, const im_paged_kv *kv, const in
     IM_REQUIRE(!share_memory(seq_len_out_dev, 4ll * v.nseq, v.len, 4ll * v.nseq), "the new lengths lie over the old ones");
     IM_REQUIRE(!share_memory(seq_len_out_dev, 4ll * v.nseq, count_dev, 4ll * v.nseq) && !share_memory(seq_len_out_dev, 4ll * v.nseq, accepted_dev, 4ll * v.nseq * max_accept),
                "the new lengths lie over the accepted places");
+    IM_REQUIRE(v.nseq == 0 || !share_memory(seq_len_out_dev, 4ll * v.nseq, v.table, 4 * ((v.nseq - 1) * v.table_stride + v.width)), "the new lengths lie over the page table");
     const long long cols = (long long)v.layers * 2 * v.nkv * (v.hd / 8);
     IM_REQUIRE(cols <= INT_MAX - kKeepThreads, "too many layers and heads");
     rc = paged_device(dev);

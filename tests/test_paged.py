@@ -172,3 +172,12 @@ def test_plain_attention_by_hand():
     assert np.allclose(out.ravel(), [13 / 3, 15 / 4])
     out, _, _ = op.attention(keys, values, table, [0], [0, 2], q, 1.0, mask=np.array([[2], [0]]))
     assert out.ravel().tolist() == [8.0, 0.0]
+
+
+# ------------------------------------------------------------------------------------------------ keeping over the page table
+@pytest.mark.parametrize("out, table, word", [
+    (3 * PTR, {}, "page table"), (3 * PTR - 8, {}, "page table"), (3 * PTR + 47, {}, "page table"), (3 * PTR + 48, {}, GOOD), (3 * PTR - 12, {}, GOOD),
+    (3 * PTR + 76, dict(table_stride=8), "page table"), (3 * PTR + 80, dict(table_stride=8), GOOD), (3 * PTR, dict(num_seqs=0), GOOD)])
+def test_new_lengths_over_the_page_table_are_refused(lib, out, table, word):
+    kv = _kv(**table)
+    assert word in _message(lib, lib.im_cuda_paged_keep(None, C.addressof(kv), PTR, 4, PTR, out, None))
