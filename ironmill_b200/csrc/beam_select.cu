@@ -419,7 +419,9 @@ __global__ void __launch_bounds__(kSelThreads) beam_join_kernel(const __grid_con
 }
 
 // Few beams over few elements: a cluster per group, a CTA per slice of a beam; the first one joins what it finds in the others' shared memory. One
-// launch, no scratch.
+// launch, no scratch: the host's part of a call is what there is to save (four beams over 32768: 12.6 us a call from Python, 17.8 in two launches). On the
+// device two launches are the shorter ones, 7.2 us against 10.0 in a captured graph, and the more so the longer the slices (four beams: of 65536 7.8 and
+// 12.0, of 128256 9.4 and 21.4) and the fewer the clusters that the GPU holds leave free (40 searches of four beams 13.8 and 15.5): the limits.
 constexpr int kSelCluster = 8, kSelClusterSlice = 32768;
 template <int DT, bool ANY>
 __global__ void __launch_bounds__(kSelThreads) beam_cluster_kernel(const __grid_constant__ Select p) {
@@ -445,14 +447,14 @@ __global__ void __launch_bounds__(kSelThreads) beam_cluster_kernel(const __grid_
     if (rank == 0) join_group(p, group, ms, true, js);
 }
 
-// Slices of a row: as many as the GPU holds blocks of all rows at a time (a second wave of a few would cost as much as a full one), none below kSelLeast
-// elements.
 // Slices of a beam where a cluster takes a group, 0 where it does not.
 int cluster_slices(const Device *dev, int groups, int beams, int vocab) {
     if (beams > kSelCluster) return 0;
     const int n = std::max(1, std::min(kSelCluster / beams, (vocab + kSelLeast - 1) / kSelLeast));
     return (vocab + n - 1) / n <= kSelClusterSlice && (long long)groups * beams * n <= 2ll * dev->sm_count ? n : 0;
 }
+// Slices of a row: as many as the GPU holds blocks of all rows at a time (a second wave of a few would cost as much as a full one), none below kSelLeast
+// elements.
 int select_slices(const Device *dev, int groups, int beams, int vocab) {
     const long long rows = (long long)groups * beams;
     const long long want = (long long)kSelResident * dev->sm_count / rows, most = (vocab + kSelLeast - 1) / kSelLeast;

@@ -50,9 +50,6 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uin
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool there) {  // zeros where there is no source
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
 
 // CL: instead of shares of the list of all tiles, a cluster of CTAs per item, each with an equal run of its tiles; they join what they have
 // through each other's shared memory, in the same launch and without scratch.
@@ -410,7 +407,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
 // brings maxima and sums. (A block per row with the shares' divisions in loops took 25 us for 64 items of 104 rows.)
 constexpr int kJoinWarps = 8;
 template <bool BF16, int R, int HD>
-__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __grid_constant__ PagedAttn p, int units) {
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __grid_constant__ PagedAttn p) {
     constexpr int V = HD / 32;
     pdl_trigger();
     pdl_wait();
@@ -488,8 +485,7 @@ AttnPlan attn_plan(const Device *dev, int nseq, int nkv, int hd, int group, int 
 template <bool BF16, int R, int HD>
 int join_launch(const PagedAttn &p, int units, cudaStream_t st) {
     const long long rows = std::min<long long>(R, (long long)p.max_new * p.group);
-    IM_CUDA_CHECK(launch_k(paged_join_kernel<BF16, R, HD>, dim3((unsigned)(units * p.kv.nkv), (unsigned)((rows + kJoinWarps - 1) / kJoinWarps)), dim3(kJoinWarps * 32), 0, st, p,
-                           units));
+    IM_CUDA_CHECK(launch_k(paged_join_kernel<BF16, R, HD>, dim3((unsigned)(units * p.kv.nkv), (unsigned)((rows + kJoinWarps - 1) / kJoinWarps)), dim3(kJoinWarps * 32), 0, st, p));
     return IM_OK;
 }
 
@@ -568,7 +564,7 @@ IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int
     p.qs = q_stride; p.os = out_stride;
     p.start = token_start_dev;
     p.mask = mask_dev; p.mask_words = mask_words;
-    p.nh = num_heads; p.group = num_heads / kv->num_kv_heads; p.tokens = num_tokens; p.max_new = max_new;
+    p.group = num_heads / kv->num_kv_heads; p.tokens = num_tokens; p.max_new = max_new;
     p.scale2 = scale * 1.4426950408889634f;
     if (p.scale2 == 0.0f) p.scale2 = 1e-30f;  // every position alike, without 0 * inf at the hidden ones
     p.row_tiles = plan.row_tiles;

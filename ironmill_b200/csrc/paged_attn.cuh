@@ -13,7 +13,7 @@ struct PagedAttn {
     long long qs, os;
     const int *start;
     const uint64_t *mask;
-    int mask_words, nh, group, tokens, max_new;
+    int mask_words, group, tokens, max_new;
     float scale2;             // scale / ln 2: scores in powers of two
     int row_tiles;            // row tiles of a sequence: ceil(max_new * group / rows of a tile)
     int ctas;                 // CTAs of the attention kernel
@@ -192,6 +192,10 @@ __device__ __forceinline__ Share warp_share(const PagedAttn &p, int units, Paged
     at.fresh = __shfl_sync(0xffffffffu, u.fresh, s.unit);
     at.end = __shfl_sync(0xffffffffu, u.end, s.unit);
     return s;
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool there) {  // zeros where there is no source
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 
 // A row whose sums are not finite, from the positions it sees alone: on the tensor cores a weight of zero times an infinite or missing value of a

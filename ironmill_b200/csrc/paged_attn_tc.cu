@@ -165,10 +165,6 @@ __device__ __forceinline__ void copies_landed() { asm volatile("fence.proxy.asyn
 template <int R>
 __device__ __forceinline__ float *tc_part(float *part_o, size_t slot, int hd, int row, int col) { return part_o + (slot * (hd / 4) + col / 4) * (R * 4) + row * 4 + col % 4; }
 
-__device__ __forceinline__ void zcopy(uint32_t dst, const void *src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-
 template <bool BF16, int KB, bool WIDE>
 __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_constant__ PagedAttn p, int units, int *err) {
     using Shape = TcShape<KB, WIDE>;
@@ -248,7 +244,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const int r = (i0 + i) * RPI;
-                    zcopy(at + r * 128 + (((c & 7) ^ ((r + r0) & 7)) << 4), base + (o[i] < 0 ? 0 : o[i] + c * 8), o[i] >= 0);
+                    cp16(at + r * 128 + (((c & 7) ^ ((r + r0) & 7)) << 4), base + (o[i] < 0 ? 0 : o[i] + c * 8), o[i] >= 0);
                 }
             }
         };
@@ -652,7 +648,7 @@ __device__ __forceinline__ unsigned join_parts(const PagedAttn &p, const PagedUn
 // after the other at 1.4 us a position, other warps ran out of patience. 32 rows of each of 128 items over 1000 positions: 45 ms there, 0.9 here.)
 // No shared memory and few registers: the kernel above leaves little of them free (with 2 KB a block eight portions of 128 tokens behind 500 took 44.9 us, 43.4 so).
 template <bool BF16, int KB, bool WIDE>
-__global__ void __launch_bounds__(kTcJoinThreads, WIDE ? 9 : 12) paged_tc_join_kernel(const __grid_constant__ PagedAttn p, int units) {
+__global__ void __launch_bounds__(kTcJoinThreads, WIDE ? 9 : 12) paged_tc_join_kernel(const __grid_constant__ PagedAttn p) {
     constexpr int R = TcShape<KB, WIDE>::kRows, HD = 64 * KB, N = WIDE ? 8 : 4;  // N: parts that are requested together
     pdl_trigger();
     pdl_wait();
@@ -673,7 +669,7 @@ int tc_launch(const Device *dev, const PagedAttn &p, int units, cudaStream_t st)
     IM_CUDA_CHECK(launch_k(paged_tc_kernel<BF16, KB, WIDE>, dim3(p.ctas), dim3(kTcThreads), (size_t)S::kSmem, st, p, units, dev->err_flag));
     const long long rows = std::min<long long>(S::kRows, (long long)p.max_new * p.group);
     IM_CUDA_CHECK(launch_k(paged_tc_join_kernel<BF16, KB, WIDE>, dim3((unsigned)(units * p.kv.nkv), (unsigned)((rows + 31) / 32 * (16 * KB) / (kTcJoinThreads / 32))),
-                           dim3(kTcJoinThreads), 0, st, p, units));
+                           dim3(kTcJoinThreads), 0, st, p));
     return IM_OK;
 }
 

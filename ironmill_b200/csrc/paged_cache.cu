@@ -66,7 +66,7 @@ struct Append {
     long long ks, vs, qs, qos;
     const int *start, *pos;
     const void *cosc, *sinc;
-    int nh, tokens, max_pos, rot;
+    int nh, max_pos, rot;
 };
 
 // Four entries of a table at a multiple of four: rows have head_dim / 2 of them, a multiple of four.
@@ -363,7 +363,7 @@ IM_EXPORT int im_cuda_paged_append(im_device *dev, const im_paged_kv *kv, int la
     a.ks = k_stride; a.vs = v_stride; a.qs = q_stride; a.qos = q_out_stride;
     a.start = token_start_dev; a.pos = position_dev;
     a.cosc = cos_dev; a.sinc = sin_dev;
-    a.nh = num_heads; a.tokens = num_tokens; a.max_pos = max_pos; a.rot = rotary_dim;
+    a.nh = num_heads; a.max_pos = max_pos; a.rot = rotary_dim;
     int lanes = 1;
     while (lanes * 8 < kv->head_dim) lanes *= 2;
     const bool bf16 = kv->dtype == IM_DTYPE_BF16, f32 = table_dtype == IM_DTYPE_F32;
