@@ -301,6 +301,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             const uint32_t one = elected();
             const uint64_t qd = desc_sw128(smem_u32(Qs), 16), kd = desc_sw128(smem_u32(Ks), 16), vd = desc_sw128(smem_u32(Vs), BLK);
             int ks = 0, vs = 0, turn0 = 0, turn1 = 0;     // slots; weights of the halves that were waited for
+            int used0 = 0, used1 = 0;                     // items that the halves' accumulators were used for
             uint32_t kturn = 0, vturn = 0;                // parities of the slots' turns
             auto wait = [&](uint64_t *bar, uint32_t parity) {
                 if (ok && !mbar_try_wait(bar, parity)) ok = wait_for(bar, parity, err);
@@ -346,17 +347,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             while (it.next()) {
                 const int T = (int)uniform(it.t1 - it.t0);
                 wait(qfull, it.index & 1);
-                auto drained = [&]() {  // the outputs of the item before have been read
-                    if (it.index > 0) {
-                        wait(&oempty[0], (it.index - 1) & 1);
-                        wait(&oempty[1], (it.index - 1) & 1);
-                    }
+                auto drained = [&](int halves) {  // the outputs of the item before that these halves had rows of have been read
+                    if (used0 > 0) wait(&oempty[0], (used0 - 1) & 1);
+                    used0++;
+                    if (halves < 2) return;
+                    if (used1 > 0) wait(&oempty[1], (used1 - 1) & 1);
+                    used1++;
                 };
                 if constexpr (WIDE) {
                     const int halves = (int)uniform(it.u.rows > 128 ? 2 : 1);
 #pragma unroll 1
                     for (int t = 0; t <= T; t++) {
-                        if (t == 1) drained();
+                        if (t == 1) drained(halves);
 #pragma unroll 1
                         for (int h = 0; h < halves; h++) {
                             if (t > 0) {
@@ -375,7 +377,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 } else {
 #pragma unroll 1
                     for (int t = 0; t < T + 2; t++) {
-                        if (t == 2) drained();
+                        if (t == 2) drained(2);
                         if (t >= 2) {
                             wait(&vfull[vs], vturn);
                             values(t & 1, t < 4, t >= T);
@@ -557,7 +559,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             }
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&oempty[h]);
+            // (a wide tile's half without rows has nothing to wait for, and must not run ahead of the products' waits by phases of its own)
+            if (lane == 0 && (!WIDE || jobs > 0)) mbar_arrive(&oempty[h]);
             // Rows whose sums are not finite are noted and left to the joining launch: nothing here waits for them
             unsigned bad = __ballot_sync(0xffffffffu, live && !(worst == 0.0f));
             if constexpr (!WIDE) {  // the first half's warps note what either found

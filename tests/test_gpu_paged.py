@@ -932,3 +932,25 @@ def test_negative_lengths_count_as_zero_and_long_ones_as_the_table(dev, nodes, h
     assert all(torch.equal(a, b) for a, b in zip(*runs))
     k0 = runs[0][1]
     assert k0[0, table[0, 0], :, 0].any() and runs[0][4].tolist() == [3, 23, 3, 67]
+
+
+# ------------------------------------------------------------------------------------------------ ragged batches in wide tiles
+def _no_wait_ran_out(dev):
+    from ironmill_b200._lib import check, lib
+    check(lib().im_cuda_device_check_error(dev.handle))
+
+
+@pytest.mark.parametrize("dtype, dim, heads, kv_heads, new, most, max_new", [
+    ("bf16", 128, 32, 4, [200] + [1] * 31, 900, 200), ("f16", 128, 12, 3, [1] * 40 + [90], 700, 90), ("f16", 64, 20, 1, [1] * 60, 900, 21), ("bf16", 64, 16, 4, [0, 40, 3, 0, 17, 1, 1, 2, 33] * 4, 800, 60),
+    ("bf16", 128, 16, 4, [33, 1, 33, 1, 1, 33, 1, 1, 1, 33, 1], 3000, 33), ("f16", 128, 24, 3, [20, 5, 17, 16, 2], 5000, 40), ("bf16", 128, 32, 4, [80], 589, 130)])
+def test_wide_tiles_that_few_rows_of_a_sequence_fill(dev, dtype, dim, heads, kv_heads, new, most, max_new):
+    """Portions of prompts beside single tokens: a CTA has items one after the other whose rows leave half of its warps without any."""
+    rng = H.rng_for("ragged", most + heads)
+    lengths = [most, *rng.integers(0, most, len(new) - 1).tolist()]
+    c = Cache(dev, rng, [a + b for a, b in zip(lengths, new)], lengths, kv_heads=kv_heads, dim=dim, page=48, dtype=dtype)
+    first = _check_attention(dev, c, H.rng_for("ragged-q"), new, heads, dtype, max_new=max_new)[0]
+    _no_wait_ran_out(dev)
+    masks = np.concatenate([_tree(rng, n, -(-max_new // 64)) for n in new if n])
+    _check_attention(dev, c, H.rng_for("ragged-q"), new, heads, dtype, max_new=max_new, mask=masks, max_len=0)
+    _no_wait_ran_out(dev)
+    assert (_check_attention(dev, c, H.rng_for("ragged-q"), new, heads, dtype, max_new=max_new)[0] == first).all()
