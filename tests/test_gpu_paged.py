@@ -934,6 +934,20 @@ def test_negative_lengths_count_as_zero_and_long_ones_as_the_table(dev, nodes, h
     assert k0[0, table[0, 0], :, 0].any() and runs[0][4].tolist() == [3, 23, 3, 67]
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("groups, beams, vocab, picks", [(1, 3, 30001, 16), (2, 12, 5001, 64), (1, 1, 1025, 7), (30, 8, 20003, 9)])
+def test_thousands_of_equal_logits_in_rows_that_start_anywhere(dev, dtype, groups, beams, vocab, picks):
+    from ironmill_b200 import ops
+    rng = H.rng_for("few", vocab)
+    few = rng.integers(0, 4, (groups, vocab))
+    x = torch.from_numpy(np.repeat(few[:, None], beams, 1)).to(device="cuda", dtype=TYPES[dtype])
+    x[:, :, 2::5] = -np.inf
+    few[:, 2::5] = -1
+    _, parent, token = ops.beam_select(dev, x, torch.zeros((groups, beams), device="cuda"), picks)
+    for g in range(groups):
+        assert parent[g].tolist() == [0] * picks and token[g].tolist() == np.flatnonzero(few[g] == 3)[:picks].tolist()
+
+
 # ------------------------------------------------------------------------------------------------ ragged batches in wide tiles
 def _no_wait_ran_out(dev):
     from ironmill_b200._lib import check, lib
