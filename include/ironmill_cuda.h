@@ -337,7 +337,7 @@ int im_cuda_paged_append(im_device *dev, const im_paged_kv *kv, int layer, const
  * A row that sees nothing gets zeros; infinities and NaN in rows that a token does not see do not reach it.  f32 scores, sums
  * and accumulation, one rounding of the output.  Softmax weights enter their product as a sum of two terms of the cache's type (relative error
  * 2^-16 in bf16, 2^-22 in fp16), or as one (2^-8, 2^-11) in every sequence of a call with max_new * num_heads / num_kv_heads > 128 and heads
- * of 64 or 128; fp16 weights below 2^-26 of the row's largest are off by up to 2^-37 of it.  q, out: as q in paged_append; out does not lie over q.
+ * of 64 or 128; fp16 weights below 2^-26 of the row's largest are off by up to 2^-37 of it.  q, out: as q in paged_append; out lies over nothing that is read.
  * max_new: no sequence has more new tokens (further ones are left as they are).  max_len: no sequence has more rows, the new ones
  * included (0: the table's width); a smaller value costs time, not results.  scratch_dev: 16-byte aligned,
  * im_cuda_paged_attention_scratch_bytes for the same kv, heads, max_new and max_len (short contexts need none; those of a larger
@@ -349,7 +349,7 @@ int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int layer, co
 
 /* The accepted path of a tree: in every layer row seq_len + accepted_dev[s, j] becomes row seq_len + j, j = 0 .. count_dev[s] - 1
  * (accepted [num_seqs, max_accept], each path in order from the root: accepted[s, j] >= j; an entry below j is not moved).
- * seq_len_out_dev [num_seqs], not over what is read: seq_len + count. */
+ * seq_len_out_dev [num_seqs], not over what is read: seq_len + count.  At most 65535 sequences (paged_reorder too). */
 int im_cuda_paged_keep(im_device *dev, const im_paged_kv *kv, const int *accepted_dev, int max_accept, const int *count_dev, int *seq_len_out_dev,
                        void *stream);
 
@@ -359,7 +359,7 @@ int im_cuda_paged_keep(im_device *dev, const im_paged_kv *kv, const int *accepte
  * parent keeps its row; each further one shares the earlier pages and gets, in order, those that a beam without a child holds
  * alone (there are as many such beams), with the rows of the parent's last page copied to the first of them, in every layer; where its row
  * has more entries left than that beam's had, they become -1.  table_out_dev (rows table_out_stride apart, 0 = table_width) and seq_len_out_dev get the new rows and lengths; they may
- * not lie over what is read, nor over each other. */
+ * not lie over what is read, nor over each other.  Groups of at most 256. */
 int im_cuda_paged_reorder(im_device *dev, const im_paged_kv *kv, const int *parent_dev, int group, int *table_out_dev, int64_t table_out_stride,
                           int *seq_len_out_dev, void *stream);
 
@@ -369,7 +369,8 @@ int im_cuda_paged_reorder(im_device *dev, const im_paged_kv *kv, const int *pare
  * elements apart (0 = vocab); score_dev f32 [groups * beams].  done_dev (u8 [groups * beams] or NULL): a finished beam has one continuation,
  * end_token at its own score, and its logits are not read.  Values of -inf and NaN are not picked (nor anything of a beam whose logits
  * hold a NaN or +inf); where fewer than `picks` are left, the rest gets score -inf, parent -1 and token -1.
- * score_out f32 (not over score), parent_out (beam in the group) and token_out i32: [groups, picks].  1 <= beams <= 64, 1 <= picks <= 64.
+ * score_out f32, parent_out (beam in the group) and token_out i32: [groups, picks], over nothing that is read, nor over each other.
+ * 1 <= beams <= 64, 1 <= picks <= 64, groups * beams <= 65535.
  * Greedy decoding's pick (crates/ironmill-inference/src/sampling.rs:331-339) takes the last maximal index; this takes the first.
  * scratch_dev: 16-byte aligned, calls whose kernels may overlap need one each; few beams over few logits need none. */
 size_t im_cuda_beam_select_scratch_bytes(const im_device *dev, int groups, int beams, int vocab, int picks);

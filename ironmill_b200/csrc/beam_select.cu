@@ -11,7 +11,7 @@
 //                     A collected element's rank is the number of better ones. Where a list overflows (ties, rising rows) the elements are picked one
 //                     after the other from memory instead.
 //   joining           the same with the slices' picks as elements and 64-bit values.
-// Eight beams of 32 searches over 128256 f32 logits, 16 picks (131 MB): 31 us, of them 28 for the slices (4.7 TB/s, 72 % of a copy).
+// Eight beams of 32 searches over 128256 f32 logits, 16 picks (131 MB): 32 us, of them 28 for the slices (4.7 TB/s, 72 % of a copy).
 // Sums are f32 per thread over its elements with one running maximum, joined in a fixed order: a run repeats bit by bit. Which elements are a thread's
 // goes by their place in the row alone, wherever the row starts: equal rows get equal sums, and their candidates tie as they should.
 #include <cuda_bf16.h>

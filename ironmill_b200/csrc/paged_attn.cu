@@ -3,7 +3,7 @@
 //   out[t, h] = sum_j p_j v_j,  p = softmax over the visible rows j of scale * q[t, h] . k_j
 //
 // What bounds it is the read of K and V: every (sequence, KV head) is read once for all the rows (token, query head) that share it, here up
-// to 16 (more: paged_attn_tc.cu). 32 sequences of up to 8192 rows, 32 / 8 heads (579 MB): 103 us, 5.6 TB/s, 86 % of a copy. The tiles of 64 positions of all (row tile, KV head) items form one list, cut into equal shares, one per CTA, whatever the lengths
+// to 16 (more: paged_attn_tc.cu). 32 sequences of up to 8192 rows, 32 / 8 heads (579 MB): 106 us, 5.5 TB/s, 84 % of a copy. The tiles of 64 positions of all (row tile, KV head) items form one list, cut into equal shares, one per CTA, whatever the lengths
 // are; an item that a cut divides leaves partial sums, which a second launch joins.
 //
 // In a CTA four warps take 16 positions of each tile and work on their own: each keeps a ring of K and V slices (cp.async, 16 bytes per lane, rows

@@ -16,10 +16,11 @@
 // K, V and queries come by 16-byte cp.async of four warps, rows looked up in the page table: any page size, rows that are not there are zeros and
 // known to be none (a bit per row). The copies run ahead over the ends of items as far as the slots allow.
 //
-// Bounds. Up to 128 rows: the copies, 3200 clocks a tile of 64 KB (20 bytes a clock and SM, 5.6 TB/s), with some 13 us around them (eight sequences of up to 4001
-// rows: 34 us). WIDE: a half's chain, 2600 clocks of weights and as many for its products (64 clocks each), while the other half has its turn: a
-// sequence of 100003 rows and 256 rows of queries 138 us, 2.9 TB/s, 760 TFLOP/s. The loops are short on purpose: unrolled, the three kinds of warps
-// waited for instructions more than for anything else (286 us against 200 then).
+// Bounds. Up to 128 rows: the copies, 3200 clocks a tile of 64 KB (20 bytes a clock and SM, 5.6 TB/s). Eight sequences of up to 4001 rows, 34 us: 5.6 until a
+// CTA's first scores, 12.6 its tiles, 3.6 its outputs, 5.1 until the slowest CTA is there, 1.3 until the join starts, 5.6 the join. WIDE: a half's chain, 2600
+// clocks of weights and as many for its products (64 clocks each), while the other half has its turn: a sequence of 100003 rows and 256 rows of queries 141 us,
+// 2.9 TB/s, 745 TFLOP/s. The loops are short on purpose: unrolled, the three kinds of warps waited for instructions more than for anything else (286 us
+// against 200 then).
 //
 // All waits are bounded: one that runs out sets the device error word, every warp then runs to its end.
 #include <limits.h>

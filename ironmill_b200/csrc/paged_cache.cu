@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(kAppendThreads, FORM == 3 ? 2 : 5) paged_appen
 // A thread owns 16 bytes of a head's row in one layer of keys or values and moves them for j = 0, 1, ...: what row j receives
 // comes from a row at or behind it (accepted[j] >= j), so no source has been overwritten when it is read, and no thread waits for another.
 // Eight sources are requested before the first is written: a source among the eight targets is read first. 64 paths of up to 8 rows in 32
-// layers (76 MB): 10.5 us.
+// layers (76 MB): 10.5 to 12 us, by what L2 still holds.
 constexpr int kKeepThreads = 256, kKeepSeg = 256, kKeepAhead = 8;
 
 __global__ void __launch_bounds__(kKeepThreads)
