@@ -330,6 +330,17 @@ int im_cuda_paged_append(im_device *dev, const im_paged_kv *kv, int layer, const
                          const int *token_start_dev, int num_tokens, const void *q_dev, int64_t q_stride, void *q_out_dev, int64_t q_out_stride,
                          int num_heads, const void *cos_dev, const void *sin_dev, int table_dtype, int max_pos, int rotary_dim, int neighbours,
                          const int *position_dev, void *stream);
+/* The same with norms and positions of several axes.  Where q_norm_dev / k_norm_dev [head_dim] (norm_dtype: the cache's type or IM_DTYPE_F32; 16-byte aligned) are
+ * not NULL, every head of the queries / keys is x * rsqrt(mean(x^2) + eps) * w before it is rotated; f32 up to the one rounding behind the rotation
+ * (fused_qk_norm_rope, crates/ironmill-inference/src/metal/shaders/norm/fused_qk_norm_rope.metal:43-124, for contiguous caches: im_cuda_qk_norm_rope).
+ * num_axes 1 to 4.  More than one (time, height and width of images and video): position_dev [num_axes, num_tokens], and pair_axis_host [rotary_dim / 2] (read during
+ * the call) names the axis of every pair: pair i is rotated by entry i of the row of that axis's position.  A token with a row outside the table on any
+ * axis is neither written nor rotated.  One axis: as above, pair_axis_host is not read.  q_out_dev lies over none of the weights, tables and positions. */
+int im_cuda_paged_append_normed(im_device *dev, const im_paged_kv *kv, int layer, const void *k_dev, int64_t k_stride, const void *v_dev, int64_t v_stride,
+                                const int *token_start_dev, int num_tokens, const void *q_dev, int64_t q_stride, void *q_out_dev, int64_t q_out_stride,
+                                int num_heads, const void *cos_dev, const void *sin_dev, int table_dtype, int max_pos, int rotary_dim, int neighbours,
+                                const int *position_dev, const void *q_norm_dev, const void *k_norm_dev, int norm_dtype, float eps,
+                                const uint8_t *pair_axis_host, int num_axes, void *stream);
 
 /* out[t, h] = softmax(scale * q[t, h] . K^T) V of the new tokens, whose own rows are in the cache already.  Head h reads KV head
  * h / (num_heads / num_kv_heads).  A token sees all seq_len rows before the new ones, and of the new rows: without a mask its own and

@@ -205,6 +205,174 @@ __global__ void __launch_bounds__(kAppendThreads, FORM == 3 ? 2 : 5) paged_appen
     }
 }
 
+// ------------------------------------------------------------------------------------------------ append with norms and several axes
+//   y = x * rsqrt(mean(x^2) + eps) * w per head (keys and queries, each if it has weights), then pair i of y's columns turned by entry i of the table row
+//   of position[axis of i]; f32 from the load to the one rounding at the end.
+// The same blocks and lookups as above, but a lane owns both columns of its pairs (four of them: two words of 8 bytes, which lie side by side where
+// neighbours belong together and half of rotary_dim apart where the halves do), so that rotation exchanges nothing between lanes, and every cosine and sine
+// is loaded once instead of by both lanes of a pair. A head's sum of squares is the only exchange: log2(lanes) shuffles.
+constexpr int kAxes = 4;
+struct AppendMore {
+    const void *qn, *kn;  // weights or NULL
+    int norm_f32, axes;
+    float eps, inv_dim;
+    uint32_t axis[8];     // two bits a pair: 128 of them
+};
+
+// Four norm weights from column d on.
+template <bool BF16>
+__device__ __forceinline__ void weights4(const void *w, int f32, int d, float *out) {
+    if (f32) {
+        *reinterpret_cast<float4 *>(out) = __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(w) + d));
+    } else {
+        const uint2 u = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(w) + d));
+        const float2 lo = unpack16<BF16>(u.x), hi = unpack16<BF16>(u.y);
+        out[0] = lo.x; out[1] = lo.y; out[2] = hi.x; out[3] = hi.y;
+    }
+}
+
+// FORM: 0 halves, rotary_dim a multiple of 8; 1 neighbours (and rotary_dim 0); 2 halves of any even size, column by column.
+constexpr int kNormedHeads = 3;
+template <bool BF16, int FORM, bool F32>
+__global__ void __launch_bounds__(kAppendThreads, 3) paged_append_normed_kernel(const __grid_constant__ Append a, const __grid_constant__ AppendMore m, int lanes) {
+    pdl_trigger();
+    pdl_wait();
+    const int token = blockIdx.x, tid = threadIdx.x;
+    const int c = tid & (lanes - 1), first = tid / lanes, per = blockDim.x / lanes;
+    const int hd = a.kv.hd, heads = a.nh + 2 * a.kv.nkv, half = a.rot / 2;
+    const bool mine = 8 * c < hd;
+    // this lane's pairs 4 c .. 4 c + 3; the columns behind the rotated ones are pairs of neighbours that are not turned
+    const int e0 = 4 * c, colA = FORM == 0 && e0 < half ? e0 : 2 * e0, colB = FORM == 0 && e0 < half ? half + e0 : 2 * e0 + 4;
+    auto column = [&](int i) {  // FORM 2: of word i / 4, place i % 4
+        const int e = e0 + i % 4;
+        return e < half ? e + (i / 4) * half : 2 * e + i / 4;
+    };
+    auto source = [&](int h) {
+        return h < a.nh ? a.q + token * a.qs + (long long)h * hd
+                        : h < a.nh + a.kv.nkv ? a.k + token * a.ks + (long long)(h - a.nh) * hd : a.v + token * a.vs + (long long)(h - a.nh - a.kv.nkv) * hd;
+    };
+    bool placed = false;
+    long long at = -1;
+    float cs[4], sn[4], wq[8], wk[8];
+#pragma unroll 1
+    for (int h0 = first; h0 - first < heads; h0 += per * kNormedHeads) {  // the same count for every lane of a warp
+        uint2 x[kNormedHeads][2];
+#pragma unroll
+        for (int i = 0; i < kNormedHeads; i++) {
+            const int h = h0 + i * per;
+            x[i][0] = x[i][1] = make_uint2(0, 0);
+            if (mine && h < heads) {
+                const uint16_t *src = source(h);
+                if (FORM < 2) {
+                    x[i][0] = *reinterpret_cast<const uint2 *>(src + colA);
+                    x[i][1] = *reinterpret_cast<const uint2 *>(src + colB);
+                } else {
+                    uint16_t v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[j] = src[column(j)];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) x[i][j] = make_uint2(v[4 * j] | (uint32_t)v[4 * j + 1] << 16, v[4 * j + 2] | (uint32_t)v[4 * j + 3] << 16);
+                }
+            }
+        }
+        if (!placed) {
+            placed = true;
+            const int lo = __ldg(a.start), hi = __ldg(a.start + a.kv.nseq);
+            if (token < lo || token >= hi) return;
+            const int seq = paged_seq_of(a.start, a.kv.nseq, token), place = token - __ldg(a.start + seq);
+            const long long r = (long long)a.kv.length(seq) + place;
+            if (place < 0 || r > INT_MAX) return;
+            if (a.rot > 0) {
+                int p[kAxes];
+                bool there = true;
+#pragma unroll
+                for (int k = 0; k < kAxes; k++) {
+                    p[k] = k >= m.axes ? 0 : a.pos ? __ldg(a.pos + (long long)k * gridDim.x + token) : (int)r;
+                    there = there && (unsigned)p[k] < (unsigned)a.max_pos;
+                }
+                if (!there) return;
+                const uint32_t axes = m.axis[(c >> 2) & 7] >> (8 * (c & 3));  // (sixteen pairs a word)
+#pragma unroll
+                for (int j = 0; j < 4; j++) cs[j] = 1.0f, sn[j] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < kAxes; k++) {  // the rows of the axes that this lane's pairs have
+                    bool any = false;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) any = any || (e0 + j < half && (axes >> (2 * j) & 3) == k);
+                    if (!any) continue;
+                    float s[4], t[4];
+                    angles4<F32>(a.cosc, (long long)p[k] * (hd / 2) + e0, s);
+                    angles4<F32>(a.sinc, (long long)p[k] * (hd / 2) + e0, t);
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (e0 + j < half && (axes >> (2 * j) & 3) == k) cs[j] = s[j], sn[j] = t[j];
+                }
+            }
+            if (mine) {
+                if (FORM < 2) {
+                    if (m.qn) weights4<BF16>(m.qn, m.norm_f32, colA, wq), weights4<BF16>(m.qn, m.norm_f32, colB, wq + 4);
+                    if (m.kn) weights4<BF16>(m.kn, m.norm_f32, colA, wk), weights4<BF16>(m.kn, m.norm_f32, colB, wk + 4);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const int d = column(j);
+                        if (m.qn) wq[j] = m.norm_f32 ? __ldg(static_cast<const float *>(m.qn) + d) : one16<BF16>(static_cast<const uint16_t *>(m.qn) + d);
+                        if (m.kn) wk[j] = m.norm_f32 ? __ldg(static_cast<const float *>(m.kn) + d) : one16<BF16>(static_cast<const uint16_t *>(m.kn) + d);
+                    }
+                }
+            }
+            at = a.kv.row_of(seq, (int)r);
+        }
+#pragma unroll
+        for (int i = 0; i < kNormedHeads; i++) {
+            const int h = h0 + i * per;
+            const bool is_q = h < a.nh, is_v = h >= a.nh + a.kv.nkv;
+            float f[8];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const float2 lo = unpack16<BF16>(x[i][j].x), hi = unpack16<BF16>(x[i][j].y);
+                f[4 * j] = lo.x; f[4 * j + 1] = lo.y; f[4 * j + 2] = hi.x; f[4 * j + 3] = hi.y;
+            }
+            if (m.qn || m.kn) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) sum = fmaf(f[j], f[j], sum);
+                for (int o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                if (is_q ? m.qn != nullptr : !is_v && m.kn != nullptr) {
+                    const float r = rsqrtf(fmaf(sum, m.inv_dim, m.eps));
+#pragma unroll
+                    for (int j = 0; j < 8; j++) f[j] = f[j] * r * (is_q ? wq[j] : wk[j]);
+                }
+            }
+            if (!mine || h >= heads) continue;
+            uint2 y[2] = {x[i][0], x[i][1]};
+            if (!is_v) {
+                if (a.rot > 0) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        if (e0 + j >= half) continue;  // not turned
+                        float &p = f[FORM == 1 ? 2 * j : j], &q = f[FORM == 1 ? 2 * j + 1 : 4 + j];
+                        const float u = p * cs[j] - q * sn[j], v = q * cs[j] + p * sn[j];
+                        p = u;
+                        q = v;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 2; j++) y[j] = make_uint2(pack16<BF16>(f[4 * j], f[4 * j + 1]), pack16<BF16>(f[4 * j + 2], f[4 * j + 3]));
+            }
+            if (!is_q && at < 0) continue;
+            uint16_t *to = is_q ? a.qo + token * a.qos + (long long)h * hd : (is_v ? a.vc : a.kc) + at + (long long)(is_v ? h - a.nh - a.kv.nkv : h - a.nh) * a.kv.page * hd;
+            if (FORM < 2) {
+                *reinterpret_cast<uint2 *>(to + colA) = y[0];
+                *reinterpret_cast<uint2 *>(to + colB) = y[1];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) to[column(j)] = (uint16_t)((j & 2 ? y[j / 4].y : y[j / 4].x) >> (16 * (j & 1)));
+            }
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ keep
 // A thread owns 16 bytes of a head's row in one layer of keys or values and moves them for j = 0, 1, ...: what row j receives
 // comes from a row at or behind it (accepted[j] >= j), so no source has been overwritten when it is read, and no thread waits for another.
@@ -323,18 +491,22 @@ __global__ void __launch_bounds__(kReorderThreads)
 }  // namespace im
 
 // ---- C ABI ------------------------------------------------------------------------------------------------------
-IM_EXPORT int im_cuda_paged_append(im_device *dev, const im_paged_kv *kv, int layer, const void *k_dev, int64_t k_stride, const void *v_dev, int64_t v_stride,
-                                   const int *token_start_dev, int num_tokens, const void *q_dev, int64_t q_stride, void *q_out_dev, int64_t q_out_stride,
-                                   int num_heads, const void *cos_dev, const void *sin_dev, int table_dtype, int max_pos, int rotary_dim, int neighbours,
-                                   const int *position_dev, void *stream) {
-    IM_GUARD_BEGIN
-    using namespace im;
-    Append a;
+namespace im {
+namespace {
+
+// What the calls that append have in common: their arguments checked, the kernels' filled in. empty: there is nothing to do.
+int append_args(im_device *dev, const im_paged_kv *kv, int layer, const void *k_dev, int64_t k_stride, const void *v_dev, int64_t v_stride, const int *token_start_dev,
+                int num_tokens, const void *q_dev, int64_t q_stride, void *q_out_dev, int64_t q_out_stride, int num_heads, const void *cos_dev, const void *sin_dev,
+                int table_dtype, int max_pos, int rotary_dim, int neighbours, const int *position_dev, Append *a, bool *empty) {
+    *empty = false;
     IM_REQUIRE(layer >= 0, "layer %d", layer);
-    int rc = paged_view(kv, layer, &a.kv);
+    int rc = paged_view(kv, layer, &a->kv);
     if (rc != IM_OK) return rc;
     IM_REQUIRE(num_tokens >= 0, "bad argument");
-    if (num_tokens == 0 || kv->num_seqs == 0) return paged_device(dev);
+    if (num_tokens == 0 || kv->num_seqs == 0) {
+        *empty = true;
+        return paged_device(dev);
+    }
     IM_REQUIRE(k_dev && v_dev && token_start_dev, "bad argument");
     IM_REQUIRE(!q_dev == !q_out_dev && (q_dev ? num_heads > 0 : num_heads == 0), "queries need their output and number of heads");
     const int64_t row = (int64_t)kv->num_kv_heads * kv->head_dim, q_row = (int64_t)num_heads * kv->head_dim, most = (int64_t)1 << 40;
@@ -353,19 +525,42 @@ IM_EXPORT int im_cuda_paged_append(im_device *dev, const im_paged_kv *kv, int la
     IM_REQUIRE(neighbours == 0 || neighbours == 1, "neighbours is 0 or 1");
     rc = paged_device(dev);
     if (rc != IM_OK) return rc;
-    const int64_t at = layer * (int64_t)a.kv.layer_stride;
-    a.kc = static_cast<uint16_t *>(kv->k_dev) + at;
-    a.vc = static_cast<uint16_t *>(kv->v_dev) + at;
-    a.k = static_cast<const uint16_t *>(k_dev);
-    a.v = static_cast<const uint16_t *>(v_dev);
-    a.q = static_cast<const uint16_t *>(q_dev);
-    a.qo = static_cast<uint16_t *>(q_out_dev);
-    a.ks = k_stride; a.vs = v_stride; a.qs = q_stride; a.qos = q_out_stride;
-    a.start = token_start_dev; a.pos = position_dev;
-    a.cosc = cos_dev; a.sinc = sin_dev;
-    a.nh = num_heads; a.max_pos = max_pos; a.rot = rotary_dim;
+    const int64_t at = layer * (int64_t)a->kv.layer_stride;
+    a->kc = static_cast<uint16_t *>(kv->k_dev) + at;
+    a->vc = static_cast<uint16_t *>(kv->v_dev) + at;
+    a->k = static_cast<const uint16_t *>(k_dev);
+    a->v = static_cast<const uint16_t *>(v_dev);
+    a->q = static_cast<const uint16_t *>(q_dev);
+    a->qo = static_cast<uint16_t *>(q_out_dev);
+    a->ks = k_stride; a->vs = v_stride; a->qs = q_stride; a->qos = q_out_stride;
+    a->start = token_start_dev; a->pos = position_dev;
+    a->cosc = cos_dev; a->sinc = sin_dev;
+    a->nh = num_heads; a->max_pos = max_pos; a->rot = rotary_dim;
+    return IM_OK;
+}
+
+// Lanes that hold a head.
+int append_lanes(int head_dim) {
     int lanes = 1;
-    while (lanes * 8 < kv->head_dim) lanes *= 2;
+    while (lanes * 8 < head_dim) lanes *= 2;
+    return lanes;
+}
+
+}  // namespace
+}  // namespace im
+
+IM_EXPORT int im_cuda_paged_append(im_device *dev, const im_paged_kv *kv, int layer, const void *k_dev, int64_t k_stride, const void *v_dev, int64_t v_stride,
+                                   const int *token_start_dev, int num_tokens, const void *q_dev, int64_t q_stride, void *q_out_dev, int64_t q_out_stride,
+                                   int num_heads, const void *cos_dev, const void *sin_dev, int table_dtype, int max_pos, int rotary_dim, int neighbours,
+                                   const int *position_dev, void *stream) {
+    IM_GUARD_BEGIN
+    using namespace im;
+    Append a;
+    bool empty;
+    const int rc = append_args(dev, kv, layer, k_dev, k_stride, v_dev, v_stride, token_start_dev, num_tokens, q_dev, q_stride, q_out_dev, q_out_stride, num_heads, cos_dev, sin_dev,
+                               table_dtype, max_pos, rotary_dim, neighbours, position_dev, &a, &empty);
+    if (rc != IM_OK || empty) return rc;
+    const int lanes = append_lanes(kv->head_dim);
     const bool bf16 = kv->dtype == IM_DTYPE_BF16, f32 = table_dtype == IM_DTYPE_F32;
     const int form = rotary_dim == 0 ? 0 : neighbours ? 2 : rotary_dim % 16 == 0 ? 1 : 3;
     void (*kern)(Append, int) = nullptr;
@@ -378,6 +573,48 @@ IM_EXPORT int im_cuda_paged_append(im_device *dev, const im_paged_kv *kv, int la
     }
 #undef IM_FORM
     IM_CUDA_CHECK(launch_k(kern, dim3((unsigned)num_tokens), dim3(num_tokens > 4 * dev->sm_count ? kAppendSmall : kAppendThreads), 0, as_stream(stream), a, lanes));
+    return IM_OK;
+    IM_GUARD_END
+}
+
+IM_EXPORT int im_cuda_paged_append_normed(im_device *dev, const im_paged_kv *kv, int layer, const void *k_dev, int64_t k_stride, const void *v_dev, int64_t v_stride,
+                                          const int *token_start_dev, int num_tokens, const void *q_dev, int64_t q_stride, void *q_out_dev, int64_t q_out_stride,
+                                          int num_heads, const void *cos_dev, const void *sin_dev, int table_dtype, int max_pos, int rotary_dim, int neighbours,
+                                          const int *position_dev, const void *q_norm_dev, const void *k_norm_dev, int norm_dtype, float eps, const uint8_t *pair_axis_host,
+                                          int num_axes, void *stream) {
+    IM_GUARD_BEGIN
+    using namespace im;
+    IM_REQUIRE(!q_norm_dev || q_dev, "norm weights of queries without queries");
+    IM_REQUIRE((!q_norm_dev && !k_norm_dev) || (kv && (norm_dtype == IM_DTYPE_F32 || norm_dtype == kv->dtype)), "norm weights are of the cache's type or f32 (got dtype %d)", norm_dtype);
+    IM_REQUIRE(aligned16(q_norm_dev) && aligned16(k_norm_dev), "norm weights have to be 16-byte aligned");
+    IM_REQUIRE(eps >= 0.0f && eps - eps == 0.0f, "eps has to be finite and not negative");
+    IM_REQUIRE(num_axes >= 1 && num_axes <= kAxes, "%d axes (at most %d)", num_axes, kAxes);
+    IM_REQUIRE(num_axes == 1 || (rotary_dim > 0 && position_dev && pair_axis_host), "several axes need a rotation, positions and the axis of every pair");
+    Append a;
+    bool empty;
+    const int rc = append_args(dev, kv, layer, k_dev, k_stride, v_dev, v_stride, token_start_dev, num_tokens, q_dev, q_stride, q_out_dev, q_out_stride, num_heads, cos_dev, sin_dev,
+                               table_dtype, max_pos, rotary_dim, neighbours, position_dev, &a, &empty);
+    if (rc != IM_OK || empty) return rc;
+    AppendMore m{};
+    m.qn = q_norm_dev; m.kn = k_norm_dev;
+    m.norm_f32 = norm_dtype == IM_DTYPE_F32;
+    m.axes = num_axes;
+    m.eps = eps;
+    m.inv_dim = 1.0f / kv->head_dim;
+    for (int i = 0; num_axes > 1 && i < rotary_dim / 2; i++) {
+        IM_REQUIRE(pair_axis_host[i] < num_axes, "pair %d on axis %d of %d", i, pair_axis_host[i], num_axes);
+        m.axis[i / 16] |= (uint32_t)pair_axis_host[i] << (2 * (i % 16));
+    }
+    const int lanes = append_lanes(kv->head_dim);
+    const bool bf16 = kv->dtype == IM_DTYPE_BF16, f32 = table_dtype == IM_DTYPE_F32;
+    void (*kern)(Append, AppendMore, int) = nullptr;
+#define IM_FORM(F) \
+    (bf16 ? (f32 ? paged_append_normed_kernel<true, F, true> : paged_append_normed_kernel<true, F, false>) : (f32 ? paged_append_normed_kernel<false, F, true> : paged_append_normed_kernel<false, F, false>))
+    if (neighbours || rotary_dim == 0) kern = IM_FORM(1);
+    else if (rotary_dim % 8 == 0) kern = IM_FORM(0);
+    else kern = IM_FORM(2);
+#undef IM_FORM
+    IM_CUDA_CHECK(launch_k(kern, dim3((unsigned)num_tokens), dim3(num_tokens > 4 * dev->sm_count ? kAppendSmall : kAppendThreads), 0, as_stream(stream), a, m, lanes));
     return IM_OK;
     IM_GUARD_END
 }

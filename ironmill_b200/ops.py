@@ -466,11 +466,20 @@ class PagedKV:
         self.scratch_bytes = {}  # of attention, by heads and new tokens
 
 
-def paged_append(kv: PagedKV, layer: int, k, v, token_start, q=None, cos=None, sin=None, positions=None, rotary_dim=None, neighbours=False, q_out=None):
+def _norm_of(w, dim: int, dtype, ordinal: int):
+    """(address, type) of the norm weights of a head."""
+    assert w.shape == (dim,) and w.dtype in (dtype, torch.float32) and w.is_contiguous() and w.get_device() == ordinal, (w.shape, w.dtype, w.device)
+    return w.data_ptr(), _DTYPES[w.dtype]
+
+
+def paged_append(kv: PagedKV, layer: int, k, v, token_start, q=None, cos=None, sin=None, positions=None, rotary_dim=None, neighbours=False, q_out=None, q_norm=None,
+                 k_norm=None, eps=1e-6, pair_axis=None):
     """Keys and values [tokens, kv_heads, head_dim] of new tokens into the pages, keys and queries q [tokens, heads, head_dim] rotated on the
     way (returned in q_out, which may be q). token_start int32 [sequences + 1]; cos, sin [positions, head_dim / 2] fp16 or f32; positions
     int32 [tokens]: rows of the tables, where they are not the rows of the cache; neighbours: columns (2 i, 2 i + 1) belong together
-    instead of the halves'. Without tables nothing is rotated."""
+    instead of the halves'. Without tables nothing is rotated. q_norm, k_norm [head_dim] (the cache's type or f32, both of one): every head becomes
+    x / sqrt(mean(x^2) + eps) * w before it is rotated. pair_axis (bytes, one for each of the rotary_dim / 2 pairs): pair i is rotated by positions[pair_axis[i]],
+    positions int32 [axes, tokens], up to four axes."""
     n, dim, dtype, on = k.shape[0], kv.head_dim, kv.dtype, kv.ordinal
     ks, vs = _rows_of(k, n, kv.kv_heads, dim, dtype, on), _rows_of(v, n, kv.kv_heads, dim, dtype, on)
     heads = qs = qos = max_pos = table = 0
@@ -495,8 +504,27 @@ def paged_append(kv: PagedKV, layer: int, k, v, token_start, q=None, cos=None, s
     else:
         assert sin is None and not rotary_dim
         rotary_dim = 0
-    _launch(on, lib().im_cuda_paged_append, kv.dev.handle, kv.ref, layer, k.data_ptr(), ks, v.data_ptr(), vs, _ints(token_start, on, kv.num_seqs + 1), n, qp, qs, op, qos,
-            heads, cp, sp, table, max_pos, rotary_dim, 1 if neighbours else 0, None if positions is None else _ints(positions, on, n))
+    args = (kv.dev.handle, kv.ref, layer, k.data_ptr(), ks, v.data_ptr(), vs, _ints(token_start, on, kv.num_seqs + 1), n, qp, qs, op, qos, heads, cp, sp, table, max_pos, rotary_dim,
+            1 if neighbours else 0)
+    if q_norm is None and k_norm is None and pair_axis is None:
+        _launch(on, lib().im_cuda_paged_append, *args, None if positions is None else _ints(positions, on, n))
+        return q_out
+    axes, at = 1, None
+    if pair_axis is not None:
+        axes = positions.shape[0]
+        assert len(pair_axis) == rotary_dim // 2, (len(pair_axis), rotary_dim)
+        at, pair_axis = _ints(positions, on, axes, n) if n else None, bytes(pair_axis)
+    elif positions is not None:
+        at = _ints(positions, on, n)
+    qw = kw = None
+    norm = kind = 0
+    if q_norm is not None:
+        qw, norm = _norm_of(q_norm, dim, dtype, on)
+    if k_norm is not None:
+        kw, kind = _norm_of(k_norm, dim, dtype, on)
+        assert qw is None or kind == norm, (q_norm.dtype, k_norm.dtype)
+        norm = kind
+    _launch(on, lib().im_cuda_paged_append_normed, *args, at, qw, kw, norm, eps, pair_axis if axes > 1 else None, axes)
     return q_out
 
 
