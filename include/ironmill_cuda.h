@@ -358,6 +358,18 @@ int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int layer, co
                             int num_heads, const int *token_start_dev, int num_tokens, int max_new, const uint64_t *mask_dev, int mask_words,
                             float scale, int max_len, void *scratch_dev, size_t scratch_bytes, void *stream);
 
+/* The same where sequences share their first pages: those are read once for all the sequences of a group (one instruction before many prompts, one prompt
+ * before many answers).  Group g has the sequences group_start_dev[g] .. group_start_dev[g + 1] - 1 (group_start [num_groups + 1], not decreasing); the
+ * first prefix_pages_dev[g] entries of their table rows are the same, and each has at least those pages' rows before its new tokens (what comes out otherwise is
+ * unspecified).  Sequences before the first group and from the last one's end on share nothing.  A group's new tokens count one after
+ * the other; max_group_new: no group has more (further ones are left as they are).  max_prefix: no group shares more rows (0: the table's width), max_len: as above; smaller
+ * values cost time, not results.  Weights enter their product as in paged_attention, by the rows of a group for the shared pages. */
+size_t im_cuda_paged_prefix_attention_scratch_bytes(const im_device *dev, const im_paged_kv *kv, int num_heads, int max_new, int num_groups, int max_group_new);
+int im_cuda_paged_prefix_attention(im_device *dev, const im_paged_kv *kv, int layer, const void *q_dev, int64_t q_stride, void *out_dev, int64_t out_stride,
+                                   int num_heads, const int *token_start_dev, int num_tokens, int max_new, const int *group_start_dev, int num_groups,
+                                   int max_group_new, const int *prefix_pages_dev, int max_prefix, const uint64_t *mask_dev, int mask_words, float scale,
+                                   int max_len, void *scratch_dev, size_t scratch_bytes, void *stream);
+
 /* The accepted path of a tree: in every layer row seq_len + accepted_dev[s, j] becomes row seq_len + j, j = 0 .. count_dev[s] - 1
  * (accepted [num_seqs, max_accept], each path in order from the root: accepted[s, j] >= j; an entry below j is not moved).
  * seq_len_out_dev [num_seqs], not over what is read: seq_len + count.  At most 65535 sequences (paged_reorder too). */

@@ -53,7 +53,7 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uin
 
 // CL: instead of shares of the list of all tiles, a cluster of CTAs per item, each with an equal run of its tiles; they join what they have
 // through each other's shared memory, in the same launch and without scratch.
-template <bool BF16, int HD, bool CL>
+template <bool BF16, int HD, bool CL, int MODE>
 __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kernel(const __grid_constant__ PagedAttn p, int units) {
     using S = PaShape<HD>;
     // fp16 weights: 2^15 at the row's maximum instead of 1, so that they are normal numbers down to 2^-29 of it (exact to 2^-40 below)
@@ -77,25 +77,25 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
         const int C = (int)cluster_size(), item = blockIdx.x / C, rank = (int)cluster_rank();
         share.unit = item / p.kv.nkv;
         share.head = item - share.unit * p.kv.nkv;
-        f_u = paged_unit<R>(p, share.unit);
-        const int n = unit_tiles<kPaTile>(f_u);
+        f_u = paged_unit<R, MODE>(p, share.unit);
+        const int n = unit_tiles<kPaTile, MODE>(f_u);
         if (n == 0) return;  // all of the cluster
         share.from = share.tile = (int)((long long)n * rank / C);
         share.to = (long long)n * (rank + 1) / C;
     } else {
-        share = units <= 32 ? warp_share<R, kPaTile>(p, units, f_u) : find_share<R, kPaTile, kPaThreads>(p, units, sums, f_u);
+        share = units <= 32 ? warp_share<R, kPaTile, MODE>(p, units, f_u) : find_share<R, kPaTile, kPaThreads, MODE>(p, units, sums, f_u);
         if (share.from >= share.to) return;
     }
     const int count = (int)(share.to - share.from);
 
     // ---- the copies' cursor: one slice ahead of the copies, so that a page number is there when it is needed
     int f_unit = share.unit, f_head = share.head, f_tile = share.tile, f_left = count;
-    int f_tiles = unit_tiles<kPaTile>(f_u);
+    int f_tiles = unit_tiles<kPaTile, MODE>(f_u);
     int n_page = -1, n_slot = 0, n_head = 0;  // of the slice that is copied next: this lane's row (lane & 15)
     auto fetch = [&]() {
         n_page = -1;
         if (f_left <= 0) return;
-        const int pos = f_tile * kPaTile + warp * kPaSlice + (lane & 15);
+        const int pos = unit_from<MODE>(f_u) + f_tile * kPaTile + warp * kPaSlice + (lane & 15);
         if (pos < f_u.end) {
             const int pg = pos / p.kv.page;
             n_slot = pos - pg * p.kv.page;
@@ -108,8 +108,8 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
             if (++f_head == p.kv.nkv) {
                 f_head = 0;
                 while (f_left > 0 && ++f_unit < units) {
-                    f_u = paged_unit<R>(p, f_unit);
-                    f_tiles = unit_tiles<kPaTile>(f_u);
+                    f_u = paged_unit<R, MODE>(p, f_unit);
+                    f_tiles = unit_tiles<kPaTile, MODE>(f_u);
                     if (f_tiles > 0) break;
                 }
             }
@@ -152,8 +152,8 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
     bool first_item = true;
     int odd_item = 0;
     while (done < count) {
-        PagedUnit u = paged_unit<R>(p, unit);
-        const int tiles = unit_tiles<kPaTile>(u);
+        PagedUnit u = paged_unit<R, MODE>(p, unit);
+        const int tiles = unit_tiles<kPaTile, MODE>(u);
         if (tiles == 0) {
             unit++;
             continue;
@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
                     mma16<BF16>(s[1], qf[ks], b[2], b[3]);
                 }
             }
-            const int pos0 = tile * kPaTile + warp * kPaSlice;
+            const int pos0 = unit_from<MODE>(u) + tile * kPaTile + warp * kPaSlice;
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
@@ -274,9 +274,9 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
         }
         __syncthreads();
         if (tid == 0) bad_rows[!odd_item] = 0;  // every thread has looked at the last item's
-        const bool whole = !CL && t0 == 0 && t1 == tiles;
-        const size_t part = ((size_t)blockIdx.x * 2 + (first_item ? 0 : 1)) * R;
-        if (!CL && tid == 0) note_span(p, unit, head, t0, t1, tiles, blockIdx.x, first_item ? 0 : 1);
+        const bool whole = MODE == kAttend && !CL && t0 == 0 && t1 == tiles;
+        const size_t part = part_slot<MODE>(p, unit, head, t0, t1, tiles, blockIdx.x, first_item ? 0 : 1) * R;
+        if (!CL && tid == 0) note_span<MODE>(p, unit, head, t0, t1, tiles, blockIdx.x, first_item ? 0 : 1);
         float f[2];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
             for (int r = warp; r < u.rows; r += kPaWarps) {
                 if (!(bad >> r & 1)) continue;
                 float x[HD / 32], M, L;
-                plain_row<BF16, HD>(p, u, head, r, t0 * kPaTile, min(t1 * kPaTile, u.end), x, M, L);
+                plain_row<BF16, HD>(p, u, head, r, unit_from<MODE>(u) + t0 * kPaTile, min(unit_from<MODE>(u) + t1 * kPaTile, u.end), x, M, L);
                 const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
                 const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
                 for (int i = 0; i < HD / 32; i++) {
@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
         const int C = (int)cluster_size(), rank = (int)cluster_rank();
         if (count == 0 && tid < R) joint[tid] = make_float2(-INFINITY, 0.0f);
         cluster_sync();
-        const PagedUnit u = paged_unit<R>(p, share.unit);
+        const PagedUnit u = paged_unit<R, MODE>(p, share.unit);
         for (int i = rank * kPaThreads + tid; i < u.rows * CH; i += C * kPaThreads) {
             const int r = i / CH, c = i % CH * 8;
             float M = -INFINITY, L = 0.0f, o[8];
@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __gri
     pdl_wait();
     const int item = blockIdx.x, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, lane = threadIdx.x & 31, r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5);
     const int2 span = *reinterpret_cast<const int2 *>(p.spans + 2 * (long long)item);
-    const PagedUnit u = paged_unit<R>(p, unit);
+    const PagedUnit u = paged_unit<R, kAttend>(p, unit);
     if (r >= u.rows || span.x < 0) return;  // (a unit without tiles has no rows)
     const size_t slot0 = span.x;
     const int c = span.x >> 1, parts = span.y - c + 1;
@@ -494,15 +494,38 @@ int attn_launch(const Device *dev, const PagedAttn &p, int units, int cluster, c
     using S = PaShape<HD>;
     static DeviceOnce once;
     if (once.first(dev->ordinal)) {
-        IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, false>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
-        IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, true>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+        IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, false, kAttend>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+        IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, true, kAttend>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     }
     if (cluster) {
-        IM_CUDA_CHECK(launch_cluster(paged_attn_kernel<BF16, HD, true>, dim3((unsigned)(units * p.kv.nkv * cluster)), dim3(kPaThreads), cluster, (size_t)S::kSmem, st, p, units));
+        IM_CUDA_CHECK(launch_cluster(paged_attn_kernel<BF16, HD, true, kAttend>, dim3((unsigned)(units * p.kv.nkv * cluster)), dim3(kPaThreads), cluster, (size_t)S::kSmem, st, p, units));
         return IM_OK;
     }
-    IM_CUDA_CHECK(launch_k(paged_attn_kernel<BF16, HD, false>, dim3(p.ctas), dim3(kPaThreads), (size_t)S::kSmem, st, p, units));
+    IM_CUDA_CHECK(launch_k(paged_attn_kernel<BF16, HD, false, kAttend>, dim3(p.ctas), dim3(kPaThreads), (size_t)S::kSmem, st, p, units));
     return join_launch<BF16, S::kRows, HD>(p, units, st);
+}
+
+template <bool BF16, int HD, int MODE>
+int part_launch(const Device *dev, const PagedAttn &p, int units, cudaStream_t st) {
+    using S = PaShape<HD>;
+    static DeviceOnce once;
+    if (once.first(dev->ordinal)) IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, false, MODE>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+    IM_CUDA_CHECK(launch_k(paged_attn_kernel<BF16, HD, false, MODE>, dim3(p.ctas), dim3(kPaThreads), (size_t)S::kSmem, st, p, units));
+    return IM_OK;
+}
+
+}  // namespace
+
+int paged_part_launch(const Device *dev, const PagedAttn &p, bool bf16, int mode, int units, cudaStream_t st) {
+#define IM_MODE(B, HD) (mode == kShared ? part_launch<B, HD, kShared>(dev, p, units, st) : part_launch<B, HD, kOwn>(dev, p, units, st))
+#define IM_RUN(HD) (bf16 ? IM_MODE(true, HD) : IM_MODE(false, HD))
+    switch (p.kv.hd) {
+    case 64: return IM_RUN(64);
+    case 128: return IM_RUN(128);
+    default: return IM_RUN(256);
+    }
+#undef IM_RUN
+#undef IM_MODE
 }
 
 // Rows that no sequence passes.
@@ -517,7 +540,44 @@ int attn_check(const im_paged_kv *kv, int num_heads, int max_new) {
     return IM_OK;
 }
 
-}  // namespace
+// What calls have in common: their arguments checked, p filled in but for the plan. empty: there is nothing to do.
+int attn_args(im_device *dev, const im_paged_kv *kv, int layer, const void *q_dev, int64_t q_stride, void *out_dev, int64_t out_stride, int num_heads,
+              const int *token_start_dev, int num_tokens, int max_new, const uint64_t *mask_dev, int mask_words, float scale, int max_len, PagedAttn *p, bool *empty) {
+    *empty = false;
+    IM_REQUIRE(layer >= 0, "layer %d", layer);
+    int rc = paged_view(kv, layer, &p->kv);
+    if (rc == IM_OK) rc = attn_check(kv, num_heads, max_new);
+    if (rc != IM_OK) return rc;
+    IM_REQUIRE(num_tokens >= 0 && max_len >= 0, "bad argument");
+    if (num_tokens == 0 || kv->num_seqs == 0) {
+        *empty = true;
+        return paged_device(dev);
+    }
+    IM_REQUIRE(q_dev && out_dev && token_start_dev, "bad argument");
+    const int64_t row = (int64_t)num_heads * kv->head_dim, most = (int64_t)1 << 40;
+    IM_REQUIRE(q_stride >= row && out_stride >= row && q_stride <= most && out_stride <= most && q_stride % 8 == 0 && out_stride % 8 == 0 && aligned16(q_dev) && aligned16(out_dev),
+               "rows of queries and outputs have to be 16-byte aligned and apart");
+    IM_REQUIRE(!share_rows(q_dev, 2 * q_stride, out_dev, 2 * out_stride, 2 * row, num_tokens), "the outputs lie over the queries");
+    IM_REQUIRE(!mask_dev || (mask_words >= 1 && mask_words <= 1 << 20), "a mask of %d words a token", mask_words);
+    IM_REQUIRE(scale == scale && scale - scale == 0.0f, "scale is not finite");
+    rc = paged_device(dev);
+    if (rc != IM_OK) return rc;
+    const int64_t at = layer * (int64_t)p->kv.layer_stride;
+    p->kc = static_cast<const uint16_t *>(kv->k_dev) + at;
+    p->vc = static_cast<const uint16_t *>(kv->v_dev) + at;
+    p->q = static_cast<const uint16_t *>(q_dev);
+    p->out = static_cast<uint16_t *>(out_dev);
+    p->qs = q_stride; p->os = out_stride;
+    p->start = token_start_dev;
+    p->mask = mask_dev; p->mask_words = mask_words;
+    p->group = num_heads / kv->num_kv_heads; p->tokens = num_tokens; p->max_new = max_new;
+    p->scale2 = scale * 1.4426950408889634f;
+    if (p->scale2 == 0.0f) p->scale2 = 1e-30f;  // every position alike, without 0 * inf at the hidden ones
+    p->group_start = p->prefix_pages = nullptr;
+    p->groups = p->whole_slot = 0;
+    return IM_OK;
+}
+
 }  // namespace im
 
 IM_EXPORT size_t im_cuda_paged_attention_scratch_bytes(const im_device *dev, const im_paged_kv *kv, int num_heads, int max_new, int max_len) {
@@ -537,36 +597,13 @@ IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int
     IM_GUARD_BEGIN
     using namespace im;
     PagedAttn p;
-    IM_REQUIRE(layer >= 0, "layer %d", layer);
-    int rc = paged_view(kv, layer, &p.kv);
-    if (rc == IM_OK) rc = attn_check(kv, num_heads, max_new);
-    if (rc != IM_OK) return rc;
-    IM_REQUIRE(num_tokens >= 0 && max_len >= 0, "bad argument");
-    if (num_tokens == 0 || kv->num_seqs == 0) return paged_device(dev);
-    IM_REQUIRE(q_dev && out_dev && token_start_dev, "bad argument");
-    const int64_t row = (int64_t)num_heads * kv->head_dim, most = (int64_t)1 << 40;
-    IM_REQUIRE(q_stride >= row && out_stride >= row && q_stride <= most && out_stride <= most && q_stride % 8 == 0 && out_stride % 8 == 0 && aligned16(q_dev) && aligned16(out_dev),
-               "rows of queries and outputs have to be 16-byte aligned and apart");
-    IM_REQUIRE(!share_rows(q_dev, 2 * q_stride, out_dev, 2 * out_stride, 2 * row, num_tokens), "the outputs lie over the queries");
-    IM_REQUIRE(!mask_dev || (mask_words >= 1 && mask_words <= 1 << 20), "a mask of %d words a token", mask_words);
-    IM_REQUIRE(scale == scale && scale - scale == 0.0f, "scale is not finite");
-    rc = paged_device(dev);
-    if (rc != IM_OK) return rc;
+    bool empty;
+    const int rc = attn_args(dev, kv, layer, q_dev, q_stride, out_dev, out_stride, num_heads, token_start_dev, num_tokens, max_new, mask_dev, mask_words, scale, max_len, &p, &empty);
+    if (rc != IM_OK || empty) return rc;
     max_len = attn_length(p.kv, max_len);
     const AttnPlan plan = attn_plan(dev, p.kv.nseq, p.kv.nkv, p.kv.hd, num_heads / kv->num_kv_heads, max_new, max_len);
     IM_REQUIRE(plan.bytes == 0 || (scratch_dev && aligned16(scratch_dev) && scratch_bytes >= plan.bytes), "paged attention needs %zu bytes of 16-byte aligned scratch (got %zu)", plan.bytes,
                scratch_dev ? scratch_bytes : (size_t)0);
-    const int64_t at = layer * (int64_t)p.kv.layer_stride;
-    p.kc = static_cast<const uint16_t *>(kv->k_dev) + at;
-    p.vc = static_cast<const uint16_t *>(kv->v_dev) + at;
-    p.q = static_cast<const uint16_t *>(q_dev);
-    p.out = static_cast<uint16_t *>(out_dev);
-    p.qs = q_stride; p.os = out_stride;
-    p.start = token_start_dev;
-    p.mask = mask_dev; p.mask_words = mask_words;
-    p.group = num_heads / kv->num_kv_heads; p.tokens = num_tokens; p.max_new = max_new;
-    p.scale2 = scale * 1.4426950408889634f;
-    if (p.scale2 == 0.0f) p.scale2 = 1e-30f;  // every position alike, without 0 * inf at the hidden ones
     p.row_tiles = plan.row_tiles;
     p.ctas = plan.ctas;
     // no more CTAs than tiles

@@ -21,7 +21,15 @@ struct PagedAttn {
     float2 *part_ml;          // [ctas, 2, rows of a tile]: maximum, sum of weights
     int *spans;               // [units, KV heads, 2]: the slot of an item's first part (-1: one CTA had all of it), the CTA of its last one
     unsigned *odd;            // tcgen05: [units, KV heads, 8]: rows of an item that one CTA had whose sums are not finite (rows of parts: a NaN in part_ml)
+    // sequences in groups that share their first pages (paged_prefix.cu)
+    const int *group_start, *prefix_pages;  // [groups + 1] sequences, [groups]
+    int groups;
+    int whole_slot;           // kShared, kOwn: slots from here on are those of items that one CTA had, by item
 };
+
+// What a launch computes: attention; the part of it over the pages that a group of sequences shares, all the group's rows together; the part over the
+// rows of their own. The parts leave sums (never outputs) for another launch to join.
+enum PagedMode { kAttend, kShared, kOwn };
 
 // A unit: a tile of rows (token, query head of the KV head) of one sequence, rows token-major.
 struct PagedUnit {
@@ -29,14 +37,51 @@ struct PagedUnit {
     int tok0;                 // the sequence's first new token
     int len, fresh;           // rows before the new ones; new ones that lie in the table
     int end;                  // no row of the unit sees a position from here on
+    int from;                 // kOwn: its first position
 };
+template <int MODE>
+__device__ __forceinline__ int unit_from(const PagedUnit &u) { return MODE == kOwn ? u.from : 0; }
 
-template <int R>
-__device__ __forceinline__ PagedUnit paged_unit(const PagedAttn &p, int u) {
+// The group of a sequence, -1 where it has none: the last that starts at or before it.
+__device__ __forceinline__ int paged_group_of(const PagedAttn &p, int seq) {
+    if (p.groups == 0 || seq < __ldg(p.group_start) || seq >= __ldg(p.group_start + p.groups)) return -1;
+    int lo = 0, hi = p.groups;  // it lies in [lo, hi)
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (__ldg(p.group_start + mid) <= seq) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+// Rows that the sequences of a group share.
+__device__ __forceinline__ int prefix_rows(const PagedAttn &p, int group) { return group < 0 ? 0 : min(max(__ldg(p.prefix_pages + group), 0), p.kv.width) * p.kv.page; }
+
+template <int MODE>
+__device__ __forceinline__ PagedUnit paged_unit_of(const PagedAttn &p, int u, int R) {
     PagedUnit x;
     x.seq = u / p.row_tiles;
     x.row0 = (u - x.seq * p.row_tiles) * R;
+    if constexpr (MODE == kShared) {  // of a group: its tokens lie one after the other, its pages are the first sequence's
+        const int first = __ldg(p.group_start + x.seq), last = __ldg(p.group_start + x.seq + 1);
+        const bool good = first >= 0 && last >= first && last <= p.kv.nseq;
+        const int a = good ? __ldg(p.start + first) : 0, b = good ? __ldg(p.start + last) : 0;
+        const int n = a < 0 || b > p.tokens || b < a ? 0 : b - a;
+        x.len = prefix_rows(p, x.seq);
+        x.seq = min(max(first, 0), p.kv.nseq - 1);
+        x.tok0 = a;
+        x.fresh = 0;
+        x.rows = min(max(min(n, p.max_new) * p.group - x.row0, 0), R);
+        x.end = x.rows == 0 ? 0 : x.len;
+        if (x.end == 0) x.rows = 0;
+        x.from = 0;
+        return x;
+    }
     x.len = p.kv.length(x.seq);
+    x.from = 0;
+    if constexpr (MODE == kOwn) {
+        x.from = prefix_rows(p, paged_group_of(p, x.seq));
+        x.len = max(x.len, x.from);
+    }
     const int a = __ldg(p.start + x.seq), b = __ldg(p.start + x.seq + 1);
     x.tok0 = a;
     const int n = a < 0 || b > p.tokens || b < a ? 0 : b - a;  // (tokens that the arrays do not have)
@@ -46,6 +91,9 @@ __device__ __forceinline__ PagedUnit paged_unit(const PagedAttn &p, int u) {
     x.end = x.rows == 0 ? 0 : x.len + (p.mask ? x.fresh : min(x.fresh, last + 1));
     return x;
 }
+
+template <int R, int MODE>
+__device__ __forceinline__ PagedUnit paged_unit(const PagedAttn &p, int u) { return paged_unit_of<MODE>(p, u, R); }
 
 // Whether the t-th new token of a sequence sees position `pos`, pos < end of its unit.
 __device__ __forceinline__ bool paged_sees(const PagedAttn &p, const PagedUnit &u, int t, int pos) {
@@ -82,14 +130,23 @@ __device__ __forceinline__ long long block_scan(int v, long long *sums) {
     return total;
 }
 
-template <int TILE>
-__device__ __forceinline__ int unit_tiles(const PagedUnit &u) { return (u.end + TILE - 1) / TILE; }
+template <int TILE, int MODE>
+__device__ __forceinline__ int unit_tiles(const PagedUnit &u) { return MODE == kOwn ? (max(u.end - u.from, 0) + TILE - 1) / TILE : (u.end + TILE - 1) / TILE; }
 
 // Says where the parts of an item lie that CTA `cta` has tiles t0 .. t1 - 1 of, its `slot`-th (0, 1) part if it does not have all of them.
+template <int MODE>
 __device__ __forceinline__ void note_span(const PagedAttn &p, int unit, int head, int t0, int t1, int tiles, int cta, int slot) {
-    int *span = p.spans + 2 * ((long long)unit * p.kv.nkv + head);
-    if (t0 == 0) span[0] = t1 == tiles ? -1 : 2 * cta + slot;
+    const long long item = (long long)unit * p.kv.nkv + head;
+    int *span = p.spans + 2 * item;
+    if (t0 == 0) span[0] = t1 < tiles ? 2 * cta + slot : MODE == kAttend ? -1 : (int)(p.whole_slot + item);
     if (t1 == tiles) span[1] = cta;
+}
+
+// The slot of a CTA's part of an item, its `slot`-th if it does not have all of it.
+template <int MODE>
+__device__ __forceinline__ size_t part_slot(const PagedAttn &p, int unit, int head, int t0, int t1, int tiles, int cta, int slot) {
+    if (MODE != kAttend && t0 == 0 && t1 == tiles) return p.whole_slot + (size_t)unit * p.kv.nkv + head;
+    return (size_t)cta * 2 + slot;
 }
 
 // Where a CTA's share starts.
@@ -107,7 +164,7 @@ __device__ __forceinline__ long long share_at(long long total, int n, int c) {
     return q * c + (uint32_t)((int)(total - q * n) * c) / (uint32_t)n;
 }
 
-template <int R, int TILE, int THREADS>
+template <int R, int TILE, int THREADS, int MODE>
 __device__ __forceinline__ Share find_share(const PagedAttn &p, int units, long long *sums, PagedUnit &at) {
     int *found = reinterpret_cast<int *>(sums + THREADS + 32);  // unit, head, tile
     Share s;
@@ -123,7 +180,7 @@ __device__ __forceinline__ Share find_share(const PagedAttn &p, int units, long 
             const int u = u0 + threadIdx.x;
             long long all = total;
             if (pass == 0 || !once) {
-                n = u < units ? unit_tiles<TILE>(paged_unit<R>(p, u)) : 0;
+                n = u < units ? unit_tiles<TILE, MODE>(paged_unit<R, MODE>(p, u)) : 0;
                 all = block_scan<THREADS>(n, sums);
             }
             if (pass == 0) {
@@ -152,17 +209,17 @@ __device__ __forceinline__ Share find_share(const PagedAttn &p, int units, long 
     s.unit = found[0];
     s.head = found[1];
     s.tile = found[2];
-    at = paged_unit<R>(p, s.unit);
+    at = paged_unit<R, MODE>(p, s.unit);
     __syncthreads();  // everyone has read found[]: `sums` may lie where the caller's warps, not all at a time, write next
     return s;
 }
 
 // The same by every warp for itself, for up to 32 units: a lane per unit, no synchronisation of the block.
-template <int R, int TILE>
+template <int R, int TILE, int MODE>
 __device__ __forceinline__ Share warp_share(const PagedAttn &p, int units, PagedUnit &at) {
     const int lane = threadIdx.x & 31;
-    PagedUnit u = paged_unit<R>(p, min(lane, units - 1));
-    const int n = lane < units ? unit_tiles<TILE>(u) : 0;  // (32 sequences of 2^31 rows in tiles of 64: 2^30)
+    PagedUnit u = paged_unit<R, MODE>(p, min(lane, units - 1));
+    const int n = lane < units ? unit_tiles<TILE, MODE>(u) : 0;  // (32 sequences of 2^31 rows in tiles of 64: 2^30)
     int sum = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -191,6 +248,7 @@ __device__ __forceinline__ Share warp_share(const PagedAttn &p, int units, Paged
     at.len = __shfl_sync(0xffffffffu, u.len, s.unit);
     at.fresh = __shfl_sync(0xffffffffu, u.fresh, s.unit);
     at.end = __shfl_sync(0xffffffffu, u.end, s.unit);
+    at.from = MODE == kOwn ? __shfl_sync(0xffffffffu, u.from, s.unit) : 0;
     return s;
 }
 
@@ -260,5 +318,19 @@ __device__ __noinline__ void plain_row(const PagedAttn &p, const PagedUnit &u, i
 // kernel of paged_attn.cu is the one to use; CTAs = SMs.
 int paged_tc_rows(int hd, long long rows);
 int paged_tc_launch(const Device *dev, const PagedAttn &p, bool bf16, int rows, int units, cudaStream_t st);
+
+// Rows that no sequence passes.
+int attn_length(const PagedView &v, int max_len);
+// What calls have in common: heads and new tokens checked; all arguments checked and p filled in but for the plan (empty: there is nothing to do).
+int attn_check(const im_paged_kv *kv, int num_heads, int max_new);
+int attn_args(im_device *dev, const im_paged_kv *kv, int layer, const void *q_dev, int64_t q_stride, void *out_dev, int64_t out_stride, int num_heads,
+              const int *token_start_dev, int num_tokens, int max_new, const uint64_t *mask_dev, int mask_words, float scale, int max_len, PagedAttn *p, bool *empty);
+
+// The kernels of both files with the sums of a part as their result (paged_prefix.cu): MODE kShared or kOwn; no join.
+int paged_part_launch(const Device *dev, const PagedAttn &p, bool bf16, int mode, int units, cudaStream_t st);
+int paged_tc_part_launch(const Device *dev, const PagedAttn &p, bool bf16, int mode, int rows, int units, cudaStream_t st);
+// Sums of weighted values that a share of paged_attn_tc.cu leaves: four columns of all rows after another, since a warp that writes (and one that joins) has a row per lane.
+template <int R>
+__device__ __forceinline__ float *tc_part(float *part_o, size_t slot, int hd, int row, int col) { return part_o + (slot * (hd / 4) + col / 4) * (R * 4) + row * 4 + col % 4; }
 
 }  // namespace im

@@ -55,7 +55,7 @@ struct TcShape {
 };
 
 // The items of a CTA's share, one after the other; every warp walks them for itself.
-template <int R>
+template <int R, int MODE>
 struct Items {
     const PagedAttn &p;
     const int units;
@@ -69,7 +69,7 @@ struct Items {
             unit = s.unit;
             head = s.head - 1;
             u = first;
-            tiles = unit_tiles<kTcTile>(u);
+            tiles = unit_tiles<kTcTile, MODE>(u);
             tile = s.tile;
         }
     }
@@ -79,8 +79,8 @@ struct Items {
             head = 0;
             do {
                 if (++unit >= units) return false;
-                u = paged_unit<R>(p, unit);
-                tiles = unit_tiles<kTcTile>(u);
+                u = paged_unit<R, MODE>(p, unit);
+                tiles = unit_tiles<kTcTile, MODE>(u);
             } while (tiles == 0);
         }
         t0 = tile;
@@ -162,11 +162,8 @@ __device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b) {
 __device__ __forceinline__ void both_halves() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 // What copies of other threads have written, once their barrier says so, before the tensor cores read it.
 __device__ __forceinline__ void copies_landed() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// Sums of weighted values that a share leaves: four columns of all rows after another, since a warp that writes (and one that joins) has a row per lane.
-template <int R>
-__device__ __forceinline__ float *tc_part(float *part_o, size_t slot, int hd, int row, int col) { return part_o + (slot * (hd / 4) + col / 4) * (R * 4) + row * 4 + col % 4; }
 
-template <bool BF16, int KB, bool WIDE>
+template <bool BF16, int KB, bool WIDE, int MODE>
 __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_constant__ PagedAttn p, int units, int *err) {
     using Shape = TcShape<KB, WIDE>;
     constexpr int kTerms = WIDE ? 1 : 2;  // 16-bit terms of a weight
@@ -218,8 +215,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     pdl_trigger();  // after the allocation: a successor on this SM cannot take the columns first
     pdl_wait();
     PagedUnit at;
-    const Share share = units <= 32 ? warp_share<R, kTcTile>(p, units, at) : find_share<R, kTcTile, kTcThreads>(p, units, reinterpret_cast<long long *>(Qs), at);  // (the copies start behind its last barrier)
-    Items<R> it(p, units, share, at);
+    const Share share = units <= 32 ? warp_share<R, kTcTile, MODE>(p, units, at) : find_share<R, kTcTile, kTcThreads, MODE>(p, units, reinterpret_cast<long long *>(Qs), at);  // (the copies start behind its last barrier)
+    Items<R, MODE> it(p, units, share, at);
     bool ok = true;
     if (warp >= kTcCopy) {
         // ---- copies: this warp's 32 rows of every 128
@@ -262,7 +259,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
         };
         while (it.next()) {
             const PagedUnit &u = it.u;
-            long long o = lookup(u, it.head, it.t0 * kTcTile + w0 + lane);
+            long long o = lookup(u, it.head, unit_from<MODE>(u) + it.t0 * kTcTile + w0 + lane);
             if (it.index > 0) room(qempty, (it.index - 1) & 1);
             for (int h = 0; h < (WIDE && u.rows > 128 ? 2 : 1); h++) {
                 const int r = h * 128 + w0 + lane;
@@ -273,7 +270,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             for (int t = it.t0; t < it.t1; t++) {
                 const int ks = kc % SK, vs = vc % SV;
                 // the places of the next tile's rows are looked up while this one is requested
-                const long long next = t + 1 < it.t1 ? lookup(u, it.head, (t + 1) * kTcTile + w0 + lane) : -1;
+                const long long next = t + 1 < it.t1 ? lookup(u, it.head, unit_from<MODE>(u) + (t + 1) * kTcTile + w0 + lane) : -1;
                 if (kc >= SK) room(&kempty[ks], (kc / SK - 1) & 1);
                 const unsigned word = __ballot_sync(0xffffffffu, o >= 0);
                 if (lane == 0) {
@@ -412,7 +409,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 if (ok && !wait_for(&sfull[h], seen & 1, err)) ok = false;
                 seen++;
                 fence_after();
-                const int p0 = (it.t0 + t) * kTcTile;
+                const int p0 = unit_from<MODE>(u) + (it.t0 + t) * kTcTile;
                 const uint32_t *rows = there + ((tiles_before + t) & 7) * 4;
                 const bool part = (rows[0] & rows[1] & rows[2] & rows[3]) != 0xffffffffu || p0 + kTcTile > u.len;  // some row does not see all of the tile
                 float top = -INFINITY;
@@ -520,9 +517,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             }
             fence_after();
             const bool live = R_ < u.rows && ok;
-            const bool whole = it.t0 == 0 && it.t1 == it.tiles;
-            const size_t slot = (size_t)blockIdx.x * 2 + (it.index == 0 ? 0 : 1);
-            if (tid == 0) note_span(p, it.unit, it.head, it.t0, it.t1, it.tiles, blockIdx.x, it.index == 0 ? 0 : 1);
+            const bool whole = MODE == kAttend && it.t0 == 0 && it.t1 == it.tiles;
+            const size_t slot = part_slot<MODE>(p, it.unit, it.head, it.t0, it.t1, it.tiles, blockIdx.x, it.index == 0 ? 0 : 1);
+            if (tid == 0) note_span<MODE>(p, it.unit, it.head, it.t0, it.t1, it.tiles, blockIdx.x, it.index == 0 ? 0 : 1);
             const float inv = whole ? (l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l) : 1.0f;
             uint16_t *out = p.out + (u.tok0 + token) * p.os + (long long)(it.head * p.group + (u.row0 + min(R_, u.rows - 1)) % p.group) * HD;
             float worst = 0.0f;
@@ -589,7 +586,7 @@ constexpr int kTcJoinThreads = 128, kTcJoinWarps = kTcJoinThreads / 32;
 template <bool BF16, int R, int HD>
 __device__ __noinline__ void odd_rows_again(const PagedAttn &p, int unit, int head, int rows, unsigned bad, int warp, int warps) {
     const int lane = threadIdx.x & 31;
-    const PagedUnit u = paged_unit<R>(p, unit);
+    const PagedUnit u = paged_unit<R, kAttend>(p, unit);
 #pragma unroll 1
     for (int n = 0; bad; n++, bad &= bad - 1) {
         if (n % warps != warp) continue;
@@ -659,7 +656,7 @@ __global__ void __launch_bounds__(kTcJoinThreads, WIDE ? 9 : 12) paged_tc_join_k
     const int item = blockIdx.x, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, lane = threadIdx.x & 31;
     const int w = blockIdx.y * kTcJoinWarps + (threadIdx.x >> 5), rows = w / (HD / 4), r = rows * 32 + lane, c = w % (HD / 4) * 4;
     const int2 span = *reinterpret_cast<const int2 *>(p.spans + 2 * (long long)item);
-    const PagedUnit u = paged_unit<R>(p, unit);
+    const PagedUnit u = paged_unit<R, kAttend>(p, unit);
     if (rows * 32 >= u.rows) return;  // (a unit without tiles has no rows)
     const unsigned bad = span.x < 0 ? p.odd[(long long)item * 8 + rows] : join_parts<BF16, HD, R, N>(p, u, span, head, r, c);
     if (bad) odd_rows_again<BF16, R, HD>(p, unit, head, rows, bad, w % (HD / 4), HD / 4);
@@ -669,15 +666,33 @@ template <bool BF16, int KB, bool WIDE>
 int tc_launch(const Device *dev, const PagedAttn &p, int units, cudaStream_t st) {
     using S = TcShape<KB, WIDE>;
     static DeviceOnce once;
-    if (once.first(dev->ordinal)) IM_CUDA_CHECK(cudaFuncSetAttribute((paged_tc_kernel<BF16, KB, WIDE>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
-    IM_CUDA_CHECK(launch_k(paged_tc_kernel<BF16, KB, WIDE>, dim3(p.ctas), dim3(kTcThreads), (size_t)S::kSmem, st, p, units, dev->err_flag));
+    if (once.first(dev->ordinal)) IM_CUDA_CHECK(cudaFuncSetAttribute((paged_tc_kernel<BF16, KB, WIDE, kAttend>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+    IM_CUDA_CHECK(launch_k(paged_tc_kernel<BF16, KB, WIDE, kAttend>, dim3(p.ctas), dim3(kTcThreads), (size_t)S::kSmem, st, p, units, dev->err_flag));
     const long long rows = std::min<long long>(S::kRows, (long long)p.max_new * p.group);
     IM_CUDA_CHECK(launch_k(paged_tc_join_kernel<BF16, KB, WIDE>, dim3((unsigned)(units * p.kv.nkv), (unsigned)((rows + 31) / 32 * (16 * KB) / (kTcJoinThreads / 32))),
                            dim3(kTcJoinThreads), 0, st, p));
     return IM_OK;
 }
 
+template <bool BF16, int KB, bool WIDE, int MODE>
+int tc_part_launch(const Device *dev, const PagedAttn &p, int units, cudaStream_t st) {
+    using S = TcShape<KB, WIDE>;
+    static DeviceOnce once;
+    if (once.first(dev->ordinal)) IM_CUDA_CHECK(cudaFuncSetAttribute((paged_tc_kernel<BF16, KB, WIDE, MODE>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+    IM_CUDA_CHECK(launch_k(paged_tc_kernel<BF16, KB, WIDE, MODE>, dim3(p.ctas), dim3(kTcThreads), (size_t)S::kSmem, st, p, units, dev->err_flag));
+    return IM_OK;
+}
+
 }  // namespace
+
+int paged_tc_part_launch(const Device *dev, const PagedAttn &p, bool bf16, int mode, int rows, int units, cudaStream_t st) {
+#define IM_MODE(B, KB, W) (mode == kShared ? tc_part_launch<B, KB, W, kShared>(dev, p, units, st) : tc_part_launch<B, KB, W, kOwn>(dev, p, units, st))
+#define IM_RUN(B, KB) (rows == 256 ? IM_MODE(B, KB, true) : IM_MODE(B, KB, false))
+    if (p.kv.hd == 64) return bf16 ? IM_RUN(true, 1) : IM_RUN(false, 1);
+    return bf16 ? IM_RUN(true, 2) : IM_RUN(false, 2);
+#undef IM_RUN
+#undef IM_MODE
+}
 
 int paged_tc_rows(int hd, long long rows) {
     if (hd != 64 && hd != 128) return 0;

@@ -574,6 +574,60 @@ def paged_attention(kv: PagedKV, layer: int, q, token_start, max_new: int, scale
     return out
 
 
+def _outputs_for(q, out, kv: PagedKV):
+    """(tensor, stride) of outputs like q's tokens."""
+    n, heads, dim = q.shape
+    if out is None:
+        return torch.empty_like(q, memory_format=torch.contiguous_format), heads * dim
+    return out, _rows_of(out, n, heads, dim, kv.dtype, kv.ordinal)
+
+
+def _mask_of(mask, n: int, ordinal: int):
+    """(address, words) of a mask int64 [tokens, words] or None."""
+    if mask is None:
+        return None, 0
+    assert mask.dim() == 2 and mask.dtype is torch.int64 and mask.shape[0] == n and mask.is_contiguous() and mask.get_device() == ordinal, (mask.shape, mask.dtype)
+    return mask.data_ptr(), mask.shape[1]
+
+
+def _scratch_of(scratch, nbytes: int, kv: PagedKV):
+    """(tensor that has to live until the launch, address, bytes) of scratch given or made."""
+    if scratch is None:
+        if not nbytes:
+            return None, None, 0
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=kv.device)
+    else:
+        assert scratch.dtype is torch.uint8 and scratch.get_device() == kv.ordinal and scratch.is_contiguous()
+    return scratch, scratch.data_ptr(), scratch.numel()
+
+
+def _prefix_bytes(kv: PagedKV, *key) -> int:
+    nbytes = kv.scratch_bytes.get(key)
+    if nbytes is None:
+        nbytes = kv.scratch_bytes[key] = int(lib().im_cuda_paged_prefix_attention_scratch_bytes(kv.dev.handle, kv.ref, *key))
+    return nbytes
+
+
+def paged_prefix_attention_scratch(kv: PagedKV, heads: int, max_new: int, groups: int, max_group_new: int) -> torch.Tensor:
+    """Scratch for paged_prefix_attention calls of this cache with so many heads, new tokens and groups; calls that may overlap need one each."""
+    return torch.empty(max(_prefix_bytes(kv, heads, max_new, groups, max_group_new), 16), dtype=torch.uint8, device=kv.device)
+
+
+def paged_prefix_attention(kv: PagedKV, layer: int, q, token_start, max_new: int, scale: float, group_start, max_group_new: int, prefix_pages, max_prefix=0, mask=None, max_len=0,
+                           out=None, scratch=None):
+    """paged_attention where the sequences group_start[g] .. group_start[g + 1] - 1 (int32 [groups + 1]) have the first prefix_pages[g] (int32 [groups]) pages of
+    their table rows in common: those are read once for a group. max_group_new, max_prefix: the most new tokens of a group, the most rows that one shares."""
+    n, heads, dim = q.shape
+    on, groups = kv.ordinal, prefix_pages.shape[0]
+    qs = _rows_of(q, n, heads, kv.head_dim, kv.dtype, on)
+    out, os_ = _outputs_for(q, out, kv)
+    mp, words = _mask_of(mask, n, on)
+    scratch, at, nbytes = _scratch_of(scratch, _prefix_bytes(kv, heads, max_new, groups, max_group_new) if scratch is None else 0, kv)
+    _launch(on, lib().im_cuda_paged_prefix_attention, kv.dev.handle, kv.ref, layer, q.data_ptr(), qs, out.data_ptr(), os_, heads, _ints(token_start, on, kv.num_seqs + 1), n, max_new,
+            _ints(group_start, on, groups + 1), groups, max_group_new, _ints(prefix_pages, on, groups), max_prefix, mp, words, scale, max_len, at, nbytes)
+    return out
+
+
 def paged_keep(kv: PagedKV, accepted, counts, lengths_out=None):
     """The accepted path of every drafted tree, accepted int32 [sequences, most] (places among the new rows, from the root on), counts int32
     [sequences], moves up behind the rows before it, in every layer. Returns the new lengths (kv.point_at)."""
