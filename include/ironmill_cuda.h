@@ -370,6 +370,30 @@ int im_cuda_paged_prefix_attention(im_device *dev, const im_paged_kv *kv, int la
                                    int max_group_new, const int *prefix_pages_dev, int max_prefix, const uint64_t *mask_dev, int mask_words, float scale,
                                    int max_len, void *scratch_dev, size_t scratch_bytes, void *stream);
 
+/* paged_attention that also adds up what the rows of the cache are worth: weights[s, g, r] += sum of the softmax weights of row r over the call's new tokens of
+ * sequence s and the query heads of KV head g; a new token's own row starts with this call's sum, whatever was there.  f32, in the same order on every run: a repeated call on
+ * the same sums gives the same bits.  weights_dev f32 [num_seqs, num_kv_heads, rows], sequences and heads seq_stride and head_stride elements apart; rows from `rows` on
+ * are not counted, and neither sums of sequences without new tokens nor those behind a sequence's last row are touched.  weights_dev lies over
+ * nothing that is read.  Up to 16 rows (max_new * num_heads / num_kv_heads) the scratch grows with max_len (4 bytes a row and position, up to 256 MB): say what it is.  Scratch of a
+ * larger max_len is enough for a smaller one. */
+size_t im_cuda_paged_attention_weights_scratch_bytes(const im_device *dev, const im_paged_kv *kv, int num_heads, int max_new, int max_len);
+int im_cuda_paged_attention_weights(im_device *dev, const im_paged_kv *kv, int layer, const void *q_dev, int64_t q_stride, void *out_dev, int64_t out_stride,
+                                    int num_heads, const int *token_start_dev, int num_tokens, int max_new, const uint64_t *mask_dev, int mask_words,
+                                    float scale, int max_len, float *weights_dev, int64_t seq_stride, int64_t head_stride, int rows, void *scratch_dev,
+                                    size_t scratch_bytes, void *stream);
+
+/* Eviction by such sums, in every layer.  A sequence of more than `budget` rows keeps the last `recent` of them and, for every layer and KV head on its own, the budget - recent
+ * rows before those with the largest weights (ties: the lowest row; NaN counts as -inf).  With H = budget - recent: a kept row below H stays where
+ * it is, the kept ones behind come, in order, to the places of rows below H that leave, and the recent rows follow in order from H on.  The rows' order is another
+ * afterwards: give the next tokens their positions (position_dev of paged_append).  weights, weights_out f32 [num_layers, num_seqs, num_kv_heads, table_width * page_size],
+ * layers, sequences and heads apart by their strides; weights_out gets the sums of the rows where they lie now (and of sequences that fit, as they are), entries from the new
+ * length on are left as they are.  seq_len_out_dev [num_seqs]: min(seq_len, budget).  A sequence's pages up to its length are its own (not shared with another).  A row that is
+ * not there is not moved, nor is one moved to a place that is not there.  weights_out and seq_len_out lie over nothing that is read, nor over each other. */
+size_t im_cuda_paged_evict_scratch_bytes(const im_device *dev, const im_paged_kv *kv, int budget, int recent);
+int im_cuda_paged_evict(im_device *dev, const im_paged_kv *kv, const float *weights_dev, int64_t layer_stride, int64_t seq_stride, int64_t head_stride, int budget,
+                        int recent, float *weights_out_dev, int64_t out_layer_stride, int64_t out_seq_stride, int64_t out_head_stride, int *seq_len_out_dev,
+                        void *scratch_dev, size_t scratch_bytes, void *stream);
+
 /* The accepted path of a tree: in every layer row seq_len + accepted_dev[s, j] becomes row seq_len + j, j = 0 .. count_dev[s] - 1
  * (accepted [num_seqs, max_accept], each path in order from the root: accepted[s, j] >= j; an entry below j is not moved).
  * seq_len_out_dev [num_seqs], not over what is read: seq_len + count.  At most 65535 sequences (paged_reorder too). */

@@ -33,24 +33,6 @@ struct PaShape {
     static constexpr int kSmem = kRing + kMerge + kPaWarps * kRows * 8;
 };
 
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
-}
-__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t at) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
-}
-template <bool BF16>
-__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    if (BF16)
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
 // CL: instead of shares of the list of all tiles, a cluster of CTAs per item, each with an equal run of its tiles; they join what they have
 // through each other's shared memory, in the same launch and without scratch.
 template <bool BF16, int HD, bool CL, int MODE>
@@ -225,6 +207,16 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
                         if (!(there >> at & 1) || !paged_sees(p, u, tok[j >> 1], pos0 + at)) s[n][j] = -INFINITY;
                     }
             }
+            if (MODE == kWeigh && p.scores && pos0 < p.score_cap) {  // (a multiple of a tile)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int r = (lane >> 2) + 8 * i;
+                    float *to = p.scores + (((long long)unit * p.kv.nkv + head) * p.score_rows + r) * p.score_cap + pos0 + (lane & 3) * 2;
+                    if (r < u.rows)
+#pragma unroll
+                        for (int n = 0; n < 2; n++) *reinterpret_cast<float2 *>(to + n * 8) = make_float2(s[n][2 * i], s[n][2 * i + 1]);
+                }
+            }
             uint32_t w[4], w2[4];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -274,7 +266,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
         }
         __syncthreads();
         if (tid == 0) bad_rows[!odd_item] = 0;  // every thread has looked at the last item's
-        const bool whole = MODE == kAttend && !CL && t0 == 0 && t1 == tiles;
+        const bool whole = whole_items<MODE>() && !CL && t0 == 0 && t1 == tiles;
         const size_t part = part_slot<MODE>(p, unit, head, t0, t1, tiles, blockIdx.x, first_item ? 0 : 1) * R;
         if (!CL && tid == 0) note_span<MODE>(p, unit, head, t0, t1, tiles, blockIdx.x, first_item ? 0 : 1);
         float f[2];
@@ -344,6 +336,8 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
                 if (CL) joint[r] = row_ml(r);
                 else p.part_ml[part + r] = row_ml(r);
             }
+        if (MODE == kWeigh && whole)
+            for (int r = tid; r < u.rows; r += kPaThreads) p.stat[((long long)unit * p.kv.nkv + head) * R + r] = row_ml(r);
         __syncthreads();
         if (const unsigned bad = bad_rows[odd_item]) {
             for (int r = warp; r < u.rows; r += kPaWarps) {
@@ -399,6 +393,28 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
             *reinterpret_cast<uint4 *>(p.out + (u.tok0 + t) * p.os + (long long)(share.head * p.group + g) * HD + c) =
                 make_uint4(pack16<BF16>(o[0] * inv, o[1] * inv), pack16<BF16>(o[2] * inv, o[3] * inv), pack16<BF16>(o[4] * inv, o[5] * inv), pack16<BF16>(o[6] * inv, o[7] * inv));
         }
+        if constexpr (MODE == kWeigh) {  // the sums of this CTA's positions
+            __shared__ RowNorm norms[R];
+            if (tid < u.rows) {
+                float M = -INFINITY, L = 0.0f;
+                for (int k = 0; k < C; k++) M = fmaxf(M, remote2(of_rank(joint + tid, k)).x);
+                for (int k = 0; k < C; k++) {
+                    const float2 x = remote2(of_rank(joint + tid, k));
+                    if (!(x.x == -INFINITY && x.y == 0.0f)) L += x.y * ex2(x.x - M);
+                }
+                norms[tid] = RowNorm(make_float2(M, L));
+                if (!p.scores && rank == 0) p.stat[(long long)(blockIdx.x / C) * R + tid] = make_float2(M, L);
+            }
+            __syncthreads();
+            const float *scores = p.scores + (long long)(blockIdx.x / C) * p.score_rows * p.score_cap;
+            for (int pos = (int)share.from * kPaTile + tid; p.scores && pos < min((int)share.to * kPaTile, u.end); pos += kPaThreads) {
+                float v = 0.0f;
+                if (pos >= p.score_cap) v = plain_sum<BF16, HD>(p, u, share.head, pos, norms);
+                else
+                    for (int r = 0; r < u.rows; r++) v += norms[r].weight(scores[(long long)r * p.score_cap + pos]);
+                add_sum(p, u, share.head, pos, v);
+            }
+        }
         cluster_sync();  // nobody leaves while another reads what it has
     }
 }
@@ -406,14 +422,14 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
 // Items that a cut divides: a warp per row, HD / 32 columns a lane. The parts of an item lie with the CTAs that its tiles fall to; a lane per part
 // brings maxima and sums. (A block per row with the shares' divisions in loops took 25 us for 64 items of 104 rows.)
 constexpr int kJoinWarps = 8;
-template <bool BF16, int R, int HD>
+template <bool BF16, int R, int HD, int MODE>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __grid_constant__ PagedAttn p) {
     constexpr int V = HD / 32;
     pdl_trigger();
     pdl_wait();
     const int item = blockIdx.x, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, lane = threadIdx.x & 31, r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5);
     const int2 span = *reinterpret_cast<const int2 *>(p.spans + 2 * (long long)item);
-    const PagedUnit u = paged_unit<R, kAttend>(p, unit);
+    const PagedUnit u = paged_unit<R, MODE>(p, unit);
     if (r >= u.rows || span.x < 0) return;  // (a unit without tiles has no rows)
     const size_t slot0 = span.x;
     const int c = span.x >> 1, parts = span.y - c + 1;
@@ -443,6 +459,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __gri
             for (int j = 0; j < V; j++) o[j] += g == 0.0f ? 0.0f : v[j] * g;
         }
     }
+    if (MODE == kWeigh && lane == 0) p.stat[(long long)item * R + r] = make_float2(M, L);
     const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
     const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
     uint32_t *dst = reinterpret_cast<uint32_t *>(p.out + (u.tok0 + t) * p.os + (long long)(head * p.group + g) * HD + lane * V);
@@ -450,12 +467,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __gri
     for (int j = 0; j < V; j += 2) dst[j / 2] = pack16<BF16>(o[j] * inv, o[j + 1] * inv);
 }
 
-struct AttnPlan {
-    int rows, tile, row_tiles, units, ctas;
-    int cluster;  // CTAs per item that join in the launch; 0: shares
-    size_t bytes;
-};
 constexpr int kClusterMost = 8;
+
+}  // namespace
+
 AttnPlan attn_plan(const Device *dev, int nseq, int nkv, int hd, int group, int max_new, int max_len) {
     AttnPlan a;
     // Up to 16 rows of a KV head (and heads of 256, whose scores and outputs tensor memory does not hold twice) on mma.sync, more on tcgen05. Eight sequences of
@@ -482,27 +497,41 @@ AttnPlan attn_plan(const Device *dev, int nseq, int nkv, int hd, int group, int 
     return a;
 }
 
-template <bool BF16, int R, int HD>
+void attn_lay_out(PagedAttn *p, const AttnPlan &plan, int max_len, void *at) {
+    p->row_tiles = plan.row_tiles;
+    // no more CTAs than tiles
+    const long long tiles = (long long)plan.units * p->kv.nkv * ((max_len + (long long)plan.tile - 1) / plan.tile);
+    p->ctas = (int)std::max(1ll, std::min<long long>(plan.ctas, tiles));
+    const size_t slots = (size_t)plan.ctas * 2 * plan.rows;
+    p->part_o = static_cast<float *>(at);
+    p->part_ml = reinterpret_cast<float2 *>(p->part_o + slots * p->kv.hd);
+    p->spans = reinterpret_cast<int *>(p->part_ml + slots);
+    p->odd = reinterpret_cast<unsigned *>(p->spans + 2ll * plan.units * p->kv.nkv);
+}
+
+namespace {
+
+template <bool BF16, int R, int HD, int MODE>
 int join_launch(const PagedAttn &p, int units, cudaStream_t st) {
     const long long rows = std::min<long long>(R, (long long)p.max_new * p.group);
-    IM_CUDA_CHECK(launch_k(paged_join_kernel<BF16, R, HD>, dim3((unsigned)(units * p.kv.nkv), (unsigned)((rows + kJoinWarps - 1) / kJoinWarps)), dim3(kJoinWarps * 32), 0, st, p));
+    IM_CUDA_CHECK(launch_k(paged_join_kernel<BF16, R, HD, MODE>, dim3((unsigned)(units * p.kv.nkv), (unsigned)((rows + kJoinWarps - 1) / kJoinWarps)), dim3(kJoinWarps * 32), 0, st, p));
     return IM_OK;
 }
 
-template <bool BF16, int HD>
+template <bool BF16, int HD, int MODE>
 int attn_launch(const Device *dev, const PagedAttn &p, int units, int cluster, cudaStream_t st) {
     using S = PaShape<HD>;
     static DeviceOnce once;
     if (once.first(dev->ordinal)) {
-        IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, false, kAttend>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
-        IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, true, kAttend>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+        IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, false, MODE>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+        IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, true, MODE>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     }
     if (cluster) {
-        IM_CUDA_CHECK(launch_cluster(paged_attn_kernel<BF16, HD, true, kAttend>, dim3((unsigned)(units * p.kv.nkv * cluster)), dim3(kPaThreads), cluster, (size_t)S::kSmem, st, p, units));
+        IM_CUDA_CHECK(launch_cluster(paged_attn_kernel<BF16, HD, true, MODE>, dim3((unsigned)(units * p.kv.nkv * cluster)), dim3(kPaThreads), cluster, (size_t)S::kSmem, st, p, units));
         return IM_OK;
     }
-    IM_CUDA_CHECK(launch_k(paged_attn_kernel<BF16, HD, false, kAttend>, dim3(p.ctas), dim3(kPaThreads), (size_t)S::kSmem, st, p, units));
-    return join_launch<BF16, S::kRows, HD>(p, units, st);
+    IM_CUDA_CHECK(launch_k(paged_attn_kernel<BF16, HD, false, MODE>, dim3(p.ctas), dim3(kPaThreads), (size_t)S::kSmem, st, p, units));
+    return join_launch<BF16, S::kRows, HD, MODE>(p, units, st);
 }
 
 template <bool BF16, int HD, int MODE>
@@ -526,6 +555,16 @@ int paged_part_launch(const Device *dev, const PagedAttn &p, bool bf16, int mode
     }
 #undef IM_RUN
 #undef IM_MODE
+}
+
+int paged_weigh_launch(const Device *dev, const PagedAttn &p, bool bf16, int units, int cluster, cudaStream_t st) {
+#define IM_RUN(HD) (bf16 ? attn_launch<true, HD, kWeigh>(dev, p, units, cluster, st) : attn_launch<false, HD, kWeigh>(dev, p, units, cluster, st))
+    switch (p.kv.hd) {
+    case 64: return IM_RUN(64);
+    case 128: return IM_RUN(128);
+    default: return IM_RUN(256);
+    }
+#undef IM_RUN
 }
 
 // Rows that no sequence passes.
@@ -575,6 +614,8 @@ int attn_args(im_device *dev, const im_paged_kv *kv, int layer, const void *q_de
     if (p->scale2 == 0.0f) p->scale2 = 1e-30f;  // every position alike, without 0 * inf at the hidden ones
     p->group_start = p->prefix_pages = nullptr;
     p->groups = p->whole_slot = 0;
+    p->stat = nullptr;
+    p->scores = p->sums = nullptr;
     return IM_OK;
 }
 
@@ -604,20 +645,11 @@ IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int
     const AttnPlan plan = attn_plan(dev, p.kv.nseq, p.kv.nkv, p.kv.hd, num_heads / kv->num_kv_heads, max_new, max_len);
     IM_REQUIRE(plan.bytes == 0 || (scratch_dev && aligned16(scratch_dev) && scratch_bytes >= plan.bytes), "paged attention needs %zu bytes of 16-byte aligned scratch (got %zu)", plan.bytes,
                scratch_dev ? scratch_bytes : (size_t)0);
-    p.row_tiles = plan.row_tiles;
-    p.ctas = plan.ctas;
-    // no more CTAs than tiles
-    const long long tiles = (long long)plan.units * p.kv.nkv * ((max_len + (long long)plan.tile - 1) / plan.tile);
-    p.ctas = (int)std::max(1ll, std::min<long long>(p.ctas, tiles));
-    const size_t slots = (size_t)plan.ctas * 2 * plan.rows;
-    p.part_o = static_cast<float *>(scratch_dev);
-    p.part_ml = reinterpret_cast<float2 *>(p.part_o + slots * p.kv.hd);
-    p.spans = reinterpret_cast<int *>(p.part_ml + slots);
-    p.odd = reinterpret_cast<unsigned *>(p.spans + 2ll * plan.units * p.kv.nkv);
+    attn_lay_out(&p, plan, max_len, scratch_dev);
     const cudaStream_t st = as_stream(stream);
     const bool bf16 = kv->dtype == IM_DTYPE_BF16;
     if (plan.rows >= 128) return paged_tc_launch(dev, p, bf16, plan.rows, plan.units, st);
-#define IM_RUN(HD) (bf16 ? attn_launch<true, HD>(dev, p, plan.units, plan.cluster, st) : attn_launch<false, HD>(dev, p, plan.units, plan.cluster, st))
+#define IM_RUN(HD) (bf16 ? attn_launch<true, HD, kAttend>(dev, p, plan.units, plan.cluster, st) : attn_launch<false, HD, kAttend>(dev, p, plan.units, plan.cluster, st))
     switch (kv->head_dim) {
     case 64: return IM_RUN(64);
     case 128: return IM_RUN(128);

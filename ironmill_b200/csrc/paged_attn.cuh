@@ -25,11 +25,21 @@ struct PagedAttn {
     const int *group_start, *prefix_pages;  // [groups + 1] sequences, [groups]
     int groups;
     int whole_slot;           // kShared, kOwn: slots from here on are those of items that one CTA had, by item
+    // sums of softmax weights (paged_weights.cu)
+    float2 *stat;             // [units, KV heads, rows of a tile]: maximum and sum of weights of every row
+    float *scores;            // or NULL: [units, KV heads, score_rows, score_cap]: scores of the positions before score_cap, in powers of two
+    int score_cap, score_rows;
+    float *sums;              // [sequences, KV heads, sum_cols]
+    long long sum_seq, sum_head;
+    int sum_cols;
 };
 
 // What a launch computes: attention; the part of it over the pages that a group of sequences shares, all the group's rows together; the part over the
-// rows of their own. The parts leave sums (never outputs) for another launch to join.
-enum PagedMode { kAttend, kShared, kOwn };
+// rows of their own. The parts leave sums (never outputs) for another launch to join. kWeigh: attention that says what each row's weights were normed by, and
+// where there is room for them the scores.
+enum PagedMode { kAttend, kShared, kOwn, kWeigh };
+template <int MODE>
+constexpr bool whole_items() { return MODE == kAttend || MODE == kWeigh; }  // an item that one CTA had is done
 
 // A unit: a tile of rows (token, query head of the KV head) of one sequence, rows token-major.
 struct PagedUnit {
@@ -138,15 +148,29 @@ template <int MODE>
 __device__ __forceinline__ void note_span(const PagedAttn &p, int unit, int head, int t0, int t1, int tiles, int cta, int slot) {
     const long long item = (long long)unit * p.kv.nkv + head;
     int *span = p.spans + 2 * item;
-    if (t0 == 0) span[0] = t1 < tiles ? 2 * cta + slot : MODE == kAttend ? -1 : (int)(p.whole_slot + item);
+    if (t0 == 0) span[0] = t1 < tiles ? 2 * cta + slot : whole_items<MODE>() ? -1 : (int)(p.whole_slot + item);
     if (t1 == tiles) span[1] = cta;
 }
 
 // The slot of a CTA's part of an item, its `slot`-th if it does not have all of it.
 template <int MODE>
 __device__ __forceinline__ size_t part_slot(const PagedAttn &p, int unit, int head, int t0, int t1, int tiles, int cta, int slot) {
-    if (MODE != kAttend && t0 == 0 && t1 == tiles) return p.whole_slot + (size_t)unit * p.kv.nkv + head;
+    if (!whole_items<MODE>() && t0 == 0 && t1 == tiles) return p.whole_slot + (size_t)unit * p.kv.nkv + head;
     return (size_t)cta * 2 + slot;
+}
+
+// A row's weight of a position, 2^(score - maximum) / sum, as an exponent and a factor: zero where the row sees nothing.
+struct RowNorm {
+    float base, inv;
+    __device__ __forceinline__ RowNorm() {}
+    __device__ __forceinline__ RowNorm(float2 ml) : base(ml.x == -INFINITY ? 0.0f : ml.x), inv(ml.y > 0.0f ? 1.0f / ml.y : ml.y == 0.0f ? 0.0f : ml.y) {}
+    __device__ __forceinline__ float weight(float score) const { return ex2(score - base) * inv; }
+};
+// Adds to the sum of a position of a unit's sequence; a new row's sum starts with this call.
+__device__ __forceinline__ void add_sum(const PagedAttn &p, const PagedUnit &u, int head, int pos, float v) {
+    if (pos >= p.sum_cols) return;
+    float *at = p.sums + u.seq * p.sum_seq + head * p.sum_head + pos;
+    *at = pos >= u.len ? v : *at + v;
 }
 
 // Where a CTA's share starts.
@@ -256,6 +280,24 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool there) 
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+template <bool BF16>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (BF16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
 // A row whose sums are not finite, from the positions it sees alone: on the tensor cores a weight of zero times an infinite or missing value of a
 // position that the row does not see is a NaN. A warp, 32 positions at a time, one a lane for the scores; o: this lane's columns (lane, lane + 32, ...).
 template <bool BF16, int HD>
@@ -314,6 +356,35 @@ __device__ __noinline__ void plain_row(const PagedAttn &p, const PagedUnit &u, i
     }
 }
 
+// The sum of a position's weights over the rows of a unit, from queries and keys: a position a lane (-1: none), rows' norms in `norms`. For positions that a
+// call has no room for the scores of.
+template <bool BF16, int HD>
+__device__ __noinline__ float plain_sum(const PagedAttn &p, const PagedUnit &u, int head, int pos, const RowNorm *norms) {
+    const long long at = pos >= 0 && pos < u.end ? p.kv.row_of(u.seq, pos) : -1;
+    const uint16_t *kc = p.kc + (long long)head * p.kv.page * HD + (at < 0 ? 0 : at);
+    float v = 0.0f;
+#pragma unroll 1
+    for (int r = 0; r < u.rows; r++) {
+        const int t = (u.row0 + r) / p.group, h = head * p.group + (u.row0 + r) % p.group;
+        if (at < 0 || !paged_sees(p, u, t, pos)) continue;
+        const uint16_t *q = p.q + (u.tok0 + t) * p.qs + (long long)h * HD;
+        float d = 0.0f;
+#pragma unroll 4
+        for (int c = 0; c < HD; c += 8) {
+            const uint4 a = *reinterpret_cast<const uint4 *>(q + c), b = *reinterpret_cast<const uint4 *>(kc + c);
+            const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float2 f = unpack16<BF16>(x[j]), g = unpack16<BF16>(y[j]);
+                d = fmaf(f.x, g.x, d);
+                d = fmaf(f.y, g.y, d);
+            }
+        }
+        v += norms[r].weight(d * p.scale2);
+    }
+    return v;
+}
+
 // Many rows of a KV head on the tcgen05 tensor cores (paged_attn_tc.cu): rows of a tile for so many rows of a sequence, 0 where the
 // kernel of paged_attn.cu is the one to use; CTAs = SMs.
 int paged_tc_rows(int hd, long long rows);
@@ -329,6 +400,17 @@ int attn_args(im_device *dev, const im_paged_kv *kv, int layer, const void *q_de
 // The kernels of both files with the sums of a part as their result (paged_prefix.cu): MODE kShared or kOwn; no join.
 int paged_part_launch(const Device *dev, const PagedAttn &p, bool bf16, int mode, int units, cudaStream_t st);
 int paged_tc_part_launch(const Device *dev, const PagedAttn &p, bool bf16, int mode, int rows, int units, cudaStream_t st);
+// Attention and the norms of every row's weights (paged_weights.cu): where `cluster` is not zero, the sums too. With joins.
+int paged_weigh_launch(const Device *dev, const PagedAttn &p, bool bf16, int units, int cluster, cudaStream_t st);
+int paged_tc_weigh_launch(const Device *dev, const PagedAttn &p, bool bf16, int rows, int units, cudaStream_t st);
+struct AttnPlan {
+    int rows, tile, row_tiles, units, ctas;
+    int cluster;  // CTAs per item that join in the launch; 0: shares
+    size_t bytes;
+};
+AttnPlan attn_plan(const Device *dev, int nseq, int nkv, int hd, int group, int max_new, int max_len);
+// A plan in the arguments of a launch, its scratch from `at` on.
+void attn_lay_out(PagedAttn *p, const AttnPlan &plan, int max_len, void *at);
 // Sums of weighted values that a share of paged_attn_tc.cu leaves: four columns of all rows after another, since a warp that writes (and one that joins) has a row per lane.
 template <int R>
 __device__ __forceinline__ float *tc_part(float *part_o, size_t slot, int hd, int row, int col) { return part_o + (slot * (hd / 4) + col / 4) * (R * 4) + row * 4 + col % 4; }

@@ -628,6 +628,75 @@ def paged_prefix_attention(kv: PagedKV, layer: int, q, token_start, max_new: int
     return out
 
 
+def _weights_bytes(kv: PagedKV, heads: int, max_new: int, max_len: int) -> int:
+    key = ("weights", heads, max_new, max_len.bit_length())  # what is enough for the next power of two
+    nbytes = kv.scratch_bytes.get(key)
+    if nbytes is None:
+        most = min(1 << max_len.bit_length(), 2 ** 31 - 1) if max_len else 0
+        nbytes = kv.scratch_bytes[key] = int(lib().im_cuda_paged_attention_weights_scratch_bytes(kv.dev.handle, kv.ref, heads, max_new, most))
+    return nbytes
+
+
+def paged_attention_weights_scratch(kv: PagedKV, heads: int, max_new: int, max_len: int = 0) -> torch.Tensor:
+    """Scratch for paged_attention_weights calls of this cache with so many heads, new tokens and rows (or fewer rows); calls that may overlap need one each."""
+    return torch.empty(max(_weights_bytes(kv, heads, max_new, max_len), 16), dtype=torch.uint8, device=kv.device)
+
+
+def paged_attention_weights(kv: PagedKV, layer: int, q, token_start, max_new: int, scale: float, weights, mask=None, max_len=0, out=None, scratch=None):
+    """paged_attention, and weights f32 [sequences, kv_heads, rows] get the softmax weights of every row added, over the call's new tokens and the query
+    heads of a KV head; the new tokens' own rows start with this call's. Say max_len: the scratch grows with it."""
+    n, heads, dim = q.shape
+    on = kv.ordinal
+    qs = _rows_of(q, n, heads, kv.head_dim, kv.dtype, on)
+    out, os_ = _outputs_for(q, out, kv)
+    mp, words = _mask_of(mask, n, on)
+    assert weights.dim() == 3 and weights.shape[:2] == (kv.num_seqs, kv.kv_heads) and weights.dtype is torch.float32 and weights.get_device() == on, (weights.shape, weights.dtype)
+    rows, (ss, sh, sr) = weights.shape[2], weights.stride()
+    assert sr == 1 or rows == 1, weights.stride()
+    scratch, at, nbytes = _scratch_of(scratch, _weights_bytes(kv, heads, max_new, max_len) if scratch is None else 0, kv)
+    _launch(on, lib().im_cuda_paged_attention_weights, kv.dev.handle, kv.ref, layer, q.data_ptr(), qs, out.data_ptr(), os_, heads, _ints(token_start, on, kv.num_seqs + 1), n, max_new,
+            mp, words, scale, max_len, weights.data_ptr(), ss, sh if kv.kv_heads > 1 else rows, rows, at, nbytes)
+    return out
+
+
+def _evict_bytes(kv: PagedKV, budget: int, recent: int) -> int:
+    key = ("evict", budget, recent)
+    nbytes = kv.scratch_bytes.get(key)
+    if nbytes is None:
+        nbytes = kv.scratch_bytes[key] = int(lib().im_cuda_paged_evict_scratch_bytes(kv.dev.handle, kv.ref, budget, recent))
+    return nbytes
+
+
+def paged_evict_scratch(kv: PagedKV, budget: int, recent: int) -> torch.Tensor:
+    """Scratch for paged_evict calls of this cache; calls that may overlap need one each."""
+    return torch.empty(max(_evict_bytes(kv, budget, recent), 16), dtype=torch.uint8, device=kv.device)
+
+
+def _sums_of(x, kv: PagedKV):
+    """Strides of sums f32 [layers, sequences, kv_heads, rows of the page table]."""
+    rows = kv.page_table.shape[1] * kv.struct.page_size
+    assert x.shape == (kv.layers, kv.num_seqs, kv.kv_heads, rows) and x.dtype is torch.float32 and x.get_device() == kv.ordinal, (x.shape, x.dtype)
+    sl, ss, sh, sr = x.stride()
+    assert sr == 1 or rows == 1, x.stride()
+    return sl, ss, sh if kv.kv_heads > 1 else rows
+
+
+def paged_evict(kv: PagedKV, weights, budget: int, recent: int, weights_out=None, lengths_out=None, scratch=None):
+    """Sequences of more than `budget` rows keep the last `recent` and, of the others, those with the largest weights (f32 [layers, sequences, kv_heads, rows of the
+    page table], as paged_attention_weights adds them up; ties: the lowest row), for every layer and KV head on its own. Rows that stay are moved into the first `budget`
+    places, their order is another then (positions of the next tokens: paged_append). Returns the new lengths (kv.point_at) and weights_out, the
+    weights of the rows where they lie now; what weights_out holds behind them is left as it is."""
+    on = kv.ordinal
+    if weights_out is None:
+        weights_out = torch.empty_like(weights, memory_format=torch.contiguous_format)
+    if lengths_out is None:
+        lengths_out = torch.empty_like(kv.lengths)
+    scratch, at, nbytes = _scratch_of(scratch, _evict_bytes(kv, budget, recent) if scratch is None else 0, kv)
+    _launch(on, lib().im_cuda_paged_evict, kv.dev.handle, kv.ref, weights.data_ptr(), *_sums_of(weights, kv), budget, recent, weights_out.data_ptr(), *_sums_of(weights_out, kv),
+            _ints(lengths_out, on, kv.num_seqs), at, nbytes)
+    return lengths_out, weights_out
+
+
 def paged_keep(kv: PagedKV, accepted, counts, lengths_out=None):
     """The accepted path of every drafted tree, accepted int32 [sequences, most] (places among the new rows, from the root on), counts int32
     [sequences], moves up behind the rows before it, in every layer. Returns the new lengths (kv.point_at)."""
