@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
                 make_uint4(pack16<BF16>(o[0] * inv, o[1] * inv), pack16<BF16>(o[2] * inv, o[3] * inv), pack16<BF16>(o[4] * inv, o[5] * inv), pack16<BF16>(o[6] * inv, o[7] * inv));
         }
         if constexpr (MODE == kWeigh) {  // the sums of this CTA's positions
-            __shared__ RowNorm norms[R];
+            __shared__ float norms[R];
             if (tid < u.rows) {
                 float M = -INFINITY, L = 0.0f;
                 for (int k = 0; k < C; k++) M = fmaxf(M, remote2(of_rank(joint + tid, k)).x);
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
                     const float2 x = remote2(of_rank(joint + tid, k));
                     if (!(x.x == -INFINITY && x.y == 0.0f)) L += x.y * ex2(x.x - M);
                 }
-                norms[tid] = RowNorm(make_float2(M, L));
+                norms[tid] = row_norm(make_float2(M, L));
                 if (!p.scores && rank == 0) p.stat[(long long)(blockIdx.x / C) * R + tid] = make_float2(M, L);
             }
             __syncthreads();
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
                 float v = 0.0f;
                 if (pos >= p.score_cap) v = plain_sum<BF16, HD>(p, u, share.head, pos, norms);
                 else
-                    for (int r = 0; r < u.rows; r++) v += norms[r].weight(scores[(long long)r * p.score_cap + pos]);
+                    for (int r = 0; r < u.rows; r++) v += ex2(scores[(long long)r * p.score_cap + pos] + norms[r]);
                 add_sum(p, u, share.head, pos, v);
             }
         }

@@ -159,18 +159,13 @@ __device__ __forceinline__ size_t part_slot(const PagedAttn &p, int unit, int he
     return (size_t)cta * 2 + slot;
 }
 
-// A row's weight of a position, 2^(score - maximum) / sum, as an exponent and a factor: zero where the row sees nothing.
-struct RowNorm {
-    float base, inv;
-    __device__ __forceinline__ RowNorm() {}
-    __device__ __forceinline__ RowNorm(float2 ml) : base(ml.x == -INFINITY ? 0.0f : ml.x), inv(ml.y > 0.0f ? 1.0f / ml.y : ml.y == 0.0f ? 0.0f : ml.y) {}
-    __device__ __forceinline__ float weight(float score) const { return ex2(score - base) * inv; }
-};
+// A row's weight of a position is 2^(score + norm): minus its maximum and the logarithm of its sum of weights, -inf where it sees nothing.
+__device__ __forceinline__ float row_norm(float2 ml) { return ml.y > 0.0f ? -(ml.x + log2f(ml.y)) : ml.y == 0.0f ? -INFINITY : ml.y; }
 // Adds to the sum of a position of a unit's sequence; a new row's sum starts with this call.
-__device__ __forceinline__ void add_sum(const PagedAttn &p, const PagedUnit &u, int head, int pos, float v) {
+__device__ __forceinline__ void add_sum(const PagedAttn &p, const PagedUnit &u, int head, int pos, float v, bool first = true) {
     if (pos >= p.sum_cols) return;
     float *at = p.sums + u.seq * p.sum_seq + head * p.sum_head + pos;
-    *at = pos >= u.len ? v : *at + v;
+    *at = first && pos >= u.len ? v : *at + v;
 }
 
 // Where a CTA's share starts.
@@ -359,7 +354,7 @@ __device__ __noinline__ void plain_row(const PagedAttn &p, const PagedUnit &u, i
 // The sum of a position's weights over the rows of a unit, from queries and keys: a position a lane (-1: none), rows' norms in `norms`. For positions that a
 // call has no room for the scores of.
 template <bool BF16, int HD>
-__device__ __noinline__ float plain_sum(const PagedAttn &p, const PagedUnit &u, int head, int pos, const RowNorm *norms) {
+__device__ __noinline__ float plain_sum(const PagedAttn &p, const PagedUnit &u, int head, int pos, const float *norms) {
     const long long at = pos >= 0 && pos < u.end ? p.kv.row_of(u.seq, pos) : -1;
     const uint16_t *kc = p.kc + (long long)head * p.kv.page * HD + (at < 0 ? 0 : at);
     float v = 0.0f;
@@ -380,7 +375,7 @@ __device__ __noinline__ float plain_sum(const PagedAttn &p, const PagedUnit &u, 
                 d = fmaf(f.y, g.y, d);
             }
         }
-        v += norms[r].weight(d * p.scale2);
+        v += ex2(fmaf(d, p.scale2, norms[r]));
     }
     return v;
 }

@@ -28,13 +28,11 @@
 
 #include <algorithm>
 
-#include "paged_attn.cuh"
+#include "paged_tc.cuh"
 
 namespace im {
 namespace {
 
-// warps 0-7: weights; 8: products; 9-12: copies
-constexpr int kTcTile = 128, kTcThreads = 13 * 32, kTcMma = 8, kTcCopy = 9, kTcCopyWarps = 4;
 // Growth of a row's maximum (in powers of two) that is left in the weights; power of two that a weight has at the maximum: fp16 weights come up to 2^15, so that
 // they are normal numbers down to 2^-26 of the maximum (exact to 2^-37 below). bf16 has the range of f32. (A growth
 // of 2^8 left in fp16 too: 120.3 us instead of 125.8 for 256 rows over 100003 positions where the scores' spread is four nats, no difference at one.)
@@ -52,44 +50,6 @@ struct TcShape {
     static constexpr int kTiles = kQ + (kK + kV) * kSlot;
     static constexpr int kSmem = (kSmall + 1023) / 1024 * 1024 + kTiles;
     static_assert(kSmem <= 232448, "shared memory of an SM");
-};
-
-// The items of a CTA's share, one after the other; every warp walks them for itself.
-template <int R, int MODE>
-struct Items {
-    const PagedAttn &p;
-    const int units;
-    int unit, head, tile;
-    long long left;
-    PagedUnit u;
-    int tiles, t0, t1, index;
-    __device__ __forceinline__ Items(const PagedAttn &p, int units, const Share &s, const PagedUnit &first)
-        : p(p), units(units), unit(s.unit - 1), head(p.kv.nkv - 1), tile(0), left(s.to - s.from), tiles(0), t0(0), t1(0), index(-1) {
-        if (left > 0) {
-            unit = s.unit;
-            head = s.head - 1;
-            u = first;
-            tiles = unit_tiles<kTcTile, MODE>(u);
-            tile = s.tile;
-        }
-    }
-    __device__ __forceinline__ bool next() {
-        if (left <= 0) return false;
-        if (++head == p.kv.nkv) {
-            head = 0;
-            do {
-                if (++unit >= units) return false;
-                u = paged_unit<R, MODE>(p, unit);
-                tiles = unit_tiles<kTcTile, MODE>(u);
-            } while (tiles == 0);
-        }
-        t0 = tile;
-        t1 = (int)min((long long)tiles, t0 + left);
-        left -= t1 - t0;
-        tile = 0;
-        index++;
-        return true;
-    }
 };
 
 // Bit j: the t-th new token sees position pos + j (32 of them); the rows' being there is another matter.
@@ -114,54 +74,9 @@ __device__ __forceinline__ uint32_t sees32(const PagedAttn &p, const PagedUnit &
     return shift == 0 ? bits : bits << shift | ((1u << shift) - 1);
 }
 
-// Products and commits of one lane (`one`) of a converged warp: what they name is the same in all lanes, and uniform() says so where the compiler
-// cannot see it; from registers of a single lane it would move every operand of every product to a uniform register first.
-__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
-__device__ __forceinline__ uint32_t elected() {
-    uint32_t one;
-    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}\n" : "=r"(one));
-    return one;
-}
-__device__ __forceinline__ void umma_ss(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %5, 0;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(one)
-                 : "memory");
-}
-__device__ __forceinline__ void umma_ts(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {  // A operand in tensor memory
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %5, 0;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(one)
-                 : "memory");
-}
-__device__ __forceinline__ void umma_commit(uint32_t one, uint64_t *bar) {
-    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)), "r"(one)
-                 : "memory");
-}
-// Two f32 side by side.
-__device__ __forceinline__ uint64_t two(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ float2 of_two(uint64_t x) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 // The 256 threads of both halves.
 __device__ __forceinline__ void both_halves() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-// What copies of other threads have written, once their barrier says so, before the tensor cores read it.
-__device__ __forceinline__ void copies_landed() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
 
 template <bool BF16, int KB, bool WIDE, int MODE>
 __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_constant__ PagedAttn p, int units, int *err) {

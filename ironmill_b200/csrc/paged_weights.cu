@@ -5,14 +5,14 @@
 // A weight is known once its row's maximum and sum over all positions are: the attention kernels leave both for every row, and a second look at the scores
 // follows. Up to 16 rows of a KV head (single tokens) the scores themselves are kept, 4 bytes a row and position against 4 * head_dim of keys
 // and values, and a position's thread adds up its rows' weights; short contexts do it in the attention's own launch. With more rows keeping the scores would
-// cost more than the keys: they are computed again, transposed: positions in the rows of mma.sync's tiles, query rows in their columns, so that a position's sum
-// stays in four lanes. Every position is one thread's (or four lanes') own: no atomics, and the same sums on every run.
+// cost more than the keys: the tensor cores compute them again, transposed: positions in the lanes of tensor memory, query rows in its columns, so that a position
+// is one thread's. No atomics, and the same sums on every run.
 #include <limits.h>
 #include <math.h>
 
 #include <algorithm>
 
-#include "paged_attn.cuh"
+#include "paged_tc.cuh"
 
 namespace im {
 namespace {
@@ -23,13 +23,13 @@ constexpr int kSumThreads = 256;
 template <bool BF16, int HD>
 __global__ void __launch_bounds__(kSumThreads) paged_sum_kernel(const __grid_constant__ PagedAttn p) {
     constexpr int R = 16;
-    __shared__ RowNorm norms[R];
+    __shared__ float norms[R];
     pdl_trigger();
     pdl_wait();
     const int item = blockIdx.x, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, tid = threadIdx.x;
     const PagedUnit u = paged_unit<R, kWeigh>(p, unit);
     if ((int)blockIdx.y * kSumThreads >= u.end) return;
-    if (tid < u.rows) norms[tid] = RowNorm(p.stat[(long long)item * R + tid]);
+    if (tid < u.rows) norms[tid] = row_norm(p.stat[(long long)item * R + tid]);
     __syncthreads();
     const float *scores = p.scores + (long long)item * p.score_rows * p.score_cap;
     for (long long pos = (long long)blockIdx.y * kSumThreads + tid; pos < u.end; pos += (long long)gridDim.y * kSumThreads) {
@@ -38,111 +38,270 @@ __global__ void __launch_bounds__(kSumThreads) paged_sum_kernel(const __grid_con
             v = plain_sum<BF16, HD>(p, u, head, (int)pos, norms);
         } else {
 #pragma unroll 4
-            for (int r = 0; r < u.rows; r++) v += norms[r].weight(scores[(long long)r * p.score_cap + pos]);
+            for (int r = 0; r < u.rows; r++) v += ex2(scores[(long long)r * p.score_cap + pos] + norms[r]);
         }
         add_sum(p, u, head, (int)pos, v);
     }
 }
 
-// Sums from queries and keys: a block takes 128 positions of a sequence's KV head, 16 a warp, their keys in registers, and all of its rows, 64 at a time.
-constexpr int kWeighThreads = 256, kWeighTile = 128, kWeighRows = 64;
-template <int HD>
+// Sums from queries and keys on tcgen05, one CTA per SM, an equal share of the list of all (sequence, KV head) items' tiles of 128 positions. Up to
+// kBlockRows of an item's rows stay in shared memory while its tiles of keys pass (more: once more, block by block):
+//     S^T = K Q^T    128 positions x up to 256 rows, f32 in tensor memory, two buffers
+//     sum += 2^(scale S^T + norm of the row), a position per thread, two sets of four warps, every other tile each
+// What bounds it is the exponentials, 16 a clock and SM: 2048 clocks for a tile of 256 rows, of which the products take 1024.
+// All waits are bounded: one that runs out sets the device error word, every warp then runs to its end.
+template <int KB>
 struct WeighShape {
-    static constexpr int kKeys = kWeighTile * HD * 2, kRows = kWeighRows * HD * 2;
-    static constexpr int kSmem = kKeys > 2 * kRows ? kKeys : 2 * kRows;  // the keys' place is the queries' once they are in registers
+    static constexpr int kBlockRows = KB == 4 ? 128 : 256;
+    static constexpr int kBlock = 128 * 128, kSlot = KB * kBlock;  // bytes of 128 positions of 64 columns, of a tile of keys
+    static constexpr int kQBlock = kBlockRows * 128, kQ = KB * kQBlock;
+    static constexpr int kK = KB == 4 ? 2 : KB == 2 ? 4 : 6;       // tiles of keys
+    static constexpr int kBars = 2 * kK + 2 + 4;
+    static constexpr int kSmall = 8 * 16 + kBlockRows * 4 + kTcCopyWarps * 32 * 8 + kBars * 8 + 16;  // presence bits, norms, offsets, barriers, address
+    static constexpr int kTiles = kQ + kK * kSlot;
+    static constexpr int kSmem = (kSmall + 1023) / 1024 * 1024 + kTiles;
+    static_assert(kSmem <= 232448, "shared memory of an SM");
 };
+constexpr int kAllRows = 1 << 30;  // a unit is a sequence
 
-template <bool BF16, int HD>
-__global__ void __launch_bounds__(kWeighThreads, HD == 256 ? 1 : 2) paged_weigh_kernel(const __grid_constant__ PagedAttn p, int R) {
-    using S = WeighShape<HD>;
-    constexpr int KS = HD / 16, CH = HD / 8, RPI = kWeighThreads / CH;
-    extern __shared__ __align__(128) unsigned char weigh_smem[];
-    __shared__ long long offs[kWeighTile];
-    __shared__ RowNorm norms[2][kWeighRows];
+// Bit j: row `row` + j of a sequence (token, query head) sees position pos.
+__device__ __forceinline__ uint32_t rows_seeing(const PagedAttn &p, const PagedUnit &u, int row, int pos) {
+    const int d = pos - u.len, n = u.rows - row;  // place among the new rows
+    const uint32_t are = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
+    if (pos >= u.end || d >= u.fresh) return 0u;
+    if (d < 0) return are;
+    if (!p.mask) {  // those of the d-th token and of later ones
+        const long long from = (long long)d * p.group - row;
+        return from <= 0 ? are : from >= 32 ? 0u : are & ~((1u << from) - 1);
+    }
+    if (d >= 64 * p.mask_words) return 0u;
+    uint32_t seen = 0;
+    int t = row / p.group, left = p.group - (row - t * p.group);  // rows of token t from here on
+    const uint64_t *word = p.mask + (long long)(u.tok0 + t) * p.mask_words + (d >> 6);
+#pragma unroll 1
+    for (int j = 0; j < 32 && j < n; word += p.mask_words, left = p.group) {
+        const int m = min(left, 32 - j);
+        if (__ldg(word) >> (d & 63) & 1) seen |= (m == 32 ? 0xffffffffu : (1u << m) - 1) << j;
+        j += m;
+    }
+    return seen & are;
+}
+
+template <bool BF16, int KB>
+__global__ void __launch_bounds__(kTcThreads, 1) paged_weigh_kernel(const __grid_constant__ PagedAttn p, int units, int stat_rows, int stat_tiles, int *err) {
+    using S = WeighShape<KB>;
+    constexpr int HD = 64 * KB, SK = S::kK, BR = S::kBlockRows;
+    extern __shared__ __align__(16) unsigned char weigh_smem[];
+    uint32_t *there = reinterpret_cast<uint32_t *>(weigh_smem);               // [8 tiles][4]: bit j of word w: row 32 w + j of the tile is in the cache
+    float *norms = reinterpret_cast<float *>(there + 32);                     // [BR]
+    long long *offs = reinterpret_cast<long long *>(norms + BR);              // [copying warps][32]
+    uint64_t *kfull = reinterpret_cast<uint64_t *>(offs + kTcCopyWarps * 32), *kempty = kfull + SK, *qfull = kempty + SK, *qempty = qfull + 1, *sfull = qempty + 1, *sempty = sfull + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(sempty + 2);
+    unsigned char *Qs = weigh_smem + (S::kSmem - S::kTiles), *Ks = Qs + S::kQ;
+    if (smem_u32(Qs) % 1024 != 0) {
+        if (threadIdx.x == 0) atomicExch(err, 1);
+        return;
+    }
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) {
+        for (int i = 0; i < SK; i++) {
+            mbar_init(&kfull[i], kTcCopyWarps * 33);  // threads whose copies are there; warps that have said which rows are
+            mbar_init(&kempty[i], 1);
+        }
+        mbar_init(qfull, kTcCopyWarps * 33);          // (and which norms)
+        mbar_init(qempty, 1 + 8);                     // products done; warps that have read the norms
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&sfull[i], 1);
+            mbar_init(&sempty[i], 4);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kTcMma) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = uniform(*tmem_slot);
     pdl_trigger();
     pdl_wait();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int seq = blockIdx.x / p.kv.nkv, head = blockIdx.x - seq * p.kv.nkv;
-    const PagedUnit u = paged_unit_of<kWeigh>(p, seq * p.row_tiles, INT_MAX);  // all rows of the sequence
-    const uint32_t smem = smem_u32(weigh_smem);
-    const int c = tid % CH, r0 = tid / CH;  // a thread's 16 bytes of a row
-    auto queries = [&](int row0, int buf) {  // 64 rows and their norms
+    PagedUnit at;
+    const Share share = units <= 32 ? warp_share<kAllRows, kTcTile, kWeigh>(p, units, at) : find_share<kAllRows, kTcTile, kTcThreads, kWeigh>(p, units, reinterpret_cast<long long *>(Qs), at);
+    Items<kAllRows, kWeigh> it(p, units, share, at);
+    bool ok = true;
+    int block = 0;  // blocks of rows so far
+    auto columns = [&](const PagedUnit &u, int row0) { return min((u.rows - row0 + 31) / 32 * 32, BR); };
+    if (warp >= kTcCopy) {
+        // ---- copies
+        const int w0 = (warp - kTcCopy) * 32;
+        long long *mine = offs + w0;
+        auto room = [&](uint64_t *bar, uint32_t parity) {
+            if (ok && !mbar_try_wait(bar, parity)) ok = wait_for(bar, parity, err);
+            __syncwarp();
+        };
+        auto requested = [&](uint64_t *bar) {
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+        };
+        // 32 rows, the first at dst, whose offsets (elements from base; -1: none) lanes name; blocks of 64 columns `apart` bytes from one another
+        auto rows32 = [&](unsigned char *dst, int apart, const uint16_t *base, long long o) {
+            constexpr int CH = 8 * KB, RPI = 32 / CH > 0 ? 32 / CH : 1;
+            __syncwarp();
+            mine[lane] = o;
+            __syncwarp();
+            const int c = lane % CH, r0 = lane / CH;
+            const uint32_t to = smem_u32(dst) + (c >> 3) * apart + r0 * 128;
+#pragma unroll 1
+            for (int i0 = 0; i0 < 32 / RPI; i0 += 8) {
+                long long x[8];
 #pragma unroll
-        for (int i = 0; i < kWeighRows / RPI; i++) {
-            const int r = i * RPI + r0, row = row0 + r;
-            const bool there = row < u.rows;
-            const int t = row / p.group, h = head * p.group + row - t * p.group;
-            cp16(smem + buf * S::kRows + r * (HD * 2) + ((c ^ (r & 7)) << 4), p.q + (there ? (u.tok0 + t) * p.qs + (long long)h * HD + c * 8 : 0), there);
-        }
-        if (tid < kWeighRows) {
-            const int row = row0 + tid, unit = seq * p.row_tiles + row / R;
-            norms[buf][tid] = RowNorm(row < u.rows ? p.stat[((long long)unit * p.kv.nkv + head) * R + row % R] : make_float2(0.0f, 0.0f));
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    for (long long tile0 = (long long)blockIdx.y * kWeighTile; tile0 < u.end; tile0 += (long long)gridDim.y * kWeighTile) {
-        const int p0 = (int)tile0;
-        __syncthreads();  // the tile before is done
-        if (tid < kWeighTile) offs[tid] = p0 + tid < u.end ? p.kv.row_of(seq, p0 + tid) : -1;
-        __syncthreads();
-        for (int r = r0; r < kWeighTile; r += RPI) {
-            const long long at = offs[r];
-            cp16(smem + r * (HD * 2) + ((c ^ (r & 7)) << 4), p.kc + (at < 0 ? 0 : at + (long long)head * p.kv.page * HD + c * 8), at >= 0);
-        }
-        asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
-        __syncthreads();
-        uint32_t kf[KS][4];
-        {
-            const int r = warp * 16 + (lane & 15);
+                for (int i = 0; i < 8; i++) x[i] = mine[(i0 + i) * RPI + r0];
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) ldsm4(kf[ks], smem + r * (HD * 2) + (((2 * ks + (lane >> 4)) ^ (r & 7)) << 4));
-        }
-        __syncthreads();
-        queries(0, 0);
-        float sum[2] = {0.0f, 0.0f};
-        const int chunks = (u.rows + kWeighRows - 1) / kWeighRows, pos = p0 + warp * 16 + (lane >> 2);
-        for (int k = 0; k < chunks; k++) {
-            if (k + 1 < chunks) queries((k + 1) * kWeighRows, (k + 1) & 1);
-            else asm volatile("cp.async.commit_group;" ::: "memory");
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            __syncthreads();
-            const uint32_t qs = smem + (k & 1) * S::kRows;
-            const bool edge = p0 + warp * 16 + 16 > u.len || (k + 1) * kWeighRows > u.rows;  // some row does not see some position, or is none
-#pragma unroll 2
-            for (int j = 0; j < kWeighRows / 8; j++) {
-                if (k * kWeighRows + j * 8 >= u.rows) break;
-                float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                const int r = j * 8 + (lane & 7);
-#pragma unroll
-                for (int ks = 0; ks < KS; ks += 2) {
-                    uint32_t b[4];
-                    ldsm4(b, qs + r * (HD * 2) + (((2 * ks + (lane >> 3)) ^ (r & 7)) << 4));
-                    mma16<BF16>(s, kf[ks], b[0], b[1]);
-                    mma16<BF16>(s, kf[ks + 1], b[2], b[3]);
+                for (int i = 0; i < 8; i++) {
+                    const int r = (i0 + i) * RPI;
+                    cp16(to + r * 128 + (((c & 7) ^ ((r + r0) & 7)) << 4), base + (x[i] < 0 ? 0 : x[i] + c * 8), x[i] >= 0);
                 }
-                const int at = j * 8 + (lane & 3) * 2;
-                const RowNorm a = norms[k & 1][at], b = norms[k & 1][at + 1];
-                float w[4] = {a.weight(s[0] * p.scale2), b.weight(s[1] * p.scale2), a.weight(s[2] * p.scale2), b.weight(s[3] * p.scale2)};
-                if (edge) {
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int row = k * kWeighRows + at + (i & 1), x = pos + (i >> 1) * 8;
-                        if (row >= u.rows || x >= u.end || !paged_sees(p, u, row / p.group, x)) w[i] = 0.0f;
-                    }
-                }
-                sum[0] += w[0] + w[1];
-                sum[1] += w[2] + w[3];
             }
-            __syncthreads();  // everyone has read the rows before others come in their place
+        };
+        int kc = 0;
+        auto lookup = [&](const PagedUnit &u, int head, int pos) -> long long {
+            if (pos >= u.end) return -1;
+            const long long o = p.kv.row_of(u.seq, pos);
+            return o < 0 ? -1 : o + (long long)head * p.kv.page * HD;
+        };
+        while (it.next()) {
+            const PagedUnit &u = it.u;
+            for (int row0 = 0; row0 < u.rows; row0 += BR, block++) {
+                long long o = lookup(u, it.head, it.t0 * kTcTile + w0 + lane);
+                if (block > 0) room(qempty, (block - 1) & 1);
+                const int n = columns(u, row0);
+                for (int r = w0; r < n; r += kTcCopyWarps * 32) {
+                    const int row = row0 + r + lane, t = row / p.group, g = row - t * p.group;
+                    const bool is = row < u.rows;
+                    rows32(Qs + r * 128, S::kQBlock, p.q, is ? (u.tok0 + t) * p.qs + (long long)(it.head * p.group + g) * HD : -1);
+                    norms[r + lane] = is ? row_norm(p.stat[(((long long)u.seq * stat_tiles + row / stat_rows) * p.kv.nkv + it.head) * stat_rows + row % stat_rows]) : -INFINITY;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(qfull);
+                requested(qfull);
+                for (int t = it.t0; t < it.t1; t++) {
+                    const int ks = kc % SK;
+                    const long long next = t + 1 < it.t1 ? lookup(u, it.head, (t + 1) * kTcTile + w0 + lane) : -1;
+                    if (kc >= SK) room(&kempty[ks], (kc / SK - 1) & 1);
+                    const unsigned word = __ballot_sync(0xffffffffu, o >= 0);
+                    if (lane == 0) {
+                        there[(kc & 7) * 4 + w0 / 32] = word;
+                        mbar_arrive(&kfull[ks]);
+                    }
+                    rows32(Ks + ks * S::kSlot + w0 * 128, S::kBlock, p.kc, o);
+                    requested(&kfull[ks]);
+                    kc++;
+                    o = next;
+                }
+            }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (warp == kTcMma) {
+        // ---- products; instruction descriptor as in paged_attn_tc.cu, N (rows) in bits 17-22
+        constexpr uint32_t kType = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(128 >> 4) << 24);
+        const uint32_t one = elected();
+        const uint64_t qd = desc_sw128(smem_u32(Qs), 16), kd = desc_sw128(smem_u32(Ks), 16);
+        int ks = 0, tile = 0;
+        uint32_t kturn = 0;
+        auto wait = [&](uint64_t *bar, uint32_t parity) {
+            if (ok && !mbar_try_wait(bar, parity)) ok = wait_for(bar, parity, err);
+            __syncwarp();
+        };
+        while (it.next()) {
+            for (int row0 = 0; row0 < it.u.rows; row0 += BR, block++) {
+                const uint32_t idesc = kType | (uniform(columns(it.u, row0)) >> 3 << 17);
+                wait(qfull, block & 1);
+#pragma unroll 1
+                for (int t = it.t0; t < it.t1; t++, tile++) {
+                    wait(&kfull[ks], kturn);
+                    if (tile >= 2) wait(&sempty[tile & 1], (tile / 2 - 1) & 1);
+                    copies_landed();
+                    fence_after();
+                    if (ok) {
+                        const uint64_t a = kd + ks * (S::kSlot / 16);
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
-            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
-            const int x = pos + i * 8;
-            if ((lane & 3) == 0 && x < u.end) add_sum(p, u, head, x, offs[x - p0] < 0 ? 0.0f : sum[i]);
+                        for (int j = 0; j < KB * 4; j++)
+                            umma_ss(one, tmem + (uint32_t)((tile & 1) * 256), a + (j / 4 * S::kBlock + (j & 3) * 32) / 16, qd + (j / 4 * S::kQBlock + (j & 3) * 32) / 16, idesc, j > 0);
+                        umma_commit(one, &sfull[tile & 1]);
+                        umma_commit(one, &kempty[ks]);
+                        if (t == it.t1 - 1) umma_commit(one, qempty);
+                    }
+                    if (++ks == SK) ks = 0, kturn ^= 1;
+                }
+            }
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncwarp();
+    } else {
+        // ---- sums: a position per thread
+        const int h = warp >> 2, r = (warp & 3) * 32 + lane;
+        const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(h * 256);
+        const uint64_t scale_two = two(p.scale2, p.scale2);
+        int tile = 0;
+        while (it.next()) {
+            const PagedUnit &u = it.u;
+            for (int row0 = 0; row0 < u.rows; row0 += BR, block++) {
+                if (ok && !wait_for(qfull, block & 1, err)) ok = false;  // the norms
+                const int n = columns(u, row0);
+                for (int t = it.t0; t < it.t1; t++, tile++) {
+                    if ((tile & 1) != h) continue;
+                    if (ok && !wait_for(&sfull[h], (tile / 2) & 1, err)) ok = false;
+                    fence_after();
+                    const int pos = t * kTcTile + r;
+                    const bool is = (there[(tile & 7) * 4 + (warp & 3)] >> lane & 1u) != 0;
+                    const bool edge = t * kTcTile + kTcTile > u.len;  // some row may not see some position
+                    uint64_t sum[2] = {0, 0};
+#pragma unroll 1
+                    for (int c = 0; c < n; c += 32) {
+                        uint32_t s[32];
+                        ld32(ts + (uint32_t)c, s);
+                        float4 a[8];
+#pragma unroll
+                        for (int j = 0; j < 8; j++) a[j] = *reinterpret_cast<const float4 *>(norms + c + 4 * j);
+                        tmem_wait_ld();
+                        if (edge) {
+                            const uint32_t seen = rows_seeing(p, u, row0 + c, pos);
+#pragma unroll
+                            for (int j = 0; j < 32; j++)
+                                if (!(seen >> j & 1u)) s[j] = p.scale2 < 0.0f ? 0x7f800000u : 0xff800000u;  // a score of -inf
+                        }
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const float2 e0 = of_two(fma_two(two(__uint_as_float(s[4 * j]), __uint_as_float(s[4 * j + 1])), scale_two, two(a[j].x, a[j].y)));
+                            const float2 e1 = of_two(fma_two(two(__uint_as_float(s[4 * j + 2]), __uint_as_float(s[4 * j + 3])), scale_two, two(a[j].z, a[j].w)));
+                            sum[0] = add_two(sum[0], two(ex2(e0.x), ex2(e0.y)));
+                            sum[1] = add_two(sum[1], two(ex2(e1.x), ex2(e1.y)));
+                        }
+                    }
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sempty[h]);
+                    const float2 x = of_two(sum[0]), y = of_two(sum[1]);
+                    float v = (x.x + x.y) + (y.x + y.y);
+                    // an infinite or missing key times the zeros that fill up the rows, or something that is one: from the rows that see it alone
+                    if (__any_sync(0xffffffffu, is && !(v - v == 0.0f))) {
+                        PagedUnit part = u;
+                        part.row0 = row0;
+                        part.rows = min(u.rows - row0, BR);
+                        const float w = plain_sum<BF16, HD>(p, part, it.head, pos, norms);
+                        if (!(v - v == 0.0f)) v = w;
+                    }
+                    if (pos < u.end) add_sum(p, u, it.head, pos, is ? v : 0.0f, row0 == 0);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(qempty);
+            }
+        }
+    }
+    fence_before();
+    sync_and_settle(ok);
+    if (warp == kTcMma) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
 }
 
@@ -176,14 +335,18 @@ WeighPlan weigh_plan(const Device *dev, const PagedView &v, int group, int max_n
 
 template <bool BF16, int HD>
 int sums(const Device *dev, const PagedAttn &p, const WeighPlan &plan, int max_len, cudaStream_t st) {
-    using S = WeighShape<HD>;
+    if (p.scores) {
+        const unsigned blocks = (unsigned)std::max(1ll, std::min((max_len + (long long)kSumThreads - 1) / kSumThreads, 65535ll));
+        IM_CUDA_CHECK(launch_k(paged_sum_kernel<BF16, HD>, dim3((unsigned)(plan.attn.units * p.kv.nkv), blocks), dim3(kSumThreads), 0, st, p));
+        return IM_OK;
+    }
+    using S = WeighShape<HD / 64>;
     static DeviceOnce once;
-    if (once.first(dev->ordinal)) IM_CUDA_CHECK(cudaFuncSetAttribute((paged_weigh_kernel<BF16, HD>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
-    const auto blocks = [&](long long positions) { return (unsigned)std::max(1ll, std::min((max_len + positions - 1) / positions, 65535ll)); };
-    if (p.scores)
-        IM_CUDA_CHECK(launch_k(paged_sum_kernel<BF16, HD>, dim3((unsigned)(plan.attn.units * p.kv.nkv), blocks(kSumThreads)), dim3(kSumThreads), 0, st, p));
-    else
-        IM_CUDA_CHECK(launch_k(paged_weigh_kernel<BF16, HD>, dim3((unsigned)(p.kv.nseq * p.kv.nkv), blocks(kWeighTile)), dim3(kWeighThreads), (size_t)S::kSmem, st, p, plan.attn.rows));
+    if (once.first(dev->ordinal)) IM_CUDA_CHECK(cudaFuncSetAttribute((paged_weigh_kernel<BF16, HD / 64>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+    PagedAttn w = p;
+    w.row_tiles = 1;
+    w.ctas = (int)std::max(1ll, std::min<long long>(dev->sm_count, (long long)p.kv.nseq * p.kv.nkv * ((max_len + (long long)kTcTile - 1) / kTcTile)));
+    IM_CUDA_CHECK(launch_k(paged_weigh_kernel<BF16, HD / 64>, dim3(w.ctas), dim3(kTcThreads), (size_t)S::kSmem, st, w, p.kv.nseq, plan.attn.rows, plan.attn.row_tiles, dev->err_flag));
     return IM_OK;
 }
 
