@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
     auto fetch = [&]() {
         n_page = -1;
         if (f_left <= 0) return;
-        const int pos = unit_from<MODE>(f_u) + f_tile * kPaTile + warp * kPaSlice + (lane & 15);
+        const int pos = f_tile * kPaTile + warp * kPaSlice + (lane & 15);
         if (pos < f_u.end) {
             const int pg = pos / p.kv.page;
             n_slot = pos - pg * p.kv.page;
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
                     mma16<BF16>(s[1], qf[ks], b[2], b[3]);
                 }
             }
-            const int pos0 = unit_from<MODE>(u) + tile * kPaTile + warp * kPaSlice;
+            const int pos0 = tile * kPaTile + warp * kPaSlice;
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
@@ -266,8 +266,8 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
         }
         __syncthreads();
         if (tid == 0) bad_rows[!odd_item] = 0;  // every thread has looked at the last item's
-        const bool whole = whole_items<MODE>() && !CL && t0 == 0 && t1 == tiles;
-        const size_t part = part_slot<MODE>(p, unit, head, t0, t1, tiles, blockIdx.x, first_item ? 0 : 1) * R;
+        const bool whole = !CL && t0 == 0 && t1 == tiles;
+        const size_t part = ((size_t)blockIdx.x * 2 + (first_item ? 0 : 1)) * R;
         if (!CL && tid == 0) note_span<MODE>(p, unit, head, t0, t1, tiles, blockIdx.x, first_item ? 0 : 1);
         float f[2];
 #pragma unroll
@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
             for (int r = warp; r < u.rows; r += kPaWarps) {
                 if (!(bad >> r & 1)) continue;
                 float x[HD / 32], M, L;
-                plain_row<BF16, HD>(p, u, head, r, unit_from<MODE>(u) + t0 * kPaTile, min(unit_from<MODE>(u) + t1 * kPaTile, u.end), x, M, L);
+                plain_row<BF16, HD>(p, u, head, r, t0 * kPaTile, min(t1 * kPaTile, u.end), x, M, L);
                 const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
                 const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
                 for (int i = 0; i < HD / 32; i++) {
@@ -534,28 +534,7 @@ int attn_launch(const Device *dev, const PagedAttn &p, int units, int cluster, c
     return join_launch<BF16, S::kRows, HD, MODE>(p, units, st);
 }
 
-template <bool BF16, int HD, int MODE>
-int part_launch(const Device *dev, const PagedAttn &p, int units, cudaStream_t st) {
-    using S = PaShape<HD>;
-    static DeviceOnce once;
-    if (once.first(dev->ordinal)) IM_CUDA_CHECK(cudaFuncSetAttribute((paged_attn_kernel<BF16, HD, false, MODE>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
-    IM_CUDA_CHECK(launch_k(paged_attn_kernel<BF16, HD, false, MODE>, dim3(p.ctas), dim3(kPaThreads), (size_t)S::kSmem, st, p, units));
-    return IM_OK;
-}
-
 }  // namespace
-
-int paged_part_launch(const Device *dev, const PagedAttn &p, bool bf16, int mode, int units, cudaStream_t st) {
-#define IM_MODE(B, HD) (mode == kShared ? part_launch<B, HD, kShared>(dev, p, units, st) : part_launch<B, HD, kOwn>(dev, p, units, st))
-#define IM_RUN(HD) (bf16 ? IM_MODE(true, HD) : IM_MODE(false, HD))
-    switch (p.kv.hd) {
-    case 64: return IM_RUN(64);
-    case 128: return IM_RUN(128);
-    default: return IM_RUN(256);
-    }
-#undef IM_RUN
-#undef IM_MODE
-}
 
 int paged_weigh_launch(const Device *dev, const PagedAttn &p, bool bf16, int units, int cluster, cudaStream_t st) {
 #define IM_RUN(HD) (bf16 ? attn_launch<true, HD, kWeigh>(dev, p, units, cluster, st) : attn_launch<false, HD, kWeigh>(dev, p, units, cluster, st))
@@ -613,7 +592,7 @@ int attn_args(im_device *dev, const im_paged_kv *kv, int layer, const void *q_de
     p->scale2 = scale * 1.4426950408889634f;
     if (p->scale2 == 0.0f) p->scale2 = 1e-30f;  // every position alike, without 0 * inf at the hidden ones
     p->group_start = p->prefix_pages = nullptr;
-    p->groups = p->whole_slot = 0;
+    p->groups = p->whole_slot = p->early = 0;
     p->stat = nullptr;
     p->scores = p->sums = nullptr;
     return IM_OK;

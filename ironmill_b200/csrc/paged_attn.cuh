@@ -25,6 +25,7 @@ struct PagedAttn {
     const int *group_start, *prefix_pages;  // [groups + 1] sequences, [groups]
     int groups;
     int whole_slot;           // kShared, kOwn: slots from here on are those of items that one CTA had, by item
+    int early;                // kOwn: a kShared launch that this one needs nothing of may still run (see paged_prefix.cu)
     // sums of softmax weights (paged_weights.cu)
     float2 *stat;             // [units, KV heads, rows of a tile]: maximum and sum of weights of every row
     float *scores;            // or NULL: [units, KV heads, score_rows, score_cap]: scores of the positions before score_cap, in powers of two
@@ -392,8 +393,7 @@ int attn_check(const im_paged_kv *kv, int num_heads, int max_new);
 int attn_args(im_device *dev, const im_paged_kv *kv, int layer, const void *q_dev, int64_t q_stride, void *out_dev, int64_t out_stride, int num_heads,
               const int *token_start_dev, int num_tokens, int max_new, const uint64_t *mask_dev, int mask_words, float scale, int max_len, PagedAttn *p, bool *empty);
 
-// The kernels of both files with the sums of a part as their result (paged_prefix.cu): MODE kShared or kOwn; no join.
-int paged_part_launch(const Device *dev, const PagedAttn &p, bool bf16, int mode, int units, cudaStream_t st);
+// The kernel of paged_attn_tc.cu with the sums of a part as its result (paged_prefix.cu): MODE kShared or kOwn; no join.
 int paged_tc_part_launch(const Device *dev, const PagedAttn &p, bool bf16, int mode, int rows, int units, cudaStream_t st);
 // Attention and the norms of every row's weights (paged_weights.cu): where `cluster` is not zero, the sums too. With joins.
 int paged_weigh_launch(const Device *dev, const PagedAttn &p, bool bf16, int units, int cluster, cudaStream_t st);

@@ -127,8 +127,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     __syncthreads();
     fence_after();
     const uint32_t tmem = uniform(*tmem_slot);
-    pdl_trigger();  // after the allocation: a successor on this SM cannot take the columns first
-    pdl_wait();
+    if constexpr (MODE == kShared) {
+        pdl_wait();     // what starts behind the trigger finds everything before this launch done
+        pdl_trigger();
+    } else {
+        pdl_trigger();  // after the allocation: a successor on this SM cannot take the columns first
+        if (MODE != kOwn || !p.early) pdl_wait();
+    }
     PagedUnit at;
     const Share share = units <= 32 ? warp_share<R, kTcTile, MODE>(p, units, at) : find_share<R, kTcTile, kTcThreads, MODE>(p, units, reinterpret_cast<long long *>(Qs), at);  // (the copies start behind its last barrier)
     Items<R, MODE> it(p, units, share, at);
@@ -490,6 +495,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     }
     fence_before();
     sync_and_settle(ok);
+    if (MODE == kOwn && p.early && blockIdx.x == 0) pdl_wait();  // this launch ends after the one before it
     if (warp == kTcMma) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");

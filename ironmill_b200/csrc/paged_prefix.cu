@@ -3,10 +3,15 @@
 //   out[t, h] = (sum_shared 2^(s_j - M) v_j + sum_own 2^(s_j - M) v_j) / (sum_shared 2^(s_j - M) + sum_own 2^(s_j - M))
 //
 // Softmax sums over two sets of positions add up once both refer to the same maximum. The first set, the shared pages, is the same for all tokens of a group,
-// whose rows (token, query head of a KV head) lie one after the other: for the kernels of paged_attn.cu and paged_attn_tc.cu a group is one sequence
-// with all these rows and without new positions (kShared), so that its keys and values are read once and its rows fill the tensor cores' tiles. The second
-// set, each sequence's own rows, is a sequence that starts behind its prefix (kOwn). Both leave sums, maximum and weighted values in f32, and the launch
-// below joins them, a warp per (token, query head).
+// whose rows (token, query head of a KV head) lie one after the other: a group is one sequence with all these rows and without new positions (kShared), so
+// that its keys and values are read once and its rows fill the tensor cores' tiles. The second set, each sequence's own rows, is a sequence that starts
+// behind its prefix (kOwn). Both leave sums, maximum and weighted values in f32, and a last launch joins them.
+//
+// More than 16 rows of a unit go to paged_attn_tc.cu. Up to 16 rows (single tokens' own rows, small groups) are taken here by CTAs that each read one run
+// of positions, all of it requested at once, and end: several per SM in different phases hide the lookups, the loads' latency and the joining of
+// warps behind each other's loads. (Equal shares of one list, as in paged_attn.cu, spend most of short items' time on their ends.)
+// The launch for the own rows needs nothing of the one for the shared rows and starts beside it: kShared triggers its successor once everything before it is
+// done, the successor does not wait at its start, and its first CTA waits at its end, so that the join finds both done.
 #include <limits.h>
 #include <math.h>
 
@@ -17,117 +22,417 @@
 namespace im {
 namespace {
 
-// One of the two sets as the join sees it.
+// One of the two sets.
 struct PartSet {
     PagedAttn p;
-    int rows;  // of a tile
-    int tc;    // parts in the order of paged_attn_tc.cu, a NaN as the sum of weights of a row that has to be done again
+    int rows;    // of a tile
+    int tc;      // by paged_attn_tc.cu: a NaN as the sum of weights of a row that has to be done again
+    int chunks;  // else: CTAs, and so parts, of an item
 };
 struct PrefixJoin {
     PartSet shared, own;
     int group_new;
 };
 
-constexpr int kPjWarps = 8;
+// ------------------------------------------------------------------------------------------------ up to 16 rows
+constexpr int kPtWarps = 4, kPtThreads = kPtWarps * 32, kPtRows = 16;
+template <int HD>
+struct PtShape {
+    static constexpr int kSlices = HD == 256 ? 1 : 2;          // of 16 positions, a warp's
+    static constexpr int kChunk = kPtWarps * kSlices * 16;
+    static constexpr int kPitch = HD + 8;                      // floats of a row of sums in shared memory
+    static constexpr int kKeys = kSlices * 16 * HD * 2, kSums = kPtRows * kPitch * 4;
+    static constexpr int kWarp = 2 * kKeys > kSums ? 2 * kKeys : kSums;  // sums take the place of keys and values
+    static constexpr int kSmem = kPtWarps * kWarp;
+};
 
-// Adds what the parts of row `r` of an item hold to a row's maximum, sum and columns lane * V .. of its values.
+// Chunks c, c + set.chunks, ... of an item.
 template <bool BF16, int HD, int MODE>
-__device__ __forceinline__ void add_parts(const PartSet &s, int unit, int head, const PagedUnit &u, int r, float &M, float &L, float (&o)[HD / 32]) {
-    constexpr int V = HD / 32;
-    const PagedAttn &p = s.p;
-    const int lane = threadIdx.x & 31, R = s.rows;
-    const int2 span = *reinterpret_cast<const int2 *>(p.spans + 2 * ((long long)unit * p.kv.nkv + head));
-    const bool whole = span.x >= p.whole_slot;
-    const int c = span.x >> 1, parts = whole ? 1 : span.y - c + 1;
-    auto slot = [&](int i) { return i == 0 ? (size_t)span.x : (size_t)(c + i) * 2; };
-    for (int i0 = 0; i0 < parts; i0 += 32) {
-        const float2 x = i0 + lane < parts ? p.part_ml[slot(i0 + lane) * R + r] : make_float2(-INFINITY, 0.0f);
-        if (s.tc && __any_sync(0xffffffffu, x.y != x.y)) {  // not finite on the tensor cores: the whole row again, from the positions that it sees
-            float y[V], m, l;
-            plain_row<BF16, HD>(p, u, head, r, unit_from<MODE>(u), u.end, y, m, l);
-            if (m == -INFINITY && l == 0.0f) return;
-            const float top = fmaxf(M, m), f = ex2(m - top), corr = M == top ? 1.0f : ex2(M - top);
-            M = top;
-            L = L * corr + l * f;
+__device__ __forceinline__ void part_of_item(const PartSet &set, int item, int c, unsigned char *smem, float2 *ml, unsigned &bad_rows) {
+    using S = PtShape<HD>;
+    constexpr float kLift = BF16 ? 0.0f : 15.0f;  // fp16 weights: 2^15 at the row's maximum, as in paged_attn.cu
+    constexpr int R = kPtRows, KS = HD / 16, NT = HD / 8, CH = HD / 8, SL = S::kSlices;
+    const PagedAttn &p = set.p;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int unit = item / p.kv.nkv, head = item - unit * p.kv.nkv;
+    const PagedUnit u = paged_unit<R, MODE>(p, unit);
+    const int from = unit_from<MODE>(u), all = max(u.end - from + S::kChunk - 1, 0) / S::kChunk;
+    if (c >= all) return;
+    unsigned char *mine = smem + warp * S::kWarp;
+    const uint32_t ks_at = smem_u32(mine), vs_at = ks_at + S::kKeys;
+    uint32_t qf[KS][4];
+    int tok[2];
 #pragma unroll
-            for (int j = 0; j < V; j++) {  // column lane * V + j lies with lane (lane * V + j) % 32
-                float v = 0.0f;
+    for (int i = 0; i < 2; i++) tok[i] = (u.row0 + min((lane >> 2) + 8 * i, u.rows - 1)) / p.group;
+    float m[2], l[2], o[NT][4];
 #pragma unroll
-                for (int k = 0; k < V; k++) {
-                    const float w = __shfl_sync(0xffffffffu, y[k], (lane * V + j) & 31);
-                    if ((lane * V + j) / 32 == k) v = w;
-                }
-                o[j] = o[j] * corr + v * f;
+    for (int i = 0; i < 2; i++) m[i] = -INFINITY, l[i] = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NT; n++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[n][j] = 0.0f;
+    bool first = true;
+    for (int k = c; k < all; k += set.chunks) {
+        const int pos0 = from + k * S::kChunk + warp * (SL * 16);
+        const int pos = pos0 + (lane & (SL * 16 - 1));
+        const long long row = pos < u.end ? p.kv.row_of(u.seq, pos) : -1;
+        const unsigned there = __ballot_sync(0xffffffffu, row >= 0);
+        const long long off = row < 0 ? -1 : row + (long long)head * p.kv.page * HD;
+        constexpr int RPI = 32 / CH > 0 ? 32 / CH : 1;  // rows of one request of the warp
+        __syncwarp();  // the chunk before has been read
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++) {
+#pragma unroll
+            for (int i = 0; i < SL * 16 / RPI; i++) {
+                const int r = i * RPI + (RPI > 1 ? lane / CH : 0), c8 = lane & (CH - 1);
+                const long long at = __shfl_sync(0xffffffffu, off, r);
+                cp16((kv ? vs_at : ks_at) + r * (HD * 2) + ((c8 ^ (r & 7)) << 4), (kv ? p.vc : p.kc) + (at < 0 ? 0 : at + c8 * 8), at >= 0);
             }
-            return;
+            asm volatile("cp.async.commit_group;" ::: "memory");
         }
-        const float top = fmaxf(M, warp_max(x.x)), corr = M == top ? 1.0f : ex2(M - top);
-        const float f = x.x == -INFINITY && x.y == 0.0f ? 0.0f : ex2(x.x - top);  // (nothing seen in this part)
-        M = top;
-        L = L * corr + warp_sum(x.y * f);
+        if (first) {  // queries: A fragments, rows lane / 4 and lane / 4 + 8
+            first = false;
 #pragma unroll
-        for (int j = 0; j < V; j++) o[j] *= corr;
-        const int m = min(32, parts - i0);
-#pragma unroll 4
-        for (int i = 0; i < m; i++) {
-            const float g = __shfl_sync(0xffffffffu, f, i);
-            const float *src = s.tc ? p.part_o + (slot(i0 + i) * (HD / 4) + lane * V / 4) * (R * 4) + r * 4 + lane * V % 4 : p.part_o + (slot(i0 + i) * R + r) * HD + lane * V;
-            float v[V];
-            if constexpr (V == 2) *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(src);
-            else
+            for (int i = 0; i < 2; i++) {
+                const int r = (lane >> 2) + 8 * i;
+                const uint32_t *src = reinterpret_cast<const uint32_t *>(p.q + (u.tok0 + tok[i]) * p.qs + (long long)(head * p.group + (u.row0 + r) % p.group) * HD);
 #pragma unroll
-                for (int j = 0; j < V; j += 4) *reinterpret_cast<float4 *>(v + j) = *reinterpret_cast<const float4 *>(src + j);
+                for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-            for (int j = 0; j < V; j++) o[j] += g == 0.0f ? 0.0f : v[j] * g;
+                    for (int j = 0; j < 2; j++) qf[ks][2 * j + i] = r < u.rows ? __ldg(src + ks * 8 + j * 4 + (lane & 3)) : 0u;
+            }
         }
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncwarp();
+        float s[2 * SL][4];
+#pragma unroll
+        for (int n = 0; n < 2 * SL; n++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) s[n][j] = 0.0f;
+#pragma unroll
+        for (int sl = 0; sl < SL; sl++) {
+            const int r = sl * 16 + (lane & 7) + ((lane >> 4) << 3), hi = (lane >> 3) & 1;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                uint32_t b[4];
+                ldsm4(b, ks_at + r * (HD * 2) + (((2 * ks + hi) ^ (r & 7)) << 4));
+                mma16<BF16>(s[2 * sl], qf[ks], b[0], b[1]);
+                mma16<BF16>(s[2 * sl + 1], qf[ks], b[2], b[3]);
+            }
+        }
+        const unsigned full = SL == 2 ? 0xffffffffu : 0xffffu;
+        const bool part = (there & full) != full || (MODE == kOwn && pos0 + SL * 16 > u.len);  // some row may not see some position
+#pragma unroll
+        for (int n = 0; n < 2 * SL; n++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                s[n][j] *= p.scale2;
+                if (part) {
+                    const int at = n * 8 + (lane & 3) * 2 + (j & 1);
+                    if (!(there >> at & 1) || !paged_sees(p, u, tok[j >> 1], pos0 + at)) s[n][j] = -INFINITY;
+                }
+            }
+        uint32_t w[SL][4], w2[SL][4];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < 2 * SL; n++) top = fmaxf(top, fmaxf(s[n][2 * i], s[n][2 * i + 1]));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            if (__any_sync(0xffffffffu, top > m[i])) {
+                const float m_new = fmaxf(m[i], top), corr = m_new == -INFINITY ? 1.0f : ex2(m[i] - m_new);
+                m[i] = m_new;
+                l[i] *= corr;
+#pragma unroll
+                for (int n = 0; n < NT; n++) o[n][2 * i] *= corr, o[n][2 * i + 1] *= corr;
+            }
+            const float base = m[i] == -INFINITY ? 0.0f : m[i] - kLift;
+            float sum = 0.0f;
+#pragma unroll
+            for (int n = 0; n < 2 * SL; n++) {  // weights as two 16-bit terms
+                const float x0 = ex2(s[n][2 * i] - base), x1 = ex2(s[n][2 * i + 1] - base);
+                sum += x0 + x1;
+                const uint32_t x = pack16<BF16>(x0, x1);
+                const float2 back = unpack16<BF16>(x);
+                w[n / 2][2 * (n & 1) + i] = x;
+                w2[n / 2][2 * (n & 1) + i] = pack16<BF16>(x0 - back.x, x1 - back.y);
+            }
+            l[i] += sum;
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncwarp();
+#pragma unroll
+        for (int sl = 0; sl < SL; sl++) {
+            const int r = sl * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), hi = lane >> 4;
+#pragma unroll
+            for (int n = 0; n < NT; n += 2) {
+                uint32_t b[4];
+                ldsm4t(b, vs_at + r * (HD * 2) + (((n + hi) ^ (r & 7)) << 4));
+                mma16<BF16>(o[n], w[sl], b[0], b[1]);
+                mma16<BF16>(o[n + 1], w[sl], b[2], b[3]);
+                mma16<BF16>(o[n], w2[sl], b[0], b[1]);
+                mma16<BF16>(o[n + 1], w2[sl], b[2], b[3]);
+            }
+        }
+    }
+    // ---- four warps' sums joined, in order
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+        l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+        if ((lane & 3) == 0) ml[warp * R + (lane >> 2) + 8 * i] = make_float2(m[i], l[i]);
+    }
+    __syncwarp();
+    float *sums = reinterpret_cast<float *>(mine);
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int r = (lane >> 2) + 8 * i;
+        if (r < u.rows)
+#pragma unroll
+            for (int n = 0; n < NT; n++) *reinterpret_cast<float2 *>(sums + r * S::kPitch + n * 8 + (lane & 3) * 2) = make_float2(o[n][2 * i], o[n][2 * i + 1]);
+    }
+    if (tid == 0) bad_rows = 0;
+    __syncthreads();
+    const size_t slot = ((size_t)item * set.chunks + c) * R;
+    for (int i = tid; i < u.rows * (HD / 4); i += kPtThreads) {
+        const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+        float M = -INFINITY, L = 0.0f, worst = 0.0f;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < kPtWarps; k++) M = fmaxf(M, ml[k * R + r].x);
+#pragma unroll
+        for (int k = 0; k < kPtWarps; k++) {
+            const float2 a = ml[k * R + r];
+            const float4 v = *reinterpret_cast<const float4 *>(smem + k * S::kWarp + (r * S::kPitch + d) * 4);
+            if (a.x == -INFINITY && a.y == 0.0f) {  // nothing seen: zeros, or zeros times something that is not finite
+                continue;
+            }
+            const float f = ex2(a.x - M);
+            L += a.y * f;
+            x.x += v.x * f; x.y += v.y * f; x.z += v.z * f; x.w += v.w * f;
+        }
+        worst = x.x * 0.0f + x.y * 0.0f + x.z * 0.0f + x.w * 0.0f;
+        if (worst != 0.0f) atomicOr(&bad_rows, 1u << r);
+        *reinterpret_cast<float4 *>(p.part_o + (slot + r) * HD + d) = x;
+        if (d == 0) p.part_ml[slot + r] = make_float2(M - kLift, L);  // (plain_row has no lift)
+    }
+    __syncthreads();
+    if (const unsigned bad = bad_rows) {
+        for (int r = warp; r < u.rows; r += kPtWarps) {
+            if (!(bad >> r & 1)) continue;
+            float M = -INFINITY, L = 0.0f, x[HD / 32];
+#pragma unroll
+            for (int i = 0; i < HD / 32; i++) x[i] = 0.0f;
+            for (int k = c; k < all; k += set.chunks) {
+                float y[HD / 32], m2, l2;
+                plain_row<BF16, HD>(p, u, head, r, from + k * S::kChunk, min(from + (k + 1) * S::kChunk, u.end), y, m2, l2);
+                if (m2 == -INFINITY && l2 == 0.0f) continue;
+                const float top = fmaxf(M, m2), f = ex2(m2 - top), corr = M == top ? 1.0f : ex2(M - top);
+                M = top;
+                L = L * corr + l2 * f;
+#pragma unroll
+                for (int i = 0; i < HD / 32; i++) x[i] = x[i] * corr + y[i] * f;
+            }
+#pragma unroll
+            for (int i = 0; i < HD / 32; i++) p.part_o[(slot + r) * HD + lane + 32 * i] = x[i];
+            if (lane == 0) p.part_ml[slot + r] = make_float2(M, L);
+        }
+    }
+}
+
+// CTAs below `shared_ctas` for the shared rows, the others for the own ones.
+template <bool BF16, int HD>
+__global__ void __launch_bounds__(kPtThreads, HD == 256 ? 2 : 3) paged_part_kernel(const __grid_constant__ PrefixJoin a, int shared_ctas) {
+    extern __shared__ __align__(128) unsigned char pt_smem[];
+    __shared__ float2 ml[kPtWarps * kPtRows];
+    __shared__ unsigned bad_rows;
+    pdl_trigger();
+    if (!a.own.p.early) pdl_wait();
+    const int b = blockIdx.x;
+    if (b < shared_ctas) {
+        part_of_item<BF16, HD, kShared>(a.shared, b / a.shared.chunks, b % a.shared.chunks, pt_smem, ml, bad_rows);
+    } else {
+        const int i = b - shared_ctas;
+        part_of_item<BF16, HD, kOwn>(a.own, i / a.own.chunks, i % a.own.chunks, pt_smem, ml, bad_rows);
+    }
+    if (a.own.p.early && b == 0) pdl_wait();  // this launch ends after the one before it
+}
+
+// ------------------------------------------------------------------------------------------------ the join
+// A block takes eight rows (token, query head of one KV head, token-major), a thread four columns of one: eight rows of a column quad lie side by side in the parts of
+// paged_attn_tc.cu. Warps look the rows up, then lanes the parts' maxima and sums, 32 parts at a time; factors go to shared memory.
+constexpr int kPjRows = 8, kPjParts = 32;
+struct PjRow {
+    int token, seq;           // -1: not to be written
+    long long out;
+    int slot0[2], next[2], parts[2], r[2];  // shared, own: slot of the first part, of the second less two (tcgen05) or one, number of parts, row of the tile
+    int unit[2];              // -1: no parts
+};
+
+template <bool BF16, int HD, int MODE>
+__device__ __forceinline__ void find_parts(const PartSet &s, int unit, int head, int r, PjRow &x) {
+    constexpr int w = MODE == kOwn;
+    const PagedUnit u = paged_unit_of<MODE>(s.p, unit, s.rows);
+    const int from = unit_from<MODE>(u);
+    if (r >= u.rows || u.end <= from) return;
+    x.r[w] = r;
+    x.unit[w] = unit;
+    const long long item = (long long)unit * s.p.kv.nkv + head;
+    if (s.tc) {
+        const int2 span = *reinterpret_cast<const int2 *>(s.p.spans + 2 * item);
+        x.slot0[w] = span.x;
+        x.next[w] = (span.x >> 1) * 2;
+        x.parts[w] = span.x >= s.p.whole_slot ? 1 : span.y - (span.x >> 1) + 1;
+    } else {
+        x.slot0[w] = x.next[w] = (int)(item * s.chunks);
+        x.parts[w] = min(s.chunks, (u.end - from + PtShape<HD>::kChunk - 1) / PtShape<HD>::kChunk);
     }
 }
 
 template <bool BF16, int HD>
-__global__ void __launch_bounds__(kPjWarps * 32) paged_prefix_join_kernel(const __grid_constant__ PrefixJoin a) {
-    constexpr int V = HD / 32;
+__global__ void __launch_bounds__(2 * HD) paged_prefix_join_kernel(const __grid_constant__ PrefixJoin a) {
+    constexpr int V = HD / 32, kWarps = 2 * HD / 32;
+    __shared__ PjRow rows[kPjRows];
+    __shared__ float factor[kPjRows][kPjParts];
+    __shared__ float2 state[kPjRows];  // maximum and sum so far
+    __shared__ float corr[kPjRows];
+    __shared__ float again[kPjRows][HD];
+    __shared__ int more[2], odd;
     pdl_trigger();
     pdl_wait();
     const PagedAttn &p = a.own.p;
-    const int token = blockIdx.x, lane = threadIdx.x & 31, h = blockIdx.y * kPjWarps + (threadIdx.x >> 5);
-    if (h >= p.group * p.kv.nkv || token < __ldg(p.start) || token >= __ldg(p.start + p.kv.nseq)) return;
-    const int seq = paged_seq_of(p.start, p.kv.nseq, token), first = __ldg(p.start + seq), t = token - first;
-    if (first < 0 || t < 0 || t >= p.max_new || __ldg(p.start + seq + 1) > p.tokens || token >= __ldg(p.start + seq + 1)) return;
-    const int head = h / p.group, hq = h - head * p.group, group = paged_group_of(p, seq);
-    float M = -INFINITY, L = 0.0f, o[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) o[j] = 0.0f;
-    if (group >= 0) {
-        const long long place = (long long)token - __ldg(p.start + min(max(__ldg(p.group_start + group), 0), p.kv.nseq));
-        if (place < 0 || place >= a.group_new) return;
-        const int row = (int)place * p.group + hq, unit = group * a.shared.p.row_tiles + row / a.shared.rows, r = row % a.shared.rows;
-        const PagedUnit u = paged_unit_of<kShared>(a.shared.p, unit, a.shared.rows);
-        if (r < u.rows) add_parts<BF16, HD, kShared>(a.shared, unit, head, u, r, M, L, o);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, head = blockIdx.y;
+    if (tid < 2) more[tid] = 0;
+    if (tid == 2) odd = 0;
+    if (tid < kPjRows) state[tid] = make_float2(-INFINITY, 0.0f);
+    __syncthreads();
+    for (int i = warp; i < kPjRows; i += kWarps) {
+        const long long at = (long long)blockIdx.x * kPjRows + i;
+        PjRow x;
+        x.token = -1;
+        x.parts[0] = x.parts[1] = 0;
+        x.unit[0] = x.unit[1] = -1;
+        const int token = (int)min(at / p.group, (long long)INT_MAX), hq = (int)(at - (long long)token * p.group);
+        if (token < p.tokens && token >= __ldg(p.start) && token < __ldg(p.start + p.kv.nseq)) {
+            const int seq = paged_seq_of(p.start, p.kv.nseq, token), first = __ldg(p.start + seq), end = __ldg(p.start + seq + 1), t = token - first;
+            if (first >= 0 && t >= 0 && t < p.max_new && end <= p.tokens && token < end) {
+                const int group = paged_group_of(p, seq);
+                const long long place = group < 0 ? 0 : (long long)token - __ldg(p.start + min(max(__ldg(p.group_start + group), 0), p.kv.nseq));
+                if (place >= 0 && place < a.group_new) {
+                    x.token = token;
+                    x.seq = seq;
+                    x.out = token * p.os + (long long)(head * p.group + hq) * HD;
+                    if (group >= 0) {
+                        const int row = (int)place * p.group + hq;
+                        find_parts<BF16, HD, kShared>(a.shared, group * a.shared.p.row_tiles + row / a.shared.rows, head, row % a.shared.rows, x);
+                    }
+                    const int row = t * p.group + hq;
+                    find_parts<BF16, HD, kOwn>(a.own, seq * p.row_tiles + row / a.own.rows, head, row % a.own.rows, x);
+                }
+            }
+        }
+        if (lane == 0) {
+            rows[i] = x;
+            atomicMax(&more[0], x.parts[0]);
+            atomicMax(&more[1], x.parts[1]);
+        }
     }
-    const int row = t * p.group + hq, unit = seq * p.row_tiles + row / a.own.rows, r = row % a.own.rows;
-    const PagedUnit u = paged_unit_of<kOwn>(p, unit, a.own.rows);
-    if (r < u.rows && u.end > u.from) add_parts<BF16, HD, kOwn>(a.own, unit, head, u, r, M, L, o);
-    const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
-    uint32_t *dst = reinterpret_cast<uint32_t *>(p.out + token * p.os + (long long)h * HD + lane * V);
+    __syncthreads();
+    const int r = tid % kPjRows, q = tid / kPjRows;  // this thread's row and columns 4 q ..
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+    for (int w = 0; w < 2; w++) {
+        const PartSet &s = w ? a.own : a.shared;
+        const int most = more[w], step = s.tc ? 2 : 1;
+        for (int i0 = 0; i0 < most; i0 += kPjParts) {
+            for (int i = warp; i < kPjRows; i += kWarps) {
+                const int part = i0 + lane, n = rows[i].parts[w];
+                float2 x = make_float2(-INFINITY, 0.0f);
+                if (part < n) x = s.p.part_ml[(size_t)(part == 0 ? rows[i].slot0[w] : rows[i].next[w] + part * step) * s.rows + rows[i].r[w]];
+                const bool redo = s.tc && __any_sync(0xffffffffu, x.y != x.y);  // not finite on the tensor cores: the row is done again below
+                const float2 before = state[i];
+                const float top = fmaxf(before.x, warp_max(x.x)), c = before.x == top ? 1.0f : ex2(before.x - top);
+                const float f = x.x == -INFINITY && x.y == 0.0f ? 0.0f : ex2(x.x - top);  // (nothing seen in this part)
+                const float l = before.y * c + warp_sum(x.y * f);
+                factor[i][lane] = f;
+                __syncwarp();
+                if (lane == 0) {
+                    state[i] = make_float2(top, l);
+                    corr[i] = c;
+                    if (redo) atomicOr(&odd, 1 << i);
+                }
+            }
+            __syncthreads();
+            const float c = corr[r];
+            o = make_float4(o.x * c, o.y * c, o.z * c, o.w * c);
+            const PjRow &x = rows[r];
+            const int n = min(x.parts[w] - i0, kPjParts);
+            const size_t pitch = s.tc ? (size_t)s.rows * 4 : 4, first = s.tc ? (size_t)x.r[w] * 4 + q * pitch : (size_t)x.r[w] * HD + q * pitch;
+#pragma unroll 6
+            for (int i = 0; i < n; i++) {
+                const int part = i0 + i;
+                const size_t slot = part == 0 ? x.slot0[w] : x.next[w] + part * step;
+                const float4 v = *reinterpret_cast<const float4 *>(s.p.part_o + slot * s.rows * HD + first);
+                const float f = factor[r][i];
+                if (f != 0.0f) o.x += v.x * f, o.y += v.y * f, o.z += v.z * f, o.w += v.w * f;
+            }
+            __syncthreads();
+        }
+    }
+    // ---- rows with sums on the tensor cores that are not finite: both sets again, from the positions that the row sees alone
+    for (int w = 0; w < 2 && odd; w++) {
+        for (int i = warp; i < kPjRows; i += kWarps) {
+            if (!(odd >> i & 1)) continue;
+            const float2 before = w ? state[i] : make_float2(-INFINITY, 0.0f);
+            float y[V], m = -INFINITY, l = 0.0f;
+            if (rows[i].unit[w] >= 0) {
+                const PartSet &s = w ? a.own : a.shared;
+                const PagedUnit u = w ? paged_unit_of<kOwn>(s.p, rows[i].unit[w], s.rows) : paged_unit_of<kShared>(s.p, rows[i].unit[w], s.rows);
+                plain_row<BF16, HD>(s.p, u, head, rows[i].r[w], u.from, u.end, y, m, l);
 #pragma unroll
-    for (int j = 0; j < V; j += 2) dst[j / 2] = pack16<BF16>(o[j] * inv, o[j + 1] * inv);
+                for (int j = 0; j < V; j++) again[i][lane + 32 * j] = y[j];
+            }
+            const float top = fmaxf(before.x, m), c = before.x == top ? 1.0f : ex2(before.x - top), f = m == -INFINITY && l == 0.0f ? 0.0f : ex2(m - top);
+            __syncwarp();
+            if (lane == 0) state[i] = make_float2(top, before.y * c + l * f), corr[i] = c, factor[i][0] = f;
+        }
+        __syncthreads();
+        if (odd >> r & 1) {
+            const float c = corr[r], f = factor[r][0];
+            o = w ? make_float4(o.x * c, o.y * c, o.z * c, o.w * c) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (f != 0.0f) o.x += again[r][4 * q] * f, o.y += again[r][4 * q + 1] * f, o.z += again[r][4 * q + 2] * f, o.w += again[r][4 * q + 3] * f;
+        }
+        __syncthreads();
+    }
+    if (rows[r].token < 0) return;
+    const float L = state[r].y, inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
+    *reinterpret_cast<uint2 *>(p.out + rows[r].out + 4 * q) = make_uint2(pack16<BF16>(o.x * inv, o.y * inv), pack16<BF16>(o.z * inv, o.w * inv));
 }
 
+// ------------------------------------------------------------------------------------------------ plans
 struct PartPlan {
-    int rows, tile, row_tiles, units, ctas;
-    size_t slots, bytes;
+    int rows, row_tiles, units, tc;
+    int ctas;          // tcgen05
+    size_t slots, spans;
+    size_t bytes;
 };
+// Parts of an item where it has up to 16 rows: CTAs for about eight rounds over the GPU, at most one per chunk.
+constexpr int kMostChunks = 64;
 PartPlan part_plan(const Device *dev, int units, int nkv, int hd, long long rows) {
     PartPlan a;
     const int tc = paged_tc_rows(hd, rows);
-    a.rows = tc ? tc : 16;
-    a.tile = tc ? 128 : 64;
+    a.tc = tc > 0;
+    a.rows = tc ? tc : kPtRows;
     a.row_tiles = (int)((rows + a.rows - 1) / a.rows);
     a.units = units * a.row_tiles;
-    a.ctas = dev->sm_count * (tc || hd == 256 ? 1 : 2);
+    a.ctas = dev->sm_count;
     const size_t items = (size_t)a.units * nkv;
-    a.slots = ((size_t)a.ctas * 2 + items) * a.rows;
-    a.bytes = a.slots * hd * 4 + a.slots * 8 + (items * 8 + 15) / 16 * 16;
+    a.spans = tc ? (items * 8 + 15) / 16 * 16 : 0;
+    a.slots = 0;
+    if (tc) a.slots = ((size_t)a.ctas * 2 + items) * a.rows;
+    else if (items) a.slots = items * std::max<size_t>(1, std::min<size_t>(kMostChunks, (size_t)24 * dev->sm_count / items)) * a.rows;
+    a.bytes = a.slots * hd * 4 + a.slots * 8 + a.spans;
     return a;
 }
 
@@ -151,10 +456,15 @@ int prefix_check(const im_paged_kv *kv, int num_heads, int num_groups, int max_g
 }
 
 // The launch's own: where its sums go, from `at` on.
-unsigned char *lay_out(PagedAttn *p, const PartPlan &plan, int max_rows, unsigned char *at) {
+unsigned char *lay_out(PartSet *s, const PartPlan &plan, int max_rows, int likely_rows, unsigned char *at) {
+    PagedAttn *p = &s->p;
+    s->rows = plan.rows;
+    s->tc = plan.tc;
     p->row_tiles = plan.row_tiles;
-    const long long tiles = (long long)plan.units * p->kv.nkv * ((max_rows + (long long)plan.tile - 1) / plan.tile);
-    p->ctas = (int)std::max(1ll, std::min<long long>(plan.ctas, tiles));
+    const long long items = (long long)plan.units * p->kv.nkv;
+    p->ctas = (int)std::max(1ll, std::min<long long>(plan.ctas, items * ((max_rows + 127ll) / 128)));
+    const int chunk = p->kv.hd == 256 ? 64 : 128;
+    s->chunks = plan.tc || items == 0 ? 1 : (int)std::max(1ll, std::min<long long>((likely_rows + (long long)chunk - 1) / chunk, (long long)(plan.slots / items / plan.rows)));
     p->whole_slot = 2 * plan.ctas;
     p->part_o = reinterpret_cast<float *>(at);
     p->part_ml = reinterpret_cast<float2 *>(p->part_o + plan.slots * p->kv.hd);
@@ -164,8 +474,37 @@ unsigned char *lay_out(PagedAttn *p, const PartPlan &plan, int max_rows, unsigne
 }
 
 template <bool BF16, int HD>
-int join(const PrefixJoin &a, int heads, cudaStream_t st) {
-    IM_CUDA_CHECK(launch_k(paged_prefix_join_kernel<BF16, HD>, dim3((unsigned)a.own.p.tokens, (unsigned)((heads + kPjWarps - 1) / kPjWarps)), dim3(kPjWarps * 32), 0, st, a));
+int part_launch(const Device *dev, const PrefixJoin &a, int shared_ctas, int own_ctas, cudaStream_t st) {
+    using S = PtShape<HD>;
+    static DeviceOnce once;
+    if (once.first(dev->ordinal)) IM_CUDA_CHECK(cudaFuncSetAttribute((paged_part_kernel<BF16, HD>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+    IM_CUDA_CHECK(launch_k(paged_part_kernel<BF16, HD>, dim3((unsigned)(shared_ctas + own_ctas)), dim3(kPtThreads), (size_t)S::kSmem, st, a, shared_ctas));
+    return IM_OK;
+}
+
+template <bool BF16, int HD>
+int run(const Device *dev, PrefixJoin &a, const PrefixPlan &plan, cudaStream_t st) {
+    const int nkv = a.own.p.kv.nkv;
+    int rc = IM_OK, shared_ctas = 0, own_ctas = 0;
+    if (plan.shared.units > 0) {
+        if (plan.shared.tc) {
+            rc = paged_tc_part_launch(dev, a.shared.p, BF16, kShared, plan.shared.rows, plan.shared.units, st);
+            a.own.p.early = 1;
+        } else {
+            shared_ctas = plan.shared.units * nkv * a.shared.chunks;
+        }
+    }
+    if (rc != IM_OK) return rc;
+    if (plan.own.tc) {
+        if (shared_ctas) rc = part_launch<BF16, HD>(dev, a, shared_ctas, 0, st);
+        if (rc == IM_OK) rc = paged_tc_part_launch(dev, a.own.p, BF16, kOwn, plan.own.rows, plan.own.units, st);
+    } else {
+        own_ctas = plan.own.units * nkv * a.own.chunks;
+        rc = part_launch<BF16, HD>(dev, a, shared_ctas, own_ctas, st);
+    }
+    if (rc != IM_OK) return rc;
+    const long long rows = (long long)a.own.p.tokens * a.own.p.group;
+    IM_CUDA_CHECK(launch_k(paged_prefix_join_kernel<BF16, HD>, dim3((unsigned)((rows + kPjRows - 1) / kPjRows), (unsigned)nkv), dim3(2 * HD), 0, st, a));
     return IM_OK;
 }
 
@@ -198,6 +537,7 @@ IM_EXPORT int im_cuda_paged_prefix_attention(im_device *dev, const im_paged_kv *
     bool empty;
     rc = attn_args(dev, kv, layer, q_dev, q_stride, out_dev, out_stride, num_heads, token_start_dev, num_tokens, max_new, mask_dev, mask_words, scale, max_len, &p, &empty);
     if (rc != IM_OK || empty) return rc;
+    IM_REQUIRE(kv->num_kv_heads <= 65535, "at most 65535 key / value heads (got %d)", kv->num_kv_heads);
     const PrefixPlan plan = prefix_plan(dev, p.kv, p.group, max_new, num_groups, max_group_new);
     IM_REQUIRE(scratch_dev && aligned16(scratch_dev) && scratch_bytes >= plan.bytes, "paged prefix attention needs %zu bytes of 16-byte aligned scratch (got %zu)", plan.bytes,
                scratch_dev ? scratch_bytes : (size_t)0);
@@ -210,21 +550,11 @@ IM_EXPORT int im_cuda_paged_prefix_attention(im_device *dev, const im_paged_kv *
     a.shared.p.mask = nullptr;
     a.shared.p.max_new = max_group_new;
     a.group_new = max_group_new;
-    unsigned char *at = lay_out(&a.shared.p, plan.shared, max_prefix, static_cast<unsigned char *>(scratch_dev));
-    lay_out(&p, plan.own, max_len, at);
-    a.shared.rows = plan.shared.rows;
-    a.own.rows = plan.own.rows;
-    a.shared.tc = plan.shared.rows > 16;
-    a.own.tc = plan.own.rows > 16;
+    unsigned char *at = lay_out(&a.shared, plan.shared, max_prefix, max_prefix, static_cast<unsigned char *>(scratch_dev));
+    lay_out(&a.own, plan.own, max_len, num_groups ? std::max(1, max_len - max_prefix) : max_len, at);
     const cudaStream_t st = as_stream(stream);
     const bool bf16 = kv->dtype == IM_DTYPE_BF16;
-    const auto parts = [&](const PartSet &s, const PartPlan &q, int mode) {
-        return s.tc ? paged_tc_part_launch(dev, s.p, bf16, mode, q.rows, q.units, st) : paged_part_launch(dev, s.p, bf16, mode, q.units, st);
-    };
-    if (num_groups > 0) rc = parts(a.shared, plan.shared, kShared);
-    if (rc == IM_OK) rc = parts(a.own, plan.own, kOwn);
-    if (rc != IM_OK) return rc;
-#define IM_RUN(HD) (bf16 ? join<true, HD>(a, num_heads, st) : join<false, HD>(a, num_heads, st))
+#define IM_RUN(HD) (bf16 ? run<true, HD>(dev, a, plan, st) : run<false, HD>(dev, a, plan, st))
     switch (kv->head_dim) {
     case 64: return IM_RUN(64);
     case 128: return IM_RUN(128);
