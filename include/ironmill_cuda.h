@@ -388,11 +388,10 @@ int im_cuda_paged_attention_weights(im_device *dev, const im_paged_kv *kv, int l
  * afterwards: give the next tokens their positions (position_dev of paged_append).  weights, weights_out f32 [num_layers, num_seqs, num_kv_heads, table_width * page_size],
  * layers, sequences and heads apart by their strides; weights_out gets the sums of the rows where they lie now (and of sequences that fit, as they are), entries from the new
  * length on are left as they are.  seq_len_out_dev [num_seqs]: min(seq_len, budget).  A sequence's pages up to its length are its own (not shared with another).  A row that is
- * not there is not moved, nor is one moved to a place that is not there.  weights_out and seq_len_out lie over nothing that is read, nor over each other. */
-size_t im_cuda_paged_evict_scratch_bytes(const im_device *dev, const im_paged_kv *kv, int budget, int recent);
+ * not there is not moved, nor is one moved to a place that is not there.  Page tables of up to 2^19 rows.  weights_out and seq_len_out lie over nothing that is read, nor over each other. */
 int im_cuda_paged_evict(im_device *dev, const im_paged_kv *kv, const float *weights_dev, int64_t layer_stride, int64_t seq_stride, int64_t head_stride, int budget,
                         int recent, float *weights_out_dev, int64_t out_layer_stride, int64_t out_seq_stride, int64_t out_head_stride, int *seq_len_out_dev,
-                        void *scratch_dev, size_t scratch_bytes, void *stream);
+                        void *stream);
 
 /* The accepted path of a tree: in every layer row seq_len + accepted_dev[s, j] becomes row seq_len + j, j = 0 .. count_dev[s] - 1
  * (accepted [num_seqs, max_accept], each path in order from the root: accepted[s, j] >= j; an entry below j is not moved).

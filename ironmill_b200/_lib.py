@@ -37,7 +37,7 @@ _SIZE_RESTYPE = ("im_cuda_device_allocated_bytes", "im_cuda_buffer_length", "im_
                  "im_cuda_model_memory_bytes", "im_cuda_model_step_bytes", "im_cuda_tq_scratch_bytes",
                  "im_cuda_sdpa_f16_scratch_bytes", "im_cuda_tq_prefill_scratch_bytes",
                  "im_cuda_paged_attention_scratch_bytes", "im_cuda_paged_prefix_attention_scratch_bytes",
-                 "im_cuda_paged_attention_weights_scratch_bytes", "im_cuda_paged_evict_scratch_bytes", "im_cuda_beam_select_scratch_bytes")
+                 "im_cuda_paged_attention_weights_scratch_bytes", "im_cuda_beam_select_scratch_bytes")
 _VOID_RESTYPE = ("im_cuda_device_free", "im_cuda_buffer_free", "im_cuda_affine_weight_free", "im_cuda_model_free",
                  "im_cuda_tq_free", "im_cuda_tp_free")
 
@@ -52,8 +52,7 @@ _ARGTYPES = {
     "im_cuda_paged_prefix_attention": (_P, _P, _I, _P, _L, _P, _L, _I, _P, _I, _I, _P, _I, _I, _P, _I, _P, _I, _F, _I, _P, _Z, _P),
     "im_cuda_paged_attention_weights_scratch_bytes": (_P, _P, _I, _I, _I),
     "im_cuda_paged_attention_weights": (_P, _P, _I, _P, _L, _P, _L, _I, _P, _I, _I, _P, _I, _F, _I, _P, _L, _L, _I, _P, _Z, _P),
-    "im_cuda_paged_evict_scratch_bytes": (_P, _P, _I, _I),
-    "im_cuda_paged_evict": (_P, _P, _P, _L, _L, _L, _I, _I, _P, _L, _L, _L, _P, _P, _Z, _P),
+    "im_cuda_paged_evict": (_P, _P, _P, _L, _L, _L, _I, _I, _P, _L, _L, _L, _P, _P),
     "im_cuda_paged_keep": (_P, _P, _P, _I, _P, _P, _P),
     "im_cuda_paged_reorder": (_P, _P, _P, _I, _P, _L, _P, _P),
     "im_cuda_beam_select_scratch_bytes": (_P, _I, _I, _I, _I),

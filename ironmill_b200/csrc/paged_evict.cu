@@ -5,9 +5,9 @@
 // behind them. That moves the fewest rows: closing up in order would move nearly all of them for one that leaves, and attention does not
 // ask for their order (keys are rotated already). What order means something for, the recent rows, is kept.
 //
-// Two launches. The first finds the H-th largest sum of its (layer, sequence, head) by digits of 8 bits from the top, each a histogram in shared memory, walks the rows
-// once more in order, and lists sources and targets. The second moves rows, a block per (layer, sequence, head) of the keys or the values. HBM bounds the second, the
-// chain of passes over one list the first.
+// One launch, a block per (layer, sequence, head) and slice of the columns of keys or values. Every block finds the H-th largest sum for itself (the sums are 4 bytes beside 4 * head_dim
+// of a row): by digits of 8 bits from the top, each a histogram in shared memory; then one bit a row says whether it stays, and the i-th free place below H and the i-th row that
+// comes from behind are found by their ranks among the bits. No lists, no scratch, nothing between blocks. While some blocks of an SM choose, others move: HBM bounds the whole.
 #include <limits.h>
 
 #include <algorithm>
@@ -19,14 +19,14 @@ namespace {
 
 struct Evict {
     PagedView kv;
+    uint4 *kc, *vc;
     const float *w;
     float *w_out;
     long long w_layer, w_seq, w_head, o_layer, o_seq, o_head;
     int budget, recent;
     int *len_out;
-    int *count;  // [layers, sequences, heads]: moves
-    int *moves;  // [layers, sequences, heads, 2, most]: targets, sources
-    int most;
+    int cols;       // 16-byte columns of a slice
+    int bit_words;  // of 32 rows
 };
 
 // Larger sums have larger keys; a NaN counts as the lowest, -0 as 0.
@@ -37,6 +37,7 @@ __device__ __forceinline__ uint32_t sum_key(float w) {
 }
 
 constexpr int kEvThreads = 256, kEvWarps = kEvThreads / 32;
+constexpr int kMoveRows = 128, kMoveAhead = 8;  // rows of a batch; 16-byte pieces that a thread holds
 
 // Sums of v over the threads before this one, the block's total in `total`.
 __device__ __forceinline__ int block_before(int v, int *of_warp, int &total) {
@@ -60,21 +61,44 @@ __device__ __forceinline__ int block_before(int v, int *of_warp, int &total) {
     return before + s - v;
 }
 
-__global__ void __launch_bounds__(kEvThreads) paged_evict_select_kernel(const __grid_constant__ Evict a) {
+// The position of the set (clear: not set) bit with `rank` such bits before it, among words [lo, hi); before[w]: bits set in the words before w.
+__device__ __forceinline__ int nth_bit(const uint32_t *bits, const int *before, int lo, int hi, int rank, bool clear) {
+    // the last word whose count before it is not above rank
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1, b = clear ? mid * 32 - before[mid] : before[mid];
+        if (b <= rank) lo = mid;
+        else hi = mid;
+    }
+    uint32_t word = clear ? ~bits[lo] : bits[lo];
+    rank -= clear ? lo * 32 - before[lo] : before[lo];
+    int at = lo * 32;
+#pragma unroll
+    for (int half = 16; half > 0; half >>= 1) {
+        const int low = __popc(word & ((1u << half) - 1));
+        if (rank >= low) rank -= low, word >>= half, at += half;
+    }
+    return at;
+}
+
+__global__ void __launch_bounds__(kEvThreads, 4) paged_evict_kernel(const __grid_constant__ Evict a) {
+    extern __shared__ __align__(16) uint32_t ev_smem[];
     __shared__ int bins[kEvWarps][256];
     __shared__ int of_warp[kEvWarps];
     __shared__ int found[2];
+    uint32_t *bits = ev_smem;                                              // [bit_words]: rows that stay
+    int *before = reinterpret_cast<int *>(bits + a.bit_words);             // [bit_words + 1]: of them in the words before
+    long long *src = reinterpret_cast<long long *>(&bins[0][0]), *dst = src + kMoveRows;  // (the histograms are done then)
     pdl_trigger();
     pdl_wait();
-    const int tid = threadIdx.x, warp = tid >> 5, problem = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, problem = blockIdx.x, slice = blockIdx.y;
     const int head = problem % a.kv.nkv, seq = problem / a.kv.nkv % a.kv.nseq, layer = problem / a.kv.nkv / a.kv.nseq;
     const int n = a.kv.length(seq), H = a.budget - a.recent, old = n - a.recent;
     const float *w = a.w + layer * a.w_layer + seq * a.w_seq + head * a.w_head;
     float *out = a.w_out + layer * a.o_layer + seq * a.o_seq + head * a.o_head;
-    if (layer == 0 && head == 0 && tid == 0) a.len_out[seq] = min(n, a.budget);
+    if (layer == 0 && head == 0 && slice == 0 && tid == 0) a.len_out[seq] = min(n, a.budget);
     if (n <= a.budget) {
-        for (int i = tid; i < n; i += kEvThreads) out[i] = w[i];
-        if (tid == 0) a.count[problem] = 0;
+        if (slice == 0)
+            for (int i = tid; i < n; i += kEvThreads) out[i] = w[i];
         return;
     }
     // ---- the H-th largest key, digit by digit; `above` of the others are larger
@@ -83,8 +107,9 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_select_kernel(const __
     for (int shift = 24; shift >= 0 && H > 0; shift -= 8) {
         for (int i = tid; i < kEvWarps * 256; i += kEvThreads) (&bins[0][0])[i] = 0;
         __syncthreads();
+#pragma unroll 4
         for (int i = tid; i < old; i += kEvThreads) {
-            const uint32_t k = sum_key(w[i]);
+            const uint32_t k = sum_key(__ldg(w + i));
             if ((k & mask) == top) atomicAdd(&bins[warp][k >> shift & 255], 1);
         }
         __syncthreads();
@@ -92,97 +117,87 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_select_kernel(const __
         int mine = 0, total;
 #pragma unroll
         for (int i = 0; i < kEvWarps; i++) mine += bins[i][255 - tid];
-        const int before = above + block_before(mine, of_warp, total);
-        if (before < H && before + mine >= H) found[0] = 255 - tid, found[1] = before;
+        const int larger = above + block_before(mine, of_warp, total);
+        if (larger < H && larger + mine >= H) found[0] = 255 - tid, found[1] = larger;
         __syncthreads();
         top |= (uint32_t)found[0] << shift;
         mask |= 255u << shift;
         above = found[1];
         __syncthreads();
     }
-    const int equal = H - above;  // so many of the rows with that key stay, the lowest
-    // ---- in order of the rows: places that become free below H, rows that come from behind
-    int *to = a.moves + (long long)problem * 2 * a.most, *from = to + a.most;
-    int equals = 0, holes = 0, movers = 0;
-    for (int r0 = 0; r0 < old && H > 0; r0 += kEvThreads) {
+    // ---- which rows stay: larger keys, and of equal ones the lowest rows
+    int equal = H - above, equals = 0, stay = 0;
+    const int words = (old + 31) / 32;
+    for (int r0 = 0; r0 < words * 32; r0 += kEvThreads) {
         const int r = r0 + tid;
-        const float x = r < old ? w[r] : 0.0f;
-        const uint32_t k = r < old ? sum_key(x) : 0;
-        const bool same = r < old && k == top;
-        int total;
-        const int rank = equals + block_before(same, of_warp, total);
-        equals += total;
-        const bool stays = r < old && (k > top || (same && rank < equal));
-        const bool hole = r < H && !stays, mover = r >= H && stays;
-        const int place = block_before((hole ? 1 : 0) | (mover ? 1 << 16 : 0), of_warp, total);
-        if (hole) to[holes + (place & 0xffff)] = r;
-        if (mover) from[movers + (place >> 16)] = r;
-        holes += total & 0xffff;
-        movers += total >> 16;
-        if (r < H && stays) out[r] = x;
+        const uint32_t k = r < old && H > 0 ? sum_key(__ldg(w + r)) : 0;
+        const bool more = r < old && H > 0 && k > top, same = r < old && H > 0 && k == top;
+        const unsigned these = __ballot_sync(0xffffffffu, same);
+        // (ranks among equals matter where some of them leave: their count over the block's warps)
+        __syncthreads();
+        if (lane == 0) of_warp[warp] = __popc(these);
+        __syncthreads();
+        int rank = equals, all = 0;
+#pragma unroll
+        for (int i = 0; i < kEvWarps; i++) {
+            if (i < warp) rank += of_warp[i];
+            all += of_warp[i];
+        }
+        equals += all;
+        const unsigned word = __ballot_sync(0xffffffffu, more || (same && rank + __popc(these & ((1u << lane) - 1)) < equal));
+        if (lane == 0 && r / 32 < words) bits[r / 32] = word;
     }
     __syncthreads();
-    for (int i = tid; i < movers; i += kEvThreads) out[to[i]] = w[from[i]];
-    for (int i = tid; i < a.recent; i += kEvThreads) out[H + i] = w[old + i];
-    if (tid == 0) a.count[problem] = movers;
-}
-
-// A block per (layer, sequence, head) of keys or values. Sixteen bytes a lane; what comes from behind first (its sources lie from H on, its targets below), then the
-// recent rows, a batch read before it is written: a target lies before its source, so no batch writes over what a later one reads.
-constexpr int kMoveRows = 128;
-__global__ void __launch_bounds__(kEvThreads) paged_evict_move_kernel(const __grid_constant__ Evict a, uint4 *kc, uint4 *vc) {
-    __shared__ long long src[kMoveRows], dst[kMoveRows];
-    pdl_trigger();
-    pdl_wait();
-    const int tid = threadIdx.x, problem = blockIdx.x;
-    const int head = problem % a.kv.nkv, seq = problem / a.kv.nkv % a.kv.nseq, layer = problem / a.kv.nkv / a.kv.nseq;
-    const int n = a.kv.length(seq), H = a.budget - a.recent, old = n - a.recent;
-    if (n <= a.budget) return;
-    const int words = a.kv.hd / 8;
-    uint4 *base = (blockIdx.y ? vc : kc) + layer * (a.kv.layer_stride / 8) + (long long)head * a.kv.page * words;
-    const int *to = a.moves + (long long)problem * 2 * a.most, *from = to + a.most;
-    const int movers = a.count[problem], total = movers + a.recent;
+    for (int w0 = 0; w0 < words; w0 += kEvThreads) {
+        int total;
+        const int c = w0 + tid < words ? __popc(bits[w0 + tid]) : 0, b = stay + block_before(c, of_warp, total);
+        if (w0 + tid < words) before[w0 + tid] = b;
+        stay += total;
+    }
+    if (tid == 0) before[words] = stay;
+    __syncthreads();
+    const int low = H / 32, kept_below = before[low] + (H % 32 ? __popc(bits[low] & ((1u << (H % 32)) - 1)) : 0);  // (H < old: there is such a word, or before[words])
+    const int movers = H - kept_below, total = movers + a.recent;
+    // the i-th place that is free below H, and the i-th row from H on that stays
+    auto hole = [&](int i) { return nth_bit(bits, before, 0, words, i, true); };
+    auto mover = [&](int i) { return nth_bit(bits, before, 0, words, kept_below + i, false); };
+    if (slice == 0) {
+        for (int r = tid; r < H; r += kEvThreads)
+            if (bits[r / 32] >> (r % 32) & 1) out[r] = w[r];
+        for (int i = tid; i < movers; i += kEvThreads) out[hole(i)] = w[mover(i)];
+        for (int i = tid; i < a.recent; i += kEvThreads) out[H + i] = w[old + i];
+    }
+    // ---- the rows: what comes from behind first (its sources lie from H on, its targets below), then the recent ones, a batch read before it is
+    // written: a target lies before its source, so no batch writes over what a later one reads
+    const int per_row = a.kv.hd / 8, slices = (per_row + a.cols - 1) / a.cols, col0 = slice % slices * a.cols, cols = min(a.cols, per_row - col0);
+    uint4 *base = (slice >= slices ? a.vc : a.kc) + layer * (a.kv.layer_stride / 8) + (long long)head * a.kv.page * per_row + col0;
+    const int step = kEvThreads / cols, row = tid / cols, col = tid - row * cols;  // rows that a turn of the threads covers
     for (int i0 = 0; i0 < total;) {
         const int m = min(kMoveRows, (i0 < movers ? movers : total) - i0);
+        __syncthreads();
         if (tid < m) {
             const int i = i0 + tid;
-            const long long f = a.kv.row_of(seq, i < movers ? from[i] : old + i - movers), t = a.kv.row_of(seq, i < movers ? to[i] : H + i - movers);
+            const long long f = a.kv.row_of(seq, i < movers ? mover(i) : old + i - movers), t = a.kv.row_of(seq, i < movers ? hole(i) : H + i - movers);
             src[tid] = t < 0 || f < 0 ? -1 : f / 8;
             dst[tid] = t / 8;
         }
         __syncthreads();
-        const int pieces = m * words;
-        for (int j0 = 0; j0 < kMoveRows * 32; j0 += kEvThreads * 8) {
-            if (j0 >= pieces) break;
-            uint4 x[8];
+        for (int r0 = 0; r0 < m; r0 += step * kMoveAhead) {
+            uint4 x[kMoveAhead];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int at = j0 + j * kEvThreads + tid;
-                if (at < pieces && src[at / words] >= 0) x[j] = base[src[at / words] + at % words];
+            for (int j = 0; j < kMoveAhead; j++) {
+                const int r = r0 + j * step + row;
+                if (row < step && r < m && src[r] >= 0) x[j] = base[src[r] + col];
             }
-            __syncthreads();
+            if (i0 >= movers) __syncthreads();
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int at = j0 + j * kEvThreads + tid;
-                if (at < pieces && src[at / words] >= 0) base[dst[at / words] + at % words] = x[j];
+            for (int j = 0; j < kMoveAhead; j++) {
+                const int r = r0 + j * step + row;
+                if (row < step && r < m && src[r] >= 0) base[dst[r] + col] = x[j];
             }
         }
-        __syncthreads();
         i0 += m;
     }
-}
-
-struct EvictPlan {
-    long long problems;
-    int most;
-    size_t bytes;
-};
-EvictPlan evict_plan(const PagedView &v, int budget, int recent) {
-    EvictPlan a;
-    a.problems = (long long)v.layers * v.nseq * v.nkv;
-    a.most = (int)std::min<long long>(budget - recent, std::max(0, v.rows - budget));  // a mover leaves a place behind H, and every row from H on that stays has one before it
-    a.bytes = (size_t)a.problems * 4 + (size_t)a.problems * 2 * a.most * 4;
-    return a;
 }
 
 int evict_check(int budget, int recent) {
@@ -190,22 +205,14 @@ int evict_check(int budget, int recent) {
     return IM_OK;
 }
 
+constexpr int kEvRows = 1 << 19;  // bits and counts of so many rows fit an SM's shared memory
+
 }  // namespace
 }  // namespace im
 
-IM_EXPORT size_t im_cuda_paged_evict_scratch_bytes(const im_device *dev, const im_paged_kv *kv, int budget, int recent) {
-    try {
-        im::PagedView v;
-        if (!dev || im::paged_view(kv, -1, &v) != IM_OK || im::evict_check(budget, recent) != IM_OK) return 0;
-        return im::evict_plan(v, budget, recent).bytes;
-    } catch (...) {
-        return 0;
-    }
-}
-
 IM_EXPORT int im_cuda_paged_evict(im_device *dev, const im_paged_kv *kv, const float *weights_dev, int64_t layer_stride, int64_t seq_stride, int64_t head_stride, int budget,
                                   int recent, float *weights_out_dev, int64_t out_layer_stride, int64_t out_seq_stride, int64_t out_head_stride, int *seq_len_out_dev,
-                                  void *scratch_dev, size_t scratch_bytes, void *stream) {
+                                  void *stream) {
     IM_GUARD_BEGIN
     using namespace im;
     Evict a;
@@ -214,6 +221,7 @@ IM_EXPORT int im_cuda_paged_evict(im_device *dev, const im_paged_kv *kv, const f
     if (rc == IM_OK) rc = evict_check(budget, recent);
     if (rc != IM_OK) return rc;
     IM_REQUIRE(v.nseq == 0 || (weights_dev && weights_out_dev && seq_len_out_dev), "bad argument");
+    IM_REQUIRE(v.rows <= kEvRows, "eviction takes page tables of up to %d rows (got %d)", kEvRows, v.rows);
     const long long most = 1ll << 40;
     const auto apart = [&](int64_t layer, int64_t seq, int64_t head) {
         return head >= v.rows && head <= most / v.nkv && seq <= most && layer <= most && (v.nseq <= 1 || seq >= (v.nkv - 1) * head + v.rows) &&
@@ -221,8 +229,8 @@ IM_EXPORT int im_cuda_paged_evict(im_device *dev, const im_paged_kv *kv, const f
     };
     IM_REQUIRE(apart(layer_stride, seq_stride, head_stride) && apart(out_layer_stride, out_seq_stride, out_head_stride),
                "sums have a row for each of the page table's %d, those of different layers, sequences and heads apart", v.rows);
-    const EvictPlan plan = evict_plan(v, budget, recent);
-    IM_REQUIRE(plan.problems <= INT_MAX, "too many layers, sequences and heads");
+    const long long problems = (long long)v.layers * v.nseq * v.nkv;
+    IM_REQUIRE(problems <= INT_MAX, "too many layers, sequences and heads");
     if (v.nseq > 0) {
         IM_REQUIRE(reinterpret_cast<uintptr_t>(weights_dev) % 4 == 0 && reinterpret_cast<uintptr_t>(weights_out_dev) % 4 == 0, "the sums are not 4-byte aligned");
         const auto span = [&](int64_t layer, int64_t seq, int64_t head) { return 4 * ((v.layers - 1) * layer + (v.nseq - 1) * seq + (v.nkv - 1) * head + v.rows); };
@@ -237,8 +245,8 @@ IM_EXPORT int im_cuda_paged_evict(im_device *dev, const im_paged_kv *kv, const f
     rc = paged_device(dev);
     if (rc != IM_OK) return rc;
     if (v.nseq == 0) return IM_OK;
-    IM_REQUIRE(scratch_dev && aligned16(scratch_dev) && scratch_bytes >= plan.bytes, "eviction needs %zu bytes of 16-byte aligned scratch (got %zu)", plan.bytes,
-               scratch_dev ? scratch_bytes : (size_t)0);
+    a.kc = static_cast<uint4 *>(kv->k_dev);
+    a.vc = static_cast<uint4 *>(kv->v_dev);
     a.w = weights_dev;
     a.w_out = weights_out_dev;
     a.w_layer = layer_stride; a.w_seq = seq_stride; a.w_head = head_stride;
@@ -246,12 +254,18 @@ IM_EXPORT int im_cuda_paged_evict(im_device *dev, const im_paged_kv *kv, const f
     a.budget = budget;
     a.recent = recent;
     a.len_out = seq_len_out_dev;
-    a.count = static_cast<int *>(scratch_dev);
-    a.moves = a.count + plan.problems;
-    a.most = plan.most;
-    const cudaStream_t st = as_stream(stream);
-    IM_CUDA_CHECK(launch_k(paged_evict_select_kernel, dim3((unsigned)plan.problems), dim3(kEvThreads), 0, st, a));
-    IM_CUDA_CHECK(launch_k(paged_evict_move_kernel, dim3((unsigned)plan.problems, 2), dim3(kEvThreads), 0, st, a, static_cast<uint4 *>(kv->k_dev), static_cast<uint4 *>(kv->v_dev)));
+    // Blocks for about four on each SM, a block all columns of keys or values where there are many (layer, sequence, head), 32 bytes of a row at least where there are few
+    const int per_row = v.hd / 8;
+    a.cols = per_row;
+    while (a.cols > 2 && 2 * problems * ((per_row + a.cols - 1) / a.cols) < 3ll * dev->sm_count) a.cols = (a.cols + 1) / 2;
+    const int slices = (per_row + a.cols - 1) / a.cols;
+    a.bit_words = (v.rows + 31) / 32;
+    const size_t smem = (size_t)(2 * a.bit_words + 1) * 4;
+    if (smem > 32768) {
+        static DeviceOnce once;
+        if (once.first(dev->ordinal)) IM_CUDA_CHECK(cudaFuncSetAttribute(paged_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * (kEvRows / 32) + 1) * 4));
+    }
+    IM_CUDA_CHECK(launch_k(paged_evict_kernel, dim3((unsigned)problems, (unsigned)(2 * slices)), dim3(kEvThreads), smem, as_stream(stream), a));
     return IM_OK;
     IM_GUARD_END
 }

@@ -659,19 +659,6 @@ def paged_attention_weights(kv: PagedKV, layer: int, q, token_start, max_new: in
     return out
 
 
-def _evict_bytes(kv: PagedKV, budget: int, recent: int) -> int:
-    key = ("evict", budget, recent)
-    nbytes = kv.scratch_bytes.get(key)
-    if nbytes is None:
-        nbytes = kv.scratch_bytes[key] = int(lib().im_cuda_paged_evict_scratch_bytes(kv.dev.handle, kv.ref, budget, recent))
-    return nbytes
-
-
-def paged_evict_scratch(kv: PagedKV, budget: int, recent: int) -> torch.Tensor:
-    """Scratch for paged_evict calls of this cache; calls that may overlap need one each."""
-    return torch.empty(max(_evict_bytes(kv, budget, recent), 16), dtype=torch.uint8, device=kv.device)
-
-
 def _sums_of(x, kv: PagedKV):
     """Strides of sums f32 [layers, sequences, kv_heads, rows of the page table]."""
     rows = kv.page_table.shape[1] * kv.struct.page_size
@@ -681,7 +668,7 @@ def _sums_of(x, kv: PagedKV):
     return sl, ss, sh if kv.kv_heads > 1 else rows
 
 
-def paged_evict(kv: PagedKV, weights, budget: int, recent: int, weights_out=None, lengths_out=None, scratch=None):
+def paged_evict(kv: PagedKV, weights, budget: int, recent: int, weights_out=None, lengths_out=None):
     """Sequences of more than `budget` rows keep the last `recent` and, of the others, those with the largest weights (f32 [layers, sequences, kv_heads, rows of the
     page table], as paged_attention_weights adds them up; ties: the lowest row), for every layer and KV head on its own. Rows that stay are moved into the first `budget`
     places, their order is another then (positions of the next tokens: paged_append). Returns the new lengths (kv.point_at) and weights_out, the
@@ -691,9 +678,8 @@ def paged_evict(kv: PagedKV, weights, budget: int, recent: int, weights_out=None
         weights_out = torch.empty_like(weights, memory_format=torch.contiguous_format)
     if lengths_out is None:
         lengths_out = torch.empty_like(kv.lengths)
-    scratch, at, nbytes = _scratch_of(scratch, _evict_bytes(kv, budget, recent) if scratch is None else 0, kv)
     _launch(on, lib().im_cuda_paged_evict, kv.dev.handle, kv.ref, weights.data_ptr(), *_sums_of(weights, kv), budget, recent, weights_out.data_ptr(), *_sums_of(weights_out, kv),
-            _ints(lengths_out, on, kv.num_seqs), at, nbytes)
+            _ints(lengths_out, on, kv.num_seqs))
     return lengths_out, weights_out
 
 

@@ -278,8 +278,8 @@ def test_a_captured_eviction_follows_lengths_and_sums(dev):
     c = Cache(dev, rng, [300, 200], [300, 200], layers=2)
     lengths, w = _ints(c.lengths), torch.zeros((2, 2, 2, c.table.shape[1] * 16), device="cuda")
     c.kv.point_at(_ints(c.table), lengths)
-    w_out, len_out, scratch = torch.zeros_like(w), torch.zeros_like(lengths), ops.paged_evict_scratch(c.kv, 100, 20)
-    call = lambda: ops.paged_evict(c.kv, w, 100, 20, weights_out=w_out, lengths_out=len_out, scratch=scratch)  # noqa: E731
+    w_out, len_out = torch.zeros_like(w), torch.zeros_like(lengths)
+    call = lambda: ops.paged_evict(c.kv, w, 100, 20, weights_out=w_out, lengths_out=len_out)  # noqa: E731
     call()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
