@@ -5,8 +5,8 @@
 // behind them. That moves the fewest rows: closing up in order would move nearly all of them for one that leaves, and attention does not
 // ask for their order (keys are rotated already). What order means something for, the recent rows, is kept.
 //
-// One launch, a block per (layer, sequence, head) and slice of the columns of keys or values. Every block finds the H-th largest sum for itself (the sums are 4 bytes beside 4 * head_dim
-// of a row): by digits of 8 bits from the top, each a histogram in shared memory; then one bit a row says whether it stays, and the i-th free place below H and the i-th row that
+// One launch, a block per (layer, sequence, head) and slice of the columns of keys and values. Every block finds the H-th largest sum for itself (the sums are 4 bytes beside 4 * head_dim
+// of a row): by digits of 11 bits from the top, each a histogram in shared memory, the later ones of those keys alone that share the first; then one bit a row says whether it stays, and the i-th free place below H and the i-th row that
 // comes from behind are found by their ranks among the bits. No lists, no scratch, nothing between blocks. While some blocks of an SM choose, others move: HBM bounds the whole.
 #include <limits.h>
 
@@ -25,7 +25,7 @@ struct Evict {
     long long w_layer, w_seq, w_head, o_layer, o_seq, o_head;
     int budget, recent;
     int *len_out;
-    int cols;       // 16-byte columns of a slice
+    int cols;       // 16-byte columns of a slice, of a row's keys and values one after the other
     int bit_words;  // of 32 rows
 };
 
@@ -37,6 +37,7 @@ __device__ __forceinline__ uint32_t sum_key(float w) {
 }
 
 constexpr int kEvThreads = 256, kEvWarps = kEvThreads / 32;
+constexpr int kListed = 1024;                   // keys that are picked out
 constexpr int kMoveRows = 128, kMoveAhead = 8;  // rows of a batch; 16-byte pieces that a thread holds
 
 // Sums of v over the threads before this one, the block's total in `total`.
@@ -82,15 +83,16 @@ __device__ __forceinline__ int nth_bit(const uint32_t *bits, const int *before, 
 
 __global__ void __launch_bounds__(kEvThreads, 4) paged_evict_kernel(const __grid_constant__ Evict a) {
     extern __shared__ __align__(16) uint32_t ev_smem[];
-    __shared__ int bins[kEvWarps][256];
+    __shared__ __align__(16) int bins[2048];
+    __shared__ uint32_t list[kListed];
     __shared__ int of_warp[kEvWarps];
-    __shared__ int found[2];
+    __shared__ int found[3];
     uint32_t *bits = ev_smem;                                              // [bit_words]: rows that stay
     int *before = reinterpret_cast<int *>(bits + a.bit_words);             // [bit_words + 1]: of them in the words before
-    long long *src = reinterpret_cast<long long *>(&bins[0][0]), *dst = src + kMoveRows;  // (the histograms are done then)
+    long long *src = reinterpret_cast<long long *>(bins), *dst = src + 2 * kMoveRows;  // (the histograms are done then)
     pdl_trigger();
     pdl_wait();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, problem = blockIdx.x, slice = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 31, problem = blockIdx.x, slice = blockIdx.y;
     const int head = problem % a.kv.nkv, seq = problem / a.kv.nkv % a.kv.nseq, layer = problem / a.kv.nkv / a.kv.nseq;
     const int n = a.kv.length(seq), H = a.budget - a.recent, old = n - a.recent;
     const float *w = a.w + layer * a.w_layer + seq * a.w_seq + head * a.w_head;
@@ -101,51 +103,77 @@ __global__ void __launch_bounds__(kEvThreads, 4) paged_evict_kernel(const __grid
             for (int i = tid; i < n; i += kEvThreads) out[i] = w[i];
         return;
     }
-    // ---- the H-th largest key, digit by digit; `above` of the others are larger
+    // ---- the H-th largest key, digit by digit from the top; `above` of the others are larger, `equals` are the same. Once few enough share the digits
+    // found they are picked out, and the next digits are theirs.
     uint32_t top = 0, mask = 0;
-    int above = 0;
-    for (int shift = 24; shift >= 0 && H > 0; shift -= 8) {
-        for (int i = tid; i < kEvWarps * 256; i += kEvThreads) (&bins[0][0])[i] = 0;
-        __syncthreads();
+    int above = 0, equals = old, listed = -1;
+    for (int digit = 0; digit < 3 && H > 0; digit++) {
+        const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, count = digit < 2 ? 2048 : 1024;
+        for (int i = tid; i < count; i += kEvThreads) bins[i] = 0;
+        if (listed < 0 && digit > 0 && equals <= kListed) {
+            if (tid == 0) found[2] = 0;
+            __syncthreads();
 #pragma unroll 4
-        for (int i = tid; i < old; i += kEvThreads) {
-            const uint32_t k = sum_key(__ldg(w + i));
-            if ((k & mask) == top) atomicAdd(&bins[warp][k >> shift & 255], 1);
+            for (int i = tid; i < old; i += kEvThreads) {
+                const uint32_t k = sum_key(__ldg(w + i));
+                if ((k & mask) == top) list[atomicAdd(&found[2], 1)] = k;
+            }
+            listed = equals;
         }
         __syncthreads();
-        // thread t has digit 255 - t: counts from the top
-        int mine = 0, total;
-#pragma unroll
-        for (int i = 0; i < kEvWarps; i++) mine += bins[i][255 - tid];
-        const int larger = above + block_before(mine, of_warp, total);
-        if (larger < H && larger + mine >= H) found[0] = 255 - tid, found[1] = larger;
+        if (listed >= 0) {
+            for (int i = tid; i < listed; i += kEvThreads)
+                if ((list[i] & mask) == top) atomicAdd(&bins[list[i] >> shift & (count - 1)], 1);
+        } else {
+#pragma unroll 4
+            for (int i = tid; i < old; i += kEvThreads) {
+                const uint32_t k = sum_key(__ldg(w + i));
+                if ((k & mask) == top) atomicAdd(&bins[k >> shift & (count - 1)], 1);
+            }
+        }
+        __syncthreads();
+        // a thread has `each` bins, the first one the highest
+        const int each = count / kEvThreads;
+        int mine = 0, sum;
+        for (int i = 0; i < each; i++) mine += bins[count - 1 - tid * each - i];
+        int larger = above + block_before(mine, of_warp, sum);
+        if (larger < H && larger + mine >= H)
+            for (int i = 0; i < each; i++) {
+                const int bin = count - 1 - tid * each - i, n_bin = bins[bin];
+                if (larger + n_bin >= H) {
+                    found[0] = bin, found[1] = larger, found[2] = n_bin;
+                    break;
+                }
+                larger += n_bin;
+            }
         __syncthreads();
         top |= (uint32_t)found[0] << shift;
-        mask |= 255u << shift;
+        mask |= (uint32_t)(count - 1) << shift;
         above = found[1];
+        equals = found[2];
         __syncthreads();
     }
     // ---- which rows stay: larger keys, and of equal ones the lowest rows
-    int equal = H - above, equals = 0, stay = 0;
-    const int words = (old + 31) / 32;
-    for (int r0 = 0; r0 < words * 32; r0 += kEvThreads) {
-        const int r = r0 + tid;
-        const uint32_t k = r < old && H > 0 ? sum_key(__ldg(w + r)) : 0;
-        const bool more = r < old && H > 0 && k > top, same = r < old && H > 0 && k == top;
-        const unsigned these = __ballot_sync(0xffffffffu, same);
-        // (ranks among equals matter where some of them leave: their count over the block's warps)
-        __syncthreads();
-        if (lane == 0) of_warp[warp] = __popc(these);
-        __syncthreads();
-        int rank = equals, all = 0;
-#pragma unroll
-        for (int i = 0; i < kEvWarps; i++) {
-            if (i < warp) rank += of_warp[i];
-            all += of_warp[i];
+    const int equal = H - above, words = (old + 31) / 32;
+    int stay = 0;
+    if (H == 0 || equals == equal) {
+        for (int r0 = 0; r0 < words * 32; r0 += kEvThreads) {
+            const int r = r0 + tid;
+            const unsigned word = __ballot_sync(0xffffffffu, r < old && H > 0 && sum_key(__ldg(w + r)) >= top);
+            if (lane == 0 && r / 32 < words) bits[r / 32] = word;
         }
-        equals += all;
-        const unsigned word = __ballot_sync(0xffffffffu, more || (same && rank + __popc(these & ((1u << lane) - 1)) < equal));
-        if (lane == 0 && r / 32 < words) bits[r / 32] = word;
+    } else {
+        int passed = 0;  // equal ones so far
+        for (int r0 = 0; r0 < words * 32; r0 += kEvThreads) {
+            const int r = r0 + tid;
+            const uint32_t k = r < old ? sum_key(__ldg(w + r)) : 0;
+            const bool same = r < old && k == top;
+            int all;
+            const int rank = passed + block_before(same, of_warp, all);
+            passed += all;
+            const unsigned word = __ballot_sync(0xffffffffu, (r < old && k > top) || (same && rank < equal));
+            if (lane == 0 && r / 32 < words) bits[r / 32] = word;
+        }
     }
     __syncthreads();
     for (int w0 = 0; w0 < words; w0 += kEvThreads) {
@@ -168,35 +196,41 @@ __global__ void __launch_bounds__(kEvThreads, 4) paged_evict_kernel(const __grid
         for (int i = tid; i < a.recent; i += kEvThreads) out[H + i] = w[old + i];
     }
     // ---- the rows: what comes from behind first (its sources lie from H on, its targets below), then the recent ones, a batch read before it is
-    // written: a target lies before its source, so no batch writes over what a later one reads
-    const int per_row = a.kv.hd / 8, slices = (per_row + a.cols - 1) / a.cols, col0 = slice % slices * a.cols, cols = min(a.cols, per_row - col0);
-    uint4 *base = (slice >= slices ? a.vc : a.kc) + layer * (a.kv.layer_stride / 8) + (long long)head * a.kv.page * per_row + col0;
-    const int step = kEvThreads / cols, row = tid / cols, col = tid - row * cols;  // rows that a turn of the threads covers
-    for (int i0 = 0; i0 < total;) {
-        const int m = min(kMoveRows, (i0 < movers ? movers : total) - i0);
-        __syncthreads();
-        if (tid < m) {
-            const int i = i0 + tid;
-            const long long f = a.kv.row_of(seq, i < movers ? mover(i) : old + i - movers), t = a.kv.row_of(seq, i < movers ? hole(i) : H + i - movers);
-            src[tid] = t < 0 || f < 0 ? -1 : f / 8;
-            dst[tid] = t / 8;
-        }
-        __syncthreads();
+    // written: a target lies before its source, so no batch writes over what a later one reads. The places of the next batch are looked up while one is on its way.
+    const int per_row = a.kv.hd / 8, col0 = slice * a.cols, cols = min(a.cols, 2 * per_row - col0);
+    const int step = kEvThreads / cols, row = tid / cols, col = col0 + tid - row * cols;  // rows that a turn of the threads covers
+    uint4 *base = (col >= per_row ? a.vc + col - per_row : a.kc + col) + layer * (a.kv.layer_stride / 8) + (long long)head * a.kv.page * per_row;
+    auto batch = [&](int i0) { return min(kMoveRows, (i0 < movers ? movers : total) - i0); };
+    auto places = [&](int i0, int buf) {
+        const int i = i0 + tid;
+        if (tid >= batch(i0)) return;
+        const long long f = a.kv.row_of(seq, i < movers ? mover(i) : old + i - movers), t = a.kv.row_of(seq, i < movers ? hole(i) : H + i - movers);
+        src[buf * kMoveRows + tid] = t < 0 || f < 0 ? -1 : f / 8;
+        dst[buf * kMoveRows + tid] = t / 8;
+    };
+    __syncthreads();
+    if (total > 0) places(0, 0);
+    __syncthreads();
+    for (int i0 = 0, buf = 0; i0 < total; buf ^= 1) {
+        const int m = batch(i0);
+        const long long *from = src + buf * kMoveRows, *to = dst + buf * kMoveRows;
         for (int r0 = 0; r0 < m; r0 += step * kMoveAhead) {
             uint4 x[kMoveAhead];
 #pragma unroll
             for (int j = 0; j < kMoveAhead; j++) {
                 const int r = r0 + j * step + row;
-                if (row < step && r < m && src[r] >= 0) x[j] = base[src[r] + col];
+                if (row < step && r < m && from[r] >= 0) x[j] = base[from[r]];
             }
+            if (r0 == 0 && i0 + m < total) places(i0 + m, buf ^ 1);
             if (i0 >= movers) __syncthreads();
 #pragma unroll
             for (int j = 0; j < kMoveAhead; j++) {
                 const int r = r0 + j * step + row;
-                if (row < step && r < m && src[r] >= 0) base[dst[r] + col] = x[j];
+                if (row < step && r < m && from[r] >= 0) base[to[r]] = x[j];
             }
         }
         i0 += m;
+        __syncthreads();
     }
 }
 
@@ -254,18 +288,18 @@ IM_EXPORT int im_cuda_paged_evict(im_device *dev, const im_paged_kv *kv, const f
     a.budget = budget;
     a.recent = recent;
     a.len_out = seq_len_out_dev;
-    // Blocks for about four on each SM, a block all columns of keys or values where there are many (layer, sequence, head), 32 bytes of a row at least where there are few
+    // A block all of a row where there are many (layer, sequence, head), down to 32 bytes of it where there are few
     const int per_row = v.hd / 8;
-    a.cols = per_row;
-    while (a.cols > 2 && 2 * problems * ((per_row + a.cols - 1) / a.cols) < 3ll * dev->sm_count) a.cols = (a.cols + 1) / 2;
-    const int slices = (per_row + a.cols - 1) / a.cols;
+    a.cols = 2 * per_row;
+    while (a.cols > 2 && problems * ((2 * per_row + a.cols - 1) / a.cols) < 3ll * dev->sm_count) a.cols = (a.cols + 1) / 2;
+    const int slices = (2 * per_row + a.cols - 1) / a.cols;
     a.bit_words = (v.rows + 31) / 32;
     const size_t smem = (size_t)(2 * a.bit_words + 1) * 4;
     if (smem > 32768) {
         static DeviceOnce once;
         if (once.first(dev->ordinal)) IM_CUDA_CHECK(cudaFuncSetAttribute(paged_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * (kEvRows / 32) + 1) * 4));
     }
-    IM_CUDA_CHECK(launch_k(paged_evict_kernel, dim3((unsigned)problems, (unsigned)(2 * slices)), dim3(kEvThreads), smem, as_stream(stream), a));
+    IM_CUDA_CHECK(launch_k(paged_evict_kernel, dim3((unsigned)problems, (unsigned)slices), dim3(kEvThreads), smem, as_stream(stream), a));
     return IM_OK;
     IM_GUARD_END
 }
