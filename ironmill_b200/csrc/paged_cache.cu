@@ -210,19 +210,66 @@ __global__ void __launch_bounds__(kAppendThreads, FORM == 3 ? 2 : 5) paged_appen
 //   of position[axis of i]; f32 from the load to the one rounding at the end.
 // The same blocks and lookups as above, but a lane owns both columns of its pairs (four of them: two words of 8 bytes, which lie side by side where
 // neighbours belong together and half of rotary_dim apart where the halves do), so that rotation exchanges nothing between lanes, and every cosine and sine
-// is loaded once instead of by both lanes of a pair. A head's sum of squares is the only exchange: log2(lanes) shuffles.
+// is loaded once instead of by both lanes of a pair. What bounds it is instructions: a token's weights, cosines and sines are multiplied once, a head
+// is then two products and a factor an element, two elements at a time; its sum of squares is the only exchange, log2(lanes) shuffles.
 constexpr int kAxes = 4;
 struct AppendMore {
     const void *qn, *kn;  // weights or NULL
-    int norm_f32, axes;
+    int norm_f32, axes, neighbours;
     float eps, inv_dim;
     uint32_t axis[8];     // two bits a pair: 128 of them
 };
 
-// Four norm weights from column d on.
+// Where a token goes: the offset of its row in the cache (-1: it has none there) and the rows of the tables; false: it is left alone.
+__device__ __forceinline__ bool append_place(const Append &a, const AppendMore &m, int token, long long &at, int (&pos)[kAxes]) {
+    const int lo = __ldg(a.start), hi = __ldg(a.start + a.kv.nseq);
+    if (token < lo || token >= hi) return false;
+    const int seq = paged_seq_of(a.start, a.kv.nseq, token), place = token - __ldg(a.start + seq);
+    const long long r = (long long)a.kv.length(seq) + place;
+    if (place < 0 || r > INT_MAX) return false;
+    bool there = true;
+    if (a.rot > 0) {
+#pragma unroll
+        for (int k = 0; k < kAxes; k++) {
+            pos[k] = k >= m.axes ? 0 : a.pos ? __ldg(a.pos + (long long)k * gridDim.x + token) : (int)r;
+            there = there && (unsigned)pos[k] < (unsigned)a.max_pos;
+        }
+    }
+    at = a.kv.row_of(seq, (int)r);
+    return there;
+}
+// Cosines and sines of pairs e0 .. e0 + 3 (e0 a multiple of 4): from the rows of the axes that they have.
+template <bool F32>
+__device__ __forceinline__ void append_angles(const Append &a, const AppendMore &m, const int (&pos)[kAxes], int e0, float *cs, float *sn) {
+    const int half = a.rot / 2;
+    const uint32_t axes = m.axis[e0 / 16 & 7] >> (2 * (e0 & 15));  // (sixteen pairs a word)
+#pragma unroll
+    for (int j = 0; j < 4; j++) cs[j] = 1.0f, sn[j] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kAxes; k++) {
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < 4; j++) any = any || (e0 + j < half && (axes >> (2 * j) & 3) == k);
+        if (!any) continue;
+        float s[4], t[4];
+        angles4<F32>(a.cosc, (long long)pos[k] * (a.kv.hd / 2) + e0, s);
+        angles4<F32>(a.sinc, (long long)pos[k] * (a.kv.hd / 2) + e0, t);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (e0 + j < half && (axes >> (2 * j) & 3) == k) cs[j] = s[j], sn[j] = t[j];
+    }
+}
+template <bool BF16>
+__device__ __forceinline__ float norm_weight(const void *w, int f32, int d) {
+    return !w ? 1.0f : f32 ? __ldg(static_cast<const float *>(w) + d) : one16<BF16>(static_cast<const uint16_t *>(w) + d);
+}
+// Four norm weights from column d on, a multiple of 4.
 template <bool BF16>
 __device__ __forceinline__ void weights4(const void *w, int f32, int d, float *out) {
-    if (f32) {
+    if (!w) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) out[j] = 1.0f;
+    } else if (f32) {
         *reinterpret_cast<float4 *>(out) = __ldg(reinterpret_cast<const float4 *>(static_cast<const float *>(w) + d));
     } else {
         const uint2 u = __ldg(reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(w) + d));
@@ -231,145 +278,156 @@ __device__ __forceinline__ void weights4(const void *w, int f32, int d, float *o
     }
 }
 
-// FORM: 0 halves, rotary_dim a multiple of 8; 1 neighbours (and rotary_dim 0); 2 halves of any even size, column by column.
-constexpr int kNormedHeads = 3;
-template <bool BF16, int FORM, bool F32>
-__global__ void __launch_bounds__(kAppendThreads, 3) paged_append_normed_kernel(const __grid_constant__ Append a, const __grid_constant__ AppendMore m, int lanes) {
+// rotary_dim a multiple of 8: the four pairs of a lane are turned or none is.
+constexpr int kNormedHeads = 4;
+template <bool BF16, bool NB, bool F32>
+__global__ void __launch_bounds__(kAppendThreads, 4) paged_append_normed_kernel(const __grid_constant__ Append a, const __grid_constant__ AppendMore m, int lanes) {
     pdl_trigger();
     pdl_wait();
     const int token = blockIdx.x, tid = threadIdx.x;
     const int c = tid & (lanes - 1), first = tid / lanes, per = blockDim.x / lanes;
-    const int hd = a.kv.hd, heads = a.nh + 2 * a.kv.nkv, half = a.rot / 2;
-    const bool mine = 8 * c < hd;
-    // this lane's pairs 4 c .. 4 c + 3; the columns behind the rotated ones are pairs of neighbours that are not turned
-    const int e0 = 4 * c, colA = FORM == 0 && e0 < half ? e0 : 2 * e0, colB = FORM == 0 && e0 < half ? half + e0 : 2 * e0 + 4;
-    auto column = [&](int i) {  // FORM 2: of word i / 4, place i % 4
-        const int e = e0 + i % 4;
-        return e < half ? e + (i / 4) * half : 2 * e + i / 4;
-    };
-    auto source = [&](int h) {
-        return h < a.nh ? a.q + token * a.qs + (long long)h * hd
-                        : h < a.nh + a.kv.nkv ? a.k + token * a.ks + (long long)(h - a.nh) * hd : a.v + token * a.vs + (long long)(h - a.nh - a.kv.nkv) * hd;
-    };
-    bool placed = false;
-    long long at = -1;
-    float cs[4], sn[4], wq[8], wk[8];
-#pragma unroll 1
-    for (int h0 = first; h0 - first < heads; h0 += per * kNormedHeads) {  // the same count for every lane of a warp
-        uint2 x[kNormedHeads][2];
+    const int hd = a.kv.hd, half = a.rot / 2, e0 = 4 * c;
+    const bool mine = 8 * c < hd, turned = e0 < half;
+    const int colA = !NB && turned ? e0 : 2 * e0, colB = !NB && turned ? half + e0 : 2 * e0 + 4;
+    uint2 x[kNormedHeads][2];
+    auto load = [&](const uint16_t *src, int h0, int heads) {
 #pragma unroll
         for (int i = 0; i < kNormedHeads; i++) {
             const int h = h0 + i * per;
             x[i][0] = x[i][1] = make_uint2(0, 0);
             if (mine && h < heads) {
-                const uint16_t *src = source(h);
-                if (FORM < 2) {
-                    x[i][0] = *reinterpret_cast<const uint2 *>(src + colA);
-                    x[i][1] = *reinterpret_cast<const uint2 *>(src + colB);
-                } else {
-                    uint16_t v[8];
-#pragma unroll
-                    for (int j = 0; j < 8; j++) v[j] = src[column(j)];
-#pragma unroll
-                    for (int j = 0; j < 2; j++) x[i][j] = make_uint2(v[4 * j] | (uint32_t)v[4 * j + 1] << 16, v[4 * j + 2] | (uint32_t)v[4 * j + 3] << 16);
-                }
+                x[i][0] = *reinterpret_cast<const uint2 *>(src + h * hd + colA);
+                x[i][1] = *reinterpret_cast<const uint2 *>(src + h * hd + colB);
             }
         }
-        if (!placed) {
-            placed = true;
-            const int lo = __ldg(a.start), hi = __ldg(a.start + a.kv.nseq);
-            if (token < lo || token >= hi) return;
-            const int seq = paged_seq_of(a.start, a.kv.nseq, token), place = token - __ldg(a.start + seq);
-            const long long r = (long long)a.kv.length(seq) + place;
-            if (place < 0 || r > INT_MAX) return;
-            if (a.rot > 0) {
-                int p[kAxes];
-                bool there = true;
+    };
+    const bool queries = a.nh > 0;
+    const uint16_t *src = queries ? a.q + token * a.qs : a.k + token * a.ks;
+    load(src, first, queries ? a.nh : a.kv.nkv);  // the first heads are requested before the lookups
+    long long at;
+    int pos[kAxes];
+    if (!append_place(a, m, token, at, pos)) return;
+    float cs[4], sn[4];
+    if (a.rot > 0 && mine) append_angles<F32>(a, m, pos, e0, cs, sn);
+    else
 #pragma unroll
-                for (int k = 0; k < kAxes; k++) {
-                    p[k] = k >= m.axes ? 0 : a.pos ? __ldg(a.pos + (long long)k * gridDim.x + token) : (int)r;
-                    there = there && (unsigned)p[k] < (unsigned)a.max_pos;
-                }
-                if (!there) return;
-                const uint32_t axes = m.axis[(c >> 2) & 7] >> (8 * (c & 3));  // (sixteen pairs a word)
-#pragma unroll
-                for (int j = 0; j < 4; j++) cs[j] = 1.0f, sn[j] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < kAxes; k++) {  // the rows of the axes that this lane's pairs have
-                    bool any = false;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) any = any || (e0 + j < half && (axes >> (2 * j) & 3) == k);
-                    if (!any) continue;
-                    float s[4], t[4];
-                    angles4<F32>(a.cosc, (long long)p[k] * (hd / 2) + e0, s);
-                    angles4<F32>(a.sinc, (long long)p[k] * (hd / 2) + e0, t);
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (e0 + j < half && (axes >> (2 * j) & 3) == k) cs[j] = s[j], sn[j] = t[j];
-                }
-            }
+        for (int j = 0; j < 4; j++) cs[j] = 1.0f, sn[j] = 0.0f;
+    // an element and its partner in the pair: y = (x C + partner S) r. Words A (0, 1) and B (2, 3) of two elements each; partners: the other word's, or (NB)
+    // the word's own, exchanged
+    auto turn = [&](const void *norm, const uint16_t *src, int heads, uint16_t *dst, long long dst_head, bool loaded) {
+        uint64_t C[4], S[4];
+        {
+            float wa[4], wb[4];
             if (mine) {
-                if (FORM < 2) {
-                    if (m.qn) weights4<BF16>(m.qn, m.norm_f32, colA, wq), weights4<BF16>(m.qn, m.norm_f32, colB, wq + 4);
-                    if (m.kn) weights4<BF16>(m.kn, m.norm_f32, colA, wk), weights4<BF16>(m.kn, m.norm_f32, colB, wk + 4);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const int d = column(j);
-                        if (m.qn) wq[j] = m.norm_f32 ? __ldg(static_cast<const float *>(m.qn) + d) : one16<BF16>(static_cast<const uint16_t *>(m.qn) + d);
-                        if (m.kn) wk[j] = m.norm_f32 ? __ldg(static_cast<const float *>(m.kn) + d) : one16<BF16>(static_cast<const uint16_t *>(m.kn) + d);
-                    }
-                }
+                weights4<BF16>(norm, m.norm_f32, colA, wa);
+                weights4<BF16>(norm, m.norm_f32, colB, wb);
             }
-            at = a.kv.row_of(seq, (int)r);
-        }
-#pragma unroll
-        for (int i = 0; i < kNormedHeads; i++) {
-            const int h = h0 + i * per;
-            const bool is_q = h < a.nh, is_v = h >= a.nh + a.kv.nkv;
-            float f[8];
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const float2 lo = unpack16<BF16>(x[i][j].x), hi = unpack16<BF16>(x[i][j].y);
-                f[4 * j] = lo.x; f[4 * j + 1] = lo.y; f[4 * j + 2] = hi.x; f[4 * j + 3] = hi.y;
-            }
-            if (m.qn || m.kn) {
-                float sum = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; j++) sum = fmaf(f[j], f[j], sum);
-                for (int o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                if (is_q ? m.qn != nullptr : !is_v && m.kn != nullptr) {
-                    const float r = rsqrtf(fmaf(sum, m.inv_dim, m.eps));
-#pragma unroll
-                    for (int j = 0; j < 8; j++) f[j] = f[j] * r * (is_q ? wq[j] : wk[j]);
-                }
-            }
-            if (!mine || h >= heads) continue;
-            uint2 y[2] = {x[i][0], x[i][1]};
-            if (!is_v) {
-                if (a.rot > 0) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        if (e0 + j >= half) continue;  // not turned
-                        float &p = f[FORM == 1 ? 2 * j : j], &q = f[FORM == 1 ? 2 * j + 1 : 4 + j];
-                        const float u = p * cs[j] - q * sn[j], v = q * cs[j] + p * sn[j];
-                        p = u;
-                        q = v;
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 2; j++) y[j] = make_uint2(pack16<BF16>(f[4 * j], f[4 * j + 1]), pack16<BF16>(f[4 * j + 2], f[4 * j + 3]));
-            }
-            if (!is_q && at < 0) continue;
-            uint16_t *to = is_q ? a.qo + token * a.qos + (long long)h * hd : (is_v ? a.vc : a.kc) + at + (long long)(is_v ? h - a.nh - a.kv.nkv : h - a.nh) * a.kv.page * hd;
-            if (FORM < 2) {
-                *reinterpret_cast<uint2 *>(to + colA) = y[0];
-                *reinterpret_cast<uint2 *>(to + colB) = y[1];
+            if (NB) {
+                C[0] = two(wa[0] * cs[0], wa[1] * cs[0]); C[1] = two(wa[2] * cs[1], wa[3] * cs[1]);
+                C[2] = two(wb[0] * cs[2], wb[1] * cs[2]); C[3] = two(wb[2] * cs[3], wb[3] * cs[3]);
+                S[0] = two(-wa[1] * sn[0], wa[0] * sn[0]); S[1] = two(-wa[3] * sn[1], wa[2] * sn[1]);
+                S[2] = two(-wb[1] * sn[2], wb[0] * sn[2]); S[3] = two(-wb[3] * sn[3], wb[2] * sn[3]);
             } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++) to[column(j)] = (uint16_t)((j & 2 ? y[j / 4].y : y[j / 4].x) >> (16 * (j & 1)));
+                C[0] = two(wa[0] * cs[0], wa[1] * cs[1]); C[1] = two(wa[2] * cs[2], wa[3] * cs[3]);
+                C[2] = two(wb[0] * cs[0], wb[1] * cs[1]); C[3] = two(wb[2] * cs[2], wb[3] * cs[3]);
+                S[0] = two(-wb[0] * sn[0], -wb[1] * sn[1]); S[1] = two(-wb[2] * sn[2], -wb[3] * sn[3]);
+                S[2] = two(wa[0] * sn[0], wa[1] * sn[1]); S[3] = two(wa[2] * sn[2], wa[3] * sn[3]);
             }
         }
+#pragma unroll 1
+        for (int h0 = first; h0 - first < heads; h0 += per * kNormedHeads) {  // the same count for every lane of a warp
+            if (!loaded) load(src, h0, heads);
+            loaded = false;
+#pragma unroll
+            for (int i = 0; i < kNormedHeads; i++) {
+                const int h = h0 + i * per;
+                if (h0 - first + i * per >= heads) break;  // (uniform)
+                uint64_t X[4], P[4];
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float2 lo = unpack16<BF16>(x[i][j].x), hi = unpack16<BF16>(x[i][j].y);
+                    X[2 * j] = two(lo.x, lo.y);
+                    X[2 * j + 1] = two(hi.x, hi.y);
+                    if (NB) P[2 * j] = two(lo.y, lo.x), P[2 * j + 1] = two(hi.y, hi.x);
+                }
+                if (!NB) P[0] = X[2], P[1] = X[3], P[2] = X[0], P[3] = X[1];
+                float r = 1.0f;
+                if (norm) {
+                    const float2 q = of_two(add_two(fma_two(X[0], X[0], mul_two(X[1], X[1])), fma_two(X[2], X[2], mul_two(X[3], X[3]))));
+                    float sum = q.x + q.y;
+                    for (int o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    r = rsqrtf(fmaf(sum, m.inv_dim, m.eps));
+                }
+                const uint64_t rr = two(r, r);
+                uint32_t y[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    uint64_t v = mul_two(X[j], C[j]);
+                    if (turned) v = fma_two(P[j], S[j], v);
+                    const float2 f = of_two(mul_two(v, rr));
+                    y[j] = pack16<BF16>(f.x, f.y);
+                }
+                if (mine && h < heads && dst) {
+                    *reinterpret_cast<uint2 *>(dst + h * dst_head + colA) = make_uint2(y[0], y[1]);
+                    *reinterpret_cast<uint2 *>(dst + h * dst_head + colB) = make_uint2(y[2], y[3]);
+                }
+            }
+        }
+    };
+    const long long head = (long long)a.kv.page * hd;
+    if (queries) turn(m.qn, src, a.nh, a.qo + token * a.qos, hd, true);
+    turn(m.kn, a.k + token * a.ks, a.kv.nkv, at < 0 ? nullptr : a.kc + at, head, !queries);
+    if (at < 0 || !mine) return;
+    const uint16_t *v = a.v + token * a.vs + 8 * c;
+    uint16_t *to = a.vc + at + 8 * c;
+#pragma unroll 2
+    for (int h = first; h < a.kv.nkv; h += per) *reinterpret_cast<uint4 *>(to + h * head) = *reinterpret_cast<const uint4 *>(v + h * hd);
+}
+
+// Any even rotary_dim, column by column: the columns behind the rotated ones are pairs of neighbours that are not turned.
+template <bool BF16, bool F32>
+__global__ void __launch_bounds__(kAppendThreads) paged_append_odd_kernel(const __grid_constant__ Append a, const __grid_constant__ AppendMore m, int lanes) {
+    pdl_trigger();
+    pdl_wait();
+    const int token = blockIdx.x, tid = threadIdx.x;
+    const int c = tid & (lanes - 1), first = tid / lanes, per = blockDim.x / lanes;
+    const int hd = a.kv.hd, heads = a.nh + 2 * a.kv.nkv, half = a.rot / 2, e0 = 4 * c;
+    const bool mine = 8 * c < hd;
+    auto column = [&](int i) {  // of pair e0 + i % 4, its first or (i >= 4) second one
+        const int e = e0 + i % 4;
+        return !m.neighbours && e < half ? e + (i / 4) * half : 2 * e + i / 4;
+    };
+    long long at;
+    int pos[kAxes];
+    if (!append_place(a, m, token, at, pos)) return;
+    float cs[4], sn[4];
+    if (a.rot > 0 && mine) append_angles<F32>(a, m, pos, e0, cs, sn);
+#pragma unroll 1
+    for (int h = first; h - first < heads; h += per) {  // the same count for every lane of a warp
+        const bool is_q = h < a.nh, is_v = h >= a.nh + a.kv.nkv, live = mine && h < heads;
+        const uint16_t *src = is_q ? a.q + token * a.qs + (long long)h * hd : !is_v ? a.k + token * a.ks + (long long)(h - a.nh) * hd : a.v + token * a.vs + (long long)(h - a.nh - a.kv.nkv) * hd;
+        uint16_t raw[8];
+        float f[8], sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            raw[j] = live ? src[column(j)] : (uint16_t)0;
+            f[j] = one16<BF16>(raw + j);
+            sum = fmaf(f[j], f[j], sum);
+        }
+        for (int o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (!live || (!is_q && at < 0)) continue;
+        uint16_t *to = is_q ? a.qo + token * a.qos + (long long)h * hd : (is_v ? a.vc : a.kc) + at + (long long)(is_v ? h - a.nh - a.kv.nkv : h - a.nh) * a.kv.page * hd;
+        const void *norm = is_q ? m.qn : m.kn;
+        const float r = norm ? rsqrtf(fmaf(sum, m.inv_dim, m.eps)) : 1.0f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float p = f[j] * r * norm_weight<BF16>(norm, m.norm_f32, column(j)), q = f[j + 4] * r * norm_weight<BF16>(norm, m.norm_f32, column(j + 4));
+            const bool turned = e0 + j < half;
+            const float y = turned ? p * cs[j] - q * sn[j] : p, z = turned ? q * cs[j] + p * sn[j] : q;
+            if (!is_v) raw[j] = (uint16_t)pack16<BF16>(y, 0.0f), raw[j + 4] = (uint16_t)pack16<BF16>(z, 0.0f);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) to[column(j)] = raw[j];
     }
 }
 
@@ -599,6 +657,7 @@ IM_EXPORT int im_cuda_paged_append_normed(im_device *dev, const im_paged_kv *kv,
     m.qn = q_norm_dev; m.kn = k_norm_dev;
     m.norm_f32 = norm_dtype == IM_DTYPE_F32;
     m.axes = num_axes;
+    m.neighbours = neighbours;
     m.eps = eps;
     m.inv_dim = 1.0f / kv->head_dim;
     for (int i = 0; num_axes > 1 && i < rotary_dim / 2; i++) {
@@ -608,11 +667,8 @@ IM_EXPORT int im_cuda_paged_append_normed(im_device *dev, const im_paged_kv *kv,
     const int lanes = append_lanes(kv->head_dim);
     const bool bf16 = kv->dtype == IM_DTYPE_BF16, f32 = table_dtype == IM_DTYPE_F32;
     void (*kern)(Append, AppendMore, int) = nullptr;
-#define IM_FORM(F) \
-    (bf16 ? (f32 ? paged_append_normed_kernel<true, F, true> : paged_append_normed_kernel<true, F, false>) : (f32 ? paged_append_normed_kernel<false, F, true> : paged_append_normed_kernel<false, F, false>))
-    if (neighbours || rotary_dim == 0) kern = IM_FORM(1);
-    else if (rotary_dim % 8 == 0) kern = IM_FORM(0);
-    else kern = IM_FORM(2);
+#define IM_FORM(B, F) (rotary_dim % 8 ? paged_append_odd_kernel<B, F> : neighbours ? paged_append_normed_kernel<B, true, F> : paged_append_normed_kernel<B, false, F>)
+    kern = bf16 ? (f32 ? IM_FORM(true, true) : IM_FORM(true, false)) : (f32 ? IM_FORM(false, true) : IM_FORM(false, false));
 #undef IM_FORM
     IM_CUDA_CHECK(launch_k(kern, dim3((unsigned)num_tokens), dim3(num_tokens > 4 * dev->sm_count ? kAppendSmall : kAppendThreads), 0, as_stream(stream), a, m, lanes));
     return IM_OK;
