@@ -238,25 +238,20 @@ __device__ __forceinline__ bool append_place(const Append &a, const AppendMore &
     at = a.kv.row_of(seq, (int)r);
     return there;
 }
-// Cosines and sines of pairs e0 .. e0 + 3 (e0 a multiple of 4): from the rows of the axes that they have.
+// Cosines and sines of pairs e0 .. e0 + 3 (e0 a multiple of 4, below rotary_dim / 2), each from the row of its axis: all four from the first one's, and those of other axes again.
 template <bool F32>
 __device__ __forceinline__ void append_angles(const Append &a, const AppendMore &m, const int (&pos)[kAxes], int e0, float *cs, float *sn) {
-    const int half = a.rot / 2;
-    const uint32_t axes = m.axis[e0 / 16 & 7] >> (2 * (e0 & 15));  // (sixteen pairs a word)
+    const uint32_t axes = m.axis[e0 / 16 & 7] >> (2 * (e0 & 15)) & 255u;  // (sixteen pairs a word)
+    auto row = [&](uint32_t k) { return (long long)(k == 0 ? pos[0] : k == 1 ? pos[1] : k == 2 ? pos[2] : pos[3]) * (a.kv.hd / 2); };
+    const long long at = row(axes & 3);
+    angles4<F32>(a.cosc, at + e0, cs);
+    angles4<F32>(a.sinc, at + e0, sn);
+    if (axes == (axes & 3) * 0x55u) return;
 #pragma unroll
-    for (int j = 0; j < 4; j++) cs[j] = 1.0f, sn[j] = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kAxes; k++) {
-        bool any = false;
-#pragma unroll
-        for (int j = 0; j < 4; j++) any = any || (e0 + j < half && (axes >> (2 * j) & 3) == k);
-        if (!any) continue;
-        float s[4], t[4];
-        angles4<F32>(a.cosc, (long long)pos[k] * (a.kv.hd / 2) + e0, s);
-        angles4<F32>(a.sinc, (long long)pos[k] * (a.kv.hd / 2) + e0, t);
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (e0 + j < half && (axes >> (2 * j) & 3) == k) cs[j] = s[j], sn[j] = t[j];
+    for (int j = 1; j < 4; j++) {
+        const long long e = row(axes >> (2 * j) & 3) + e0 + j;
+        cs[j] = F32 ? __ldg(static_cast<const float *>(a.cosc) + e) : __half2float(__ldg(static_cast<const __half *>(a.cosc) + e));
+        sn[j] = F32 ? __ldg(static_cast<const float *>(a.sinc) + e) : __half2float(__ldg(static_cast<const __half *>(a.sinc) + e));
     }
 }
 template <bool BF16>
@@ -280,12 +275,12 @@ __device__ __forceinline__ void weights4(const void *w, int f32, int d, float *o
 
 // rotary_dim a multiple of 8: the four pairs of a lane are turned or none is.
 constexpr int kNormedHeads = 4;
-template <bool BF16, bool NB, bool F32>
-__global__ void __launch_bounds__(kAppendThreads, 4) paged_append_normed_kernel(const __grid_constant__ Append a, const __grid_constant__ AppendMore m, int lanes) {
+template <bool BF16, bool NB, bool F32, int LANES>
+__global__ void __launch_bounds__(kAppendThreads, 4) paged_append_normed_kernel(const __grid_constant__ Append a, const __grid_constant__ AppendMore m) {
     pdl_trigger();
     pdl_wait();
     const int token = blockIdx.x, tid = threadIdx.x;
-    const int c = tid & (lanes - 1), first = tid / lanes, per = blockDim.x / lanes;
+    const int c = tid % LANES, first = tid / LANES, per = blockDim.x / LANES;
     const int hd = a.kv.hd, half = a.rot / 2, e0 = 4 * c;
     const bool mine = 8 * c < hd, turned = e0 < half;
     const int colA = !NB && turned ? e0 : 2 * e0, colB = !NB && turned ? half + e0 : 2 * e0 + 4;
@@ -308,7 +303,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) paged_append_normed_kernel(
     int pos[kAxes];
     if (!append_place(a, m, token, at, pos)) return;
     float cs[4], sn[4];
-    if (a.rot > 0 && mine) append_angles<F32>(a, m, pos, e0, cs, sn);
+    if (turned && mine) append_angles<F32>(a, m, pos, e0, cs, sn);
     else
 #pragma unroll
         for (int j = 0; j < 4; j++) cs[j] = 1.0f, sn[j] = 0.0f;
@@ -355,7 +350,8 @@ __global__ void __launch_bounds__(kAppendThreads, 4) paged_append_normed_kernel(
                 if (norm) {
                     const float2 q = of_two(add_two(fma_two(X[0], X[0], mul_two(X[1], X[1])), fma_two(X[2], X[2], mul_two(X[3], X[3]))));
                     float sum = q.x + q.y;
-                    for (int o = lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    #pragma unroll
+                    for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                     r = rsqrtf(fmaf(sum, m.inv_dim, m.eps));
                 }
                 const uint64_t rr = two(r, r);
@@ -401,7 +397,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_odd_kernel(const 
     int pos[kAxes];
     if (!append_place(a, m, token, at, pos)) return;
     float cs[4], sn[4];
-    if (a.rot > 0 && mine) append_angles<F32>(a, m, pos, e0, cs, sn);
+    if (e0 < half && mine) append_angles<F32>(a, m, pos, e0, cs, sn);
 #pragma unroll 1
     for (int h = first; h - first < heads; h += per) {  // the same count for every lane of a warp
         const bool is_q = h < a.nh, is_v = h >= a.nh + a.kv.nkv, live = mine && h < heads;
@@ -666,11 +662,20 @@ IM_EXPORT int im_cuda_paged_append_normed(im_device *dev, const im_paged_kv *kv,
     }
     const int lanes = append_lanes(kv->head_dim);
     const bool bf16 = kv->dtype == IM_DTYPE_BF16, f32 = table_dtype == IM_DTYPE_F32;
-    void (*kern)(Append, AppendMore, int) = nullptr;
-#define IM_FORM(B, F) (rotary_dim % 8 ? paged_append_odd_kernel<B, F> : neighbours ? paged_append_normed_kernel<B, true, F> : paged_append_normed_kernel<B, false, F>)
+    const dim3 grid((unsigned)num_tokens), block(num_tokens > 4 * dev->sm_count ? kAppendSmall : kAppendThreads);
+    if (rotary_dim % 8) {
+        void (*odd)(Append, AppendMore, int) = bf16 ? (f32 ? paged_append_odd_kernel<true, true> : paged_append_odd_kernel<true, false>)
+                                                    : (f32 ? paged_append_odd_kernel<false, true> : paged_append_odd_kernel<false, false>);
+        IM_CUDA_CHECK(launch_k(odd, grid, block, 0, as_stream(stream), a, m, lanes));
+        return IM_OK;
+    }
+    void (*kern)(Append, AppendMore) = nullptr;
+#define IM_LANES(B, N, F) (lanes == 32 ? paged_append_normed_kernel<B, N, F, 32> : lanes == 16 ? paged_append_normed_kernel<B, N, F, 16> : paged_append_normed_kernel<B, N, F, 8>)
+#define IM_FORM(B, F) (neighbours ? IM_LANES(B, true, F) : IM_LANES(B, false, F))
     kern = bf16 ? (f32 ? IM_FORM(true, true) : IM_FORM(true, false)) : (f32 ? IM_FORM(false, true) : IM_FORM(false, false));
 #undef IM_FORM
-    IM_CUDA_CHECK(launch_k(kern, dim3((unsigned)num_tokens), dim3(num_tokens > 4 * dev->sm_count ? kAppendSmall : kAppendThreads), 0, as_stream(stream), a, m, lanes));
+#undef IM_LANES
+    IM_CUDA_CHECK(launch_k(kern, grid, block, 0, as_stream(stream), a, m));
     return IM_OK;
     IM_GUARD_END
 }
