@@ -419,53 +419,15 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
     }
 }
 
-// Items that a cut divides: a warp per row, HD / 32 columns a lane. The parts of an item lie with the CTAs that its tiles fall to; a lane per part
-// brings maxima and sums. (A block per row with the shares' divisions in loops took 25 us for 64 items of 104 rows.)
+// Items that a cut divides: eight rows a block.
 constexpr int kJoinWarps = 8;
 template <bool BF16, int R, int HD, int MODE>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __grid_constant__ PagedAttn p) {
-    constexpr int V = HD / 32;
     pdl_trigger();
     pdl_wait();
-    const int item = blockIdx.x, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, lane = threadIdx.x & 31, r = blockIdx.y * kJoinWarps + (threadIdx.x >> 5);
-    const int2 span = *reinterpret_cast<const int2 *>(p.spans + 2 * (long long)item);
-    const PagedUnit u = paged_unit<R, MODE>(p, unit);
-    if (r >= u.rows || span.x < 0) return;  // (a unit without tiles has no rows)
-    const size_t slot0 = span.x;
-    const int c = span.x >> 1, parts = span.y - c + 1;
-    auto at = [&](int i) { return (i == 0 ? slot0 : (size_t)(c + i) * 2) * R + r; };
-    float M = -INFINITY, L = 0.0f, o[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) o[j] = 0.0f;
-    for (int i0 = 0; i0 < parts; i0 += 32) {
-        const float2 x = i0 + lane < parts ? p.part_ml[at(i0 + lane)] : make_float2(-INFINITY, 0.0f);
-        const float top = fmaxf(M, warp_max(x.x)), corr = M == top ? 1.0f : ex2(M - top);
-        const float f = x.x == -INFINITY && x.y == 0.0f ? 0.0f : ex2(x.x - top);  // (nothing seen in this part)
-        M = top;
-        L = L * corr + warp_sum(x.y * f);
-#pragma unroll
-        for (int j = 0; j < V; j++) o[j] *= corr;
-        const int m = min(32, parts - i0);
-#pragma unroll 4
-        for (int i = 0; i < m; i++) {
-            const float *src = p.part_o + at(i0 + i) * HD + lane * V;
-            const float g = __shfl_sync(0xffffffffu, f, i);
-            float v[V];
-            if constexpr (V == 2) *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(src);
-            else
-#pragma unroll
-                for (int j = 0; j < V; j += 4) *reinterpret_cast<float4 *>(v + j) = *reinterpret_cast<const float4 *>(src + j);
-#pragma unroll
-            for (int j = 0; j < V; j++) o[j] += g == 0.0f ? 0.0f : v[j] * g;
-        }
-    }
-    if (MODE == kWeigh && lane == 0) p.stat[(long long)item * R + r] = make_float2(M, L);
-    const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
-    const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
-    uint32_t *dst = reinterpret_cast<uint32_t *>(p.out + (u.tok0 + t) * p.os + (long long)(head * p.group + g) * HD + lane * V);
-#pragma unroll
-    for (int j = 0; j < V; j += 2) dst[j / 2] = pack16<BF16>(o[j] * inv, o[j + 1] * inv);
+    join_row<BF16, R, HD, MODE>(p, blockIdx.x, blockIdx.y * kJoinWarps + (threadIdx.x >> 5));
 }
+
 
 constexpr int kClusterMost = 8;
 
@@ -519,7 +481,7 @@ int join_launch(const PagedAttn &p, int units, cudaStream_t st) {
 }
 
 template <bool BF16, int HD, int MODE>
-int attn_launch(const Device *dev, const PagedAttn &p, int units, int cluster, cudaStream_t st) {
+int attn_launch(const Device *dev, const PagedAttn &p, int units, int cluster, bool joins, cudaStream_t st) {
     using S = PaShape<HD>;
     static DeviceOnce once;
     if (once.first(dev->ordinal)) {
@@ -531,13 +493,13 @@ int attn_launch(const Device *dev, const PagedAttn &p, int units, int cluster, c
         return IM_OK;
     }
     IM_CUDA_CHECK(launch_k(paged_attn_kernel<BF16, HD, false, MODE>, dim3(p.ctas), dim3(kPaThreads), (size_t)S::kSmem, st, p, units));
-    return join_launch<BF16, S::kRows, HD, MODE>(p, units, st);
+    return joins ? join_launch<BF16, S::kRows, HD, MODE>(p, units, st) : IM_OK;
 }
 
 }  // namespace
 
-int paged_weigh_launch(const Device *dev, const PagedAttn &p, bool bf16, int units, int cluster, cudaStream_t st) {
-#define IM_RUN(HD) (bf16 ? attn_launch<true, HD, kWeigh>(dev, p, units, cluster, st) : attn_launch<false, HD, kWeigh>(dev, p, units, cluster, st))
+int paged_weigh_launch(const Device *dev, const PagedAttn &p, bool bf16, int units, int cluster, bool joins, cudaStream_t st) {
+#define IM_RUN(HD) (bf16 ? attn_launch<true, HD, kWeigh>(dev, p, units, cluster, joins, st) : attn_launch<false, HD, kWeigh>(dev, p, units, cluster, joins, st))
     switch (p.kv.hd) {
     case 64: return IM_RUN(64);
     case 128: return IM_RUN(128);
@@ -628,7 +590,7 @@ IM_EXPORT int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int
     const cudaStream_t st = as_stream(stream);
     const bool bf16 = kv->dtype == IM_DTYPE_BF16;
     if (plan.rows >= 128) return paged_tc_launch(dev, p, bf16, plan.rows, plan.units, st);
-#define IM_RUN(HD) (bf16 ? attn_launch<true, HD, kAttend>(dev, p, plan.units, plan.cluster, st) : attn_launch<false, HD, kAttend>(dev, p, plan.units, plan.cluster, st))
+#define IM_RUN(HD) (bf16 ? attn_launch<true, HD, kAttend>(dev, p, plan.units, plan.cluster, true, st) : attn_launch<false, HD, kAttend>(dev, p, plan.units, plan.cluster, true, st))
     switch (kv->head_dim) {
     case 64: return IM_RUN(64);
     case 128: return IM_RUN(128);

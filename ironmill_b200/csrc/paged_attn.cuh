@@ -381,6 +381,50 @@ __device__ __noinline__ float plain_sum(const PagedAttn &p, const PagedUnit &u, 
     return v;
 }
 
+// Row r of an item that a cut divides, by a warp, HD / 32 columns a lane. The parts of an item lie with the CTAs that its tiles fall to; a lane per part
+// brings maxima and sums. (A block per row with the shares' divisions in loops took 25 us for 64 items of 104 rows.)
+template <bool BF16, int R, int HD, int MODE>
+__device__ __forceinline__ void join_row(const PagedAttn &p, int item, int r) {
+    constexpr int V = HD / 32;
+    const int unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, lane = threadIdx.x & 31;
+    const int2 span = *reinterpret_cast<const int2 *>(p.spans + 2 * (long long)item);
+    const PagedUnit u = paged_unit<R, MODE>(p, unit);
+    if (r >= u.rows || span.x < 0) return;  // (a unit without tiles has no rows)
+    const size_t slot0 = span.x;
+    const int c = span.x >> 1, parts = span.y - c + 1;
+    auto at = [&](int i) { return (i == 0 ? slot0 : (size_t)(c + i) * 2) * R + r; };
+    float M = -INFINITY, L = 0.0f, o[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) o[j] = 0.0f;
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+        const float2 x = i0 + lane < parts ? p.part_ml[at(i0 + lane)] : make_float2(-INFINITY, 0.0f);
+        const float top = fmaxf(M, warp_max(x.x)), corr = M == top ? 1.0f : ex2(M - top);
+        const float f = x.x == -INFINITY && x.y == 0.0f ? 0.0f : ex2(x.x - top);  // (nothing seen in this part)
+        M = top;
+        L = L * corr + warp_sum(x.y * f);
+#pragma unroll
+        for (int j = 0; j < V; j++) o[j] *= corr;
+        const int m = min(32, parts - i0);
+#pragma unroll 4
+        for (int i = 0; i < m; i++) {
+            const float *src = p.part_o + at(i0 + i) * HD + lane * V;
+            const float g = __shfl_sync(0xffffffffu, f, i);
+            float v[V];
+            if constexpr (V == 2) *reinterpret_cast<float2 *>(v) = *reinterpret_cast<const float2 *>(src);
+            else
+#pragma unroll
+                for (int j = 0; j < V; j += 4) *reinterpret_cast<float4 *>(v + j) = *reinterpret_cast<const float4 *>(src + j);
+#pragma unroll
+            for (int j = 0; j < V; j++) o[j] += g == 0.0f ? 0.0f : v[j] * g;
+        }
+    }
+    if (MODE == kWeigh && lane == 0) p.stat[(long long)item * R + r] = make_float2(M, L);
+    const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
+    const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
+    uint32_t *dst = reinterpret_cast<uint32_t *>(p.out + (u.tok0 + t) * p.os + (long long)(head * p.group + g) * HD + lane * V);
+#pragma unroll
+    for (int j = 0; j < V; j += 2) dst[j / 2] = pack16<BF16>(o[j] * inv, o[j + 1] * inv);
+}
 // Many rows of a KV head on the tcgen05 tensor cores (paged_attn_tc.cu): rows of a tile for so many rows of a sequence, 0 where the
 // kernel of paged_attn.cu is the one to use; CTAs = SMs.
 int paged_tc_rows(int hd, long long rows);
@@ -395,8 +439,8 @@ int attn_args(im_device *dev, const im_paged_kv *kv, int layer, const void *q_de
 
 // The kernel of paged_attn_tc.cu with the sums of a part as its result (paged_prefix.cu): MODE kShared or kOwn; no join.
 int paged_tc_part_launch(const Device *dev, const PagedAttn &p, bool bf16, int mode, int rows, int units, cudaStream_t st);
-// Attention and the norms of every row's weights (paged_weights.cu): where `cluster` is not zero, the sums too. With joins.
-int paged_weigh_launch(const Device *dev, const PagedAttn &p, bool bf16, int units, int cluster, cudaStream_t st);
+// Attention and the norms of every row's weights (paged_weights.cu): where `cluster` is not zero, the sums too. joins: with the join of what the cuts divide (tcgen05: always).
+int paged_weigh_launch(const Device *dev, const PagedAttn &p, bool bf16, int units, int cluster, bool joins, cudaStream_t st);
 int paged_tc_weigh_launch(const Device *dev, const PagedAttn &p, bool bf16, int rows, int units, cudaStream_t st);
 struct AttnPlan {
     int rows, tile, row_tiles, units, ctas;

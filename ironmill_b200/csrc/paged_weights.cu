@@ -17,30 +17,70 @@
 namespace im {
 namespace {
 
-constexpr int kSumThreads = 256;
+constexpr int kSumThreads = 256, kSumWarps = kSumThreads / 32, kSumPositions = 4 * kSumThreads;
 
-// Sums from scores: a block takes kSumThreads positions of an item at a time.
+// Behind attention in shares, in one launch: blocks below `joins` join the outputs of items that a cut divides, eight rows each, the others add up the weights of an item, four positions a
+// thread. Both find the rows' maxima and sums in the parts.
 template <bool BF16, int HD>
-__global__ void __launch_bounds__(kSumThreads) paged_sum_kernel(const __grid_constant__ PagedAttn p) {
+__global__ void __launch_bounds__(kSumThreads) paged_sum_kernel(const __grid_constant__ PagedAttn p, int joins, int row_blocks, int chunks) {
     constexpr int R = 16;
     __shared__ float norms[R];
     pdl_trigger();
     pdl_wait();
-    const int item = blockIdx.x, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if ((int)blockIdx.x < joins) {
+        join_row<BF16, R, HD, kWeigh>(p, blockIdx.x / row_blocks, (blockIdx.x % row_blocks) * kSumWarps + warp);
+        return;
+    }
+    const int item = (blockIdx.x - joins) / chunks, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, chunk = (blockIdx.x - joins) % chunks;
     const PagedUnit u = paged_unit<R, kWeigh>(p, unit);
-    if ((int)blockIdx.y * kSumThreads >= u.end) return;
-    if (tid < u.rows) norms[tid] = row_norm(p.stat[(long long)item * R + tid]);
+    if ((long long)chunk * kSumPositions >= u.end) return;
+    const int2 span = *reinterpret_cast<const int2 *>(p.spans + 2 * (long long)item);
+    for (int r = warp; r < u.rows; r += kSumWarps) {
+        float2 ml;
+        if (span.x < 0) {
+            ml = p.stat[(long long)item * R + r];
+        } else {
+            const int c = span.x >> 1, parts = span.y - c + 1;
+            float M = -INFINITY, L = 0.0f;
+            for (int i = lane; i < parts; i += 32) {
+                const float2 x = p.part_ml[(i == 0 ? (size_t)span.x : (size_t)(c + i) * 2) * R + r];
+                if (x.x == -INFINITY && x.y == 0.0f) continue;
+                const float top = fmaxf(M, x.x);
+                L = (M == top ? L : L * ex2(M - top)) + x.y * ex2(x.x - top);
+                M = top;
+            }
+            const float top = warp_max(M);
+            ml = make_float2(top, warp_sum(M == -INFINITY && L == 0.0f ? 0.0f : L * ex2(M - top)));
+        }
+        if (lane == 0) norms[r] = row_norm(ml);
+    }
     __syncthreads();
     const float *scores = p.scores + (long long)item * p.score_rows * p.score_cap;
-    for (long long pos = (long long)blockIdx.y * kSumThreads + tid; pos < u.end; pos += (long long)gridDim.y * kSumThreads) {
-        float v = 0.0f;
-        if (pos >= p.score_cap) {
-            v = plain_sum<BF16, HD>(p, u, head, (int)pos, norms);
-        } else {
+    float *sums = p.sums + u.seq * p.sum_seq + head * p.sum_head;
+    const bool aligned = reinterpret_cast<uintptr_t>(sums) % 16 == 0;
+    for (long long at = (long long)chunk * kSumPositions + 4 * tid; at < u.end; at += (long long)chunks * kSumPositions) {
+        const int pos = (int)at;
+        if (pos + 4 <= p.score_cap) {  // (a multiple of 64)
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-            for (int r = 0; r < u.rows; r++) v += ex2(scores[(long long)r * p.score_cap + pos] + norms[r]);
+            for (int r = 0; r < u.rows; r++) {
+                const float4 s = *reinterpret_cast<const float4 *>(scores + (long long)r * p.score_cap + pos);
+                v.x += ex2(s.x + norms[r]); v.y += ex2(s.y + norms[r]); v.z += ex2(s.z + norms[r]); v.w += ex2(s.w + norms[r]);
+            }
+            if (aligned && pos + 4 <= min(u.len, p.sum_cols)) {
+                float4 *to = reinterpret_cast<float4 *>(sums + pos);
+                const float4 o = *to;
+                *to = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
+            } else {
+                const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (pos + j < u.end) add_sum(p, u, head, pos + j, x[j]);
+            }
+        } else {
+            for (int j = 0; j < 4 && pos + j < u.end; j++) add_sum(p, u, head, pos + j, plain_sum<BF16, HD>(p, u, head, pos + j, norms));
         }
-        add_sum(p, u, head, (int)pos, v);
     }
 }
 
@@ -255,14 +295,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_weigh_kernel(const __grid
                     const bool is = (there[(tile & 7) * 4 + (warp & 3)] >> lane & 1u) != 0;
                     const bool edge = t * kTcTile + kTcTile > u.len;  // some row may not see some position
                     uint64_t sum[2] = {0, 0};
-#pragma unroll 1
-                    for (int c = 0; c < n; c += 32) {
-                        uint32_t s[32];
-                        ld32(ts + (uint32_t)c, s);
-                        float4 a[8];
-#pragma unroll
-                        for (int j = 0; j < 8; j++) a[j] = *reinterpret_cast<const float4 *>(norms + c + 4 * j);
-                        tmem_wait_ld();
+                    auto add = [&](uint32_t *s, int c) {  // 32 columns
                         if (edge) {
                             const uint32_t seen = rows_seeing(p, u, row0 + c, pos);
 #pragma unroll
@@ -271,11 +304,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_weigh_kernel(const __grid
                         }
 #pragma unroll
                         for (int j = 0; j < 8; j++) {
-                            const float2 e0 = of_two(fma_two(two(__uint_as_float(s[4 * j]), __uint_as_float(s[4 * j + 1])), scale_two, two(a[j].x, a[j].y)));
-                            const float2 e1 = of_two(fma_two(two(__uint_as_float(s[4 * j + 2]), __uint_as_float(s[4 * j + 3])), scale_two, two(a[j].z, a[j].w)));
+                            const float4 a = *reinterpret_cast<const float4 *>(norms + c + 4 * j);
+                            const float2 e0 = of_two(fma_two(two(__uint_as_float(s[4 * j]), __uint_as_float(s[4 * j + 1])), scale_two, two(a.x, a.y)));
+                            const float2 e1 = of_two(fma_two(two(__uint_as_float(s[4 * j + 2]), __uint_as_float(s[4 * j + 3])), scale_two, two(a.z, a.w)));
                             sum[0] = add_two(sum[0], two(ex2(e0.x), ex2(e0.y)));
                             sum[1] = add_two(sum[1], two(ex2(e1.x), ex2(e1.y)));
                         }
+                    };
+                    uint32_t s0[32], s1[32];  // the next columns are on their way while these are added
+                    ld32(ts, s0);
+#pragma unroll 1
+                    for (int c = 0; c < n; c += 64) {
+                        tmem_wait_ld();
+                        if (c + 32 < n) ld32(ts + (uint32_t)(c + 32), s1);
+                        add(s0, c);
+                        if (c + 32 >= n) break;
+                        tmem_wait_ld();
+                        if (c + 64 < n) ld32(ts + (uint32_t)(c + 64), s0);
+                        add(s1, c + 32);
                     }
                     fence_before();
                     __syncwarp();
@@ -336,8 +382,9 @@ WeighPlan weigh_plan(const Device *dev, const PagedView &v, int group, int max_n
 template <bool BF16, int HD>
 int sums(const Device *dev, const PagedAttn &p, const WeighPlan &plan, int max_len, cudaStream_t st) {
     if (p.scores) {
-        const unsigned blocks = (unsigned)std::max(1ll, std::min((max_len + (long long)kSumThreads - 1) / kSumThreads, 65535ll));
-        IM_CUDA_CHECK(launch_k(paged_sum_kernel<BF16, HD>, dim3((unsigned)(plan.attn.units * p.kv.nkv), blocks), dim3(kSumThreads), 0, st, p));
+        const long long items = (long long)plan.attn.units * p.kv.nkv, row_blocks = (plan.rows + kSumWarps - 1) / kSumWarps;
+        const long long chunks = std::max(1ll, std::min<long long>((max_len + (long long)kSumPositions - 1) / kSumPositions, (1ll << 30) / items));
+        IM_CUDA_CHECK(launch_k(paged_sum_kernel<BF16, HD>, dim3((unsigned)(items * (row_blocks + chunks))), dim3(kSumThreads), 0, st, p, (int)(items * row_blocks), (int)row_blocks, (int)chunks));
         return IM_OK;
     }
     using S = WeighShape<HD / 64>;
@@ -398,7 +445,7 @@ IM_EXPORT int im_cuda_paged_attention_weights(im_device *dev, const im_paged_kv 
     p.sum_cols = rows;
     const cudaStream_t st = as_stream(stream);
     const bool bf16 = kv->dtype == IM_DTYPE_BF16;
-    rc = plan.attn.rows >= 128 ? paged_tc_weigh_launch(dev, p, bf16, plan.attn.rows, plan.attn.units, st) : paged_weigh_launch(dev, p, bf16, plan.attn.units, plan.attn.cluster, st);
+    rc = plan.attn.rows >= 128 ? paged_tc_weigh_launch(dev, p, bf16, plan.attn.rows, plan.attn.units, st) : paged_weigh_launch(dev, p, bf16, plan.attn.units, plan.attn.cluster, !p.scores, st);
     if (rc != IM_OK || (plan.attn.cluster && p.scores)) return rc;
 #define IM_RUN(HD) (bf16 ? sums<true, HD>(dev, p, plan, max_len, st) : sums<false, HD>(dev, p, plan, max_len, st))
     switch (kv->head_dim) {
