@@ -74,8 +74,6 @@ __device__ __forceinline__ uint32_t sees32(const PagedAttn &p, const PagedUnit &
     return shift == 0 ? bits : bits << shift | ((1u << shift) - 1);
 }
 
-// The 256 threads of both halves.
-__device__ __forceinline__ void both_halves() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 
 template <bool BF16, int KB, bool WIDE, int MODE>

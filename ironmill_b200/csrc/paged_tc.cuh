@@ -68,6 +68,8 @@ __device__ __forceinline__ void umma_commit(uint32_t one, uint64_t *bar) {
                  "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)), "r"(one)
                  : "memory");
 }
+// The 256 threads of both sets of four warps.
+__device__ __forceinline__ void both_halves() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 // What copies of other threads have written, once their barrier says so, before the tensor cores read it.
 __device__ __forceinline__ void copies_landed() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 

@@ -148,8 +148,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_weigh_kernel(const __grid
             mbar_init(&kfull[i], kTcCopyWarps * 33);  // threads whose copies are there; warps that have said which rows are
             mbar_init(&kempty[i], 1);
         }
-        mbar_init(qfull, kTcCopyWarps * 33);          // (and which norms)
-        mbar_init(qempty, 1 + 8);                     // products done; warps that have read the norms
+        mbar_init(qfull, kTcCopyWarps * 32);
+        mbar_init(qempty, 1);
         for (int i = 0; i < 2; i++) {
             mbar_init(&sfull[i], 1);
             mbar_init(&sempty[i], 4);
@@ -219,10 +219,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_weigh_kernel(const __grid
                     const int row = row0 + r + lane, t = row / p.group, g = row - t * p.group;
                     const bool is = row < u.rows;
                     rows32(Qs + r * 128, S::kQBlock, p.q, is ? (u.tok0 + t) * p.qs + (long long)(it.head * p.group + g) * HD : -1);
-                    norms[r + lane] = is ? row_norm(p.stat[(((long long)u.seq * stat_tiles + row / stat_rows) * p.kv.nkv + it.head) * stat_rows + row % stat_rows]) : -INFINITY;
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(qfull);
                 requested(qfull);
                 for (int t = it.t0; t < it.t1; t++) {
                     const int ks = kc % SK;
@@ -285,8 +282,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_weigh_kernel(const __grid
         while (it.next()) {
             const PagedUnit &u = it.u;
             for (int row0 = 0; row0 < u.rows; row0 += BR, block++) {
-                if (ok && !wait_for(qfull, block & 1, err)) ok = false;  // the norms
                 const int n = columns(u, row0);
+                both_halves();  // the norms before have been read
+                if (tid < n) {
+                    const int row = row0 + tid;
+                    norms[tid] = row < u.rows ? row_norm(p.stat[(((long long)u.seq * stat_tiles + row / stat_rows) * p.kv.nkv + it.head) * stat_rows + row % stat_rows]) : -INFINITY;
+                }
+                both_halves();
                 for (int t = it.t0; t < it.t1; t++, tile++) {
                     if ((tile & 1) != h) continue;
                     if (ok && !wait_for(&sfull[h], (tile / 2) & 1, err)) ok = false;
@@ -305,8 +307,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_weigh_kernel(const __grid
 #pragma unroll
                         for (int j = 0; j < 8; j++) {
                             const float4 a = *reinterpret_cast<const float4 *>(norms + c + 4 * j);
-                            const float2 e0 = of_two(fma_two(two(__uint_as_float(s[4 * j]), __uint_as_float(s[4 * j + 1])), scale_two, two(a.x, a.y)));
-                            const float2 e1 = of_two(fma_two(two(__uint_as_float(s[4 * j + 2]), __uint_as_float(s[4 * j + 3])), scale_two, two(a.z, a.w)));
+                            const uint64_t x0 = fma_two(two(__uint_as_float(s[4 * j]), __uint_as_float(s[4 * j + 1])), scale_two, two(a.x, a.y));
+                            const uint64_t x1 = fma_two(two(__uint_as_float(s[4 * j + 2]), __uint_as_float(s[4 * j + 3])), scale_two, two(a.z, a.w));
+                            const float2 e0 = of_two(x0), e1 = of_two(x1);
                             sum[0] = add_two(sum[0], two(ex2(e0.x), ex2(e0.y)));
                             sum[1] = add_two(sum[1], two(ex2(e1.x), ex2(e1.y)));
                         }
@@ -338,8 +341,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_weigh_kernel(const __grid
                     }
                     if (pos < u.end) add_sum(p, u, it.head, pos, is ? v : 0.0f, row0 == 0);
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(qempty);
             }
         }
     }
