@@ -261,10 +261,10 @@ __global__ void __launch_bounds__(kPtThreads, HD == 256 ? 2 : 3) paged_part_kern
 
 // ------------------------------------------------------------------------------------------------ the join
 // A block takes eight rows (token, query head of one KV head, token-major), a thread four columns of one: eight rows of a column quad lie side by side in the parts of
-// paged_attn_tc.cu. Warps look the rows up, then lanes the parts' maxima and sums, 32 parts at a time; factors go to shared memory.
+// paged_attn_tc.cu. Eight lanes look the rows up, then lanes the parts' maxima and sums, 32 parts at a time; factors go to shared memory.
 constexpr int kPjRows = 8, kPjParts = 32;
 struct PjRow {
-    int token, seq;           // -1: not to be written
+    int token;                // -1: not to be written
     long long out;
     int slot0[2], next[2], parts[2], r[2];  // shared, own: slot of the first part, of the second less two (tcgen05) or one, number of parts, row of the tile
     int unit[2];              // -1: no parts
@@ -303,40 +303,40 @@ __global__ void __launch_bounds__(2 * HD) paged_prefix_join_kernel(const __grid_
     pdl_wait();
     const PagedAttn &p = a.own.p;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, head = blockIdx.y;
-    if (tid < 2) more[tid] = 0;
-    if (tid == 2) odd = 0;
-    if (tid < kPjRows) state[tid] = make_float2(-INFINITY, 0.0f);
-    __syncthreads();
-    for (int i = warp; i < kPjRows; i += kWarps) {
-        const long long at = (long long)blockIdx.x * kPjRows + i;
+    if (tid < kPjRows) {  // a lane per row: the lookups are many instructions
+        const long long at = (long long)blockIdx.x * kPjRows + tid;
         PjRow x;
         x.token = -1;
         x.parts[0] = x.parts[1] = 0;
         x.unit[0] = x.unit[1] = -1;
         const int token = (int)min(at / p.group, (long long)INT_MAX), hq = (int)(at - (long long)token * p.group);
         if (token < p.tokens && token >= __ldg(p.start) && token < __ldg(p.start + p.kv.nseq)) {
-            const int seq = paged_seq_of(p.start, p.kv.nseq, token), first = __ldg(p.start + seq), end = __ldg(p.start + seq + 1), t = token - first;
+            int seq = 0;  // the last that starts at or before the token
+            for (int hi = p.kv.nseq; hi - seq > 1;) {
+                const int mid = (seq + hi) / 2;
+                if (__ldg(p.start + mid) <= token) seq = mid;
+                else hi = mid;
+            }
+            const int first = __ldg(p.start + seq), end = __ldg(p.start + seq + 1), t = token - first;
             if (first >= 0 && t >= 0 && t < p.max_new && end <= p.tokens && token < end) {
                 const int group = paged_group_of(p, seq);
                 const long long place = group < 0 ? 0 : (long long)token - __ldg(p.start + min(max(__ldg(p.group_start + group), 0), p.kv.nseq));
                 if (place >= 0 && place < a.group_new) {
                     x.token = token;
-                    x.seq = seq;
                     x.out = token * p.os + (long long)(head * p.group + hq) * HD;
                     if (group >= 0) {
-                        const int row = (int)place * p.group + hq;
-                        find_parts<BF16, HD, kShared>(a.shared, group * a.shared.p.row_tiles + row / a.shared.rows, head, row % a.shared.rows, x);
+                        const int row = (int)place * p.group + hq, tile = row / a.shared.rows;
+                        find_parts<BF16, HD, kShared>(a.shared, group * a.shared.p.row_tiles + tile, head, row - tile * a.shared.rows, x);
                     }
-                    const int row = t * p.group + hq;
-                    find_parts<BF16, HD, kOwn>(a.own, seq * p.row_tiles + row / a.own.rows, head, row % a.own.rows, x);
+                    const int row = t * p.group + hq, tile = row / a.own.rows;
+                    find_parts<BF16, HD, kOwn>(a.own, seq * p.row_tiles + tile, head, row - tile * a.own.rows, x);
                 }
             }
         }
-        if (lane == 0) {
-            rows[i] = x;
-            atomicMax(&more[0], x.parts[0]);
-            atomicMax(&more[1], x.parts[1]);
-        }
+        rows[tid] = x;
+        const int shared = __reduce_max_sync((1u << kPjRows) - 1, x.parts[0]), own = __reduce_max_sync((1u << kPjRows) - 1, x.parts[1]);
+        if (tid == 0) more[0] = shared, more[1] = own, odd = 0;
+        state[tid] = make_float2(-INFINITY, 0.0f);
     }
     __syncthreads();
     const int r = tid % kPjRows, q = tid / kPjRows;  // this thread's row and columns 4 q ..
@@ -473,6 +473,22 @@ unsigned char *lay_out(PartSet *s, const PartPlan &plan, int max_rows, int likel
     return at + plan.bytes;
 }
 
+// CTAs of a tcgen05 launch for the shared rows beside which the own rows are read by others: as many as make both end together. In SM microseconds, both measured: a tile of
+// 128 positions 2.7 (256 rows) or 2.1 (128) and 8 for a CTA's start and outputs; 20 KB of own rows one, of which a sequence has about half the longest's. (64 sequences of up to
+// 700 rows behind 8192: 74 us with all SMs for the shared rows first, 65 with half, 60 with 48 of 148, 63 with 36; 8 x 8 behind 3000: 68, 65, 74, 90.)
+int shared_ctas_beside(const Device *dev, const PrefixJoin &a, const PrefixPlan &plan, int max_prefix, int max_len) {
+    const int sms = dev->sm_count, nkv = a.own.p.kv.nkv;
+    const double tiles = (double)plan.shared.units * nkv * ((max_prefix + 127) / 128) * (plan.shared.rows == 256 ? 2.7 : 2.1);
+    const double own = (double)plan.own.units * nkv * std::max(1, max_len - max_prefix) * 0.5 * a.own.p.kv.hd * 4 / 20e3;
+    int lo = 1, hi = sms;  // fewer CTAs leave more time and more SMs for the own rows
+    while (lo < hi) {
+        const int c = (lo + hi) / 2;
+        if ((sms - c) * (8 + tiles / c) > own) lo = c + 1;
+        else hi = c;
+    }
+    return std::min(lo, a.shared.p.ctas);
+}
+
 template <bool BF16, int HD>
 int part_launch(const Device *dev, const PrefixJoin &a, int shared_ctas, int own_ctas, cudaStream_t st) {
     using S = PtShape<HD>;
@@ -483,11 +499,12 @@ int part_launch(const Device *dev, const PrefixJoin &a, int shared_ctas, int own
 }
 
 template <bool BF16, int HD>
-int run(const Device *dev, PrefixJoin &a, const PrefixPlan &plan, cudaStream_t st) {
+int run(const Device *dev, PrefixJoin &a, const PrefixPlan &plan, int max_prefix, int max_len, cudaStream_t st) {
     const int nkv = a.own.p.kv.nkv;
     int rc = IM_OK, shared_ctas = 0, own_ctas = 0;
     if (plan.shared.units > 0) {
         if (plan.shared.tc) {
+            if (!plan.own.tc) a.shared.p.ctas = shared_ctas_beside(dev, a, plan, max_prefix, max_len);
             rc = paged_tc_part_launch(dev, a.shared.p, BF16, kShared, plan.shared.rows, plan.shared.units, st);
             a.own.p.early = 1;
         } else {
@@ -554,7 +571,7 @@ IM_EXPORT int im_cuda_paged_prefix_attention(im_device *dev, const im_paged_kv *
     lay_out(&a.own, plan.own, max_len, num_groups ? std::max(1, max_len - max_prefix) : max_len, at);
     const cudaStream_t st = as_stream(stream);
     const bool bf16 = kv->dtype == IM_DTYPE_BF16;
-#define IM_RUN(HD) (bf16 ? run<true, HD>(dev, a, plan, st) : run<false, HD>(dev, a, plan, st))
+#define IM_RUN(HD) (bf16 ? run<true, HD>(dev, a, plan, max_prefix, max_len, st) : run<false, HD>(dev, a, plan, max_prefix, max_len, st))
     switch (kv->head_dim) {
     case 64: return IM_RUN(64);
     case 128: return IM_RUN(128);
