@@ -125,12 +125,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     __syncthreads();
     fence_after();
     const uint32_t tmem = uniform(*tmem_slot);
-    if constexpr (MODE == kShared) {
-        pdl_wait();     // what starts behind the trigger finds everything before this launch done
-        pdl_trigger();
+    if constexpr (MODE == kShared || MODE == kOwn) {
+        if (MODE == kShared || !p.early) pdl_wait();
+        pdl_trigger();  // what starts behind it finds everything before the call done
     } else {
         pdl_trigger();  // after the allocation: a successor on this SM cannot take the columns first
-        if (MODE != kOwn || !p.early) pdl_wait();
+        pdl_wait();
     }
     PagedUnit at;
     const Share share = units <= 32 ? warp_share<R, kTcTile, MODE>(p, units, at) : find_share<R, kTcTile, kTcThreads, MODE>(p, units, reinterpret_cast<long long *>(Qs), at);  // (the copies start behind its last barrier)

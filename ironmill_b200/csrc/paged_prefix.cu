@@ -247,8 +247,8 @@ __global__ void __launch_bounds__(kPtThreads, HD == 256 ? 2 : 3) paged_part_kern
     extern __shared__ __align__(128) unsigned char pt_smem[];
     __shared__ float2 ml[kPtWarps * kPtRows];
     __shared__ unsigned bad_rows;
-    pdl_trigger();
     if (!a.own.p.early) pdl_wait();
+    pdl_trigger();  // (the join looks up what this call was given before it waits)
     const int b = blockIdx.x;
     if (b < shared_ctas) {
         part_of_item<BF16, HD, kShared>(a.shared, b / a.shared.chunks, b % a.shared.chunks, pt_smem, ml, bad_rows);
@@ -261,24 +261,29 @@ __global__ void __launch_bounds__(kPtThreads, HD == 256 ? 2 : 3) paged_part_kern
 
 // ------------------------------------------------------------------------------------------------ the join
 // A block takes eight rows (token, query head of one KV head, token-major), a thread four columns of one: eight rows of a column quad lie side by side in the parts of
-// paged_attn_tc.cu. Eight lanes look the rows up, then lanes the parts' maxima and sums, 32 parts at a time; factors go to shared memory.
+// paged_attn_tc.cu. What bounds it is the chain of lookups, so eight lanes find their rows' units before the launches in front of this one are done (those trigger it when
+// everything before the call is), then places of parts, then 32 parts at a time of both sets: maxima and sums a lane each, factors to shared memory, values.
 constexpr int kPjRows = 8, kPjParts = 32;
 struct PjRow {
     int token;                // -1: not to be written
     long long out;
-    int slot0[2], next[2], parts[2], r[2];  // shared, own: slot of the first part, of the second less two (tcgen05) or one, number of parts, row of the tile
-    int unit[2];              // -1: no parts
+    int unit[2], r[2];        // shared, own: the unit (-1: no parts) and row of its tile
+    int slot0[2], next[2], parts[2];  // slot of the first part, of the others less their steps, number of parts
 };
 
-template <bool BF16, int HD, int MODE>
-__device__ __forceinline__ void find_parts(const PartSet &s, int unit, int head, int r, PjRow &x) {
+template <int HD, int MODE>
+__device__ __forceinline__ void find_unit(const PartSet &s, int unit, int r, PjRow &x) {
     constexpr int w = MODE == kOwn;
     const PagedUnit u = paged_unit_of<MODE>(s.p, unit, s.rows);
     const int from = unit_from<MODE>(u);
     if (r >= u.rows || u.end <= from) return;
     x.r[w] = r;
     x.unit[w] = unit;
-    const long long item = (long long)unit * s.p.kv.nkv + head;
+    x.parts[w] = min(s.chunks, (u.end - from + PtShape<HD>::kChunk - 1) / PtShape<HD>::kChunk);  // (where it is not by tcgen05)
+}
+__device__ __forceinline__ void find_parts(const PartSet &s, int w, int head, PjRow &x) {
+    if (x.unit[w] < 0) return;
+    const long long item = (long long)x.unit[w] * s.p.kv.nkv + head;
     if (s.tc) {
         const int2 span = *reinterpret_cast<const int2 *>(s.p.spans + 2 * item);
         x.slot0[w] = span.x;
@@ -286,9 +291,9 @@ __device__ __forceinline__ void find_parts(const PartSet &s, int unit, int head,
         x.parts[w] = span.x >= s.p.whole_slot ? 1 : span.y - (span.x >> 1) + 1;
     } else {
         x.slot0[w] = x.next[w] = (int)(item * s.chunks);
-        x.parts[w] = min(s.chunks, (u.end - from + PtShape<HD>::kChunk - 1) / PtShape<HD>::kChunk);
     }
 }
+__device__ __forceinline__ size_t slot_of(const PartSet &s, int w, const PjRow &x, int part) { return part == 0 ? x.slot0[w] : x.next[w] + part * (s.tc ? 2 : 1); }
 
 template <bool BF16, int HD>
 __global__ void __launch_bounds__(2 * HD) paged_prefix_join_kernel(const __grid_constant__ PrefixJoin a) {
@@ -298,17 +303,15 @@ __global__ void __launch_bounds__(2 * HD) paged_prefix_join_kernel(const __grid_
     __shared__ float2 state[kPjRows];  // maximum and sum so far
     __shared__ float corr[kPjRows];
     __shared__ float again[kPjRows][HD];
-    __shared__ int more[2], odd;
+    __shared__ int most, odd;
     pdl_trigger();
-    pdl_wait();
     const PagedAttn &p = a.own.p;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, head = blockIdx.y;
-    if (tid < kPjRows) {  // a lane per row: the lookups are many instructions
+    PjRow x;
+    x.token = x.unit[0] = x.unit[1] = -1;
+    x.parts[0] = x.parts[1] = 0;
+    if (tid < kPjRows) {  // a lane per row
         const long long at = (long long)blockIdx.x * kPjRows + tid;
-        PjRow x;
-        x.token = -1;
-        x.parts[0] = x.parts[1] = 0;
-        x.unit[0] = x.unit[1] = -1;
         const int token = (int)min(at / p.group, (long long)INT_MAX), hq = (int)(at - (long long)token * p.group);
         if (token < p.tokens && token >= __ldg(p.start) && token < __ldg(p.start + p.kv.nseq)) {
             int seq = 0;  // the last that starts at or before the token
@@ -326,59 +329,63 @@ __global__ void __launch_bounds__(2 * HD) paged_prefix_join_kernel(const __grid_
                     x.out = token * p.os + (long long)(head * p.group + hq) * HD;
                     if (group >= 0) {
                         const int row = (int)place * p.group + hq, tile = row / a.shared.rows;
-                        find_parts<BF16, HD, kShared>(a.shared, group * a.shared.p.row_tiles + tile, head, row - tile * a.shared.rows, x);
+                        find_unit<HD, kShared>(a.shared, group * a.shared.p.row_tiles + tile, row - tile * a.shared.rows, x);
                     }
                     const int row = t * p.group + hq, tile = row / a.own.rows;
-                    find_parts<BF16, HD, kOwn>(a.own, seq * p.row_tiles + tile, head, row - tile * a.own.rows, x);
+                    find_unit<HD, kOwn>(a.own, seq * p.row_tiles + tile, row - tile * a.own.rows, x);
                 }
             }
         }
+    }
+    pdl_wait();
+    if (tid < kPjRows) {
+        find_parts(a.shared, 0, head, x);
+        find_parts(a.own, 1, head, x);
         rows[tid] = x;
-        const int shared = __reduce_max_sync((1u << kPjRows) - 1, x.parts[0]), own = __reduce_max_sync((1u << kPjRows) - 1, x.parts[1]);
-        if (tid == 0) more[0] = shared, more[1] = own, odd = 0;
         state[tid] = make_float2(-INFINITY, 0.0f);
+        const int n = __reduce_max_sync((1u << kPjRows) - 1, x.parts[0] + x.parts[1]);
+        if (tid == 0) most = n, odd = 0;
     }
     __syncthreads();
     const int r = tid % kPjRows, q = tid / kPjRows;  // this thread's row and columns 4 q ..
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const size_t pitch0 = a.shared.tc ? (size_t)a.shared.rows * 4 : 4, pitch1 = a.own.tc ? (size_t)a.own.rows * 4 : 4;
+    const float *base0 = a.shared.p.part_o + rows[r].r[0] * (a.shared.tc ? 4 : HD) + q * pitch0, *base1 = p.part_o + rows[r].r[1] * (a.own.tc ? 4 : HD) + q * pitch1;
+    const int parts0 = rows[r].parts[0], parts = parts0 + rows[r].parts[1];
 #pragma unroll 1
-    for (int w = 0; w < 2; w++) {
-        const PartSet &s = w ? a.own : a.shared;
-        const int most = more[w], step = s.tc ? 2 : 1;
-        for (int i0 = 0; i0 < most; i0 += kPjParts) {
-            for (int i = warp; i < kPjRows; i += kWarps) {
-                const int part = i0 + lane, n = rows[i].parts[w];
-                float2 x = make_float2(-INFINITY, 0.0f);
-                if (part < n) x = s.p.part_ml[(size_t)(part == 0 ? rows[i].slot0[w] : rows[i].next[w] + part * step) * s.rows + rows[i].r[w]];
-                const bool redo = s.tc && __any_sync(0xffffffffu, x.y != x.y);  // not finite on the tensor cores: the row is done again below
-                const float2 before = state[i];
-                const float top = fmaxf(before.x, warp_max(x.x)), c = before.x == top ? 1.0f : ex2(before.x - top);
-                const float f = x.x == -INFINITY && x.y == 0.0f ? 0.0f : ex2(x.x - top);  // (nothing seen in this part)
-                const float l = before.y * c + warp_sum(x.y * f);
-                factor[i][lane] = f;
-                __syncwarp();
-                if (lane == 0) {
-                    state[i] = make_float2(top, l);
-                    corr[i] = c;
-                    if (redo) atomicOr(&odd, 1 << i);
-                }
+    for (int i0 = 0; i0 < most; i0 += kPjParts) {
+        for (int i = warp; i < kPjRows; i += kWarps) {
+            const PjRow &y = rows[i];
+            const int part = i0 + lane, w = part >= y.parts[0], k = w ? part - y.parts[0] : part;
+            const PartSet &s = w ? a.own : a.shared;
+            float2 ml = make_float2(-INFINITY, 0.0f);
+            if (part < y.parts[0] + y.parts[1]) ml = s.p.part_ml[slot_of(s, w, y, k) * s.rows + y.r[w]];
+            const bool redo = __any_sync(0xffffffffu, s.tc && ml.y != ml.y);  // not finite on the tensor cores: the row is done again below
+            const float2 before = state[i];
+            const float top = fmaxf(before.x, warp_max(ml.x)), c = before.x == top ? 1.0f : ex2(before.x - top);
+            const float f = ml.x == -INFINITY && ml.y == 0.0f ? 0.0f : ex2(ml.x - top);  // (nothing seen in this part)
+            const float l = before.y * c + warp_sum(ml.y * f);
+            factor[i][lane] = f;
+            __syncwarp();
+            if (lane == 0) {
+                state[i] = make_float2(top, l);
+                corr[i] = c;
+                if (redo) atomicOr(&odd, 1 << i);
             }
-            __syncthreads();
-            const float c = corr[r];
-            o = make_float4(o.x * c, o.y * c, o.z * c, o.w * c);
-            const PjRow &x = rows[r];
-            const int n = min(x.parts[w] - i0, kPjParts);
-            const size_t pitch = s.tc ? (size_t)s.rows * 4 : 4, first = s.tc ? (size_t)x.r[w] * 4 + q * pitch : (size_t)x.r[w] * HD + q * pitch;
-#pragma unroll 6
-            for (int i = 0; i < n; i++) {
-                const int part = i0 + i;
-                const size_t slot = part == 0 ? x.slot0[w] : x.next[w] + part * step;
-                const float4 v = *reinterpret_cast<const float4 *>(s.p.part_o + slot * s.rows * HD + first);
-                const float f = factor[r][i];
-                if (f != 0.0f) o.x += v.x * f, o.y += v.y * f, o.z += v.z * f, o.w += v.w * f;
-            }
-            __syncthreads();
         }
+        __syncthreads();
+        const float c = corr[r];
+        o = make_float4(o.x * c, o.y * c, o.z * c, o.w * c);
+        const int n = min(parts - i0, kPjParts);
+#pragma unroll 8
+        for (int i = 0; i < n; i++) {
+            const int part = i0 + i;
+            const float4 v = *reinterpret_cast<const float4 *>(part < parts0 ? base0 + slot_of(a.shared, 0, rows[r], part) * a.shared.rows * HD
+                                                                               : base1 + slot_of(a.own, 1, rows[r], part - parts0) * a.own.rows * HD);
+            const float f = factor[r][i];
+            if (f != 0.0f) o.x += v.x * f, o.y += v.y * f, o.z += v.z * f, o.w += v.w * f;
+        }
+        __syncthreads();
     }
     // ---- rows with sums on the tensor cores that are not finite: both sets again, from the positions that the row sees alone
     for (int w = 0; w < 2 && odd; w++) {
