@@ -336,11 +336,17 @@ int im_cuda_paged_append(im_device *dev, const im_paged_kv *kv, int layer, const
  * num_axes 1 to 4.  More than one (time, height and width of images and video): position_dev [num_axes, num_tokens], and pair_axis_host [rotary_dim / 2] (read during
  * the call) names the axis of every pair: pair i is rotated by entry i of the row of that axis's position.  A token with a row outside the table on any
  * axis is neither written nor rotated.  One axis: as above, pair_axis_host is not read.  q_out_dev lies over none of the weights, tables and positions. */
-int im_cuda_paged_append_normed(im_device *dev, const im_paged_kv *kv, int layer, const void *k_dev, int64_t k_stride, const void *v_dev, int64_t v_stride,
-                                const int *token_start_dev, int num_tokens, const void *q_dev, int64_t q_stride, void *q_out_dev, int64_t q_out_stride,
-                                int num_heads, const void *cos_dev, const void *sin_dev, int table_dtype, int max_pos, int rotary_dim, int neighbours,
-                                const int *position_dev, const void *q_norm_dev, const void *k_norm_dev, int norm_dtype, float eps,
-                                const uint8_t *pair_axis_host, int num_axes, void *stream);
+typedef struct im_paged_append_args { /* as the arguments of paged_append; clear it before filling it */
+    const void *k_dev, *v_dev, *q_dev;
+    void *q_out_dev;
+    const int *token_start_dev, *position_dev;
+    const void *cos_dev, *sin_dev, *q_norm_dev, *k_norm_dev;
+    const uint8_t *pair_axis_host;
+    int64_t k_stride, v_stride, q_stride, q_out_stride;
+    int layer, num_tokens, num_heads, table_dtype, max_pos, rotary_dim, neighbours, norm_dtype, num_axes;
+    float eps;
+} im_paged_append_args;
+int im_cuda_paged_append_normed(im_device *dev, const im_paged_kv *kv, const im_paged_append_args *args, void *stream);
 
 /* out[t, h] = softmax(scale * q[t, h] . K^T) V of the new tokens, whose own rows are in the cache already.  Head h reads KV head
  * h / (num_heads / num_kv_heads).  A token sees all seq_len rows before the new ones, and of the new rows: without a mask its own and
@@ -365,10 +371,23 @@ int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int layer, co
  * the other; max_group_new: no group has more (further ones are left as they are).  max_prefix: no group shares more rows (0: the table's width), max_len: as above; smaller
  * values cost time, not results.  Weights enter their product as in paged_attention, by the rows of a group for the shared pages. */
 size_t im_cuda_paged_prefix_attention_scratch_bytes(const im_device *dev, const im_paged_kv *kv, int num_heads, int max_new, int num_groups, int max_group_new);
-int im_cuda_paged_prefix_attention(im_device *dev, const im_paged_kv *kv, int layer, const void *q_dev, int64_t q_stride, void *out_dev, int64_t out_stride,
-                                   int num_heads, const int *token_start_dev, int num_tokens, int max_new, const int *group_start_dev, int num_groups,
-                                   int max_group_new, const int *prefix_pages_dev, int max_prefix, const uint64_t *mask_dev, int mask_words, float scale,
-                                   int max_len, void *scratch_dev, size_t scratch_bytes, void *stream);
+typedef struct im_paged_attention_args { /* as the arguments of paged_attention; clear it before filling it */
+    const void *q_dev;
+    void *out_dev;
+    const int *token_start_dev;
+    const uint64_t *mask_dev;
+    void *scratch_dev;
+    size_t scratch_bytes;
+    int64_t q_stride, out_stride;
+    int layer, num_heads, num_tokens, max_new, mask_words, max_len;
+    float scale;
+} im_paged_attention_args;
+typedef struct im_paged_prefix_args {
+    im_paged_attention_args attention;
+    const int *group_start_dev, *prefix_pages_dev;
+    int num_groups, max_group_new, max_prefix;
+} im_paged_prefix_args;
+int im_cuda_paged_prefix_attention(im_device *dev, const im_paged_kv *kv, const im_paged_prefix_args *args, void *stream);
 
 /* paged_attention that also adds up what the rows of the cache are worth: weights[s, g, r] += sum of the softmax weights of row r over the call's new tokens of
  * sequence s and the query heads of KV head g; a new token's own row starts with this call's sum, whatever was there.  f32, in the same order on every run: a repeated call on
@@ -377,10 +396,13 @@ int im_cuda_paged_prefix_attention(im_device *dev, const im_paged_kv *kv, int la
  * nothing that is read.  Up to 16 rows (max_new * num_heads / num_kv_heads) the scratch grows with max_len (4 bytes a row and position, up to 256 MB): say what it is.  Scratch of a
  * larger max_len is enough for a smaller one. */
 size_t im_cuda_paged_attention_weights_scratch_bytes(const im_device *dev, const im_paged_kv *kv, int num_heads, int max_new, int max_len);
-int im_cuda_paged_attention_weights(im_device *dev, const im_paged_kv *kv, int layer, const void *q_dev, int64_t q_stride, void *out_dev, int64_t out_stride,
-                                    int num_heads, const int *token_start_dev, int num_tokens, int max_new, const uint64_t *mask_dev, int mask_words,
-                                    float scale, int max_len, float *weights_dev, int64_t seq_stride, int64_t head_stride, int rows, void *scratch_dev,
-                                    size_t scratch_bytes, void *stream);
+typedef struct im_paged_weights_args {
+    im_paged_attention_args attention;
+    float *weights_dev;
+    int64_t seq_stride, head_stride;
+    int rows;
+} im_paged_weights_args;
+int im_cuda_paged_attention_weights(im_device *dev, const im_paged_kv *kv, const im_paged_weights_args *args, void *stream);
 
 /* Eviction by such sums, in every layer.  A sequence of more than `budget` rows keeps the last `recent` of them and, for every layer and KV head on its own, the budget - recent
  * rows before those with the largest weights (ties: the lowest row; NaN counts as -inf).  With H = budget - recent: a kept row below H stays where
@@ -389,9 +411,15 @@ int im_cuda_paged_attention_weights(im_device *dev, const im_paged_kv *kv, int l
  * layers, sequences and heads apart by their strides; weights_out gets the sums of the rows where they lie now (and of sequences that fit, as they are), entries from the new
  * length on are left as they are.  seq_len_out_dev [num_seqs]: min(seq_len, budget).  A sequence's pages up to its length are its own (not shared with another).  A row that is
  * not there is not moved, nor is one moved to a place that is not there.  Page tables of up to 2^19 rows.  weights_out and seq_len_out lie over nothing that is read, nor over each other. */
-int im_cuda_paged_evict(im_device *dev, const im_paged_kv *kv, const float *weights_dev, int64_t layer_stride, int64_t seq_stride, int64_t head_stride, int budget,
-                        int recent, float *weights_out_dev, int64_t out_layer_stride, int64_t out_seq_stride, int64_t out_head_stride, int *seq_len_out_dev,
-                        void *stream);
+typedef struct im_paged_evict_args {
+    const float *weights_dev;
+    float *weights_out_dev;
+    int *seq_len_out_dev;
+    int64_t layer_stride, seq_stride, head_stride;             /* of weights */
+    int64_t out_layer_stride, out_seq_stride, out_head_stride; /* of weights_out */
+    int budget, recent;
+} im_paged_evict_args;
+int im_cuda_paged_evict(im_device *dev, const im_paged_kv *kv, const im_paged_evict_args *args, void *stream);
 
 /* The accepted path of a tree: in every layer row seq_len + accepted_dev[s, j] becomes row seq_len + j, j = 0 .. count_dev[s] - 1
  * (accepted [num_seqs, max_accept], each path in order from the root: accepted[s, j] >= j; an entry below j is not moved).

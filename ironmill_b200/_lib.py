@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libironmill_cuda.so")
@@ -45,14 +46,14 @@ _P, _I, _L, _F, _Z = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
 # Calls between two forwards are short: with their argument types known, plain numbers and addresses are passed.
 _ARGTYPES = {
     "im_cuda_paged_append": (_P, _P, _I, _P, _L, _P, _L, _P, _I, _P, _L, _P, _L, _I, _P, _P, _I, _I, _I, _I, _P, _P),
-    "im_cuda_paged_append_normed": (_P, _P, _I, _P, _L, _P, _L, _P, _I, _P, _L, _P, _L, _I, _P, _P, _I, _I, _I, _I, _P, _P, _P, _I, _F, _P, _I, _P),
+    "im_cuda_paged_append_normed": (_P, _P, _P, _P),
     "im_cuda_paged_attention_scratch_bytes": (_P, _P, _I, _I, _I),
     "im_cuda_paged_attention": (_P, _P, _I, _P, _L, _P, _L, _I, _P, _I, _I, _P, _I, _F, _I, _P, _Z, _P),
     "im_cuda_paged_prefix_attention_scratch_bytes": (_P, _P, _I, _I, _I, _I),
-    "im_cuda_paged_prefix_attention": (_P, _P, _I, _P, _L, _P, _L, _I, _P, _I, _I, _P, _I, _I, _P, _I, _P, _I, _F, _I, _P, _Z, _P),
+    "im_cuda_paged_prefix_attention": (_P, _P, _P, _P),
     "im_cuda_paged_attention_weights_scratch_bytes": (_P, _P, _I, _I, _I),
-    "im_cuda_paged_attention_weights": (_P, _P, _I, _P, _L, _P, _L, _I, _P, _I, _I, _P, _I, _F, _I, _P, _L, _L, _I, _P, _Z, _P),
-    "im_cuda_paged_evict": (_P, _P, _P, _L, _L, _L, _I, _I, _P, _L, _L, _L, _P, _P),
+    "im_cuda_paged_attention_weights": (_P, _P, _P, _P),
+    "im_cuda_paged_evict": (_P, _P, _P, _P),
     "im_cuda_paged_keep": (_P, _P, _P, _I, _P, _P, _P),
     "im_cuda_paged_reorder": (_P, _P, _P, _I, _P, _L, _P, _P),
     "im_cuda_beam_select_scratch_bytes": (_P, _I, _I, _I, _I),
@@ -88,6 +89,14 @@ def lib() -> C.CDLL:
             if hasattr(_lib, name):
                 getattr(_lib, name).restype = None
     return _lib
+
+
+# Arguments that a call takes in a struct (im_paged_append_args and so on, include/ironmill_cuda.h): packing them is a fraction of what ctypes takes to convert as many
+# arguments one by one. NULL is 0.
+APPEND_ARGS = struct.Struct("11P4q9if")
+PREFIX_ARGS = struct.Struct("5PN2q6if4x2P3i4x")
+WEIGHTS_ARGS = struct.Struct("5PN2q6if4xP2qi4x")
+EVICT_ARGS = struct.Struct("3P6q2i")
 
 
 class PagedKvStruct(C.Structure):

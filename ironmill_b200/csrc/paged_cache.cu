@@ -631,39 +631,37 @@ IM_EXPORT int im_cuda_paged_append(im_device *dev, const im_paged_kv *kv, int la
     IM_GUARD_END
 }
 
-IM_EXPORT int im_cuda_paged_append_normed(im_device *dev, const im_paged_kv *kv, int layer, const void *k_dev, int64_t k_stride, const void *v_dev, int64_t v_stride,
-                                          const int *token_start_dev, int num_tokens, const void *q_dev, int64_t q_stride, void *q_out_dev, int64_t q_out_stride,
-                                          int num_heads, const void *cos_dev, const void *sin_dev, int table_dtype, int max_pos, int rotary_dim, int neighbours,
-                                          const int *position_dev, const void *q_norm_dev, const void *k_norm_dev, int norm_dtype, float eps, const uint8_t *pair_axis_host,
-                                          int num_axes, void *stream) {
+IM_EXPORT int im_cuda_paged_append_normed(im_device *dev, const im_paged_kv *kv, const im_paged_append_args *args, void *stream) {
     IM_GUARD_BEGIN
     using namespace im;
-    IM_REQUIRE(!q_norm_dev || q_dev, "norm weights of queries without queries");
-    IM_REQUIRE((!q_norm_dev && !k_norm_dev) || (kv && (norm_dtype == IM_DTYPE_F32 || norm_dtype == kv->dtype)), "norm weights are of the cache's type or f32 (got dtype %d)", norm_dtype);
-    IM_REQUIRE(aligned16(q_norm_dev) && aligned16(k_norm_dev), "norm weights have to be 16-byte aligned");
-    IM_REQUIRE(eps >= 0.0f && eps - eps == 0.0f, "eps has to be finite and not negative");
-    IM_REQUIRE(num_axes >= 1 && num_axes <= kAxes, "%d axes (at most %d)", num_axes, kAxes);
-    IM_REQUIRE(num_axes == 1 || (rotary_dim > 0 && position_dev && pair_axis_host), "several axes need a rotation, positions and the axis of every pair");
+    IM_REQUIRE(kv && args, "kv or args is NULL");
+    const im_paged_append_args &x = *args;
+    IM_REQUIRE(!x.q_norm_dev || x.q_dev, "norm weights of queries without queries");
+    IM_REQUIRE((!x.q_norm_dev && !x.k_norm_dev) || x.norm_dtype == IM_DTYPE_F32 || x.norm_dtype == kv->dtype, "norm weights are of the cache's type or f32 (got dtype %d)", x.norm_dtype);
+    IM_REQUIRE(aligned16(x.q_norm_dev) && aligned16(x.k_norm_dev), "norm weights have to be 16-byte aligned");
+    IM_REQUIRE(x.eps >= 0.0f && x.eps - x.eps == 0.0f, "eps has to be finite and not negative");
+    IM_REQUIRE(x.num_axes >= 1 && x.num_axes <= kAxes, "%d axes (at most %d)", x.num_axes, kAxes);
+    IM_REQUIRE(x.num_axes == 1 || (x.rotary_dim > 0 && x.position_dev && x.pair_axis_host), "several axes need a rotation, positions and the axis of every pair");
     Append a;
     bool empty;
-    const int rc = append_args(dev, kv, layer, k_dev, k_stride, v_dev, v_stride, token_start_dev, num_tokens, q_dev, q_stride, q_out_dev, q_out_stride, num_heads, cos_dev, sin_dev,
-                               table_dtype, max_pos, rotary_dim, neighbours, position_dev, &a, &empty);
+    const int rc = append_args(dev, kv, x.layer, x.k_dev, x.k_stride, x.v_dev, x.v_stride, x.token_start_dev, x.num_tokens, x.q_dev, x.q_stride, x.q_out_dev, x.q_out_stride, x.num_heads,
+                               x.cos_dev, x.sin_dev, x.table_dtype, x.max_pos, x.rotary_dim, x.neighbours, x.position_dev, &a, &empty);
     if (rc != IM_OK || empty) return rc;
     AppendMore m{};
-    m.qn = q_norm_dev; m.kn = k_norm_dev;
-    m.norm_f32 = norm_dtype == IM_DTYPE_F32;
-    m.axes = num_axes;
-    m.neighbours = neighbours;
-    m.eps = eps;
+    m.qn = x.q_norm_dev; m.kn = x.k_norm_dev;
+    m.norm_f32 = x.norm_dtype == IM_DTYPE_F32;
+    m.axes = x.num_axes;
+    m.neighbours = x.neighbours;
+    m.eps = x.eps;
     m.inv_dim = 1.0f / kv->head_dim;
-    for (int i = 0; num_axes > 1 && i < rotary_dim / 2; i++) {
-        IM_REQUIRE(pair_axis_host[i] < num_axes, "pair %d on axis %d of %d", i, pair_axis_host[i], num_axes);
-        m.axis[i / 16] |= (uint32_t)pair_axis_host[i] << (2 * (i % 16));
+    for (int i = 0; x.num_axes > 1 && i < x.rotary_dim / 2; i++) {
+        IM_REQUIRE(x.pair_axis_host[i] < x.num_axes, "pair %d on axis %d of %d", i, x.pair_axis_host[i], x.num_axes);
+        m.axis[i / 16] |= (uint32_t)x.pair_axis_host[i] << (2 * (i % 16));
     }
     const int lanes = append_lanes(kv->head_dim);
-    const bool bf16 = kv->dtype == IM_DTYPE_BF16, f32 = table_dtype == IM_DTYPE_F32;
-    const dim3 grid((unsigned)num_tokens), block(num_tokens > 4 * dev->sm_count ? kAppendSmall : kAppendThreads);
-    if (rotary_dim % 8) {
+    const bool bf16 = kv->dtype == IM_DTYPE_BF16, f32 = x.table_dtype == IM_DTYPE_F32;
+    const dim3 grid((unsigned)x.num_tokens), block(x.num_tokens > 4 * dev->sm_count ? kAppendSmall : kAppendThreads);
+    if (x.rotary_dim % 8) {
         void (*odd)(Append, AppendMore, int) = bf16 ? (f32 ? paged_append_odd_kernel<true, true> : paged_append_odd_kernel<true, false>)
                                                     : (f32 ? paged_append_odd_kernel<false, true> : paged_append_odd_kernel<false, false>);
         IM_CUDA_CHECK(launch_k(odd, grid, block, 0, as_stream(stream), a, m, lanes));
@@ -671,7 +669,7 @@ IM_EXPORT int im_cuda_paged_append_normed(im_device *dev, const im_paged_kv *kv,
     }
     void (*kern)(Append, AppendMore) = nullptr;
 #define IM_LANES(B, N, F) (lanes == 32 ? paged_append_normed_kernel<B, N, F, 32> : lanes == 16 ? paged_append_normed_kernel<B, N, F, 16> : paged_append_normed_kernel<B, N, F, 8>)
-#define IM_FORM(B, F) (neighbours ? IM_LANES(B, true, F) : IM_LANES(B, false, F))
+#define IM_FORM(B, F) (x.neighbours ? IM_LANES(B, true, F) : IM_LANES(B, false, F))
     kern = bf16 ? (f32 ? IM_FORM(true, true) : IM_FORM(true, false)) : (f32 ? IM_FORM(false, true) : IM_FORM(false, false));
 #undef IM_FORM
 #undef IM_LANES

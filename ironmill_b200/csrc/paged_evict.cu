@@ -244,36 +244,36 @@ constexpr int kEvRows = 1 << 19;  // bits and counts of so many rows fit an SM's
 }  // namespace
 }  // namespace im
 
-IM_EXPORT int im_cuda_paged_evict(im_device *dev, const im_paged_kv *kv, const float *weights_dev, int64_t layer_stride, int64_t seq_stride, int64_t head_stride, int budget,
-                                  int recent, float *weights_out_dev, int64_t out_layer_stride, int64_t out_seq_stride, int64_t out_head_stride, int *seq_len_out_dev,
-                                  void *stream) {
+IM_EXPORT int im_cuda_paged_evict(im_device *dev, const im_paged_kv *kv, const im_paged_evict_args *args, void *stream) {
     IM_GUARD_BEGIN
     using namespace im;
+    IM_REQUIRE(args, "args is NULL");
+    const im_paged_evict_args &x = *args;
     Evict a;
     PagedView &v = a.kv;
     int rc = paged_view(kv, -1, &v);
-    if (rc == IM_OK) rc = evict_check(budget, recent);
+    if (rc == IM_OK) rc = evict_check(x.budget, x.recent);
     if (rc != IM_OK) return rc;
-    IM_REQUIRE(v.nseq == 0 || (weights_dev && weights_out_dev && seq_len_out_dev), "bad argument");
+    IM_REQUIRE(v.nseq == 0 || (x.weights_dev && x.weights_out_dev && x.seq_len_out_dev), "bad argument");
     IM_REQUIRE(v.rows <= kEvRows, "eviction takes page tables of up to %d rows (got %d)", kEvRows, v.rows);
     const long long most = 1ll << 40;
     const auto apart = [&](int64_t layer, int64_t seq, int64_t head) {
         return head >= v.rows && head <= most / v.nkv && seq <= most && layer <= most && (v.nseq <= 1 || seq >= (v.nkv - 1) * head + v.rows) &&
                (v.layers == 1 || layer >= (std::max(v.nseq, 1) - 1) * seq + (v.nkv - 1) * head + v.rows) && layer <= most / v.layers && seq <= most / std::max(v.nseq, 1);
     };
-    IM_REQUIRE(apart(layer_stride, seq_stride, head_stride) && apart(out_layer_stride, out_seq_stride, out_head_stride),
+    IM_REQUIRE(apart(x.layer_stride, x.seq_stride, x.head_stride) && apart(x.out_layer_stride, x.out_seq_stride, x.out_head_stride),
                "sums have a row for each of the page table's %d, those of different layers, sequences and heads apart", v.rows);
     const long long problems = (long long)v.layers * v.nseq * v.nkv;
     IM_REQUIRE(problems <= INT_MAX, "too many layers, sequences and heads");
     if (v.nseq > 0) {
-        IM_REQUIRE(reinterpret_cast<uintptr_t>(weights_dev) % 4 == 0 && reinterpret_cast<uintptr_t>(weights_out_dev) % 4 == 0, "the sums are not 4-byte aligned");
+        IM_REQUIRE(reinterpret_cast<uintptr_t>(x.weights_dev) % 4 == 0 && reinterpret_cast<uintptr_t>(x.weights_out_dev) % 4 == 0, "the sums are not 4-byte aligned");
         const auto span = [&](int64_t layer, int64_t seq, int64_t head) { return 4 * ((v.layers - 1) * layer + (v.nseq - 1) * seq + (v.nkv - 1) * head + v.rows); };
-        const long long in = span(layer_stride, seq_stride, head_stride), out = span(out_layer_stride, out_seq_stride, out_head_stride), lens = 4ll * v.nseq,
+        const long long in = span(x.layer_stride, x.seq_stride, x.head_stride), out = span(x.out_layer_stride, x.out_seq_stride, x.out_head_stride), lens = 4ll * v.nseq,
                         table = 4 * ((v.nseq - 1) * v.table_stride + v.width);
-        IM_REQUIRE(!share_memory(weights_out_dev, out, weights_dev, in) && !share_memory(weights_out_dev, out, v.len, lens) && !share_memory(weights_out_dev, out, v.table, table),
+        IM_REQUIRE(!share_memory(x.weights_out_dev, out, x.weights_dev, in) && !share_memory(x.weights_out_dev, out, v.len, lens) && !share_memory(x.weights_out_dev, out, v.table, table),
                    "the new sums lie over what is read");
-        IM_REQUIRE(!share_memory(seq_len_out_dev, lens, weights_dev, in) && !share_memory(seq_len_out_dev, lens, v.len, lens) && !share_memory(seq_len_out_dev, lens, v.table, table) &&
-                       !share_memory(seq_len_out_dev, lens, weights_out_dev, out),
+        IM_REQUIRE(!share_memory(x.seq_len_out_dev, lens, x.weights_dev, in) && !share_memory(x.seq_len_out_dev, lens, v.len, lens) && !share_memory(x.seq_len_out_dev, lens, v.table, table) &&
+                       !share_memory(x.seq_len_out_dev, lens, x.weights_out_dev, out),
                    "the new lengths lie over what is read or the new sums");
     }
     rc = paged_device(dev);
@@ -281,13 +281,13 @@ IM_EXPORT int im_cuda_paged_evict(im_device *dev, const im_paged_kv *kv, const f
     if (v.nseq == 0) return IM_OK;
     a.kc = static_cast<uint4 *>(kv->k_dev);
     a.vc = static_cast<uint4 *>(kv->v_dev);
-    a.w = weights_dev;
-    a.w_out = weights_out_dev;
-    a.w_layer = layer_stride; a.w_seq = seq_stride; a.w_head = head_stride;
-    a.o_layer = out_layer_stride; a.o_seq = out_seq_stride; a.o_head = out_head_stride;
-    a.budget = budget;
-    a.recent = recent;
-    a.len_out = seq_len_out_dev;
+    a.w = x.weights_dev;
+    a.w_out = x.weights_out_dev;
+    a.w_layer = x.layer_stride; a.w_seq = x.seq_stride; a.w_head = x.head_stride;
+    a.o_layer = x.out_layer_stride; a.o_seq = x.out_seq_stride; a.o_head = x.out_head_stride;
+    a.budget = x.budget;
+    a.recent = x.recent;
+    a.len_out = x.seq_len_out_dev;
     // A block all of a row where there are many (layer, sequence, head), down to 32 bytes of it where there are few
     const int per_row = v.hd / 8;
     a.cols = 2 * per_row;

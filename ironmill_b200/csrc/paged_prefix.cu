@@ -545,36 +545,34 @@ IM_EXPORT size_t im_cuda_paged_prefix_attention_scratch_bytes(const im_device *d
     }
 }
 
-IM_EXPORT int im_cuda_paged_prefix_attention(im_device *dev, const im_paged_kv *kv, int layer, const void *q_dev, int64_t q_stride, void *out_dev, int64_t out_stride,
-                                             int num_heads, const int *token_start_dev, int num_tokens, int max_new, const int *group_start_dev, int num_groups,
-                                             int max_group_new, const int *prefix_pages_dev, int max_prefix, const uint64_t *mask_dev, int mask_words, float scale, int max_len,
-                                             void *scratch_dev, size_t scratch_bytes, void *stream) {
+IM_EXPORT int im_cuda_paged_prefix_attention(im_device *dev, const im_paged_kv *kv, const im_paged_prefix_args *args, void *stream) {
     IM_GUARD_BEGIN
     using namespace im;
     PrefixJoin a;
     PagedAttn &p = a.own.p;
-    IM_REQUIRE(kv && kv->num_kv_heads > 0, "kv is NULL or has no heads");
+    IM_REQUIRE(kv && args && kv->num_kv_heads > 0, "kv or args is NULL, or there are no heads");
+    const im_paged_attention_args &x = args->attention;
+    const int num_heads = x.num_heads, num_groups = args->num_groups, max_group_new = args->max_group_new;
     int rc = prefix_check(kv, num_heads, num_groups, max_group_new);
     if (rc != IM_OK) return rc;
-    IM_REQUIRE(num_groups == 0 || (group_start_dev && prefix_pages_dev), "groups need their first sequences and numbers of shared pages");
-    IM_REQUIRE(max_prefix >= 0, "max_prefix %d", max_prefix);
+    IM_REQUIRE(num_groups == 0 || (args->group_start_dev && args->prefix_pages_dev), "groups need their first sequences and numbers of shared pages");
+    IM_REQUIRE(args->max_prefix >= 0, "max_prefix %d", args->max_prefix);
     bool empty;
-    rc = attn_args(dev, kv, layer, q_dev, q_stride, out_dev, out_stride, num_heads, token_start_dev, num_tokens, max_new, mask_dev, mask_words, scale, max_len, &p, &empty);
+    rc = attn_args(dev, kv, x.layer, x.q_dev, x.q_stride, x.out_dev, x.out_stride, num_heads, x.token_start_dev, x.num_tokens, x.max_new, x.mask_dev, x.mask_words, x.scale, x.max_len, &p, &empty);
     if (rc != IM_OK || empty) return rc;
     IM_REQUIRE(kv->num_kv_heads <= 65535, "at most 65535 key / value heads (got %d)", kv->num_kv_heads);
-    const PrefixPlan plan = prefix_plan(dev, p.kv, p.group, max_new, num_groups, max_group_new);
-    IM_REQUIRE(scratch_dev && aligned16(scratch_dev) && scratch_bytes >= plan.bytes, "paged prefix attention needs %zu bytes of 16-byte aligned scratch (got %zu)", plan.bytes,
-               scratch_dev ? scratch_bytes : (size_t)0);
-    max_len = attn_length(p.kv, max_len);
-    max_prefix = std::min(attn_length(p.kv, max_prefix), max_len);
-    p.group_start = group_start_dev;
-    p.prefix_pages = prefix_pages_dev;
+    const PrefixPlan plan = prefix_plan(dev, p.kv, p.group, x.max_new, num_groups, max_group_new);
+    IM_REQUIRE(x.scratch_dev && aligned16(x.scratch_dev) && x.scratch_bytes >= plan.bytes, "paged prefix attention needs %zu bytes of 16-byte aligned scratch (got %zu)", plan.bytes,
+               x.scratch_dev ? x.scratch_bytes : (size_t)0);
+    const int max_len = attn_length(p.kv, x.max_len), max_prefix = std::min(attn_length(p.kv, args->max_prefix), max_len);
+    p.group_start = args->group_start_dev;
+    p.prefix_pages = args->prefix_pages_dev;
     p.groups = num_groups;
     a.shared.p = p;
     a.shared.p.mask = nullptr;
     a.shared.p.max_new = max_group_new;
     a.group_new = max_group_new;
-    unsigned char *at = lay_out(&a.shared, plan.shared, max_prefix, max_prefix, static_cast<unsigned char *>(scratch_dev));
+    unsigned char *at = lay_out(&a.shared, plan.shared, max_prefix, max_prefix, static_cast<unsigned char *>(x.scratch_dev));
     lay_out(&a.own, plan.own, max_len, num_groups ? std::max(1, max_len - max_prefix) : max_len, at);
     const cudaStream_t st = as_stream(stream);
     const bool bf16 = kv->dtype == IM_DTYPE_BF16;

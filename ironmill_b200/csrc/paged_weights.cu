@@ -411,31 +411,35 @@ IM_EXPORT size_t im_cuda_paged_attention_weights_scratch_bytes(const im_device *
     }
 }
 
-IM_EXPORT int im_cuda_paged_attention_weights(im_device *dev, const im_paged_kv *kv, int layer, const void *q_dev, int64_t q_stride, void *out_dev, int64_t out_stride,
-                                              int num_heads, const int *token_start_dev, int num_tokens, int max_new, const uint64_t *mask_dev, int mask_words, float scale,
-                                              int max_len, float *weights_dev, int64_t seq_stride, int64_t head_stride, int rows, void *scratch_dev, size_t scratch_bytes,
-                                              void *stream) {
+IM_EXPORT int im_cuda_paged_attention_weights(im_device *dev, const im_paged_kv *kv, const im_paged_weights_args *args, void *stream) {
     IM_GUARD_BEGIN
     using namespace im;
     PagedAttn p;
     bool empty;
-    IM_REQUIRE(kv && kv->num_kv_heads > 0, "kv is NULL or has no heads");
+    IM_REQUIRE(kv && args && kv->num_kv_heads > 0, "kv or args is NULL, or there are no heads");
+    const im_paged_attention_args &x = args->attention;
+    const int rows = args->rows;
+    const int64_t seq_stride = args->seq_stride, head_stride = args->head_stride;
+    float *const weights_dev = args->weights_dev;
     const int64_t most = (int64_t)1 << 40;
     IM_REQUIRE(rows >= 1 && head_stride >= rows && head_stride <= most && seq_stride <= most && head_stride <= most / kv->num_kv_heads &&
                    (kv->num_seqs <= 1 || seq_stride >= (kv->num_kv_heads - 1) * head_stride + rows),
                "sums of different sequences and heads overlap");
-    int rc = attn_args(dev, kv, layer, q_dev, q_stride, out_dev, out_stride, num_heads, token_start_dev, num_tokens, max_new, mask_dev, mask_words, scale, max_len, &p, &empty);
+    if (x.num_tokens > 0 && kv->num_seqs > 0) {
+        IM_REQUIRE(weights_dev && reinterpret_cast<uintptr_t>(weights_dev) % 4 == 0, "the sums are NULL or not 4-byte aligned");
+        const long long span = 4 * ((kv->num_seqs - 1) * (long long)seq_stride + (kv->num_kv_heads - 1) * head_stride + rows), row = 2ll * x.num_heads * kv->head_dim;
+        IM_REQUIRE(!share_memory(weights_dev, span, x.q_dev, 2 * (x.num_tokens - 1) * (long long)x.q_stride + row) && !share_memory(weights_dev, span, x.out_dev, 2 * (x.num_tokens - 1) * (long long)x.out_stride + row),
+                   "the sums lie over the queries or the outputs");
+    }
+    int rc = attn_args(dev, kv, x.layer, x.q_dev, x.q_stride, x.out_dev, x.out_stride, x.num_heads, x.token_start_dev, x.num_tokens, x.max_new, x.mask_dev, x.mask_words, x.scale, x.max_len, &p,
+                       &empty);
     if (rc != IM_OK || empty) return rc;
-    IM_REQUIRE(weights_dev && reinterpret_cast<uintptr_t>(weights_dev) % 4 == 0, "the sums are NULL or not 4-byte aligned");
-    const long long span = 4 * ((kv->num_seqs - 1) * (long long)seq_stride + (kv->num_kv_heads - 1) * head_stride + rows), row = 2ll * num_heads * kv->head_dim;
-    IM_REQUIRE(!share_memory(weights_dev, span, q_dev, 2 * (num_tokens - 1) * (long long)q_stride + row) && !share_memory(weights_dev, span, out_dev, 2 * (num_tokens - 1) * (long long)out_stride + row),
-               "the sums lie over the queries or the outputs");
-    max_len = attn_length(p.kv, max_len);
-    const WeighPlan plan = weigh_plan(dev, p.kv, p.group, max_new, max_len);
-    IM_REQUIRE(plan.used == 0 || (scratch_dev && aligned16(scratch_dev) && scratch_bytes >= plan.used), "paged attention with sums needs %zu bytes of 16-byte aligned scratch (got %zu)",
-               plan.used, scratch_dev ? scratch_bytes : (size_t)0);
-    attn_lay_out(&p, plan.attn, max_len, scratch_dev);
-    unsigned char *at = static_cast<unsigned char *>(scratch_dev) + plan.attn_bytes;
+    const int max_len = attn_length(p.kv, x.max_len);
+    const WeighPlan plan = weigh_plan(dev, p.kv, p.group, x.max_new, max_len);
+    IM_REQUIRE(plan.used == 0 || (x.scratch_dev && aligned16(x.scratch_dev) && x.scratch_bytes >= plan.used), "paged attention with sums needs %zu bytes of 16-byte aligned scratch (got %zu)",
+               plan.used, x.scratch_dev ? x.scratch_bytes : (size_t)0);
+    attn_lay_out(&p, plan.attn, max_len, x.scratch_dev);
+    unsigned char *at = static_cast<unsigned char *>(x.scratch_dev) + plan.attn_bytes;
     p.stat = reinterpret_cast<float2 *>(at);
     p.scores = plan.cap ? reinterpret_cast<float *>(at + plan.stat_bytes) : nullptr;
     p.score_cap = plan.cap;

@@ -12,7 +12,7 @@ import ctypes as C
 import numpy as np
 import torch
 
-from ._lib import IM_DTYPE_BF16, IM_DTYPE_F16, IM_DTYPE_F32, PagedKvStruct, check, lib, vp
+from ._lib import APPEND_ARGS, EVICT_ARGS, IM_DTYPE_BF16, IM_DTYPE_F16, IM_DTYPE_F32, PREFIX_ARGS, WEIGHTS_ARGS, PagedKvStruct, check, lib, vp
 
 
 def _stream():
@@ -504,27 +504,30 @@ def paged_append(kv: PagedKV, layer: int, k, v, token_start, q=None, cos=None, s
     else:
         assert sin is None and not rotary_dim
         rotary_dim = 0
-    args = (kv.dev.handle, kv.ref, layer, k.data_ptr(), ks, v.data_ptr(), vs, _ints(token_start, on, kv.num_seqs + 1), n, qp, qs, op, qos, heads, cp, sp, table, max_pos, rotary_dim,
-            1 if neighbours else 0)
     if q_norm is None and k_norm is None and pair_axis is None:
-        _launch(on, lib().im_cuda_paged_append, *args, None if positions is None else _ints(positions, on, n))
+        _launch(on, lib().im_cuda_paged_append, kv.dev.handle, kv.ref, layer, k.data_ptr(), ks, v.data_ptr(), vs, _ints(token_start, on, kv.num_seqs + 1), n, qp, qs, op, qos, heads,
+                cp, sp, table, max_pos, rotary_dim, 1 if neighbours else 0, None if positions is None else _ints(positions, on, n))
         return q_out
-    axes, at = 1, None
+    axes, at, of_pair = 1, 0, 0
     if pair_axis is not None:
         axes = positions.shape[0]
         assert len(pair_axis) == rotary_dim // 2, (len(pair_axis), rotary_dim)
-        at, pair_axis = _ints(positions, on, axes, n) if n else None, bytes(pair_axis)
+        at = _ints(positions, on, axes, n) if n else 0
+        if axes > 1:
+            pair_axis = bytes(pair_axis)
+            of_pair = C.cast(pair_axis, C.c_void_p).value
     elif positions is not None:
         at = _ints(positions, on, n)
-    qw = kw = None
-    norm = kind = 0
+    qw = kw = norm = 0
     if q_norm is not None:
         qw, norm = _norm_of(q_norm, dim, dtype, on)
     if k_norm is not None:
         kw, kind = _norm_of(k_norm, dim, dtype, on)
-        assert qw is None or kind == norm, (q_norm.dtype, k_norm.dtype)
+        assert not qw or kind == norm, (q_norm.dtype, k_norm.dtype)
         norm = kind
-    _launch(on, lib().im_cuda_paged_append_normed, *args, at, qw, kw, norm, eps, pair_axis if axes > 1 else None, axes)
+    _launch(on, lib().im_cuda_paged_append_normed, kv.dev.handle, kv.ref,
+            APPEND_ARGS.pack(k.data_ptr(), v.data_ptr(), qp or 0, op or 0, _ints(token_start, on, kv.num_seqs + 1), at, cp or 0, sp or 0, qw, kw, of_pair, ks, vs, qs, qos, layer, n, heads, table,
+                             max_pos, rotary_dim, 1 if neighbours else 0, norm, axes, eps))
     return q_out
 
 
@@ -578,14 +581,14 @@ def _outputs_for(q, out, kv: PagedKV):
     """(tensor, stride) of outputs like q's tokens."""
     n, heads, dim = q.shape
     if out is None:
-        return torch.empty_like(q, memory_format=torch.contiguous_format), heads * dim
+        return torch.empty_like(q) if q.is_contiguous() else torch.empty_like(q, memory_format=torch.contiguous_format), heads * dim
     return out, _rows_of(out, n, heads, dim, kv.dtype, kv.ordinal)
 
 
 def _mask_of(mask, n: int, ordinal: int):
-    """(address, words) of a mask int64 [tokens, words] or None."""
+    """(address, words) of a mask int64 [tokens, words]; 0 where there is none."""
     if mask is None:
-        return None, 0
+        return 0, 0
     assert mask.dim() == 2 and mask.dtype is torch.int64 and mask.shape[0] == n and mask.is_contiguous() and mask.get_device() == ordinal, (mask.shape, mask.dtype)
     return mask.data_ptr(), mask.shape[1]
 
@@ -594,7 +597,7 @@ def _scratch_of(scratch, nbytes: int, kv: PagedKV):
     """(tensor that has to live until the launch, address, bytes) of scratch given or made."""
     if scratch is None:
         if not nbytes:
-            return None, None, 0
+            return None, 0, 0
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=kv.device)
     else:
         assert scratch.dtype is torch.uint8 and scratch.get_device() == kv.ordinal and scratch.is_contiguous()
@@ -623,8 +626,9 @@ def paged_prefix_attention(kv: PagedKV, layer: int, q, token_start, max_new: int
     out, os_ = _outputs_for(q, out, kv)
     mp, words = _mask_of(mask, n, on)
     scratch, at, nbytes = _scratch_of(scratch, _prefix_bytes(kv, heads, max_new, groups, max_group_new) if scratch is None else 0, kv)
-    _launch(on, lib().im_cuda_paged_prefix_attention, kv.dev.handle, kv.ref, layer, q.data_ptr(), qs, out.data_ptr(), os_, heads, _ints(token_start, on, kv.num_seqs + 1), n, max_new,
-            _ints(group_start, on, groups + 1), groups, max_group_new, _ints(prefix_pages, on, groups), max_prefix, mp, words, scale, max_len, at, nbytes)
+    _launch(on, lib().im_cuda_paged_prefix_attention, kv.dev.handle, kv.ref,
+            PREFIX_ARGS.pack(q.data_ptr(), out.data_ptr(), _ints(token_start, on, kv.num_seqs + 1), mp, at, nbytes, qs, os_, layer, heads, n, max_new, words, max_len, scale,
+                             _ints(group_start, on, groups + 1), _ints(prefix_pages, on, groups), groups, max_group_new, max_prefix))
     return out
 
 
@@ -654,8 +658,9 @@ def paged_attention_weights(kv: PagedKV, layer: int, q, token_start, max_new: in
     rows, (ss, sh, sr) = weights.shape[2], weights.stride()
     assert sr == 1 or rows == 1, weights.stride()
     scratch, at, nbytes = _scratch_of(scratch, _weights_bytes(kv, heads, max_new, max_len) if scratch is None else 0, kv)
-    _launch(on, lib().im_cuda_paged_attention_weights, kv.dev.handle, kv.ref, layer, q.data_ptr(), qs, out.data_ptr(), os_, heads, _ints(token_start, on, kv.num_seqs + 1), n, max_new,
-            mp, words, scale, max_len, weights.data_ptr(), ss, sh if kv.kv_heads > 1 else rows, rows, at, nbytes)
+    _launch(on, lib().im_cuda_paged_attention_weights, kv.dev.handle, kv.ref,
+            WEIGHTS_ARGS.pack(q.data_ptr(), out.data_ptr(), _ints(token_start, on, kv.num_seqs + 1), mp, at, nbytes, qs, os_, layer, heads, n, max_new, words, max_len, scale,
+                              weights.data_ptr(), ss, sh if kv.kv_heads > 1 else rows, rows))
     return out
 
 
@@ -678,8 +683,8 @@ def paged_evict(kv: PagedKV, weights, budget: int, recent: int, weights_out=None
         weights_out = torch.empty_like(weights, memory_format=torch.contiguous_format)
     if lengths_out is None:
         lengths_out = torch.empty_like(kv.lengths)
-    _launch(on, lib().im_cuda_paged_evict, kv.dev.handle, kv.ref, weights.data_ptr(), *_sums_of(weights, kv), budget, recent, weights_out.data_ptr(), *_sums_of(weights_out, kv),
-            _ints(lengths_out, on, kv.num_seqs))
+    _launch(on, lib().im_cuda_paged_evict, kv.dev.handle, kv.ref,
+            EVICT_ARGS.pack(weights.data_ptr(), weights_out.data_ptr(), _ints(lengths_out, on, kv.num_seqs), *_sums_of(weights, kv), *_sums_of(weights_out, kv), budget, recent))
     return lengths_out, weights_out
 
 
