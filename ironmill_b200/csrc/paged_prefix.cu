@@ -43,12 +43,13 @@ struct PtShape {
     static constexpr int kPitch = HD + 8;                      // floats of a row of sums in shared memory
     static constexpr int kKeys = kSlices * 16 * HD * 2, kSums = kPtRows * kPitch * 4;
     static constexpr int kWarp = 2 * kKeys > kSums ? 2 * kKeys : kSums;  // sums take the place of keys and values
-    static constexpr int kSmem = kPtWarps * kWarp;
+    static constexpr int kQ = kPtRows * HD * 2;                // queries, behind the warps' places
+    static constexpr int kSmem = kPtWarps * kWarp + kQ;
 };
 
 // Chunks c, c + set.chunks, ... of an item.
 template <bool BF16, int HD, int MODE>
-__device__ __forceinline__ void part_of_item(const PartSet &set, int item, int c, unsigned char *smem, float2 *ml, unsigned &bad_rows) {
+__device__ __forceinline__ void part_of_item(const PartSet &set, int item, int c, unsigned char *smem, long long (*offs)[32], float2 *ml, unsigned &bad_rows) {
     using S = PtShape<HD>;
     constexpr float kLift = BF16 ? 0.0f : 15.0f;  // fp16 weights: 2^15 at the row's maximum, as in paged_attn.cu
     constexpr int R = kPtRows, KS = HD / 16, NT = HD / 8, CH = HD / 8, SL = S::kSlices;
@@ -60,7 +61,11 @@ __device__ __forceinline__ void part_of_item(const PartSet &set, int item, int c
     if (c >= all) return;
     unsigned char *mine = smem + warp * S::kWarp;
     const uint32_t ks_at = smem_u32(mine), vs_at = ks_at + S::kKeys;
-    uint32_t qf[KS][4];
+    const uint32_t q_at = smem_u32(smem + kPtWarps * S::kWarp);
+    for (int i = tid; i < R * CH; i += kPtThreads) {  // queries, on their way with the first keys
+        const int r = i / CH, c8 = i % CH, row = u.row0 + r, t = row / p.group;
+        cp16(q_at + r * (HD * 2) + ((c8 ^ (r & 7)) << 4), p.q + (r < u.rows ? (u.tok0 + t) * p.qs + (long long)(head * p.group + row - t * p.group) * HD + c8 * 8 : 0), r < u.rows);
+    }
     int tok[2];
 #pragma unroll
     for (int i = 0; i < 2; i++) tok[i] = (u.row0 + min((lane >> 2) + 8 * i, u.rows - 1)) / p.group;
@@ -77,47 +82,40 @@ __device__ __forceinline__ void part_of_item(const PartSet &set, int item, int c
         const int pos = pos0 + (lane & (SL * 16 - 1));
         const long long row = pos < u.end ? p.kv.row_of(u.seq, pos) : -1;
         const unsigned there = __ballot_sync(0xffffffffu, row >= 0);
-        const long long off = row < 0 ? -1 : row + (long long)head * p.kv.page * HD;
         constexpr int RPI = 32 / CH > 0 ? 32 / CH : 1;  // rows of one request of the warp
         __syncwarp();  // the chunk before has been read
+        if (lane < SL * 16) offs[warp][lane] = row < 0 ? -1 : row + (long long)head * p.kv.page * HD;
+        __syncwarp();
 #pragma unroll
         for (int kv = 0; kv < 2; kv++) {
 #pragma unroll
             for (int i = 0; i < SL * 16 / RPI; i++) {
                 const int r = i * RPI + (RPI > 1 ? lane / CH : 0), c8 = lane & (CH - 1);
-                const long long at = __shfl_sync(0xffffffffu, off, r);
+                const long long at = offs[warp][r];
                 cp16((kv ? vs_at : ks_at) + r * (HD * 2) + ((c8 ^ (r & 7)) << 4), (kv ? p.vc : p.kc) + (at < 0 ? 0 : at + c8 * 8), at >= 0);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
-        if (first) {  // queries: A fragments, rows lane / 4 and lane / 4 + 8
-            first = false;
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int r = (lane >> 2) + 8 * i;
-                const uint32_t *src = reinterpret_cast<const uint32_t *>(p.q + (u.tok0 + tok[i]) * p.qs + (long long)(head * p.group + (u.row0 + r) % p.group) * HD);
-#pragma unroll
-                for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++) qf[ks][2 * j + i] = r < u.rows ? __ldg(src + ks * 8 + j * 4 + (lane & 3)) : 0u;
-            }
-        }
         asm volatile("cp.async.wait_group 1;" ::: "memory");
-        __syncwarp();
+        if (first) __syncthreads();  // everyone's queries
+        else __syncwarp();
+        first = false;
         float s[2 * SL][4];
 #pragma unroll
         for (int n = 0; n < 2 * SL; n++)
 #pragma unroll
             for (int j = 0; j < 4; j++) s[n][j] = 0.0f;
 #pragma unroll
-        for (int sl = 0; sl < SL; sl++) {
-            const int r = sl * 16 + (lane & 7) + ((lane >> 4) << 3), hi = (lane >> 3) & 1;
+        for (int ks = 0; ks < KS; ks++) {
+            uint32_t qf[4];
+            ldsm4(qf, q_at + (lane & 15) * (HD * 2) + (((2 * ks + (lane >> 4)) ^ (lane & 7)) << 4));
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
+            for (int sl = 0; sl < SL; sl++) {
+                const int r = sl * 16 + (lane & 7) + ((lane >> 4) << 3), hi = (lane >> 3) & 1;
                 uint32_t b[4];
                 ldsm4(b, ks_at + r * (HD * 2) + (((2 * ks + hi) ^ (r & 7)) << 4));
-                mma16<BF16>(s[2 * sl], qf[ks], b[0], b[1]);
-                mma16<BF16>(s[2 * sl + 1], qf[ks], b[2], b[3]);
+                mma16<BF16>(s[2 * sl], qf, b[0], b[1]);
+                mma16<BF16>(s[2 * sl + 1], qf, b[2], b[3]);
             }
         }
         const unsigned full = SL == 2 ? 0xffffffffu : 0xffffu;
@@ -144,8 +142,9 @@ __device__ __forceinline__ void part_of_item(const PartSet &set, int item, int c
                 const float m_new = fmaxf(m[i], top), corr = m_new == -INFINITY ? 1.0f : ex2(m[i] - m_new);
                 m[i] = m_new;
                 l[i] *= corr;
+                if (k > c)
 #pragma unroll
-                for (int n = 0; n < NT; n++) o[n][2 * i] *= corr, o[n][2 * i + 1] *= corr;
+                    for (int n = 0; n < NT; n++) o[n][2 * i] *= corr, o[n][2 * i + 1] *= corr;
             }
             const float base = m[i] == -INFINITY ? 0.0f : m[i] - kLift;
             float sum = 0.0f;
@@ -246,15 +245,16 @@ template <bool BF16, int HD>
 __global__ void __launch_bounds__(kPtThreads, HD == 256 ? 2 : 3) paged_part_kernel(const __grid_constant__ PrefixJoin a, int shared_ctas) {
     extern __shared__ __align__(128) unsigned char pt_smem[];
     __shared__ float2 ml[kPtWarps * kPtRows];
+    __shared__ long long offs[kPtWarps][32];
     __shared__ unsigned bad_rows;
     if (!a.own.p.early) pdl_wait();
     pdl_trigger();  // (the join looks up what this call was given before it waits)
     const int b = blockIdx.x;
     if (b < shared_ctas) {
-        part_of_item<BF16, HD, kShared>(a.shared, b / a.shared.chunks, b % a.shared.chunks, pt_smem, ml, bad_rows);
+        part_of_item<BF16, HD, kShared>(a.shared, b / a.shared.chunks, b % a.shared.chunks, pt_smem, offs, ml, bad_rows);
     } else {
         const int i = b - shared_ctas;
-        part_of_item<BF16, HD, kOwn>(a.own, i / a.own.chunks, i % a.own.chunks, pt_smem, ml, bad_rows);
+        part_of_item<BF16, HD, kOwn>(a.own, i / a.own.chunks, i % a.own.chunks, pt_smem, offs, ml, bad_rows);
     }
     if (a.own.p.early && b == 0) pdl_wait();  // this launch ends after the one before it
 }
