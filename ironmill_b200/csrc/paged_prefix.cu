@@ -47,6 +47,16 @@ struct PtShape {
     static constexpr int kSmem = kPtWarps * kWarp + kQ;
 };
 
+// cp16 of what is read once: first to leave L2, where the parts are to stay until they are joined.
+__device__ __forceinline__ uint64_t read_once() {
+    uint64_t policy;
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
+__device__ __forceinline__ void cp16_once(uint32_t dst, const void *src, bool there, uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0), "l"(policy) : "memory");
+}
+
 // Chunks c, c + set.chunks, ... of an item.
 template <bool BF16, int HD, int MODE>
 __device__ __forceinline__ void part_of_item(const PartSet &set, int item, int c, unsigned char *smem, long long (*offs)[32], float2 *ml, unsigned &bad_rows) {
@@ -61,6 +71,7 @@ __device__ __forceinline__ void part_of_item(const PartSet &set, int item, int c
     if (c >= all) return;
     unsigned char *mine = smem + warp * S::kWarp;
     const uint32_t ks_at = smem_u32(mine), vs_at = ks_at + S::kKeys;
+    const uint64_t once = read_once();
     const uint32_t q_at = smem_u32(smem + kPtWarps * S::kWarp);
     for (int i = tid; i < R * CH; i += kPtThreads) {  // queries, on their way with the first keys
         const int r = i / CH, c8 = i % CH, row = u.row0 + r, t = row / p.group;
@@ -92,7 +103,7 @@ __device__ __forceinline__ void part_of_item(const PartSet &set, int item, int c
             for (int i = 0; i < SL * 16 / RPI; i++) {
                 const int r = i * RPI + (RPI > 1 ? lane / CH : 0), c8 = lane & (CH - 1);
                 const long long at = offs[warp][r];
-                cp16((kv ? vs_at : ks_at) + r * (HD * 2) + ((c8 ^ (r & 7)) << 4), (kv ? p.vc : p.kc) + (at < 0 ? 0 : at + c8 * 8), at >= 0);
+                cp16_once((kv ? vs_at : ks_at) + r * (HD * 2) + ((c8 ^ (r & 7)) << 4), (kv ? p.vc : p.kc) + (at < 0 ? 0 : at + c8 * 8), at >= 0, once);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
@@ -263,7 +274,7 @@ __global__ void __launch_bounds__(kPtThreads, HD == 256 ? 2 : 3) paged_part_kern
 // A block takes eight rows (token, query head of one KV head, token-major), a thread four columns of one: eight rows of a column quad lie side by side in the parts of
 // paged_attn_tc.cu. What bounds it is the chain of lookups, so eight lanes find their rows' units before the launches in front of this one are done (those trigger it when
 // everything before the call is), then places of parts, then 32 parts at a time of both sets: maxima and sums a lane each, factors to shared memory, values.
-constexpr int kPjRows = 8, kPjParts = 32;
+constexpr int kPjRows = 8, kPjParts = 32, kPjAhead = 6;
 struct PjRow {
     int token;                // -1: not to be written
     long long out;
@@ -377,13 +388,20 @@ __global__ void __launch_bounds__(2 * HD) paged_prefix_join_kernel(const __grid_
         const float c = corr[r];
         o = make_float4(o.x * c, o.y * c, o.z * c, o.w * c);
         const int n = min(parts - i0, kPjParts);
-#pragma unroll 8
-        for (int i = 0; i < n; i++) {
-            const int part = i0 + i;
-            const float4 v = *reinterpret_cast<const float4 *>(part < parts0 ? base0 + slot_of(a.shared, 0, rows[r], part) * a.shared.rows * HD
-                                                                               : base1 + slot_of(a.own, 1, rows[r], part - parts0) * a.own.rows * HD);
-            const float f = factor[r][i];
-            if (f != 0.0f) o.x += v.x * f, o.y += v.y * f, o.z += v.z * f, o.w += v.w * f;
+#pragma unroll 1
+        for (int i = 0; i < n; i += kPjAhead) {  // requested together: one after the other they took a microsecond for two
+            float4 v[kPjAhead];
+#pragma unroll
+            for (int j = 0; j < kPjAhead; j++) {
+                const int part = i0 + min(i + j, n - 1);
+                v[j] = *reinterpret_cast<const float4 *>(part < parts0 ? base0 + slot_of(a.shared, 0, rows[r], part) * a.shared.rows * HD
+                                                                       : base1 + slot_of(a.own, 1, rows[r], part - parts0) * a.own.rows * HD);
+            }
+#pragma unroll
+            for (int j = 0; j < kPjAhead; j++) {
+                const float f = i + j < n ? factor[r][i + j] : 0.0f;
+                if (f != 0.0f) o.x += v[j].x * f, o.y += v[j].y * f, o.z += v[j].z * f, o.w += v[j].w * f;
+            }
         }
         __syncthreads();
     }
@@ -424,11 +442,11 @@ struct PartPlan {
     size_t slots, spans;
     size_t bytes;
 };
-// Parts of an item where it has up to 16 rows: CTAs for about eight rounds over the GPU, at most one per chunk.
-constexpr int kMostChunks = 64;
-PartPlan part_plan(const Device *dev, int units, int nkv, int hd, long long rows) {
+// tc: rows of a tile on tcgen05, 0: tiles of 16 here, with CTAs for two rounds over the GPU, at most one a chunk (8 x 8 sequences behind 3000 rows: 58 us with four times as
+// many, whose parts are as many more, 53 so).
+constexpr int kMostChunks = 64, kRounds = 6;
+PartPlan part_plan(const Device *dev, int units, int nkv, int hd, long long rows, int tc) {
     PartPlan a;
-    const int tc = paged_tc_rows(hd, rows);
     a.tc = tc > 0;
     a.rows = tc ? tc : kPtRows;
     a.row_tiles = (int)((rows + a.rows - 1) / a.rows);
@@ -438,7 +456,7 @@ PartPlan part_plan(const Device *dev, int units, int nkv, int hd, long long rows
     a.spans = tc ? (items * 8 + 15) / 16 * 16 : 0;
     a.slots = 0;
     if (tc) a.slots = ((size_t)a.ctas * 2 + items) * a.rows;
-    else if (items) a.slots = items * std::max<size_t>(1, std::min<size_t>(kMostChunks, (size_t)24 * dev->sm_count / items)) * a.rows;
+    else if (items) a.slots = items * std::max<size_t>(1, std::min<size_t>(kMostChunks, (size_t)kRounds * dev->sm_count / items)) * a.rows;
     a.bytes = a.slots * hd * 4 + a.slots * 8 + a.spans;
     return a;
 }
@@ -447,11 +465,18 @@ struct PrefixPlan {
     PartPlan shared, own;
     size_t bytes;
 };
-PrefixPlan prefix_plan(const Device *dev, const PagedView &v, int group, int max_new, int groups, int max_group_new) {
+// Shared rows that make CTAs for half of the places that the GPU has for them, in tiles of 16, are taken that way, whatever their number: a launch of paged_attn_tc.cu takes
+// 18 us at least. (32 rows of a KV head behind 640, 80 CTAs: 18.5 us there, 12.3 here; behind 1500, 192: 21.6 and 14.6; 64 rows behind 1500, 384: 23.3 and 26.7.)
+// bytes: enough for any max_prefix.
+PrefixPlan prefix_plan(const Device *dev, const PagedView &v, int group, int max_new, int groups, int max_group_new, int max_prefix) {
     PrefixPlan a;
-    a.shared = part_plan(dev, groups, v.nkv, v.hd, (long long)max_group_new * group);
-    a.own = part_plan(dev, v.nseq, v.nkv, v.hd, (long long)max_new * group);
-    a.bytes = a.shared.bytes + a.own.bytes;
+    const long long rows = (long long)max_group_new * group;
+    const int tc = paged_tc_rows(v.hd, rows), chunk = v.hd == 256 ? 64 : 128;
+    const PartPlan there = part_plan(dev, groups, v.nkv, v.hd, rows, tc), here = part_plan(dev, groups, v.nkv, v.hd, rows, 0);
+    const bool few = (long long)here.units * v.nkv * ((max_prefix + (long long)chunk - 1) / chunk) <= 3ll * dev->sm_count / 2;
+    a.shared = few ? here : there;
+    a.own = part_plan(dev, v.nseq, v.nkv, v.hd, (long long)max_new * group, paged_tc_rows(v.hd, (long long)max_new * group));
+    a.bytes = a.own.bytes + (tc && (long long)here.units * v.nkv <= 3ll * dev->sm_count / 2 ? std::max(here.bytes, there.bytes) : there.bytes);
     return a;
 }
 
@@ -539,7 +564,7 @@ IM_EXPORT size_t im_cuda_paged_prefix_attention_scratch_bytes(const im_device *d
     try {
         im::PagedView v;
         if (!dev || im::paged_view(kv, 0, &v) != IM_OK || im::attn_check(kv, num_heads, max_new) != IM_OK || im::prefix_check(kv, num_heads, num_groups, max_group_new) != IM_OK) return 0;
-        return im::prefix_plan(dev, v, num_heads / v.nkv, max_new, num_groups, max_group_new).bytes;
+        return im::prefix_plan(dev, v, num_heads / v.nkv, max_new, num_groups, max_group_new, 0).bytes;
     } catch (...) {
         return 0;
     }
@@ -561,10 +586,10 @@ IM_EXPORT int im_cuda_paged_prefix_attention(im_device *dev, const im_paged_kv *
     rc = attn_args(dev, kv, x.layer, x.q_dev, x.q_stride, x.out_dev, x.out_stride, num_heads, x.token_start_dev, x.num_tokens, x.max_new, x.mask_dev, x.mask_words, x.scale, x.max_len, &p, &empty);
     if (rc != IM_OK || empty) return rc;
     IM_REQUIRE(kv->num_kv_heads <= 65535, "at most 65535 key / value heads (got %d)", kv->num_kv_heads);
-    const PrefixPlan plan = prefix_plan(dev, p.kv, p.group, x.max_new, num_groups, max_group_new);
+    const int max_len = attn_length(p.kv, x.max_len), max_prefix = std::min(attn_length(p.kv, args->max_prefix), max_len);
+    const PrefixPlan plan = prefix_plan(dev, p.kv, p.group, x.max_new, num_groups, max_group_new, max_prefix);
     IM_REQUIRE(x.scratch_dev && aligned16(x.scratch_dev) && x.scratch_bytes >= plan.bytes, "paged prefix attention needs %zu bytes of 16-byte aligned scratch (got %zu)", plan.bytes,
                x.scratch_dev ? x.scratch_bytes : (size_t)0);
-    const int max_len = attn_length(p.kv, x.max_len), max_prefix = std::min(attn_length(p.kv, args->max_prefix), max_len);
     p.group_start = args->group_start_dev;
     p.prefix_pages = args->prefix_pages_dev;
     p.groups = num_groups;
