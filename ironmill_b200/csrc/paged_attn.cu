@@ -421,11 +421,11 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
 
 // Items that a cut divides: eight rows a block.
 constexpr int kJoinWarps = 8;
-template <bool BF16, int R, int HD, int MODE>
+template <bool BF16, int R, int HD>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __grid_constant__ PagedAttn p) {
     pdl_trigger();
     pdl_wait();
-    join_row<BF16, R, HD, MODE>(p, blockIdx.x, blockIdx.y * kJoinWarps + (threadIdx.x >> 5));
+    join_row<BF16, R, HD>(p, blockIdx.x, blockIdx.y * kJoinWarps + (threadIdx.x >> 5));
 }
 
 
@@ -473,10 +473,10 @@ void attn_lay_out(PagedAttn *p, const AttnPlan &plan, int max_len, void *at) {
 
 namespace {
 
-template <bool BF16, int R, int HD, int MODE>
+template <bool BF16, int R, int HD>
 int join_launch(const PagedAttn &p, int units, cudaStream_t st) {
     const long long rows = std::min<long long>(R, (long long)p.max_new * p.group);
-    IM_CUDA_CHECK(launch_k(paged_join_kernel<BF16, R, HD, MODE>, dim3((unsigned)(units * p.kv.nkv), (unsigned)((rows + kJoinWarps - 1) / kJoinWarps)), dim3(kJoinWarps * 32), 0, st, p));
+    IM_CUDA_CHECK(launch_k(paged_join_kernel<BF16, R, HD>, dim3((unsigned)(units * p.kv.nkv), (unsigned)((rows + kJoinWarps - 1) / kJoinWarps)), dim3(kJoinWarps * 32), 0, st, p));
     return IM_OK;
 }
 
@@ -493,7 +493,7 @@ int attn_launch(const Device *dev, const PagedAttn &p, int units, int cluster, b
         return IM_OK;
     }
     IM_CUDA_CHECK(launch_k(paged_attn_kernel<BF16, HD, false, MODE>, dim3(p.ctas), dim3(kPaThreads), (size_t)S::kSmem, st, p, units));
-    return joins ? join_launch<BF16, S::kRows, HD, MODE>(p, units, st) : IM_OK;
+    return joins ? join_launch<BF16, S::kRows, HD>(p, units, st) : IM_OK;
 }
 
 }  // namespace
@@ -555,7 +555,7 @@ int attn_args(im_device *dev, const im_paged_kv *kv, int layer, const void *q_de
     if (p->scale2 == 0.0f) p->scale2 = 1e-30f;  // every position alike, without 0 * inf at the hidden ones
     p->group_start = p->prefix_pages = nullptr;
     p->groups = p->whole_slot = p->early = 0;
-    p->stat = nullptr;
+    p->stat = p->stat_parts = nullptr;
     p->scores = p->sums = nullptr;
     return IM_OK;
 }

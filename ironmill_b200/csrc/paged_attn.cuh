@@ -27,7 +27,8 @@ struct PagedAttn {
     int whole_slot;           // kShared, kOwn: slots from here on are those of items that one CTA had, by item
     int early;                // kOwn: a kShared launch that this one needs nothing of may still run (see paged_prefix.cu)
     // sums of softmax weights (paged_weights.cu)
-    float2 *stat;             // [units, KV heads, rows of a tile]: maximum and sum of weights of every row
+    float2 *stat;             // [units, KV heads, rows of a tile]: maximum and sum of weights of every row of an item that one CTA (or cluster) had
+    float2 *stat_parts;       // tcgen05: [slots, rows of a tile]: of the others' parts, where part_ml may have a NaN instead
     float *scores;            // or NULL: [units, KV heads, score_rows, score_cap]: scores of the positions before score_cap, in powers of two
     int score_cap, score_rows;
     float *sums;              // [sequences, KV heads, sum_cols]
@@ -383,12 +384,12 @@ __device__ __noinline__ float plain_sum(const PagedAttn &p, const PagedUnit &u, 
 
 // Row r of an item that a cut divides, by a warp, HD / 32 columns a lane. The parts of an item lie with the CTAs that its tiles fall to; a lane per part
 // brings maxima and sums. (A block per row with the shares' divisions in loops took 25 us for 64 items of 104 rows.)
-template <bool BF16, int R, int HD, int MODE>
+template <bool BF16, int R, int HD>
 __device__ __forceinline__ void join_row(const PagedAttn &p, int item, int r) {
     constexpr int V = HD / 32;
     const int unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, lane = threadIdx.x & 31;
     const int2 span = *reinterpret_cast<const int2 *>(p.spans + 2 * (long long)item);
-    const PagedUnit u = paged_unit<R, MODE>(p, unit);
+    const PagedUnit u = paged_unit<R, kAttend>(p, unit);
     if (r >= u.rows || span.x < 0) return;  // (a unit without tiles has no rows)
     const size_t slot0 = span.x;
     const int c = span.x >> 1, parts = span.y - c + 1;
@@ -418,7 +419,6 @@ __device__ __forceinline__ void join_row(const PagedAttn &p, int item, int r) {
             for (int j = 0; j < V; j++) o[j] += g == 0.0f ? 0.0f : v[j] * g;
         }
     }
-    if (MODE == kWeigh && lane == 0) p.stat[(long long)item * R + r] = make_float2(M, L);
     const float inv = L > 0.0f ? 1.0f / L : L == 0.0f ? 0.0f : L;
     const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
     uint32_t *dst = reinterpret_cast<uint32_t *>(p.out + (u.tok0 + t) * p.os + (long long)(head * p.group + g) * HD + lane * V);
@@ -439,6 +439,31 @@ int attn_args(im_device *dev, const im_paged_kv *kv, int layer, const void *q_de
 
 // The kernel of paged_attn_tc.cu with the sums of a part as its result (paged_prefix.cu): MODE kShared or kOwn; no join.
 int paged_tc_part_launch(const Device *dev, const PagedAttn &p, bool bf16, int mode, int rows, int units, cudaStream_t st);
+// Adds the parts i, i + step, ... of a row, maxima and sums of weights, at `ml`: slots of R rows. Eight are requested together.
+__device__ __forceinline__ float2 row_parts(const float2 *ml, int2 span, int R, int r, int i, int step) {
+    const int c = span.x >> 1, parts = span.y - c + 1;
+    float M = -INFINITY, L = 0.0f;
+#pragma unroll 1
+    for (; i < parts; i += 8 * step) {
+        float2 x[8];
+        float top = M;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const int at = min(i + k * step, parts - 1);
+            x[k] = ml[(at == 0 ? (size_t)span.x : (size_t)(c + at) * 2) * R + r];
+        }
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            if (i + k * step >= parts) x[k] = make_float2(-INFINITY, 0.0f);
+            top = fmaxf(top, x[k].x);
+        }
+        L = M == top ? L : L * ex2(M - top);
+#pragma unroll
+        for (int k = 0; k < 8; k++) L += x[k].x == -INFINITY && x[k].y == 0.0f ? 0.0f : x[k].y * ex2(x[k].x - top);
+        M = top;
+    }
+    return make_float2(M, L);
+}
 // Attention and the norms of every row's weights (paged_weights.cu): where `cluster` is not zero, the sums too. joins: with the join of what the cuts divide (tcgen05: always).
 int paged_weigh_launch(const Device *dev, const PagedAttn &p, bool bf16, int units, int cluster, bool joins, cudaStream_t st);
 int paged_tc_weigh_launch(const Device *dev, const PagedAttn &p, bool bf16, int rows, int units, cudaStream_t st);

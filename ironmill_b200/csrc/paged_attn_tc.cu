@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             if (WIDE || h == 0) {
                 if (whole && lane == 0) p.odd[((long long)it.unit * p.kv.nkv + it.head) * 8 + warp] = bad;
                 if (live && !whole) p.part_ml[slot * R + R_] = make_float2(m - kLift, bad >> lane & 1u ? NAN : l);
-                if (MODE == kWeigh && live && whole) p.stat[((long long)it.unit * p.kv.nkv + it.head) * R + R_] = make_float2(m - kLift, l);
+                if (MODE == kWeigh && live) (whole ? p.stat[((long long)it.unit * p.kv.nkv + it.head) * R + R_] : p.stat_parts[slot * R + R_]) = make_float2(m - kLift, l);
             }
         }
     }
@@ -503,17 +503,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
 constexpr int kTcJoinThreads = 128, kTcJoinWarps = kTcJoinThreads / 32;
 // Rows 32 * rows + j of an item, j a bit of `bad`, from the positions they see alone: every `warps`-th of them, by a warp. (By itself and from numbers
 // alone: what it needs of registers and memory is no cost where no row is odd.)
-template <bool BF16, int R, int HD, int MODE>
+template <bool BF16, int R, int HD>
 __device__ __noinline__ void odd_rows_again(const PagedAttn &p, int unit, int head, int rows, unsigned bad, int warp, int warps) {
     const int lane = threadIdx.x & 31;
-    const PagedUnit u = paged_unit<R, MODE>(p, unit);
+    const PagedUnit u = paged_unit<R, kAttend>(p, unit);
 #pragma unroll 1
     for (int n = 0; bad; n++, bad &= bad - 1) {
         if (n % warps != warp) continue;
         const int r = rows * 32 + __ffs(bad) - 1;
         float o[HD / 32], m, l;
         plain_row<BF16, HD>(p, u, head, r, 0, u.end, o, m, l);
-        if (MODE == kWeigh && lane == 0) p.stat[((long long)unit * p.kv.nkv + head) * R + r] = make_float2(m, l);
         const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : l;
         uint16_t *out = p.out + (u.tok0 + (u.row0 + r) / p.group) * p.os + (long long)(head * p.group + (u.row0 + r) % p.group) * HD + lane;
 #pragma unroll
@@ -522,8 +521,8 @@ __device__ __noinline__ void odd_rows_again(const PagedAttn &p, int unit, int he
 }
 
 // Four columns of row r of an item that a cut divides. Returns the lanes whose rows are not finite: those are not written.
-template <bool BF16, int HD, int R, int N, int MODE>
-__device__ __forceinline__ unsigned join_parts(const PagedAttn &p, const PagedUnit &u, int unit, int2 span, int head, int r, int c) {
+template <bool BF16, int HD, int R, int N>
+__device__ __forceinline__ unsigned join_parts(const PagedAttn &p, const PagedUnit &u, int2 span, int head, int r, int c) {
     const bool live = r < u.rows;
     const int first = span.x >> 1, parts = span.y - first + 1, at = min(r, u.rows - 1);
     float M = -INFINITY, L = 0.0f;
@@ -559,7 +558,6 @@ __device__ __forceinline__ unsigned join_parts(const PagedAttn &p, const PagedUn
     }
     const unsigned bad = __ballot_sync(0xffffffffu, live && L != L);
     if (!live || L != L) return bad;
-    if (MODE == kWeigh && c == 0) p.stat[((long long)unit * p.kv.nkv + head) * R + r] = make_float2(M, L);
     const float inv = L > 0.0f ? 1.0f / L : 0.0f;
     const int t = (u.row0 + r) / p.group, g = (u.row0 + r) % p.group;
     *reinterpret_cast<uint2 *>(p.out + (u.tok0 + t) * p.os + (long long)(head * p.group + g) * HD + c) = make_uint2(pack2<BF16>(o.x * inv, o.y * inv), pack2<BF16>(o.z * inv, o.w * inv));
@@ -573,15 +571,16 @@ __device__ __forceinline__ unsigned join_parts(const PagedAttn &p, const PagedUn
 template <bool BF16, int KB, bool WIDE, int MODE>
 __global__ void __launch_bounds__(kTcJoinThreads, WIDE ? 9 : 12) paged_tc_join_kernel(const __grid_constant__ PagedAttn p) {
     constexpr int R = TcShape<KB, WIDE>::kRows, HD = 64 * KB, N = WIDE ? 8 : 4;  // N: parts that are requested together
-    pdl_trigger();
+    if (MODE != kWeigh) pdl_trigger();
     pdl_wait();
+    if (MODE == kWeigh) pdl_trigger();  // (what adds up the weights starts beside this launch, and needs the attention done)
     const int item = blockIdx.x, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, lane = threadIdx.x & 31;
     const int w = blockIdx.y * kTcJoinWarps + (threadIdx.x >> 5), rows = w / (HD / 4), r = rows * 32 + lane, c = w % (HD / 4) * 4;
     const int2 span = *reinterpret_cast<const int2 *>(p.spans + 2 * (long long)item);
     const PagedUnit u = paged_unit<R, MODE>(p, unit);
     if (rows * 32 >= u.rows) return;  // (a unit without tiles has no rows)
-    const unsigned bad = span.x < 0 ? p.odd[(long long)item * 8 + rows] : join_parts<BF16, HD, R, N, MODE>(p, u, unit, span, head, r, c);
-    if (bad) odd_rows_again<BF16, R, HD, MODE>(p, unit, head, rows, bad, w % (HD / 4), HD / 4);
+    const unsigned bad = span.x < 0 ? p.odd[(long long)item * 8 + rows] : join_parts<BF16, HD, R, N>(p, u, span, head, r, c);
+    if (bad) odd_rows_again<BF16, R, HD>(p, unit, head, rows, bad, w % (HD / 4), HD / 4);
 }
 
 template <bool BF16, int KB, bool WIDE, int MODE>

@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(kSumThreads) paged_sum_kernel(const __grid_con
     pdl_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if ((int)blockIdx.x < joins) {
-        join_row<BF16, R, HD, kWeigh>(p, blockIdx.x / row_blocks, (blockIdx.x % row_blocks) * kSumWarps + warp);
+        join_row<BF16, R, HD>(p, blockIdx.x / row_blocks, (blockIdx.x % row_blocks) * kSumWarps + warp);
         return;
     }
     const int item = (blockIdx.x - joins) / chunks, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv, chunk = (blockIdx.x - joins) % chunks;
@@ -41,17 +41,9 @@ __global__ void __launch_bounds__(kSumThreads) paged_sum_kernel(const __grid_con
         if (span.x < 0) {
             ml = p.stat[(long long)item * R + r];
         } else {
-            const int c = span.x >> 1, parts = span.y - c + 1;
-            float M = -INFINITY, L = 0.0f;
-            for (int i = lane; i < parts; i += 32) {
-                const float2 x = p.part_ml[(i == 0 ? (size_t)span.x : (size_t)(c + i) * 2) * R + r];
-                if (x.x == -INFINITY && x.y == 0.0f) continue;
-                const float top = fmaxf(M, x.x);
-                L = (M == top ? L : L * ex2(M - top)) + x.y * ex2(x.x - top);
-                M = top;
-            }
-            const float top = warp_max(M);
-            ml = make_float2(top, warp_sum(M == -INFINITY && L == 0.0f ? 0.0f : L * ex2(M - top)));
+            ml = row_parts(p.part_ml, span, R, r, lane, 32);
+            const float top = warp_max(ml.x);
+            ml = make_float2(top, warp_sum(ml.x == -INFINITY && ml.y == 0.0f ? 0.0f : ml.y * ex2(ml.x - top)));
         }
         if (lane == 0) norms[r] = row_norm(ml);
     }
@@ -128,7 +120,7 @@ __device__ __forceinline__ uint32_t rows_seeing(const PagedAttn &p, const PagedU
 }
 
 template <bool BF16, int KB>
-__global__ void __launch_bounds__(kTcThreads, 1) paged_weigh_kernel(const __grid_constant__ PagedAttn p, int units, int stat_rows, int stat_tiles, int *err) {
+__global__ void __launch_bounds__(kTcThreads, 1) paged_weigh_kernel(const __grid_constant__ PagedAttn p, int units, int stat_rows, int stat_tiles, const float2 *parts, int *err) {
     using S = WeighShape<KB>;
     constexpr int HD = 64 * KB, SK = S::kK, BR = S::kBlockRows;
     extern __shared__ __align__(16) unsigned char weigh_smem[];
@@ -165,7 +157,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_weigh_kernel(const __grid
     fence_after();
     const uint32_t tmem = uniform(*tmem_slot);
     pdl_trigger();
-    pdl_wait();
+    if (!p.early) pdl_wait();
     PagedUnit at;
     const Share share = units <= 32 ? warp_share<kAllRows, kTcTile, kWeigh>(p, units, at) : find_share<kAllRows, kTcTile, kTcThreads, kWeigh>(p, units, reinterpret_cast<long long *>(Qs), at);
     Items<kAllRows, kWeigh> it(p, units, share, at);
@@ -286,7 +278,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_weigh_kernel(const __grid
                 both_halves();  // the norms before have been read
                 if (tid < n) {
                     const int row = row0 + tid;
-                    norms[tid] = row < u.rows ? row_norm(p.stat[(((long long)u.seq * stat_tiles + row / stat_rows) * p.kv.nkv + it.head) * stat_rows + row % stat_rows]) : -INFINITY;
+                    float2 ml = make_float2(-INFINITY, 0.0f);
+                    if (row < u.rows) {
+                        const int tile = row / stat_rows, r = row - tile * stat_rows;
+                        const long long item = ((long long)u.seq * stat_tiles + tile) * p.kv.nkv + it.head;
+                        const int2 span = parts ? *reinterpret_cast<const int2 *>(p.spans + 2 * item) : make_int2(-1, 0);
+                        ml = span.x < 0 ? p.stat[item * stat_rows + r] : row_parts(parts, span, stat_rows, r, 0, 1);
+                    }
+                    norms[tid] = row_norm(ml);
                 }
                 both_halves();
                 for (int t = it.t0; t < it.t1; t++, tile++) {
@@ -346,6 +345,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_weigh_kernel(const __grid
     }
     fence_before();
     sync_and_settle(ok);
+    if (p.early && blockIdx.x == 0) pdl_wait();  // this launch ends after the one before it
     if (warp == kTcMma) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
@@ -365,7 +365,7 @@ WeighPlan weigh_plan(const Device *dev, const PagedView &v, int group, int max_n
     a.attn = attn_plan(dev, v.nseq, v.nkv, v.hd, group, max_new, max_len);
     const size_t items = (size_t)a.attn.units * v.nkv;
     a.attn_bytes = (a.attn.bytes + 15) / 16 * 16;
-    a.stat_bytes = items * a.attn.rows * 8;
+    a.stat_bytes = (items + (a.attn.rows > 16 ? 2 * (size_t)a.attn.ctas : 0)) * a.attn.rows * 8;
     a.rows = group * max_new;
     a.cap = 0;
     size_t most = 0;
@@ -393,8 +393,10 @@ int sums(const Device *dev, const PagedAttn &p, const WeighPlan &plan, int max_l
     if (once.first(dev->ordinal)) IM_CUDA_CHECK(cudaFuncSetAttribute((paged_weigh_kernel<BF16, HD / 64>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     PagedAttn w = p;
     w.row_tiles = 1;
+    w.early = plan.attn.rows > 16;  // the join in front of it triggers it once the attention is done
     w.ctas = (int)std::max(1ll, std::min<long long>(dev->sm_count, (long long)p.kv.nseq * p.kv.nkv * ((max_len + (long long)kTcTile - 1) / kTcTile)));
-    IM_CUDA_CHECK(launch_k(paged_weigh_kernel<BF16, HD / 64>, dim3(w.ctas), dim3(kTcThreads), (size_t)S::kSmem, st, w, p.kv.nseq, plan.attn.rows, plan.attn.row_tiles, dev->err_flag));
+    IM_CUDA_CHECK(launch_k(paged_weigh_kernel<BF16, HD / 64>, dim3(w.ctas), dim3(kTcThreads), (size_t)S::kSmem, st, w, p.kv.nseq, plan.attn.rows, plan.attn.row_tiles,
+                           plan.attn.cluster ? nullptr : plan.attn.rows > 16 ? p.stat_parts : p.part_ml, dev->err_flag));
     return IM_OK;
 }
 
@@ -441,6 +443,7 @@ IM_EXPORT int im_cuda_paged_attention_weights(im_device *dev, const im_paged_kv 
     attn_lay_out(&p, plan.attn, max_len, x.scratch_dev);
     unsigned char *at = static_cast<unsigned char *>(x.scratch_dev) + plan.attn_bytes;
     p.stat = reinterpret_cast<float2 *>(at);
+    p.stat_parts = p.stat + (size_t)plan.attn.units * p.kv.nkv * plan.attn.rows;
     p.scores = plan.cap ? reinterpret_cast<float *>(at + plan.stat_bytes) : nullptr;
     p.score_cap = plan.cap;
     p.score_rows = plan.rows;
