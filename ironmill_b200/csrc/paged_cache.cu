@@ -636,12 +636,12 @@ IM_EXPORT int im_cuda_paged_append_normed(im_device *dev, const im_paged_kv *kv,
     using namespace im;
     IM_REQUIRE(kv && args, "kv or args is NULL");
     const im_paged_append_args &x = *args;
-    IM_REQUIRE(!x.q_norm_dev || x.q_dev, "norm weights of queries without queries");
+    IM_REQUIRE(!x.q_norm_dev || x.num_heads > 0, "norm weights of queries without queries");
     IM_REQUIRE((!x.q_norm_dev && !x.k_norm_dev) || x.norm_dtype == IM_DTYPE_F32 || x.norm_dtype == kv->dtype, "norm weights are of the cache's type or f32 (got dtype %d)", x.norm_dtype);
     IM_REQUIRE(aligned16(x.q_norm_dev) && aligned16(x.k_norm_dev), "norm weights have to be 16-byte aligned");
     IM_REQUIRE(x.eps >= 0.0f && x.eps - x.eps == 0.0f, "eps has to be finite and not negative");
     IM_REQUIRE(x.num_axes >= 1 && x.num_axes <= kAxes, "%d axes (at most %d)", x.num_axes, kAxes);
-    IM_REQUIRE(x.num_axes == 1 || (x.rotary_dim > 0 && x.position_dev && x.pair_axis_host), "several axes need a rotation, positions and the axis of every pair");
+    IM_REQUIRE(x.num_axes == 1 || (x.rotary_dim > 0 && (x.position_dev || x.num_tokens == 0) && x.pair_axis_host), "several axes need a rotation, positions and the axis of every pair");
     Append a;
     bool empty;
     const int rc = append_args(dev, kv, x.layer, x.k_dev, x.k_stride, x.v_dev, x.v_stride, x.token_start_dev, x.num_tokens, x.q_dev, x.q_stride, x.q_out_dev, x.q_out_stride, x.num_heads,

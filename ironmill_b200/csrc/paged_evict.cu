@@ -104,12 +104,12 @@ __global__ void __launch_bounds__(kEvThreads, 4) paged_evict_kernel(const __grid
         return;
     }
     // ---- the H-th largest key, digit by digit from the top; `above` of the others are larger, `equals` are the same. Once few enough share the digits
-    // found they are picked out, and the next digits are theirs.
+    // found they are picked out, and the next digits are theirs; where all that share them stay, the rest of the key does not matter.
     uint32_t top = 0, mask = 0;
     int above = 0, equals = old, listed = -1;
-    for (int digit = 0; digit < 3 && H > 0; digit++) {
+    for (int digit = 0; digit < 3 && H > 0 && equals > H - above; digit++) {
         const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, count = digit < 2 ? 2048 : 1024;
-        for (int i = tid; i < count; i += kEvThreads) bins[i] = 0;
+        for (int i = 4 * tid; i < count; i += 4 * kEvThreads) *reinterpret_cast<int4 *>(bins + i) = make_int4(0, 0, 0, 0);
         if (listed < 0 && digit > 0 && equals <= kListed) {
             if (tid == 0) found[2] = 0;
             __syncthreads();

@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(kSumThreads) paged_sum_kernel(const __grid_con
     const bool aligned = reinterpret_cast<uintptr_t>(sums) % 16 == 0;
     for (long long at = (long long)chunk * kSumPositions + 4 * tid; at < u.end; at += (long long)chunks * kSumPositions) {
         const int pos = (int)at;
-        if (pos + 4 <= p.score_cap) {  // (a multiple of 64)
+        if (at + 4 <= p.score_cap) {  // (a multiple of 64)
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
             for (int r = 0; r < u.rows; r++) {
@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kSumThreads) paged_sum_kernel(const __grid_con
                     if (pos + j < u.end) add_sum(p, u, head, pos + j, x[j]);
             }
         } else {
-            for (int j = 0; j < 4 && pos + j < u.end; j++) add_sum(p, u, head, pos + j, plain_sum<BF16, HD>(p, u, head, pos + j, norms));
+            for (int j = 0; j < 4 && at + j < u.end; j++) add_sum(p, u, head, pos + j, plain_sum<BF16, HD>(p, u, head, pos + j, norms));
         }
     }
 }

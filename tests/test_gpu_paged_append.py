@@ -155,3 +155,22 @@ def test_without_norms_and_axes_the_plain_append_runs(dev):
     # the same formula, contracted differently: a step of the type at most
     for a, b in zip(*got):
         assert ((a.float() - b.float()).abs() <= 2.0 ** -10 * b.float().abs() + 2.0 ** -21).all()
+
+
+def test_no_tokens(dev):
+    from ironmill_b200 import ops
+    c = Cache(dev, H.rng_for("append-none"), [30], [20])
+    x, cos = torch.zeros((0, 8, 128), dtype=torch.float16, device="cuda"), torch.ones((9, 64), dtype=torch.float16, device="cuda")
+    w = torch.ones(128, dtype=torch.float16, device="cuda")
+    before = c.k.clone()
+    q = ops.paged_append(c.kv, 0, x[:, :2], x[:, 2:4], _ints([0, 0]), q=x[:, 4:], cos=cos, sin=cos, positions=torch.zeros((3, 0), dtype=torch.int32, device="cuda"), q_norm=w, k_norm=w,
+                         pair_axis=bytes([i % 3 for i in range(64)]))
+    assert q.shape == (0, 4, 128) and (c.k == before).all()
+
+
+def test_heads_of_which_some_lie_in_other_rows_of_a_wider_tensor(dev):
+    """Parts of one row per token, as a projection leaves them, tokens far apart; norm weights of another type than the cache's are f32."""
+    rng = H.rng_for("append-wide")
+    for dim, norm_type in ((128, "f32"), (64, None), (96, "f32")):
+        c = Cache(dev, rng, [50, 20], [40, 0], dim=dim, kv_heads=2, dtype="bf16")
+        _check(dev, c, rng, [9, 20], 6, "bf16", dim, axes=3, axis=[i * 3 // (dim // 2) for i in range(dim // 2)], norm_type=norm_type, table="f32")

@@ -290,3 +290,53 @@ def test_a_captured_eviction_follows_lengths_and_sums(dev):
         graph.replay()
         assert len_out.tolist() == om.evict(ko, vo, c.table, lens, _np(w), want, 100, 20).tolist()
         assert (_np(w_out) == want).all() and (_np(c.k) == ko).all() and (_np(c.v) == vo).all()
+
+
+# ------------------------------------------------------------------------------------------------ together, as a server uses them
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("new", [1, 12])
+def test_a_run_of_appending_attending_weighing_and_evicting(dev, dtype, new):
+    """Two sequences over two layers and several steps: positions go on counting while the caches stay within their budget. Nothing waits in between."""
+    from ironmill_b200 import ops
+    rng = H.rng_for("evict-run", new)
+    budget, recent, steps, heads, page = 40, 10, 6, 8, 16
+    c = Cache(dev, rng, [budget + 2 * new + 8] * 2, [20, 45], kv_heads=2, page=page, layers=2, dtype=dtype)
+    rows = c.table.shape[1] * page
+    starts, position = [0, new, 2 * new], [20, 45]
+    angle = np.arange(200)[:, None] * 1e4 ** (-np.arange(64) / 64)
+    cos, sin = (torch.from_numpy(f(angle)).float().cuda() for f in (np.cos, np.sin))
+    norm = (1 + _randn(rng, (128,), "f32", 0.1)).float()
+    w = [torch.rand((2, 2, 2, rows), device="cuda"), torch.zeros((2, 2, 2, rows), device="cuda")]
+    k64, v64, w64 = _np(c.k), _np(c.v), _np(w[0])
+    lens = list(c.lengths)
+    lengths = _ints(lens)
+    ins, outs = [], []
+    for _ in range(steps):
+        at = np.concatenate([np.arange(p, p + new) for p in position])
+        x = [(_randn(rng, (2 * new, heads, 128), dtype), _randn(rng, (2 * new, 2, 128), dtype), _randn(rng, (2 * new, 2, 128), dtype)) for _ in range(2)]
+        ins.append((at, x))
+        c.kv.point_at(c.kv.page_table, lengths)
+        for layer, (q, k, v) in enumerate(x):
+            q = ops.paged_append(c.kv, layer, k, v, _ints(starts), q=q, cos=cos, sin=sin, positions=_ints(at), q_norm=norm, k_norm=norm)
+            outs.append((q, ops.paged_attention_weights(c.kv, layer, q, _ints(starts), new, 0.088, w[0][layer], max_len=rows)))
+        c.kv.point_at(c.kv.page_table, lengths + new)
+        lengths, _ = ops.paged_evict(c.kv, w[0], budget, recent, weights_out=w[1])
+        w.reverse()
+        position = [p + new for p in position]
+    torch.cuda.synchronize()
+    # the same from the restatement: what the kernels rounded (rotated queries and keys) is taken from it, so that both choose among the same sums up to f32
+    for step, (at, x) in enumerate(ins):
+        for layer, (q, k, v) in enumerate(x):
+            turned, _, _ = om.append(k64[layer], v64[layer], c.table, lens, starts, _np(k), _np(v), _np(q), _np(cos), _np(sin), 128, False, [at], _np(norm), _np(norm), 1e-6)
+            k64[layer] = np.where(k64[layer] == 0, 0, torch.from_numpy(k64[layer]).to(TYPES[dtype]).double().numpy())
+            got_q, got = outs[2 * step + layer]
+            assert np.abs(_np(got_q) - turned).max() < 0.05
+            want, mass, dot, w64[layer] = om.attention(k64[layer], v64[layer], c.table, lens, starts, _np(got_q), 0.088, None, w64[layer])
+            assert np.abs(_np(got) - want).max() < (3e-2 if dtype == "bf16" else 4e-3)
+        lens = [n + new for n in lens]
+        out64 = np.zeros_like(w64)
+        lens = om.evict(k64, v64, c.table, lens, w64, out64, budget, recent).tolist()
+        w64 = out64
+    assert lengths.tolist() == lens
+    for s, n in enumerate(lens):
+        assert np.abs(_np(w[0])[:, s, :, :n] - w64[:, s, :, :n]).max() < 1e-2

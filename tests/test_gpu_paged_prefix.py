@@ -269,3 +269,32 @@ def test_two_calls_at_once_on_streams_of_their_own(dev):
         torch.cuda.synchronize()
         for a, b in zip(got, alone):
             assert (a == b).all()
+
+
+def test_no_tokens_and_one_sequence_alone(dev):
+    from ironmill_b200 import ops
+    rng = H.rng_for("prefix-alone")
+    c = _cache(dev, rng, [1], [3], [7], [1])
+    _check(dev, c, rng, [1], [3], [1], 4, "f16")
+    q = torch.zeros((0, 4, 128), dtype=torch.float16, device="cuda")
+    assert ops.paged_prefix_attention(c.kv, 0, q, _ints([0, 0]), 1, 0.1, _ints([0, 1]), 1, _ints([3])).shape == q.shape
+
+
+@pytest.mark.parametrize("seqs, nodes", [(3, 1), (12, 1), (40, 1), (4, 26)])
+def test_calls_in_a_row_follow_what_the_ones_before_them_wrote(dev, seqs, nodes):
+    """Appending and attending in turns on one stream, without waiting: each call finds what those before it wrote, whatever starts beside what."""
+    from ironmill_b200 import ops
+    rng = H.rng_for("prefix-chain", seqs + nodes)
+    c = _cache(dev, rng, [seqs], [30], [8] * seqs, [nodes] * seqs, page=32)
+    starts, n = _ints(_starts([nodes] * seqs)), seqs * nodes
+    steps = [(_randn(rng, (n, 8, 128), "f16"), _randn(rng, (n, 2, 128), "f16"), _randn(rng, (n, 2, 128), "f16")) for _ in range(6)]
+    got = []
+    for q, k, v in steps:
+        ops.paged_append(c.kv, 0, k, v, starts)
+        got.append(ops.paged_prefix_attention(c.kv, 0, q, starts, nodes, 0.1, _ints([0, seqs]), n, _ints([30])))
+    torch.cuda.synchronize()
+    for (q, k, v), out in zip(steps, got):
+        ops.paged_append(c.kv, 0, k, v, starts)
+        torch.cuda.synchronize()
+        want, _, _ = op.attention(_np(c.k[0]), _np(c.v[0]), c.table, c.lengths, _starts([nodes] * seqs), _np(q), 0.1)
+        assert np.abs(_np(out) - want).max() < 2e-3
