@@ -1,5 +1,5 @@
-// A paged cache of keys and values: appending with rotation, keeping the accepted path of a drafted tree, reordering the beams of a search.
-// All three move rows and compute next to nothing: HBM bounds them where they are large, the chain of lookups (sequence of a
+// A paged cache of keys and values: appending with rotation (and norms), keeping the accepted path of a drafted tree, reordering the beams of a search.
+// All of them move rows and compute next to nothing: HBM bounds them where they are large, the chain of lookups (sequence of a
 // token -> its length -> its page) where they are small. 16 bytes per lane everywhere.
 #include <limits.h>
 
@@ -210,8 +210,10 @@ __global__ void __launch_bounds__(kAppendThreads, FORM == 3 ? 2 : 5) paged_appen
 //   of position[axis of i]; f32 from the load to the one rounding at the end.
 // The same blocks and lookups as above, but a lane owns both columns of its pairs (four of them: two words of 8 bytes, which lie side by side where
 // neighbours belong together and half of rotary_dim apart where the halves do), so that rotation exchanges nothing between lanes, and every cosine and sine
-// is loaded once instead of by both lanes of a pair. What bounds it is instructions: a token's weights, cosines and sines are multiplied once, a head
+// is loaded once instead of by both lanes of a pair. A token's weights, cosines and sines are multiplied once, a head
 // is then two products and a factor an element, two elements at a time; its sum of squares is the only exchange, log2(lanes) shuffles.
+// 8 prompts of up to 1900 tokens of 48 heads, three axes (260 MB): 57 us, 4.6 TB/s, 70 % of a copy; instructions issued in two of three clocks, and loads waited for, bound it (82 us with 16
+// bytes a lane of both halves, partners by shuffles and a loop of shuffles). Blocks of 64 threads 57 us, of 32 as much, of 128 66, of 256 103; 32 tokens, in blocks of 256, 6 us.
 constexpr int kAxes = 4;
 struct AppendMore {
     const void *qn, *kn;  // weights or NULL
