@@ -193,6 +193,23 @@ def test_a_captured_call_with_sums_follows_lengths(dev, heads, new):
         assert abs(float(sums.sum()) - 3 * new * heads) < 1e-2
 
 
+@pytest.mark.parametrize("dtype, dim, heads, new", [("f16", 128, 8, 1), ("bf16", 64, 6, 2), ("f16", 256, 4, 3)])
+def test_sums_where_the_scores_have_no_room(dev, dtype, dim, heads, new):
+    """A table of five million rows, of which little is there, and no word of it: scores of so many are not kept, they are computed again."""
+    rng = H.rng_for("sums-no-room", dim)
+    c = Cache(dev, rng, [300 + new, 77 + new], [300, 77], dim=dim, page=256, dtype=dtype)
+    c.table = np.concatenate([c.table, np.full((2, 20000), -1)], 1)
+    c.kv.point_at(_ints(c.table), _ints(c.lengths))
+    _check(dev, c, rng, [new, new], heads, dtype, max_len=0, cols=400)
+
+
+@pytest.mark.parametrize("heads, new", [(8, 1), (8, 26), (8, 64)])
+def test_sums_in_a_layer_of_pages_that_lie_apart(dev, heads, new):
+    rng = H.rng_for("sums-apart", new)
+    c = Cache(dev, rng, [700 + new, 90 + new], [700, 90], page=32, layers=3, apart=True, dtype="bf16")
+    _check(dev, c, rng, [new, new], heads, "bf16", layer=2)
+
+
 # ------------------------------------------------------------------------------------------------ eviction
 def _evict(dev, c, rng, budget, recent, weights=None, strided=False):
     from ironmill_b200 import ops

@@ -298,3 +298,20 @@ def test_calls_in_a_row_follow_what_the_ones_before_them_wrote(dev, seqs, nodes)
         torch.cuda.synchronize()
         want, _, _ = op.attention(_np(c.k[0]), _np(c.v[0]), c.table, c.lengths, _starts([nodes] * seqs), _np(q), 0.1)
         assert np.abs(_np(out) - want).max() < 2e-3
+
+
+@pytest.mark.parametrize("seqs, nodes", [(3, 1), (40, 1), (6, 26)])
+def test_a_layer_of_pages_that_lie_apart(dev, seqs, nodes):
+    rng = H.rng_for("prefix-apart", seqs + nodes)
+    c = _cache(dev, rng, [seqs], [9], [int(x) for x in rng.integers(0, 300, seqs)], [nodes] * seqs, page=32, layers=3, apart=True, dtype="bf16")
+    _check(dev, c, rng, [seqs], [9], [nodes] * seqs, 8, "bf16", layer=1, strided=True)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_few_shared_rows_in_small_tiles_and_many_in_large_ones_agree(dev, dim):
+    """The same call by either kernel: what is announced of the prefix decides."""
+    rng = H.rng_for("prefix-either", dim)
+    for seqs in (5, 9, 20):
+        c = _cache(dev, rng, [seqs], [6], [int(x) for x in rng.integers(0, 60, seqs)], [1] * seqs, page=64, dim=dim)
+        for most in (6 * 64, 0, 1, 100000):
+            _check(dev, c, rng, [seqs], [6], [1] * seqs, 8, "f16", max_prefix=most, max_len=0)
