@@ -446,9 +446,9 @@ struct PartPlan {
     size_t slots, spans;
     size_t bytes;
 };
-// tc: rows of a tile on tcgen05, 0: tiles of 16 here, with CTAs for two rounds over the GPU, at most one a chunk (8 x 8 sequences behind 3000 rows: 58 us with four times as
-// many, whose parts are as many more, 53 so).
-constexpr int kMostChunks = 64, kRounds = 6;
+// tc: rows of a tile on tcgen05, 0: tiles of 16 here, with at most four CTAs an SM and at most one a chunk: more of them even out sequences of different lengths, but each
+// leaves a part to join (32 sequences behind 4096 rows: 33 us with four, 37 with six, 40 with 24; 8 x 8 behind 3000: 53 with four or six, 57 with 24; 64 behind 8192: 53 with any).
+constexpr int kMostChunks = 64, kRounds = 4;
 PartPlan part_plan(const Device *dev, int units, int nkv, int hd, long long rows, int tc) {
     PartPlan a;
     a.tc = tc > 0;
