@@ -122,7 +122,7 @@ def test_prefix_attention_refuses(lib, change, word):
 
 @pytest.mark.parametrize("change, word", [
     (dict(w=0), "NULL"), (dict(w=17 * PTR + 2), "4-byte"), (dict(rows=0), "overlap"), (dict(sh=63), "overlap"), (dict(ss=127), "overlap"), (dict(w=PTR), "queries or the outputs"),
-    (dict(w=9 * PTR + 2048), "queries or the outputs"), (dict(w=9 * PTR + 3072), GOOD), (dict(ss=0), "overlap"), (dict(sh=-64), "overlap"), (dict(sh=1 << 50), "overlap")])
+    (dict(w=9 * PTR + 2048), "queries or the outputs"), (dict(w=9 * PTR + 4096), GOOD), (dict(ss=0), "overlap"), (dict(sh=-64), "overlap"), (dict(sh=1 << 50), "overlap")])
 def test_attention_with_sums_refuses(lib, change, word):
     assert word in _message(lib, _weights(lib, _kv(), **change))
 
