@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
                 if (pos >= p.score_cap) v = plain_sum<BF16, HD>(p, u, share.head, pos, norms);
                 else
                     for (int r = 0; r < u.rows; r++) v += ex2(scores[(long long)r * p.score_cap + pos] + norms[r]);
-                add_sum(p, u, share.head, pos, v);
+                add_sum(p, u, share.head, pos, seen_sum<BF16, HD>(p, u, share.head, pos, norms, v));
             }
         }
         cluster_sync();  // nobody leaves while another reads what it has

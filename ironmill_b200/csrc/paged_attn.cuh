@@ -382,6 +382,13 @@ __device__ __noinline__ float plain_sum(const PagedAttn &p, const PagedUnit &u, 
     return v;
 }
 
+// The sum `v` of a position's weights from kept scores, where it is not a number: a row with such a sum of weights is one wherever its scores are, at positions too that it does
+// not see. Those that all rows see stay, new rows and what is not there are taken from the rows that see them alone.
+template <bool BF16, int HD>
+__device__ __forceinline__ float seen_sum(const PagedAttn &p, const PagedUnit &u, int head, int pos, const float *norms, float v) {
+    return v == v || (pos < u.len && p.kv.row_of(u.seq, pos) >= 0) ? v : plain_sum<BF16, HD>(p, u, head, pos, norms);
+}
+
 // Row r of an item that a cut divides, by a warp, HD / 32 columns a lane. The parts of an item lie with the CTAs that its tiles fall to; a lane per part
 // brings maxima and sums. (A block per row with the shares' divisions in loops took 25 us for 64 items of 104 rows.)
 template <bool BF16, int R, int HD>

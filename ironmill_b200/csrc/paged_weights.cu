@@ -64,7 +64,8 @@ __global__ void __launch_bounds__(kSumThreads) paged_sum_kernel(const __grid_con
                 const float4 s = *reinterpret_cast<const float4 *>(scores + (long long)r * p.score_cap + pos);
                 v.x += ex2(s.x + norms[r]); v.y += ex2(s.y + norms[r]); v.z += ex2(s.z + norms[r]); v.w += ex2(s.w + norms[r]);
             }
-            if (aligned && pos + 4 <= min(u.len, p.sum_cols)) {
+            const float all = (v.x + v.y) + (v.z + v.w);
+            if (all == all && aligned && pos + 4 <= min(u.len, p.sum_cols)) {
                 float4 *to = reinterpret_cast<float4 *>(sums + pos);
                 const float4 o = *to;
                 *to = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
@@ -72,7 +73,7 @@ __global__ void __launch_bounds__(kSumThreads) paged_sum_kernel(const __grid_con
                 const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    if (pos + j < u.end) add_sum(p, u, head, pos + j, x[j]);
+                    if (pos + j < u.end) add_sum(p, u, head, pos + j, seen_sum<BF16, HD>(p, u, head, pos + j, norms, x[j]));
             }
         } else {
             for (int j = 0; j < 4 && at + j < u.end; j++) add_sum(p, u, head, pos + j, plain_sum<BF16, HD>(p, u, head, pos + j, norms));
