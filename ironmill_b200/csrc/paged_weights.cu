@@ -438,6 +438,12 @@ IM_EXPORT int im_cuda_paged_attention_weights(im_device *dev, const im_paged_kv 
         const long long span = 4 * ((kv->num_seqs - 1) * (long long)seq_stride + (kv->num_kv_heads - 1) * head_stride + rows), row = 2ll * x.num_heads * kv->head_dim;
         IM_REQUIRE(!share_memory(weights_dev, span, x.q_dev, 2 * (x.num_tokens - 1) * (long long)x.q_stride + row) && !share_memory(weights_dev, span, x.out_dev, 2 * (x.num_tokens - 1) * (long long)x.out_stride + row),
                    "the sums lie over the queries or the outputs");
+        PagedView v;
+        const int rc = paged_view(kv, x.layer, &v);
+        if (rc != IM_OK) return rc;
+        IM_REQUIRE(!share_memory(weights_dev, span, v.table, 4 * ((v.nseq - 1) * v.table_stride + v.width)) && !share_memory(weights_dev, span, v.len, 4ll * v.nseq) &&
+                       !share_memory(weights_dev, span, x.token_start_dev, 4ll * (v.nseq + 1)) && (!x.mask_dev || !share_memory(weights_dev, span, x.mask_dev, 8ll * x.num_tokens * x.mask_words)),
+                   "the sums lie over the page table, the lengths, the tokens' starts or the mask");
     }
     int rc = attn_args(dev, kv, x.layer, x.q_dev, x.q_stride, x.out_dev, x.out_stride, x.num_heads, x.token_start_dev, x.num_tokens, x.max_new, x.mask_dev, x.mask_words, x.scale, x.max_len, &p,
                        &empty);
