@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(kPaThreads, HD == 256 ? 1 : 2) paged_attn_kern
         share.from = share.tile = (int)((long long)n * rank / C);
         share.to = (long long)n * (rank + 1) / C;
     } else {
-        share = units <= 32 ? warp_share<R, kPaTile, MODE>(p, units, f_u) : find_share<R, kPaTile, kPaThreads, MODE>(p, units, sums, f_u);
+        share = units <= 32 ? warp_share<R, kPaTile, MODE>(p, units, p.ctas, f_u) : find_share<R, kPaTile, kPaThreads, MODE>(p, units, p.ctas, sums, f_u);
         if (share.from >= share.to) return;
     }
     const int count = (int)(share.to - share.from);
@@ -554,7 +554,7 @@ int attn_args(im_device *dev, const im_paged_kv *kv, int layer, const void *q_de
     p->scale2 = scale * 1.4426950408889634f;
     if (p->scale2 == 0.0f) p->scale2 = 1e-30f;  // every position alike, without 0 * inf at the hidden ones
     p->group_start = p->prefix_pages = nullptr;
-    p->groups = p->whole_slot = p->early = 0;
+    p->groups = p->whole_slot = p->beside = p->early = 0;
     p->stat = p->stat_parts = nullptr;
     p->scores = p->sums = nullptr;
     return IM_OK;

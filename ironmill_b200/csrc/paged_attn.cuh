@@ -25,6 +25,7 @@ struct PagedAttn {
     const int *group_start, *prefix_pages;  // [groups + 1] sequences, [groups]
     int groups;
     int whole_slot;           // kShared, kOwn: slots from here on are those of items that one CTA had, by item
+    int beside;               // kShared: the own rows are read by others at the same time, only as many CTAs as shared_ctas_beside() says take part
     int early;                // kOwn: a kShared launch that this one needs nothing of may still run (see paged_prefix.cu)
     // sums of softmax weights (paged_weights.cu)
     float2 *stat;             // [units, KV heads, rows of a tile]: maximum and sum of weights of every row of an item that one CTA (or cluster) had
@@ -185,8 +186,9 @@ __device__ __forceinline__ long long share_at(long long total, int n, int c) {
     return q * c + (uint32_t)((int)(total - q * n) * c) / (uint32_t)n;
 }
 
-template <int R, int TILE, int THREADS, int MODE>
-__device__ __forceinline__ Share find_share(const PagedAttn &p, int units, long long *sums, PagedUnit &at) {
+// LONG: of the units with more than `above` tiles alone, for CTA `cta` of `ctas`.
+template <int R, int TILE, int THREADS, int MODE, bool LONG = false>
+__device__ __forceinline__ Share find_share(const PagedAttn &p, int units, int ctas, long long *sums, PagedUnit &at, int above = 0, int cta = blockIdx.x) {
     int *found = reinterpret_cast<int *>(sums + THREADS + 32);  // unit, head, tile
     Share s;
     long long total = 0, before = 0;
@@ -202,6 +204,7 @@ __device__ __forceinline__ Share find_share(const PagedAttn &p, int units, long 
             long long all = total;
             if (pass == 0 || !once) {
                 n = u < units ? unit_tiles<TILE, MODE>(paged_unit<R, MODE>(p, u)) : 0;
+                if (LONG && n <= above) n = 0;
                 all = block_scan<THREADS>(n, sums);
             }
             if (pass == 0) {
@@ -220,9 +223,9 @@ __device__ __forceinline__ Share find_share(const PagedAttn &p, int units, long 
         }
         if (pass == 0) {
             const long long tiles = total * p.kv.nkv;
-            const int shares = share_count(tiles, p.ctas);
-            s.from = share_at(tiles, shares, blockIdx.x);
-            s.to = share_at(tiles, shares, blockIdx.x + 1);
+            const int shares = share_count(tiles, ctas);
+            s.from = share_at(tiles, shares, cta);
+            s.to = share_at(tiles, shares, cta + 1);
             if (s.from >= s.to) return s;
         }
     }
@@ -237,7 +240,7 @@ __device__ __forceinline__ Share find_share(const PagedAttn &p, int units, long 
 
 // The same by every warp for itself, for up to 32 units: a lane per unit, no synchronisation of the block.
 template <int R, int TILE, int MODE>
-__device__ __forceinline__ Share warp_share(const PagedAttn &p, int units, PagedUnit &at) {
+__device__ __forceinline__ Share warp_share(const PagedAttn &p, int units, int ctas, PagedUnit &at) {
     const int lane = threadIdx.x & 31;
     PagedUnit u = paged_unit<R, MODE>(p, min(lane, units - 1));
     const int n = lane < units ? unit_tiles<TILE, MODE>(u) : 0;  // (32 sequences of 2^31 rows in tiles of 64: 2^30)
@@ -250,7 +253,7 @@ __device__ __forceinline__ Share warp_share(const PagedAttn &p, int units, Paged
     const int all = __shfl_sync(0xffffffffu, sum, 31);
     Share s;
     const long long total = (long long)all * p.kv.nkv;
-    const int shares = share_count(total, p.ctas);
+    const int shares = share_count(total, ctas);
     s.from = share_at(total, shares, blockIdx.x);
     s.to = share_at(total, shares, blockIdx.x + 1);
     s.unit = s.head = s.tile = 0;
@@ -271,6 +274,41 @@ __device__ __forceinline__ Share warp_share(const PagedAttn &p, int units, Paged
     at.end = __shfl_sync(0xffffffffu, u.end, s.unit);
     at.from = MODE == kOwn ? __shfl_sync(0xffffffffu, u.from, s.unit) : 0;
     return s;
+}
+
+// CTAs of a tcgen05 launch for the shared rows beside which the own rows are read by others: as many as make both end together, by what there is of both in this call (what a
+// host knows, the longest sequence and the longest prefix, says little of either where they are not all alike). In SM microseconds: a tile of 128 positions 4 (256 rows) or 2.1
+// (128) and 2 for a CTA's start; 55 own rows of a KV head one, whatever the heads' width. Fitted to 36 calls (16 to 64 sequences behind 2048 to 16000 rows, heads of 64 and 128, own rows alike and
+// spread) with 12 .. 148 CTAs each: 4 % above the best number of CTAs on average, 17 % at most. (64 sequences of 700 rows of their own behind 8192: 112 us with 12 CTAs, 60 with 36, 62 with 74, 80 with 148.)
+template <int R, int TILE, int THREADS>
+__device__ __forceinline__ int shared_ctas_beside(const PagedAttn &p, long long *sums) {
+    float tiles = 0.0f, rows = 0.0f;
+    // (Every sequence counts, with new tokens or without, and every group as one of max_group_new tokens: one latency of loads. Which group a sequence is in and how many
+    // tokens a group has would be chains of them, 2 us.)
+    for (int i = threadIdx.x; i < max(p.kv.nseq, p.groups); i += THREADS) {
+        const int len = i < p.kv.nseq ? p.kv.length(i) : 0, g = min(i, p.groups - 1);
+        const int n = max(__ldg(p.group_start + g + 1) - __ldg(p.group_start + g), 0), prefix = prefix_rows(p, g);
+        rows += len;
+        if (i >= p.groups || n == 0) continue;
+        rows -= (float)n * prefix;
+        tiles += (float)p.row_tiles * ((prefix + TILE - 1) / TILE);
+    }
+    float2 *of_warp = reinterpret_cast<float2 *>(sums);
+    const float2 mine = make_float2(warp_sum(tiles), warp_sum(rows));
+    if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = mine;
+    __syncthreads();
+    tiles = rows = 0.0f;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; w++) tiles += of_warp[w].x, rows += of_warp[w].y;
+    __syncthreads();  // (`sums` is written again)
+    const float shared = tiles * p.kv.nkv * (R == 256 ? 4.0f : 2.1f), own = max(rows, 0.0f) * p.kv.nkv * (1 / 55.0f);
+    int lo = 1, hi = p.ctas;  // fewer CTAs leave more time and more SMs for the own rows
+    while (lo < hi) {
+        const int c = (lo + hi) / 2;
+        if ((p.ctas - c) * (2.0f + shared / c) > own) lo = c + 1;
+        else hi = c;
+    }
+    return lo;
 }
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool there) {  // zeros where there is no source

@@ -133,7 +133,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
         pdl_wait();
     }
     PagedUnit at;
-    const Share share = units <= 32 ? warp_share<R, kTcTile, MODE>(p, units, at) : find_share<R, kTcTile, kTcThreads, MODE>(p, units, reinterpret_cast<long long *>(Qs), at);  // (the copies start behind its last barrier)
+    int ctas = p.ctas;
+    if constexpr (MODE == kShared) ctas = p.beside ? shared_ctas_beside<R, kTcTile, kTcThreads>(p, reinterpret_cast<long long *>(Qs)) : ctas;
+    Share share{};
+    if (MODE != kShared || (int)blockIdx.x < ctas)  // (the others make room as soon as they know)
+        share = units <= 32 ? warp_share<R, kTcTile, MODE>(p, units, ctas, at)
+                            : find_share<R, kTcTile, kTcThreads, MODE>(p, units, ctas, reinterpret_cast<long long *>(Qs), at);  // (the copies start behind its last barrier)
     Items<R, MODE> it(p, units, share, at);
     bool ok = true;
     if (warp >= kTcCopy) {

@@ -7,9 +7,11 @@
 // that its keys and values are read once and its rows fill the tensor cores' tiles. The second set, each sequence's own rows, is a sequence that starts
 // behind its prefix (kOwn). Both leave sums, maximum and weighted values in f32, and a last launch joins them.
 //
-// More than 16 rows of a unit go to paged_attn_tc.cu. Up to 16 rows (single tokens' own rows, small groups) are taken here by CTAs that each read one run
-// of positions, all of it requested at once, and end: several per SM in different phases hide the lookups, the loads' latency and the joining of
-// warps behind each other's loads. (Equal shares of one list, as in paged_attn.cu, spend most of short items' time on their ends.)
+// More than 16 rows of a unit go to paged_attn_tc.cu. Up to 16 rows (single tokens' own rows, small groups, heads of 256) are taken here, a chunk of 128 positions (64 for heads of 256) at a
+// time, by CTAs that each have a few chunks of one item and end: several per SM in different phases hide the lookups, the loads' latency and the joining of
+// warps behind each other's loads. (Equal shares of one list, as in paged_attn.cu, spend most of short items' time on their ends.) How many CTAs an item needs the host cannot
+// know: where one sequence has far more rows of its own than the others, or is in no group, its items are longer than their CTAs' few chunks, and those items are left to equal
+// shares of further CTAs, which look them up on the device.
 // The launch for the own rows needs nothing of the one for the shared rows and starts beside it: kShared triggers its successor once everything before it is
 // done, the successor does not wait at its start, and its first CTA waits at its end, so that the join finds both done.
 //
@@ -31,7 +33,9 @@ struct PartSet {
     PagedAttn p;
     int rows;    // of a tile
     int tc;      // by paged_attn_tc.cu: a NaN as the sum of weights of a row that has to be done again
-    int chunks;  // else: CTAs, and so parts, of an item
+    int chunks;  // else: CTAs, and so parts, of an item of up to `direct` chunks of positions; longer ones are cut into equal shares
+    int direct, share_ctas;
+    int units, cut_slot;  // slots from here on: two a CTA with a share (tc: from 0 on); items that one CTA had: their first own slot
 };
 struct PrefixJoin {
     PartSet shared, own;
@@ -61,18 +65,16 @@ __device__ __forceinline__ void cp16_once(uint32_t dst, const void *src, bool th
     asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0), "l"(policy) : "memory");
 }
 
-// Chunks c, c + set.chunks, ... of an item.
+// Chunks k0, k0 + step, ... below k1 of an item, its part `slot`.
 template <bool BF16, int HD, int MODE>
-__device__ __forceinline__ void part_of_item(const PartSet &set, int item, int c, unsigned char *smem, long long (*offs)[32], float2 *ml, unsigned &bad_rows) {
+__device__ __forceinline__ void part_of_item(const PartSet &set, const PagedUnit &u, int head, int k0, int k1, int step, size_t slot, unsigned char *smem, long long (*offs)[32], float2 *ml,
+                                             unsigned &bad_rows) {
     using S = PtShape<HD>;
     constexpr float kLift = BF16 ? 0.0f : 15.0f;  // fp16 weights: 2^15 at the row's maximum, as in paged_attn.cu
     constexpr int R = kPtRows, KS = HD / 16, NT = HD / 8, CH = HD / 8, SL = S::kSlices;
     const PagedAttn &p = set.p;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int unit = item / p.kv.nkv, head = item - unit * p.kv.nkv;
-    const PagedUnit u = paged_unit<R, MODE>(p, unit);
-    const int from = unit_from<MODE>(u), all = max(u.end - from + S::kChunk - 1, 0) / S::kChunk;
-    if (c >= all) return;
+    const int from = unit_from<MODE>(u);
     unsigned char *mine = smem + warp * S::kWarp;
     const uint32_t ks_at = smem_u32(mine), vs_at = ks_at + S::kKeys;
     const uint64_t once = read_once();
@@ -92,7 +94,7 @@ __device__ __forceinline__ void part_of_item(const PartSet &set, int item, int c
 #pragma unroll
         for (int j = 0; j < 4; j++) o[n][j] = 0.0f;
     bool first = true;
-    for (int k = c; k < all; k += set.chunks) {
+    for (int k = k0; k < k1; k += step) {
         const int pos0 = from + k * S::kChunk + warp * (SL * 16);
         const int pos = pos0 + (lane & (SL * 16 - 1));
         const long long row = pos < u.end ? p.kv.row_of(u.seq, pos) : -1;
@@ -157,7 +159,7 @@ __device__ __forceinline__ void part_of_item(const PartSet &set, int item, int c
                 const float m_new = fmaxf(m[i], top), corr = m_new == -INFINITY ? 1.0f : ex2(m[i] - m_new);
                 m[i] = m_new;
                 l[i] *= corr;
-                if (k > c)
+                if (k > k0)
 #pragma unroll
                     for (int n = 0; n < NT; n++) o[n][2 * i] *= corr, o[n][2 * i + 1] *= corr;
             }
@@ -208,7 +210,7 @@ __device__ __forceinline__ void part_of_item(const PartSet &set, int item, int c
     }
     if (tid == 0) bad_rows = 0;
     __syncthreads();
-    const size_t slot = ((size_t)item * set.chunks + c) * R;
+    slot *= R;
     for (int i = tid; i < u.rows * (HD / 4); i += kPtThreads) {
         const int r = i / (HD / 4), d = i % (HD / 4) * 4;
         float M = -INFINITY, L = 0.0f, worst = 0.0f;
@@ -238,7 +240,7 @@ __device__ __forceinline__ void part_of_item(const PartSet &set, int item, int c
             float M = -INFINITY, L = 0.0f, x[HD / 32];
 #pragma unroll
             for (int i = 0; i < HD / 32; i++) x[i] = 0.0f;
-            for (int k = c; k < all; k += set.chunks) {
+            for (int k = k0; k < k1; k += step) {
                 float y[HD / 32], m2, l2;
                 plain_row<BF16, HD>(p, u, head, r, from + k * S::kChunk, min(from + (k + 1) * S::kChunk, u.end), y, m2, l2);
                 if (m2 == -INFINITY && l2 == 0.0f) continue;
@@ -255,22 +257,80 @@ __device__ __forceinline__ void part_of_item(const PartSet &set, int item, int c
     }
 }
 
-// CTAs below `shared_ctas` for the shared rows, the others for the own ones.
+// A CTA's share: where it is, what is left of it, and a unit that the threads look for.
+struct PtShare {
+    int unit, head, next, nth;
+    long long left;
+};
+// Chunks c, c + chunks, ... of an item that is not long.
+template <bool BF16, int HD, int MODE>
+__device__ __forceinline__ void direct_part(const PartSet &set, int b, unsigned char *smem, long long (*offs)[32], float2 *ml, unsigned &bad_rows) {
+    const PagedAttn &p = set.p;
+    const int item = b / set.chunks, c = b - item * set.chunks, unit = item / p.kv.nkv, head = item - unit * p.kv.nkv;
+    const PagedUnit u = paged_unit<kPtRows, MODE>(p, unit);
+    const int all = unit_tiles<PtShape<HD>::kChunk, MODE>(u);
+    if (c < all && all <= set.direct) part_of_item<BF16, HD, MODE>(set, u, head, c, all, set.chunks, (size_t)b, smem, offs, ml, bad_rows);
+}
+
+// An equal share of the list of the long items' chunks, item by item. (By itself: what it needs of registers is no cost of the kernel above. The share lies in shared memory.)
+template <bool BF16, int HD, int MODE>
+__device__ __noinline__ void share_parts(const PartSet &set, int cta, unsigned char *smem, long long (*offs)[32], float2 *ml, unsigned &bad_rows, PtShare &share) {
+    constexpr int R = kPtRows, TILE = PtShape<HD>::kChunk;
+    const PagedAttn &p = set.p;
+    const int tid = threadIdx.x;
+    PagedUnit u;
+    const Share s = find_share<R, TILE, kPtThreads, MODE, true>(p, set.units, set.share_ctas, reinterpret_cast<long long *>(smem), u, set.direct, cta);
+    if (s.from >= s.to) return;
+    if (tid == 0) share = PtShare{s.unit, s.head, INT_MAX, 0, s.to - s.from};
+    int head = s.head, k0 = s.tile;
+    __syncthreads();
+    for (;;) {
+        const int all = unit_tiles<TILE, MODE>(u), item = share.unit * p.kv.nkv + head, k1 = (int)min((long long)all, k0 + share.left);
+        const size_t slot = k0 == 0 && k1 == all ? (size_t)item * set.chunks : set.cut_slot + 2 * (size_t)cta + share.nth;
+        int *span = p.spans + 2 * (long long)item;
+        if (tid == 0 && k0 == 0) span[0] = (int)slot;
+        if (tid == 0 && k1 == all) span[1] = cta;
+        __syncthreads();
+        if (tid == 0) share.left -= k1 - k0;
+        part_of_item<BF16, HD, MODE>(set, u, head, k0, k1, 1, slot, smem, offs, ml, bad_rows);
+        __syncthreads();
+        if (share.left <= 0) return;
+        // the next item: of the next head, or of the next long unit, which the threads look for together
+        const int unit = share.unit;
+        head = share.head + 1;
+        k0 = 0;
+        if (head == p.kv.nkv) {
+            head = 0;
+            for (int u0 = unit + 1; u0 < set.units; u0 += kPtThreads) {
+                const int x = u0 + tid;
+                if (x < set.units && unit_tiles<TILE, MODE>(paged_unit<R, MODE>(p, x)) > set.direct) atomicMin(&share.next, x);
+                if (__syncthreads_or(share.next != INT_MAX)) break;
+            }
+            if (share.next == INT_MAX) return;
+            u = paged_unit<R, MODE>(p, share.next);
+        }
+        const int next = head ? unit : share.next;
+        __syncthreads();
+        if (tid == 0) share = PtShare{next, head, INT_MAX, 1, share.left};
+        __syncthreads();
+    }
+}
+
+// CTAs, one set after the other: for items of the shared rows and of the own ones, then for shares of the long ones of either.
 template <bool BF16, int HD>
-__global__ void __launch_bounds__(kPtThreads, HD == 256 ? 2 : 3) paged_part_kernel(const __grid_constant__ PrefixJoin a, int shared_ctas) {
+__global__ void __launch_bounds__(kPtThreads, HD == 256 ? 2 : 3) paged_part_kernel(const __grid_constant__ PrefixJoin a, int shared_ctas, int own_ctas) {
     extern __shared__ __align__(128) unsigned char pt_smem[];
     __shared__ float2 ml[kPtWarps * kPtRows];
     __shared__ long long offs[kPtWarps][32];
     __shared__ unsigned bad_rows;
+    __shared__ PtShare share;
     if (!a.own.p.early) pdl_wait();
     pdl_trigger();  // (the join looks up what this call was given before it waits)
-    const int b = blockIdx.x;
-    if (b < shared_ctas) {
-        part_of_item<BF16, HD, kShared>(a.shared, b / a.shared.chunks, b % a.shared.chunks, pt_smem, offs, ml, bad_rows);
-    } else {
-        const int i = b - shared_ctas;
-        part_of_item<BF16, HD, kOwn>(a.own, i / a.own.chunks, i % a.own.chunks, pt_smem, offs, ml, bad_rows);
-    }
+    const int b = blockIdx.x, i = b - shared_ctas, cta = i - own_ctas, own_cta = shared_ctas ? cta - a.shared.share_ctas : cta;
+    if (i < 0) direct_part<BF16, HD, kShared>(a.shared, b, pt_smem, offs, ml, bad_rows);
+    else if (cta < 0) direct_part<BF16, HD, kOwn>(a.own, i, pt_smem, offs, ml, bad_rows);
+    else if (own_cta < 0) share_parts<BF16, HD, kShared>(a.shared, cta, pt_smem, offs, ml, bad_rows, share);
+    else share_parts<BF16, HD, kOwn>(a.own, own_cta, pt_smem, offs, ml, bad_rows, share);
     if (a.own.p.early && b == 0) pdl_wait();  // this launch ends after the one before it
 }
 
@@ -283,7 +343,7 @@ struct PjRow {
     int token;                // -1: not to be written
     long long out;
     int unit[2], r[2];        // shared, own: the unit (-1: no parts) and row of its tile
-    int slot0[2], next[2], parts[2];  // slot of the first part, of the others less their steps, number of parts
+    int slot0[2], next[2], step[2], parts[2];  // slot of the first part, of the others less their steps; number of parts
 };
 
 template <int HD, int MODE>
@@ -294,21 +354,26 @@ __device__ __forceinline__ void find_unit(const PartSet &s, int unit, int r, PjR
     if (r >= u.rows || u.end <= from) return;
     x.r[w] = r;
     x.unit[w] = unit;
-    x.parts[w] = min(s.chunks, (u.end - from + PtShape<HD>::kChunk - 1) / PtShape<HD>::kChunk);  // (where it is not by tcgen05)
+    const int all = (u.end - from + PtShape<HD>::kChunk - 1) / PtShape<HD>::kChunk;
+    x.parts[w] = s.tc || all > s.direct ? -1 : min(s.chunks, all);  // (-1: the spans say)
 }
 __device__ __forceinline__ void find_parts(const PartSet &s, int w, int head, PjRow &x) {
     if (x.unit[w] < 0) return;
     const long long item = (long long)x.unit[w] * s.p.kv.nkv + head;
-    if (s.tc) {
+    if (x.parts[w] < 0) {
         const int2 span = *reinterpret_cast<const int2 *>(s.p.spans + 2 * item);
+        const int cta = (span.x - s.cut_slot) >> 1;
+        const bool whole = s.tc ? span.x >= s.p.whole_slot : span.x < s.cut_slot;
         x.slot0[w] = span.x;
-        x.next[w] = (span.x >> 1) * 2;
-        x.parts[w] = span.x >= s.p.whole_slot ? 1 : span.y - (span.x >> 1) + 1;
+        x.next[w] = s.cut_slot + 2 * cta;
+        x.step[w] = 2;
+        x.parts[w] = whole ? 1 : span.y - cta + 1;
     } else {
         x.slot0[w] = x.next[w] = (int)(item * s.chunks);
+        x.step[w] = 1;
     }
 }
-__device__ __forceinline__ size_t slot_of(const PartSet &s, int w, const PjRow &x, int part) { return part == 0 ? x.slot0[w] : x.next[w] + part * (s.tc ? 2 : 1); }
+__device__ __forceinline__ size_t slot_of(int w, const PjRow &x, int part) { return part == 0 ? x.slot0[w] : x.next[w] + part * x.step[w]; }
 
 template <bool BF16, int HD>
 __global__ void __launch_bounds__(2 * HD) paged_prefix_join_kernel(const __grid_constant__ PrefixJoin a) {
@@ -374,7 +439,7 @@ __global__ void __launch_bounds__(2 * HD) paged_prefix_join_kernel(const __grid_
             const int part = i0 + lane, w = part >= y.parts[0], k = w ? part - y.parts[0] : part;
             const PartSet &s = w ? a.own : a.shared;
             float2 ml = make_float2(-INFINITY, 0.0f);
-            if (part < y.parts[0] + y.parts[1]) ml = s.p.part_ml[slot_of(s, w, y, k) * s.rows + y.r[w]];
+            if (part < y.parts[0] + y.parts[1]) ml = s.p.part_ml[slot_of(w, y, k) * s.rows + y.r[w]];
             const bool redo = __any_sync(0xffffffffu, s.tc && ml.y != ml.y);  // not finite on the tensor cores: the row is done again below
             const float2 before = state[i];
             const float top = fmaxf(before.x, warp_max(ml.x)), c = before.x == top ? 1.0f : ex2(before.x - top);
@@ -398,8 +463,8 @@ __global__ void __launch_bounds__(2 * HD) paged_prefix_join_kernel(const __grid_
 #pragma unroll
             for (int j = 0; j < kPjAhead; j++) {
                 const int part = i0 + min(i + j, n - 1);
-                v[j] = *reinterpret_cast<const float4 *>(part < parts0 ? base0 + slot_of(a.shared, 0, rows[r], part) * a.shared.rows * HD
-                                                                       : base1 + slot_of(a.own, 1, rows[r], part - parts0) * a.own.rows * HD);
+                v[j] = *reinterpret_cast<const float4 *>(part < parts0 ? base0 + slot_of(0, rows[r], part) * a.shared.rows * HD
+                                                                       : base1 + slot_of(1, rows[r], part - parts0) * a.own.rows * HD);
             }
 #pragma unroll
             for (int j = 0; j < kPjAhead; j++) {
@@ -442,25 +507,27 @@ __global__ void __launch_bounds__(2 * HD) paged_prefix_join_kernel(const __grid_
 // ------------------------------------------------------------------------------------------------ plans
 struct PartPlan {
     int rows, row_tiles, units, tc;
-    int ctas;          // tcgen05
+    int ctas;          // with shares
+    int most_chunks;   // not tcgen05: CTAs of an item
     size_t slots, spans;
     size_t bytes;
 };
 // tc: rows of a tile on tcgen05, 0: tiles of 16 here, with at most four CTAs an SM and at most one a chunk: more of them even out sequences of different lengths, but each
 // leaves a part to join (32 sequences behind 4096 rows: 33 us with four, 37 with six, 40 with 24; 8 x 8 behind 3000: 53 with four or six, 57 with 24; 64 behind 8192: 53 with any).
-constexpr int kMostChunks = 64, kRounds = 4;
+// Items of more than kTurns chunks a CTA are cut into equal shares of further CTAs, two an SM (four users behind 30000 rows and one of 30000 by itself: 607 us without, 80 so; three an SM
+// 83, and 73 instead of 70 for 63 users behind 8192; the number of turns, 4 to 32, makes no difference there, and up to 15 % either way for sequences that are all alike).
+constexpr int kMostChunks = 64, kRounds = 4, kTurns = 8, kShareCtas = 2;
 PartPlan part_plan(const Device *dev, int units, int nkv, int hd, long long rows, int tc) {
     PartPlan a;
     a.tc = tc > 0;
     a.rows = tc ? tc : kPtRows;
     a.row_tiles = (int)((rows + a.rows - 1) / a.rows);
     a.units = units * a.row_tiles;
-    a.ctas = dev->sm_count;
+    a.ctas = tc ? dev->sm_count : kShareCtas * dev->sm_count;
     const size_t items = (size_t)a.units * nkv;
-    a.spans = tc ? (items * 8 + 15) / 16 * 16 : 0;
-    a.slots = 0;
-    if (tc) a.slots = ((size_t)a.ctas * 2 + items) * a.rows;
-    else if (items) a.slots = items * std::max<size_t>(1, std::min<size_t>(kMostChunks, (size_t)kRounds * dev->sm_count / items)) * a.rows;
+    a.spans = (items * 8 + 15) / 16 * 16;
+    a.most_chunks = items ? (int)std::max<size_t>(1, std::min<size_t>(kMostChunks, (size_t)kRounds * dev->sm_count / items)) : 1;
+    a.slots = items == 0 ? 0 : ((size_t)a.ctas * 2 + items * (tc ? 1 : a.most_chunks)) * a.rows;
     a.bytes = a.slots * hd * 4 + a.slots * 8 + a.spans;
     return a;
 }
@@ -498,9 +565,14 @@ unsigned char *lay_out(PartSet *s, const PartPlan &plan, int max_rows, int likel
     s->tc = plan.tc;
     p->row_tiles = plan.row_tiles;
     const long long items = (long long)plan.units * p->kv.nkv;
-    p->ctas = (int)std::max(1ll, std::min<long long>(plan.ctas, items * ((max_rows + 127ll) / 128)));
     const int chunk = p->kv.hd == 256 ? 64 : 128;
-    s->chunks = plan.tc || items == 0 ? 1 : (int)std::max(1ll, std::min<long long>((likely_rows + (long long)chunk - 1) / chunk, (long long)(plan.slots / items / plan.rows)));
+    p->ctas = (int)std::max(1ll, std::min<long long>(plan.ctas, items * ((max_rows + (plan.tc ? 128ll : chunk) - 1) / (plan.tc ? 128 : chunk))));
+    s->chunks = plan.tc ? 1 : (int)std::max(1ll, std::min<long long>((likely_rows + (long long)chunk - 1) / chunk, plan.most_chunks));
+    const bool long_ones = !plan.tc && items > 0 && (max_rows + (long long)chunk - 1) / chunk > (long long)s->chunks * kTurns;
+    s->direct = long_ones ? s->chunks * kTurns : INT_MAX;
+    s->share_ctas = long_ones ? p->ctas : 0;
+    s->units = plan.units;
+    s->cut_slot = plan.tc ? 0 : (int)(items * s->chunks);
     p->whole_slot = 2 * plan.ctas;
     p->part_o = reinterpret_cast<float *>(at);
     p->part_ml = reinterpret_cast<float2 *>(p->part_o + plan.slots * p->kv.hd);
@@ -509,38 +581,23 @@ unsigned char *lay_out(PartSet *s, const PartPlan &plan, int max_rows, int likel
     return at + plan.bytes;
 }
 
-// CTAs of a tcgen05 launch for the shared rows beside which the own rows are read by others: as many as make both end together. In SM microseconds, both measured: a tile of
-// 128 positions 2.7 (256 rows) or 2.1 (128) and 8 for a CTA's start and outputs; 20 KB of own rows one, of which a sequence has about half the longest's. (64 sequences of up to
-// 700 rows behind 8192: 74 us with all SMs for the shared rows first, 65 with half, 60 with 48 of 148, 63 with 36; 8 x 8 behind 3000: 68, 65, 74, 90.)
-int shared_ctas_beside(const Device *dev, const PrefixJoin &a, const PrefixPlan &plan, int max_prefix, int max_len) {
-    const int sms = dev->sm_count, nkv = a.own.p.kv.nkv;
-    const double tiles = (double)plan.shared.units * nkv * ((max_prefix + 127) / 128) * (plan.shared.rows == 256 ? 2.7 : 2.1);
-    const double own = (double)plan.own.units * nkv * std::max(1, max_len - max_prefix) * 0.5 * a.own.p.kv.hd * 4 / 20e3;
-    int lo = 1, hi = sms;  // fewer CTAs leave more time and more SMs for the own rows
-    while (lo < hi) {
-        const int c = (lo + hi) / 2;
-        if ((sms - c) * (8 + tiles / c) > own) lo = c + 1;
-        else hi = c;
-    }
-    return std::min(lo, a.shared.p.ctas);
-}
-
 template <bool BF16, int HD>
 int part_launch(const Device *dev, const PrefixJoin &a, int shared_ctas, int own_ctas, cudaStream_t st) {
     using S = PtShape<HD>;
     static DeviceOnce once;
     if (once.first(dev->ordinal)) IM_CUDA_CHECK(cudaFuncSetAttribute((paged_part_kernel<BF16, HD>), cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
-    IM_CUDA_CHECK(launch_k(paged_part_kernel<BF16, HD>, dim3((unsigned)(shared_ctas + own_ctas)), dim3(kPtThreads), (size_t)S::kSmem, st, a, shared_ctas));
+    const int shares = (shared_ctas ? a.shared.share_ctas : 0) + (own_ctas ? a.own.share_ctas : 0);
+    IM_CUDA_CHECK(launch_k(paged_part_kernel<BF16, HD>, dim3((unsigned)(shared_ctas + own_ctas + shares)), dim3(kPtThreads), (size_t)S::kSmem, st, a, shared_ctas, own_ctas));
     return IM_OK;
 }
 
 template <bool BF16, int HD>
-int run(const Device *dev, PrefixJoin &a, const PrefixPlan &plan, int max_prefix, int max_len, cudaStream_t st) {
+int run(const Device *dev, PrefixJoin &a, const PrefixPlan &plan, cudaStream_t st) {
     const int nkv = a.own.p.kv.nkv;
     int rc = IM_OK, shared_ctas = 0, own_ctas = 0;
     if (plan.shared.units > 0) {
         if (plan.shared.tc) {
-            if (!plan.own.tc) a.shared.p.ctas = shared_ctas_beside(dev, a, plan, max_prefix, max_len);
+            a.shared.p.beside = !plan.own.tc;
             rc = paged_tc_part_launch(dev, a.shared.p, BF16, kShared, plan.shared.rows, plan.shared.units, st);
             a.own.p.early = 1;
         } else {
@@ -601,11 +658,11 @@ IM_EXPORT int im_cuda_paged_prefix_attention(im_device *dev, const im_paged_kv *
     a.shared.p.mask = nullptr;
     a.shared.p.max_new = max_group_new;
     a.group_new = max_group_new;
-    unsigned char *at = lay_out(&a.shared, plan.shared, max_prefix, max_prefix, static_cast<unsigned char *>(x.scratch_dev));
+    unsigned char *at = lay_out(&a.shared, plan.shared, plan.shared.tc ? max_prefix : max_len, max_prefix, static_cast<unsigned char *>(x.scratch_dev));
     lay_out(&a.own, plan.own, max_len, num_groups ? std::max(1, max_len - max_prefix) : max_len, at);
     const cudaStream_t st = as_stream(stream);
     const bool bf16 = kv->dtype == IM_DTYPE_BF16;
-#define IM_RUN(HD) (bf16 ? run<true, HD>(dev, a, plan, max_prefix, max_len, st) : run<false, HD>(dev, a, plan, max_prefix, max_len, st))
+#define IM_RUN(HD) (bf16 ? run<true, HD>(dev, a, plan, st) : run<false, HD>(dev, a, plan, st))
     switch (kv->head_dim) {
     case 64: return IM_RUN(64);
     case 128: return IM_RUN(128);

@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_weigh_kernel(const __grid
     pdl_trigger();
     if (!p.early) pdl_wait();
     PagedUnit at;
-    const Share share = units <= 32 ? warp_share<kAllRows, kTcTile, kWeigh>(p, units, at) : find_share<kAllRows, kTcTile, kTcThreads, kWeigh>(p, units, reinterpret_cast<long long *>(Qs), at);
+    const Share share = units <= 32 ? warp_share<kAllRows, kTcTile, kWeigh>(p, units, p.ctas, at) : find_share<kAllRows, kTcTile, kTcThreads, kWeigh>(p, units, p.ctas, reinterpret_cast<long long *>(Qs), at);
     Items<kAllRows, kWeigh> it(p, units, share, at);
     bool ok = true;
     int block = 0;  // blocks of rows so far
