@@ -510,8 +510,9 @@ def paged_append(kv: PagedKV, layer: int, k, v, token_start, q=None, cos=None, s
         return q_out
     axes, at, of_pair = 1, 0, 0
     if pair_axis is not None:
+        assert positions is not None and positions.dim() == 2, "the axes of pairs without positions of axes"
         axes = positions.shape[0]
-        assert len(pair_axis) == rotary_dim // 2, (len(pair_axis), rotary_dim)
+        assert len(pair_axis) == rotary_dim // 2 and (axes > 1 or not any(pair_axis)), (len(pair_axis), rotary_dim, axes)
         at = _ints(positions, on, axes, n) if n else 0
         if axes > 1:
             pair_axis = bytes(pair_axis)
