@@ -26,3 +26,13 @@ def test_sums_may_lie_right_beside_it(lib, change):  # noqa: F811
 def test_rows_of_a_page_table_that_lie_apart_count_as_a_whole(lib):  # noqa: F811
     assert "table" in _message(lib, _weights(lib, _kv(table_stride=100), w=3 * PTR + 800))
     assert _message(lib, _weights(lib, _kv(table_stride=100), w=3 * PTR + 816)) == GOOD
+
+
+@pytest.mark.parametrize("tokens, row", [(1, 512), (2, 512), (5, 512), (5, 640)])
+def test_sums_may_lie_right_behind_and_right_before_queries_and_outputs(lib, tokens, row):  # noqa: F811
+    """Four heads of 128 columns of two bytes a token, rows apart by `row` elements: the last one ends with its heads."""
+    end = 2 * row * (tokens - 1) + 1024
+    shape = dict(n=tokens, qs=row, os=row, q=6 * PTR)
+    for at in (6 * PTR, 9 * PTR):
+        for w, word in ((at + end, GOOD), (at + end - 4, "queries or the outputs"), (at - SPAN, GOOD), (at - SPAN + 4, "queries or the outputs")):
+            assert word in _message(lib, _weights(lib, _kv(), **dict(shape, w=w))), (at, w)
