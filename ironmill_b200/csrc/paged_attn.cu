@@ -516,7 +516,7 @@ int attn_check(const im_paged_kv *kv, int num_heads, int max_new) {
     IM_REQUIRE(num_heads > 0 && num_heads % kv->num_kv_heads == 0, "num_heads has to be a multiple of num_kv_heads (got %d and %d)", num_heads, kv->num_kv_heads);
     IM_REQUIRE(max_new >= 1, "max_new has to be at least 1 (got %d)", max_new);
     const long long tiles = ((long long)(num_heads / kv->num_kv_heads) * max_new + 15) / 16;
-    IM_REQUIRE(tiles * std::max(kv->num_seqs, 1) * kv->num_kv_heads <= 1 << 24, "%d sequences of %d new tokens are too many for one call", kv->num_seqs, max_new);
+    IM_REQUIRE(tiles <= (1 << 24) / std::max(kv->num_seqs, 1) / kv->num_kv_heads, "%d sequences of %d new tokens are too many for one call", kv->num_seqs, max_new);
     return IM_OK;
 }
 

@@ -555,7 +555,7 @@ PrefixPlan prefix_plan(const Device *dev, const PagedView &v, int group, int max
 int prefix_check(const im_paged_kv *kv, int num_heads, int num_groups, int max_group_new) {
     IM_REQUIRE(num_groups >= 0 && max_group_new >= 1, "%d groups of %d new tokens", num_groups, max_group_new);
     const long long tiles = ((long long)(num_heads / kv->num_kv_heads) * max_group_new + 15) / 16;
-    IM_REQUIRE(tiles * std::max(num_groups, 1) * kv->num_kv_heads <= 1 << 24, "%d groups of %d new tokens are too many for one call", num_groups, max_group_new);
+    IM_REQUIRE(tiles <= (1 << 24) / std::max(num_groups, 1) / kv->num_kv_heads, "%d groups of %d new tokens are too many for one call", num_groups, max_group_new);
     return IM_OK;
 }
 

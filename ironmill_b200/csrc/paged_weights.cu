@@ -430,7 +430,7 @@ IM_EXPORT int im_cuda_paged_attention_weights(im_device *dev, const im_paged_kv 
     const int64_t seq_stride = args->seq_stride, head_stride = args->head_stride;
     float *const weights_dev = args->weights_dev;
     const int64_t most = (int64_t)1 << 40;
-    IM_REQUIRE(rows >= 1 && head_stride >= rows && head_stride <= most && seq_stride <= most && head_stride <= most / kv->num_kv_heads &&
+    IM_REQUIRE(rows >= 1 && head_stride >= rows && seq_stride <= most / std::max(kv->num_seqs, 1) && head_stride <= most / kv->num_kv_heads &&
                    (kv->num_seqs <= 1 || seq_stride >= (kv->num_kv_heads - 1) * head_stride + rows),
                "sums of different sequences and heads overlap");
     if (x.num_tokens > 0 && kv->num_seqs > 0) {
