@@ -369,7 +369,8 @@ int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int layer, co
  * first prefix_pages_dev[g] entries of their table rows are the same, and each has at least those pages' rows before its new tokens (what comes out otherwise is
  * unspecified).  Sequences before the first group and from the last one's end on share nothing.  A group's new tokens count one after
  * the other; max_group_new: no group has more (further ones are left as they are).  max_prefix: no group shares more rows (0: the table's width), max_len: as above; smaller
- * values cost time, not results.  Weights enter their product as in paged_attention, by the rows of a group for the shared pages. */
+ * values cost time, not results.  Weights enter their product as in paged_attention, by the rows (tokens x query heads of a KV head) of a group for the shared pages: more than 128 of
+ * them as one 16-bit term.  Where no sequence has more than 16 rows (single tokens) they keep both terms, as they have by themselves. */
 size_t im_cuda_paged_prefix_attention_scratch_bytes(const im_device *dev, const im_paged_kv *kv, int num_heads, int max_new, int num_groups, int max_group_new);
 typedef struct im_paged_attention_args { /* as the arguments of paged_attention; clear it before filling it */
     const void *q_dev;
