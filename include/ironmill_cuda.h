@@ -364,8 +364,8 @@ int im_cuda_paged_attention(im_device *dev, const im_paged_kv *kv, int layer, co
                             int num_heads, const int *token_start_dev, int num_tokens, int max_new, const uint64_t *mask_dev, int mask_words,
                             float scale, int max_len, void *scratch_dev, size_t scratch_bytes, void *stream);
 
-/* The same where sequences share their first pages: those are read once for all the sequences of a group (one instruction before many prompts, one prompt
- * before many answers).  Group g has the sequences group_start_dev[g] .. group_start_dev[g + 1] - 1 (group_start [num_groups + 1], not decreasing); the
+/* The same where sequences share their first pages: those are read for all the sequences of a group together (one instruction before many prompts, one prompt
+ * before many answers), once for every 256 rows (tokens x query heads of a KV head) of the group; heads of 256: for every 16.  Group g has the sequences group_start_dev[g] .. group_start_dev[g + 1] - 1 (group_start [num_groups + 1], not decreasing); the
  * first prefix_pages_dev[g] entries of their table rows are the same, and each has at least those pages' rows before its new tokens (what comes out otherwise is
  * unspecified).  Sequences before the first group and from the last one's end on share nothing.  A group's new tokens count one after
  * the other; max_group_new: no group has more (further ones are left as they are).  max_prefix: no group shares more rows (0: the table's width), max_len: as above; smaller

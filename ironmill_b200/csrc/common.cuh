@@ -148,6 +148,11 @@ int v2_repack(const uint8_t *codes0, const __half2 *sz0, const uint8_t *codes1, 
 // tail; pdl_wait() returns once the predecessor has completed and its writes are visible.  Every kernel
 // launched through launch_k() must therefore call pdl_wait() before it reads anything a predecessor wrote
 // and before its first global write.
+// One exception: a kernel may leave the wait at its start out where the launch directly before it (a) is of the same call,
+// (b) triggers (pdl_trigger()) only after its own pdl_wait(), so that everything before the call is done when this kernel
+// starts, and (c) writes nothing that this kernel reads or writes, and reads nothing that it writes. Block 0 of this kernel
+// then calls pdl_wait() before it ends: who waits for this launch has waited for the one before it. So do the own rows of
+// paged_prefix.cu and paged_weigh_kernel; no launch may come between the two of such a pair.
 
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_k(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args &&...args) {

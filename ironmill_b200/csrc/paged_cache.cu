@@ -1,6 +1,6 @@
 // A paged cache of keys and values: appending with rotation (and norms), keeping the accepted path of a drafted tree, reordering the beams of a search.
 // All of them move rows and compute next to nothing: HBM bounds them where they are large, the chain of lookups (sequence of a
-// token -> its length -> its page) where they are small. 16 bytes per lane everywhere.
+// token -> its length -> its page) where they are small. 16 bytes a lane and access (8 where keys and queries are normed, 2 where they are and rotary_dim is no multiple of 8).
 #include <limits.h>
 
 #include <algorithm>
@@ -382,7 +382,8 @@ __global__ void __launch_bounds__(kAppendThreads, 4) paged_append_normed_kernel(
     for (int h = first; h < a.kv.nkv; h += per) *reinterpret_cast<uint4 *>(to + h * head) = *reinterpret_cast<const uint4 *>(v + h * hd);
 }
 
-// Any even rotary_dim, column by column: the columns behind the rotated ones are pairs of neighbours that are not turned.
+// Any even rotary_dim, column by column: the columns behind the rotated ones are pairs of neighbours that are not turned. Loads and stores of 2 bytes bound it: the 8 prompts above with
+// a rotary_dim of 100 137 us (2.4 times as long), 32 tokens 11.8 us a call as the others.
 template <bool BF16, bool F32>
 __global__ void __launch_bounds__(kAppendThreads) paged_append_odd_kernel(const __grid_constant__ Append a, const __grid_constant__ AppendMore m, int lanes) {
     pdl_trigger();

@@ -4,7 +4,7 @@
 //
 // Softmax sums over two sets of positions add up once both refer to the same maximum. The first set, the shared pages, is the same for all tokens of a group,
 // whose rows (token, query head of a KV head) lie one after the other: a group is one sequence with all these rows and without new positions (kShared), so
-// that its keys and values are read once and its rows fill the tensor cores' tiles. The second set, each sequence's own rows, is a sequence that starts
+// that its keys and values are read once for every 256 rows (every 16 of heads of 256) and its rows fill the tensor cores' tiles. The second set, each sequence's own rows, is a sequence that starts
 // behind its prefix (kOwn). Both leave sums, maximum and weighted values in f32, and a last launch joins them.
 //
 // More than 16 rows of a unit go to paged_attn_tc.cu. Up to 16 rows (single tokens' own rows, small groups, heads of 256) are taken here, a chunk of 128 positions (64 for heads of 256) at a
@@ -15,9 +15,11 @@
 // The launch for the own rows needs nothing of the one for the shared rows and starts beside it: kShared triggers its successor once everything before it is
 // done, the successor does not wait at its start, and its first CTA waits at its end, so that the join finds both done.
 //
-// 64 sequences of up to 700 rows of their own behind 8192 (8.98 GFLOP, 132 MB): 54 us, of which the launches of both sets, side by side, 42 (41 SMs for the shared rows: 12.5 tiles of 128
-// positions and 256 rows at 2.7 us; the others for the own rows, 3 TB/s) and the join 12, which is the latency of its three loads one after the other and 12 MB of parts from L2. 16 trees of 26
-// nodes behind 30000 rows: 240 us, 855 TFLOP/s, bound by the turns that the halves of a wide tile take (paged_attn_tc.cu).
+// 64 sequences of up to 700 rows of their own behind 8192 (8.98 GFLOP, 132 MB): 52 us, of which the launches of both sets, side by side, 40 (58 SMs for the shared rows, 9 tiles of 128
+// positions and 256 rows each; the others for the own rows, 3 TB/s) and the join 12, which is the latency of its three loads one after the other and 12 MB of parts from L2. 16 trees of 26
+// nodes behind 30000 rows: 254 to 282 us in calls in a row, 730 to 810 TFLOP/s, by what the power cap leaves (240 us and 855 before it is reached), bound by the turns that the halves of a
+// wide tile take (paged_attn_tc.cu). Heads of 64: 42 us for the first, 223 for the trees. Heads of 256 read the shared rows in tiles of 16 rows here, each tile all of them and a chunk only
+// when the one before it is done: 230 us, and 3.5 ms for the trees, 6 and 14 times their floors.
 #include <limits.h>
 #include <math.h>
 

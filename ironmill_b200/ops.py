@@ -620,7 +620,8 @@ def paged_prefix_attention_scratch(kv: PagedKV, heads: int, max_new: int, groups
 def paged_prefix_attention(kv: PagedKV, layer: int, q, token_start, max_new: int, scale: float, group_start, max_group_new: int, prefix_pages, max_prefix=0, mask=None, max_len=0,
                            out=None, scratch=None):
     """paged_attention where the sequences group_start[g] .. group_start[g + 1] - 1 (int32 [groups + 1]) have the first prefix_pages[g] (int32 [groups]) pages of
-    their table rows in common: those are read once for a group. max_group_new, max_prefix: the most new tokens of a group, the most rows that one shares."""
+    their table rows in common: those are read once for every 256 rows (new tokens times query heads of a KV head) of a group, heads of 256 once for every 16.
+    max_group_new, max_prefix: the most new tokens of a group, the most rows that one shares."""
     n, heads, dim = q.shape
     on, groups = kv.ordinal, prefix_pages.shape[0]
     qs = _rows_of(q, n, heads, kv.head_dim, kv.dtype, on)
